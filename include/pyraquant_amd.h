@@ -367,6 +367,71 @@ int pq_fold_weight(const void* w, int32_t dtype, int64_t N, int64_t K, int64_t l
                    int64_t n_smooth, const float* shift, int64_t n_shift, const void* bias_in, void* w_out,
                    int64_t ldo, void* bias_out, hipStream_t stream);
 
+/*
+ * ---- Microscaled 4-bit layers, and the tuning of their low-rank branch (no reference counterpart) -------------------
+ *
+ * Format. 32 consecutive values of a row share 2^E, E = max(floor(log2(max |x|)) - 2, -127), stored as the byte E + 127;
+ * each value is the nearest of {0, 0.5, 1, 1.5, 2, 3, 4, 6} 2^E with its sign (sign, 2 exponent bits, 1 mantissa bit), ties to
+ * the even mantissa, saturated at 6. A block with an infinity or a NaN has byte 255 and codes 0: it is NaN, and so is every
+ * output that sums over it. A block of zeros has byte 0 and codes 0.
+ *
+ * Packed layout of [R, K], K % 32 == 0, with KT = ceil(K / 128), RB = ceil(R / 16):
+ *   codes  RB * KT * 1024 bytes: the packed K64 layout of the bytes (two values each, the even k in the low nibble), K padded
+ *          with zeros to a multiple of 128;
+ *   scales RB * KT * 64 bytes: block (rb, kt) at (rb * KT + kt) * 64 holds 4 bytes for each of its 16 rows, those of the
+ *          stage's scale blocks 0, 2, 1, 3.
+ * The 8-bit codes of a checkpoint are row-major [R, K] int8 on the same scales: q8 = clamp(rint(x 2^(4 - E)), -127, 127),
+ * worth 2^(E - 4) each (codes 0 in a block that is NaN).
+ *
+ * pq_mx_quant: rows x [M, K] (dtype PQ_BF16, PQ_F16 or PQ_F32, row stride ldx) to codes and scales; q8 [M, K] is written in
+ * the same pass unless NULL. codes and q8 16-byte aligned; x of any alignment and stride of its elements (16-byte aligned rows
+ * are read with wide loads).
+ */
+int pq_mx_quant(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* codes, uint8_t* scales, int8_t* q8,
+                hipStream_t stream);
+
+/* The values of codes (bits = 4: packed; bits = 8: a checkpoint's row-major codes) as out [M, K] of dtype PQ_BF16, PQ_F16 or
+ * PQ_F32, row stride ldo; out and its rows 16-byte aligned. */
+int pq_mx_values(const void* codes, const uint8_t* scales, int32_t bits, int64_t M, int64_t K, void* out, int32_t dtype,
+                 int64_t ldo, hipStream_t stream);
+
+/*
+ * y[m, n] = sum_k xh[m, k] wh[n, k] (+ sum_r t[m, r] l2t[n, r]) (+ bias[n]), summed in fp32, rounded once to dtype (PQ_BF16 or
+ * PQ_F16). a, w: packed 4-bit matrices [M, K] and [N, K]. t [M, R] (row stride ldt) and l2t [N, R] of dtype, R in {32, 64}, or
+ * NULL. K % 32 == 0, N % 16 == 0, M <= 2^30; operands 16-byte aligned, ldc and ldt multiples of 8.
+ */
+int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales, const float* bias,
+               const void* t, int64_t ldt, const void* l2t, int64_t R, void* c, int64_t ldc, int32_t dtype, int64_t M, int64_t N,
+               int64_t K, hipStream_t stream);
+
+/*
+ * The low-rank factors in the orders the layer's kernels read them, zero-padded from rank R to P (32 or 64): lr_A [K, R] (row
+ * stride lda) to At [P, K] and Ap [K, P], lr_B [R, N] (row stride ldb) to Bt [N, P] and Bp [P, N]; an output may be NULL. All
+ * 16-bit.
+ */
+int pq_mx_factors(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, int64_t N, int64_t R, int64_t P, void* At,
+                  void* Ap, void* Bt, void* Bp, hipStream_t stream);
+
+/*
+ * dx[m, k] = sum_n dy[m, n] wh[n, k] (+ sum_r dt[m, r] ap[k, r]): the gradient of a layer's input over its packed 4-bit weight
+ * [N, K], widened to dtype on the way to the matrix instructions (exact; in fp16, for 2^-22 <= 2^E <= 2^13), summed in fp32.
+ * dy [M, N], dx [M, K] of dtype; dt [M, R] and ap [K, R] contiguous, R in {32, 64}, or NULL. Operands 16-byte aligned, lddy and
+ * lddx multiples of 8.
+ */
+int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, const uint8_t* w, const uint8_t* w_scales, const void* dt,
+                     const void* ap, int64_t R, void* dx, int64_t lddx, int64_t M, int64_t N, int64_t K, hipStream_t stream);
+
+/*
+ * The gradients of the low-rank factors and the bias: dB[r, n] = sum_m t[m, r] dy[m, n] ([R, N]), dA[k, r] = sum_m xt[m, k]
+ * dt[m, r] ([K, R], xt: the values of the checkpoint q8 with x_scales), dbias[n] = sum_m dy[m, n] (fp32). An output that is
+ * NULL is not computed, and what only it needs (dy and t for dB and dbias; dt, q8 and x_scales for dA) may be NULL too. t and dt are [M, P], zero past rank R. Sums in fp32, in an order that depends on the sizes alone; dA and dB rounded to dtype.
+ * The workspace (pq_mx_grad_factors_workspace_size bytes) may hold anything.
+ */
+int64_t pq_mx_grad_factors_workspace_size(int64_t M, int64_t K, int64_t N, int64_t P);
+int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, const void* t, const void* dt, const int8_t* q8,
+                       const uint8_t* x_scales, int64_t M, int64_t K, int64_t N, int64_t R, int64_t P, void* dA, void* dB,
+                       float* dbias, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

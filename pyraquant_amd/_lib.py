@@ -44,6 +44,13 @@ EXPORTS = (
     "pq_int8_linear",
     "pq_int8_linear_noalloc",
     "pq_int8_linear_noalloc_max_bytes",
+    "pq_mx_quant",
+    "pq_mx_values",
+    "pq_mx_gemm",
+    "pq_mx_factors",
+    "pq_mx_grad_input",
+    "pq_mx_grad_factors_workspace_size",
+    "pq_mx_grad_factors",
 )
 
 _p = ctypes.c_void_p
@@ -80,6 +87,14 @@ _SIGNATURES = {
     "pq_int8_linear_noalloc": ([_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i64,
                                 _p], ctypes.c_int),
     "pq_int8_linear_noalloc_max_bytes": ([], _i64),
+    "pq_mx_quant": ([_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p], ctypes.c_int),
+    "pq_mx_values": ([_p, _p, _i32, _i64, _i64, _p, _i32, _i64, _p], ctypes.c_int),
+    "pq_mx_gemm": ([_p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p], ctypes.c_int),
+    "pq_mx_factors": ([_p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
+    "pq_mx_grad_input": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p], ctypes.c_int),
+    "pq_mx_grad_factors_workspace_size": ([_i64, _i64, _i64, _i64], _i64),
+    "pq_mx_grad_factors": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p],
+                           ctypes.c_int),
 }
 
 _lib = None

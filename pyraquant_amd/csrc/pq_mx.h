@@ -1,0 +1,171 @@
+// Microscaled 4-bit blocks (gfx950): the format, its conversions and its packed layout.
+//
+// 32 consecutive values of a row share one power of two 2^E, E = floor(log2(max |x|)) - 2 (at least -127), stored as the
+// byte E + 127. Each value is the nearest of {0, 0.5, 1, 1.5, 2, 3, 4, 6} 2^E with its sign (1 sign, 2 exponent, 1 mantissa
+// bit), ties to the even mantissa, saturated at 6. With that E the largest |x| 2^-E lies in [4, 8), so the top of the grid
+// is used and only values in (7, 8) 2^E lose more than half a step. A block holding an infinity or a NaN has byte 255 (the
+// whole block is NaN) and codes 0; a block of zeros has byte 0 and codes 0.
+//
+// The 8-bit codes of a training layer's checkpoint are rint(x 2^(4 - E)) in [-127, 127] on the same E, worth 2^(E - 4)
+// each: |x| < 2^(E + 3), so seven bits and the sign cover the block, and one scale array serves both.
+#pragma once
+
+#include "pq_common.h"
+
+namespace pq {
+namespace mx {
+
+constexpr int kBlock = 32;     // values that share a scale
+constexpr int kNaN = 255;      // scale byte of a block that is NaN
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+
+// ---- packed layout ---------------------------------------------------------------------------------------------------
+// A matrix [R, K] (K % 32 == 0) is cut into KT = ceil(K / 128) stages of 128 values and ceil(R / 16) row blocks.
+// Codes: block (rb, kt), 1 KB at (rb KT + kt) 1024, is the packed K64 layout of the bytes (two values each, the even k in the
+// low nibble): the 32 values of scale block b (of 4) of row r are the 16 bytes at 64 r + 16 (b ^ k64_swz(r)).
+// Scales: 64 bytes at (rb KT + kt) 64, four for each row, in the order of blocks 0, 2, 1, 3: a matrix instruction over 64
+// values takes blocks 2 s (lanes 0-31) and 2 s + 1 (lanes 32-63) in its step s, so each half reads the two bytes it needs
+// as one 16-bit word. Rows past R and blocks past K are zeros.
+__host__ __device__ __forceinline__ int stages(int64_t K) { return (int)((K + 127) / 128); }
+__host__ __device__ __forceinline__ int64_t code_offset(int64_t row, int kt, int b, int KT) {
+  const int r = (int)(row & 15);
+  return ((row >> 4) * KT + kt) * 1024 + r * 64 + ((b ^ k64_swz(r)) << 4);
+}
+__host__ __device__ __forceinline__ int scale_slot(int b) { return (b >> 1) | ((b & 1) << 1); }
+__host__ __device__ __forceinline__ int64_t scale_offset(int64_t row, int kt, int b, int KT) {
+  return ((row >> 4) * KT + kt) * 64 + (row & 15) * 4 + scale_slot(b);
+}
+
+// 2^(byte - 127) as the conversion instructions take it (they read the exponent field; 0x400000 is 2^-127 itself).
+__device__ __forceinline__ float scale_value(int byte) {
+  return __uint_as_float(max((uint32_t)byte << 23, 0x400000u));
+}
+
+// ---- a block of 32 values in registers, as 16 words of two 16-bit values or 32 floats ------------------------------
+template <int DT>
+struct Block {
+  static constexpr int WORDS = DT == PQ_F32 ? 32 : 16;
+  uint32_t w[WORDS];
+
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0;
+  }
+  // 32 values at p: 16-byte loads where VEC, else one by one
+  template <bool VEC>
+  __device__ __forceinline__ void load(const void* p) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < WORDS / 4; ++i) {
+        const v4u v = reinterpret_cast<const v4u*>(p)[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
+      }
+    } else if constexpr (DT == PQ_F32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) w[i] = static_cast<const uint32_t*>(p)[i];
+    } else {
+      const uint16_t* h = static_cast<const uint16_t*>(p);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+    }
+  }
+  __device__ __forceinline__ float value(int i) const {   // i: a constant after unrolling
+    if constexpr (DT == PQ_F32) return __uint_as_float(w[i]);
+    else return i & 1 ? hi16_to_f32<DT>(w[i >> 1]) : lo16_to_f32<DT>(w[i >> 1]);
+  }
+  // The scale byte. The largest magnitude is found on the bits without the sign, which order as the values do (and put
+  // infinities and NaNs on top).
+  __device__ __forceinline__ int scale_byte() const {
+    uint32_t e;
+    if constexpr (DT == PQ_F32) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) m = max(m, w[i] & 0x7fffffffu);
+      e = m >> 23;
+    } else {
+      us2 m = us2{0, 0};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, w[i] & 0x7fff7fffu));
+      const uint32_t a = max((uint32_t)m[0], (uint32_t)m[1]);
+      if constexpr (DT == PQ_BF16) e = a >> 7;
+      else e = a >= 0x7c00u ? 255u : __float_as_uint(lo16_to_f32<PQ_F16>(a)) >> 23;
+    }
+    return e == 255u ? kNaN : max((int)e - 2, 0);
+  }
+  // the 4-bit codes, two to a byte
+  __device__ __forceinline__ v4i codes(int byte) const {
+    const float s = scale_value(byte);
+    v4i c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t o = 0;
+      if constexpr (DT == PQ_F32) {
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, value(8 * i + 0), value(8 * i + 1), s, 0);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, value(8 * i + 2), value(8 * i + 3), s, 1);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, value(8 * i + 4), value(8 * i + 5), s, 2);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, value(8 * i + 6), value(8 * i + 7), s, 3);
+      } else if constexpr (DT == PQ_BF16) {
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, w[4 * i + 0]), s, 0);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, w[4 * i + 1]), s, 1);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, w[4 * i + 2]), s, 2);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, w[4 * i + 3]), s, 3);
+      } else {
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, w[4 * i + 0]), s, 0);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, w[4 * i + 1]), s, 1);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, w[4 * i + 2]), s, 2);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, w[4 * i + 3]), s, 3);
+      }
+      c[i] = byte == kNaN ? 0 : (int)o;
+    }
+    return c;
+  }
+  // the 8-bit codes: x 2^(131 - byte), rounded by adding 1.5 2^23 (to nearest even; the sum's low byte is the code). ldexp,
+  // not a product: below byte 4 that power of two is no float.
+  __device__ __forceinline__ void codes8(int byte, v4i (&q)[2]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t b[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float f = __builtin_amdgcn_ldexpf(value(4 * i + e), 131 - byte);
+        f = __builtin_amdgcn_fmed3f(f, -127.0f, 127.0f) + 12582912.0f;
+        b[e] = __float_as_uint(f);
+      }
+      const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400);
+      q[i >> 2][i & 3] = byte == kNaN ? 0 : (int)(lo | (hi << 16));
+    }
+  }
+};
+
+// Two 4-bit values (byte SEL of `c`) as two 16-bit values times `s` (scale_value); exact for bf16, and for fp16 where the
+// result is a normal or a two-bit subnormal number.
+template <int DT, int SEL>
+__device__ __forceinline__ uint32_t widen2(uint32_t c, float s) {
+  if constexpr (DT == PQ_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, SEL));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, SEL));
+}
+// Eight 4-bit values (one word) as four words of two 16-bit values.
+template <int DT>
+__device__ __forceinline__ v4u widen8(uint32_t c, float s) {
+  return v4u{widen2<DT, 0>(c, s), widen2<DT, 1>(c, s), widen2<DT, 2>(c, s), widen2<DT, 3>(c, s)};
+}
+template <int DT>
+constexpr uint32_t nan2() { return DT == PQ_BF16 ? 0x7fc07fc0u : 0x7e007e00u; }
+
+// Four 8-bit codes (one word) times 2^(byte - 131), as two words of two 16-bit values.
+template <int DT>
+__device__ __forceinline__ v2u restore4(uint32_t q, float s) {
+  float f[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = (float)((int)(q << (24 - 8 * e)) >> 24) * s;
+  return v2u{pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3])};
+}
+// 2^(byte - 131), NaN for a block that is NaN.
+__device__ __forceinline__ float restore_scale(int byte) {
+  return byte == kNaN ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(1.0f, byte - 131);
+}
+
+}  // namespace mx
+}  // namespace pq

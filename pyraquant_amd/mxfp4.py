@@ -1,0 +1,421 @@
+"""Microscaled 4-bit layers for MI355X (gfx950): Linears whose weights and activations are 4-bit floating point with a shared
+power of two per 32 values, and the tuning of their low-rank branch over frozen weights.
+
+  quant_mxfp4(x) -> Mxfp4Matrix                     rows to 4-bit codes and scales (and the 8-bit codes of a checkpoint)
+  dequant_mxfp4(q, dtype)                            back to values
+  checkpoint_values(q8, q, dtype)                    the values of the 8-bit codes
+  mxfp4_gemm(xq, wq, bias, out_dtype, t=, l2t=)      the product, with the low-rank term and the bias in its epilogue
+  mxfp4_grad_input(dy, wq, dt=, lr_Ap=)              the input's gradient, from the 4-bit weight as it is stored
+  lowrank_grads(dy, t, dt, q8, xq, rank)             the gradients of lr_A, lr_B and the bias, from the 8-bit checkpoint
+  Mxfp4Linear, convert_linears_to_mxfp4              the layer, and a model's Linears made into it
+
+The format: E = floor(log2(max |x|)) - 2 over 32 consecutive values of a row, each held as the nearest of 0, 0.5, 1, 1.5, 2, 3,
+4, 6 times 2^E (ties to an even last bit, saturated at 6). A block with an infinity or a NaN is NaN.
+
+Tuning. ``Mxfp4Linear(lin, lowrank=(A, B), trainable=True)`` keeps the weight in 4 bits and makes lr_A, lr_B and the bias
+parameters. What its backward pass keeps of the input are 8-bit codes, rint(x 2^(4 - E)) on the same E, written in the
+quantizer's pass over x (half the bytes of x): they give lr_A's gradient. The rounding of x to 4 bits counts as the identity.
+
+Every kernel runs on the caller's current stream; nothing synchronises. CPU tensors raise AssertionError; a missing library
+raises at the first call.
+"""
+from __future__ import annotations
+
+from typing import Callable, Dict, NamedTuple, Optional, Tuple
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .int8_exec import LOWRANK_A_ATTR, LOWRANK_B_ATTR, is_bf16_whitelisted, lowrank_down
+
+BLOCK = 32        # values that share a scale
+MAX_RANK = 64     # of a low-rank branch (the kernels hold 32 or 64; lower ranks run zero-padded)
+_DTYPES = {torch.bfloat16: _lib.PQ_BF16, torch.float16: _lib.PQ_F16, torch.float32: _lib.PQ_F32}
+
+
+class Mxfp4Matrix(NamedTuple):
+    """A [rows, cols] matrix in 4 bits: packed codes and scales (flat uint8 tensors, pq_mx_quant's layout)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    rows: int
+    cols: int
+
+
+def _stages(rows: int, cols: int) -> int:
+    return (rows + 15) // 16 * ((cols + 127) // 128)
+
+
+def _check_cuda(*tensors) -> None:
+    dev = None
+    for t in tensors:
+        if t is not None:
+            assert t.is_cuda, "the 4-bit layers run on the GPU only (got a CPU tensor)"
+            assert dev is None or t.device == dev, f"operands on {dev} and {t.device}"
+            dev = t.device
+
+
+def _check_matrix(q: Mxfp4Matrix) -> None:
+    units = _stages(q.rows, q.cols)
+    assert q.cols > 0 and q.cols % BLOCK == 0, q.cols
+    for t, size in ((q.codes, 1024), (q.scales, 64)):
+        assert t.dtype == torch.uint8 and t.is_contiguous() and t.numel() >= units * size, (t.dtype, tuple(t.shape), q.rows, q.cols)
+
+
+def _dtype16(dt: torch.dtype) -> int:
+    return _lib.dtype_code(dt)
+
+
+def _plain(x: torch.Tensor) -> torch.Tensor:
+    x = x.detach()
+    return x.resolve_neg() if x.is_neg() else x
+
+
+def _rows(x2: torch.Tensor) -> torch.Tensor:
+    """x2 as the kernels read it: rows of consecutive elements, 16-byte aligned, none over another (a copy where not)."""
+    x2 = _plain(x2)
+    M, K = x2.shape
+    if x2.stride(1) != 1 or (M > 1 and (x2.stride(0) < K or x2.stride(0) * x2.element_size() % 16)) or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
+def _stride(x2: torch.Tensor) -> int:
+    """Row stride (that of a single row says nothing)."""
+    return x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
+
+
+# --------------------------------------------------------------------------- quantization
+def quant_mxfp4(x2: torch.Tensor, checkpoint: bool = False):
+    """x2 [M, K] (bf16, fp16 or fp32, K % 32 == 0) -> Mxfp4Matrix; with ``checkpoint`` (Mxfp4Matrix, q8): q8 [M, K] int8,
+    the codes a backward pass keeps, on the same scales. Row-slice views pass without a copy."""
+    assert x2.dim() == 2, x2.shape
+    _check_cuda(x2)
+    if x2.dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {x2.dtype} (expected bfloat16, float16 or float32)")
+    M, K = x2.shape
+    assert K > 0 and K % BLOCK == 0, f"K = {K} is not a multiple of {BLOCK}"
+    x2 = _plain(x2)
+    if M > 1 and (x2.stride(1) != 1 or x2.stride(0) < K) or x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    units = _stages(M, K)
+    codes = torch.empty(units * 1024, dtype=torch.uint8, device=x2.device)
+    scales = torch.empty(units * 64, dtype=torch.uint8, device=x2.device)
+    q8 = torch.empty((M, K), dtype=torch.int8, device=x2.device) if checkpoint else None
+    _lib.check(_lib.load().pq_mx_quant(_lib.ptr(x2), _DTYPES[x2.dtype], M, K, _stride(x2), _lib.ptr(codes), _lib.ptr(scales),
+                                       _lib.ptr(q8), _lib.stream_of(x2.device)), "quant_mxfp4")
+    q = Mxfp4Matrix(codes, scales, M, K)
+    return (q, q8) if checkpoint else q
+
+
+def _values(codes, scales, bits, M, K, dtype):
+    _check_cuda(codes, scales)
+    if dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {dtype} (expected bfloat16, float16 or float32)")
+    out = torch.empty((M, K), dtype=dtype, device=codes.device)
+    _lib.check(_lib.load().pq_mx_values(_lib.ptr(codes), _lib.ptr(scales), bits, M, K, _lib.ptr(out), _DTYPES[dtype], K,
+                                        _lib.stream_of(codes.device)), "mxfp4 values")
+    return out
+
+
+def dequant_mxfp4(q: Mxfp4Matrix, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values a 4-bit matrix holds, [rows, cols] (exact in bf16 and fp32; in fp16 for scales of 2^-22 to 2^13)."""
+    _check_matrix(q)
+    return _values(q.codes, q.scales, 4, q.rows, q.cols, dtype)
+
+
+def checkpoint_values(q8: torch.Tensor, q: Mxfp4Matrix, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of a checkpoint's 8-bit codes on the scales of the matrix quantized with them."""
+    _check_matrix(q)
+    assert q8.dtype == torch.int8 and q8.is_contiguous() and tuple(q8.shape) == (q.rows, q.cols), (q8.dtype, tuple(q8.shape))
+    return _values(q8, q.scales, 8, q.rows, q.cols, dtype)
+
+
+# --------------------------------------------------------------------------- product and gradients
+def mxfp4_gemm(xq: Mxfp4Matrix, wq: Mxfp4Matrix, bias: Optional[torch.Tensor], out_dtype: torch.dtype, *,
+               t: Optional[torch.Tensor] = None, l2t: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[M, N] = xq @ wq^T (+ t @ l2t^T) (+ bias), summed in fp32, rounded once. t [M, R] and l2t [N, R] in out_dtype, R 32 or
+    64; bias fp32 [N]; N % 16 == 0."""
+    _check_matrix(xq)
+    _check_matrix(wq)
+    _check_cuda(xq.codes, xq.scales, wq.codes, wq.scales, bias, t, l2t, out)
+    assert xq.cols == wq.cols, (xq.cols, wq.cols)
+    M, N, K = xq.rows, wq.rows, xq.cols
+    code = _dtype16(out_dtype)
+    if bias is not None:
+        assert bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == N, (bias.dtype, tuple(bias.shape), N)
+    R, ldt = 0, 0
+    if t is not None:
+        assert l2t is not None and t.dtype == l2t.dtype == out_dtype and t.stride(1) == 1 and l2t.is_contiguous()
+        assert t.dim() == 2 and t.shape[0] >= M and tuple(l2t.shape) == (N, t.shape[1]), (tuple(t.shape), tuple(l2t.shape), M, N)
+        R, ldt = t.shape[1], _stride(t)
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=xq.codes.device)
+    assert out.dtype == out_dtype and tuple(out.shape) == (M, N) and out.stride(1) == 1, (out.dtype, tuple(out.shape))
+    _lib.check(_lib.load().pq_mx_gemm(_lib.ptr(xq.codes), _lib.ptr(xq.scales), _lib.ptr(wq.codes), _lib.ptr(wq.scales),
+                                      _lib.ptr(bias), _lib.ptr(t), ldt, _lib.ptr(l2t), R, _lib.ptr(out), _stride(out), code,
+                                      M, N, K, _lib.stream_of(out.device)), "mxfp4_gemm")
+    return out
+
+
+def mxfp4_grad_input(dy: torch.Tensor, wq: Mxfp4Matrix, dt: Optional[torch.Tensor] = None,
+                     lr_Ap: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dx [M, K] = dy @ wq (+ dt @ lr_Ap^T): wq's values in dy's type, sums in fp32. dt [M, R] and lr_Ap [K, R] contiguous, R 32
+    or 64."""
+    _check_matrix(wq)
+    _check_cuda(dy, wq.codes, wq.scales, dt, lr_Ap)
+    assert dy.dim() == 2 and dy.shape[1] == wq.rows, (tuple(dy.shape), wq.rows)
+    code = _dtype16(dy.dtype)
+    dy = _rows(dy)
+    M, N, K = dy.shape[0], wq.rows, wq.cols
+    R = 0
+    if dt is not None:
+        R = dt.shape[1]
+        assert lr_Ap is not None and dt.dtype == lr_Ap.dtype == dy.dtype and dt.is_contiguous() and lr_Ap.is_contiguous()
+        assert tuple(dt.shape) == (M, R) and tuple(lr_Ap.shape) == (K, R), (tuple(dt.shape), tuple(lr_Ap.shape), M, K)
+    dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
+    _lib.check(_lib.load().pq_mx_grad_input(_lib.ptr(dy), code, _stride(dy), _lib.ptr(wq.codes), _lib.ptr(wq.scales),
+                                            _lib.ptr(dt), _lib.ptr(lr_Ap), R, _lib.ptr(dx), K, M, N, K,
+                                            _lib.stream_of(dy.device)), "mxfp4_grad_input")
+    return dx
+
+
+def lowrank_grads(dy: Optional[torch.Tensor], t: Optional[torch.Tensor], dt: Optional[torch.Tensor], q8: Optional[torch.Tensor],
+                  x_scales: Optional[torch.Tensor], rank: int, want_A: bool = True, want_B: bool = True, want_bias: bool = True):
+    """(dA [K, rank], dB [rank, N], dbias [N] fp32), None for those not wanted: dB = t^T dy, dbias = sum of dy's rows, dA =
+    checkpoint^T dt. t and dt are [M, P], P 32 or 64 >= rank, zero past rank; q8 and x_scales as quant_mxfp4 gave them. What no
+    wanted gradient needs may be None."""
+    if not (want_A or want_B or want_bias):
+        return None, None, None
+    ref = dt if want_A else t
+    _check_cuda(dy, t, dt, q8, x_scales)
+    M, P = ref.shape
+    dt16, dev = ref.dtype, ref.device
+    code = _dtype16(dt16)
+    K = N = BLOCK
+    if want_A:
+        assert q8.dtype == torch.int8 and q8.is_contiguous() and q8.shape[0] == M and dt.is_contiguous()
+        K = q8.shape[1]
+        assert x_scales.dtype == torch.uint8 and x_scales.numel() >= _stages(M, K) * 64
+    if want_B or want_bias:
+        assert dy.dim() == 2 and dy.shape[0] == M and dy.dtype == dt16 and tuple(t.shape) == (M, P) and t.is_contiguous()
+        dy = _rows(dy)
+        N = dy.shape[1]
+    assert 1 <= rank <= P, (rank, P)
+    dA = torch.empty((K, rank), dtype=dt16, device=dev) if want_A else None
+    dB = torch.empty((rank, N), dtype=dt16, device=dev) if want_B else None
+    db = torch.empty(N, dtype=torch.float32, device=dev) if want_bias else None
+    if M == 0:
+        return tuple(None if g is None else g.zero_() for g in (dA, dB, db))
+    L = _lib.load()
+    ws = torch.empty(L.pq_mx_grad_factors_workspace_size(M, K, N, P), dtype=torch.uint8, device=dev)
+    _lib.check(L.pq_mx_grad_factors(_lib.ptr(dy), code, _stride(dy) if want_B or want_bias else N, _lib.ptr(t), _lib.ptr(dt),
+                                    _lib.ptr(q8), _lib.ptr(x_scales), M, K, N, rank, P, _lib.ptr(dA), _lib.ptr(dB),
+                                    _lib.ptr(db), _lib.ptr(ws), ws.numel(), _lib.stream_of(dev)), "lowrank_grads")
+    return dA, dB, db
+
+
+def _padded_rank(R: int) -> int:
+    assert 1 <= R <= MAX_RANK, f"rank {R}: the 4-bit layers take 1 to {MAX_RANK}"
+    return 32 if R <= 32 else 64
+
+
+def lay_out_factors(lr_A: torch.Tensor, lr_B: torch.Tensor, down: bool = True, up: bool = True):
+    """lr_A [K, R] and lr_B [R, N] in the kernels' orders, zero-padded to rank P (32 or 64), from one launch: At [P, K] and
+    Bt [N, P] (``down``: what the forward pass reads), Ap [K, P] and Bp [P, N] (``up``: what the backward pass reads), None
+    where not asked for."""
+    _check_cuda(lr_A, lr_B)
+    assert lr_A.dim() == 2 and lr_B.dim() == 2 and lr_A.shape[1] == lr_B.shape[0], (tuple(lr_A.shape), tuple(lr_B.shape))
+    assert lr_A.dtype == lr_B.dtype, (lr_A.dtype, lr_B.dtype)
+    _dtype16(lr_A.dtype)
+    A, B = _plain(lr_A), _plain(lr_B)
+    if A.stride(1) != 1 or A.stride(0) < A.shape[1]:
+        A = A.contiguous()
+    if B.stride(1) != 1 or B.stride(0) < B.shape[1]:
+        B = B.contiguous()
+    (K, R), N = A.shape, B.shape[1]
+    P = _padded_rank(R)
+    new = lambda on, *shape: torch.empty(shape, dtype=A.dtype, device=A.device) if on else None   # noqa: E731
+    At, Ap, Bt, Bp = new(down, P, K), new(up, K, P), new(down, N, P), new(up, P, N)
+    _lib.check(_lib.load().pq_mx_factors(_lib.ptr(A), max(A.stride(0), R), _lib.ptr(B), max(B.stride(0), N), K, N, R, P,
+                                         _lib.ptr(At), _lib.ptr(Ap), _lib.ptr(Bt), _lib.ptr(Bp), _lib.stream_of(A.device)),
+               "lay_out_factors")
+    return At, Ap, Bt, Bp
+
+
+# --------------------------------------------------------------------------- the layer
+class _Linear4(torch.autograd.Function):
+    """y [M, N] of x2 [M, K]. lr_A and lr_B: the factors [K, R] and [R, N], or in the kernels' forward order [P, K] and [N, P]
+    (``laid_out``)."""
+
+    @staticmethod
+    def forward(ctx, x2, lr_A, lr_B, bias, codes, scales, N, laid_out):
+        M, K = x2.shape
+        wq = Mxfp4Matrix(codes, scales, N, K)
+        need_x, need_A, need_B, need_b = ctx.needs_input_grad[:4]
+        back = need_x or need_A or need_B or need_b
+        x2 = _rows(x2)
+        q8 = t = Ap = Bp = None
+        xq = quant_mxfp4(x2, need_A)
+        if need_A:
+            xq, q8 = xq
+        Bt = None
+        if lr_A is not None:
+            if laid_out:
+                At, Bt = lr_A, lr_B
+                if back:   # the other two orders, by the same rule with the factors' roles exchanged
+                    Bp, _, Ap, _ = lay_out_factors(Bt, At, True, False)
+            else:
+                At, Ap, Bt, Bp = lay_out_factors(lr_A, lr_B, True, back)
+            t = lowrank_down(x2, At)
+        y = mxfp4_gemm(xq, wq, bias, x2.dtype, t=t, l2t=Bt)
+        if back:
+            ctx.save_for_backward(q8, xq.scales if need_A else None, t if need_B or need_b else None, Ap, Bp, codes, scales)
+            ctx.wq_shape, ctx.rank = (N, K), None if lr_A is None or laid_out else lr_A.shape[1]
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        q8, x_scales, t, Ap, Bp, codes, scales = ctx.saved_tensors
+        need_x, need_A, need_B, need_b = ctx.needs_input_grad[:4]
+        wq = Mxfp4Matrix(codes, scales, *ctx.wq_shape)
+        dy = _rows(dy)
+        dt = lowrank_down(dy, Bp) if Bp is not None and (need_x or need_A) else None
+        dA, dB, db = lowrank_grads(dy, t, dt, q8, x_scales, ctx.rank, need_A, need_B, need_b)
+        dx = mxfp4_grad_input(dy, wq, dt, Ap) if need_x else None
+        return dx, dA, dB, db, None, None, None, None
+
+
+class Mxfp4Linear(nn.Module):
+    """4-bit stand-in for nn.Linear: y = x4 @ w4^T (+ (x @ lr_A) @ lr_B) (+ bias), x4 and w4 the microscaled 4-bit values of x
+    and the weight; in_features % 32 == 0, out_features % 16 == 0, low rank up to 64. Inputs are bf16 or fp16, and the
+    low-rank factors are used in the input's type.
+
+    Buffers ``weight_codes`` and ``weight_scales`` hold the weight. ``trainable=False`` keeps the low-rank branch in the
+    kernels' order (``lr_At`` [P, K], ``lr_Bt`` [N, P], zero-padded to P = 32 or 64; ``lr_A`` and ``lr_B`` give it back) and
+    the bias in fp32 as buffers. ``trainable=True`` (needs a low-rank branch) makes ``lr_A`` [K, R], ``lr_B`` [R, N] and
+    ``bias`` parameters; freeze() turns such a layer into the other kind. Gradients flow to the input of either."""
+
+    def __init__(self, lin: nn.Linear, device: Optional[torch.device] = None,
+                 lowrank: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, trainable: bool = False):
+        super().__init__()
+        w = lin.weight.detach()
+        if device is not None:
+            w = w.to(device)
+        self.out_features, self.in_features = N, K = w.shape
+        assert N % 16 == 0 and N > 0, f"out_features {N} is not a multiple of 16"
+        q = quant_mxfp4(w)
+        self.register_buffer("weight_codes", q.codes)
+        self.register_buffer("weight_scales", q.scales)
+        A, B = lowrank if lowrank is not None else (getattr(lin, LOWRANK_A_ATTR, None), getattr(lin, LOWRANK_B_ATTR, None))
+        self.rank = 0
+        if A is not None and B is not None:
+            A, B = A.detach().to(w.device), B.detach().to(w.device)
+            assert A.dim() == 2 and B.dim() == 2 and A.shape[0] == K and B.shape == (A.shape[1], N), (
+                tuple(A.shape), tuple(B.shape), K, N)
+            self.rank = int(A.shape[1])
+            _padded_rank(self.rank)
+        assert self.rank or not trainable, "trainable=True tunes a low-rank branch, and the layer has none"
+        self.trainable = bool(trainable)
+        bias = None if lin.bias is None else lin.bias.detach().to(w.device, torch.float32).contiguous()
+        if trainable:
+            self.lr_A, self.lr_B = nn.Parameter(A.clone().contiguous()), nn.Parameter(B.clone().contiguous())
+            self.bias = None if bias is None else nn.Parameter(bias.clone())
+        else:
+            self._keep(A if self.rank else None, B if self.rank else None, bias)
+
+    def _keep(self, A, B, bias) -> None:
+        """The low-rank branch and the bias as buffers, the branch in the kernels' order."""
+        At = Bt = None
+        if A is not None:
+            if A.dtype not in (torch.bfloat16, torch.float16):
+                A, B = A.to(torch.bfloat16), B.to(torch.bfloat16)
+            At, _, Bt, _ = lay_out_factors(A, B.to(A.dtype), True, False)
+        self.register_buffer("lr_At", At)
+        self.register_buffer("lr_Bt", Bt)
+        self.register_buffer("bias", bias)
+
+    def freeze(self) -> "Mxfp4Linear":
+        """Turns a trainable layer into one that serves: its low-rank branch laid out once, nothing left to tune."""
+        if self.trainable:
+            A, B, bias = self.lr_A.detach(), self.lr_B.detach(), self.bias
+            del self.lr_A, self.lr_B, self.bias
+            self.trainable = False
+            self._keep(A, B, None if bias is None else bias.detach().float().contiguous())
+        return self
+
+    def __getattr__(self, name):
+        if name in ("lr_A", "lr_B") and "lr_At" in self.__dict__.get("_buffers", ()):
+            if self.lr_At is None:
+                return None
+            return (self.lr_At[: self.rank].t() if name == "lr_A" else self.lr_Bt[:, : self.rank].t()).contiguous()
+        return super().__getattr__(name)
+
+    def _apply(self, fn, recurse=True):
+        """A module-wide cast leaves a bias buffer in fp32, as the kernels read it."""
+        keep = self._buffers.get("bias")
+        super()._apply(fn, recurse)
+        new = self._buffers.get("bias")
+        if keep is not None and new.dtype != torch.float32:
+            self._buffers["bias"] = keep.to(new.device)
+        return self
+
+    def weight(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values of the 4-bit weight, [N, K]."""
+        return dequant_mxfp4(Mxfp4Matrix(self.weight_codes, self.weight_scales, self.out_features, self.in_features), dtype)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        assert x.shape[-1] == self.in_features, (tuple(x.shape), self.in_features)
+        _check_cuda(x, self.weight_codes)
+        dt = x.dtype
+        _dtype16(dt)
+        x2 = x if x.dim() == 2 else x.reshape(-1, self.in_features)
+        bias = self.bias
+        if bias is not None and bias.dtype != torch.float32:
+            bias = bias.float()
+        if self.trainable:
+            A, B = self.lr_A, self.lr_B
+        else:
+            A, B = self.lr_At, self.lr_Bt
+        if A is not None and (A.dtype != dt or B.dtype != dt):
+            A, B = A.to(dt), B.to(dt)
+        y = _Linear4.apply(x2, A, B, bias, self.weight_codes, self.weight_scales, self.out_features, not self.trainable)
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self) -> str:
+        lr = f", low-rank r={self.rank}" + (" (trainable)" if self.trainable else "") if self.rank else ""
+        return f"in={self.in_features}, out={self.out_features}, mxfp4 W / A{lr} (HIP gfx950)"
+
+
+# --------------------------------------------------------------------------- model conversion
+def convert_linears_to_mxfp4(model: nn.Module, device: Optional[str] = "cuda",
+                             whitelist: Callable[[str], bool] = is_bf16_whitelisted,
+                             trainable: bool = False) -> Dict[str, object]:
+    """Replaces the token-level nn.Linear layers by Mxfp4Linear in place, as convert_linears_to_int8 does by Int8Linear, and
+    returns the same kind of statistics. Layers whose sizes the 4-bit kernels do not take (in_features % 32, out_features %
+    16) stay as they are, with the whitelisted ones. A low-rank branch attached under LOWRANK_A_ATTR / LOWRANK_B_ATTR is
+    carried over; ``trainable`` makes the branches and biases of the layers that have one parameters, and every other
+    parameter of the model is left as it is."""
+    dev = torch.device(device) if device is not None else None
+    n4, n_keep, p4, p_keep, kept = 0, 0, 0, 0, []
+    for name, lin in [(n, m) for n, m in model.named_modules() if isinstance(m, nn.Linear)]:
+        if whitelist(name) or lin.in_features % BLOCK or lin.out_features % 16:
+            n_keep += 1
+            p_keep += lin.weight.numel()
+            kept.append(name)
+            continue
+        parent_name, _, attr = name.rpartition(".")
+        parent = model.get_submodule(parent_name) if parent_name else model
+        has_lr = getattr(lin, LOWRANK_A_ATTR, None) is not None and getattr(lin, LOWRANK_B_ATTR, None) is not None
+        setattr(parent, attr, Mxfp4Linear(lin, device=dev, trainable=trainable and has_lr))
+        n4 += 1
+        p4 += lin.weight.numel()
+        del lin
+    if dev is not None and dev.type == "cuda":
+        torch.cuda.synchronize()
+    return {"n_mxfp4_linear": n4, "n_bf16_linear_kept": n_keep, "params_mxfp4": p4, "params_bf16_linear_kept": p_keep,
+            "bf16_kept_names": kept, "mxfp4_weight_gib": p4 * (1 / 2 + 1 / BLOCK) / 2**30, "bf16_equiv_gib": p4 * 2 / 2**30}
