@@ -405,6 +405,16 @@ int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, cons
                int64_t K, hipStream_t stream);
 
 /*
+ * A layer in one call: pq_mx_quant of x into codes and scales (and q8 unless NULL), t = x l1t^T into t [M, R] where R is 32 or 64
+ * (0: no low-rank branch), and pq_mx_gemm into y [M, N] (row stride ldy). The caller's codes, scales, q8 and t have the sizes
+ * given above and may hold anything; up to 32 rows without q8 are quantized inside the product, which leaves codes and scales
+ * alone. 16-byte aligned operands, ldx and ldy multiples of 8.
+ */
+int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, const uint8_t* w_scales,
+                 const float* bias, const void* l1t, const void* l2t, int64_t R, void* y, int64_t ldy, int64_t N, uint8_t* codes,
+                 uint8_t* scales, int8_t* q8, void* t, hipStream_t stream);
+
+/*
  * The low-rank factors in the orders the layer's kernels read them, zero-padded from rank R to P (32 or 64): lr_A [K, R] (row
  * stride lda) to At [P, K] and Ap [K, P], lr_B [R, N] (row stride ldb) to Bt [N, P] and Bp [P, N]; an output may be NULL. All
  * 16-bit.

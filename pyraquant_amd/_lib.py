@@ -47,6 +47,7 @@ EXPORTS = (
     "pq_mx_quant",
     "pq_mx_values",
     "pq_mx_gemm",
+    "pq_mx_linear",
     "pq_mx_factors",
     "pq_mx_grad_input",
     "pq_mx_grad_factors_workspace_size",
@@ -90,6 +91,7 @@ _SIGNATURES = {
     "pq_mx_quant": ([_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p], ctypes.c_int),
     "pq_mx_values": ([_p, _p, _i32, _i64, _i64, _p, _i32, _i64, _p], ctypes.c_int),
     "pq_mx_gemm": ([_p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p], ctypes.c_int),
+    "pq_mx_linear": ([_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
     "pq_mx_factors": ([_p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
     "pq_mx_grad_input": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p], ctypes.c_int),
     "pq_mx_grad_factors_workspace_size": ([_i64, _i64, _i64, _i64], _i64),

@@ -6,6 +6,9 @@
 // column operand an activation row m, so each lane holds 4 consecutive n of one output row.
 #include "pq_mx.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace pq {
 namespace mx {
 namespace {
@@ -17,6 +20,7 @@ struct GemmArgs {
   uint16_t* c;
   int64_t ldt, ldc;
   int M, N, KT;
+  int tiles_m, tiles_n;
 };
 
 // One step over 64 values: both operands 4-bit (format code 4), scale byte S of each scale word.
@@ -34,70 +38,415 @@ __device__ __forceinline__ v16f mfma16(v4i a, v4i b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// Four waves, each a 64 x 64 part of a 128 x 128 block, fragments straight from memory into registers.
-template <int DT, int R>
-__global__ __launch_bounds__(256) void mx_gemm_kernel(const GemmArgs p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n0 = blockIdx.x * 128 + (wave & 1) * 64, m0 = blockIdx.y * 128 + (wave >> 1) * 64;
-  if (n0 >= p.N || m0 >= p.M) return;
-  const int l32 = lane & 31, half = lane >> 5, r16 = lane & 15, sw = k64_swz(r16);
-  const int last_n = (p.N - 1) >> 4, last_m = (p.M - 1) >> 4;
-  int64_t wb[2], ab[2];
+// Workgroup id -> (tile_m, tile_n): ids are dealt round-robin over the 8 XCDs, so each XCD takes a contiguous run of the
+// tiles, rastered in groups of `group` m-tiles so that the tiles it works on at a time share rows of both operands in its L2.
+__device__ __forceinline__ void tile_of(int bid, int blocks, int tiles_m, int tiles_n, int group, int& tm, int& tn) {
+  const int per = blocks >> 3, rem = blocks & 7, xcd = bid & 7;
+  const int at = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (bid >> 3);
+  const int g = at / (group * tiles_n), first = g * group, size = min(tiles_m - first, group), r = at - g * group * tiles_n;
+  tm = first + r % size;
+  tn = r / size;
+}
+
+// Workgroup barrier that leaves LDS-DMA in flight (__syncthreads() would wait for all of it): this wave's LDS reads are done,
+// and nothing moves across it.
+__device__ __forceinline__ void ring_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Sums of one output block, then its epilogue. WMW waves along m times 2 along n; each wave holds TI x TJ tiles of 32 x 32 (n
+// x m). K advances in stages of 128 values (64 bytes a row) through a ring of NS stages in LDS, filled by LDS-DMA: NS - 1
+// stages in flight, no registers or LDS writes spent on them. A stage is the row blocks of the packed layout as they are (the
+// swizzle keeps the ds_read_b128 of 32 rows free of bank conflicts), and after them their scale words, 4 bytes a row.
+template <int TI, int TJ, int WMW, int NS>
+struct Ring {
+  static constexpr int NW = 2 * WMW, BN = 64 * TI, BM = 32 * TJ * WMW;
+  static constexpr int CODES = (BN + BM) * 64, SLOTS = (BN + BM) / 64;   // bytes of codes; 256-byte pieces of scales
+  static constexpr int STAGE = CODES + NW * 256;                         // (a wave without a piece of scales has a slot too)
+  static constexpr int DW = BN / 16 / NW, DA = BM / 16 / NW, DPW = DW + DA + 1;   // DMA instructions a wave and stage
+  static_assert(DW * 16 * NW == BN && DA * 16 * NW == BM && SLOTS <= NW, "a stage split over the waves");
+  static constexpr int LDS = NS * STAGE;
+  static constexpr int PITCH = 144;   // output staging: 64 outputs of a row and 16 bytes of padding
+  static_assert(NW * 32 * PITCH <= LDS, "output staging in the ring");
+};
+
+template <int TI, int TJ, int WMW, int NS, int OCC, int DT, int R>
+__global__ __attribute__((amdgpu_flat_work_group_size(128 * WMW, 128 * WMW), amdgpu_waves_per_eu(OCC * WMW / 2, OCC * WMW / 2)))
+void mx_gemm_kernel(const GemmArgs p) {
+  using T = Ring<TI, TJ, WMW, NS>;
+  constexpr int NW = T::NW, BN = T::BN, BM = T::BM;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[T::LDS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave & 1, wm = wave >> 1, l32 = lane & 31, half = lane >> 5;
+  int tm, tn;
+  tile_of(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, OCC == 1 ? 6 : 8, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN, KT = p.KT;
+
+  // Row blocks past the end, and stages past the last, lie outside the buffers: their loads read nothing and give zeros.
+  const int blk_w = (min(BN, p.N - n0) + 15) >> 4, blk_a = (min(BM, p.M - m0) + 15) >> 4;
+  const int64_t wb = (int64_t)(n0 >> 4) * KT, ab = (int64_t)(m0 >> 4) * KT;
+  const auto rs_w = __builtin_amdgcn_make_buffer_rsrc((void*)(p.w + wb * 1024), (short)0, blk_w * KT * 1024, kBufferWord3);
+  const auto rs_a = __builtin_amdgcn_make_buffer_rsrc((void*)(p.a + ab * 1024), (short)0, blk_a * KT * 1024, kBufferWord3);
+  const bool w_scales = wave < BN / 64;
+  const auto rs_s = w_scales
+      ? __builtin_amdgcn_make_buffer_rsrc((void*)(p.ws + wb * 64), (short)0, blk_w * KT * 64, kBufferWord3)
+      : __builtin_amdgcn_make_buffer_rsrc((void*)(p.as + ab * 64), (short)0, wave < T::SLOTS ? blk_a * KT * 64 : 0, kBufferWord3);
+  const int vw = wave * T::DW * KT * 1024 + lane * 16, va = wave * T::DA * KT * 1024 + lane * 16;
+  const int vs = (((w_scales ? wave : wave - BN / 64) * 4 + (lane >> 4)) * KT) * 64 + (lane & 15) * 4;
+  auto dma = [&](int buf, int kt) {
+    uint8_t* const sb = smem + buf * T::STAGE;
+    const int off = kt < KT ? kt * 1024 : kOOB;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {   // (row blocks past the end repeat the last one: their outputs are not stored)
-    wb[i] = (int64_t)min((n0 + 32 * i + l32) >> 4, last_n) * p.KT;
-    ab[i] = (int64_t)min((m0 + 32 * i + l32) >> 4, last_m) * p.KT;
-  }
-  v16f acc[2][2] = {};
-  for (int kt = 0; kt < p.KT; ++kt) {
-    int ws[2], as[2];
+    for (int i = 0; i < T::DW; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_w, (lds_void_t*)(sb + (wave * T::DW + i) * 1024), 16, vw + i * KT * 1024 + off, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      ws[i] = *reinterpret_cast<const uint16_t*>(p.ws + (wb[i] + kt) * 64 + r16 * 4 + 2 * half);
-      as[i] = *reinterpret_cast<const uint16_t*>(p.as + (ab[i] + kt) * 64 + r16 * 4 + 2 * half);
+    for (int i = 0; i < T::DA; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_a, (lds_void_t*)(sb + BN * 64 + (wave * T::DA + i) * 1024), 16,
+                                               va + i * KT * 1024 + off, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_s, (lds_void_t*)(sb + T::CODES + wave * 256), 4, vs + (kt < KT ? kt * 64 : kOOB), 0, 0, 0);
+  };
+
+  const int sw = k64_swz(lane & 15);
+  const int fw = (wn * (BN / 2) + l32) * 64, fa = (BN + wm * (BM / WMW) + l32) * 64;
+  v4i w0[TI], w1[TI], a0[TJ], a1[TJ];
+  int sw_[TI], sa_[TJ];
+  auto rd = [&](v4i (&w)[TI], v4i (&a)[TJ], int buf, int s) {
+    const uint8_t* const sb = smem + buf * T::STAGE;
+    const int c = ((2 * s + half) ^ sw) << 4;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) w[i] = *reinterpret_cast<const v4i*>(sb + fw + i * 2048 + c);
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) a[j] = *reinterpret_cast<const v4i*>(sb + fa + j * 2048 + c);
+  };
+  auto rd_scales = [&](int (&w)[TI], int (&a)[TJ], int buf) {
+    const uint8_t* const sb = smem + buf * T::STAGE + T::CODES + 2 * half;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) w[i] = *reinterpret_cast<const uint16_t*>(sb + (fw >> 4) + i * 128);
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) a[j] = *reinterpret_cast<const uint16_t*>(sb + (fa >> 4) + j * 128);
+    // (kept here: the compiler would put the masking of the words between the products that use them)
+#pragma unroll
+    for (int i = 0; i < TI; ++i) asm volatile("" : "+v"(w[i]));
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) asm volatile("" : "+v"(a[j]));
+  };
+  v16f acc[TI][TJ] = {};
+  auto mm = [&](auto s, const v4i (&w)[TI], const v4i (&a)[TJ], const int (&ws)[TI], const int (&as)[TJ]) {
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[i][j] = mfma4<decltype(s)::value>(w[i], ws[i], a[j], as[j], acc[i][j]);
+  };
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+
+  if constexpr (NW == 8) {
+    // Two groups of four waves, one wave of each per SIMD, take turns: while one issues a stage's products back to back from
+    // registers, the other reads the next stage's fragments and issues its part of a DMA. Group B runs one slot behind; a
+    // workgroup barrier ends each slot. Stage s + 1 has landed at the barrier that ends slot 2 s + 1 (each group waits for
+    // all but its NS - 2 younger stages), and stage s + NS - 1 goes into the buffer of stage s - 1, which both groups have read.
+    const bool grp_b = wave >= NW / 2;
+#pragma unroll
+    for (int st = 0; st < NS - 1; ++st) dma(st, st);
+    wait_vmcnt<(NS - 2) * T::DPW>();
+    ring_barrier();
+    if (grp_b) ring_barrier();
+    int b = 0;
+    for (int s = 0; s < KT; ++s) {
+      rd(w0, a0, b, 0);
+      rd(w1, a1, b, 1);
+      rd_scales(sw_, sa_, b);
+      dma(b == 0 ? NS - 1 : b - 1, s + NS - 1);
+      if (grp_b) wait_vmcnt<(NS - 2) * T::DPW>();
+      ring_barrier();
+      mm(S0{}, w0, a0, sw_, sa_);
+      mm(S1{}, w1, a1, sw_, sa_);
+      if (!grp_b) wait_vmcnt<(NS - 2) * T::DPW>();
+      ring_barrier();
+      b = b + 1 == NS ? 0 : b + 1;
     }
-    v4i w[2][2], a[2][2];
+    if (!grp_b) ring_barrier();
+  } else {
+    // The fragments of the next half stage are read while the products of this one run; one barrier a stage.
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int st = 0; st < NS; ++st) dma(st, st);
+    wait_vmcnt<(NS - 1) * T::DPW>();
+    ring_barrier();
+    rd(w0, a0, 0, 0);
+    rd_scales(sw_, sa_, 0);
+    int b = 0;
+    for (int s = 0; s < KT; ++s) {
+      const int bn = b + 1 == NS ? 0 : b + 1;
+      rd(w1, a1, b, 1);
+      mm(S0{}, w0, a0, sw_, sa_);
+      __builtin_amdgcn_sched_barrier(0);
+      wait_vmcnt<(NS - 2) * T::DPW>();   // stage s + 1 has landed
+      ring_barrier();                    // for every wave, and buffer b is read
+      int nsw[TI], nsa[TJ];
+      rd(w0, a0, bn, 0);
+      rd_scales(nsw, nsa, bn);
+      dma(b, s + NS);
+      mm(S1{}, w1, a1, sw_, sa_);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int off = r16 * 64 + (((2 * s + half) ^ sw) << 4);
-        w[s][i] = *reinterpret_cast<const v4i*>(p.w + (wb[i] + kt) * 1024 + off);
-        a[s][i] = *reinterpret_cast<const v4i*>(p.a + (ab[i] + kt) * 1024 + off);
-      }
+      for (int i = 0; i < TI; ++i) sw_[i] = nsw[i];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        acc[i][j] = mfma4<0>(w[0][i], ws[i], a[0][j], as[j], acc[i][j]);
-        acc[i][j] = mfma4<1>(w[1][i], ws[i], a[1][j], as[j], acc[i][j]);
-      }
+      for (int j = 0; j < TJ; ++j) sa_[j] = nsa[j];
+      b = bn;
+    }
   }
+  wait_vmcnt<0>();
+  __syncthreads();   // the ring becomes the output staging
+
+  // Lane l holds, of tile (i, j): row m = 32 j + l % 32, outputs n = 32 i + 8 q + 4 (l / 32) .. + 3 in elements 4 q ... They
+  // go through LDS two weight tiles at a time so that whole 128-byte lines are stored.
+  const int nb = n0 + wn * (BN / 2), mb = m0 + wm * (BM / WMW);
+  uint8_t* const stage = smem + wave * 32 * T::PITCH;
+  v4i tv[R ? R / 16 : 1];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < TJ; ++j) {
+    if constexpr (R > 0) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int m = m0 + 32 * j + l32, n = n0 + 32 * i + l32;
-      if constexpr (R > 0) {
+      for (int s = 0; s < R / 16; ++s)
+        tv[s] = *reinterpret_cast<const v4i*>(p.t + (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + 16 * s + 8 * half);
+    }
 #pragma unroll
-        for (int s = 0; s < R / 16; ++s) {
-          const v4i b = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(n, p.N - 1) * R + 16 * s + 8 * half);
-          const v4i t = *reinterpret_cast<const v4i*>(p.t + (int64_t)min(m, p.M - 1) * p.ldt + 16 * s + 8 * half);
-          acc[i][j] = mfma16<DT>(b, t, acc[i][j]);
+    for (int ih = 0; ih < TI / 2; ++ih) {
+#pragma unroll
+      for (int ii = 0; ii < 2; ++ii) {
+        const int i = 2 * ih + ii;
+        v16f y = acc[i][j];
+        if constexpr (R > 0) {
+#pragma unroll
+          for (int s = 0; s < R / 16; ++s) {
+            const v4i l = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(nb + 32 * i + l32, p.N - 1) * R + 16 * s + 8 * half);
+            y = mfma16<DT>(l, tv[s], y);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = nb + 32 * i + 8 * q + 4 * half;
+          v4f o = v4f{y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]};
+          if (p.bias && n < p.N) {
+            const v4f bv = *reinterpret_cast<const v4f*>(p.bias + n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += bv[e];
+          }
+          *reinterpret_cast<v2u*>(stage + l32 * T::PITCH + (ii * 32 + 8 * q + 4 * half) * 2) =
+              v2u{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
         }
       }
+      const int n = nb + ih * 64 + (lane & 7) * 8, row = lane >> 3;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int nq = n0 + 32 * i + 8 * q + 4 * half;
-        if (m < p.M && nq < p.N) {
-          float y[4];
+      for (int r0 = 0; r0 < 32; r0 += 8) {
+        const int m = mb + 32 * j + r0 + row;
+        const v4u v = *reinterpret_cast<const v4u*>(stage + (r0 + row) * T::PITCH + (lane & 7) * 16);
+        if (m < p.M && n < p.N) {
+          v4u* const dst = reinterpret_cast<v4u*>(p.c + (int64_t)m * p.ldc + n);
+          if constexpr (OCC == 1) __builtin_nontemporal_store(v, dst);
+          else *dst = v;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+template <int TI, int TJ, int WMW, int NS, int OCC>
+int launch_ring(GemmArgs p, int dtype, int r, hipStream_t stream) {
+  using T = Ring<TI, TJ, WMW, NS>;
+  p.tiles_m = (p.M + T::BM - 1) / T::BM;
+  p.tiles_n = (p.N + T::BN - 1) / T::BN;
+  const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
+  if (const int st = check_grid(blocks, 128 * WMW, "mx_gemm")) return st;
+#define PQ_MXG(D, RR) \
+  hipLaunchKernelGGL((mx_gemm_kernel<TI, TJ, WMW, NS, OCC, D, RR>), dim3((unsigned)blocks), dim3(128 * WMW), 0, stream, p)
+  if (dtype == PQ_BF16) {
+    if (r == 0) PQ_MXG(PQ_BF16, 0); else if (r == 32) PQ_MXG(PQ_BF16, 32); else PQ_MXG(PQ_BF16, 64);
+  } else {
+    if (r == 0) PQ_MXG(PQ_F16, 0); else if (r == 32) PQ_MXG(PQ_F16, 32); else PQ_MXG(PQ_F16, 64);
+  }
+#undef PQ_MXG
+  return check_launch("mx_gemm");
+}
+
+// ---- few blocks --------------------------------------------------------------------------------------------------------
+// Where the blocks of the kernel above would leave most compute units idle, a workgroup of NW waves takes a block of 32 TI x 32
+// TJ and its waves every NW-th stage of K, each with all of the block's sums; fragments come from memory into registers, D
+// stages ahead, and the waves' sums are added in LDS in a fixed order. QUANT: x is 16-bit, and each lane quantizes the very
+// blocks its fragments are (32 consecutive values of a row), so few rows need no quantizer of their own before the product.
+struct SplitArgs {
+  GemmArgs g;
+  const uint16_t* x;   // QUANT
+  int64_t ldx;
+  int K;
+};
+
+template <int TI, int TJ, int NW, int D, int DT, int R, bool QUANT>
+__global__ __launch_bounds__(64 * NW) void mx_gemm_split_kernel(const SplitArgs sp) {
+  const GemmArgs& p = sp.g;
+  __shared__ float part[NW][64 * 17];   // one 32 x 32 tile of each wave, 16 sums a lane (17: spread over the banks)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 32 * TI, m0 = blockIdx.y * 32 * TJ, KT = p.KT;
+  const int l32 = lane & 31, half = lane >> 5, r16 = lane & 15, sw = k64_swz(r16);
+  int64_t wb[TI], ab[TJ];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = acc[i][j][4 * q + e] + (p.bias ? p.bias[nq + e] : 0.0f);
-          *reinterpret_cast<v2u*>(p.c + (int64_t)m * p.ldc + nq) = v2u{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+  for (int i = 0; i < TI; ++i)   // (row blocks past the end repeat the last one: their outputs are not stored)
+    wb[i] = (int64_t)min((n0 + 32 * i + l32) >> 4, (p.N - 1) >> 4) * KT;
+#pragma unroll
+  for (int j = 0; j < TJ; ++j)
+    ab[j] = QUANT ? (int64_t)(m0 + 32 * j + l32) * sp.ldx : (int64_t)min((m0 + 32 * j + l32) >> 4, (p.M - 1) >> 4) * KT;
+  struct Stage {
+    v4i w[2][TI], a[2][QUANT ? 1 : TJ];
+    Block<DT> x[2][QUANT ? TJ : 1];
+    int ws[TI], as[QUANT ? 1 : TJ];
+  } st[D];
+  auto load = [&](Stage& g, int kt) {
+#pragma unroll
+    for (int i = 0; i < TI; ++i) g.ws[i] = *reinterpret_cast<const uint16_t*>(p.ws + (wb[i] + kt) * 64 + r16 * 4 + 2 * half);
+    if constexpr (!QUANT) {
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) g.as[j] = *reinterpret_cast<const uint16_t*>(p.as + (ab[j] + kt) * 64 + r16 * 4 + 2 * half);
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int off = r16 * 64 + (((2 * s + half) ^ sw) << 4);
+#pragma unroll
+      for (int i = 0; i < TI; ++i) g.w[s][i] = *reinterpret_cast<const v4i*>(p.w + (wb[i] + kt) * 1024 + off);
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        if constexpr (QUANT) {
+          const int k = kt * 128 + (2 * s + half) * kBlock;
+          if (m0 + 32 * j + l32 < p.M && k < sp.K) g.x[s][j].template load<true>(sp.x + ab[j] + k);
+          else g.x[s][j].zero();
+        } else {
+          g.a[s][j] = *reinterpret_cast<const v4i*>(p.a + (ab[j] + kt) * 1024 + off);
+        }
+      }
+    }
+  };
+  v16f acc[TI][TJ] = {};
+  auto products = [&](auto s, const Stage& g) {
+    constexpr int S = decltype(s)::value;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      v4i a;
+      int as;
+      if constexpr (QUANT) {
+        as = g.x[S][j].scale_byte();
+        a = g.x[S][j].codes(as);
+        as = as << (8 * S);
+      } else {
+        a = g.a[S][j];
+        as = g.as[j];
+      }
+#pragma unroll
+      for (int i = 0; i < TI; ++i) acc[i][j] = mfma4<S>(g.w[S][i], g.ws[i], a, as, acc[i][j]);
+    }
+  };
+  const int mine = (KT - wave + NW - 1) / NW;   // stages wave, wave + NW, ..
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (d < mine) load(st[d], wave + d * NW);
+  for (int c = 0; c < mine; c += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (c + d < mine) {
+        products(std::integral_constant<int, 0>{}, st[d]);
+        products(std::integral_constant<int, 1>{}, st[d]);
+        if (c + d + D < mine) load(st[d], wave + (c + d + D) * NW);
+      }
+    }
+  }
+  // The waves' sums, a tile at a time; thread t adds element t of the 1024 (4 outputs of a row for each of 256 threads).
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      if (i + j) __syncthreads();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) part[wave][lane * 17 + r] = acc[i][j][r];
+      __syncthreads();
+      if (wave == (i * TJ + j) % NW) {   // one wave joins the tile: its lanes hold the layout the low-rank products have
+        v16f y = {};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float s = 0.0f;
+#pragma unroll
+          for (int u = 0; u < NW; ++u) s += part[u][lane * 17 + r];
+          y[r] = s;
+        }
+        const int m = m0 + 32 * j + l32;
+        if constexpr (R > 0) {
+#pragma unroll
+          for (int s = 0; s < R / 16; ++s) {
+            const v4i l = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(n0 + 32 * i + l32, p.N - 1) * R + 16 * s + 8 * half);
+            const v4i t = *reinterpret_cast<const v4i*>(p.t + (int64_t)min(m, p.M - 1) * p.ldt + 16 * s + 8 * half);
+            y = mfma16<DT>(l, t, y);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = n0 + 32 * i + 8 * q + 4 * half;
+          if (m < p.M && n < p.N) {
+            v4f o = v4f{y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]};
+            if (p.bias) {
+              const v4f bv = *reinterpret_cast<const v4f*>(p.bias + n);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[e] += bv[e];
+            }
+            *reinterpret_cast<v2u*>(p.c + (int64_t)m * p.ldc + n) = v2u{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
+          }
         }
       }
     }
 }
+
+template <int TI, int TJ, int NW, int D, bool QUANT>
+int launch_split(const SplitArgs& p, int dtype, int r, hipStream_t stream) {
+  const int64_t bm = (p.g.M + 32 * TJ - 1) / (32 * TJ), bn = (p.g.N + 32 * TI - 1) / (32 * TI);
+  if (bm > 65535) return set_error(PQ_ESHAPE, "mx_gemm: M=%d too large", p.g.M);
+  if (const int st = check_grid(bn, 64 * NW, "mx_gemm")) return st;
+#define PQ_MXP(D_, RR)                                                                                              \
+  hipLaunchKernelGGL((mx_gemm_split_kernel<TI, TJ, NW, D, D_, RR, QUANT>), dim3((unsigned)bn, (unsigned)bm), dim3(64 * NW), \
+                     0, stream, p)
+  if (dtype == PQ_BF16) {
+    if (r == 0) PQ_MXP(PQ_BF16, 0); else if (r == 32) PQ_MXP(PQ_BF16, 32); else PQ_MXP(PQ_BF16, 64);
+  } else {
+    if (r == 0) PQ_MXP(PQ_F16, 0); else if (r == 32) PQ_MXP(PQ_F16, 32); else PQ_MXP(PQ_F16, 64);
+  }
+#undef PQ_MXP
+  return check_launch("mx_gemm");
+}
+
+// The block of a product, by how its blocks fill the chip. us, K = 3072 unless said (bf16, rank 32, bias):
+//   M x K x N            256x256  128x128  128x64  128x256  32x32 split
+//   65536 x 3072 x 12288   1562     1839    2294     1893       -
+//   4096 x 3072 x 3072     31.1     33.1    39.0     38.9     92.3
+//   2050 x 1280 x 5120     17.7     21.3    22.5     22.9     48.3      180 blocks of 256 x 256
+//   512 x 3072 x 12288     24.9     24.2    24.3     20.0     47.6      192 blocks of 128 x 256, 384 of 128 x 128
+//   1024 x 3072 x 3072     23.3     12.6    11.7     17.5     24.8      384 blocks of 128 x 64
+//   512 x 12288 x 3072     65.9     30.4    25.1     49.3     39.3
+//   256 x 3072 x 3072      23.3     11.5     8.5     17.0      8.1      768 blocks of 32 x 32
+//   154 x 2048 x 1280      18.5      9.2     6.7     13.1      4.2
+//   1 x 12288 x 3072       62.6     28.3    21.4     47.3      8.7
+// (n x m; 256 x 256 and 128 x 256: one workgroup per CU, 128 x 128 and 128 x 64: two.)
+int launch_gemm(const GemmArgs& p, int dtype, int r, hipStream_t stream) {
+  auto blocks = [&](int bn, int bm) { return (int64_t)((p.N + bn - 1) / bn) * ((p.M + bm - 1) / bm); };
+  int cus = persistent_workgroups(stream);
+  if (cus <= 0) cus = 256;
+  if (blocks(32, 32) <= 3 * cus) return launch_split<1, 1, 8, 4, false>({p, nullptr, 0, 0}, dtype, r, stream);
+  if (blocks(256, 256) > cus / 2) return launch_ring<4, 2, 4, 4, 1>(p, dtype, r, stream);
+  if (blocks(128, 256) <= cus && blocks(128, 128) > cus) return launch_ring<2, 2, 4, 4, 1>(p, dtype, r, stream);
+  if (blocks(128, 64) <= 2 * cus) return launch_ring<2, 1, 2, 4, 2>(p, dtype, r, stream);
+  return launch_ring<2, 2, 2, 4, 2>(p, dtype, r, stream);
+}
+
+// Rows that the product's own lanes quantize: a block's lanes hold 32 rows, so each row is quantized once per 32 outputs.
+constexpr int kQuantRows = 32;
 
 }  // namespace
 }  // namespace mx
@@ -121,17 +470,32 @@ extern "C" int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8
       ldc % 8 || (uintptr_t)bias % 16 || (t && ((uintptr_t)t % 16 || (uintptr_t)l2t % 16 || ldt % 8)))
     return set_error(PQ_EALIGN, "pq_mx_gemm: operands 16-byte aligned, ldc and ldt multiples of 8");
   mx::GemmArgs p{a, a_scales, w, w_scales, bias, static_cast<const uint16_t*>(t), static_cast<const uint16_t*>(l2t),
-                 static_cast<uint16_t*>(c), ldt, ldc, (int)M, (int)N, mx::stages(K)};
-  const int64_t bn = (N + 127) / 128, bm = (M + 127) / 128;
-  if (bm > 65535) return set_error(PQ_ESHAPE, "pq_mx_gemm: M=%lld too large", (long long)M);
-  const dim3 grid((unsigned)bn, (unsigned)bm), block(256);
-  const int r = t ? (int)R : 0;
-#define PQ_MXG(D, RR) hipLaunchKernelGGL((mx::mx_gemm_kernel<D, RR>), grid, block, 0, stream, p)
-  if (dtype == PQ_BF16) {
-    if (r == 0) PQ_MXG(PQ_BF16, 0); else if (r == 32) PQ_MXG(PQ_BF16, 32); else PQ_MXG(PQ_BF16, 64);
-  } else {
-    if (r == 0) PQ_MXG(PQ_F16, 0); else if (r == 32) PQ_MXG(PQ_F16, 32); else PQ_MXG(PQ_F16, 64);
-  }
-#undef PQ_MXG
-  return check_launch("mx_gemm");
+                 static_cast<uint16_t*>(c), ldt, ldc, (int)M, (int)N, mx::stages(K), 0, 0};
+  return mx::launch_gemm(p, dtype, t ? (int)R : 0, stream);
+}
+
+extern "C" int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w,
+                            const uint8_t* w_scales, const float* bias, const void* l1t, const void* l2t, int64_t R, void* y,
+                            int64_t ldy, int64_t N, uint8_t* codes, uint8_t* scales, int8_t* q8, void* t, hipStream_t stream) {
+  if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || ldx < K || ldy < N || ldy >= (1LL << 31) || M > (1 << 30) ||
+      N > (1 << 30) || K > (1 << 22))
+    return set_error(PQ_ESHAPE, "pq_mx_linear: M=%lld N=%lld K=%lld ldx=%lld ldy=%lld (N %% 16 == 0, K %% 32 == 0)", (long long)M,
+                     (long long)N, (long long)K, (long long)ldx, (long long)ldy);
+  if (dtype != PQ_BF16 && dtype != PQ_F16) return set_error(PQ_EDTYPE, "pq_mx_linear: dtype %d", dtype);
+  if (R != 0 && R != 32 && R != 64) return set_error(PQ_ESHAPE, "pq_mx_linear: rank %lld (0, 32 or 64)", (long long)R);
+  if (M == 0) return PQ_OK;
+  if (!x || !w || !w_scales || !y || !codes || !scales || (R && (!l1t || !l2t || !t)))
+    return set_error(PQ_EINVAL, "pq_mx_linear: null pointer");
+  if ((uintptr_t)x % 16 || ldx % 8 || (uintptr_t)w % 16 || (uintptr_t)w_scales % 16 || (uintptr_t)y % 16 || ldy % 8 ||
+      (uintptr_t)bias % 16 || (uintptr_t)codes % 16 || (uintptr_t)scales % 16 || (uintptr_t)q8 % 16 ||
+      (R && ((uintptr_t)l1t % 16 || (uintptr_t)l2t % 16 || (uintptr_t)t % 16)))
+    return set_error(PQ_EALIGN, "pq_mx_linear: operands 16-byte aligned, ldx and ldy multiples of 8");
+  mx::GemmArgs p{codes, scales, w, w_scales, bias, static_cast<const uint16_t*>(R ? t : nullptr), static_cast<const uint16_t*>(l2t),
+                 static_cast<uint16_t*>(y), R, ldy, (int)M, (int)N, mx::stages(K), 0, 0};
+  if (R)
+    if (const int st = pq_lowrank_down(x, dtype, M, K, ldx, M, nullptr, l1t, R, t, R, stream)) return st;
+  if (M <= mx::kQuantRows && !q8)
+    return mx::launch_split<1, 1, 8, 2, true>({p, static_cast<const uint16_t*>(x), ldx, (int)K}, dtype, (int)R, stream);
+  if (const int st = pq_mx_quant(x, dtype, M, K, ldx, codes, scales, q8, stream)) return st;
+  return mx::launch_gemm(p, dtype, (int)R, stream);
 }

@@ -247,6 +247,28 @@ def lay_out_factors(lr_A: torch.Tensor, lr_B: torch.Tensor, down: bool = True, u
 
 
 # --------------------------------------------------------------------------- the layer
+def _layer_call(x2, w_codes, w_scales, N, bias, At, Bt, keep_x=False, keep_t=False):
+    """(y, q8, x_scales, t) of one layer call (pq_mx_linear) on rows as _rows gives them; q8 and x_scales where ``keep_x``, t
+    where ``keep_t``, else None. What is not kept shares one allocation that ends with the call."""
+    M, K = x2.shape
+    dev, dt = x2.device, x2.dtype
+    code = _dtype16(dt)
+    units, P = _stages(M, K), 0 if At is None else At.shape[0]
+    t_bytes = 2 * M * P
+    y = torch.empty((M, N), dtype=dt, device=dev)
+    q8 = torch.empty((M, K), dtype=torch.int8, device=dev) if keep_x else None
+    x_scales = torch.empty(units * 64, dtype=torch.uint8, device=dev) if keep_x else None
+    t = torch.empty((M, P), dtype=dt, device=dev) if keep_t else None
+    work = torch.empty(units * (1024 if keep_x else 1088) + (0 if keep_t else t_bytes), dtype=torch.uint8, device=dev)
+    codes = work.data_ptr()
+    scales = x_scales.data_ptr() if keep_x else codes + units * 1024
+    t_at = t.data_ptr() if keep_t else codes + units * (1024 if keep_x else 1088)
+    _lib.check(_lib.load().pq_mx_linear(x2.data_ptr(), code, M, K, _stride(x2), w_codes.data_ptr(), w_scales.data_ptr(),
+                                        _lib.ptr(bias), _lib.ptr(At), _lib.ptr(Bt), P, y.data_ptr(), N, N, codes, scales,
+                                        _lib.ptr(q8), t_at if P else None, _lib.stream_of(dev)), "mxfp4 layer")
+    return y, q8, x_scales, t
+
+
 class _Linear4(torch.autograd.Function):
     """y [M, N] of x2 [M, K]. lr_A and lr_B: the factors [K, R] and [R, N], or in the kernels' forward order [P, K] and [N, P]
     (``laid_out``)."""
@@ -254,15 +276,10 @@ class _Linear4(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2, lr_A, lr_B, bias, codes, scales, N, laid_out):
         M, K = x2.shape
-        wq = Mxfp4Matrix(codes, scales, N, K)
         need_x, need_A, need_B, need_b = ctx.needs_input_grad[:4]
         back = need_x or need_A or need_B or need_b
         x2 = _rows(x2)
-        q8 = t = Ap = Bp = None
-        xq = quant_mxfp4(x2, need_A)
-        if need_A:
-            xq, q8 = xq
-        Bt = None
+        At = Ap = Bt = Bp = None
         if lr_A is not None:
             if laid_out:
                 At, Bt = lr_A, lr_B
@@ -270,10 +287,9 @@ class _Linear4(torch.autograd.Function):
                     Bp, _, Ap, _ = lay_out_factors(Bt, At, True, False)
             else:
                 At, Ap, Bt, Bp = lay_out_factors(lr_A, lr_B, True, back)
-            t = lowrank_down(x2, At)
-        y = mxfp4_gemm(xq, wq, bias, x2.dtype, t=t, l2t=Bt)
+        y, q8, x_scales, t = _layer_call(x2, codes, scales, N, bias, At, Bt, need_A, need_B or need_b)
         if back:
-            ctx.save_for_backward(q8, xq.scales if need_A else None, t if need_B or need_b else None, Ap, Bp, codes, scales)
+            ctx.save_for_backward(q8, x_scales, t, Ap, Bp, codes, scales)
             ctx.wq_shape, ctx.rank = (N, K), None if lr_A is None or laid_out else lr_A.shape[1]
         return y
 
@@ -383,6 +399,9 @@ class Mxfp4Linear(nn.Module):
             A, B = self.lr_At, self.lr_Bt
         if A is not None and (A.dtype != dt or B.dtype != dt):
             A, B = A.to(dt), B.to(dt)
+        if not self.trainable and not (torch.is_grad_enabled() and x.requires_grad):
+            y = _layer_call(_rows(x2), self.weight_codes, self.weight_scales, self.out_features, bias, A, B)[0]
+            return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)
         y = _Linear4.apply(x2, A, B, bias, self.weight_codes, self.weight_scales, self.out_features, not self.trainable)
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)
 
