@@ -426,10 +426,13 @@ int pq_mx_factors(const void* A, int64_t lda, const void* B, int64_t ldb, int64_
  * dx[m, k] = sum_n dy[m, n] wh[n, k] (+ sum_r dt[m, r] ap[k, r]): the gradient of a layer's input over its packed 4-bit weight
  * [N, K], widened to dtype on the way to the matrix instructions (exact; in fp16, for 2^-22 <= 2^E <= 2^13), summed in fp32.
  * dy [M, N], dx [M, K] of dtype; dt [M, R] and ap [K, R] contiguous, R in {32, 64}, or NULL. Operands 16-byte aligned, lddy and
- * lddx multiples of 8.
+ * lddx multiples of 8, lddy <= 2^21. A workspace of pq_mx_grad_input_workspace_size bytes (0 for most sizes) that may hold
+ * anything.
  */
+int64_t pq_mx_grad_input_workspace_size(int64_t M, int64_t N, int64_t K);
 int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, const uint8_t* w, const uint8_t* w_scales, const void* dt,
-                     const void* ap, int64_t R, void* dx, int64_t lddx, int64_t M, int64_t N, int64_t K, hipStream_t stream);
+                     const void* ap, int64_t R, void* dx, int64_t lddx, int64_t M, int64_t N, int64_t K, void* workspace,
+                     int64_t workspace_bytes, hipStream_t stream);
 
 /*
  * The gradients of the low-rank factors and the bias: dB[r, n] = sum_m t[m, r] dy[m, n] ([R, N]), dA[k, r] = sum_m xt[m, k]

@@ -49,6 +49,7 @@ EXPORTS = (
     "pq_mx_gemm",
     "pq_mx_linear",
     "pq_mx_factors",
+    "pq_mx_grad_input_workspace_size",
     "pq_mx_grad_input",
     "pq_mx_grad_factors_workspace_size",
     "pq_mx_grad_factors",
@@ -93,7 +94,8 @@ _SIGNATURES = {
     "pq_mx_gemm": ([_p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p], ctypes.c_int),
     "pq_mx_linear": ([_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
     "pq_mx_factors": ([_p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
-    "pq_mx_grad_input": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p], ctypes.c_int),
+    "pq_mx_grad_input_workspace_size": ([_i64, _i64, _i64], _i64),
+    "pq_mx_grad_input": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p], ctypes.c_int),
     "pq_mx_grad_factors_workspace_size": ([_i64, _i64, _i64, _i64], _i64),
     "pq_mx_grad_factors": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p],
                            ctypes.c_int),

@@ -30,33 +30,6 @@ __device__ __forceinline__ v16f mfma4(v4i a, int sa, v4i b, int sb, v16f c) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, b8, c, 4, 4, S, sa, S, sb);
 }
 
-template <int DT>
-__device__ __forceinline__ v16f mfma16(v4i a, v4i b, v16f c) {
-  if constexpr (DT == PQ_BF16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-}
-
-// Workgroup id -> (tile_m, tile_n): ids are dealt round-robin over the 8 XCDs, so each XCD takes a contiguous run of the
-// tiles, rastered in groups of `group` m-tiles so that the tiles it works on at a time share rows of both operands in its L2.
-__device__ __forceinline__ void tile_of(int bid, int blocks, int tiles_m, int tiles_n, int group, int& tm, int& tn) {
-  const int per = blocks >> 3, rem = blocks & 7, xcd = bid & 7;
-  const int at = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (bid >> 3);
-  const int g = at / (group * tiles_n), first = g * group, size = min(tiles_m - first, group), r = at - g * group * tiles_n;
-  tm = first + r % size;
-  tn = r / size;
-}
-
-// Workgroup barrier that leaves LDS-DMA in flight (__syncthreads() would wait for all of it): this wave's LDS reads are done,
-// and nothing moves across it.
-__device__ __forceinline__ void ring_barrier() {
-  __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_sched_barrier(0);
-}
-
 // Sums of one output block, then its epilogue. WMW waves along m times 2 along n; each wave holds TI x TJ tiles of 32 x 32 (n
 // x m). K advances in stages of 128 values (64 bytes a row) through a ring of NS stages in LDS, filled by LDS-DMA: NS - 1
 // stages in flight, no registers or LDS writes spent on them. A stage is the row blocks of the packed layout as they are (the
@@ -127,6 +100,8 @@ void mx_gemm_kernel(const GemmArgs p) {
     for (int i = 0; i < TI; ++i) w[i] = *reinterpret_cast<const uint16_t*>(sb + (fw >> 4) + i * 128);
 #pragma unroll
     for (int j = 0; j < TJ; ++j) a[j] = *reinterpret_cast<const uint16_t*>(sb + (fa >> 4) + j * 128);
+  };
+  auto settle = [&](int (&w)[TI], int (&a)[TJ]) {
     // (kept here: the compiler would put the masking of the words between the products that use them)
 #pragma unroll
     for (int i = 0; i < TI; ++i) asm volatile("" : "+v"(w[i]));
@@ -160,6 +135,7 @@ void mx_gemm_kernel(const GemmArgs p) {
       rd(w1, a1, b, 1);
       rd_scales(sw_, sa_, b);
       dma(b == 0 ? NS - 1 : b - 1, s + NS - 1);
+      settle(sw_, sa_);
       if (grp_b) wait_vmcnt<(NS - 2) * T::DPW>();
       ring_barrier();
       mm(S0{}, w0, a0, sw_, sa_);
@@ -422,27 +398,26 @@ int launch_split(const SplitArgs& p, int dtype, int r, hipStream_t stream) {
   return check_launch("mx_gemm");
 }
 
-// The block of a product, by how its blocks fill the chip. us, K = 3072 unless said (bf16, rank 32, bias):
-//   M x K x N            256x256  128x128  128x64  128x256  32x32 split
+// The block of a product, by how its blocks fill the chip. us (bf16, rank 32, bias):
+//   M x K x N            256x256  128x128  128x64  128x256  32x32 split   (n x m; 256x256, 128x256: one workgroup per CU)
 //   65536 x 3072 x 12288   1562     1839    2294     1893       -
 //   4096 x 3072 x 3072     31.1     33.1    39.0     38.9     92.3
 //   2050 x 1280 x 5120     17.7     21.3    22.5     22.9     48.3      180 blocks of 256 x 256
 //   512 x 3072 x 12288     24.9     24.2    24.3     20.0     47.6      192 blocks of 128 x 256, 384 of 128 x 128
-//   1024 x 3072 x 3072     23.3     12.6    11.7     17.5     24.8      384 blocks of 128 x 64
+//   1024 x 3072 x 3072     23.3     12.6    11.7     17.5     24.8      384 blocks of 128 x 64, 192 of 128 x 128
 //   512 x 12288 x 3072     65.9     30.4    25.1     49.3     39.3
 //   256 x 3072 x 3072      23.3     11.5     8.5     17.0      8.1      768 blocks of 32 x 32
 //   154 x 2048 x 1280      18.5      9.2     6.7     13.1      4.2
 //   1 x 12288 x 3072       62.6     28.3    21.4     47.3      8.7
-// (n x m; 256 x 256 and 128 x 256: one workgroup per CU, 128 x 128 and 128 x 64: two.)
+// (128 x 128 wins nowhere and is not built. What the last line gets fits two of its workgroups per CU at once.)
 int launch_gemm(const GemmArgs& p, int dtype, int r, hipStream_t stream) {
   auto blocks = [&](int bn, int bm) { return (int64_t)((p.N + bn - 1) / bn) * ((p.M + bm - 1) / bm); };
   int cus = persistent_workgroups(stream);
   if (cus <= 0) cus = 256;
   if (blocks(32, 32) <= 3 * cus) return launch_split<1, 1, 8, 4, false>({p, nullptr, 0, 0}, dtype, r, stream);
   if (blocks(256, 256) > cus / 2) return launch_ring<4, 2, 4, 4, 1>(p, dtype, r, stream);
-  if (blocks(128, 256) <= cus && blocks(128, 128) > cus) return launch_ring<2, 2, 4, 4, 1>(p, dtype, r, stream);
-  if (blocks(128, 64) <= 2 * cus) return launch_ring<2, 1, 2, 4, 2>(p, dtype, r, stream);
-  return launch_ring<2, 2, 2, 4, 2>(p, dtype, r, stream);
+  if (blocks(128, 128) > cus) return launch_ring<2, 2, 4, 4, 1>(p, dtype, r, stream);
+  return launch_ring<2, 1, 2, 4, 2>(p, dtype, r, stream);
 }
 
 // Rows that the product's own lanes quantize: a block's lanes hold 32 rows, so each row is quantized once per 32 outputs.

@@ -10,20 +10,18 @@ namespace pq {
 namespace mx {
 namespace {
 
-template <int DT>
-__device__ __forceinline__ v16f mfma16(v4i a, v4i b, v16f c) {
-  if constexpr (DT == PQ_BF16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-}
-
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s_t;
+typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
 
 // Matrix operand from a tile held row-major along the other axis: lane l gets, of column c0 + l % 32, the 8 rows
 // r0 + 8 (l / 32) .. + 7. Each 16 lanes read a 4 x 16 patch (8 bytes a lane) that the transposing read hands back by
 // columns. `at(row, chunk)`: address of the 16 bytes holding columns 8 chunk .. of a row.
+//
+// Such a tile's rows are a multiple of 256 bytes, and 16 lanes read 32 bytes of each of 4 consecutive rows (32 lanes 64): chunk c
+// of a row sits at c ^ spread(row), so that those fall on distinct banks in 128- and in 256-byte windows (bits 1-2 of the
+// four values of spread are distinct, and so are bits 2-3).
+__device__ __forceinline__ int spread(int row) { return (0xca60 >> ((row & 3) << 2)) & 15; }
 template <typename At>
 __device__ __forceinline__ v4i read_columns(At at, int r0, int c0, int lane) {
   const int i = lane & 15, row = r0 + 8 * (lane >> 5) + (i >> 2), col = c0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
@@ -41,65 +39,102 @@ struct DxArgs {
   uint16_t* dx;
   int64_t lddy, lddx;
   int M, N, K, KT;
+  int tiles_m, tiles_k;
+  float* part;   // a split over n: [slices][M][K], `slice` n each
+  int slice;
 };
 
-// A workgroup of four waves: 128 rows m x 128 columns k (one stage of the packed weight), 64 n a step. The 4-bit weights are
-// widened to 16 bits on their way into LDS, and read back by columns.
-template <int DT, int R>
+// Few blocks: a workgroup of four waves takes 64 rows m x 128 columns k (one stage of the packed weight), 64 n a step. dy and
+// the 4-bit weights of the next two steps are on their way into registers while the products of this one run, then go to the
+// other of two LDS buffers, the weights widened to 16 bits on the way; they are read back by columns. One barrier a step.
+// SPLIT: blockIdx.z takes a slice of n and leaves its sums in fp32 in p.part [slices][M][K] for mx_dx_join_kernel.
+template <int DT, int R, bool SPLIT>
 __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
-  __shared__ __attribute__((aligned(16))) uint8_t sa[128 * 128];   // [m][64 n]
-  __shared__ __attribute__((aligned(16))) uint8_t sw[64 * 256];    // [n][128 k]
+  constexpr int BM = 64, A = BM * 128, W = 64 * 256, LA = BM / 32, TJ = BM / 64;   // 16-byte loads of dy a thread; m tiles of a wave
+  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * (A + W)];      // [m][64 n] and [n][128 k], twice
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int kt = blockIdx.x, k0 = kt * 128, m0 = blockIdx.y * 128;
-  const int wk = (wave & 1) * 64, wm = (wave >> 1) * 64;
+  const int kt = blockIdx.x, k0 = kt * 128, m0 = blockIdx.y * BM;
+  const int wk = (wave & 1) * 64, wm = (wave >> 1) * (BM / 2);
   const int l32 = lane & 31, half = lane >> 5;
-  auto a_at = [&](int row, int chunk) { return sa + row * 128 + ((chunk ^ (row & 7)) << 4); };
-  auto w_at = [&](int row, int chunk) { return sw + row * 256 + ((chunk ^ ((row & 3) << 2)) << 4); };
-  v16f acc[2][2] = {};   // [k tile][m tile]
-  for (int n0 = 0; n0 < p.N; n0 += 64) {
-    __syncthreads();
+  const int first = SPLIT ? blockIdx.z * p.slice : 0, end = SPLIT ? min(p.N, first + p.slice) : p.N;
+  const int arow = tid >> 3, achunk = tid & 7, wrow = tid >> 2, wb = tid & 3;
+  const bool in_k = k0 + wb * 32 < p.K;
+  struct Step {
+    v4u dy[LA], c;
+    int byte;
+  } next[2];
+  auto load = [&](Step& g, int n0) {
+    const int n = n0 + achunk * 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {   // dy: 8 chunks of 8 n a row, 32 rows a pass
-      const int row = i * 32 + (tid >> 3), chunk = tid & 7, n = n0 + chunk * 8;
-      v4u v = v4u{0, 0, 0, 0};
-      if (m0 + row < p.M && n < p.N) v = *reinterpret_cast<const v4u*>(p.dy + (int64_t)(m0 + row) * p.lddy + n);
-      *reinterpret_cast<v4u*>(a_at(row, chunk)) = v;
+    for (int i = 0; i < LA; ++i) {
+      const int m = m0 + arow + 32 * i;
+      g.dy[i] = v4u{0, 0, 0, 0};
+      if (m < p.M && n < end) g.dy[i] = *reinterpret_cast<const v4u*>(p.dy + (int64_t)m * p.lddy + n);
     }
-    {   // weights: a thread widens one block of 32 k of one n
-      const int row = tid >> 2, b = tid & 3, n = n0 + row;
-      const bool in = n < p.N && k0 + b * 32 < p.K;
-      v4u c = v4u{0, 0, 0, 0};
-      int byte = 0;
-      if (in) {
-        c = *reinterpret_cast<const v4u*>(p.w + code_offset(n, kt, b, p.KT));
-        byte = p.ws[scale_offset(n, kt, b, p.KT)];
-      }
-      const float s = scale_value(byte);
-      constexpr uint32_t nn = nan2<DT>();
+    g.c = v4u{0, 0, 0, 0};
+    g.byte = 0;
+    if (in_k && n0 + wrow < end) {
+      g.c = *reinterpret_cast<const v4u*>(p.w + code_offset(n0 + wrow, kt, wb, p.KT));
+      g.byte = p.ws[scale_offset(n0 + wrow, kt, wb, p.KT)];
+    }
+  };
+  auto store = [&](const Step& g, int buf) {
+    uint8_t* const sa = smem + buf * (A + W);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<v4u*>(w_at(row, b * 4 + i)) = byte == kNaN ? v4u{nn, nn, nn, nn} : widen8<DT>(c[i], s);
+    for (int i = 0; i < LA; ++i) {
+      const int row = arow + 32 * i;
+      *reinterpret_cast<v4u*>(sa + row * 128 + ((achunk ^ (row & 7)) << 4)) = g.dy[i];
     }
+    const float s = scale_value(g.byte);
+    const uint32_t nan = g.byte == kNaN ? nan2<DT>() : 0;   // (such a block's codes are 0: or-ing makes every value NaN)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<v4u*>(sa + A + wrow * 256 + (((wb * 4 + i) ^ spread(wrow)) << 4)) = widen8<DT>(g.c[i], s) | nan;
+  };
+  v16f acc[2][TJ] = {};   // [k tile][m tile]
+  load(next[0], first);
+  load(next[1], first + 64);
+  store(next[0], 0);
+  auto step = [&](Step& coming, Step& after, int n0, int buf) {   // after: the step two ahead; coming: the next
     __syncthreads();
+    load(after, n0 + 128);   // (past the end: loads nothing)
+    const uint8_t* const sa = smem + buf * (A + W);
+    auto w_at = [&](int row, int chunk) { return sa + A + row * 256 + ((chunk ^ spread(row)) << 4); };
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      v4i w[2], a[2];
+      v4i w[2], a[TJ];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        w[i] = read_columns(w_at, 16 * s, wk + 32 * i, lane);
-        a[i] = *reinterpret_cast<const v4i*>(a_at(wm + 32 * i + l32, 2 * s + half));
+      for (int i = 0; i < 2; ++i) w[i] = read_columns(w_at, 16 * s, wk + 32 * i, lane);
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        const int row = wm + 32 * j + l32;
+        a[j] = *reinterpret_cast<const v4i*>(sa + row * 128 + (((2 * s + half) ^ (row & 7)) << 4));
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<DT>(w[i], a[j], acc[i][j]);
+        for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16<DT>(w[i], a[j], acc[i][j]);
     }
+    store(coming, buf ^ 1);
+  };
+  for (int n0 = first; n0 < end; n0 += 128) {
+    step(next[1], next[0], n0, 0);
+    if (n0 + 64 < end) step(next[0], next[1], n0 + 64, 1);
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < TJ; ++j) {
       const int m = m0 + wm + 32 * j + l32, kk = k0 + wk + 32 * i;
+      if (SPLIT) {
+        if (m < p.M && kk < p.K) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<v4f*>(p.part + ((int64_t)blockIdx.z * p.M + m) * p.K + kk + 8 * q + 4 * half) =
+                v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        }
+        continue;
+      }
       if constexpr (R > 0) {
 #pragma unroll
         for (int s = 0; s < R / 16; ++s) {
@@ -114,6 +149,241 @@ __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
           *reinterpret_cast<v2u*>(p.dx + (int64_t)m * p.lddx + kk + 8 * q + 4 * half) =
               v2u{pack2<DT>(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack2<DT>(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
       }
+    }
+}
+
+// dx from the slices' sums, added in order, and the low-rank term. A wave takes 32 rows x 32 columns.
+template <int DT, int R>
+__global__ __launch_bounds__(256) void mx_dx_join_kernel(const DxArgs p, int slices) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, half = lane >> 5;
+  const int kk = blockIdx.x * 128 + wave * 32, m = blockIdx.y * 32 + l32;
+  if (kk >= p.K) return;
+  v16f acc = {};
+  if (m < p.M) {
+    for (int z = 0; z < slices; ++z) {
+      const float* const src = p.part + ((int64_t)z * p.M + m) * p.K + kk + 4 * half;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const v4f v = *reinterpret_cast<const v4f*>(src + 8 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[4 * q + e] += v[e];
+      }
+    }
+  }
+  if constexpr (R > 0) {
+#pragma unroll
+    for (int s = 0; s < R / 16; ++s) {
+      const v4i b = *reinterpret_cast<const v4i*>(p.ap + (int64_t)(kk + l32) * R + 16 * s + 8 * half);
+      const v4i t = *reinterpret_cast<const v4i*>(p.dt + (int64_t)min(m, p.M - 1) * R + 16 * s + 8 * half);
+      acc = mfma16<DT>(b, t, acc);
+    }
+  }
+  if (m < p.M) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<v2u*>(p.dx + (int64_t)m * p.lddx + kk + 8 * q + 4 * half) =
+          v2u{pack2<DT>(acc[4 * q], acc[4 * q + 1]), pack2<DT>(acc[4 * q + 2], acc[4 * q + 3])};
+  }
+}
+
+// A workgroup of eight waves: 256 rows m x 256 columns k, each wave 64 x 128 of it (2 x 4 tiles). n advances in steps of 32.
+//  * dy comes by LDS-DMA in stages of 64 n (whole 128-byte lines of a row) through a ring of three; 16-byte chunk c of a row
+//    sits at c ^ (row % 8), so the fragments' ds_read_b128 meet no bank conflicts.
+//  * The weight's codes and scales come by LDS-DMA as they are stored, through a ring of five steps; a step ahead of its
+//    use each thread widens 16 of them to 16 bits into one of two [32 n][256 k] buffers, whose transposing reads give
+//    fragments along n. So a weight is widened once per 256 rows, and memory and cache hold it in 4 bits.
+//  * Two groups of four waves, one of each per SIMD, take turns: one issues a step's 16 products back to back while the other
+//    reads its fragments, widens its part of the next step's weights and issues its DMA. Group B runs one slot behind.
+// In its memory phase of step s a wave issues half of dy stage s / 2 + 2 and its part of codes s + 5. Slot 2 s reads dy step s
+// and codes s + 2, all issued by phase s - 3; the barrier before it has every wave wait for all but its two younger phases.
+// LDS, per step: fragments 8 waves x 12 KB, dy 16 KB in, weights 16 KB in: as many cycles as the products take (bf16 products
+// of 32 x 32 x 16 at 32 cycles, 128 bytes of LDS a cycle), so the kernel is bound by both at once, and by the power limit.
+struct DxTile {
+  // (64 bytes after each KB of codes: the 128 values that two of them hold of a row are read together)
+  static constexpr int DY = 256 * 128, BLOCK = 1024 + 64, CODES = 4 * BLOCK + 1024, W = 32 * 512;
+  static constexpr int AT_CODES = 3 * DY, AT_W = AT_CODES + 5 * CODES, LDS = AT_W + 2 * W + 3 * 1024;   // (and room for the three
+  static constexpr int PITCH = 144;                                                                     // waves that bring nothing)
+};
+
+template <int DT, int R>
+__global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
+void mx_dx_ring_kernel(const DxArgs p) {
+  using T = DxTile;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[T::LDS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wk = wave & 1, wm = wave >> 1, l32 = lane & 31, half = lane >> 5;
+  int tm, tk;
+  tile_of(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_k, 6, tm, tk);
+  const int m0 = tm * 256, k0 = tk * 256, kt0 = tk * 2, KT = p.KT;
+  const int rows = min(256, p.M - m0), NB = (p.N + 15) >> 4, steps = (p.N + 31) >> 5;
+
+  // Loads outside their buffers give zeros: rows past M and n past N of dy, and n past N or k past K of the weight.
+  const auto rs_dy = __builtin_amdgcn_make_buffer_rsrc((void*)(p.dy + (int64_t)m0 * p.lddy), (short)0,
+                                                       (int)(((rows - 1) * p.lddy + p.N) * 2), kBufferWord3);
+  const int lddy2 = (int)p.lddy * 2;
+  const int dchunk = (lane & 7) ^ (lane >> 3);   // row % 8 == lane / 8
+  const int vdy = (wave * 32 + (lane >> 3)) * lddy2 + dchunk * 16;
+  // Codes: wave w < 4 brings row block w / 2, stage kt0 + w % 2 of a step; wave 4 the scales, 64 bytes for each of the four;
+  // the others bring nothing (a step counts the same number of DMA instructions for every wave).
+  const int unit = wave < 4 ? 1024 : wave == 4 ? 64 : 0, kb = wave < 4 ? wave & 1 : (lane >> 2) & 1;
+  const int vc = kt0 + kb < KT && (wave < 4 || lane < 16)
+      ? ((wave < 4 ? wave >> 1 : lane >> 3) * KT + kt0 + kb) * unit + (wave < 4 ? lane : lane & 3) * 16 : kOOB;
+  // (the steps go out in order: a pointer, the row blocks left and the ring's slot move along)
+  const uint8_t* cptr = wave < 4 ? p.w : p.ws;
+  const int64_t cstep = (int64_t)2 * KT * unit;
+  int cleft = NB, cslot = 0;
+  const int cdst = wave < 4 ? wave * T::BLOCK : 4 * T::BLOCK;
+  auto dma_codes = [&]() {
+    const uint64_t at = (uint64_t)cptr;   // (the same in every lane: kept in scalar registers)
+    const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at) |
+                          (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32;
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, __builtin_amdgcn_readfirstlane(max(0, min(2, cleft)) * KT * unit), kBufferWord3);
+    uint8_t* const dst = smem + (wave <= 4 ? T::AT_CODES + cslot * T::CODES + cdst : T::LDS - 1024 * (8 - wave));
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)dst, 16, vc, 0, 0, 0);
+    cptr += cstep;
+    cleft -= 2;
+    cslot = cslot == 4 ? 0 : cslot + 1;
+  };
+  auto dma = [&](int u) {   // phase u's part: dy half u % 2 of stage u / 2 + 2, codes u + 5
+    const int st = (u >> 1) + 2, n = st * 64 + dchunk * 8;
+    uint8_t* const sb = smem + st % 3 * T::DY + wave * 4096 + (u & 1) * 2048;
+    const int off = n < p.N ? vdy + (u & 1) * 16 * lddy2 + st * 128 : kOOB;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_dy, (lds_void_t*)sb, 16, off, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_dy, (lds_void_t*)(sb + 1024), 16, n < p.N ? off + 8 * lddy2 : kOOB, 0, 0, 0);
+    dma_codes();
+  };
+  // 16 values of a step: row n = tid / 16 of 32, columns 16 (tid % 16) .. Read in one phase, widened in the next: neither waits
+  // for the other. (Lanes 4-7 of 8 store their second half first: eight lanes' 16-byte stores meet no bank twice.)
+  const int wr = tid >> 4, wc = tid & 15, wblk = (wr >> 4) * 2 + (wc >> 3), wb4 = (wc & 7) >> 1, turn = (wc >> 2) & 1;
+  v2u wq;
+  int wbyte;
+  v4u wide[2];
+  int rslot = 0;   // (read in order too)
+  auto rd_codes = [&]() {
+    const uint8_t* const cb = smem + T::AT_CODES + rslot * T::CODES;
+    rslot = rslot == 4 ? 0 : rslot + 1;
+    wq = *reinterpret_cast<const v2u*>(cb + wblk * T::BLOCK + (wr & 15) * 64 + ((wb4 ^ k64_swz(wr & 15)) << 4) + (wc & 1) * 8);
+    wbyte = cb[4 * T::BLOCK + wblk * 64 + (wr & 15) * 4 + scale_slot(wb4)];
+  };
+  auto widen = [&]() {
+    const float s = scale_value(wbyte);
+    const uint32_t nan = wbyte == kNaN ? nan2<DT>() : 0;   // (such a block's codes are 0: or-ing makes every value NaN)
+    wide[0] = widen8<DT>(turn ? wq[1] : wq[0], s) | nan;
+    wide[1] = widen8<DT>(turn ? wq[0] : wq[1], s) | nan;
+  };
+  auto put = [&](int c) {
+    uint8_t* const row = smem + T::AT_W + (c & 1) * T::W + wr * 512;
+    *reinterpret_cast<v4u*>(row + (((2 * wc + turn) ^ spread(wr)) << 4)) = wide[0];
+    *reinterpret_cast<v4u*>(row + (((2 * wc + 1 - turn) ^ spread(wr)) << 4)) = wide[1];
+  };
+  // Fragments of the weight (read_columns, in one block of assembly that ends with its own wait: the compiler would wait for
+  // every DMA in flight before the builtin's reads). Four tiles of 32 columns, rows 0-15 and 16-31 of the step.
+  v4i a[2][2];
+  uint32_t wat[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 8 * half + ((lane & 15) >> 2), col = wk * 128 + 32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    wat[i] = (uint32_t)(uintptr_t)(lds_u8_t*)(smem + T::AT_W) + row * 512 + (((col >> 3) ^ spread(row)) << 4) + (col & 4) * 2;
+  }
+  auto rd_dy = [&](int s) {
+    const uint8_t* const ab = smem + (s >> 1) % 3 * T::DY;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = wm * 64 + 32 * j + l32, chunk = (s & 1) * 4 + 2 * h + half;
+        a[h][j] = *reinterpret_cast<const v4i*>(ab + row * 128 + ((chunk ^ (row & 7)) << 4));
+      }
+  };
+  v16f acc[4][2] = {};
+  const bool grp_b = wave >= 4;
+  dma_codes();
+#pragma unroll
+  for (int u = -4; u < 0; ++u) dma(u);
+  wait_vmcnt<6>();
+  ring_barrier();
+  rd_codes();
+  widen();
+  put(0);
+  rd_codes();
+  widen();
+  ring_barrier();
+  if (grp_b) ring_barrier();
+  for (int s = 0; s < steps; ++s) {
+    put(s + 1);
+    rd_codes();
+    rd_dy(s);
+    dma(s);
+    const uint32_t flip = (s & 1) * T::W;
+    v4i w0, w1, w2, w3, w4, w5, w6, w7;
+    asm volatile(
+        "ds_read_b64_tr_b16 v[220:221], %[p0]\n\tds_read_b64_tr_b16 v[222:223], %[p0] offset:2048\n\t"
+        "ds_read_b64_tr_b16 v[224:225], %[p1]\n\tds_read_b64_tr_b16 v[226:227], %[p1] offset:2048\n\t"
+        "ds_read_b64_tr_b16 v[228:229], %[p2]\n\tds_read_b64_tr_b16 v[230:231], %[p2] offset:2048\n\t"
+        "ds_read_b64_tr_b16 v[232:233], %[p3]\n\tds_read_b64_tr_b16 v[234:235], %[p3] offset:2048\n\t"
+        "ds_read_b64_tr_b16 v[236:237], %[p0] offset:8192\n\tds_read_b64_tr_b16 v[238:239], %[p0] offset:10240\n\t"
+        "ds_read_b64_tr_b16 v[240:241], %[p1] offset:8192\n\tds_read_b64_tr_b16 v[242:243], %[p1] offset:10240\n\t"
+        "ds_read_b64_tr_b16 v[244:245], %[p2] offset:8192\n\tds_read_b64_tr_b16 v[246:247], %[p2] offset:10240\n\t"
+        "ds_read_b64_tr_b16 v[248:249], %[p3] offset:8192\n\tds_read_b64_tr_b16 v[250:251], %[p3] offset:10240\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&{v[220:223]}"(w0), "=&{v[224:227]}"(w1), "=&{v[228:231]}"(w2), "=&{v[232:235]}"(w3), "=&{v[236:239]}"(w4),
+          "=&{v[240:243]}"(w5), "=&{v[244:247]}"(w6), "=&{v[248:251]}"(w7)
+        : [p0] "v"(wat[0] + flip), [p1] "v"(wat[1] + flip), [p2] "v"(wat[2] + flip), [p3] "v"(wat[3] + flip)
+        : "memory");
+    if (grp_b) wait_vmcnt<6>();
+    ring_barrier();
+    const v4i w[2][4] = {{w0, w1, w2, w3}, {w4, w5, w6, w7}};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<DT>(w[h][i], a[h][j], acc[i][j]);
+    widen();   // (between the products)
+    asm volatile("" : "+v"(wide[0]), "+v"(wide[1]));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+    }
+    if (!grp_b) wait_vmcnt<6>();
+    ring_barrier();
+  }
+  if (!grp_b) ring_barrier();
+  wait_vmcnt<0>();
+  __syncthreads();   // the rings become the output staging
+
+  const int kb0 = k0 + wk * 128, mb = m0 + wm * 64;
+  uint8_t* const stage = smem + wave * 32 * T::PITCH;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int ih = 0; ih < 2; ++ih) {
+#pragma unroll
+      for (int ii = 0; ii < 2; ++ii) {
+        const int i = 2 * ih + ii;
+        v16f y = acc[i][j];
+        if constexpr (R > 0) {
+#pragma unroll
+          for (int s = 0; s < R / 16; ++s) {
+            const v4i l = *reinterpret_cast<const v4i*>(p.ap + (int64_t)min(kb0 + 32 * i + l32, p.K - 1) * R + 16 * s + 8 * half);
+            const v4i t = *reinterpret_cast<const v4i*>(p.dt + (int64_t)min(mb + 32 * j + l32, p.M - 1) * R + 16 * s + 8 * half);
+            y = mfma16<DT>(l, t, y);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<v2u*>(stage + l32 * T::PITCH + (ii * 32 + 8 * q + 4 * half) * 2) =
+              v2u{pack2<DT>(y[4 * q], y[4 * q + 1]), pack2<DT>(y[4 * q + 2], y[4 * q + 3])};
+      }
+      const int k = kb0 + ih * 64 + (lane & 7) * 8, row = lane >> 3;
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += 8) {
+        const int m = mb + 32 * j + r0 + row;
+        const v4u v = *reinterpret_cast<const v4u*>(stage + (r0 + row) * T::PITCH + (lane & 7) * 16);
+        if (m < p.M && k < p.K) *reinterpret_cast<v4u*>(p.dx + (int64_t)m * p.lddx + k) = v;
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -136,7 +406,7 @@ __global__ __launch_bounds__(256) void mx_rowsum_kernel(const SumArgs p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c0 = blockIdx.x * 128, s0 = blockIdx.y * p.rows;
   const int end = min(p.M, s0 + p.rows);
-  auto z_at = [&](int row, int chunk) { return sz + row * 256 + ((chunk ^ ((row & 3) << 2)) << 4); };
+  auto z_at = [&](int row, int chunk) { return sz + row * 256 + ((chunk ^ spread(row)) << 4); };
   auto v_at = [&](int row, int chunk) { return sv + row * R * 2 + (chunk << 4); };
   const uint32_t one2 = DT == PQ_BF16 ? 0x3f803f80u : 0x3c003c00u;
   const v4i ones = {(int)one2, (int)one2, (int)one2, (int)one2};
@@ -200,23 +470,98 @@ __global__ __launch_bounds__(256) void mx_rowsum_kernel(const SumArgs p) {
   }
 }
 
-// The slices' sums added in order: out[r, c] (TRANS: out[c, r]) rounded to 16 bits, and the column sums in 32.
+// The slices' sums added in order: out[r, c] (TRANS: out[c, r]) rounded to 16 bits, and the column sums in 32. A thread sums one element, eight slices' loads in flight.
+__device__ __forceinline__ float sum_slices(const float* at, int slices, int64_t step) {
+  float s = 0.0f;
+  int i = 0;
+  for (; i + 8 <= slices; i += 8) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = at[(i + e) * step];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += v[e];
+  }
+  for (; i < slices; ++i) s += at[i * step];
+  return s;
+}
 template <int DT, bool TRANS>
 __global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ part, const float* __restrict__ part_cols,
                                                       int slices, int P, int R, int C, uint16_t* __restrict__ out,
                                                       float* __restrict__ cols) {
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63);
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), r = blockIdx.y * 4 + (threadIdx.x >> 6);
   if (c >= C) return;
-  for (int r = threadIdx.x >> 6; out && r < R; r += 4) {
-    float s = 0.0f;
-    for (int i = 0; i < slices; ++i) s += part[((int64_t)i * P + r) * C + c];
-    out[TRANS ? (int64_t)c * R + r : (int64_t)r * C + c] = (uint16_t)f32_to_16_bits<DT>(s);
+  if (out && r < R)
+    out[TRANS ? (int64_t)c * R + r : (int64_t)r * C + c] =
+        (uint16_t)f32_to_16_bits<DT>(sum_slices(part + (int64_t)r * C + c, slices, (int64_t)P * C));
+  if (cols && r == 0) cols[c] = sum_slices(part_cols + c, slices, C);
+}
+
+// How dx is computed: 256 x 256 blocks where they fill more than half the chip's 256 compute units; else 64 x 128 blocks, with
+// n cut into `slices` where that ends sooner. An estimate in us: a 64-n step of a block takes 0.62 where no more than three
+// blocks share a compute unit; a split costs a launch and 8 bytes an element and slice. Measured (bf16, rank 32):
+//   M x K x N            256 x 256  64 x 128, 1 slice  2 slices  4      8
+//   16384 x 3072 x 12288      1069       1838              -      -      -
+//   4352 x 3072 x 3072        89.2      132.3           160.4  188.9  306.5
+//   2050 x 5120 x 1280        42.5       54.0            78.9   99.2  168.9      180 blocks of 256 x 256
+//   2050 x 1280 x 5120       126.9       69.4            62.4   67.7   76.9
+//   1000 x 1312 x 1040        30.7       13.4            20.1   22.2   26.4
+//   512 x 3072 x 12288       292.7      124.3            90.8   71.5   78.2
+//   154 x 2048 x 640          21.1        8.8             9.5    9.5    9.6
+//   64 x 3072 x 3072          73.3       29.6            21.0   15.0   13.6
+struct DxPlan {
+  bool ring;
+  int slices, slice;
+};
+DxPlan dx_plan(int64_t M, int64_t N, int64_t K) {
+  if (((M + 255) / 256) * ((K + 255) / 256) > 128) return {true, 1, 0};
+  const int64_t blocks = ((M + 63) / 64) * stages(K);
+  const int steps = (int)((N + 63) / 64);
+  double best = 0;
+  int slices = 1;
+  for (int s = 1; s <= 8 && s <= steps; ++s) {
+    const double t = (steps + s - 1) / s * 0.62 * std::max(1.0, (double)(blocks * s) / 768) + (s > 1 ? 4 + s * (double)(M * K) * 2e-6 : 0);
+    if (s == 1 || t < best) best = t, slices = s;
   }
-  if (cols && threadIdx.x < 64) {
-    float s = 0.0f;
-    for (int i = 0; i < slices; ++i) s += part_cols[(int64_t)i * C + c];
-    cols[c] = s;
+  const int per = (steps + slices - 1) / slices;
+  return {false, (steps + per - 1) / per, per * 64};
+}
+
+int launch_dx(DxArgs p, int dtype, int r, hipStream_t stream) {
+#define PQ_MXD(...)                                                                                        \
+  do {                                                                                                     \
+    if (dtype == PQ_BF16) {                                                                                \
+      if (r == 0) PQ_MXK(PQ_BF16, 0); else if (r == 32) PQ_MXK(PQ_BF16, 32); else PQ_MXK(PQ_BF16, 64);     \
+    } else {                                                                                               \
+      if (r == 0) PQ_MXK(PQ_F16, 0); else if (r == 32) PQ_MXK(PQ_F16, 32); else PQ_MXK(PQ_F16, 64);        \
+    }                                                                                                      \
+  } while (0)
+  const DxPlan plan = dx_plan(p.M, p.N, p.K);
+  if (plan.ring) {
+    p.tiles_m = (p.M + 255) / 256;
+    p.tiles_k = (p.K + 255) / 256;
+    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_k;
+    if (const int st = check_grid(blocks, 512, "mx_grad_input")) return st;
+#define PQ_MXK(D, RR) hipLaunchKernelGGL((mx_dx_ring_kernel<D, RR>), dim3((unsigned)blocks), dim3(512), 0, stream, p)
+    PQ_MXD();
+#undef PQ_MXK
+    return check_launch("mx_grad_input");
   }
+  const dim3 grid((unsigned)p.KT, (unsigned)((p.M + 63) / 64), (unsigned)plan.slices);   // (at most 128 x 4 blocks of rows)
+  p.slice = plan.slice;
+  if (plan.slices == 1) {
+#define PQ_MXK(D, RR) hipLaunchKernelGGL((mx_dx_kernel<D, RR, false>), grid, dim3(256), 0, stream, p)
+    PQ_MXD();
+#undef PQ_MXK
+    return check_launch("mx_grad_input");
+  }
+  if (dtype == PQ_BF16) hipLaunchKernelGGL((mx_dx_kernel<PQ_BF16, 0, true>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((mx_dx_kernel<PQ_F16, 0, true>), grid, dim3(256), 0, stream, p);
+  const dim3 join((unsigned)((p.K + 127) / 128), (unsigned)((p.M + 31) / 32));
+#define PQ_MXK(D, RR) hipLaunchKernelGGL((mx_dx_join_kernel<D, RR>), join, dim3(256), 0, stream, p, plan.slices)
+  PQ_MXD();
+#undef PQ_MXK
+#undef PQ_MXD
+  return check_launch("mx_grad_input");
 }
 
 // Row slices of mx_rowsum_kernel: enough workgroups to fill the chip, none of fewer than 64 rows.
@@ -232,13 +577,19 @@ int row_slices(int64_t M, int64_t C) {
 
 using namespace pq;
 
+extern "C" int64_t pq_mx_grad_input_workspace_size(int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 16 || K < 32 || M > (1 << 30) || N > (1 << 21) || K > (1 << 22)) return 0;
+  const mx::DxPlan plan = mx::dx_plan(M, N, K);
+  return plan.slices > 1 ? 4 * plan.slices * M * K : 0;
+}
+
 extern "C" int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, const uint8_t* w, const uint8_t* w_scales,
                                 const void* dt, const void* ap, int64_t R, void* dx, int64_t lddx, int64_t M, int64_t N,
-                                int64_t K, hipStream_t stream) {
+                                int64_t K, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || lddy < N || lddx < K || M > (1 << 30) ||
-      N > (1 << 30) || K > (1 << 22))
-    return set_error(PQ_ESHAPE, "pq_mx_grad_input: M=%lld N=%lld K=%lld (N %% 16 == 0, K %% 32 == 0)", (long long)M,
-                     (long long)N, (long long)K);
+      lddy > (1 << 21) || K > (1 << 22))
+    return set_error(PQ_ESHAPE, "pq_mx_grad_input: M=%lld N=%lld K=%lld lddy=%lld (N %% 16 == 0, K %% 32 == 0, lddy <= 2^21)",
+                     (long long)M, (long long)N, (long long)K, (long long)lddy);
   if (dtype != PQ_BF16 && dtype != PQ_F16) return set_error(PQ_EDTYPE, "pq_mx_grad_input: dtype %d", dtype);
   if (dt && R != 32 && R != 64) return set_error(PQ_ESHAPE, "pq_mx_grad_input: rank %lld (32 or 64)", (long long)R);
   if (M == 0) return PQ_OK;
@@ -247,18 +598,11 @@ extern "C" int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, con
       (uintptr_t)dt % 16 || (uintptr_t)ap % 16)
     return set_error(PQ_EALIGN, "pq_mx_grad_input: operands 16-byte aligned, lddy and lddx multiples of 8");
   mx::DxArgs p{static_cast<const uint16_t*>(dy), w, w_scales, static_cast<const uint16_t*>(dt), static_cast<const uint16_t*>(ap),
-               static_cast<uint16_t*>(dx), lddy, lddx, (int)M, (int)N, (int)K, mx::stages(K)};
-  if ((M + 127) / 128 > 65535) return set_error(PQ_ESHAPE, "pq_mx_grad_input: M=%lld too large", (long long)M);
-  const dim3 grid((unsigned)p.KT, (unsigned)((M + 127) / 128)), block(256);
-  const int r = dt ? (int)R : 0;
-#define PQ_MXD(D, RR) hipLaunchKernelGGL((mx::mx_dx_kernel<D, RR>), grid, block, 0, stream, p)
-  if (dtype == PQ_BF16) {
-    if (r == 0) PQ_MXD(PQ_BF16, 0); else if (r == 32) PQ_MXD(PQ_BF16, 32); else PQ_MXD(PQ_BF16, 64);
-  } else {
-    if (r == 0) PQ_MXD(PQ_F16, 0); else if (r == 32) PQ_MXD(PQ_F16, 32); else PQ_MXD(PQ_F16, 64);
-  }
-#undef PQ_MXD
-  return check_launch("mx_grad_input");
+               static_cast<uint16_t*>(dx), lddy, lddx, (int)M, (int)N, (int)K, mx::stages(K), 0, 0, static_cast<float*>(workspace), 0};
+  const int64_t need = pq_mx_grad_input_workspace_size(M, N, K);
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+    return set_error(PQ_EINVAL, "pq_mx_grad_input: a workspace of %lld bytes, 16-byte aligned", (long long)need);
+  return mx::launch_dx(p, dtype, dt ? (int)R : 0, stream);
 }
 
 extern "C" int64_t pq_mx_grad_factors_workspace_size(int64_t M, int64_t K, int64_t N, int64_t P) {
@@ -287,7 +631,7 @@ extern "C" int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, c
   mx::SumArgs b{dy, nullptr, static_cast<const uint16_t*>(t), part, part + (int64_t)sb * P * N, lddy, (int)M, (int)N, 0, rows(sb)};
   mx::SumArgs a{q8, x_scales, static_cast<const uint16_t*>(dt), part, nullptr, K, (int)M, (int)K, mx::stages(K), rows(sk)};
   const dim3 gb((unsigned)((N + 127) / 128), (unsigned)sb), ga((unsigned)((K + 127) / 128), (unsigned)sk), block(256);
-  const dim3 jb((unsigned)((N + 63) / 64)), ja((unsigned)((K + 63) / 64));
+  const dim3 jb((unsigned)((N + 63) / 64), (unsigned)((R + 3) / 4)), ja((unsigned)((K + 63) / 64), (unsigned)((R + 3) / 4));
 #define PQ_MXS(D, PP)                                                                                                     \
   do {                                                                                                                   \
     if (dbias) hipLaunchKernelGGL((mx::mx_rowsum_kernel<D, PP, false, true>), gb, block, 0, stream, b);                  \

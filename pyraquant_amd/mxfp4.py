@@ -177,9 +177,12 @@ def mxfp4_grad_input(dy: torch.Tensor, wq: Mxfp4Matrix, dt: Optional[torch.Tenso
         assert lr_Ap is not None and dt.dtype == lr_Ap.dtype == dy.dtype and dt.is_contiguous() and lr_Ap.is_contiguous()
         assert tuple(dt.shape) == (M, R) and tuple(lr_Ap.shape) == (K, R), (tuple(dt.shape), tuple(lr_Ap.shape), M, K)
     dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
-    _lib.check(_lib.load().pq_mx_grad_input(_lib.ptr(dy), code, _stride(dy), _lib.ptr(wq.codes), _lib.ptr(wq.scales),
-                                            _lib.ptr(dt), _lib.ptr(lr_Ap), R, _lib.ptr(dx), K, M, N, K,
-                                            _lib.stream_of(dy.device)), "mxfp4_grad_input")
+    L = _lib.load()
+    size = L.pq_mx_grad_input_workspace_size(M, N, K)
+    ws = torch.empty(size, dtype=torch.uint8, device=dy.device) if size else None
+    _lib.check(L.pq_mx_grad_input(_lib.ptr(dy), code, _stride(dy), _lib.ptr(wq.codes), _lib.ptr(wq.scales),
+                                  _lib.ptr(dt), _lib.ptr(lr_Ap), R, _lib.ptr(dx), K, M, N, K, _lib.ptr(ws), size,
+                                  _lib.stream_of(dy.device)), "mxfp4_grad_input")
     return dx
 
 

@@ -44,11 +44,16 @@ def test_gemm_and_gradient_refusals():
     assert gemm(M=(1 << 30) + 1) == L.PQ_ESHAPE and gemm(M=0, a=None, c=None) == L.PQ_OK
 
     def dx(dy=P, ld=64, dt=None, ap=None, R=0, out=P, ldo=64, ty=0, M=4, N=64, K=64):
-        return lib.pq_mx_grad_input(dy, ty, ld, P, P, dt, ap, R, out, ldo, M, N, K, None)
+        return lib.pq_mx_grad_input(dy, ty, ld, P, P, dt, ap, R, out, ldo, M, N, K, None, 0, None)
 
     assert dx(N=24, ld=24) == L.PQ_ESHAPE and dx(K=33, ldo=40) == L.PQ_ESHAPE and dx(ld=32) == L.PQ_ESHAPE
     assert dx(ty=3) == L.PQ_EDTYPE and dx(dy=None) == L.PQ_EINVAL and dx(dy=ODD) == L.PQ_EALIGN and dx(ldo=68) == L.PQ_EALIGN
     assert dx(dt=P, ap=P, R=48) == L.PQ_ESHAPE and dx(dt=P, R=32) == L.PQ_EINVAL and dx(M=0, dy=None) == L.PQ_OK
+
+    big = dict(M=64, N=12288, K=1280, ld=12288, ldo=1280)      # few rows, a long sum: split, in a workspace
+    assert lib.pq_mx_grad_input_workspace_size(64, 12288, 1280) > 0 and dx(**big) == L.PQ_EINVAL
+    assert b"workspace" in lib.pq_last_error() and lib.pq_mx_grad_input_workspace_size(65536, 3072, 3072) == 0
+    assert dx(ld=(1 << 21) + 8) == L.PQ_ESHAPE
 
     def factors(dy=P, t=P, dt=P, q8=P, sc=P, M=4, K=64, N=64, R=8, PP=32, dA=P, dB=P, ws=P, size=1 << 40, ty=0):
         return lib.pq_mx_grad_factors(dy, ty, N, t, dt, q8, sc, M, K, N, R, PP, dA, dB, P, ws, size, None)

@@ -204,6 +204,48 @@ def test_layer_gradients(cuda, dtype, M, K, N, R):
         _inside(g, r[k], bound[k], k)
 
 
+@pytest.mark.parametrize("M,K,N", [(40, 96, 4112), (300, 288, 2080), (4128, 2080, 48), (8300, 1056, 112)])
+def test_input_gradient_of_every_kind_of_block(cuda, M, K, N):
+    """Sums cut into slices (few rows, a long n) and large blocks (more than half the chip's worth of 256 x 256, ragged both
+    ways)."""
+    import pyraquant_amd._lib as L
+    from pyraquant_amd.mxfp4 import mxfp4_grad_input, quant_mxfp4
+
+    split = L.load().pq_mx_grad_input_workspace_size(M, N, K) > 0
+    large = -(-M // 256) * -(-K // 256) > 128
+    assert split == (M < 1000) and large == (M > 1000)
+    g = torch.Generator(device="cuda").manual_seed(M)
+    for dtype, R in ((torch.bfloat16, 32), (torch.float16, 64)):
+        w = (torch.randn(N, K, generator=g, device=cuda) * 0.02).to(dtype)
+        dy, dt, ap = (torch.randn(*s, generator=g, device=cuda).to(dtype) for s in ((M, N), (M, R), (K, R)))
+        got = mxfp4_grad_input(dy, quant_mxfp4(w), dt, ap)
+        wh, u = ref.four_bits(w.cpu()).cuda(), U[dtype]      # (the oracle's values; sums in 64 bits on the GPU)
+        want = dy.double() @ wh + dt.double() @ ap.double().t()
+        terms = dy.double().abs() @ wh.abs() + dt.double().abs() @ ap.double().abs().t()
+        off = (N + R) * 2.0 ** -23 * terms
+        _inside(got, want.cpu(), (off + u * (want.abs() + off)).cpu() + 2.0 ** -25, (M, K, N, dtype))
+        assert torch.equal(got, mxfp4_grad_input(dy, quant_mxfp4(w), dt, ap))
+
+
+@pytest.mark.parametrize("M,K,N,R", [(2100, 160, 4112, 0), (600, 1056, 7056, 32), (513, 96, 2064, 64), (1100, 352, 912, 32)])
+def test_product_of_every_kind_of_block(cuda, M, K, N, R):
+    """Sizes whose product runs in blocks of 256 x 256, 128 x 256 and 128 x 64 (n x m), all of them ragged."""
+    from pyraquant_amd.mxfp4 import mxfp4_gemm, quant_mxfp4
+
+    g = torch.Generator(device="cuda").manual_seed(M)
+    for dtype in BOTH:
+        x, w = torch.randn(M, K, generator=g, device=cuda).to(dtype), (torch.randn(N, K, generator=g, device=cuda) * 0.02).to(dtype)
+        t, l2t = (torch.randn(n, R, generator=g, device=cuda).to(dtype) if R else None for n in (M, N))
+        bias = torch.randn(N, generator=g, device=cuda)
+        got = mxfp4_gemm(quant_mxfp4(x), quant_mxfp4(w), bias, dtype, t=t, l2t=l2t)
+        xh, wh, u = ref.four_bits(x.cpu()).cuda(), ref.four_bits(w.cpu()).cuda(), U[dtype]
+        want, terms = xh @ wh.t() + bias, xh.abs() @ wh.abs().t() + bias.abs()
+        if R:
+            want, terms = want + t.double() @ l2t.double().t(), terms + t.double().abs() @ l2t.double().abs().t()
+        off = (K + R + 2) * 2.0 ** -23 * terms
+        _inside(got, want.cpu(), (off + u * (want.abs() + off)).cpu() + 2.0 ** -25, (M, K, N, dtype))
+
+
 def test_gradients_against_differences(cuda):
     """In lr_A, lr_B and the bias the layer is a polynomial: along a direction (a, b, c), the loss sum(dy y) changes by the
     gradients' product with it plus the second-order term sum(dy (x a) b), so central differences of the oracle's y cancel that
