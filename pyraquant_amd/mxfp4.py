@@ -25,7 +25,6 @@ from typing import Callable, Dict, NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .int8_exec import LOWRANK_A_ATTR, LOWRANK_B_ATTR, is_bf16_whitelisted, lowrank_down
@@ -250,63 +249,13 @@ def lay_out_factors(lr_A: torch.Tensor, lr_B: torch.Tensor, down: bool = True, u
 
 
 # --------------------------------------------------------------------------- the layer
-def _layer_call(x2, w_codes, w_scales, N, bias, At, Bt, keep_x=False, keep_t=False):
-    """(y, q8, x_scales, t) of one layer call (pq_mx_linear) on rows as _rows gives them; q8 and x_scales where ``keep_x``, t
-    where ``keep_t``, else None. What is not kept shares one allocation that ends with the call."""
-    M, K = x2.shape
-    dev, dt = x2.device, x2.dtype
-    code = _dtype16(dt)
-    units, P = _stages(M, K), 0 if At is None else At.shape[0]
-    t_bytes = 2 * M * P
-    y = torch.empty((M, N), dtype=dt, device=dev)
-    q8 = torch.empty((M, K), dtype=torch.int8, device=dev) if keep_x else None
-    x_scales = torch.empty(units * 64, dtype=torch.uint8, device=dev) if keep_x else None
-    t = torch.empty((M, P), dtype=dt, device=dev) if keep_t else None
-    work = torch.empty(units * (1024 if keep_x else 1088) + (0 if keep_t else t_bytes), dtype=torch.uint8, device=dev)
-    codes = work.data_ptr()
-    scales = x_scales.data_ptr() if keep_x else codes + units * 1024
-    t_at = t.data_ptr() if keep_t else codes + units * (1024 if keep_x else 1088)
-    _lib.check(_lib.load().pq_mx_linear(x2.data_ptr(), code, M, K, _stride(x2), w_codes.data_ptr(), w_scales.data_ptr(),
-                                        _lib.ptr(bias), _lib.ptr(At), _lib.ptr(Bt), P, y.data_ptr(), N, N, codes, scales,
-                                        _lib.ptr(q8), t_at if P else None, _lib.stream_of(dev)), "mxfp4 layer")
-    return y, q8, x_scales, t
+_layer = None   # _mx.so's layer call, loaded at the first use
 
 
-class _Linear4(torch.autograd.Function):
-    """y [M, N] of x2 [M, K]. lr_A and lr_B: the factors [K, R] and [R, N], or in the kernels' forward order [P, K] and [N, P]
-    (``laid_out``)."""
-
-    @staticmethod
-    def forward(ctx, x2, lr_A, lr_B, bias, codes, scales, N, laid_out):
-        M, K = x2.shape
-        need_x, need_A, need_B, need_b = ctx.needs_input_grad[:4]
-        back = need_x or need_A or need_B or need_b
-        x2 = _rows(x2)
-        At = Ap = Bt = Bp = None
-        if lr_A is not None:
-            if laid_out:
-                At, Bt = lr_A, lr_B
-                if back:   # the other two orders, by the same rule with the factors' roles exchanged
-                    Bp, _, Ap, _ = lay_out_factors(Bt, At, True, False)
-            else:
-                At, Ap, Bt, Bp = lay_out_factors(lr_A, lr_B, True, back)
-        y, q8, x_scales, t = _layer_call(x2, codes, scales, N, bias, At, Bt, need_A, need_B or need_b)
-        if back:
-            ctx.save_for_backward(q8, x_scales, t, Ap, Bp, codes, scales)
-            ctx.wq_shape, ctx.rank = (N, K), None if lr_A is None or laid_out else lr_A.shape[1]
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        q8, x_scales, t, Ap, Bp, codes, scales = ctx.saved_tensors
-        need_x, need_A, need_B, need_b = ctx.needs_input_grad[:4]
-        wq = Mxfp4Matrix(codes, scales, *ctx.wq_shape)
-        dy = _rows(dy)
-        dt = lowrank_down(dy, Bp) if Bp is not None and (need_x or need_A) else None
-        dA, dB, db = lowrank_grads(dy, t, dt, q8, x_scales, ctx.rank, need_A, need_B, need_b)
-        dx = mxfp4_grad_input(dy, wq, dt, Ap) if need_x else None
-        return dx, dA, dB, db, None, None, None, None
+def _load_layer():
+    global _layer
+    _layer = _lib.load_mx()
+    return _layer
 
 
 class Mxfp4Linear(nn.Module):
@@ -343,7 +292,7 @@ class Mxfp4Linear(nn.Module):
         bias = None if lin.bias is None else lin.bias.detach().to(w.device, torch.float32).contiguous()
         if trainable:
             self.lr_A, self.lr_B = nn.Parameter(A.clone().contiguous()), nn.Parameter(B.clone().contiguous())
-            self.bias = None if bias is None else nn.Parameter(bias.clone())
+            self.register_parameter("bias", None if bias is None else nn.Parameter(bias.clone()))
         else:
             self._keep(A if self.rank else None, B if self.rank else None, bias)
 
@@ -389,24 +338,18 @@ class Mxfp4Linear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         assert x.shape[-1] == self.in_features, (tuple(x.shape), self.in_features)
-        _check_cuda(x, self.weight_codes)
+        d, trainable = self._buffers, self.trainable
+        if trainable:
+            p = self._parameters
+            A, B, bias = p["lr_A"], p["lr_B"], p["bias"]
+        else:
+            A, B, bias = d["lr_At"], d["lr_Bt"], d["bias"]
         dt = x.dtype
-        _dtype16(dt)
-        x2 = x if x.dim() == 2 else x.reshape(-1, self.in_features)
-        bias = self.bias
+        if A is not None and (A.dtype != dt or B.dtype != dt) and dt in (torch.bfloat16, torch.float16):
+            A, B = A.to(dt), B.to(dt)
         if bias is not None and bias.dtype != torch.float32:
             bias = bias.float()
-        if self.trainable:
-            A, B = self.lr_A, self.lr_B
-        else:
-            A, B = self.lr_At, self.lr_Bt
-        if A is not None and (A.dtype != dt or B.dtype != dt):
-            A, B = A.to(dt), B.to(dt)
-        if not self.trainable and not (torch.is_grad_enabled() and x.requires_grad):
-            y = _layer_call(_rows(x2), self.weight_codes, self.weight_scales, self.out_features, bias, A, B)[0]
-            return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)
-        y = _Linear4.apply(x2, A, B, bias, self.weight_codes, self.weight_scales, self.out_features, not self.trainable)
-        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)
+        return (_layer or _load_layer())(x, d["weight_codes"], d["weight_scales"], A, B, bias, self.out_features, not trainable)
 
     def extra_repr(self) -> str:
         lr = f", low-rank r={self.rank}" + (" (trainable)" if self.trainable else "") if self.rank else ""
