@@ -405,22 +405,38 @@ int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, cons
                int64_t K, hipStream_t stream);
 
 /*
- * A layer in one call: pq_mx_quant of x into codes and scales (and q8 unless NULL), t = x l1t^T into t [M, R] where R is 32 or 64
- * (0: no low-rank branch), and pq_mx_gemm into y [M, N] (row stride ldy). The caller's codes, scales, q8 and t have the sizes
+ * A layer in one call: pq_mx_quant of x into codes and scales (and q8 unless NULL), t = x lr_A into t [M, R] where R is 32 or 64 (0:
+ * no low-rank branch; l1f: lr_A in fragment order, l2t: lr_B's rows [N, R], both from pq_mx_factors), and pq_mx_gemm into y [M, N] (row stride ldy). The caller's codes, scales, q8 and t have the sizes
  * given above and may hold anything; up to 32 rows without q8 are quantized inside the product, which leaves codes and scales
- * alone. 16-byte aligned operands, ldx and ldy multiples of 8.
+ * alone. 16-byte aligned operands, ldx and ldy multiples of 8. With a low-rank branch, a workspace of
+ * pq_mx_lowrank_workspace_size(M, K, R) bytes (0 but for few long rows) that may hold anything.
  */
 int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, const uint8_t* w_scales,
-                 const float* bias, const void* l1t, const void* l2t, int64_t R, void* y, int64_t ldy, int64_t N, uint8_t* codes,
-                 uint8_t* scales, int8_t* q8, void* t, hipStream_t stream);
+                 const float* bias, const void* l1f, const void* l2t, int64_t R, void* y, int64_t ldy, int64_t N, uint8_t* codes,
+                 uint8_t* scales, int8_t* q8, void* t, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /*
- * The low-rank factors in the orders the layer's kernels read them, zero-padded from rank R to P (32 or 64): lr_A [K, R] (row
- * stride lda) to At [P, K] and Ap [K, P], lr_B [R, N] (row stride ldb) to Bt [N, P] and Bp [P, N]; an output may be NULL. All
- * 16-bit.
+ * The low-rank factors in the orders the layer's kernels read them, zero-padded from rank R to P (32 or 64), 16-bit, from one
+ * launch. A factor has C columns (k of lr_A, n of lr_B). A and B come as rows [C, R] (PQ_MX_BY_COLUMN, row stride ld), rows
+ * [R, C] (PQ_MX_BY_RANK, row stride ld), or fragments (PQ_MX_FRAGMENTS, as written here). Results, NULL where not wanted: ap
+ * [K, P] and bt [N, P] rows, af and bf fragments (ceil(C / 128) * 128 * P values, zeros past C; value (c, r) at
+ * ((((c >> 7) * 4 + ((c >> 3) & 3)) * (P / 16) + (r >> 4)) * 64 + ((c >> 5) & 3) * 16 + (r & 15)) * 8 + (c & 7)).
+ * The forward pass reads af and bt, the backward pass ap and bf. Results 16-byte aligned.
  */
-int pq_mx_factors(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, int64_t N, int64_t R, int64_t P, void* At,
-                  void* Ap, void* Bt, void* Bp, hipStream_t stream);
+#define PQ_MX_BY_COLUMN 0
+#define PQ_MX_BY_RANK 1
+#define PQ_MX_FRAGMENTS 2
+int pq_mx_factors(const void* A, int64_t lda, int32_t a_order, const void* B, int64_t ldb, int32_t b_order, int64_t K, int64_t N,
+                  int64_t R, int64_t P, void* af, void* ap, void* bt, void* bf, hipStream_t stream);
+
+/*
+ * t[m, r] = sum_k x[m, k] l1[k, r] ([M, R] of dtype, R in {32, 64}), l1 in fragment order (pq_mx_factors), summed in fp32 and
+ * rounded to dtype (PQ_BF16 or PQ_F16). K % 16 == 0; operands 16-byte aligned, ldx a multiple of 8. A workspace of
+ * pq_mx_lowrank_workspace_size bytes (0 but for few long rows) that may hold anything.
+ */
+int64_t pq_mx_lowrank_workspace_size(int64_t M, int64_t K, int64_t R);
+int pq_mx_lowrank_down(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R, void* t,
+                       void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /*
  * dx[m, k] = sum_n dy[m, n] wh[n, k] (+ sum_r dt[m, r] ap[k, r]): the gradient of a layer's input over its packed 4-bit weight

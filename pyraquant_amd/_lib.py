@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpqint8.s
 
 PQ_OK, PQ_EINVAL, PQ_ESHAPE, PQ_EALIGN, PQ_EDTYPE, PQ_ELAUNCH = 0, -1, -2, -3, -4, -5
 PQ_BF16, PQ_F16, PQ_I32, PQ_F32 = 0, 1, 2, 3
+PQ_MX_BY_COLUMN, PQ_MX_BY_RANK, PQ_MX_FRAGMENTS = 0, 1, 2   # orders of a low-rank factor (pq_mx_factors)
 PQ_ACCUMULATE = 0x100   # OR'ed into pq_int8_gemm_packed's out_dtype
 ABI_VERSION = 3
 
@@ -49,6 +50,8 @@ EXPORTS = (
     "pq_mx_gemm",
     "pq_mx_linear",
     "pq_mx_factors",
+    "pq_mx_lowrank_workspace_size",
+    "pq_mx_lowrank_down",
     "pq_mx_grad_input_workspace_size",
     "pq_mx_grad_input",
     "pq_mx_grad_factors_workspace_size",
@@ -92,8 +95,11 @@ _SIGNATURES = {
     "pq_mx_quant": ([_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p], ctypes.c_int),
     "pq_mx_values": ([_p, _p, _i32, _i64, _i64, _p, _i32, _i64, _p], ctypes.c_int),
     "pq_mx_gemm": ([_p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p], ctypes.c_int),
-    "pq_mx_linear": ([_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
-    "pq_mx_factors": ([_p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
+    "pq_mx_linear": ([_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p],
+                     ctypes.c_int),
+    "pq_mx_factors": ([_p, _i64, _i32, _p, _i64, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
+    "pq_mx_lowrank_workspace_size": ([_i64, _i64, _i64], _i64),
+    "pq_mx_lowrank_down": ([_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _p], ctypes.c_int),
     "pq_mx_grad_input_workspace_size": ([_i64, _i64, _i64], _i64),
     "pq_mx_grad_input": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p], ctypes.c_int),
     "pq_mx_grad_factors_workspace_size": ([_i64, _i64, _i64, _i64], _i64),

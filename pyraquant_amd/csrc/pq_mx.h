@@ -15,6 +15,12 @@
 namespace pq {
 namespace mx {
 
+// t = x l1t^T [M, R] and, unless codes is NULL, the codes of x (and q8), in one pass (pq_mx.hip). K % 16 == 0 (32 with codes),
+// 16-byte aligned rows, R 32 or 64, l1f: l1t in fragment order (pq_mx_factors); arguments checked by the caller.
+int lowrank(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R, uint8_t* codes,
+            uint8_t* scales, int8_t* q8, void* t, void* workspace, hipStream_t stream);
+int64_t lowrank_workspace(int64_t M, int64_t K, int64_t R);   // bytes of its workspace (0: none)
+
 constexpr int kBlock = 32;     // values that share a scale
 constexpr int kNaN = 255;      // scale byte of a block that is NaN
 

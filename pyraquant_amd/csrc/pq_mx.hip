@@ -7,6 +7,9 @@
 // 1/32 written (and 1 for the 8-bit codes).
 #include "pq_mx.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace pq {
 namespace mx {
 namespace {
@@ -40,6 +43,110 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(const void* __restrict__ 
       o[1] = q[1];
     }
   }
+}
+
+// t = x l1t^T ([M, R], 16-bit) and, where QUANT, the codes of x, in one pass over x. A workgroup takes 16 RG rows and its NW
+// waves every NW-th stage of 128 values, 16 rows at a time as above: what a lane holds of x for its block is also its operand
+// of the 16 x 16 x 32 products (8 consecutive values of a row; the order of k within the sum is free as long as l1t's operand
+// has the same), so x is read once and needs no other lane or LDS. l1t comes from the cache in fragment order (1 KB a load, zeros
+// past K), once per RG row groups. The
+// waves' sums are added in LDS in a fixed order and rounded once: t is rounded to 16 bits because the products that take it do.
+template <int DT, int R, int RG, int NW, bool QUANT, bool CKPT>
+__global__ __launch_bounds__(64 * NW) void mx_lowrank_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t M, int K, int KT,
+                                                             const uint16_t* __restrict__ l1f, uint8_t* __restrict__ codes,
+                                                             uint8_t* __restrict__ scales, int8_t* __restrict__ q8,
+                                                             uint16_t* __restrict__ t, float* __restrict__ partial) {
+  constexpr int C = R / 16;                                  // column tiles of t
+  __shared__ float part[NW][RG * C][64 * 4 + 4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, b = lane >> 4;
+  const int64_t m0 = (int64_t)blockIdx.x * (16 * RG);
+  v4f acc[RG][C] = {};
+  for (int kt = blockIdx.y * NW + wave; kt < KT; kt += NW * (int)gridDim.y) {
+    const int k = kt * 128 + b * kBlock;
+    Block<DT> blk[RG];
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      const int64_t row = m0 + 16 * g + l16;
+      const uint16_t* const src = x + row * ldx + k;
+      if (QUANT) {   // whole blocks
+        if (row < M && k < K) blk[g].template load<true>(src);
+        else blk[g].zero();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v4u v = v4u{0, 0, 0, 0};
+          if (row < M && k + 8 * i < K) v = *reinterpret_cast<const v4u*>(src + 8 * i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) blk[g].w[4 * i + e] = v[e];
+        }
+      }
+    }
+    v4i l[4][C];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        l[i][c] = *reinterpret_cast<const v4i*>(l1f + (((int64_t)kt * 4 + i) * C + c) * 512 + lane * 8);
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      const int64_t row = m0 + 16 * g + l16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v4i xv = {(int)blk[g].w[4 * i], (int)blk[g].w[4 * i + 1], (int)blk[g].w[4 * i + 2], (int)blk[g].w[4 * i + 3]};
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[g][c] = mfma16_16<DT>(l[i][c], xv, acc[g][c]);
+      }
+      if (QUANT && row < ((M + 15) & ~15LL)) {
+        const int byte = blk[g].scale_byte();
+        scales[scale_offset(row, kt, b, KT)] = (uint8_t)byte;
+        *reinterpret_cast<v4i*>(codes + code_offset(row, kt, b, KT)) = blk[g].codes(byte);
+        if (CKPT && row < M && k < K) {
+          v4i q[2];
+          blk[g].codes8(byte, q);
+          v4i* const o = reinterpret_cast<v4i*>(q8 + row * K + k);
+          o[0] = q[0];
+          o[1] = q[1];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < RG; ++g)
+#pragma unroll
+    for (int c = 0; c < C; ++c) *reinterpret_cast<v4f*>(&part[wave][g * C + c][lane * 4]) = acc[g][c];
+  __syncthreads();
+  // lane l of tile (g, c): row 16 g + l % 16, columns 16 c + 4 (l / 16) ..
+  for (int u = threadIdx.x; u < RG * C * 64; u += 64 * NW) {
+    const int tile = u >> 6, l = u & 63;
+    v4f sum = {};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const v4f v = *reinterpret_cast<const v4f*>(&part[w][tile][l * 4]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += v[e];
+    }
+    const int64_t row = m0 + 16 * (tile / C) + (l & 15);
+    if (row >= M) continue;
+    if (partial)
+      *reinterpret_cast<v4f*>(partial + (blockIdx.y * M + row) * R + 16 * (tile % C) + 4 * (l >> 4)) = sum;
+    else
+      *reinterpret_cast<v2u*>(t + row * R + 16 * (tile % C) + 4 * (l >> 4)) = v2u{pack2<DT>(sum[0], sum[1]), pack2<DT>(sum[2], sum[3])};
+  }
+}
+
+// t from the sums of workgroups that share rows (`partial` [slices][M R]), in order; a thread takes four.
+template <int DT>
+__global__ __launch_bounds__(256) void mx_lowrank_join_kernel(const float* __restrict__ partial, int slices, int64_t n,
+                                                              uint16_t* __restrict__ t) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  v4f sum = {};
+  for (int z = 0; z < slices; ++z) {
+    const v4f v = *reinterpret_cast<const v4f*>(partial + z * n + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += v[e];
+  }
+  *reinterpret_cast<v2u*>(t + i) = v2u{pack2<DT>(sum[0], sum[1]), pack2<DT>(sum[2], sum[3])};
 }
 
 // Values of the 4-bit codes (EIGHT: of the 8-bit ones), one lane a block. ODT: output type.
@@ -93,30 +200,50 @@ __global__ __launch_bounds__(256) void mx_values_kernel(const uint8_t* __restric
   }
 }
 
-// lr_A [K, R] -> At [P, K] and Ap [K, P]; lr_B [R, N] -> Bt [N, P] and Bp [P, N]: the four orders in which the layer's
-// kernels read the factors, zero-padded from rank R to P. A workgroup takes 64 rows k (or columns n) of one factor.
-__global__ __launch_bounds__(256) void mx_factors_kernel(const uint16_t* __restrict__ A, int64_t lda,
-                                                         const uint16_t* __restrict__ B, int64_t ldb, int K, int N, int R,
-                                                         int P, uint16_t* __restrict__ At, uint16_t* __restrict__ Ap,
-                                                         uint16_t* __restrict__ Bt, uint16_t* __restrict__ Bp, int blocks_a) {
-  __shared__ uint16_t tile[64][66];   // [k or n][r]; a pitch of 33 words: both directions spread over the banks
+// The factors in the orders the layer's kernels read them, zero-padded from rank R to P. A factor is a matrix of C columns c (k of
+// lr_A, n of lr_B) by r; a workgroup takes 64 columns of one. Source: [C, R] rows (kByColumn), [R, C] rows (kByRank) or
+// fragments. Results, either or none: rows [C, P], and fragments: for each 128 columns, 8-column group i of a block and
+// 16 ranks, the 64 lanes' 16 bytes in a row, as mx_lowrank_kernel loads them.
+__host__ __device__ __forceinline__ int64_t frag_offset(int c, int r, int P) {
+  return ((((int64_t)(c >> 7) * 4 + ((c >> 3) & 3)) * (P >> 4) + (r >> 4)) * 64 + ((c >> 5) & 3) * 16 + (r & 15)) * 8 + (c & 7);
+}
+struct Factor {
+  const uint16_t* src;
+  int64_t ld;
+  int kind, C;
+  uint16_t *rows, *frags;
+};
+__global__ __launch_bounds__(256) void mx_factors_kernel(const Factor fa, const Factor fb, int R, int P, int blocks_a) {
+  __shared__ uint16_t tile[64][66];   // [c][r]; a pitch of 33 words: both directions spread over the banks
   const bool is_a = (int)blockIdx.x < blocks_a;
-  const int c0 = ((int)blockIdx.x - (is_a ? 0 : blocks_a)) * 64, C = is_a ? K : N;
+  const Factor f = is_a ? fa : fb;
+  const int c0 = ((int)blockIdx.x - (is_a ? 0 : blocks_a)) * 64;
+  if (!f.rows && !f.frags) return;
   for (int i = threadIdx.x; i < 64 * P; i += 256) {
     int c, r;
-    if (is_a) { c = i / P; r = i - c * P; }   // read along r
-    else { r = i >> 6; c = i & 63; }          // read along n
-    const bool in = c0 + c < C && r < R;
-    tile[c][r] = !in ? 0 : is_a ? A[(int64_t)(c0 + c) * lda + r] : B[(int64_t)r * ldb + c0 + c];
+    if (f.kind == PQ_MX_BY_RANK) { r = i >> 6; c = i & 63; }   // read along c
+    else { c = i / P; r = i - c * P; }                         // read along r
+    const bool in = c0 + c < f.C && r < R;
+    tile[c][r] = !in ? 0 : f.kind == PQ_MX_BY_COLUMN ? f.src[(int64_t)(c0 + c) * f.ld + r]
+                         : f.kind == PQ_MX_BY_RANK   ? f.src[(int64_t)r * f.ld + c0 + c]
+                                                     : f.src[frag_offset(c0 + c, r, P)];
   }
   __syncthreads();
-  uint16_t* const by_c = is_a ? Ap : Bt;   // [C, P]
-  uint16_t* const by_r = is_a ? At : Bp;   // [P, C]
-  for (int i = threadIdx.x; i < 64 * P; i += 256) {
-    const int c = i / P, r = i - c * P;
-    if (by_c && c0 + c < C) by_c[(int64_t)(c0 + c) * P + r] = tile[c][r];
-    const int r2 = i >> 6, c2 = i & 63;
-    if (by_r && c0 + c2 < C) by_r[(int64_t)r2 * C + c0 + c2] = tile[c2][r2];
+  for (int i = threadIdx.x; i < 8 * P; i += 256) {
+    if (f.frags) {   // 8 columns of one rank: 16 bytes
+      const int g = i & 7, r = i >> 3;
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = tile[8 * g + 2 * e][r] | ((uint32_t)tile[8 * g + 2 * e + 1][r] << 16);
+      *reinterpret_cast<v4u*>(f.frags + frag_offset(c0 + 8 * g, r, P)) = v4u{w[0], w[1], w[2], w[3]};
+    }
+    if (f.rows) {    // 8 ranks of one column
+      const int g = i % (P / 8), c = i / (P / 8);
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = tile[c][8 * g + 2 * e] | ((uint32_t)tile[c][8 * g + 2 * e + 1] << 16);
+      if (c0 + c < f.C) *reinterpret_cast<v4u*>(f.rows + (int64_t)(c0 + c) * P + 8 * g) = v4u{w[0], w[1], w[2], w[3]};
+    }
   }
 }
 
@@ -134,12 +261,73 @@ int launch_quant(const void* x, int64_t M, int64_t K, int64_t ldx, uint8_t* code
   return check_launch("mx_quant");
 }
 
+// Slices of K for few rows: a compute unit draws 75-150 GB/s, and a group of 16 rows reads all of l1t, so below 128 groups long
+// rows are shared by up to eight workgroups (512 x 12288, rank 32: 23.5 us on 32 of them).
+int lowrank_slices(int64_t M, int64_t K) {
+  const int64_t groups = (M + 15) / 16;
+  return groups >= 128 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({8, 256 / groups, stages(K) / 16}));
+}
+
+template <int DT, int R, int RG, int NW>
+int launch_lowrank(const uint16_t* x, int64_t M, int64_t K, int64_t ldx, const uint16_t* l1f, uint8_t* codes, uint8_t* scales,
+                   int8_t* q8, uint16_t* t, float* partial, int slices, hipStream_t stream) {
+  const int64_t blocks = (M + 16 * RG - 1) / (16 * RG);
+  if (const int st = check_grid(blocks, 64 * NW, "mx_lowrank")) return st;
+  const dim3 grid((unsigned)blocks, (unsigned)slices), block(64 * NW);
+  const int KT = stages(K);
+#define PQ_MXL(Q, C) \
+  hipLaunchKernelGGL((mx_lowrank_kernel<DT, R, RG, NW, Q, C>), grid, block, 0, stream, x, ldx, M, (int)K, KT, l1f, codes, scales, q8, \
+                     t, partial)
+  if (!codes) PQ_MXL(false, false); else if (q8) PQ_MXL(true, true); else PQ_MXL(true, false);
+#undef PQ_MXL
+  return check_launch("mx_lowrank");
+}
+
 }  // namespace
 }  // namespace mx
 }  // namespace pq
 
 using namespace pq;
 using namespace pq::mx;
+
+int64_t pq::mx::lowrank_workspace(int64_t M, int64_t K, int64_t R) {
+  const int slices = lowrank_slices(M, K);
+  return slices > 1 ? 4 * slices * M * R : 0;
+}
+
+// Rows a workgroup takes, and its waves (us, bf16, rank 32, with the 4-bit codes):
+//   M x K            16 rows, 16 waves  32 rows, 8 waves  64 rows, 4 waves    quantizer and product of their own
+//   65536 x 3072          134.4             105.7             100.6            160.6
+//   16384 x 3072           35.2              31.1              34.2             47.7
+//   4352 x 3072            14.1              11.8              22.9             21.0
+//   4096 x 3072             9.9              11.7              22.8             20.4
+//   2050 x 1280             5.4               6.2              11.8             11.6
+int pq::mx::lowrank(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R, uint8_t* codes,
+                    uint8_t* scales, int8_t* q8, void* t, void* workspace, hipStream_t stream) {
+  const int slices = lowrank_slices(M, K);
+  float* const partial = slices > 1 ? static_cast<float*>(workspace) : nullptr;
+  auto launch = [&](auto rg, auto nw) {
+    constexpr int RG = decltype(rg)::value, NW = decltype(nw)::value;
+#define PQ_MXL(D, RR)                                                                                               \
+  launch_lowrank<D, RR, RG, NW>(static_cast<const uint16_t*>(x), M, K, ldx, static_cast<const uint16_t*>(l1f), codes, scales, q8, \
+                                static_cast<uint16_t*>(t), partial, slices, stream)
+    if (dtype == PQ_BF16) return R == 32 ? PQ_MXL(PQ_BF16, 32) : PQ_MXL(PQ_BF16, 64);
+    return R == 32 ? PQ_MXL(PQ_F16, 32) : PQ_MXL(PQ_F16, 64);
+#undef PQ_MXL
+  };
+  using std::integral_constant;
+  const int st = M <= 16 * 256  ? launch(integral_constant<int, 1>{}, integral_constant<int, 16>{})
+                 : M < 32768    ? launch(integral_constant<int, 2>{}, integral_constant<int, 8>{})
+                                : launch(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+  if (st || !partial) return st;
+  const int64_t n = M * R;
+  const dim3 grid((unsigned)((n / 4 + 255) / 256)), block(256);
+  if (dtype == PQ_BF16)
+    hipLaunchKernelGGL((mx_lowrank_join_kernel<PQ_BF16>), grid, block, 0, stream, partial, slices, n, static_cast<uint16_t*>(t));
+  else
+    hipLaunchKernelGGL((mx_lowrank_join_kernel<PQ_F16>), grid, block, 0, stream, partial, slices, n, static_cast<uint16_t*>(t));
+  return check_launch("mx_lowrank_join");
+}
 
 extern "C" int pq_mx_quant(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* codes, uint8_t* scales,
                            int8_t* q8, hipStream_t stream) {
@@ -187,15 +375,43 @@ extern "C" int pq_mx_values(const void* codes, const uint8_t* scales, int32_t bi
   return check_launch("mx_values");
 }
 
-extern "C" int pq_mx_factors(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, int64_t N, int64_t R,
-                             int64_t P, void* At, void* Ap, void* Bt, void* Bp, hipStream_t stream) {
-  if (K < 1 || N < 1 || R < 1 || R > P || (P != 32 && P != 64) || lda < R || ldb < N || K > (1 << 30) || N > (1 << 30))
+extern "C" int pq_mx_factors(const void* A, int64_t lda, int32_t a_order, const void* B, int64_t ldb, int32_t b_order, int64_t K,
+                             int64_t N, int64_t R, int64_t P, void* af, void* ap, void* bt, void* bf, hipStream_t stream) {
+  if (K < 1 || N < 1 || R < 1 || R > P || (P != 32 && P != 64) || K > (1 << 30) || N > (1 << 30))
     return set_error(PQ_ESHAPE, "pq_mx_factors: K=%lld N=%lld R=%lld P=%lld (R <= P, P 32 or 64)", (long long)K, (long long)N,
                      (long long)R, (long long)P);
   if (!A || !B) return set_error(PQ_EINVAL, "pq_mx_factors: null pointer");
-  const int blocks_a = (int)((K + 63) / 64), blocks_b = (int)((N + 63) / 64);
-  hipLaunchKernelGGL(mx_factors_kernel, dim3(blocks_a + blocks_b), dim3(256), 0, stream, static_cast<const uint16_t*>(A), lda,
-                     static_cast<const uint16_t*>(B), ldb, (int)K, (int)N, (int)R, (int)P, static_cast<uint16_t*>(At),
-                     static_cast<uint16_t*>(Ap), static_cast<uint16_t*>(Bt), static_cast<uint16_t*>(Bp), blocks_a);
+  for (const int32_t o : {a_order, b_order})
+    if (o != PQ_MX_BY_COLUMN && o != PQ_MX_BY_RANK && o != PQ_MX_FRAGMENTS) return set_error(PQ_EINVAL, "pq_mx_factors: order %d", o);
+  auto short_rows = [&](int32_t o, int64_t ld, int64_t C) { return (o == PQ_MX_BY_COLUMN && ld < R) || (o == PQ_MX_BY_RANK && ld < C); };
+  if (short_rows(a_order, lda, K) || short_rows(b_order, ldb, N))
+    return set_error(PQ_ESHAPE, "pq_mx_factors: lda=%lld ldb=%lld", (long long)lda, (long long)ldb);
+  for (const void* p : {(const void*)af, (const void*)ap, (const void*)bt, (const void*)bf})
+    if ((uintptr_t)p % 16) return set_error(PQ_EALIGN, "pq_mx_factors: results 16-byte aligned");
+  auto u16 = [](void* p) { return static_cast<uint16_t*>(p); };
+  const Factor fa{static_cast<const uint16_t*>(A), lda, a_order, (int)K, u16(ap), u16(af)};
+  const Factor fb{static_cast<const uint16_t*>(B), ldb, b_order, (int)N, u16(bt), u16(bf)};
+  const int blocks_a = 2 * stages(K), blocks_b = 2 * stages(N);   // (64 columns each; fragments are whole stages of 128)
+  hipLaunchKernelGGL(mx_factors_kernel, dim3(blocks_a + blocks_b), dim3(256), 0, stream, fa, fb, (int)R, (int)P, blocks_a);
   return check_launch("mx_factors");
+}
+
+extern "C" int64_t pq_mx_lowrank_workspace_size(int64_t M, int64_t K, int64_t R) {
+  return M < 1 || K < 16 || K > (1 << 30) || (R != 32 && R != 64) ? 0 : lowrank_workspace(M, K, R);
+}
+
+extern "C" int pq_mx_lowrank_down(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R,
+                                  void* t, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  if (M < 0 || K < 16 || K % 16 || ldx < K || K > (1 << 30) || (R != 32 && R != 64))
+    return set_error(PQ_ESHAPE, "pq_mx_lowrank_down: M=%lld K=%lld ldx=%lld R=%lld (K %% 16 == 0, R 32 or 64)", (long long)M,
+                     (long long)K, (long long)ldx, (long long)R);
+  if (dtype != PQ_BF16 && dtype != PQ_F16) return set_error(PQ_EDTYPE, "pq_mx_lowrank_down: dtype %d", dtype);
+  if (M == 0) return PQ_OK;
+  if (!x || !l1f || !t) return set_error(PQ_EINVAL, "pq_mx_lowrank_down: null pointer");
+  if ((uintptr_t)x % 16 || ldx % 8 || (uintptr_t)l1f % 16 || (uintptr_t)t % 16)
+    return set_error(PQ_EALIGN, "pq_mx_lowrank_down: operands 16-byte aligned, ldx a multiple of 8");
+  const int64_t need = lowrank_workspace(M, K, R);
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+    return set_error(PQ_EINVAL, "pq_mx_lowrank_down: a workspace of %lld bytes, 16-byte aligned", (long long)need);
+  return lowrank(x, dtype, M, K, ldx, l1f, R, nullptr, nullptr, nullptr, t, workspace, stream);
 }

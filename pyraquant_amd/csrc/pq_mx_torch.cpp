@@ -2,7 +2,8 @@
 //
 //   layer(x, codes, scales, lr_A, lr_B, bias, out_features, laid_out) -> y
 //
-// lr_A [K, R] and lr_B [R, N], or in the kernels' order [P, K] and [N, P] (laid_out); None without a low-rank branch. Three
+// lr_A [K, R] and lr_B [R, N], or in the kernels' order (laid_out: lr_A's fragments [ceil(K / 128) 128, P], lr_B's rows [N, P]);
+// None without a low-rank branch. Three
 // allocations a forward pass that a backward pass follows (y, what the backward pass keeps, and scratch), two otherwise; the
 // backward pass runs on autograd's thread without the interpreter. Work goes to the current stream of x's device.
 #include <Python.h>
@@ -49,15 +50,17 @@ Tensor rows_of(const Tensor& t) {
 }
 int64_t stride_of(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
 
+int64_t padded(int64_t C) { return (C + 127) / 128 * 128; }   // columns of a factor's fragments
+
 // What the backward pass keeps, slices of one allocation: offsets, in bytes.
 struct Kept {
-  int64_t q8 = 0, scales, t, ap, bp, total;   // bp: at first [P, N], ap [K, P]
+  int64_t q8 = 0, scales, t, ap, bp, total;   // ap: lr_A's rows [K, P], bp: lr_B's fragments
   Kept(int64_t M, int64_t K, int64_t N, int64_t P, bool x, bool down, bool factors) {
     scales = x ? up(M * K) : 0;
     t = scales + (x ? up(units(M, K) * 64) : 0);
     ap = t + (down ? up(2 * M * P) : 0);
     bp = ap + (factors ? up(2 * K * P) : 0);
-    total = bp + (factors ? up(2 * P * N) : 0);
+    total = bp + (factors ? up(2 * P * padded(N)) : 0);
   }
 };
 
@@ -75,31 +78,33 @@ Tensor forward(const Tensor& x0, const Tensor& codes, const Tensor& scales, cons
   const Tensor x = rows_of(x0);
   const c10::DeviceGuard guard(x.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream(x.device().index()).stream();
-  const int64_t M = x.size(0), K = x.size(1), R = !A.defined() ? 0 : laid_out ? A.size(0) : A.size(1), P = R == 0 ? 0 : R <= 32 ? 32 : 64;
+  const int64_t M = x.size(0), K = x.size(1), R = !A.defined() ? 0 : A.size(1), P = R == 0 ? 0 : R <= 32 ? 32 : 64;
   const Kept k(M, K, N, P, w.A, w.B || w.b, P && w.any());
   // scratch: the codes, and what is not kept of scales and t; the forward pass's order of the factors where they come in theirs
   const int64_t s_scales = up(units(M, K) * 1024), s_t = s_scales + (w.A ? 0 : up(units(M, K) * 64));
-  const int64_t s_at = s_t + (w.B || w.b ? 0 : up(2 * M * P)), s_bt = s_at + (P && !laid_out ? up(2 * P * K) : 0);
-  const Tensor scratch = bytes(s_bt + (P && !laid_out ? up(2 * N * P) : 0), x);
+  const int64_t s_at = s_t + (w.B || w.b ? 0 : up(2 * M * P)), s_bt = s_at + (P && !laid_out ? up(2 * P * padded(K)) : 0);
+  const int64_t s_ws = s_bt + (P && !laid_out ? up(2 * N * P) : 0), ws = P && M ? pq_mx_lowrank_workspace_size(M, K, P) : 0;
+  const Tensor scratch = bytes(s_ws + ws, x);
   if (w.any()) kept = bytes(k.total, x);
   const Tensor y = at::empty({M, N}, x.options().requires_grad(false));
   uint8_t *const s = data<uint8_t>(scratch), *const h = data<uint8_t>(kept);
   const void *at = nullptr, *bt = nullptr;
   if (P && laid_out) {
     at = A.const_data_ptr(), bt = B.const_data_ptr();
-    if (w.any())   // the backward pass's orders by the same rule, the factors' roles exchanged
-      check(pq_mx_factors(bt, P, at, K, N, K, P, P, h + k.bp, nullptr, h + k.ap, nullptr, stream), "mxfp4 factors");
+    if (w.any())   // the orders of the backward pass from those of the forward pass
+      check(pq_mx_factors(at, 0, PQ_MX_FRAGMENTS, bt, P, PQ_MX_BY_COLUMN, K, N, P, P, nullptr, h + k.ap, nullptr, h + k.bp, stream),
+            "mxfp4 factors");
   } else if (P) {
-    const Tensor a = A.stride(1) != 1 || A.stride(0) < R || A.is_neg() ? A.resolve_neg().contiguous() : A;
-    const Tensor b = B.stride(1) != 1 || B.stride(0) < N || B.is_neg() ? B.resolve_neg().contiguous() : B;
+    const Tensor a = (R > 1 && A.stride(1) != 1) || A.stride(0) < R || A.is_neg() ? A.resolve_neg().clone(at::MemoryFormat::Contiguous) : A;
+    const Tensor b = B.stride(1) != 1 || B.stride(0) < N || B.is_neg() ? B.resolve_neg().clone(at::MemoryFormat::Contiguous) : B;
     at = s + s_at, bt = s + s_bt;
-    check(pq_mx_factors(a.const_data_ptr(), std::max<int64_t>(a.stride(0), R), b.const_data_ptr(), std::max<int64_t>(b.stride(0), N), K,
-                        N, R, P, s + s_at, w.any() ? h + k.ap : nullptr, s + s_bt, w.any() ? h + k.bp : nullptr, stream),
+    check(pq_mx_factors(a.const_data_ptr(), a.stride(0), PQ_MX_BY_COLUMN, b.const_data_ptr(), b.stride(0), PQ_MX_BY_RANK, K, N, R, P,
+                        s + s_at, w.any() ? h + k.ap : nullptr, s + s_bt, w.any() ? h + k.bp : nullptr, stream),
           "mxfp4 factors");
   }
   check(pq_mx_linear(x.const_data_ptr(), code_of(x), M, K, stride_of(x), data<uint8_t>(codes), data<uint8_t>(scales),
                      data<float>(bias), at, bt, P, y.data_ptr(), N, N, s, w.A ? h + k.scales : s + s_scales,
-                     w.A ? reinterpret_cast<int8_t*>(h + k.q8) : nullptr, P ? (w.B || w.b ? h + k.t : s + s_t) : nullptr, stream),
+                     w.A ? reinterpret_cast<int8_t*>(h + k.q8) : nullptr, P ? (w.B || w.b ? h + k.t : s + s_t) : nullptr, ws ? s + s_ws : nullptr, ws, stream),
         "mxfp4 layer");
   return y;
 }
@@ -114,7 +119,7 @@ struct Layer : torch::autograd::Function<Layer> {
     Tensor kept;
     const Tensor y = ::forward(x, codes, scales, A, B, bias, N, laid_out, w, kept);
     ctx->save_for_backward({kept, codes, scales});
-    ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(0), x.size(1), N, A.defined() ? (laid_out ? A.size(0) : A.size(1)) : 0,
+    ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(0), x.size(1), N, A.defined() ? A.size(1) : 0,
                                                     (int64_t)w.x | (int64_t)w.A << 1 | (int64_t)w.B << 2 | (int64_t)w.b << 3};
     return y;
   }
@@ -152,10 +157,12 @@ struct Layer : torch::autograd::Function<Layer> {
       const int64_t s_dt = need_dt ? up(2 * M * P) : 0;
       const int64_t ws_sums = sums ? pq_mx_grad_factors_workspace_size(M, K, N, P) : 0;
       const int64_t ws_dx = w.x ? pq_mx_grad_input_workspace_size(M, N, K) : 0;
-      const Tensor scratch = bytes(s_dt + up(std::max(ws_sums, ws_dx)), dy);   // (one after the other on the stream)
+      const int64_t ws_dt = need_dt ? pq_mx_lowrank_workspace_size(M, N, P) : 0;
+      const Tensor scratch = bytes(s_dt + std::max({ws_sums, ws_dx, ws_dt}), dy);   // (one after the other on the stream)
       uint8_t* const s = data<uint8_t>(scratch);
       if (need_dt)
-        check(pq_lowrank_down(dy.const_data_ptr(), code, M, N, stride_of(dy), M, nullptr, h + k.bp, P, s, P, stream), "mxfp4 dt");
+        check(pq_mx_lowrank_down(dy.const_data_ptr(), code, M, N, stride_of(dy), h + k.bp, P, s, ws_dt ? s + s_dt : nullptr, ws_dt, stream),
+              "mxfp4 dt");
       if (sums)
         check(pq_mx_grad_factors(dy.const_data_ptr(), code, stride_of(dy), w.B || w.b ? h + k.t : nullptr, s,
                                  reinterpret_cast<int8_t*>(h + k.q8), h + k.scales, M, K, N, R, P, data<void>(out[1]),
@@ -202,8 +209,9 @@ const char* wrong(const Tensor& x, const Tensor& codes, const Tensor& scales, co
   if (A.defined()) {
     if (A.dim() != 2 || B.dim() != 2 || A.scalar_type() != x.scalar_type() || B.scalar_type() != x.scalar_type())
       return "lr_A and lr_B must be matrices of x's type";
-    const int64_t R = laid_out ? A.size(0) : A.size(1);
-    if (laid_out ? A.size(1) != K || B.size(0) != N || B.size(1) != R || !A.is_contiguous() || !B.is_contiguous() || (R != 32 && R != 64)
+    const int64_t R = A.size(1);
+    if (laid_out ? A.size(0) != padded(K) || B.size(0) != N || B.size(1) != R || !A.is_contiguous() || !B.is_contiguous() ||
+                       (R != 32 && R != 64) || (uintptr_t)A.const_data_ptr() % 16 || (uintptr_t)B.const_data_ptr() % 16
                  : A.size(0) != K || B.size(0) != R || B.size(1) != N || R < 1 || R > 64)
       return "lr_A and lr_B do not fit the layer";
   }

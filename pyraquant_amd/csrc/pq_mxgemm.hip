@@ -450,8 +450,9 @@ extern "C" int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8
 }
 
 extern "C" int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w,
-                            const uint8_t* w_scales, const float* bias, const void* l1t, const void* l2t, int64_t R, void* y,
-                            int64_t ldy, int64_t N, uint8_t* codes, uint8_t* scales, int8_t* q8, void* t, hipStream_t stream) {
+                            const uint8_t* w_scales, const float* bias, const void* l1f, const void* l2t, int64_t R, void* y,
+                            int64_t ldy, int64_t N, uint8_t* codes, uint8_t* scales, int8_t* q8, void* t, void* workspace,
+                            int64_t workspace_bytes, hipStream_t stream) {
   if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || ldx < K || ldy < N || ldy >= (1LL << 31) || M > (1 << 30) ||
       N > (1 << 30) || K > (1 << 22))
     return set_error(PQ_ESHAPE, "pq_mx_linear: M=%lld N=%lld K=%lld ldx=%lld ldy=%lld (N %% 16 == 0, K %% 32 == 0)", (long long)M,
@@ -459,18 +460,25 @@ extern "C" int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, 
   if (dtype != PQ_BF16 && dtype != PQ_F16) return set_error(PQ_EDTYPE, "pq_mx_linear: dtype %d", dtype);
   if (R != 0 && R != 32 && R != 64) return set_error(PQ_ESHAPE, "pq_mx_linear: rank %lld (0, 32 or 64)", (long long)R);
   if (M == 0) return PQ_OK;
-  if (!x || !w || !w_scales || !y || !codes || !scales || (R && (!l1t || !l2t || !t)))
+  if (!x || !w || !w_scales || !y || !codes || !scales || (R && (!l1f || !l2t || !t)))
     return set_error(PQ_EINVAL, "pq_mx_linear: null pointer");
   if ((uintptr_t)x % 16 || ldx % 8 || (uintptr_t)w % 16 || (uintptr_t)w_scales % 16 || (uintptr_t)y % 16 || ldy % 8 ||
       (uintptr_t)bias % 16 || (uintptr_t)codes % 16 || (uintptr_t)scales % 16 || (uintptr_t)q8 % 16 ||
-      (R && ((uintptr_t)l1t % 16 || (uintptr_t)l2t % 16 || (uintptr_t)t % 16)))
+      (R && ((uintptr_t)l1f % 16 || (uintptr_t)l2t % 16 || (uintptr_t)t % 16)))
     return set_error(PQ_EALIGN, "pq_mx_linear: operands 16-byte aligned, ldx and ldy multiples of 8");
   mx::GemmArgs p{codes, scales, w, w_scales, bias, static_cast<const uint16_t*>(R ? t : nullptr), static_cast<const uint16_t*>(l2t),
                  static_cast<uint16_t*>(y), R, ldy, (int)M, (int)N, mx::stages(K), 0, 0};
-  if (R)
-    if (const int st = pq_lowrank_down(x, dtype, M, K, ldx, M, nullptr, l1t, R, t, R, stream)) return st;
-  if (M <= mx::kQuantRows && !q8)
+  const int64_t need = R ? mx::lowrank_workspace(M, K, R) : 0;
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+    return set_error(PQ_EINVAL, "pq_mx_linear: a workspace of %lld bytes, 16-byte aligned", (long long)need);
+  const bool inside = M <= mx::kQuantRows && !q8;   // the product quantizes the rows itself
+  if (R) {
+    if (const int st = mx::lowrank(x, dtype, M, K, ldx, l1f, R, inside ? nullptr : codes, scales, q8, t, workspace, stream))
+      return st;
+  } else if (!inside) {
+    if (const int st = pq_mx_quant(x, dtype, M, K, ldx, codes, scales, q8, stream)) return st;
+  }
+  if (inside)
     return mx::launch_split<1, 1, 8, 2, true>({p, static_cast<const uint16_t*>(x), ldx, (int)K}, dtype, (int)R, stream);
-  if (const int st = pq_mx_quant(x, dtype, M, K, ldx, codes, scales, q8, stream)) return st;
   return mx::launch_gemm(p, dtype, (int)R, stream);
 }

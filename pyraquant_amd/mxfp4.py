@@ -27,7 +27,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .int8_exec import LOWRANK_A_ATTR, LOWRANK_B_ATTR, is_bf16_whitelisted, lowrank_down
+from .int8_exec import LOWRANK_A_ATTR, LOWRANK_B_ATTR, is_bf16_whitelisted
 
 BLOCK = 32        # values that share a scale
 MAX_RANK = 64     # of a low-rank branch (the kernels hold 32 or 64; lower ranks run zero-padded)
@@ -225,27 +225,21 @@ def _padded_rank(R: int) -> int:
     return 32 if R <= 32 else 64
 
 
-def lay_out_factors(lr_A: torch.Tensor, lr_B: torch.Tensor, down: bool = True, up: bool = True):
-    """lr_A [K, R] and lr_B [R, N] in the kernels' orders, zero-padded to rank P (32 or 64), from one launch: At [P, K] and
-    Bt [N, P] (``down``: what the forward pass reads), Ap [K, P] and Bp [P, N] (``up``: what the backward pass reads), None
-    where not asked for."""
+def lay_out_factors(lr_A: torch.Tensor, lr_B: torch.Tensor):
+    """lr_A [K, R] and lr_B [R, N] as the forward pass reads them, zero-padded to rank P (32 or 64): (lr_A's fragments
+    [ceil(K / 128) * 128, P], pq_mx_factors' order, lr_B's rows [N, P])."""
     _check_cuda(lr_A, lr_B)
     assert lr_A.dim() == 2 and lr_B.dim() == 2 and lr_A.shape[1] == lr_B.shape[0], (tuple(lr_A.shape), tuple(lr_B.shape))
     assert lr_A.dtype == lr_B.dtype, (lr_A.dtype, lr_B.dtype)
     _dtype16(lr_A.dtype)
-    A, B = _plain(lr_A), _plain(lr_B)
-    if A.stride(1) != 1 or A.stride(0) < A.shape[1]:
-        A = A.contiguous()
-    if B.stride(1) != 1 or B.stride(0) < B.shape[1]:
-        B = B.contiguous()
+    A, B = _plain(lr_A).contiguous(), _plain(lr_B).contiguous()
     (K, R), N = A.shape, B.shape[1]
     P = _padded_rank(R)
-    new = lambda on, *shape: torch.empty(shape, dtype=A.dtype, device=A.device) if on else None   # noqa: E731
-    At, Ap, Bt, Bp = new(down, P, K), new(up, K, P), new(down, N, P), new(up, P, N)
-    _lib.check(_lib.load().pq_mx_factors(_lib.ptr(A), max(A.stride(0), R), _lib.ptr(B), max(B.stride(0), N), K, N, R, P,
-                                         _lib.ptr(At), _lib.ptr(Ap), _lib.ptr(Bt), _lib.ptr(Bp), _lib.stream_of(A.device)),
-               "lay_out_factors")
-    return At, Ap, Bt, Bp
+    Af = torch.empty(((K + 127) // 128 * 128, P), dtype=A.dtype, device=A.device)
+    Bt = torch.empty((N, P), dtype=A.dtype, device=A.device)
+    _lib.check(_lib.load().pq_mx_factors(_lib.ptr(A), R, _lib.PQ_MX_BY_COLUMN, _lib.ptr(B), N, _lib.PQ_MX_BY_RANK, K, N, R, P,
+                                         _lib.ptr(Af), None, _lib.ptr(Bt), None, _lib.stream_of(A.device)), "lay_out_factors")
+    return Af, Bt
 
 
 # --------------------------------------------------------------------------- the layer
@@ -264,7 +258,7 @@ class Mxfp4Linear(nn.Module):
     low-rank factors are used in the input's type.
 
     Buffers ``weight_codes`` and ``weight_scales`` hold the weight. ``trainable=False`` keeps the low-rank branch in the
-    kernels' order (``lr_At`` [P, K], ``lr_Bt`` [N, P], zero-padded to P = 32 or 64; ``lr_A`` and ``lr_B`` give it back) and
+    kernels' order (``lr_Af``, ``lr_Bt``: lay_out_factors; ``lr_A`` and ``lr_B`` give it back) and
     the bias in fp32 as buffers. ``trainable=True`` (needs a low-rank branch) makes ``lr_A`` [K, R], ``lr_B`` [R, N] and
     ``bias`` parameters; freeze() turns such a layer into the other kind. Gradients flow to the input of either."""
 
@@ -298,12 +292,12 @@ class Mxfp4Linear(nn.Module):
 
     def _keep(self, A, B, bias) -> None:
         """The low-rank branch and the bias as buffers, the branch in the kernels' order."""
-        At = Bt = None
+        Af = Bt = None
         if A is not None:
             if A.dtype not in (torch.bfloat16, torch.float16):
                 A, B = A.to(torch.bfloat16), B.to(torch.bfloat16)
-            At, _, Bt, _ = lay_out_factors(A, B.to(A.dtype), True, False)
-        self.register_buffer("lr_At", At)
+            Af, Bt = lay_out_factors(A, B.to(A.dtype))
+        self.register_buffer("lr_Af", Af)
         self.register_buffer("lr_Bt", Bt)
         self.register_buffer("bias", bias)
 
@@ -317,10 +311,13 @@ class Mxfp4Linear(nn.Module):
         return self
 
     def __getattr__(self, name):
-        if name in ("lr_A", "lr_B") and "lr_At" in self.__dict__.get("_buffers", ()):
-            if self.lr_At is None:
+        if name in ("lr_A", "lr_B") and "lr_Af" in self.__dict__.get("_buffers", ()):
+            if self.lr_Af is None:
                 return None
-            return (self.lr_At[: self.rank].t() if name == "lr_A" else self.lr_Bt[:, : self.rank].t()).contiguous()
+            if name == "lr_B":
+                return self.lr_Bt[:, : self.rank].t().contiguous()
+            f = self.lr_Af.reshape(-1, 4, self.lr_Af.shape[1] // 16, 4, 16, 8)    # stage, group, rank / 16, block, rank % 16, k
+            return f.permute(0, 3, 1, 5, 2, 4).reshape(self.lr_Af.shape)[: self.in_features, : self.rank].contiguous()
         return super().__getattr__(name)
 
     def _apply(self, fn, recurse=True):
@@ -343,7 +340,7 @@ class Mxfp4Linear(nn.Module):
             p = self._parameters
             A, B, bias = p["lr_A"], p["lr_B"], p["bias"]
         else:
-            A, B, bias = d["lr_At"], d["lr_Bt"], d["bias"]
+            A, B, bias = d["lr_Af"], d["lr_Bt"], d["bias"]
         dt = x.dtype
         if A is not None and (A.dtype != dt or B.dtype != dt) and dt in (torch.bfloat16, torch.float16):
             A, B = A.to(dt), B.to(dt)

@@ -64,8 +64,26 @@ def test_gemm_and_gradient_refusals():
     assert lib.pq_mx_grad_factors_workspace_size(0, 64, 64, 32) == 0
     small, large = (lib.pq_mx_grad_factors_workspace_size(m, 64, 64, 32) for m in (1, 100000))
     assert 0 < small < large
-    lay = lambda A=P, K=64, N=64, R=8, PP=32, lda=8: lib.pq_mx_factors(A, lda, P, N, K, N, R, PP, P, P, P, P, None)   # noqa: E731
+
+    def lay(A=P, K=64, N=64, R=8, PP=32, lda=8, ldb=64, ao=0, bo=1, out=P):
+        return lib.pq_mx_factors(A, lda, ao, P, ldb, bo, K, N, R, PP, out, P, P, P, None)
+
     assert lay(R=40) == L.PQ_ESHAPE and lay(PP=48) == L.PQ_ESHAPE and lay(lda=4) == L.PQ_ESHAPE and lay(A=None) == L.PQ_EINVAL
+    assert lay(ldb=32) == L.PQ_ESHAPE and lay(ao=3) == L.PQ_EINVAL and lay(out=ODD) == L.PQ_EALIGN
+    down = lambda x=P, K=64, ldx=64, R=32, dt=0, t=P: lib.pq_mx_lowrank_down(x, dt, 4, K, ldx, P, R, t, None, 0, None)   # noqa: E731
+    assert down(K=24, ldx=24) == L.PQ_ESHAPE and down(R=16) == L.PQ_ESHAPE and down(ldx=32) == L.PQ_ESHAPE
+    assert down(dt=3) == L.PQ_EDTYPE and down(x=None) == L.PQ_EINVAL and down(ldx=68) == L.PQ_EALIGN and down(t=ODD) == L.PQ_EALIGN
+
+    def layer(x=P, ldx=64, R=0, l1=None, l2=None, t=None, y=P, codes=P, dt=0, M=4, K=64, N=64):
+        return lib.pq_mx_linear(x, dt, M, K, ldx, P, P, None, l1, l2, R, y, N, N, codes, P, None, t, None, 0, None)
+
+    assert layer(K=48) == L.PQ_ESHAPE and layer(N=24) == L.PQ_ESHAPE and layer(R=16) == L.PQ_ESHAPE and layer(ldx=32) == L.PQ_ESHAPE
+    assert layer(dt=3) == L.PQ_EDTYPE and layer(x=None) == L.PQ_EINVAL and layer(codes=None) == L.PQ_EINVAL
+    assert layer(R=32, l1=P, l2=P) == L.PQ_EINVAL and layer(y=ODD) == L.PQ_EALIGN and layer(ldx=68) == L.PQ_EALIGN
+    assert lib.pq_mx_lowrank_workspace_size(512, 12288, 32) > 0 and lib.pq_mx_lowrank_workspace_size(4096, 12288, 32) == 0
+    assert layer(M=512, K=12288, ldx=12288, R=32, l1=P, l2=P, t=P) == L.PQ_EINVAL and b"workspace" in lib.pq_last_error()
+    assert down(K=12288, ldx=12288) == L.PQ_EINVAL and b"workspace" in lib.pq_last_error()
+    assert layer(M=0, x=None, y=None, codes=None) == L.PQ_OK
 
 
 def test_python_layer_refuses_cpu_tensors():

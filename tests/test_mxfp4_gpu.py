@@ -165,7 +165,8 @@ def test_rows_with_strides_offsets_and_signs(cuda):
 
 # ---- the layer ------------------------------------------------------------------------------------------------------
 
-SIZES = [(1, 32, 16, 0), (1, 1280, 1280, 0), (2, 96, 48, 16), (5, 160, 16, 64), (16, 128, 112, 0), (17, 608, 80, 5), (31, 2080, 144, 32),
+# (48, 4224, ..: rows shared by several workgroups; 4128 and 33000 rows: 32 and 64 rows a workgroup of the quantizer with t)
+SIZES = [(48, 4224, 32, 32), (1, 32, 16, 0), (1, 1280, 1280, 0), (2, 96, 48, 16), (5, 160, 16, 64), (16, 128, 112, 0), (17, 608, 80, 5), (31, 2080, 144, 32),
          (64, 256, 64, 0), (65, 1024, 272, 40), (129, 384, 400, 32), (257, 544, 528, 0), (300, 1312, 256, 64)]
 
 
@@ -201,6 +202,18 @@ def test_layer_gradients(cuda, dtype, M, K, N, R):
     r, bound = _bounds(x, w, A, B, bias, dy, dtype)
     for k, g in got.items():
         assert g.dtype == (torch.float32 if k == "dbias" else dtype) and tuple(g.shape) == tuple(r[k].shape), k
+        _inside(g, r[k], bound[k], k)
+
+
+@pytest.mark.parametrize("M", (4128, 33000))
+def test_many_rows_through_the_low_rank_branch(cuda, M):
+    """The quantizer that also takes x lr_A, with more rows a workgroup: codes and checkpoint through y and dA."""
+    K, N, R = 96, 32, 40
+    layer, w, (A, B), bias = _layer(K, N, R, True, torch.bfloat16, 5, trainable=True)
+    x, dy = _x(M, K, torch.bfloat16, 6), torch.randn(M, N, generator=_gen(7)).to(torch.bfloat16)
+    got = _grads(layer, x, dy)
+    r, bound = _bounds(x, w, A, B, bias, dy, torch.bfloat16)
+    for k, g in got.items():
         _inside(g, r[k], bound[k], k)
 
 
@@ -396,7 +409,7 @@ def test_parameters_in_fp32_and_module_casts(cuda):
     assert got["dA"].dtype == torch.float32 and all(torch.equal(got[k].to(every[k].dtype), every[k]) for k in every)
     served, *_ = _layer(128, 64, 16, True, torch.bfloat16, 2)
     served = served.to(torch.float16)
-    assert served.bias.dtype == torch.float32 and served.lr_At.dtype == torch.float16 and served.weight_codes.dtype == torch.uint8
+    assert served.bias.dtype == torch.float32 and served.lr_Af.dtype == torch.float16 and served.weight_codes.dtype == torch.uint8
     assert isinstance(served, Mxfp4Linear) and served(x.cuda().to(torch.float16)).dtype == torch.float16
 
 
