@@ -146,14 +146,14 @@ def load_direct():
 
 
 def load_mx():
-    """The Mxfp4Linear call of _mx.so (csrc/pq_mx_torch.cpp): layer(x, codes, scales, lr_A, lr_B, bias, N, laid_out)."""
+    """_mx.so (csrc/pq_mx_torch.cpp): the calls of mxfp4 that run without Python, layer, quant and values."""
     load()
     try:
         from . import _mx
     except ImportError as e:
         raise LibraryMissing(f"pyraquant_amd/_mx.so is not built or does not load ({e}); run "
                              "`python -m pyraquant_amd.build`") from e
-    return _mx.layer
+    return _mx
 
 
 def check(status: int, what: str) -> None:

@@ -1,6 +1,8 @@
 // The Mxfp4Linear call and its backward pass without Python between the module and the kernels: pyraquant_amd._mx.
 //
 //   layer(x, codes, scales, lr_A, lr_B, bias, out_features, laid_out) -> y
+//   quant(x, checkpoint) -> (codes, scales, q8 or None)
+//   values(codes, scales, bits, rows, cols, dtype) -> [rows, cols]
 //
 // lr_A [K, R] and lr_B [R, N], or in the kernels' order (laid_out: lr_A's fragments [ceil(K / 128) 128, P], lr_B's rows [N, P]);
 // None without a low-rank branch. Three
@@ -13,6 +15,7 @@
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -274,9 +277,98 @@ PyObject* layer(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* raise(int status, const char* what) {
+  PyErr_Format(status == PQ_EDTYPE ? PyExc_ValueError : status == PQ_ELAUNCH ? PyExc_RuntimeError : PyExc_AssertionError, "%s: %s", what,
+               pq_last_error());
+  return nullptr;
+}
+// PQ_BF16, PQ_F16 or PQ_F32; -1 with a Python error set.
+int32_t float_code(at::ScalarType t) {
+  if (t == at::kBFloat16) return PQ_BF16;
+  if (t == at::kHalf) return PQ_F16;
+  if (t == at::kFloat) return PQ_F32;
+  PyErr_SetString(PyExc_ValueError, "unsupported dtype (expected bfloat16, float16 or float32)");
+  return -1;
+}
+
+PyObject* quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor x;
+  if (nargs != 2 || !tensor_arg(args[0], false, "x", x)) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "quant(x, checkpoint)");
+    return nullptr;
+  }
+  const int checkpoint = PyObject_IsTrue(args[1]);
+  if (checkpoint < 0) return nullptr;
+  if (!x.is_cuda() || x.dim() != 2 || x.size(1) < 32 || x.size(1) % 32) {
+    PyErr_SetString(PyExc_AssertionError, !x.is_cuda() ? "the 4-bit layers run on the GPU only (got a CPU tensor)"
+                                                       : "x must be a matrix whose rows are a multiple of 32 values");
+    return nullptr;
+  }
+  const int32_t code = float_code(x.scalar_type());
+  if (code < 0) return nullptr;
+  Tensor codes, scales, q8;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    const int64_t M = x.size(0), K = x.size(1);
+    Tensor r = (x.is_neg() ? x.resolve_neg() : x).detach();
+    if (r.stride(1) != 1 || (M > 1 && r.stride(0) < K)) r = r.clone(at::MemoryFormat::Contiguous);
+    const c10::DeviceGuard guard(x.device());
+    codes = bytes(units(M, K) * 1024, r);
+    scales = bytes(units(M, K) * 64, r);
+    if (checkpoint) q8 = at::empty({M, K}, codes.options().dtype(at::kChar));
+    st = pq_mx_quant(r.const_data_ptr(), code, M, K, stride_of(r), data<uint8_t>(codes), data<uint8_t>(scales), data<int8_t>(q8),
+                     c10::hip::getCurrentHIPStream(x.device().index()).stream());
+  }
+  if (st != PQ_OK) return raise(st, "quant_mxfp4");
+  PyObject* const none = Py_None;
+  if (!checkpoint) Py_INCREF(none);
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(codes), THPVariable_Wrap(scales), checkpoint ? THPVariable_Wrap(q8) : none);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* values(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor codes, scales;
+  if (nargs != 6 || !tensor_arg(args[0], false, "codes", codes) || !tensor_arg(args[1], false, "scales", scales) ||
+      !THPDtype_Check(args[5])) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "values(codes, scales, bits, rows, cols, dtype)");
+    return nullptr;
+  }
+  const int64_t bits = PyLong_AsLongLong(args[2]), M = PyLong_AsLongLong(args[3]), K = PyLong_AsLongLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(args[5])->scalar_type;
+  const int32_t code = float_code(type);
+  if (code < 0) return nullptr;
+  const bool eight = bits == 8;
+  if (!codes.is_cuda() || !scales.is_cuda() || codes.device() != scales.device() || M < 0 || K < 32 || K % 32 || (bits != 4 && !eight) ||
+      codes.scalar_type() != (eight ? at::kChar : at::kByte) || scales.scalar_type() != at::kByte || !codes.is_contiguous() ||
+      !scales.is_contiguous() || codes.numel() < (eight ? M * K : units(M, K) * 1024) || scales.numel() < units(M, K) * 64) {
+    PyErr_SetString(PyExc_AssertionError, "codes and scales are not those of a matrix of this size on the GPU");
+    return nullptr;
+  }
+  Tensor out;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    const c10::DeviceGuard guard(codes.device());
+    out = at::empty({M, K}, codes.options().dtype(type));
+    st = pq_mx_values(codes.const_data_ptr(), data<uint8_t>(scales), (int32_t)bits, M, K, out.data_ptr(), code, K,
+                      c10::hip::getCurrentHIPStream(codes.device().index()).stream());
+  }
+  if (st != PQ_OK) return raise(st, "mxfp4 values");
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+template <typename F>
+PyCFunction fast(F* f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)); }
 PyMethodDef kMethods[] = {
-    {"layer", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(layer)), METH_FASTCALL,
+    {"layer", fast(layer), METH_FASTCALL,
      "layer(x, codes, scales, lr_A, lr_B, bias, out_features, laid_out): the Mxfp4Linear call, differentiable"},
+    {"quant", fast(quant), METH_FASTCALL, "quant(x, checkpoint): (codes, scales, q8 or None), pq_mx_quant"},
+    {"values", fast(values), METH_FASTCALL, "values(codes, scales, bits, rows, cols, dtype): [rows, cols], pq_mx_values"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_mx", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

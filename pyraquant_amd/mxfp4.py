@@ -31,7 +31,6 @@ from .int8_exec import LOWRANK_A_ATTR, LOWRANK_B_ATTR, is_bf16_whitelisted
 
 BLOCK = 32        # values that share a scale
 MAX_RANK = 64     # of a low-rank branch (the kernels hold 32 or 64; lower ranks run zero-padded)
-_DTYPES = {torch.bfloat16: _lib.PQ_BF16, torch.float16: _lib.PQ_F16, torch.float32: _lib.PQ_F32}
 
 
 class Mxfp4Matrix(NamedTuple):
@@ -41,6 +40,15 @@ class Mxfp4Matrix(NamedTuple):
     scales: torch.Tensor
     rows: int
     cols: int
+
+
+_mx = None   # _mx.so, loaded at the first use
+
+
+def _load_mx():
+    global _mx
+    _mx = _lib.load_mx()
+    return _mx
 
 
 def _stages(rows: int, cols: int) -> int:
@@ -90,46 +98,20 @@ def _stride(x2: torch.Tensor) -> int:
 def quant_mxfp4(x2: torch.Tensor, checkpoint: bool = False):
     """x2 [M, K] (bf16, fp16 or fp32, K % 32 == 0) -> Mxfp4Matrix; with ``checkpoint`` (Mxfp4Matrix, q8): q8 [M, K] int8,
     the codes a backward pass keeps, on the same scales. Row-slice views pass without a copy."""
-    assert x2.dim() == 2, x2.shape
-    _check_cuda(x2)
-    if x2.dtype not in _DTYPES:
-        raise ValueError(f"unsupported dtype {x2.dtype} (expected bfloat16, float16 or float32)")
-    M, K = x2.shape
-    assert K > 0 and K % BLOCK == 0, f"K = {K} is not a multiple of {BLOCK}"
-    x2 = _plain(x2)
-    if M > 1 and (x2.stride(1) != 1 or x2.stride(0) < K) or x2.stride(1) != 1:
-        x2 = x2.contiguous()
-    units = _stages(M, K)
-    codes = torch.empty(units * 1024, dtype=torch.uint8, device=x2.device)
-    scales = torch.empty(units * 64, dtype=torch.uint8, device=x2.device)
-    q8 = torch.empty((M, K), dtype=torch.int8, device=x2.device) if checkpoint else None
-    _lib.check(_lib.load().pq_mx_quant(_lib.ptr(x2), _DTYPES[x2.dtype], M, K, _stride(x2), _lib.ptr(codes), _lib.ptr(scales),
-                                       _lib.ptr(q8), _lib.stream_of(x2.device)), "quant_mxfp4")
-    q = Mxfp4Matrix(codes, scales, M, K)
+    codes, scales, q8 = (_mx or _load_mx()).quant(x2, checkpoint)
+    q = Mxfp4Matrix(codes, scales, *x2.shape)
     return (q, q8) if checkpoint else q
-
-
-def _values(codes, scales, bits, M, K, dtype):
-    _check_cuda(codes, scales)
-    if dtype not in _DTYPES:
-        raise ValueError(f"unsupported dtype {dtype} (expected bfloat16, float16 or float32)")
-    out = torch.empty((M, K), dtype=dtype, device=codes.device)
-    _lib.check(_lib.load().pq_mx_values(_lib.ptr(codes), _lib.ptr(scales), bits, M, K, _lib.ptr(out), _DTYPES[dtype], K,
-                                        _lib.stream_of(codes.device)), "mxfp4 values")
-    return out
 
 
 def dequant_mxfp4(q: Mxfp4Matrix, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values a 4-bit matrix holds, [rows, cols] (exact in bf16 and fp32; in fp16 for scales of 2^-22 to 2^13)."""
-    _check_matrix(q)
-    return _values(q.codes, q.scales, 4, q.rows, q.cols, dtype)
+    return (_mx or _load_mx()).values(q.codes, q.scales, 4, q.rows, q.cols, dtype)
 
 
 def checkpoint_values(q8: torch.Tensor, q: Mxfp4Matrix, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of a checkpoint's 8-bit codes on the scales of the matrix quantized with them."""
-    _check_matrix(q)
-    assert q8.dtype == torch.int8 and q8.is_contiguous() and tuple(q8.shape) == (q.rows, q.cols), (q8.dtype, tuple(q8.shape))
-    return _values(q8, q.scales, 8, q.rows, q.cols, dtype)
+    assert q8.dim() == 2 and tuple(q8.shape) == (q.rows, q.cols), (tuple(q8.shape), q.rows, q.cols)
+    return (_mx or _load_mx()).values(q8, q.scales, 8, q.rows, q.cols, dtype)
 
 
 # --------------------------------------------------------------------------- product and gradients
@@ -243,15 +225,6 @@ def lay_out_factors(lr_A: torch.Tensor, lr_B: torch.Tensor):
 
 
 # --------------------------------------------------------------------------- the layer
-_layer = None   # _mx.so's layer call, loaded at the first use
-
-
-def _load_layer():
-    global _layer
-    _layer = _lib.load_mx()
-    return _layer
-
-
 class Mxfp4Linear(nn.Module):
     """4-bit stand-in for nn.Linear: y = x4 @ w4^T (+ (x @ lr_A) @ lr_B) (+ bias), x4 and w4 the microscaled 4-bit values of x
     and the weight; in_features % 32 == 0, out_features % 16 == 0, low rank up to 64. Inputs are bf16 or fp16, and the
@@ -346,7 +319,7 @@ class Mxfp4Linear(nn.Module):
             A, B = A.to(dt), B.to(dt)
         if bias is not None and bias.dtype != torch.float32:
             bias = bias.float()
-        return (_layer or _load_layer())(x, d["weight_codes"], d["weight_scales"], A, B, bias, self.out_features, not trainable)
+        return (_mx or _load_mx()).layer(x, d["weight_codes"], d["weight_scales"], A, B, bias, self.out_features, not trainable)
 
     def extra_repr(self) -> str:
         lr = f", low-rank r={self.rank}" + (" (trainable)" if self.trainable else "") if self.rank else ""
