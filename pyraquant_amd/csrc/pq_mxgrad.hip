@@ -389,7 +389,8 @@ void mx_dx_ring_kernel(const DxArgs p) {
 
 // ---- sums over rows: part[s][r][c] = sum over the rows of slice s of v[m, r] z[m, c] -------------------------------------
 // z is dy (EIGHT false) or the 8-bit codes of x with their scales; v is t or dt, [M, R]. Column sums of z too (COLS). A
-// workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step; the order of the sums is fixed.
+// workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step; the order of the sums is fixed. Bound by
+// reading z (dy of 16384 x 12288: 88 us, 4.6 TB/s).
 struct SumArgs {
   const void* z;
   const uint8_t* scales;
@@ -397,14 +398,14 @@ struct SumArgs {
   float *part, *part_cols;
   int64_t ldz;
   int M, C, KT, rows;   // rows a slice, a multiple of 64
+  int panels, blocks;   // of 128 columns; workgroups (0: this sum is not wanted)
 };
 
 template <int DT, int R, bool EIGHT, bool COLS>
-__global__ __launch_bounds__(256) void mx_rowsum_kernel(const SumArgs p) {
-  __shared__ __attribute__((aligned(16))) uint8_t sz[64 * 256];      // [m][128 c]
-  __shared__ __attribute__((aligned(16))) uint8_t sv[64 * R * 2];    // [m][R]
+__device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* sz, uint8_t* sv) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int c0 = blockIdx.x * 128, s0 = blockIdx.y * p.rows;
+  const int slice = block / p.panels, panel = block - slice * p.panels;
+  const int c0 = panel * 128, s0 = slice * p.rows;
   const int end = min(p.M, s0 + p.rows);
   auto z_at = [&](int row, int chunk) { return sz + row * 256 + ((chunk ^ spread(row)) << 4); };
   auto v_at = [&](int row, int chunk) { return sv + row * R * 2 + (chunk << 4); };
@@ -422,7 +423,7 @@ __global__ __launch_bounds__(256) void mx_rowsum_kernel(const SumArgs p) {
         const v4u* const src = reinterpret_cast<const v4u*>(static_cast<const int8_t*>(p.z) + (int64_t)m * p.ldz + c);
         q[0] = src[0];
         q[1] = src[1];
-        byte = p.scales[scale_offset(m, blockIdx.x, b, p.KT)];
+        byte = p.scales[scale_offset(m, panel, b, p.KT)];
       }
       const float s = in ? restore_scale(byte) : 0.0f;
 #pragma unroll
@@ -462,15 +463,25 @@ __global__ __launch_bounds__(256) void mx_rowsum_kernel(const SumArgs p) {
     if (c + 8 * q >= p.C) break;
 #pragma unroll
     for (int j = 0; j < R / 32; ++j)
-      *reinterpret_cast<v4f*>(p.part + ((int64_t)blockIdx.y * R + 32 * j + (lane & 31)) * p.C + c + 8 * q) =
+      *reinterpret_cast<v4f*>(p.part + ((int64_t)slice * R + 32 * j + (lane & 31)) * p.C + c + 8 * q) =
           v4f{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
     if (COLS && (lane & 31) == 0)
-      *reinterpret_cast<v4f*>(p.part_cols + (int64_t)blockIdx.y * p.C + c + 8 * q) =
+      *reinterpret_cast<v4f*>(p.part_cols + (int64_t)slice * p.C + c + 8 * q) =
           v4f{cols[4 * q], cols[4 * q + 1], cols[4 * q + 2], cols[4 * q + 3]};
   }
 }
 
-// The slices' sums added in order: out[r, c] (TRANS: out[c, r]) rounded to 16 bits, and the column sums in 32. A thread sums one element, eight slices' loads in flight.
+// Both sums in one launch: dB and the column sums of dy (b), then dA (a).
+template <int DT, int R, bool COLS>
+__global__ __launch_bounds__(256) void mx_rowsum_kernel(const SumArgs b, const SumArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t sz[64 * 256];      // [m][128 c]
+  __shared__ __attribute__((aligned(16))) uint8_t sv[64 * R * 2];    // [m][R]
+  if ((int)blockIdx.x < b.blocks) row_sums<DT, R, false, COLS>(b, blockIdx.x, sz, sv);
+  else row_sums<DT, R, true, false>(a, blockIdx.x - b.blocks, sz, sv);
+}
+
+// The slices' sums added in order, rounded to 16 bits: dB [R, N] and dA [K, R]; and the column sums in 32. A thread sums one
+// element, eight slices' loads in flight.
 __device__ __forceinline__ float sum_slices(const float* at, int slices, int64_t step) {
   float s = 0.0f;
   int i = 0;
@@ -484,16 +495,23 @@ __device__ __forceinline__ float sum_slices(const float* at, int slices, int64_t
   for (; i < slices; ++i) s += at[i * step];
   return s;
 }
-template <int DT, bool TRANS>
-__global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ part, const float* __restrict__ part_cols,
-                                                      int slices, int P, int R, int C, uint16_t* __restrict__ out,
-                                                      float* __restrict__ cols) {
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), r = blockIdx.y * 4 + (threadIdx.x >> 6);
-  if (c >= C) return;
-  if (out && r < R)
-    out[TRANS ? (int64_t)c * R + r : (int64_t)r * C + c] =
-        (uint16_t)f32_to_16_bits<DT>(sum_slices(part + (int64_t)r * C + c, slices, (int64_t)P * C));
-  if (cols && r == 0) cols[c] = sum_slices(part_cols + c, slices, C);
+struct JoinArgs {
+  const float *part, *part_cols;
+  uint16_t* out;
+  float* cols;
+  int slices, C, groups, blocks;   // groups of 64 columns; workgroups (0: not wanted)
+};
+template <int DT>
+__global__ __launch_bounds__(256) void mx_join_kernel(const JoinArgs b, const JoinArgs a, int P, int R) {
+  const bool is_b = (int)blockIdx.x < b.blocks;
+  const JoinArgs p = is_b ? b : a;
+  const int block = (int)blockIdx.x - (is_b ? 0 : b.blocks);
+  const int c = block % p.groups * 64 + (threadIdx.x & 63), r = block / p.groups * 4 + (threadIdx.x >> 6);
+  if (c >= p.C) return;
+  if (p.out && r < R)
+    p.out[is_b ? (int64_t)r * p.C + c : (int64_t)c * R + r] =
+        (uint16_t)f32_to_16_bits<DT>(sum_slices(p.part + (int64_t)r * p.C + c, p.slices, (int64_t)P * p.C));
+  if (p.cols && r == 0) p.cols[c] = sum_slices(p.part_cols + c, p.slices, p.C);
 }
 
 // How dx is computed: 256 x 256 blocks where they fill more than half the chip's 256 compute units; else 64 x 128 blocks, with
@@ -607,8 +625,7 @@ extern "C" int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, con
 
 extern "C" int64_t pq_mx_grad_factors_workspace_size(int64_t M, int64_t K, int64_t N, int64_t P) {
   if (M < 1 || K < 32 || N < 16 || (P != 32 && P != 64)) return 0;
-  const int64_t b = (int64_t)mx::row_slices(M, N) * (P + 1) * N, a = (int64_t)mx::row_slices(M, K) * P * K;
-  return 4 * std::max(a, b);
+  return 4 * ((int64_t)mx::row_slices(M, N) * (P + 1) * N + (int64_t)mx::row_slices(M, K) * P * K);
 }
 
 extern "C" int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, const void* t, const void* dt, const int8_t* q8,
@@ -628,22 +645,23 @@ extern "C" int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, c
   float* const part = static_cast<float*>(workspace);
   const int sb = mx::row_slices(M, N), sk = mx::row_slices(M, K);
   auto rows = [&](int slices) { return (int)(((M + 63) / 64 + slices - 1) / slices * 64); };
-  mx::SumArgs b{dy, nullptr, static_cast<const uint16_t*>(t), part, part + (int64_t)sb * P * N, lddy, (int)M, (int)N, 0, rows(sb)};
-  mx::SumArgs a{q8, x_scales, static_cast<const uint16_t*>(dt), part, nullptr, K, (int)M, (int)K, mx::stages(K), rows(sk)};
-  const dim3 gb((unsigned)((N + 127) / 128), (unsigned)sb), ga((unsigned)((K + 127) / 128), (unsigned)sk), block(256);
-  const dim3 jb((unsigned)((N + 63) / 64), (unsigned)((R + 3) / 4)), ja((unsigned)((K + 63) / 64), (unsigned)((R + 3) / 4));
-#define PQ_MXS(D, PP)                                                                                                     \
-  do {                                                                                                                   \
-    if (dbias) hipLaunchKernelGGL((mx::mx_rowsum_kernel<D, PP, false, true>), gb, block, 0, stream, b);                  \
-    else if (dB) hipLaunchKernelGGL((mx::mx_rowsum_kernel<D, PP, false, false>), gb, block, 0, stream, b);               \
-    if (dB || dbias)                                                                                                     \
-      hipLaunchKernelGGL((mx::mx_join_kernel<D, false>), jb, block, 0, stream, part, b.part_cols, sb, (int)P, (int)R,    \
-                         (int)N, static_cast<uint16_t*>(dB), dbias);                                                     \
-    if (dA) {                                                                                                            \
-      hipLaunchKernelGGL((mx::mx_rowsum_kernel<D, PP, true, false>), ga, block, 0, stream, a);                           \
-      hipLaunchKernelGGL((mx::mx_join_kernel<D, true>), ja, block, 0, stream, part, nullptr, sk, (int)P, (int)R, (int)K, \
-                         static_cast<uint16_t*>(dA), nullptr);                                                           \
-    }                                                                                                                    \
+  float* const part_a = part + (int64_t)sb * (P + 1) * N;
+  const int pb = (int)((N + 127) / 128), pk = (int)((K + 127) / 128);
+  const bool want_b = dB || dbias, want_a = dA != nullptr;
+  const mx::SumArgs b{dy, nullptr, static_cast<const uint16_t*>(t), part, part + (int64_t)sb * P * N, lddy, (int)M, (int)N, 0,
+                      rows(sb), pb, want_b ? pb * sb : 0};
+  const mx::SumArgs a{q8, x_scales, static_cast<const uint16_t*>(dt), part_a, nullptr, K, (int)M, (int)K, mx::stages(K), rows(sk),
+                      pk, want_a ? pk * sk : 0};
+  const int quads = (int)((R + 3) / 4), gb = (int)((N + 63) / 64), ga = (int)((K + 63) / 64);
+  const mx::JoinArgs jb{part, b.part_cols, static_cast<uint16_t*>(dB), dbias, sb, (int)N, gb, !want_b ? 0 : gb * (dB ? quads : 1)};
+  const mx::JoinArgs ja{part_a, nullptr, static_cast<uint16_t*>(dA), nullptr, sk, (int)K, ga, want_a ? ga * quads : 0};
+  if (!want_a && !want_b) return PQ_OK;
+  const dim3 grid((unsigned)(b.blocks + a.blocks)), join((unsigned)(jb.blocks + ja.blocks)), block(256);
+#define PQ_MXS(D, PP)                                                                                       \
+  do {                                                                                                     \
+    if (dbias) hipLaunchKernelGGL((mx::mx_rowsum_kernel<D, PP, true>), grid, block, 0, stream, b, a);      \
+    else hipLaunchKernelGGL((mx::mx_rowsum_kernel<D, PP, false>), grid, block, 0, stream, b, a);           \
+    hipLaunchKernelGGL((mx::mx_join_kernel<D>), join, block, 0, stream, jb, ja, (int)P, (int)R);           \
   } while (0)
   if (dtype == PQ_BF16) {
     if (P == 32) PQ_MXS(PQ_BF16, 32); else PQ_MXS(PQ_BF16, 64);
