@@ -205,21 +205,24 @@ struct DxTile {
   static constexpr int PITCH = 144;                                                                     // waves that bring nothing)
 };
 
-template <int DT, int R>
+// SPLIT: a slice of n each, the sums left in fp32 in p.part for mx_dx_join_kernel.
+template <int DT, int R, bool SPLIT>
 __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
 void mx_dx_ring_kernel(const DxArgs p) {
   using T = DxTile;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[T::LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = wave & 1, wm = wave >> 1, l32 = lane & 31, half = lane >> 5;
+  const int tiles = p.tiles_m * p.tiles_k, z = SPLIT ? (int)blockIdx.x / tiles : 0;
   int tm, tk;
-  tile_of(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_k, 6, tm, tk);
+  tile_of((int)blockIdx.x - z * tiles, tiles, p.tiles_m, p.tiles_k, 6, tm, tk);
   const int m0 = tm * 256, k0 = tk * 256, kt0 = tk * 2, KT = p.KT;
-  const int rows = min(256, p.M - m0), NB = (p.N + 15) >> 4, steps = (p.N + 31) >> 5;
+  const int first = SPLIT ? z * p.slice : 0, N = SPLIT ? min(p.slice, p.N - first) : p.N;   // n of this block (slices: of 64)
+  const int rows = min(256, p.M - m0), NB = (N + 15) >> 4, steps = (N + 31) >> 5;
 
   // Loads outside their buffers give zeros: rows past M and n past N of dy, and n past N or k past K of the weight.
-  const auto rs_dy = __builtin_amdgcn_make_buffer_rsrc((void*)(p.dy + (int64_t)m0 * p.lddy), (short)0,
-                                                       (int)(((rows - 1) * p.lddy + p.N) * 2), kBufferWord3);
+  const auto rs_dy = __builtin_amdgcn_make_buffer_rsrc((void*)(p.dy + (int64_t)m0 * p.lddy + first), (short)0,
+                                                       (int)(((rows - 1) * p.lddy + N) * 2), kBufferWord3);
   const int lddy2 = (int)p.lddy * 2;
   const int dchunk = (lane & 7) ^ (lane >> 3);   // row % 8 == lane / 8
   const int vdy = (wave * 32 + (lane >> 3)) * lddy2 + dchunk * 16;
@@ -229,8 +232,8 @@ void mx_dx_ring_kernel(const DxArgs p) {
   const int vc = kt0 + kb < KT && (wave < 4 || lane < 16)
       ? ((wave < 4 ? wave >> 1 : lane >> 3) * KT + kt0 + kb) * unit + (wave < 4 ? lane : lane & 3) * 16 : kOOB;
   // (the steps go out in order: a pointer, the row blocks left and the ring's slot move along)
-  const uint8_t* cptr = wave < 4 ? p.w : p.ws;
   const int64_t cstep = (int64_t)2 * KT * unit;
+  const uint8_t* cptr = (wave < 4 ? p.w : p.ws) + (first >> 5) * cstep;
   int cleft = NB, cslot = 0;
   const int cdst = wave < 4 ? wave * T::BLOCK : 4 * T::BLOCK;
   auto dma_codes = [&]() {
@@ -247,9 +250,9 @@ void mx_dx_ring_kernel(const DxArgs p) {
   auto dma = [&](int u) {   // phase u's part: dy half u % 2 of stage u / 2 + 2, codes u + 5
     const int st = (u >> 1) + 2, n = st * 64 + dchunk * 8;
     uint8_t* const sb = smem + st % 3 * T::DY + wave * 4096 + (u & 1) * 2048;
-    const int off = n < p.N ? vdy + (u & 1) * 16 * lddy2 + st * 128 : kOOB;
+    const int off = n < N ? vdy + (u & 1) * 16 * lddy2 + st * 128 : kOOB;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_dy, (lds_void_t*)sb, 16, off, 0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_dy, (lds_void_t*)(sb + 1024), 16, n < p.N ? off + 8 * lddy2 : kOOB, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_dy, (lds_void_t*)(sb + 1024), 16, n < N ? off + 8 * lddy2 : kOOB, 0, 0, 0);
     dma_codes();
   };
   // 16 values of a step: row n = tid / 16 of 32, columns 16 (tid % 16) .. Read in one phase, widened in the next: neither waits
@@ -354,6 +357,20 @@ void mx_dx_ring_kernel(const DxArgs p) {
   __syncthreads();   // the rings become the output staging
 
   const int kb0 = k0 + wk * 128, mb = m0 + wm * 64;
+  if constexpr (SPLIT) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int m = mb + 32 * j + l32, kk = kb0 + 32 * i;
+        if (m >= p.M || kk >= p.K) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<v4f*>(p.part + ((int64_t)z * p.M + m) * p.K + kk + 8 * q + 4 * half) =
+              v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+      }
+    return;
+  }
   uint8_t* const stage = smem + wave * 32 * T::PITCH;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
@@ -514,38 +531,46 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const JoinArgs b, const Jo
   if (p.cols && r == 0) p.cols[c] = sum_slices(p.part_cols + c, p.slices, p.C);
 }
 
-// How dx is computed: 256 x 256 blocks where they fill more than half the chip's 256 compute units; else 64 x 128 blocks, with
-// n cut into `slices` where that ends sooner. An estimate in us: a 64-n step of a block takes 0.62 where no more than three
-// blocks share a compute unit; a split costs a launch and 8 bytes an element and slice. Measured (bf16, rank 32):
-//   M x K x N            256 x 256  64 x 128, 1 slice  2 slices  4      8
-//   16384 x 3072 x 12288      1069       1838              -      -      -
-//   4352 x 3072 x 3072        89.2      132.3           160.4  188.9  306.5
-//   2050 x 5120 x 1280        42.5       54.0            78.9   99.2  168.9      180 blocks of 256 x 256
-//   2050 x 1280 x 5120       126.9       69.4            62.4   67.7   76.9
-//   1000 x 1312 x 1040        30.7       13.4            20.1   22.2   26.4
-//   512 x 3072 x 12288       292.7      124.3            90.8   71.5   78.2
-//   154 x 2048 x 640          21.1        8.8             9.5    9.5    9.6
-//   64 x 3072 x 3072          73.3       29.6            21.0   15.0   13.6
+// How dx is computed: in blocks of 256 x 256 (m x k) or 64 x 128, with n cut into `slices` where that ends sooner, by an
+// estimate in us: 1.6 for 64 n of a 256 x 256 block (one to a compute unit) and 9 for its start and end; 0.62 for 64 n of a 64 x
+// 128 block, more where a compute unit holds more than one; 4 for a launch; 1.2 for 10^6 values of the slices' sums (fp32,
+// written and read again). Measured (bf16, rank 32, * the plan's):
+//   M x K x N            256 x 256, slices: 1  2      4      5      8   64 x 128: 1      2      4      8
+//   16384 x 3072 x 12288     1100*  1243   1368   1426   1663      1756   1945   2056   2335
+//   4352 x 3072 x 3072       89.9*   131    174    187    277       138    164    192    303
+//   2050 x 5120 x 1280       43.0*  80.2   98.1    117    163      53.1   79.8   99.6    168
+//   2050 x 1280 x 5120        132   84.0   58.0   55.2*  75.9      68.8   63.0   68.0   78.5
+//   1024 x 3072 x 12288       305    166    103   96.5*   123       151    131    134    145
+//   1024 x 3072 x 3072       80.3   61.1   47.6   47.6   66.3      42.8*  45.1   51.0   65.5
+//   512 x 3072 x 12288        303    163   93.8   80.8   65.7*      124   92.8   76.0   79.5
+//   512 x 12288 x 3072       81.3   68.4*  85.7   86.1    109      64.1   83.0   93.5    119
+//   3000 x 2048 x 2048       59.6   55.4   72.3   75.9   97.4      47.3*  65.4   77.5    102
+//   1000 x 1312 x 1040       30.9   34.7   31.8   30.9   30.5      13.2*  20.4   22.3   26.4
+//   154 x 2048 x 640         21.2   19.7   19.4   18.5   18.4       8.9*   9.5    9.5    9.6
+//   64 x 3072 x 3072         73.9   43.8   28.5   26.4   23.1      29.8   21.0   14.8   13.5*
 struct DxPlan {
   bool ring;
   int slices, slice;
 };
 DxPlan dx_plan(int64_t M, int64_t N, int64_t K) {
-  if (((M + 255) / 256) * ((K + 255) / 256) > 128) return {true, 1, 0};
-  const int64_t blocks = ((M + 63) / 64) * stages(K);
+  const int64_t large = ((M + 255) / 256) * ((K + 255) / 256), small = ((M + 63) / 64) * stages(K);
   const int steps = (int)((N + 63) / 64);
-  double best = 0;
-  int slices = 1;
-  for (int s = 1; s <= 8 && s <= steps; ++s) {
-    const double t = (steps + s - 1) / s * 0.62 * std::max(1.0, (double)(blocks * s) / 768) + (s > 1 ? 4 + s * (double)(M * K) * 2e-6 : 0);
-    if (s == 1 || t < best) best = t, slices = s;
-  }
-  const int per = (steps + slices - 1) / slices;
-  return {false, (steps + per - 1) / per, per * 64};
+  DxPlan best{true, 1, 0};
+  double least = 0;
+  for (int ring = 1; ring >= 0; --ring)
+    for (int s = 1; s <= 8 && s <= steps; ++s) {
+      const int per = (steps + s - 1) / s;
+      if ((s - 1) * per >= steps) continue;   // (no empty slice)
+      const double sharing = std::max(1.0, 0.45 + 0.58 / 256 * (double)(small * s));
+      double t = ring ? (double)((large * s + 255) / 256) * (per * 1.6 + 9) : per * 0.62 * sharing + 4;
+      if (s > 1) t += 4 + s * (double)(M * K) * 1.2e-6;
+      if ((ring && s == 1) || t < least) least = t, best = {ring == 1, s, s > 1 ? per * 64 : 0};
+    }
+  return best;
 }
 
 int launch_dx(DxArgs p, int dtype, int r, hipStream_t stream) {
-#define PQ_MXD(...)                                                                                        \
+#define PQ_MXD()                                                                                           \
   do {                                                                                                     \
     if (dtype == PQ_BF16) {                                                                                \
       if (r == 0) PQ_MXK(PQ_BF16, 0); else if (r == 32) PQ_MXK(PQ_BF16, 32); else PQ_MXK(PQ_BF16, 64);     \
@@ -554,26 +579,33 @@ int launch_dx(DxArgs p, int dtype, int r, hipStream_t stream) {
     }                                                                                                      \
   } while (0)
   const DxPlan plan = dx_plan(p.M, p.N, p.K);
-  if (plan.ring) {
-    p.tiles_m = (p.M + 255) / 256;
-    p.tiles_k = (p.K + 255) / 256;
-    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_k;
-    if (const int st = check_grid(blocks, 512, "mx_grad_input")) return st;
-#define PQ_MXK(D, RR) hipLaunchKernelGGL((mx_dx_ring_kernel<D, RR>), dim3((unsigned)blocks), dim3(512), 0, stream, p)
-    PQ_MXD();
-#undef PQ_MXK
-    return check_launch("mx_grad_input");
-  }
-  const dim3 grid((unsigned)p.KT, (unsigned)((p.M + 63) / 64), (unsigned)plan.slices);   // (at most 128 x 4 blocks of rows)
   p.slice = plan.slice;
+  p.tiles_m = (p.M + 255) / 256;
+  p.tiles_k = (p.K + 255) / 256;
+  const int64_t blocks = (int64_t)p.tiles_m * p.tiles_k * plan.slices;
+  if (plan.ring)
+    if (const int st = check_grid(blocks, 512, "mx_grad_input")) return st;
+  const dim3 ring((unsigned)blocks), grid((unsigned)p.KT, (unsigned)((p.M + 63) / 64), (unsigned)plan.slices);
   if (plan.slices == 1) {
-#define PQ_MXK(D, RR) hipLaunchKernelGGL((mx_dx_kernel<D, RR, false>), grid, dim3(256), 0, stream, p)
-    PQ_MXD();
+    if (plan.ring) {
+#define PQ_MXK(D, RR) hipLaunchKernelGGL((mx_dx_ring_kernel<D, RR, false>), ring, dim3(512), 0, stream, p)
+      PQ_MXD();
 #undef PQ_MXK
+    } else {
+#define PQ_MXK(D, RR) hipLaunchKernelGGL((mx_dx_kernel<D, RR, false>), grid, dim3(256), 0, stream, p)
+      PQ_MXD();
+#undef PQ_MXK
+    }
     return check_launch("mx_grad_input");
   }
-  if (dtype == PQ_BF16) hipLaunchKernelGGL((mx_dx_kernel<PQ_BF16, 0, true>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((mx_dx_kernel<PQ_F16, 0, true>), grid, dim3(256), 0, stream, p);
+  const bool bf16 = dtype == PQ_BF16;
+  if (plan.ring) {
+    if (bf16) hipLaunchKernelGGL((mx_dx_ring_kernel<PQ_BF16, 0, true>), ring, dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((mx_dx_ring_kernel<PQ_F16, 0, true>), ring, dim3(512), 0, stream, p);
+  } else {
+    if (bf16) hipLaunchKernelGGL((mx_dx_kernel<PQ_BF16, 0, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((mx_dx_kernel<PQ_F16, 0, true>), grid, dim3(256), 0, stream, p);
+  }
   const dim3 join((unsigned)((p.K + 127) / 128), (unsigned)((p.M + 31) / 32));
 #define PQ_MXK(D, RR) hipLaunchKernelGGL((mx_dx_join_kernel<D, RR>), join, dim3(256), 0, stream, p, plan.slices)
   PQ_MXD();

@@ -217,16 +217,14 @@ def test_many_rows_through_the_low_rank_branch(cuda, M):
         _inside(g, r[k], bound[k], k)
 
 
-@pytest.mark.parametrize("M,K,N", [(40, 96, 4112), (300, 288, 2080), (4128, 2080, 48), (8300, 1056, 112)])
-def test_input_gradient_of_every_kind_of_block(cuda, M, K, N):
-    """Sums cut into slices (few rows, a long n) and large blocks (more than half the chip's worth of 256 x 256, ragged both
-    ways)."""
+@pytest.mark.parametrize("M,K,N,split", [(40, 96, 4112, True), (300, 288, 2080, True), (1000, 1312, 1040, False), (4128, 2080, 496, False),
+                                         (8300, 1056, 112, False), (2050, 1312, 5136, True), (515, 3104, 9232, True)])
+def test_input_gradient_of_every_kind_of_block(cuda, M, K, N, split):
+    """Both kinds of block, whole sums and sums cut into slices, ragged in every direction."""
     import pyraquant_amd._lib as L
     from pyraquant_amd.mxfp4 import mxfp4_grad_input, quant_mxfp4
 
-    split = L.load().pq_mx_grad_input_workspace_size(M, N, K) > 0
-    large = -(-M // 256) * -(-K // 256) > 128
-    assert split == (M < 1000) and large == (M > 1000)
+    assert (L.load().pq_mx_grad_input_workspace_size(M, N, K) > 0) == split
     g = torch.Generator(device="cuda").manual_seed(M)
     for dtype, R in ((torch.bfloat16, 32), (torch.float16, 64)):
         w = (torch.randn(N, K, generator=g, device=cuda) * 0.02).to(dtype)
