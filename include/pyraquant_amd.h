@@ -398,7 +398,8 @@ int pq_mx_values(const void* codes, const uint8_t* scales, int32_t bits, int64_t
 /*
  * y[m, n] = sum_k xh[m, k] wh[n, k] (+ sum_r t[m, r] l2t[n, r]) (+ bias[n]), summed in fp32, rounded once to dtype (PQ_BF16 or
  * PQ_F16). a, w: packed 4-bit matrices [M, K] and [N, K]. t [M, R] (row stride ldt) and l2t [N, R] of dtype, R in {32, 64}, or
- * NULL. K % 32 == 0, N % 16 == 0, M <= 2^30; operands 16-byte aligned, ldc and ldt multiples of 8.
+ * NULL. K % 32 == 0, N % 16 == 0, M <= 2^30; operands 16-byte aligned, ldc (<= 2^21) and ldt multiples
+ * of 8.
  */
 int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales, const float* bias,
                const void* t, int64_t ldt, const void* l2t, int64_t R, void* c, int64_t ldc, int32_t dtype, int64_t M, int64_t N,
@@ -408,7 +409,7 @@ int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, cons
  * A layer in one call: pq_mx_quant of x into codes and scales (and q8 unless NULL), t = x lr_A into t [M, R] where R is 32 or 64 (0:
  * no low-rank branch; l1f: lr_A in fragment order, l2t: lr_B's rows [N, R], both from pq_mx_factors), and pq_mx_gemm into y [M, N] (row stride ldy). The caller's codes, scales, q8 and t have the sizes
  * given above and may hold anything; up to 32 rows without q8 are quantized inside the product, which leaves codes and scales
- * alone. 16-byte aligned operands, ldx and ldy multiples of 8. With a low-rank branch, a workspace of
+ * alone. 16-byte aligned operands, ldx and ldy (<= 2^21) multiples of 8. With a low-rank branch, a workspace of
  * pq_mx_lowrank_workspace_size(M, K, R) bytes (0 but for few long rows) that may hold anything.
  */
 int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, const uint8_t* w_scales,

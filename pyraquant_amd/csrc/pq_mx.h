@@ -202,6 +202,14 @@ __device__ __forceinline__ void tile_of(int bid, int blocks, int tiles_m, int ti
   tn = r / size;
 }
 
+// Lanes of a wave hand each other values through LDS (which keeps a wave's accesses in order): no instruction, but the compiler
+// may take a lane's own view of memory past it neither way.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Workgroup barrier that leaves LDS-DMA in flight (__syncthreads() would wait for all of it): this wave's LDS reads are done,
 // and nothing moves across it.
 __device__ __forceinline__ void ring_barrier() {

@@ -7,6 +7,7 @@
 #include "pq_mx.h"
 
 #include <algorithm>
+#include <algorithm>
 #include <type_traits>
 
 namespace pq {
@@ -215,6 +216,7 @@ void mx_gemm_kernel(const GemmArgs p) {
               v2u{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
         }
       }
+      wave_sync();
       const int n = nb + ih * 64 + (lane & 7) * 8, row = lane >> 3;
 #pragma unroll
       for (int r0 = 0; r0 < 32; r0 += 8) {
@@ -226,6 +228,7 @@ void mx_gemm_kernel(const GemmArgs p) {
           else *dst = v;
         }
       }
+      wave_sync();
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -246,6 +249,233 @@ int launch_ring(GemmArgs p, int dtype, int r, hipStream_t stream) {
     if (r == 0) PQ_MXG(PQ_F16, 0); else if (r == 32) PQ_MXG(PQ_F16, 32); else PQ_MXG(PQ_F16, 64);
   }
 #undef PQ_MXG
+  return check_launch("mx_gemm");
+}
+
+// ---- large products ----------------------------------------------------------------------------------------------------
+// 256 x 256 blocks on persistent workgroups of eight waves, one to a compute unit: each takes the blocks b, b + grid, .. of its
+// XCD's raster. The same ring and the same turns of two wave groups as above; what a loop over blocks adds is that the next
+// block's first stages and bias are on their way while this one's results go out:
+//  * the sums start from the bias (through LDS, 1 KB a block), so the epilogue needs no registers for it;
+//  * the epilogue's low-rank operands are loaded, then the next block's bias and stages 0 .. NS - 2 are issued into the ring that
+//    the last barrier freed, then the results go out through a staging area of their own, 16 rows of 64 outputs at a time;
+//  * results are stored with buffer stores, whose bounds replace branches: every wave issues the same 16, and the ring's waits
+//    count them (vmcnt completes in order: 16 more may be outstanding until stage NS is waited for).
+template <int DT, int R>
+__global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
+void mx_gemm_large_kernel(const GemmArgs p) {
+  constexpr int TI = 4, TJ = 2, NS = 4;
+  using T = Ring<TI, TJ, 4, NS>;
+  constexpr int BN = T::BN, BM = T::BM, DPW = T::DPW, PITCH = T::PITCH, STORES = 2 * TI * TJ;
+  constexpr int AT_STAGING = T::LDS, AT_BIAS = AT_STAGING + 8 * 16 * PITCH;   // two slots of bias, and one for the idle waves
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[AT_BIAS + 3 * 1024];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave & 1, wm = wave >> 1, l32 = lane & 31, half = lane >> 5, KT = p.KT;
+  const bool grp_b = wave >= 4, w_scales = wave < BN / 64;
+  const int vw = wave * T::DW * KT * 1024 + lane * 16, va = wave * T::DA * KT * 1024 + lane * 16;
+  const int vs = ((wave & 3) * 4 + (lane >> 4)) * KT * 64 + (lane & 15) * 4;
+  const int tiles = p.tiles_m * p.tiles_n;
+
+  int m0, n0;
+  __amdgpu_buffer_rsrc_t rs_w, rs_a, rs_s;
+  auto set = [&](int tile) {
+    int tm, tn;
+    tile_of(tile, tiles, p.tiles_m, p.tiles_n, 6, tm, tn);
+    m0 = tm * BM;
+    n0 = tn * BN;
+    const int blk_w = (min(BN, p.N - n0) + 15) >> 4, blk_a = (min(BM, p.M - m0) + 15) >> 4;
+    const int64_t wb = (int64_t)(n0 >> 4) * KT, ab = (int64_t)(m0 >> 4) * KT;
+    rs_w = __builtin_amdgcn_make_buffer_rsrc((void*)(p.w + wb * 1024), (short)0, blk_w * KT * 1024, kBufferWord3);
+    rs_a = __builtin_amdgcn_make_buffer_rsrc((void*)(p.a + ab * 1024), (short)0, blk_a * KT * 1024, kBufferWord3);
+    rs_s = __builtin_amdgcn_make_buffer_rsrc((void*)(w_scales ? p.ws + wb * 64 : p.as + ab * 64), (short)0,
+                                             (w_scales ? blk_w : blk_a) * KT * 64, kBufferWord3);
+  };
+  auto dma = [&](int buf, int kt) {
+    uint8_t* const sb = smem + buf * T::STAGE;
+    const int off = kt < KT ? kt * 1024 : kOOB;
+#pragma unroll
+    for (int i = 0; i < T::DW; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_w, (lds_void_t*)(sb + (wave * T::DW + i) * 1024), 16, vw + i * KT * 1024 + off, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < T::DA; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_a, (lds_void_t*)(sb + BN * 64 + (wave * T::DA + i) * 1024), 16,
+                                               va + i * KT * 1024 + off, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_s, (lds_void_t*)(sb + T::CODES + wave * 256), 4, vs + (kt < KT ? kt * 64 : kOOB), 0, 0, 0);
+  };
+  // The bias of a block to slot `slot` (waves 0-3, 64 values each) and its first stages; nothing past the last block (`any`).
+  auto start = [&](int slot, bool any) {
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.bias ? p.bias + n0 : (const float*)p.ws), (short)0,
+                                                      p.bias && any ? (p.N - n0) * 4 : 0, kBufferWord3);
+    uint8_t* const dst = smem + AT_BIAS + (wave < 4 ? slot * 1024 + wave * 256 : 2048 + (wave - 4) * 256);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)dst, 4, wave < 4 ? (wave * 64 + lane) * 4 : kOOB, 0, 0, 0);
+#pragma unroll
+    for (int st = 0; st < NS - 1; ++st) dma(st, any ? st : KT);
+  };
+
+  const int sw = k64_swz(lane & 15);
+  const int fw = (wn * (BN / 2) + l32) * 64, fa = (BN + wm * (BM / 4) + l32) * 64;
+  v16f acc[TI][TJ];
+  // one stage: the memory phase, a barrier, the products; `stores`: that many more instructions may be outstanding when the next
+  // stage has landed (one loop: the sums stay in their registers)
+  auto stage_step = [&](int s, int b, bool stores) {
+    auto landed = [&] {
+      if (stores) wait_vmcnt<(NS - 2) * DPW + STORES>();
+      else wait_vmcnt<(NS - 2) * DPW>();
+    };
+    const uint8_t* const sb = smem + b * T::STAGE;
+    v4i w[2][TI], a[2][TJ];
+    int ws[TI], as[TJ];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = ((2 * h + half) ^ sw) << 4;
+#pragma unroll
+      for (int i = 0; i < TI; ++i) w[h][i] = *reinterpret_cast<const v4i*>(sb + fw + i * 2048 + c);
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) a[h][j] = *reinterpret_cast<const v4i*>(sb + fa + j * 2048 + c);
+    }
+#pragma unroll
+    for (int i = 0; i < TI; ++i) ws[i] = *reinterpret_cast<const uint16_t*>(sb + T::CODES + (fw >> 4) + i * 128 + 2 * half);
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) as[j] = *reinterpret_cast<const uint16_t*>(sb + T::CODES + (fa >> 4) + j * 128 + 2 * half);
+    dma(b == 0 ? NS - 1 : b - 1, s + NS - 1);
+    // (kept here: the compiler would put the masking of the words between the products that use them)
+#pragma unroll
+    for (int i = 0; i < TI; ++i) asm volatile("" : "+v"(ws[i]));
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) asm volatile("" : "+v"(as[j]));
+    if (grp_b) landed();
+    ring_barrier();
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[i][j] = mfma4<0>(w[0][i], ws[i], a[0][j], as[j], acc[i][j]);
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[i][j] = mfma4<1>(w[1][i], ws[i], a[1][j], as[j], acc[i][j]);
+    if (!grp_b) landed();
+    ring_barrier();
+  };
+
+  int tile = blockIdx.x, slot = 0;
+  set(tile);
+  start(0, true);
+  wait_vmcnt<(NS - 2) * DPW>();   // the first block's bias and stage 0
+  while (true) {
+    ring_barrier();
+    {   // the sums start from the bias
+      const float* const bs = reinterpret_cast<const float*>(smem + AT_BIAS + slot * 1024) + wn * (BN / 2) + 4 * half;
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          v4f v = {};
+          if (p.bias) v = *reinterpret_cast<const v4f*>(bs + 32 * i + 8 * q);
+#pragma unroll
+          for (int j = 0; j < TJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = v[e];
+        }
+    }
+    if (grp_b) ring_barrier();
+    // Stages 1 and 2 are waited for with the previous block's stores still out (the first block has none).
+    const int lead = tile != (int)blockIdx.x ? NS - 2 : 0;
+    int b = 0;
+    for (int s = 0; s < KT; ++s) {
+      stage_step(s, b, s < lead);
+      b = b + 1 == NS ? 0 : b + 1;
+    }
+    if (!grp_b) ring_barrier();
+    wait_vmcnt<0>();
+    ring_barrier();   // every wave is done with the ring
+
+    // Lane l holds, of tile (i, j): row m = 32 j + l % 32, outputs n = 32 i + 8 q + 4 (l / 32) .. + 3 in elements 4 q ..
+    const int nb = n0 + wn * (BN / 2), mb = m0 + wm * (BM / 4);
+    const auto rs_c = __builtin_amdgcn_make_buffer_rsrc((void*)(p.c + (int64_t)m0 * p.ldc + n0), (short)0,
+                                                        (int)(((min(BM, p.M - m0) - 1) * p.ldc + min(BN, p.N - n0)) * 2), kBufferWord3);
+    const int valid_n = p.N - n0;
+    const int next = tile + (int)gridDim.x;
+    const bool more = next < tiles;
+    auto go_on = [&] {
+      tile = next;
+      slot ^= 1;
+      if (more) set(tile);
+      start(slot, more);
+    };
+    // The low-rank term, 32 ranks at a time; the next block starts once the last operands are asked for.
+    if constexpr (R > 0) {
+#pragma unroll
+      for (int r0 = 0; r0 < R; r0 += 32) {
+        v4i tv[TJ][2], lv[TI][2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int j = 0; j < TJ; ++j)
+            tv[j][x] = *reinterpret_cast<const v4i*>(p.t + (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + r0 + 16 * x + 8 * half);
+#pragma unroll
+          for (int i = 0; i < TI; ++i)
+            lv[i][x] = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(nb + 32 * i + l32, p.N - 1) * R + r0 + 16 * x + 8 * half);
+        }
+        if (r0 + 32 == R) go_on();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int i = 0; i < TI; ++i)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16<DT>(lv[i][x], tv[j][x], acc[i][j]);
+      }
+    } else {
+      go_on();
+    }
+    uint8_t* const out = smem + AT_STAGING + wave * 16 * PITCH;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j)
+#pragma unroll
+      for (int ih = 0; ih < TI / 2; ++ih) {
+        v2u y[2][4];
+#pragma unroll
+        for (int ii = 0; ii < 2; ++ii) {
+          const v16f& v = acc[2 * ih + ii][j];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) y[ii][q] = v2u{pack2<DT>(v[4 * q], v[4 * q + 1]), pack2<DT>(v[4 * q + 2], v[4 * q + 3])};
+        }
+#pragma unroll
+        for (int rows = 0; rows < 2; ++rows) {   // 16 of the 32 rows
+          if ((l32 >> 4) == rows) {
+#pragma unroll
+            for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<v2u*>(out + (l32 & 15) * PITCH + (ii * 32 + 8 * q + 4 * half) * 2) = y[ii][q];
+          }
+          wave_sync();
+          const int n = wn * (BN / 2) + ih * 64 + (lane & 7) * 8;
+#pragma unroll
+          for (int r0 = 0; r0 < 16; r0 += 8) {
+            const int m = wm * (BM / 4) + 32 * j + 16 * rows + r0 + (lane >> 3);
+            const v4u v = *reinterpret_cast<const v4u*>(out + (r0 + (lane >> 3)) * PITCH + (lane & 7) * 16);
+            const int off = n < valid_n ? (m * (int)p.ldc + n) * 2 : kOOB;
+            __builtin_amdgcn_raw_buffer_store_b128(v, rs_c, off, 0, 2);   // (2: streamed past the L2)
+          }
+          wave_sync();
+        }
+      }
+    if (!more) break;
+    wait_vmcnt<(NS - 2) * DPW + STORES>();   // the next block's bias and stage 0
+  }
+  wait_vmcnt<0>();   // (no DMA outlives the workgroup's LDS)
+}
+
+template <int DT>
+int launch_large(GemmArgs p, int r, int cus, hipStream_t stream) {
+  p.tiles_m = (p.M + 255) / 256;
+  p.tiles_n = (p.N + 255) / 256;
+  const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
+  if (blocks > 0x7fffffff - cus) return set_error(PQ_ESHAPE, "mx_gemm: M=%d N=%d too large", p.M, p.N);
+  const dim3 grid((unsigned)std::min<int64_t>(blocks, cus)), block(512);
+  if (r == 0) hipLaunchKernelGGL((mx_gemm_large_kernel<DT, 0>), grid, block, 0, stream, p);
+  else if (r == 32) hipLaunchKernelGGL((mx_gemm_large_kernel<DT, 32>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((mx_gemm_large_kernel<DT, 64>), grid, block, 0, stream, p);
   return check_launch("mx_gemm");
 }
 
@@ -415,7 +645,7 @@ int launch_gemm(const GemmArgs& p, int dtype, int r, hipStream_t stream) {
   int cus = persistent_workgroups(stream);
   if (cus <= 0) cus = 256;
   if (blocks(32, 32) <= 3 * cus) return launch_split<1, 1, 8, 4, false>({p, nullptr, 0, 0}, dtype, r, stream);
-  if (blocks(256, 256) > cus / 2) return launch_ring<4, 2, 4, 4, 1>(p, dtype, r, stream);
+  if (blocks(256, 256) > cus / 2) return dtype == PQ_BF16 ? launch_large<PQ_BF16>(p, r, cus, stream) : launch_large<PQ_F16>(p, r, cus, stream);
   if (blocks(128, 128) > cus) return launch_ring<2, 2, 4, 4, 1>(p, dtype, r, stream);
   return launch_ring<2, 1, 2, 4, 2>(p, dtype, r, stream);
 }
@@ -432,9 +662,9 @@ using namespace pq;
 extern "C" int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales,
                           const float* bias, const void* t, int64_t ldt, const void* l2t, int64_t R, void* c, int64_t ldc,
                           int32_t dtype, int64_t M, int64_t N, int64_t K, hipStream_t stream) {
-  if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || ldc < N || ldc >= (1LL << 31) || M > (1 << 30) ||
+  if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || ldc < N || ldc > (1 << 21) || M > (1 << 30) ||
       N > (1 << 30) || K > (1 << 22))
-    return set_error(PQ_ESHAPE, "pq_mx_gemm: M=%lld N=%lld K=%lld ldc=%lld (N %% 16 == 0, K %% 32 == 0)", (long long)M,
+    return set_error(PQ_ESHAPE, "pq_mx_gemm: M=%lld N=%lld K=%lld ldc=%lld (N %% 16 == 0, K %% 32 == 0, ldc <= 2^21)", (long long)M,
                      (long long)N, (long long)K, (long long)ldc);
   if (dtype != PQ_BF16 && dtype != PQ_F16) return set_error(PQ_EDTYPE, "pq_mx_gemm: dtype %d", dtype);
   if (t ? (R != 32 && R != 64) || ldt < R || ldt > (1 << 22) : false)
@@ -453,7 +683,7 @@ extern "C" int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, 
                             const uint8_t* w_scales, const float* bias, const void* l1f, const void* l2t, int64_t R, void* y,
                             int64_t ldy, int64_t N, uint8_t* codes, uint8_t* scales, int8_t* q8, void* t, void* workspace,
                             int64_t workspace_bytes, hipStream_t stream) {
-  if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || ldx < K || ldy < N || ldy >= (1LL << 31) || M > (1 << 30) ||
+  if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || ldx < K || ldy < N || ldy > (1 << 21) || M > (1 << 30) ||
       N > (1 << 30) || K > (1 << 22))
     return set_error(PQ_ESHAPE, "pq_mx_linear: M=%lld N=%lld K=%lld ldx=%lld ldy=%lld (N %% 16 == 0, K %% 32 == 0)", (long long)M,
                      (long long)N, (long long)K, (long long)ldx, (long long)ldy);

@@ -393,6 +393,7 @@ void mx_dx_ring_kernel(const DxArgs p) {
           *reinterpret_cast<v2u*>(stage + l32 * T::PITCH + (ii * 32 + 8 * q + 4 * half) * 2) =
               v2u{pack2<DT>(y[4 * q], y[4 * q + 1]), pack2<DT>(y[4 * q + 2], y[4 * q + 3])};
       }
+      wave_sync();
       const int k = kb0 + ih * 64 + (lane & 7) * 8, row = lane >> 3;
 #pragma unroll
       for (int r0 = 0; r0 < 32; r0 += 8) {
@@ -400,6 +401,7 @@ void mx_dx_ring_kernel(const DxArgs p) {
         const v4u v = *reinterpret_cast<const v4u*>(stage + (r0 + row) * T::PITCH + (lane & 7) * 16);
         if (m < p.M && k < p.K) *reinterpret_cast<v4u*>(p.dx + (int64_t)m * p.lddx + k) = v;
       }
+      wave_sync();
       __builtin_amdgcn_sched_barrier(0);
     }
 }

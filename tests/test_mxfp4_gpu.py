@@ -523,3 +523,37 @@ def test_example_tunes_and_serves(cuda):
     spec.loader.exec_module(example)
     bare, started, tuned, served = example.run(dim=256, tokens=512, rank=32, steps=40)
     assert tuned < started and tuned < bare and served == tuned, (bare, started, tuned, served)
+
+
+@pytest.mark.parametrize("M,K,N,R", [(4200, 32, 4208, 32), (4200, 160, 4208, 0), (8500, 416, 4368, 64), (8500, 2080, 4368, 32)])
+def test_large_products_over_several_blocks_a_workgroup(cuda, M, K, N, R):
+    """More blocks than compute units, ragged both ways, sums of one stage up to more than the ring holds, over outputs that hold
+    NaN: every element is written, and as the same product in two parts gives it (other blocks, other neighbours in time)."""
+    from pyraquant_amd.mxfp4 import mxfp4_gemm, quant_mxfp4
+
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x, w = torch.randn(M, K, generator=g, device=cuda).bfloat16(), torch.randn(N, K, generator=g, device=cuda).bfloat16()
+    t, l2t = (torch.randn(n, R, generator=g, device=cuda).bfloat16() if R else None for n in (M, N))
+    bias = torch.randn(N, generator=g, device=cuda)
+    xq, wq = quant_mxfp4(x), quant_mxfp4(w)
+    for has_bias in (True, False):
+        out = torch.full((M, N), float("nan"), dtype=torch.bfloat16, device=cuda)
+        for _ in range(3):
+            got = mxfp4_gemm(xq, wq, bias if has_bias else None, torch.bfloat16, t=t, l2t=l2t, out=out)
+        xh, wh = (quant.double() for quant in (_values_of(xq), _values_of(wq)))
+        want = xh @ wh.t() + (bias if has_bias else 0)
+        if R:
+            want = want + t.double() @ l2t.double().t()
+        terms = xh.abs() @ wh.abs().t() + bias.abs() + (t.double().abs() @ l2t.double().abs().t() if R else 0)
+        off = (K + R + 2) * 2.0 ** -23 * terms
+        bound = off + U[torch.bfloat16] * (want.abs() + off)
+        assert not bool(torch.isnan(got).any()) and bool(((got.double() - want).abs() <= bound).all())
+        rows = 160   # few rows: another kernel's blocks
+        part = mxfp4_gemm(quant_mxfp4(x[:rows]), wq, bias if has_bias else None, torch.bfloat16, t=None if t is None else t[:rows], l2t=l2t)
+        assert bool(((part.double() - want[:rows]).abs() <= bound[:rows]).all())
+
+
+def _values_of(q):
+    from pyraquant_amd.mxfp4 import dequant_mxfp4
+
+    return dequant_mxfp4(q, torch.float32)
