@@ -234,26 +234,43 @@ void mx_dx_ring_kernel(const DxArgs p) {
   // (the steps go out in order: a pointer, the row blocks left and the ring's slot move along)
   const int64_t cstep = (int64_t)2 * KT * unit;
   const uint8_t* cptr = (wave < 4 ? p.w : p.ws) + (first >> 5) * cstep;
-  int cleft = NB, cslot = 0;
-  const int cdst = wave < 4 ? wave * T::BLOCK : 4 * T::BLOCK;
+  int cleft = NB, cslot = 0, crec = __builtin_amdgcn_readfirstlane(min(2, NB) * KT * unit);
+  const int cdst = wave <= 4 ? T::AT_CODES + wave * T::BLOCK : T::LDS - 1024 * (8 - wave), cmove = wave <= 4 ? T::CODES : 0;
   auto dma_codes = [&]() {
     const uint64_t at = (uint64_t)cptr;   // (the same in every lane: kept in scalar registers)
     const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at) |
                           (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32;
-    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, __builtin_amdgcn_readfirstlane(max(0, min(2, cleft)) * KT * unit), kBufferWord3);
-    uint8_t* const dst = smem + (wave <= 4 ? T::AT_CODES + cslot * T::CODES + cdst : T::LDS - 1024 * (8 - wave));
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, crec, kBufferWord3);
+    uint8_t* const dst = smem + cdst + cslot * cmove;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)dst, 16, vc, 0, 0, 0);
+  };
+  auto next_codes = [&]() {
     cptr += cstep;
     cleft -= 2;
     cslot = cslot == 4 ? 0 : cslot + 1;
+    crec = __builtin_amdgcn_readfirstlane(max(0, min(2, cleft)) * KT * unit);
   };
-  auto dma = [&](int u) {   // phase u's part: dy half u % 2 of stage u / 2 + 2, codes u + 5
-    const int st = (u >> 1) + 2, n = st * 64 + dchunk * 8;
-    uint8_t* const sb = smem + st % 3 * T::DY + wave * 4096 + (u & 1) * 2048;
-    const int off = n < N ? vdy + (u & 1) * 16 * lddy2 + st * 128 : kOOB;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_dy, (lds_void_t*)sb, 16, off, 0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_dy, (lds_void_t*)(sb + 1024), 16, n < N ? off + 8 * lddy2 : kOOB, 0, 0, 0);
+  // Phase u's part: dy half u % 2 of stage u / 2 + 2, codes u + 5. What it and the reads below need per phase (LDS addresses,
+  // offsets) is worked out between the products of the phase before: every instruction of a memory phase counts.
+  int dslot = 0, dhalf = 0, dn = dchunk * 8, dat = vdy, doff[2];   // slot and half of the DMA; its n, and offset in the buffer
+  auto offsets = [&]() {
+    const int inside = (dn - N) >> 31;   // (all ones where n < N: no branch)
+    doff[0] = (dat & inside) | (kOOB & ~inside);
+    doff[1] = ((dat + 8 * lddy2) & inside) | (kOOB & ~inside);
+  };
+  auto dma = [&]() {
+    uint8_t* const sb = smem + dslot * T::DY + wave * 4096 + dhalf * 2048;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_dy, (lds_void_t*)sb, 16, doff[0], 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_dy, (lds_void_t*)(sb + 1024), 16, doff[1], 0, 0, 0);
     dma_codes();
+  };
+  auto next_dma = [&]() {
+    dat += dhalf ? 128 - 16 * lddy2 : 16 * lddy2;
+    dn += dhalf ? 64 : 0;
+    dslot = dhalf == 0 ? dslot : dslot == 2 ? 0 : dslot + 1;
+    dhalf ^= 1;
+    offsets();
+    next_codes();
   };
   // 16 values of a step: row n = tid / 16 of 32, columns 16 (tid % 16) .. Read in one phase, widened in the next: neither waits
   // for the other. (Lanes 4-7 of 8 store their second half first: eight lanes' 16-byte stores meet no bank twice.)
@@ -261,12 +278,19 @@ void mx_dx_ring_kernel(const DxArgs p) {
   v2u wq;
   int wbyte;
   v4u wide[2];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8_t*)smem;
+  uint32_t code_at = lds0 + T::AT_CODES + wblk * T::BLOCK + (wr & 15) * 64 + ((wb4 ^ k64_swz(wr & 15)) << 4) + (wc & 1) * 8;
+  uint32_t scale_at = lds0 + T::AT_CODES + 4 * T::BLOCK + wblk * 64 + (wr & 15) * 4 + scale_slot(wb4);
   int rslot = 0;   // (read in order too)
   auto rd_codes = [&]() {
-    const uint8_t* const cb = smem + T::AT_CODES + rslot * T::CODES;
+    wq = *(const __attribute__((address_space(3))) v2u*)(uintptr_t)code_at;
+    wbyte = *(const lds_u8_t*)(uintptr_t)scale_at;
+  };
+  auto next_rd_codes = [&]() {
+    const int move = rslot == 4 ? -4 * T::CODES : T::CODES;
+    code_at += move;
+    scale_at += move;
     rslot = rslot == 4 ? 0 : rslot + 1;
-    wq = *reinterpret_cast<const v2u*>(cb + wblk * T::BLOCK + (wr & 15) * 64 + ((wb4 ^ k64_swz(wr & 15)) << 4) + (wc & 1) * 8);
-    wbyte = cb[4 * T::BLOCK + wblk * 64 + (wr & 15) * 4 + scale_slot(wb4)];
   };
   auto widen = [&]() {
     const float s = scale_value(wbyte);
@@ -274,10 +298,12 @@ void mx_dx_ring_kernel(const DxArgs p) {
     wide[0] = widen8<DT>(turn ? wq[1] : wq[0], s) | nan;
     wide[1] = widen8<DT>(turn ? wq[0] : wq[1], s) | nan;
   };
-  auto put = [&](int c) {
-    uint8_t* const row = smem + T::AT_W + (c & 1) * T::W + wr * 512;
-    *reinterpret_cast<v4u*>(row + (((2 * wc + turn) ^ spread(wr)) << 4)) = wide[0];
-    *reinterpret_cast<v4u*>(row + (((2 * wc + 1 - turn) ^ spread(wr)) << 4)) = wide[1];
+  uint32_t put_at[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) put_at[i] = lds0 + T::AT_W + wr * 512 + (((2 * wc + (turn ^ i)) ^ spread(wr)) << 4);
+  auto put = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) *(__attribute__((address_space(3))) v4u*)(uintptr_t)put_at[i] = wide[i];
   };
   // Fragments of the weight (read_columns, in one block of assembly that ends with its own wait: the compiler would wait for
   // every DMA in flight before the builtin's reads). Four tiles of 32 columns, rows 0-15 and 16-31 of the step.
@@ -286,38 +312,46 @@ void mx_dx_ring_kernel(const DxArgs p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = 8 * half + ((lane & 15) >> 2), col = wk * 128 + 32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    wat[i] = (uint32_t)(uintptr_t)(lds_u8_t*)(smem + T::AT_W) + row * 512 + (((col >> 3) ^ spread(row)) << 4) + (col & 4) * 2;
+    wat[i] = lds0 + T::AT_W + row * 512 + (((col >> 3) ^ spread(row)) << 4) + (col & 4) * 2;
   }
-  auto rd_dy = [&](int s) {
-    const uint8_t* const ab = smem + (s >> 1) % 3 * T::DY;
+  uint32_t dy_at[2];   // (a half stage on: the same chunks with bit 2 of their number, bit 6 of the address, turned)
+#pragma unroll
+  for (int h = 0; h < 2; ++h) dy_at[h] = lds0 + (wm * 64 + l32) * 128 + (((2 * h + half) ^ (l32 & 7)) << 4);
+  int yslot = 0;
+  auto rd_dy = [&]() {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int row = wm * 64 + 32 * j + l32, chunk = (s & 1) * 4 + 2 * h + half;
-        a[h][j] = *reinterpret_cast<const v4i*>(ab + row * 128 + ((chunk ^ (row & 7)) << 4));
-      }
+      for (int j = 0; j < 2; ++j) a[h][j] = *(const __attribute__((address_space(3))) v4i*)(uintptr_t)(dy_at[h] + j * 4096);
   };
   v16f acc[4][2] = {};
   const bool grp_b = wave >= 4;
+  offsets();
   dma_codes();
+  next_codes();
 #pragma unroll
-  for (int u = -4; u < 0; ++u) dma(u);
+  for (int u = -4; u < 0; ++u) {
+    dma();
+    next_dma();
+  }
   wait_vmcnt<6>();
   ring_barrier();
   rd_codes();
+  next_rd_codes();
   widen();
-  put(0);
+  put();
   rd_codes();
+  next_rd_codes();
   widen();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) put_at[i] += T::W;
   ring_barrier();
   if (grp_b) ring_barrier();
   for (int s = 0; s < steps; ++s) {
-    put(s + 1);
-    rd_codes();
-    rd_dy(s);
-    dma(s);
-    const uint32_t flip = (s & 1) * T::W;
+    put();        // step s + 1
+    rd_codes();   // of step s + 2
+    rd_dy();
+    dma();
     v4i w0, w1, w2, w3, w4, w5, w6, w7;
     asm volatile(
         "ds_read_b64_tr_b16 v[220:221], %[p0]\n\tds_read_b64_tr_b16 v[222:223], %[p0] offset:2048\n\t"
@@ -331,7 +365,7 @@ void mx_dx_ring_kernel(const DxArgs p) {
         "s_waitcnt lgkmcnt(0)"
         : "=&{v[220:223]}"(w0), "=&{v[224:227]}"(w1), "=&{v[228:231]}"(w2), "=&{v[232:235]}"(w3), "=&{v[236:239]}"(w4),
           "=&{v[240:243]}"(w5), "=&{v[244:247]}"(w6), "=&{v[248:251]}"(w7)
-        : [p0] "v"(wat[0] + flip), [p1] "v"(wat[1] + flip), [p2] "v"(wat[2] + flip), [p3] "v"(wat[3] + flip)
+        : [p0] "v"(wat[0]), [p1] "v"(wat[1]), [p2] "v"(wat[2]), [p3] "v"(wat[3])
         : "memory");
     if (grp_b) wait_vmcnt<6>();
     ring_barrier();
@@ -342,12 +376,25 @@ void mx_dx_ring_kernel(const DxArgs p) {
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<DT>(w[h][i], a[h][j], acc[i][j]);
-    widen();   // (between the products)
-    asm volatile("" : "+v"(wide[0]), "+v"(wide[1]));
+    // Between the products: the next step's weights widened, and the next phase's addresses.
+    widen();
+    const int up = s & 1 ? -T::W : T::W, along = !(s & 1) ? 0 : yslot == 2 ? -2 * T::DY : T::DY;
+    yslot = !(s & 1) ? yslot : yslot == 2 ? 0 : yslot + 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wat[i] += up;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      put_at[i] -= up;
+      dy_at[i] = (dy_at[i] ^ 64) + along;
+    }
+    next_rd_codes();
+    next_dma();
+    asm volatile("" : "+v"(wide[0]), "+v"(wide[1]), "+v"(wat[0]), "+v"(wat[1]), "+v"(wat[2]), "+v"(wat[3]), "+v"(put_at[0]),
+                 "+v"(put_at[1]), "+v"(dy_at[0]), "+v"(dy_at[1]), "+v"(code_at), "+v"(scale_at), "+v"(doff[0]), "+v"(doff[1]));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
     }
     if (!grp_b) wait_vmcnt<6>();
     ring_barrier();
