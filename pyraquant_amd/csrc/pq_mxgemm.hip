@@ -7,7 +7,6 @@
 #include "pq_mx.h"
 
 #include <algorithm>
-#include <algorithm>
 #include <type_traits>
 
 namespace pq {
@@ -35,6 +34,7 @@ __device__ __forceinline__ v16f mfma4(v4i a, int sa, v4i b, int sb, v16f c) {
 // x m). K advances in stages of 128 values (64 bytes a row) through a ring of NS stages in LDS, filled by LDS-DMA: NS - 1
 // stages in flight, no registers or LDS writes spent on them. A stage is the row blocks of the packed layout as they are (the
 // swizzle keeps the ds_read_b128 of 32 rows free of bank conflicts), and after them their scale words, 4 bytes a row.
+// KG groups of these waves, each with a ring of its own, take every KG-th stage; their sums are added in LDS in group order.
 template <int TI, int TJ, int WMW, int NS>
 struct Ring {
   static constexpr int NW = 2 * WMW, BN = 64 * TI, BM = 32 * TJ * WMW;
@@ -44,16 +44,18 @@ struct Ring {
   static_assert(DW * 16 * NW == BN && DA * 16 * NW == BM && SLOTS <= NW, "a stage split over the waves");
   static constexpr int LDS = NS * STAGE;
   static constexpr int PITCH = 144;   // output staging: 64 outputs of a row and 16 bytes of padding
-  static_assert(NW * 32 * PITCH <= LDS, "output staging in the ring");
 };
 
-template <int TI, int TJ, int WMW, int NS, int OCC, int DT, int R>
-__global__ __attribute__((amdgpu_flat_work_group_size(128 * WMW, 128 * WMW), amdgpu_waves_per_eu(OCC * WMW / 2, OCC * WMW / 2)))
+template <int TI, int TJ, int WMW, int NS, int OCC, int KG, int DT, int R>
+__global__ __attribute__((amdgpu_flat_work_group_size(128 * WMW * KG, 128 * WMW * KG),
+                          amdgpu_waves_per_eu(OCC * WMW * KG / 2, OCC * WMW * KG / 2)))
 void mx_gemm_kernel(const GemmArgs p) {
   using T = Ring<TI, TJ, WMW, NS>;
   constexpr int NW = T::NW, BN = T::BN, BM = T::BM;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[T::LDS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ __attribute__((aligned(1024))) uint8_t rings[KG * T::LDS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW;
+  const int group = __builtin_amdgcn_readfirstlane(tid >> 6) / NW;
+  uint8_t* const smem = rings + group * T::LDS;
   const int wn = wave & 1, wm = wave >> 1, l32 = lane & 31, half = lane >> 5;
   int tm, tn;
   tile_of(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, OCC == 1 ? 6 : 8, tm, tn);
@@ -149,13 +151,13 @@ void mx_gemm_kernel(const GemmArgs p) {
   } else {
     // The fragments of the next half stage are read while the products of this one run; one barrier a stage.
 #pragma unroll
-    for (int st = 0; st < NS; ++st) dma(st, st);
+    for (int st = 0; st < NS; ++st) dma(st, st * KG + group);
     wait_vmcnt<(NS - 1) * T::DPW>();
     ring_barrier();
     rd(w0, a0, 0, 0);
     rd_scales(sw_, sa_, 0);
     int b = 0;
-    for (int s = 0; s < KT; ++s) {
+    for (int s = 0; s < KT; s += KG) {
       const int bn = b + 1 == NS ? 0 : b + 1;
       rd(w1, a1, b, 1);
       mm(S0{}, w0, a0, sw_, sa_);
@@ -165,7 +167,7 @@ void mx_gemm_kernel(const GemmArgs p) {
       int nsw[TI], nsa[TJ];
       rd(w0, a0, bn, 0);
       rd_scales(nsw, nsa, bn);
-      dma(b, s + NS);
+      dma(b, s + NS * KG + group);
       mm(S1{}, w1, a1, sw_, sa_);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -176,12 +178,40 @@ void mx_gemm_kernel(const GemmArgs p) {
     }
   }
   wait_vmcnt<0>();
-  __syncthreads();   // the ring becomes the output staging
+  __syncthreads();   // the rings become room for the groups' sums and the output staging
+  if constexpr (KG > 1) {
+    static_assert((KG - 1) * NW * TI * TJ * 4096 + NW * 32 * T::PITCH <= KG * T::LDS, "sums and staging in the rings");
+    auto sums = [&](int g, int i, int j, int q) {
+      return reinterpret_cast<v4f*>(rings) + (((((g - 1) * NW + wave) * TI + i) * TJ + j) * 4 + q) * 64 + lane;
+    };
+    if (group)
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *sums(group, i, j, q) = v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 1; g < KG; ++g)
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const v4f v = *sums(g, i, j, q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
+          }
+  }
 
   // Lane l holds, of tile (i, j): row m = 32 j + l % 32, outputs n = 32 i + 8 q + 4 (l / 32) .. + 3 in elements 4 q ... They
   // go through LDS two weight tiles at a time so that whole 128-byte lines are stored.
   const int nb = n0 + wn * (BN / 2), mb = m0 + wm * (BM / WMW);
-  uint8_t* const stage = smem + wave * 32 * T::PITCH;
+  uint8_t* const stage = rings + (KG - 1) * NW * TI * TJ * 4096 + wave * 32 * T::PITCH;
   v4i tv[R ? R / 16 : 1];
 #pragma unroll
   for (int j = 0; j < TJ; ++j) {
@@ -234,15 +264,15 @@ void mx_gemm_kernel(const GemmArgs p) {
   }
 }
 
-template <int TI, int TJ, int WMW, int NS, int OCC>
+template <int TI, int TJ, int WMW, int NS, int OCC, int KG>
 int launch_ring(GemmArgs p, int dtype, int r, hipStream_t stream) {
   using T = Ring<TI, TJ, WMW, NS>;
   p.tiles_m = (p.M + T::BM - 1) / T::BM;
   p.tiles_n = (p.N + T::BN - 1) / T::BN;
   const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
-  if (const int st = check_grid(blocks, 128 * WMW, "mx_gemm")) return st;
+  if (const int st = check_grid(blocks, 128 * WMW * KG, "mx_gemm")) return st;
 #define PQ_MXG(D, RR) \
-  hipLaunchKernelGGL((mx_gemm_kernel<TI, TJ, WMW, NS, OCC, D, RR>), dim3((unsigned)blocks), dim3(128 * WMW), 0, stream, p)
+  hipLaunchKernelGGL((mx_gemm_kernel<TI, TJ, WMW, NS, OCC, KG, D, RR>), dim3((unsigned)blocks), dim3(128 * WMW * KG), 0, stream, p)
   if (dtype == PQ_BF16) {
     if (r == 0) PQ_MXG(PQ_BF16, 0); else if (r == 32) PQ_MXG(PQ_BF16, 32); else PQ_MXG(PQ_BF16, 64);
   } else {
@@ -628,26 +658,31 @@ int launch_split(const SplitArgs& p, int dtype, int r, hipStream_t stream) {
   return check_launch("mx_gemm");
 }
 
-// The block of a product, by how its blocks fill the chip. us (bf16, rank 32, bias):
-//   M x K x N            256x256  128x128  128x64  128x256  32x32 split   (n x m; 256x256, 128x256: one workgroup per CU)
-//   65536 x 3072 x 12288   1562     1839    2294     1893       -
-//   4096 x 3072 x 3072     31.1     33.1    39.0     38.9     92.3
-//   2050 x 1280 x 5120     17.7     21.3    22.5     22.9     48.3      180 blocks of 256 x 256
-//   512 x 3072 x 12288     24.9     24.2    24.3     20.0     47.6      192 blocks of 128 x 256, 384 of 128 x 128
-//   1024 x 3072 x 3072     23.3     12.6    11.7     17.5     24.8      384 blocks of 128 x 64, 192 of 128 x 128
-//   512 x 12288 x 3072     65.9     30.4    25.1     49.3     39.3
-//   256 x 3072 x 3072      23.3     11.5     8.5     17.0      8.1      768 blocks of 32 x 32
-//   154 x 2048 x 1280      18.5      9.2     6.7     13.1      4.2
-//   1 x 12288 x 3072       62.6     28.3    21.4     47.3      8.7
-// (128 x 128 wins nowhere and is not built. What the last line gets fits two of its workgroups per CU at once.)
+// The block of a product, by how its blocks fill the chip. us of the kernel (bf16, rank 32, bias):
+//   M x K x N            256x256  128x256  128x64  128x64, 3 groups  32x32 split   (n x m; 256x256, 128x256: one workgroup per CU)
+//   65536 x 3072 x 12288   1387     1893    2294                                   (256x256: persistent, times the CUs' rounds)
+//   4096 x 3072 x 3072     27.0     38.9    39.0                       92.3
+//   2050 x 1280 x 5120     16.0     22.9    22.5                       48.3        180 blocks of 256 x 256
+//   512 x 3072 x 12288     24.9     20.0    24.3                       47.6        192 blocks of 128 x 256, 384 of 128 x 128
+//   1024 x 3072 x 3072     23.3     17.5    11.7                       24.8        384 blocks of 128 x 64
+//   512 x 12288 x 3072     65.9     49.3    26.3         22.4          39.3        192 blocks of 128 x 64, one to a CU
+//   512 x 3072 x 3072                       10.6         10.4                      the same, 24 stages of K
+//   300 x 640 x 5120                         6.2          7.4                      5 stages: the groups' join costs more
+//   256 x 3072 x 3072      23.3     17.0     8.5                        8.1        768 blocks of 32 x 32
+//   154 x 2048 x 1280      18.5     13.1     6.7                        4.2
+//   1 x 12288 x 3072       62.6     47.3    21.4                        8.7
+// (128 x 128 won nowhere and is not built. What the last column gets fits two of its workgroups per CU at once. A lone
+// workgroup of four waves leaves LDS idle between its barriers; three groups of four keep it busy: 96 stages of 12 KB in and 24
+// KB out at 128 B a clock are 14 us. Deeper rings alone changed nothing.)
 int launch_gemm(const GemmArgs& p, int dtype, int r, hipStream_t stream) {
   auto blocks = [&](int bn, int bm) { return (int64_t)((p.N + bn - 1) / bn) * ((p.M + bm - 1) / bm); };
   int cus = persistent_workgroups(stream);
   if (cus <= 0) cus = 256;
   if (blocks(32, 32) <= 3 * cus) return launch_split<1, 1, 8, 4, false>({p, nullptr, 0, 0}, dtype, r, stream);
   if (blocks(256, 256) > cus / 2) return dtype == PQ_BF16 ? launch_large<PQ_BF16>(p, r, cus, stream) : launch_large<PQ_F16>(p, r, cus, stream);
-  if (blocks(128, 128) > cus) return launch_ring<2, 2, 4, 4, 1>(p, dtype, r, stream);
-  return launch_ring<2, 1, 2, 4, 2>(p, dtype, r, stream);
+  if (blocks(128, 128) > cus) return launch_ring<2, 2, 4, 4, 1, 1>(p, dtype, r, stream);
+  if (blocks(128, 64) <= cus && p.KT > 24) return launch_ring<2, 1, 2, 4, 1, 3>(p, dtype, r, stream);
+  return launch_ring<2, 1, 2, 4, 2, 1>(p, dtype, r, stream);
 }
 
 // Rows that the product's own lanes quantize: a block's lanes hold 32 rows, so each row is quantized once per 32 outputs.

@@ -238,9 +238,11 @@ def test_input_gradient_of_every_kind_of_block(cuda, M, K, N, split):
         assert torch.equal(got, mxfp4_grad_input(dy, quant_mxfp4(w), dt, ap))
 
 
-@pytest.mark.parametrize("M,K,N,R", [(2100, 160, 4112, 0), (600, 1056, 7056, 32), (513, 96, 2064, 64), (1100, 352, 912, 32)])
+@pytest.mark.parametrize("M,K,N,R", [(2100, 160, 4112, 0), (600, 1056, 7056, 32), (513, 96, 2064, 64), (1100, 352, 912, 32),
+                                     (329, 4320, 2512, 32)])
 def test_product_of_every_kind_of_block(cuda, M, K, N, R):
-    """Sizes whose product runs in blocks of 256 x 256, 128 x 256 and 128 x 64 (n x m), all of them ragged."""
+    """Sizes whose product runs in blocks of 256 x 256, 128 x 256 and 128 x 64 (n x m), all of them ragged; the last in blocks
+    whose stages three groups of waves share, one more stage than a multiple of three."""
     from pyraquant_amd.mxfp4 import mxfp4_gemm, quant_mxfp4
 
     g = torch.Generator(device="cuda").manual_seed(M)
