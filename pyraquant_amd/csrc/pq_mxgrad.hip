@@ -455,8 +455,8 @@ void mx_dx_ring_kernel(const DxArgs p) {
 
 // ---- sums over rows: part[s][r][c] = sum over the rows of slice s of v[m, r] z[m, c] -------------------------------------
 // z is dy (EIGHT false) or the 8-bit codes of x with their scales; v is t or dt, [M, R]. Column sums of z too (COLS). A
-// workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step; the order of the sums is fixed. Bound by
-// reading z (dy of 16384 x 12288: 88 us, 4.6 TB/s).
+// workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step, the next step's rows on their way into
+// registers meanwhile; the order of the sums is fixed. Bound by reading z: 460 MB of 16384 x 3072 x 12288 in 98 us, 4.7 TB/s.
 struct SumArgs {
   const void* z;
   const uint8_t* scales;
@@ -478,41 +478,56 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
   const uint32_t one2 = DT == PQ_BF16 ? 0x3f803f80u : 0x3c003c00u;
   const v4i ones = {(int)one2, (int)one2, (int)one2, (int)one2};
   v16f acc[R / 32] = {}, cols = {};
-  for (int m0 = s0; m0 < end; m0 += 64) {
-    __syncthreads();
+  v4u zr[EIGHT ? 2 : 4], vr[R / 32];
+  int byte = 0;
+  auto load = [&](int m0) {
     if constexpr (EIGHT) {
-      const int row = tid >> 2, b = tid & 3, m = m0 + row, c = c0 + b * 32;
-      const bool in = m < end && c < p.C;
-      v4u q[2] = {};
-      int byte = 0;
-      if (in) {
+      const int m = m0 + (tid >> 2), b = tid & 3, c = c0 + b * 32;
+      zr[0] = zr[1] = v4u{0, 0, 0, 0};
+      byte = 0;
+      if (m < end && c < p.C) {
         const v4u* const src = reinterpret_cast<const v4u*>(static_cast<const int8_t*>(p.z) + (int64_t)m * p.ldz + c);
-        q[0] = src[0];
-        q[1] = src[1];
+        zr[0] = src[0];
+        zr[1] = src[1];
         byte = p.scales[scale_offset(m, panel, b, p.KT)];
-      }
-      const float s = in ? restore_scale(byte) : 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const v2u lo = restore4<DT>(q[i >> 1][2 * (i & 1)], s), hi = restore4<DT>(q[i >> 1][2 * (i & 1) + 1], s);
-        *reinterpret_cast<v4u*>(z_at(row, b * 4 + i)) = v4u{lo[0], lo[1], hi[0], hi[1]};
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = i * 16 + (tid >> 4), chunk = tid & 15, m = m0 + row, c = c0 + chunk * 8;
-        v4u x = v4u{0, 0, 0, 0};
-        if (m < end && c < p.C) x = *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(p.z) + (int64_t)m * p.ldz + c);
-        *reinterpret_cast<v4u*>(z_at(row, chunk)) = x;
+        const int m = m0 + i * 16 + (tid >> 4), c = c0 + (tid & 15) * 8;
+        zr[i] = v4u{0, 0, 0, 0};
+        if (m < end && c < p.C) zr[i] = *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(p.z) + (int64_t)m * p.ldz + c);
       }
     }
-    for (int i = tid; i < 64 * R / 8; i += 256) {
-      const int row = i / (R / 8), chunk = i % (R / 8);
-      v4u x = v4u{0, 0, 0, 0};
-      if (m0 + row < end) x = *reinterpret_cast<const v4u*>(p.v + (int64_t)(m0 + row) * R + chunk * 8);
-      *reinterpret_cast<v4u*>(v_at(row, chunk)) = x;
+#pragma unroll
+    for (int i = 0; i < R / 32; ++i) {
+      const int at = i * 256 + tid, m = m0 + at / (R / 8);
+      vr[i] = v4u{0, 0, 0, 0};
+      if (m < end) vr[i] = *reinterpret_cast<const v4u*>(p.v + (int64_t)m * R + at % (R / 8) * 8);
+    }
+  };
+  load(s0);
+  for (int m0 = s0; m0 < end; m0 += 64) {
+    __syncthreads();
+    if constexpr (EIGHT) {
+      const int row = tid >> 2, b = tid & 3;
+      const float s = restore_scale(byte);   // (past the end the codes are zeros)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v2u lo = restore4<DT>(zr[i >> 1][2 * (i & 1)], s), hi = restore4<DT>(zr[i >> 1][2 * (i & 1) + 1], s);
+        *reinterpret_cast<v4u*>(z_at(row, b * 4 + i)) = v4u{lo[0], lo[1], hi[0], hi[1]};
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<v4u*>(z_at(i * 16 + (tid >> 4), tid & 15)) = zr[i];
+    }
+#pragma unroll
+    for (int i = 0; i < R / 32; ++i) {
+      const int at = i * 256 + tid;
+      *reinterpret_cast<v4u*>(v_at(at / (R / 8), at % (R / 8))) = vr[i];
     }
     __syncthreads();
+    if (m0 + 64 < end) load(m0 + 64);   // in flight while this step's products run
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const v4i z = read_columns(z_at, 16 * s, wave * 32, lane);
@@ -663,11 +678,14 @@ int launch_dx(DxArgs p, int dtype, int r, hipStream_t stream) {
   return check_launch("mx_grad_input");
 }
 
-// Row slices of mx_rowsum_kernel: enough workgroups to fill the chip, none of fewer than 64 rows.
+// Row slices of mx_rowsum_kernel: about 384 workgroups a sum. More only add sums to write and join; fewer read too little at once.
+// us of both launches, for 256 / 384 / 512 / 1024 workgroups (bf16): 2050 x 1280 x 5120 rank 64 19.0 / 19.6 / 20.9 / 25.2,
+// 4352 x 3072 x 3072 rank 32 17.1 / 17.3 / 21.4 / 26.1, 16384 x 3072 x 12288 116 / 104 / 103 / 105.
 int row_slices(int64_t M, int64_t C) {
   const int64_t panels = (C + 127) / 128, steps = (M + 63) / 64;
-  const int64_t want = std::max<int64_t>(1, (1024 + panels - 1) / panels);
-  return (int)std::min<int64_t>({want, steps, 256});
+  const int64_t want = std::min<int64_t>({(384 + panels - 1) / panels, steps, 256});
+  const int64_t each = (steps + want - 1) / want;
+  return (int)((steps + each - 1) / each);   // (no empty slice)
 }
 
 }  // namespace
