@@ -217,16 +217,29 @@ __global__ __launch_bounds__(256) void mx_factors_kernel(const Factor fa, const 
   __shared__ uint16_t tile[64][66];   // [c][r]; a pitch of 33 words: both directions spread over the banks
   const bool is_a = (int)blockIdx.x < blocks_a;
   const Factor f = is_a ? fa : fb;
-  const int c0 = ((int)blockIdx.x - (is_a ? 0 : blocks_a)) * 64;
+  const int c0 = ((int)blockIdx.x - (is_a ? 0 : blocks_a)) * 64, log_p = P == 32 ? 5 : 6;
   if (!f.rows && !f.frags) return;
-  for (int i = threadIdx.x; i < 64 * P; i += 256) {
-    int c, r;
+  auto at = [&](int i, int& c, int& r) {
     if (f.kind == PQ_MX_BY_RANK) { r = i >> 6; c = i & 63; }   // read along c
-    else { c = i / P; r = i - c * P; }                         // read along r
-    const bool in = c0 + c < f.C && r < R;
-    tile[c][r] = !in ? 0 : f.kind == PQ_MX_BY_COLUMN ? f.src[(int64_t)(c0 + c) * f.ld + r]
-                         : f.kind == PQ_MX_BY_RANK   ? f.src[(int64_t)r * f.ld + c0 + c]
-                                                     : f.src[frag_offset(c0 + c, r, P)];
+    else { c = i >> log_p; r = i & (P - 1); }                  // read along r
+  };
+  for (int i0 = threadIdx.x; i0 < 64 * P; i0 += 8 * 256) {   // eight loads in flight (64 P is a multiple of 8 * 256)
+    uint16_t v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      int c, r;
+      at(i0 + e * 256, c, r);
+      const bool in = c0 + c < f.C && r < R;
+      v[e] = !in ? 0 : f.kind == PQ_MX_BY_COLUMN ? f.src[(int64_t)(c0 + c) * f.ld + r]
+                     : f.kind == PQ_MX_BY_RANK   ? f.src[(int64_t)r * f.ld + c0 + c]
+                                                 : f.src[frag_offset(c0 + c, r, P)];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      int c, r;
+      at(i0 + e * 256, c, r);
+      tile[c][r] = v[e];
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 8 * P; i += 256) {
@@ -238,7 +251,7 @@ __global__ __launch_bounds__(256) void mx_factors_kernel(const Factor fa, const 
       *reinterpret_cast<v4u*>(f.frags + frag_offset(c0 + 8 * g, r, P)) = v4u{w[0], w[1], w[2], w[3]};
     }
     if (f.rows) {    // 8 ranks of one column
-      const int g = i % (P / 8), c = i / (P / 8);
+      const int g = i & (P / 8 - 1), c = i >> (log_p - 3);
       uint32_t w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = tile[c][8 * g + 2 * e] | ((uint32_t)tile[c][8 * g + 2 * e + 1] << 16);
