@@ -398,19 +398,19 @@ int pq_mx_values(const void* codes, const uint8_t* scales, int32_t bits, int64_t
 /*
  * y[m, n] = sum_k xh[m, k] wh[n, k] (+ sum_r t[m, r] l2t[n, r]) (+ bias[n]), summed in fp32, rounded once to dtype (PQ_BF16 or
  * PQ_F16). a, w: packed 4-bit matrices [M, K] and [N, K]. t [M, R] (row stride ldt) and l2t [N, R] of dtype, R in {32, 64}, or
- * NULL. K % 32 == 0, N % 16 == 0, M <= 2^30; operands 16-byte aligned, ldc (<= 2^21) and ldt multiples
- * of 8.
+ * NULL. K % 32 == 0, N % 16 == 0, M <= 2^30; operands 16-byte aligned, ldc (<= 2^21) and ldt multiples of 8.
  */
 int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales, const float* bias,
                const void* t, int64_t ldt, const void* l2t, int64_t R, void* c, int64_t ldc, int32_t dtype, int64_t M, int64_t N,
                int64_t K, hipStream_t stream);
 
 /*
- * A layer in one call: pq_mx_quant of x into codes and scales (and q8 unless NULL), t = x lr_A into t [M, R] where R is 32 or 64 (0:
- * no low-rank branch; l1f: lr_A in fragment order, l2t: lr_B's rows [N, R], both from pq_mx_factors), and pq_mx_gemm into y [M, N] (row stride ldy). The caller's codes, scales, q8 and t have the sizes
- * given above and may hold anything; up to 32 rows without q8 are quantized inside the product, which leaves codes and scales
- * alone. 16-byte aligned operands, ldx and ldy (<= 2^21) multiples of 8. With a low-rank branch, a workspace of
- * pq_mx_lowrank_workspace_size(M, K, R) bytes (0 but for few long rows) that may hold anything.
+ * A layer in one call: pq_mx_quant of x into codes and scales (and q8 unless NULL), t = x lr_A into t [2, M, R] where R is 32
+ * or 64 (0: no low-rank branch; l1f: lr_A in fragment order, l2t: lr_B's rows [N, R], both from pq_mx_factors), and pq_mx_gemm into
+ * y [M, N] (row stride ldy). The caller's codes, scales, q8 and t have the sizes given above and may hold anything; up to 32 rows
+ * without q8 are quantized inside the product, which leaves codes and scales alone. 16-byte aligned operands, ldx and ldy (<=
+ * 2^21) multiples of 8. With a low-rank branch, a workspace of pq_mx_lowrank_workspace_size(M, K, R) bytes (0 but for few long
+ * rows) that may hold anything.
  */
 int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, const uint8_t* w_scales,
                  const float* bias, const void* l1f, const void* l2t, int64_t R, void* y, int64_t ldy, int64_t N, uint8_t* codes,
@@ -431,8 +431,8 @@ int pq_mx_factors(const void* A, int64_t lda, int32_t a_order, const void* B, in
                   int64_t R, int64_t P, void* af, void* ap, void* bt, void* bf, hipStream_t stream);
 
 /*
- * t[m, r] = sum_k x[m, k] l1[k, r] ([M, R] of dtype, R in {32, 64}), l1 in fragment order (pq_mx_factors), summed in fp32 and
- * rounded to dtype (PQ_BF16 or PQ_F16). K % 16 == 0; operands 16-byte aligned, ldx a multiple of 8. A workspace of
+ * t[m, r] = sum_k x[m, k] l1[k, r] ([2, M, R] of dtype, R in {32, 64}), l1 in fragment order (pq_mx_factors), summed in fp32 and
+ * stored in two parts of dtype (PQ_BF16 or PQ_F16): rounded to it, and what that rounding left out. K % 16 == 0; operands 16-byte aligned, ldx a multiple of 8. A workspace of
  * pq_mx_lowrank_workspace_size bytes (0 but for few long rows) that may hold anything.
  */
 int64_t pq_mx_lowrank_workspace_size(int64_t M, int64_t K, int64_t R);
@@ -454,8 +454,9 @@ int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, const uint8_t*
 /*
  * The gradients of the low-rank factors and the bias: dB[r, n] = sum_m t[m, r] dy[m, n] ([R, N]), dA[k, r] = sum_m xt[m, k]
  * dt[m, r] ([K, R], xt: the values of the checkpoint q8 with x_scales), dbias[n] = sum_m dy[m, n] (fp32). An output that is
- * NULL is not computed, and what only it needs (dy and t for dB and dbias; dt, q8 and x_scales for dA) may be NULL too. t and dt are [M, P], zero past rank R. Sums in fp32, in an order that depends on the sizes alone; dA and dB rounded to dtype.
- * The workspace (pq_mx_grad_factors_workspace_size bytes) may hold anything.
+ * NULL is not computed, and what only it needs (dy and t for dB and dbias; dt, q8 and x_scales for dA) may be NULL too. t and
+ * dt are [2, M, P], the two parts of each as pq_mx_lowrank_down gives them, zero past rank R. Sums in fp32, in an order that depends on the sizes alone; dA and dB rounded to dtype. The
+ * workspace (pq_mx_grad_factors_workspace_size bytes) may hold anything.
  */
 int64_t pq_mx_grad_factors_workspace_size(int64_t M, int64_t K, int64_t N, int64_t P);
 int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, const void* t, const void* dt, const int8_t* q8,

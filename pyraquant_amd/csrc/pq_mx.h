@@ -15,7 +15,7 @@
 namespace pq {
 namespace mx {
 
-// t = x l1t^T [M, R] and, unless codes is NULL, the codes of x (and q8), in one pass (pq_mx.hip). K % 16 == 0 (32 with codes),
+// t = x l1t^T [2, M, R] (two_parts) and, unless codes is NULL, the codes of x (and q8), in one pass (pq_mx.hip). K % 16 == 0 (32 with codes),
 // 16-byte aligned rows, R 32 or 64, l1f: l1t in fragment order (pq_mx_factors); arguments checked by the caller.
 int lowrank(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R, uint8_t* codes,
             uint8_t* scales, int8_t* q8, void* t, void* workspace, hipStream_t stream);
@@ -173,10 +173,27 @@ __device__ __forceinline__ float restore_scale(int byte) {
   return byte == kNaN ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(1.0f, byte - 131);
 }
 
+// Four sums as 16-bit values, and what that rounding left out, rounded too (0 where a value is not finite): the two together hold
+// a sum to twice the bits, for sums over many rows (gradients of the factors), where a rounding of t or dt to 16 bits would be
+// as large as the result's own. Terms that are added to a larger sum and rounded with it take the first part alone.
+template <int DT>
+__device__ __forceinline__ void two_parts(v4f s, v2u& hi, v2u& lo) {
+  hi = v2u{pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3])};
+  float r[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t h = e & 1 ? hi[e >> 1] >> 16 : hi[e >> 1] & 0xffff;
+    r[e] = s[e] - (DT == PQ_BF16 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h));
+    if (!(fabsf(r[e]) < INFINITY)) r[e] = 0.0f;
+  }
+  lo = v2u{pack2<DT>(r[0], r[1]), pack2<DT>(r[2], r[3])};
+}
+
 // ---- shared by the products ------------------------------------------------------------------------------------------
-// Products of 16-bit operands, fp32 sums: 32 x 32 x 16, and 16 x 16 x 32 (register to register the latter reach 2.0 PFLOP/s against
-// 1.75 in bf16, and the 4-bit 16 x 16 x 128 reach 6.95 against 6.5 of 32 x 32 x 64: at the power limit, where the registers' sums
-// are read and written half as often per operation).
+// Products of 16-bit operands, fp32 sums. From registers alone, at the power limit, 32 x 32 x 16 runs at 1.75 PFLOP/s in bf16
+// and 16 x 16 x 32 at 2.0; for 4-bit operands 32 x 32 x 64 at 6.5 and 16 x 16 x 128 at 6.95. The large kernels take the 32 x 32
+// shapes all the same: the others read half as much again from LDS for a block, and the product was 12 % slower with them, the
+// input gradient 6-8 % in one round of blocks. 16 x 16 x 32 serves the low-rank products, whose operand is a quantizer's lane.
 template <int DT>
 __device__ __forceinline__ v4f mfma16_16(v4i a, v4i b, v4f c) {
   if constexpr (DT == PQ_BF16)

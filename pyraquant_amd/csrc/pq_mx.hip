@@ -4,7 +4,8 @@
 // One lane takes one block of 32 values: its largest magnitude, its scale byte and its 16 bytes of codes need no other lane.
 // A wave takes 16 rows x 4 blocks, which is one 1 KB block of the packed layout, so its codes go out as one contiguous
 // 1 KB store and a row's 4 blocks are whole 128-byte lines of the input. Bound by memory: 2 bytes read per value, 1/2 +
-// 1/32 written (and 1 for the 8-bit codes).
+// 1/32 written (and 1 for the 8-bit codes): 65536 x 3072 bf16 in 88 us, 5.8 TB/s, and in 131 us, 5.4 TB/s, with the 8-bit codes
+// (a large copy: 5.1 TB/s); 640 x 640 in 3 us, a launch.
 #include "pq_mx.h"
 
 #include <algorithm>
@@ -45,12 +46,14 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(const void* __restrict__ 
   }
 }
 
-// t = x l1t^T ([M, R], 16-bit) and, where QUANT, the codes of x, in one pass over x. A workgroup takes 16 RG rows and its NW
+// t = x l1t^T ([2, M, R], 16-bit) and, where QUANT, the codes of x, in one pass over x. A workgroup takes 16 RG rows and its NW
 // waves every NW-th stage of 128 values, 16 rows at a time as above: what a lane holds of x for its block is also its operand
 // of the 16 x 16 x 32 products (8 consecutive values of a row; the order of k within the sum is free as long as l1t's operand
 // has the same), so x is read once and needs no other lane or LDS. l1t comes from the cache in fragment order (1 KB a load, zeros
-// past K), once per RG row groups. The
-// waves' sums are added in LDS in a fixed order and rounded once: t is rounded to 16 bits because the products that take it do.
+// past K), once per RG row groups. The waves' sums are added in LDS in a fixed order and stored as two 16-bit parts: what takes t
+// (the product's low-rank term, dB) and dt, made here too (dx, dA), are products of 16-bit operands.
+// Bound by reading x and by l1t from the cache: 65536 x 3072 with codes 101 us (the quantizer alone: 88), dy of 16384 x 12288
+// to dt in 103-110 us, 3.7-3.9 TB/s.
 template <int DT, int R, int RG, int NW, bool QUANT, bool CKPT>
 __global__ __launch_bounds__(64 * NW) void mx_lowrank_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t M, int K, int KT,
                                                              const uint16_t* __restrict__ l1f, uint8_t* __restrict__ codes,
@@ -129,8 +132,10 @@ __global__ __launch_bounds__(64 * NW) void mx_lowrank_kernel(const uint16_t* __r
     if (row >= M) continue;
     if (partial)
       *reinterpret_cast<v4f*>(partial + (blockIdx.y * M + row) * R + 16 * (tile % C) + 4 * (l >> 4)) = sum;
-    else
-      *reinterpret_cast<v2u*>(t + row * R + 16 * (tile % C) + 4 * (l >> 4)) = v2u{pack2<DT>(sum[0], sum[1]), pack2<DT>(sum[2], sum[3])};
+    else {
+      v2u* const out = reinterpret_cast<v2u*>(t + row * R + 16 * (tile % C) + 4 * (l >> 4));
+      two_parts<DT>(sum, out[0], out[M * R / 4]);
+    }
   }
 }
 
@@ -146,10 +151,11 @@ __global__ __launch_bounds__(256) void mx_lowrank_join_kernel(const float* __res
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] += v[e];
   }
-  *reinterpret_cast<v2u*>(t + i) = v2u{pack2<DT>(sum[0], sum[1]), pack2<DT>(sum[2], sum[3])};
+  two_parts<DT>(sum, *reinterpret_cast<v2u*>(t + i), *reinterpret_cast<v2u*>(t + n + i));
 }
 
-// Values of the 4-bit codes (EIGHT: of the 8-bit ones), one lane a block. ODT: output type.
+// Values of the 4-bit codes (EIGHT: of the 8-bit ones), one lane a block. ODT: output type. Bound by the store of 2 or 4 bytes a
+// value: quantizing 12288 x 3072 and this back to bf16 take 45 us together.
 template <int ODT, bool EIGHT>
 __global__ __launch_bounds__(256) void mx_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                         int64_t M, int K, int KT, void* __restrict__ out, int64_t ldo,
@@ -203,7 +209,8 @@ __global__ __launch_bounds__(256) void mx_values_kernel(const uint8_t* __restric
 // The factors in the orders the layer's kernels read them, zero-padded from rank R to P. A factor is a matrix of C columns c (k of
 // lr_A, n of lr_B) by r; a workgroup takes 64 columns of one. Source: [C, R] rows (kByColumn), [R, C] rows (kByRank) or
 // fragments. Results, either or none: rows [C, P], and fragments: for each 128 columns, 8-column group i of a block and
-// 16 ranks, the 64 lanes' 16 bytes in a row, as mx_lowrank_kernel loads them.
+// 16 ranks, the 64 lanes' 16 bytes in a row, as mx_lowrank_kernel loads them. A launch and one or two waits for memory: 4 us for
+// 2048 + 640 columns of rank 16, 5.9 for 1280 + 5120 of rank 64 (9.9 with one load in flight).
 __host__ __device__ __forceinline__ int64_t frag_offset(int c, int r, int P) {
   return ((((int64_t)(c >> 7) * 4 + ((c >> 3) & 3)) * (P >> 4) + (r >> 4)) * 64 + ((c >> 5) & 3) * 16 + (r & 15)) * 8 + (c & 7);
 }

@@ -61,7 +61,7 @@ struct Kept {
   Kept(int64_t M, int64_t K, int64_t N, int64_t P, bool x, bool down, bool factors) {
     scales = x ? up(M * K) : 0;
     t = scales + (x ? up(units(M, K) * 64) : 0);
-    ap = t + (down ? up(2 * M * P) : 0);
+    ap = t + (down ? up(4 * M * P) : 0);   // (t: two parts)
     bp = ap + (factors ? up(2 * K * P) : 0);
     total = bp + (factors ? up(2 * P * padded(N)) : 0);
   }
@@ -85,7 +85,7 @@ Tensor forward(const Tensor& x0, const Tensor& codes, const Tensor& scales, cons
   const Kept k(M, K, N, P, w.A, w.B || w.b, P && w.any());
   // scratch: the codes, and what is not kept of scales and t; the forward pass's order of the factors where they come in theirs
   const int64_t s_scales = up(units(M, K) * 1024), s_t = s_scales + (w.A ? 0 : up(units(M, K) * 64));
-  const int64_t s_at = s_t + (w.B || w.b ? 0 : up(2 * M * P)), s_bt = s_at + (P && !laid_out ? up(2 * P * padded(K)) : 0);
+  const int64_t s_at = s_t + (w.B || w.b ? 0 : up(4 * M * P)), s_bt = s_at + (P && !laid_out ? up(2 * P * padded(K)) : 0);
   const int64_t s_ws = s_bt + (P && !laid_out ? up(2 * N * P) : 0), ws = P && M ? pq_mx_lowrank_workspace_size(M, K, P) : 0;
   const Tensor scratch = bytes(s_ws + ws, x);
   if (w.any()) kept = bytes(k.total, x);
@@ -107,7 +107,8 @@ Tensor forward(const Tensor& x0, const Tensor& codes, const Tensor& scales, cons
   }
   check(pq_mx_linear(x.const_data_ptr(), code_of(x), M, K, stride_of(x), data<uint8_t>(codes), data<uint8_t>(scales),
                      data<float>(bias), at, bt, P, y.data_ptr(), N, N, s, w.A ? h + k.scales : s + s_scales,
-                     w.A ? reinterpret_cast<int8_t*>(h + k.q8) : nullptr, P ? (w.B || w.b ? h + k.t : s + s_t) : nullptr, ws ? s + s_ws : nullptr, ws, stream),
+                     w.A ? reinterpret_cast<int8_t*>(h + k.q8) : nullptr, P ? (w.B || w.b ? h + k.t : s + s_t) : nullptr,
+                     ws ? s + s_ws : nullptr, ws, stream),
         "mxfp4 layer");
   return y;
 }
@@ -157,7 +158,7 @@ struct Layer : torch::autograd::Function<Layer> {
       if (w.B) out[2] = at::empty({R, N}, opt);
       if (w.b) out[3] = at::empty({N}, opt.dtype(at::kFloat));
       const bool sums = w.A || w.B || w.b, need_dt = P && (w.x || w.A);
-      const int64_t s_dt = need_dt ? up(2 * M * P) : 0;
+      const int64_t s_dt = need_dt ? up(4 * M * P) : 0;
       const int64_t ws_sums = sums ? pq_mx_grad_factors_workspace_size(M, K, N, P) : 0;
       const int64_t ws_dx = w.x ? pq_mx_grad_input_workspace_size(M, N, K) : 0;
       const int64_t ws_dt = need_dt ? pq_mx_lowrank_workspace_size(M, N, P) : 0;

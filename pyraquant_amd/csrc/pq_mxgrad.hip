@@ -1,7 +1,8 @@
 // Gradients of a layer over frozen microscaled 4-bit weights (pq_mx.h) with a low-rank branch:
 //   y  = xh wh^T + t B + b,  t = x A
 //   dt = dy B^T,  dB = t^T dy,  db = sum_m dy,  dA = xt^T dt,  dx = dy wh + dt A^T
-// xt: the values of the 8-bit codes the forward pass kept of x. The rounding of x to 4 bits counts as the identity.
+// xt: the values of the 8-bit codes the forward pass kept of x. The rounding of x to 4 bits counts as the identity. All sums in
+// fp32. t and dt are operands of 16-bit matrix instructions, in two parts (two_parts): dA and dB take both, dx the first of dt.
 #include "pq_mx.h"
 
 #include <algorithm>
@@ -48,6 +49,7 @@ struct DxArgs {
 // the 4-bit weights of the next two steps are on their way into registers while the products of this one run, then go to the
 // other of two LDS buffers, the weights widened to 16 bits on the way; they are read back by columns. One barrier a step.
 // SPLIT: blockIdx.z takes a slice of n and leaves its sums in fp32 in p.part [slices][M][K] for mx_dx_join_kernel.
+// Bound by the steps' latency, one workgroup to a compute unit or less: 154 x 2048 x 640 9 us, 1000 x 1312 x 1040 13.
 template <int DT, int R, bool SPLIT>
 __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
   constexpr int BM = 64, A = BM * 128, W = 64 * 256, LA = BM / 32, TJ = BM / 64;   // 16-byte loads of dy a thread; m tiles of a wave
@@ -152,7 +154,8 @@ __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
     }
 }
 
-// dx from the slices' sums, added in order, and the low-rank term. A wave takes 32 rows x 32 columns.
+// dx from the slices' sums, added in order, and the low-rank term. A wave takes 32 rows x 32 columns. Bound by reading the sums:
+// five slices of 2050 x 1280 (52 MB) and rank 64 in 15 us.
 template <int DT, int R>
 __global__ __launch_bounds__(256) void mx_dx_join_kernel(const DxArgs p, int slices) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, half = lane >> 5;
@@ -197,7 +200,9 @@ __global__ __launch_bounds__(256) void mx_dx_join_kernel(const DxArgs p, int sli
 // In its memory phase of step s a wave issues half of dy stage s / 2 + 2 and its part of codes s + 5. Slot 2 s reads dy step s
 // and codes s + 2, all issued by phase s - 3; the barrier before it has every wave wait for all but its two younger phases.
 // LDS, per step: fragments 8 waves x 12 KB, dy 16 KB in, weights 16 KB in: as many cycles as the products take (bf16 products
-// of 32 x 32 x 16 at 32 cycles, 128 bytes of LDS a cycle), so the kernel is bound by both at once, and by the power limit.
+// of 32 x 32 x 16 at 32 cycles, 128 bytes of LDS a cycle), so the kernel is bound by both at once, and by the power limit:
+// 16384 x 3072 x 12288 in 1003 us, 1.24 PFLOP/s (a library's product of the weight in bf16: 1.36-1.38); 4352 x 3072 x 3072, 204
+// blocks on 256 compute units, in 77.5 us, 1.06. Moving the loads or the reads of codes between the products cost 10 %.
 struct DxTile {
   // (64 bytes after each KB of codes: the 128 values that two of them hold of a row are read together)
   static constexpr int DY = 256 * 128, BLOCK = 1024 + 64, CODES = 4 * BLOCK + 1024, W = 32 * 512;
@@ -454,9 +459,10 @@ void mx_dx_ring_kernel(const DxArgs p) {
 }
 
 // ---- sums over rows: part[s][r][c] = sum over the rows of slice s of v[m, r] z[m, c] -------------------------------------
-// z is dy (EIGHT false) or the 8-bit codes of x with their scales; v is t or dt, [M, R]. Column sums of z too (COLS). A
+// z is dy (EIGHT false) or the 8-bit codes of x with their scales; v is t or dt, the sum of its two parts [2, M, R]. Column sums of z too (COLS). A
 // workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step, the next step's rows on their way into
-// registers meanwhile; the order of the sums is fixed. Bound by reading z: 460 MB of 16384 x 3072 x 12288 in 98 us, 4.7 TB/s.
+// registers meanwhile; the order of the sums is fixed. Bound by reading z: 460 MB of 16384 x 3072 x 12288 in 92 us, 5.0 TB/s
+// (87 with the first part of v alone; results' errors then grow by 1.4).
 struct SumArgs {
   const void* z;
   const uint8_t* scales;
@@ -474,11 +480,12 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
   const int c0 = panel * 128, s0 = slice * p.rows;
   const int end = min(p.M, s0 + p.rows);
   auto z_at = [&](int row, int chunk) { return sz + row * 256 + ((chunk ^ spread(row)) << 4); };
-  auto v_at = [&](int row, int chunk) { return sv + row * R * 2 + (chunk << 4); };
+  auto hi_at = [&](int row, int chunk) { return sv + row * R * 2 + (chunk << 4); };
+  auto lo_at = [&](int row, int chunk) { return sv + (64 + row) * R * 2 + (chunk << 4); };
   const uint32_t one2 = DT == PQ_BF16 ? 0x3f803f80u : 0x3c003c00u;
   const v4i ones = {(int)one2, (int)one2, (int)one2, (int)one2};
   v16f acc[R / 32] = {}, cols = {};
-  v4u zr[EIGHT ? 2 : 4], vr[R / 32];
+  v4u zr[EIGHT ? 2 : 4], vr[R / 16];   // v: 64 rows of the first part, then of the second
   int byte = 0;
   auto load = [&](int m0) {
     if constexpr (EIGHT) {
@@ -500,10 +507,10 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
       }
     }
 #pragma unroll
-    for (int i = 0; i < R / 32; ++i) {
-      const int at = i * 256 + tid, m = m0 + at / (R / 8);
+    for (int i = 0; i < R / 16; ++i) {
+      const int at = i % (R / 32) * 256 + tid, m = m0 + at / (R / 8);
       vr[i] = v4u{0, 0, 0, 0};
-      if (m < end) vr[i] = *reinterpret_cast<const v4u*>(p.v + (int64_t)m * R + at % (R / 8) * 8);
+      if (m < end) vr[i] = *reinterpret_cast<const v4u*>(p.v + ((int64_t)(i / (R / 32)) * p.M + m) * R + at % (R / 8) * 8);
     }
   };
   load(s0);
@@ -522,17 +529,17 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
       for (int i = 0; i < 4; ++i) *reinterpret_cast<v4u*>(z_at(i * 16 + (tid >> 4), tid & 15)) = zr[i];
     }
 #pragma unroll
-    for (int i = 0; i < R / 32; ++i) {
-      const int at = i * 256 + tid;
-      *reinterpret_cast<v4u*>(v_at(at / (R / 8), at % (R / 8))) = vr[i];
-    }
+    for (int i = 0; i < R / 16; ++i) *reinterpret_cast<v4u*>(sv + (i * 256 + tid) * 16) = vr[i];
     __syncthreads();
     if (m0 + 64 < end) load(m0 + 64);   // in flight while this step's products run
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const v4i z = read_columns(z_at, 16 * s, wave * 32, lane);
 #pragma unroll
-      for (int j = 0; j < R / 32; ++j) acc[j] = mfma16<DT>(z, read_columns(v_at, 16 * s, 32 * j, lane), acc[j]);
+      for (int j = 0; j < R / 32; ++j) {
+        acc[j] = mfma16<DT>(z, read_columns(hi_at, 16 * s, 32 * j, lane), acc[j]);
+        acc[j] = mfma16<DT>(z, read_columns(lo_at, 16 * s, 32 * j, lane), acc[j]);
+      }
       if constexpr (COLS) cols = mfma16<DT>(z, ones, cols);
     }
   }
@@ -556,7 +563,7 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
 template <int DT, int R, bool COLS>
 __global__ __launch_bounds__(256) void mx_rowsum_kernel(const SumArgs b, const SumArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t sz[64 * 256];      // [m][128 c]
-  __shared__ __attribute__((aligned(16))) uint8_t sv[64 * R * 2];    // [m][R]
+  __shared__ __attribute__((aligned(16))) uint8_t sv[2 * 64 * R * 2];   // [2][m][R]
   if ((int)blockIdx.x < b.blocks) row_sums<DT, R, false, COLS>(b, blockIdx.x, sz, sv);
   else row_sums<DT, R, true, false>(a, blockIdx.x - b.blocks, sz, sv);
 }
@@ -679,7 +686,7 @@ int launch_dx(DxArgs p, int dtype, int r, hipStream_t stream) {
 }
 
 // Row slices of mx_rowsum_kernel: about 384 workgroups a sum. More only add sums to write and join; fewer read too little at once.
-// us of both launches, for 256 / 384 / 512 / 1024 workgroups (bf16): 2050 x 1280 x 5120 rank 64 19.0 / 19.6 / 20.9 / 25.2,
+// us of both launches, for 256 / 384 / 512 / 1024 workgroups (bf16, one part of v): 2050 x 1280 x 5120 rank 64 19.0 / 19.6 / 20.9 / 25.2,
 // 4352 x 3072 x 3072 rank 32 17.1 / 17.3 / 21.4 / 26.1, 16384 x 3072 x 12288 116 / 104 / 103 / 105.
 int row_slices(int64_t M, int64_t C) {
   const int64_t panels = (C + 127) / 128, steps = (M + 63) / 64;

@@ -170,13 +170,15 @@ def mxfp4_grad_input(dy: torch.Tensor, wq: Mxfp4Matrix, dt: Optional[torch.Tenso
 def lowrank_grads(dy: Optional[torch.Tensor], t: Optional[torch.Tensor], dt: Optional[torch.Tensor], q8: Optional[torch.Tensor],
                   x_scales: Optional[torch.Tensor], rank: int, want_A: bool = True, want_B: bool = True, want_bias: bool = True):
     """(dA [K, rank], dB [rank, N], dbias [N] fp32), None for those not wanted: dB = t^T dy, dbias = sum of dy's rows, dA =
-    checkpoint^T dt. t and dt are [M, P], P 32 or 64 >= rank, zero past rank; q8 and x_scales as quant_mxfp4 gave them. What no
-    wanted gradient needs may be None."""
+    checkpoint^T dt. t and dt are [2, M, P], P 32 or 64 >= rank, zero past rank, each the sum of its two parts (the value in 16
+    bits, and what that rounding left out); q8 and x_scales as quant_mxfp4 gave them. What no wanted gradient needs may be
+    None."""
     if not (want_A or want_B or want_bias):
         return None, None, None
     ref = dt if want_A else t
     _check_cuda(dy, t, dt, q8, x_scales)
-    M, P = ref.shape
+    assert ref.dim() == 3 and ref.shape[0] == 2, tuple(ref.shape)
+    _, M, P = ref.shape
     dt16, dev = ref.dtype, ref.device
     code = _dtype16(dt16)
     K = N = BLOCK
@@ -185,7 +187,7 @@ def lowrank_grads(dy: Optional[torch.Tensor], t: Optional[torch.Tensor], dt: Opt
         K = q8.shape[1]
         assert x_scales.dtype == torch.uint8 and x_scales.numel() >= _stages(M, K) * 64
     if want_B or want_bias:
-        assert dy.dim() == 2 and dy.shape[0] == M and dy.dtype == dt16 and tuple(t.shape) == (M, P) and t.is_contiguous()
+        assert dy.dim() == 2 and dy.shape[0] == M and dy.dtype == dt16 and tuple(t.shape) == (2, M, P) and t.is_contiguous()
         dy = _rows(dy)
         N = dy.shape[1]
     assert 1 <= rank <= P, (rank, P)

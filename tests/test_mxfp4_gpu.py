@@ -205,6 +205,25 @@ def test_layer_gradients(cuda, dtype, M, K, N, R):
         _inside(g, r[k], bound[k], k)
 
 
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("M,K,N,R", [(40, 64, 96, 8), (515, 288, 208, 33), (1100, 160, 2064, 32), (64, 4224, 2176, 64)])
+def test_factor_gradients_lose_nothing_in_between(cuda, dtype, M, K, N, R):
+    """dA and dB are sums of products with t and dt, which the kernels hold in two 16-bit parts: u^2 of each may be missing, not
+    u. (Sums of mixed signs: most results are far smaller than their terms, and a rounding of t or dt to 16 bits shows.)"""
+    layer, w, (A, B), bias = _layer(K, N, R, True, dtype, K + N, trainable=True)
+    x, dy = _x(M, K, dtype, M + K), (torch.randn(M, N, generator=_gen(M)) * 0.5).to(dtype)
+    got, r, (u, f) = _grads(layer, x, dy), ref.step(x, w, A, B, bias, dy), (U[dtype], 2.0 ** -23)
+    small = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    Ad, Bd, xd, dyd, xt = A.double(), B.double(), x.double(), dy.double(), ref.eight_bits(x).abs()
+    t_sum, dt_sum = K * f * (xd.abs() @ Ad.abs()), N * f * (dyd.abs() @ Bd.abs().t())
+    t_off = t_sum + u * u * ((xd @ Ad).abs() + t_sum) + small
+    dt_off = dt_sum + u * u * ((dyd @ Bd.t()).abs() + dt_sum) + small
+    a = xt.t() @ dt_off + 2 * M * f * (xt.t() @ ((dyd @ Bd.t()).abs() + dt_off))
+    b = t_off.t() @ dyd.abs() + 2 * M * f * (((xd @ Ad).abs() + t_off).t() @ dyd.abs())
+    _inside(got["dA"], r["dA"], a + u * (r["dA"].abs() + a) + small, "dA")
+    _inside(got["dB"], r["dB"], b + u * (r["dB"].abs() + b) + small, "dB")
+
+
 @pytest.mark.parametrize("M", (4128, 33000))
 def test_many_rows_through_the_low_rank_branch(cuda, M):
     """The quantizer that also takes x lr_A, with more rows a workgroup: codes and checkpoint through y and dA."""
