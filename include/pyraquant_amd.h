@@ -407,8 +407,8 @@ int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, cons
 /*
  * A layer in one call: pq_mx_quant of x into codes and scales (and q8 unless NULL), t = x lr_A into t [2, M, R] where R is 32
  * or 64 (0: no low-rank branch; l1f: lr_A in fragment order, l2t: lr_B's rows [N, R], both from pq_mx_factors), and pq_mx_gemm into
- * y [M, N] (row stride ldy). The caller's codes, scales, q8 and t have the sizes given above and may hold anything; up to 32 rows
- * without q8 are quantized inside the product, which leaves codes and scales alone. 16-byte aligned operands, ldx and ldy (<=
+ * y [M, N] (row stride ldy). The caller's codes, scales, q8 and t have the sizes given above and may hold anything; few short
+ * rows (M <= 32, K <= 2048, M K <= 32768) without q8 are quantized inside the product, which leaves codes and scales alone. 16-byte aligned operands, ldx and ldy (<=
  * 2^21) multiples of 8. With a low-rank branch, a workspace of pq_mx_lowrank_workspace_size(M, K, R) bytes (0 but for few long
  * rows) that may hold anything.
  */

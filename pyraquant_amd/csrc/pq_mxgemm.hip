@@ -519,7 +519,7 @@ int launch_large(GemmArgs p, int r, int cus, hipStream_t stream) {
 // TJ and its waves every NW-th stage of K, each with all of the block's sums; fragments come from memory into registers, D
 // stages ahead, and the waves' sums are added in LDS in a fixed order. QUANT: x is 16-bit, and each lane quantizes the very
 // blocks its fragments are (32 consecutive values of a row), so few rows need no quantizer of their own before the product.
-// Bound by the latency of a launch and of a wave's first loads: 154 x 2048 x 1280 4.2 us; 1 x 12288 x 3072 8.7 us for 20 MB.
+// Bound by the latency of a launch and of a wave's first loads: 154 x 2048 x 1280 4.2 us; 1 x 12288 x 3072 7 us for 20 MB.
 struct SplitArgs {
   GemmArgs g;
   const uint16_t* x;   // QUANT
@@ -691,8 +691,10 @@ int launch_gemm(const GemmArgs& p, int dtype, int r, hipStream_t stream) {
   return launch_ring<2, 1, 2, 4, 2, 1>(p, dtype, r, stream);
 }
 
-// Rows that the product's own lanes quantize: a block's lanes hold 32 rows, so each row is quantized once per 32 outputs.
-constexpr int kQuantRows = 32;
+// Few short rows are quantized by the product's own lanes, once per 32 outputs: a launch less. us on the GPU (bf16), quantizer and
+// product / the product alone: 1 x 1280 x 1280 5.2 / 4.3, 8 x 1536 x 1536 5.4 / 4.9, 32 x 640 x 640 5.2 / 4.2, 8 x 2048 x 1280
+// 5.7 / 5.7 (and 7.6 / 5.9 where the launches bind), but 32 x 2048 x 1280 5.9 / 7.2, 1 x 12288 x 3072 10.2 / 17.4.
+inline bool quantized_inside(int64_t M, int64_t K) { return M <= 32 && K <= 2048 && M * K <= 32768; }
 
 }  // namespace
 }  // namespace mx
@@ -742,7 +744,7 @@ extern "C" int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, 
   const int64_t need = R ? mx::lowrank_workspace(M, K, R) : 0;
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return set_error(PQ_EINVAL, "pq_mx_linear: a workspace of %lld bytes, 16-byte aligned", (long long)need);
-  const bool inside = M <= mx::kQuantRows && !q8;   // the product quantizes the rows itself
+  const bool inside = mx::quantized_inside(M, K) && !q8;   // the product quantizes the rows itself
   if (R) {
     if (const int st = mx::lowrank(x, dtype, M, K, ldx, l1f, R, inside ? nullptr : codes, scales, q8, t, workspace, stream))
       return st;

@@ -607,18 +607,18 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const JoinArgs b, const Jo
 // 128 block, more where a compute unit holds more than one; 4 for a launch; 1.2 for 10^6 values of the slices' sums (fp32,
 // written and read again). Measured (bf16, rank 32, * the plan's):
 //   M x K x N            256 x 256, slices: 1  2      4      5      8   64 x 128: 1      2      4      8
-//   16384 x 3072 x 12288     1100*  1243   1368   1426   1663      1756   1945   2056   2335
-//   4352 x 3072 x 3072       89.9*   131    174    187    277       138    164    192    303
-//   2050 x 5120 x 1280       43.0*  80.2   98.1    117    163      53.1   79.8   99.6    168
-//   2050 x 1280 x 5120        132   84.0   58.0   55.2*  75.9      68.8   63.0   68.0   78.5
-//   1024 x 3072 x 12288       305    166    103   96.5*   123       151    131    134    145
-//   1024 x 3072 x 3072       80.3   61.1   47.6   47.6   66.3      42.8*  45.1   51.0   65.5
-//   512 x 3072 x 12288        303    163   93.8   80.8   65.7*      124   92.8   76.0   79.5
-//   512 x 12288 x 3072       81.3   68.4*  85.7   86.1    109      64.1   83.0   93.5    119
-//   3000 x 2048 x 2048       59.6   55.4   72.3   75.9   97.4      47.3*  65.4   77.5    102
-//   1000 x 1312 x 1040       30.9   34.7   31.8   30.9   30.5      13.2*  20.4   22.3   26.4
-//   154 x 2048 x 640         21.2   19.7   19.4   18.5   18.4       8.9*   9.5    9.5    9.6
-//   64 x 3072 x 3072         73.9   43.8   28.5   26.4   23.1      29.8   21.0   14.8   13.5*
+//   16384 x 3072 x 12288      999*  1139   1256   1339   1578      1698   1882   2000   2303
+//   4352 x 3072 x 3072       77.2*   122    166    182    272       130    156    187    306
+//   2050 x 5120 x 1280       36.4*  76.1   96.2    114              50.2   75.9   97.5
+//   2050 x 1280 x 5120        112   73.6   54.1   51.1*  72.5      68.9   60.3   66.4   76.6
+//   1024 x 3072 x 12288       254    146   93.0   87.6*   114       151    125    129    139
+//   1024 x 3072 x 3072       70.6   54.2   44.7   44.5   64.1      42.2*  43.3   50.4   62.5
+//   512 x 3072 x 12288        254    142   83.4   73.3   58.8*      124   90.2   69.2   75.4
+//   512 x 12288 x 3072       71.2   61.7*  81.1   82.2    106      60.4   77.2   89.3    118
+//   3000 x 2048 x 2048       50.8   50.7   69.5   72.5   95.3      44.6*  59.4   72.5   97.4
+//   1000 x 1312 x 1040       29.0   33.2   30.7   30.0             13.2*  20.3   22.2
+//   154 x 2048 x 640         20.1   18.9   18.3   18.1              9.0*   9.6    9.6
+//   64 x 3072 x 3072         67.8   40.1   26.7   25.2   22.3      29.7   21.0   14.9   13.4*
 struct DxPlan {
   bool ring;
   int slices, slice;
