@@ -5,7 +5,7 @@
 // 64 values of k a step, one scale byte per lane and operand) and sum in fp32. The row operand is a weight row n and the
 // column operand an activation row m, so each lane holds 4 consecutive n of one output row.
 //
-// Large products are bound by the matrix units at the power limit (62 % busy at 1.5 GHz; from registers alone the same
+// Large products are bound by the matrix units at the power limit (52-62 % busy at 1.7-1.5 GHz; from registers alone the same
 // instructions reach 6.5 PFLOP/s): 16384 x 12288 x 12288 in 1170 us, 4.2 PFLOP/s, 65536 x 3072 x 12288 in 1387 us, 3.6. With a
 // short K the output's bytes bind (8202 x 640 x 5120: 33 us, 84 MB out), with few rows the start of a launch and LDS.
 #include "pq_mx.h"
