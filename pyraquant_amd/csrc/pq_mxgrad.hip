@@ -603,8 +603,9 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const JoinArgs b, const Jo
 }
 
 // How dx is computed: in blocks of 256 x 256 (m x k) or 64 x 128, with n cut into `slices` where that ends sooner, by an
-// estimate in us: 1.6 for 64 n of a 256 x 256 block (one to a compute unit) and 9 for its start and end; 0.62 for 64 n of a 64 x
-// 128 block, more where a compute unit holds more than one; 4 for a launch; 1.2 for 10^6 values of the slices' sums (fp32,
+// estimate in us. A 256 x 256 block, one to a compute unit: 9 for its start and end, and for 64 n 1.25 alone to 1.7 with all 256 at
+// work (the clock falls with the power they draw). A 64 x 128 block: 0.62 for 64 n, more where a compute unit holds more than
+// one, 1 for the end of each past the third, and 4 for the launch. Slices: 4 for another launch; 1.2 for 10^6 values of their sums (fp32,
 // written and read again). Measured (bf16, rank 32, * the plan's):
 //   M x K x N            256 x 256, slices: 1  2      4      5      8   64 x 128: 1      2      4      8
 //   16384 x 3072 x 12288      999*  1139   1256   1339   1578      1698   1882   2000   2303
@@ -615,6 +616,9 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const JoinArgs b, const Jo
 //   1024 x 3072 x 3072       70.6   54.2   44.7   44.5   64.1      42.2*  43.3   50.4   62.5
 //   512 x 3072 x 12288        254    142   83.4   73.3   58.8*      124   90.2   69.2   75.4
 //   512 x 12288 x 3072       71.2   61.7*  81.1   82.2    106      60.4   77.2   89.3    118
+//   5150 x 9248 x 416        70.7*   260    415                    92.4    264    428
+//   11734 x 608 x 1680       44.6*  71.5          84.7             51.6   72.8   86.5
+//   13664 x 1344 x 4704       217*   241    302    328    419       282    338    394    508
 //   3000 x 2048 x 2048       50.8   50.7   69.5   72.5   95.3      44.6*  59.4   72.5   97.4
 //   1000 x 1312 x 1040       29.0   33.2   30.7   30.0             13.2*  20.3   22.2
 //   154 x 2048 x 640         20.1   18.9   18.3   18.1              9.0*   9.6    9.6
@@ -626,14 +630,18 @@ struct DxPlan {
 DxPlan dx_plan(int64_t M, int64_t N, int64_t K) {
   const int64_t large = ((M + 255) / 256) * ((K + 255) / 256), small = ((M + 63) / 64) * stages(K);
   const int steps = (int)((N + 63) / 64);
+  auto rounds = [](int64_t blocks, int per) {   // of 256 blocks, and of those left
+    auto round = [&](double fill) { return per * (1.25 + 0.45 * fill * fill * fill) + 9; };
+    return (double)(blocks / 256) * round(1.0) + (blocks % 256 ? round((double)(blocks % 256) / 256) : 0.0);
+  };
   DxPlan best{true, 1, 0};
   double least = 0;
   for (int ring = 1; ring >= 0; --ring)
     for (int s = 1; s <= 8 && s <= steps; ++s) {
       const int per = (steps + s - 1) / s;
       if ((s - 1) * per >= steps) continue;   // (no empty slice)
-      const double sharing = std::max(1.0, 0.45 + 0.58 / 256 * (double)(small * s));
-      double t = ring ? (double)((large * s + 255) / 256) * (per * 1.6 + 9) : per * 0.62 * sharing + 4;
+      const double each = (double)(small * s) / 256;   // 64 x 128 blocks a compute unit
+      double t = ring ? rounds(large * s, per) : per * 0.62 * std::max(1.0, 0.45 + 0.58 * each) + 4 + std::max(0.0, each - 3);
       if (s > 1) t += 4 + s * (double)(M * K) * 1.2e-6;
       if ((ring && s == 1) || t < least) least = t, best = {ring == 1, s, s > 1 ? per * 64 : 0};
     }
