@@ -45,7 +45,7 @@
 extern "C" {
 #endif
 
-#define PQ_ABI_VERSION 3
+#define PQ_ABI_VERSION 4
 
 /* status codes */
 #define PQ_OK 0
@@ -398,23 +398,25 @@ int pq_mx_values(const void* codes, const uint8_t* scales, int32_t bits, int64_t
 /*
  * y[m, n] = sum_k xh[m, k] wh[n, k] (+ sum_r t[m, r] l2t[n, r]) (+ bias[n]), summed in fp32, rounded once to dtype (PQ_BF16 or
  * PQ_F16). a, w: packed 4-bit matrices [M, K] and [N, K]. t [M, R] (row stride ldt) and l2t [N, R] of dtype, R in {32, 64}, or
- * NULL. K % 32 == 0, N % 16 == 0, M <= 2^30; operands 16-byte aligned, ldc (<= 2^21) and ldt multiples of 8.
+ * NULL. K % 32 == 0, N % 16 == 0, M <= 2^30; operands 16-byte aligned, ldc (<= 2^21) and ldt multiples of 8. With dtype |
+ * PQ_MX_T32 t is fp32, as pq_mx_lowrank_down gives it (ldt a multiple of 4), and taken to twice dtype's bits.
  */
+#define PQ_MX_T32 0x200
 int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales, const float* bias,
                const void* t, int64_t ldt, const void* l2t, int64_t R, void* c, int64_t ldc, int32_t dtype, int64_t M, int64_t N,
                int64_t K, hipStream_t stream);
 
 /*
- * A layer in one call: pq_mx_quant of x into codes and scales (and q8 unless NULL), t = x lr_A into t [2, M, R] where R is 32
- * or 64 (0: no low-rank branch; l1f: lr_A in fragment order, l2t: lr_B's rows [N, R], both from pq_mx_factors), and pq_mx_gemm into
- * y [M, N] (row stride ldy). The caller's codes, scales, q8 and t have the sizes given above and may hold anything; few short
- * rows (M <= 32, K <= 2048, M K <= 32768) without q8 are quantized inside the product, which leaves codes and scales alone. 16-byte aligned operands, ldx and ldy (<=
- * 2^21) multiples of 8. With a low-rank branch, a workspace of pq_mx_lowrank_workspace_size(M, K, R) bytes (0 but for few long
+ * A layer in one call: pq_mx_quant of x into codes and scales (and q8 unless NULL), t = x lr_A into t [M, R] in fp32 where R is
+ * 32 or 64 (0: no low-rank branch; l1f: lr_A in fragment order, l2t: lr_B's rows [N, R], both from pq_mx_factors), and pq_mx_gemm
+ * into y [M, N] (row stride ldy). The caller's codes, scales, q8 and t have the sizes given above and may hold anything; few short
+ * rows (M <= 32, K <= 2048, M K <= 32768) without q8 are quantized inside the product, which leaves codes and scales alone. 16-byte
+ * aligned operands, ldx and ldy (<= 2^21) multiples of 8. With a low-rank branch, a workspace of pq_mx_lowrank_workspace_size(M, K, R) bytes (0 but for few long
  * rows) that may hold anything.
  */
 int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, const uint8_t* w_scales,
                  const float* bias, const void* l1f, const void* l2t, int64_t R, void* y, int64_t ldy, int64_t N, uint8_t* codes,
-                 uint8_t* scales, int8_t* q8, void* t, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+                 uint8_t* scales, int8_t* q8, float* t, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /*
  * The low-rank factors in the orders the layer's kernels read them, zero-padded from rank R to P (32 or 64), 16-bit, from one
@@ -431,19 +433,19 @@ int pq_mx_factors(const void* A, int64_t lda, int32_t a_order, const void* B, in
                   int64_t R, int64_t P, void* af, void* ap, void* bt, void* bf, hipStream_t stream);
 
 /*
- * t[m, r] = sum_k x[m, k] l1[k, r] ([2, M, R] of dtype, R in {32, 64}), l1 in fragment order (pq_mx_factors), summed in fp32 and
- * stored in two parts of dtype (PQ_BF16 or PQ_F16): rounded to it, and what that rounding left out. K % 16 == 0; operands 16-byte aligned, ldx a multiple of 8. A workspace of
- * pq_mx_lowrank_workspace_size bytes (0 but for few long rows) that may hold anything.
+ * t[m, r] = sum_k x[m, k] l1[k, r] ([M, R] in fp32, R in {32, 64}), x of dtype PQ_BF16 or PQ_F16, l1 in fragment order
+ * (pq_mx_factors). K % 16 == 0; operands 16-byte aligned, ldx a multiple of 8. A workspace of pq_mx_lowrank_workspace_size bytes
+ * (0 but for few long rows) that may hold anything.
  */
 int64_t pq_mx_lowrank_workspace_size(int64_t M, int64_t K, int64_t R);
-int pq_mx_lowrank_down(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R, void* t,
+int pq_mx_lowrank_down(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R, float* t,
                        void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /*
  * dx[m, k] = sum_n dy[m, n] wh[n, k] (+ sum_r dt[m, r] ap[k, r]): the gradient of a layer's input over its packed 4-bit weight
  * [N, K], widened to dtype on the way to the matrix instructions (exact; in fp16, for 2^-22 <= 2^E <= 2^13), summed in fp32.
- * dy [M, N], dx [M, K] of dtype; dt [M, R] and ap [K, R] contiguous, R in {32, 64}, or NULL. Operands 16-byte aligned, lddy and
- * lddx multiples of 8, lddy <= 2^21. A workspace of pq_mx_grad_input_workspace_size bytes (0 for most sizes) that may hold
+ * dy [M, N], dx [M, K] of dtype; dt [M, R] and ap [K, R] contiguous, R in {32, 64}, or NULL, dt fp32 with dtype | PQ_MX_T32.
+ * Operands 16-byte aligned, lddy and lddx multiples of 8, lddy <= 2^21. A workspace of pq_mx_grad_input_workspace_size bytes (0 for most sizes) that may hold
  * anything.
  */
 int64_t pq_mx_grad_input_workspace_size(int64_t M, int64_t N, int64_t K);
@@ -455,11 +457,11 @@ int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, const uint8_t*
  * The gradients of the low-rank factors and the bias: dB[r, n] = sum_m t[m, r] dy[m, n] ([R, N]), dA[k, r] = sum_m xt[m, k]
  * dt[m, r] ([K, R], xt: the values of the checkpoint q8 with x_scales), dbias[n] = sum_m dy[m, n] (fp32). An output that is
  * NULL is not computed, and what only it needs (dy and t for dB and dbias; dt, q8 and x_scales for dA) may be NULL too. t and
- * dt are [2, M, P], the two parts of each as pq_mx_lowrank_down gives them, zero past rank R. Sums in fp32, in an order that depends on the sizes alone; dA and dB rounded to dtype. The
- * workspace (pq_mx_grad_factors_workspace_size bytes) may hold anything.
+ * dt are [M, P] in fp32, as pq_mx_lowrank_down gives them, zero past rank R, and taken to twice dtype's bits. Sums in fp32, in an
+ * order that depends on the sizes alone; dA and dB rounded to dtype. The workspace (pq_mx_grad_factors_workspace_size bytes) may hold anything.
  */
 int64_t pq_mx_grad_factors_workspace_size(int64_t M, int64_t K, int64_t N, int64_t P);
-int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, const void* t, const void* dt, const int8_t* q8,
+int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, const float* t, const float* dt, const int8_t* q8,
                        const uint8_t* x_scales, int64_t M, int64_t K, int64_t N, int64_t R, int64_t P, void* dA, void* dB,
                        float* dbias, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 

@@ -15,10 +15,10 @@
 namespace pq {
 namespace mx {
 
-// t = x l1t^T [2, M, R] (two_parts) and, unless codes is NULL, the codes of x (and q8), in one pass (pq_mx.hip). K % 16 == 0 (32 with codes),
-// 16-byte aligned rows, R 32 or 64, l1f: l1t in fragment order (pq_mx_factors); arguments checked by the caller.
+// t = x l1t^T [M, R] in fp32 and, unless codes is NULL, the codes of x (and q8), in one pass (pq_mx.hip). K % 16 == 0 (32 with
+// codes), 16-byte aligned rows, R 32 or 64, l1f: l1t in fragment order (pq_mx_factors); arguments checked by the caller.
 int lowrank(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R, uint8_t* codes,
-            uint8_t* scales, int8_t* q8, void* t, void* workspace, hipStream_t stream);
+            uint8_t* scales, int8_t* q8, float* t, void* workspace, hipStream_t stream);
 int64_t lowrank_workspace(int64_t M, int64_t K, int64_t R);   // bytes of its workspace (0: none)
 
 constexpr int kBlock = 32;     // values that share a scale
@@ -173,20 +173,16 @@ __device__ __forceinline__ float restore_scale(int byte) {
   return byte == kNaN ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(1.0f, byte - 131);
 }
 
-// Four sums as 16-bit values, and what that rounding left out, rounded too (0 where a value is not finite): the two together hold
-// a sum to twice the bits, for sums over many rows (gradients of the factors), where a rounding of t or dt to 16 bits would be
-// as large as the result's own. Terms that are added to a larger sum and rounded with it take the first part alone.
+// t and dt are kept in fp32 and taken as two 16-bit parts by the products that read them: the value rounded, and what that rounding
+// left out, rounded too (0 where the value is not finite). The two together hold it to twice the bits; with the first alone the
+// rounding of t shows in every result, as large as the results' own where the low-rank term is the larger one.
 template <int DT>
-__device__ __forceinline__ void two_parts(v4f s, v2u& hi, v2u& lo) {
-  hi = v2u{pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3])};
-  float r[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t h = e & 1 ? hi[e >> 1] >> 16 : hi[e >> 1] & 0xffff;
-    r[e] = s[e] - (DT == PQ_BF16 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h));
-    if (!(fabsf(r[e]) < INFINITY)) r[e] = 0.0f;
-  }
-  lo = v2u{pack2<DT>(r[0], r[1]), pack2<DT>(r[2], r[3])};
+__device__ __forceinline__ void two_parts(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<DT>(a, b);
+  float r0 = a - lo16_to_f32<DT>(hi), r1 = b - hi16_to_f32<DT>(hi);
+  if (!(fabsf(r0) < INFINITY)) r0 = 0.0f;
+  if (!(fabsf(r1) < INFINITY)) r1 = 0.0f;
+  lo = pack2<DT>(r0, r1);
 }
 
 // ---- shared by the products ------------------------------------------------------------------------------------------
@@ -207,6 +203,41 @@ __device__ __forceinline__ v16f mfma16(v4i a, v4i b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// Eight consecutive ranks of a row of t (or dt), operand of a low-rank product. `load` asks for them, `parts` makes the operands:
+// fp32 values (wide) in two parts, 16-bit values as they are. `wide` is the same for the whole launch.
+struct RankPiece {
+  v4f raw[2];
+  __device__ __forceinline__ void load(const void* t, int64_t at, bool wide) {
+    if (wide) {
+      const v4f* const src = reinterpret_cast<const v4f*>(static_cast<const float*>(t) + at);
+      raw[0] = src[0];
+      raw[1] = src[1];
+    } else {
+      raw[0] = *reinterpret_cast<const v4f*>(static_cast<const uint16_t*>(t) + at);
+    }
+  }
+  template <int DT>
+  __device__ __forceinline__ void parts(v4i& hi, v4i& lo, bool wide) const {
+    hi = __builtin_bit_cast(v4i, raw[0]);
+    lo = v4i{0, 0, 0, 0};
+    if (wide) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t h, l;
+        two_parts<DT>(raw[e >> 1][2 * (e & 1)], raw[e >> 1][2 * (e & 1) + 1], h, l);
+        hi[e] = (int)h;
+        lo[e] = (int)l;
+      }
+    }
+  }
+};
+// y += l t^T over the 16 ranks of a piece
+template <int DT>
+__device__ __forceinline__ v16f rank_product(v4i l, v4i hi, v4i lo, v16f y, bool wide) {
+  if (wide) y = mfma16<DT>(l, lo, y);
+  return mfma16<DT>(l, hi, y);
 }
 
 // Workgroup id -> (tile_m, tile_n): ids are dealt round-robin over the 8 XCDs, so each XCD takes a contiguous run of the

@@ -46,19 +46,18 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(const void* __restrict__ 
   }
 }
 
-// t = x l1t^T ([2, M, R], 16-bit) and, where QUANT, the codes of x, in one pass over x. A workgroup takes 16 RG rows and its NW
+// t = x l1t^T ([M, R], fp32) and, where QUANT, the codes of x, in one pass over x. A workgroup takes 16 RG rows and its NW
 // waves every NW-th stage of 128 values, 16 rows at a time as above: what a lane holds of x for its block is also its operand
 // of the 16 x 16 x 32 products (8 consecutive values of a row; the order of k within the sum is free as long as l1t's operand
 // has the same), so x is read once and needs no other lane or LDS. l1t comes from the cache in fragment order (1 KB a load, zeros
-// past K), once per RG row groups. The waves' sums are added in LDS in a fixed order and stored as two 16-bit parts: what takes t
-// (the product's low-rank term, dB) and dt, made here too (dx, dA), are products of 16-bit operands.
+// past K), once per RG row groups. The waves' sums are added in LDS in a fixed order. dt, of dy, is made here too.
 // Bound by reading x and by l1t from the cache: 65536 x 3072 with codes 101 us (the quantizer alone: 88), dy of 16384 x 12288
 // to dt in 103-110 us, 3.7-3.9 TB/s.
 template <int DT, int R, int RG, int NW, bool QUANT, bool CKPT>
 __global__ __launch_bounds__(64 * NW) void mx_lowrank_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t M, int K, int KT,
                                                              const uint16_t* __restrict__ l1f, uint8_t* __restrict__ codes,
                                                              uint8_t* __restrict__ scales, int8_t* __restrict__ q8,
-                                                             uint16_t* __restrict__ t, float* __restrict__ partial) {
+                                                             float* __restrict__ t) {
   constexpr int C = R / 16;                                  // column tiles of t
   __shared__ float part[NW][RG * C][64 * 4 + 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, b = lane >> 4;
@@ -130,19 +129,13 @@ __global__ __launch_bounds__(64 * NW) void mx_lowrank_kernel(const uint16_t* __r
     }
     const int64_t row = m0 + 16 * (tile / C) + (l & 15);
     if (row >= M) continue;
-    if (partial)
-      *reinterpret_cast<v4f*>(partial + (blockIdx.y * M + row) * R + 16 * (tile % C) + 4 * (l >> 4)) = sum;
-    else {
-      v2u* const out = reinterpret_cast<v2u*>(t + row * R + 16 * (tile % C) + 4 * (l >> 4));
-      two_parts<DT>(sum, out[0], out[M * R / 4]);
-    }
+    *reinterpret_cast<v4f*>(t + (blockIdx.y * M + row) * R + 16 * (tile % C) + 4 * (l >> 4)) = sum;   // (a slice of k each)
   }
 }
 
 // t from the sums of workgroups that share rows (`partial` [slices][M R]), in order; a thread takes four.
-template <int DT>
 __global__ __launch_bounds__(256) void mx_lowrank_join_kernel(const float* __restrict__ partial, int slices, int64_t n,
-                                                              uint16_t* __restrict__ t) {
+                                                              float* __restrict__ t) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
   v4f sum = {};
@@ -151,7 +144,7 @@ __global__ __launch_bounds__(256) void mx_lowrank_join_kernel(const float* __res
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] += v[e];
   }
-  two_parts<DT>(sum, *reinterpret_cast<v2u*>(t + i), *reinterpret_cast<v2u*>(t + n + i));
+  *reinterpret_cast<v4f*>(t + i) = sum;
 }
 
 // Values of the 4-bit codes (EIGHT: of the 8-bit ones), one lane a block. ODT: output type. Bound by the store of 2 or 4 bytes a
@@ -290,14 +283,14 @@ int lowrank_slices(int64_t M, int64_t K) {
 
 template <int DT, int R, int RG, int NW>
 int launch_lowrank(const uint16_t* x, int64_t M, int64_t K, int64_t ldx, const uint16_t* l1f, uint8_t* codes, uint8_t* scales,
-                   int8_t* q8, uint16_t* t, float* partial, int slices, hipStream_t stream) {
+                   int8_t* q8, float* t, int slices, hipStream_t stream) {
   const int64_t blocks = (M + 16 * RG - 1) / (16 * RG);
   if (const int st = check_grid(blocks, 64 * NW, "mx_lowrank")) return st;
   const dim3 grid((unsigned)blocks, (unsigned)slices), block(64 * NW);
   const int KT = stages(K);
 #define PQ_MXL(Q, C) \
   hipLaunchKernelGGL((mx_lowrank_kernel<DT, R, RG, NW, Q, C>), grid, block, 0, stream, x, ldx, M, (int)K, KT, l1f, codes, scales, q8, \
-                     t, partial)
+                     t)
   if (!codes) PQ_MXL(false, false); else if (q8) PQ_MXL(true, true); else PQ_MXL(true, false);
 #undef PQ_MXL
   return check_launch("mx_lowrank");
@@ -323,14 +316,14 @@ int64_t pq::mx::lowrank_workspace(int64_t M, int64_t K, int64_t R) {
 //   4096 x 3072             9.9              11.7              22.8             20.4
 //   2050 x 1280             5.4               6.2              11.8             11.6
 int pq::mx::lowrank(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R, uint8_t* codes,
-                    uint8_t* scales, int8_t* q8, void* t, void* workspace, hipStream_t stream) {
+                    uint8_t* scales, int8_t* q8, float* t, void* workspace, hipStream_t stream) {
   const int slices = lowrank_slices(M, K);
   float* const partial = slices > 1 ? static_cast<float*>(workspace) : nullptr;
   auto launch = [&](auto rg, auto nw) {
     constexpr int RG = decltype(rg)::value, NW = decltype(nw)::value;
 #define PQ_MXL(D, RR)                                                                                               \
   launch_lowrank<D, RR, RG, NW>(static_cast<const uint16_t*>(x), M, K, ldx, static_cast<const uint16_t*>(l1f), codes, scales, q8, \
-                                static_cast<uint16_t*>(t), partial, slices, stream)
+                                partial ? partial : t, slices, stream)
     if (dtype == PQ_BF16) return R == 32 ? PQ_MXL(PQ_BF16, 32) : PQ_MXL(PQ_BF16, 64);
     return R == 32 ? PQ_MXL(PQ_F16, 32) : PQ_MXL(PQ_F16, 64);
 #undef PQ_MXL
@@ -342,10 +335,7 @@ int pq::mx::lowrank(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t 
   if (st || !partial) return st;
   const int64_t n = M * R;
   const dim3 grid((unsigned)((n / 4 + 255) / 256)), block(256);
-  if (dtype == PQ_BF16)
-    hipLaunchKernelGGL((mx_lowrank_join_kernel<PQ_BF16>), grid, block, 0, stream, partial, slices, n, static_cast<uint16_t*>(t));
-  else
-    hipLaunchKernelGGL((mx_lowrank_join_kernel<PQ_F16>), grid, block, 0, stream, partial, slices, n, static_cast<uint16_t*>(t));
+  hipLaunchKernelGGL(mx_lowrank_join_kernel, grid, block, 0, stream, partial, slices, n, t);
   return check_launch("mx_lowrank_join");
 }
 
@@ -421,7 +411,7 @@ extern "C" int64_t pq_mx_lowrank_workspace_size(int64_t M, int64_t K, int64_t R)
 }
 
 extern "C" int pq_mx_lowrank_down(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R,
-                                  void* t, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+                                  float* t, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   if (M < 0 || K < 16 || K % 16 || ldx < K || K > (1 << 30) || (R != 32 && R != 64))
     return set_error(PQ_ESHAPE, "pq_mx_lowrank_down: M=%lld K=%lld ldx=%lld R=%lld (K %% 16 == 0, R 32 or 64)", (long long)M,
                      (long long)K, (long long)ldx, (long long)R);

@@ -61,7 +61,7 @@ struct Kept {
   Kept(int64_t M, int64_t K, int64_t N, int64_t P, bool x, bool down, bool factors) {
     scales = x ? up(M * K) : 0;
     t = scales + (x ? up(units(M, K) * 64) : 0);
-    ap = t + (down ? up(4 * M * P) : 0);   // (t: two parts)
+    ap = t + (down ? up(4 * M * P) : 0);   // (t: fp32)
     bp = ap + (factors ? up(2 * K * P) : 0);
     total = bp + (factors ? up(2 * P * padded(N)) : 0);
   }
@@ -107,7 +107,7 @@ Tensor forward(const Tensor& x0, const Tensor& codes, const Tensor& scales, cons
   }
   check(pq_mx_linear(x.const_data_ptr(), code_of(x), M, K, stride_of(x), data<uint8_t>(codes), data<uint8_t>(scales),
                      data<float>(bias), at, bt, P, y.data_ptr(), N, N, s, w.A ? h + k.scales : s + s_scales,
-                     w.A ? reinterpret_cast<int8_t*>(h + k.q8) : nullptr, P ? (w.B || w.b ? h + k.t : s + s_t) : nullptr,
+                     w.A ? reinterpret_cast<int8_t*>(h + k.q8) : nullptr, P ? reinterpret_cast<float*>(w.B || w.b ? h + k.t : s + s_t) : nullptr,
                      ws ? s + s_ws : nullptr, ws, stream),
         "mxfp4 layer");
   return y;
@@ -164,17 +164,18 @@ struct Layer : torch::autograd::Function<Layer> {
       const int64_t ws_dt = need_dt ? pq_mx_lowrank_workspace_size(M, N, P) : 0;
       const Tensor scratch = bytes(s_dt + std::max({ws_sums, ws_dx, ws_dt}), dy);   // (one after the other on the stream)
       uint8_t* const s = data<uint8_t>(scratch);
+      float* const dt = reinterpret_cast<float*>(s);
       if (need_dt)
-        check(pq_mx_lowrank_down(dy.const_data_ptr(), code, M, N, stride_of(dy), h + k.bp, P, s, ws_dt ? s + s_dt : nullptr, ws_dt, stream),
+        check(pq_mx_lowrank_down(dy.const_data_ptr(), code, M, N, stride_of(dy), h + k.bp, P, dt, ws_dt ? s + s_dt : nullptr, ws_dt, stream),
               "mxfp4 dt");
       if (sums)
-        check(pq_mx_grad_factors(dy.const_data_ptr(), code, stride_of(dy), w.B || w.b ? h + k.t : nullptr, s,
+        check(pq_mx_grad_factors(dy.const_data_ptr(), code, stride_of(dy), w.B || w.b ? reinterpret_cast<float*>(h + k.t) : nullptr, dt,
                                  reinterpret_cast<int8_t*>(h + k.q8), h + k.scales, M, K, N, R, P, data<void>(out[1]),
                                  data<void>(out[2]), data<float>(out[3]), s + s_dt, ws_sums, stream),
               "mxfp4 factor gradients");
       if (w.x)
-        check(pq_mx_grad_input(dy.const_data_ptr(), code, stride_of(dy), data<uint8_t>(codes), data<uint8_t>(scales),
-                               P ? s : nullptr, P ? h + k.ap : nullptr, P, out[0].data_ptr(), K, M, N, K,
+        check(pq_mx_grad_input(dy.const_data_ptr(), code | PQ_MX_T32, stride_of(dy), data<uint8_t>(codes), data<uint8_t>(scales),
+                               P ? dt : nullptr, P ? h + k.ap : nullptr, P, out[0].data_ptr(), K, M, N, K,
                                ws_dx ? s + s_dt : nullptr, ws_dx, stream),
               "mxfp4 input gradient");
     } catch (const Refused& r) {

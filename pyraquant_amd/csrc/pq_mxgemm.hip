@@ -20,11 +20,13 @@ namespace {
 struct GemmArgs {
   const uint8_t *a, *as, *w, *ws;   // codes and scales of x and of the weight
   const float* bias;
-  const uint16_t *t, *l2t;
+  const void* t;                    // 16-bit, or fp32 (wide)
+  const uint16_t* l2t;
   uint16_t* c;
   int64_t ldt, ldc;
   int M, N, KT;
   int tiles_m, tiles_n;
+  bool wide;
 };
 
 // One step over 64 values: both operands 4-bit (format code 4), scale byte S of each scale word.
@@ -216,27 +218,28 @@ void mx_gemm_kernel(const GemmArgs p) {
   // go through LDS two weight tiles at a time so that whole 128-byte lines are stored.
   const int nb = n0 + wn * (BN / 2), mb = m0 + wm * (BM / WMW);
   uint8_t* const stage = rings + (KG - 1) * NW * TI * TJ * 4096 + wave * 32 * T::PITCH;
-  v4i tv[R ? R / 16 : 1];
 #pragma unroll
   for (int j = 0; j < TJ; ++j) {
     if constexpr (R > 0) {
 #pragma unroll
-      for (int s = 0; s < R / 16; ++s)
-        tv[s] = *reinterpret_cast<const v4i*>(p.t + (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + 16 * s + 8 * half);
+      for (int s = 0; s < R / 16; ++s) {
+        RankPiece t;
+        v4i hi, lo;
+        t.load(p.t, (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + 16 * s + 8 * half, p.wide);
+        t.parts<DT>(hi, lo, p.wide);
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+          const v4i l = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(nb + 32 * i + l32, p.N - 1) * R + 16 * s + 8 * half);
+          acc[i][j] = rank_product<DT>(l, hi, lo, acc[i][j], p.wide);
+        }
+      }
     }
 #pragma unroll
     for (int ih = 0; ih < TI / 2; ++ih) {
 #pragma unroll
       for (int ii = 0; ii < 2; ++ii) {
         const int i = 2 * ih + ii;
-        v16f y = acc[i][j];
-        if constexpr (R > 0) {
-#pragma unroll
-          for (int s = 0; s < R / 16; ++s) {
-            const v4i l = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(nb + 32 * i + l32, p.N - 1) * R + 16 * s + 8 * half);
-            y = mfma16<DT>(l, tv[s], y);
-          }
-        }
+        const v16f& y = acc[i][j];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int n = nb + 32 * i + 8 * q + 4 * half;
@@ -441,12 +444,13 @@ void mx_gemm_large_kernel(const GemmArgs p) {
     if constexpr (R > 0) {
 #pragma unroll
       for (int r0 = 0; r0 < R; r0 += 32) {
-        v4i tv[TJ][2], lv[TI][2];
+        RankPiece tv[TJ][2];
+        v4i lv[TI][2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
 #pragma unroll
           for (int j = 0; j < TJ; ++j)
-            tv[j][x] = *reinterpret_cast<const v4i*>(p.t + (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + r0 + 16 * x + 8 * half);
+            tv[j][x].load(p.t, (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + r0 + 16 * x + 8 * half, p.wide);
 #pragma unroll
           for (int i = 0; i < TI; ++i)
             lv[i][x] = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(nb + 32 * i + l32, p.N - 1) * R + r0 + 16 * x + 8 * half);
@@ -455,9 +459,12 @@ void mx_gemm_large_kernel(const GemmArgs p) {
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int i = 0; i < TI; ++i)
+          for (int j = 0; j < TJ; ++j) {
+            v4i hi, lo;
+            tv[j][x].template parts<DT>(hi, lo, p.wide);
 #pragma unroll
-            for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16<DT>(lv[i][x], tv[j][x], acc[i][j]);
+            for (int i = 0; i < TI; ++i) acc[i][j] = rank_product<DT>(lv[i][x], hi, lo, acc[i][j], p.wide);
+          }
       }
     } else {
       go_on();
@@ -626,8 +633,11 @@ __global__ __launch_bounds__(64 * NW) void mx_gemm_split_kernel(const SplitArgs 
 #pragma unroll
           for (int s = 0; s < R / 16; ++s) {
             const v4i l = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(n0 + 32 * i + l32, p.N - 1) * R + 16 * s + 8 * half);
-            const v4i t = *reinterpret_cast<const v4i*>(p.t + (int64_t)min(m, p.M - 1) * p.ldt + 16 * s + 8 * half);
-            y = mfma16<DT>(l, t, y);
+            RankPiece t;
+            v4i hi, lo;
+            t.load(p.t, (int64_t)min(m, p.M - 1) * p.ldt + 16 * s + 8 * half, p.wide);
+            t.parts<DT>(hi, lo, p.wide);
+            y = rank_product<DT>(l, hi, lo, y, p.wide);
           }
         }
 #pragma unroll
@@ -705,6 +715,8 @@ using namespace pq;
 extern "C" int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales,
                           const float* bias, const void* t, int64_t ldt, const void* l2t, int64_t R, void* c, int64_t ldc,
                           int32_t dtype, int64_t M, int64_t N, int64_t K, hipStream_t stream) {
+  const bool wide = (dtype & PQ_MX_T32) != 0;
+  dtype &= ~PQ_MX_T32;
   if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || ldc < N || ldc > (1 << 21) || M > (1 << 30) ||
       N > (1 << 30) || K > (1 << 22))
     return set_error(PQ_ESHAPE, "pq_mx_gemm: M=%lld N=%lld K=%lld ldc=%lld (N %% 16 == 0, K %% 32 == 0, ldc <= 2^21)", (long long)M,
@@ -715,16 +727,16 @@ extern "C" int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8
   if (M == 0) return PQ_OK;
   if (!a || !a_scales || !w || !w_scales || !c || (t && !l2t)) return set_error(PQ_EINVAL, "pq_mx_gemm: null pointer");
   if ((uintptr_t)a % 16 || (uintptr_t)w % 16 || (uintptr_t)a_scales % 16 || (uintptr_t)w_scales % 16 || (uintptr_t)c % 16 ||
-      ldc % 8 || (uintptr_t)bias % 16 || (t && ((uintptr_t)t % 16 || (uintptr_t)l2t % 16 || ldt % 8)))
-    return set_error(PQ_EALIGN, "pq_mx_gemm: operands 16-byte aligned, ldc and ldt multiples of 8");
-  mx::GemmArgs p{a, a_scales, w, w_scales, bias, static_cast<const uint16_t*>(t), static_cast<const uint16_t*>(l2t),
-                 static_cast<uint16_t*>(c), ldt, ldc, (int)M, (int)N, mx::stages(K), 0, 0};
+      ldc % 8 || (uintptr_t)bias % 16 || (t && ((uintptr_t)t % 16 || (uintptr_t)l2t % 16 || ldt % (wide ? 4 : 8))))
+    return set_error(PQ_EALIGN, "pq_mx_gemm: operands 16-byte aligned, ldc and ldt multiples of 8 (ldt of an fp32 t: 4)");
+  mx::GemmArgs p{a, a_scales, w, w_scales, bias, t, static_cast<const uint16_t*>(l2t),
+                 static_cast<uint16_t*>(c), ldt, ldc, (int)M, (int)N, mx::stages(K), 0, 0, wide};
   return mx::launch_gemm(p, dtype, t ? (int)R : 0, stream);
 }
 
 extern "C" int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w,
                             const uint8_t* w_scales, const float* bias, const void* l1f, const void* l2t, int64_t R, void* y,
-                            int64_t ldy, int64_t N, uint8_t* codes, uint8_t* scales, int8_t* q8, void* t, void* workspace,
+                            int64_t ldy, int64_t N, uint8_t* codes, uint8_t* scales, int8_t* q8, float* t, void* workspace,
                             int64_t workspace_bytes, hipStream_t stream) {
   if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || ldx < K || ldy < N || ldy > (1 << 21) || M > (1 << 30) ||
       N > (1 << 30) || K > (1 << 22))
@@ -739,8 +751,8 @@ extern "C" int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, 
       (uintptr_t)bias % 16 || (uintptr_t)codes % 16 || (uintptr_t)scales % 16 || (uintptr_t)q8 % 16 ||
       (R && ((uintptr_t)l1f % 16 || (uintptr_t)l2t % 16 || (uintptr_t)t % 16)))
     return set_error(PQ_EALIGN, "pq_mx_linear: operands 16-byte aligned, ldx and ldy multiples of 8");
-  mx::GemmArgs p{codes, scales, w, w_scales, bias, static_cast<const uint16_t*>(R ? t : nullptr), static_cast<const uint16_t*>(l2t),
-                 static_cast<uint16_t*>(y), R, ldy, (int)M, (int)N, mx::stages(K), 0, 0};
+  mx::GemmArgs p{codes, scales, w, w_scales, bias, R ? t : nullptr, static_cast<const uint16_t*>(l2t),
+                 static_cast<uint16_t*>(y), R, ldy, (int)M, (int)N, mx::stages(K), 0, 0, true};
   const int64_t need = R ? mx::lowrank_workspace(M, K, R) : 0;
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return set_error(PQ_EINVAL, "pq_mx_linear: a workspace of %lld bytes, 16-byte aligned", (long long)need);

@@ -2,7 +2,7 @@
 //   y  = xh wh^T + t B + b,  t = x A
 //   dt = dy B^T,  dB = t^T dy,  db = sum_m dy,  dA = xt^T dt,  dx = dy wh + dt A^T
 // xt: the values of the 8-bit codes the forward pass kept of x. The rounding of x to 4 bits counts as the identity. All sums in
-// fp32. t and dt are operands of 16-bit matrix instructions, in two parts (two_parts): dA and dB take both, dx the first of dt.
+// fp32. t and dt are fp32, and operands of 16-bit matrix instructions in two parts (two_parts).
 #include "pq_mx.h"
 
 #include <algorithm>
@@ -36,13 +36,36 @@ __device__ __forceinline__ v4i read_columns(At at, int r0, int c0, int lane) {
 struct DxArgs {
   const uint16_t* dy;
   const uint8_t *w, *ws;
-  const uint16_t *dt, *ap;   // [M, R], [K, R]
+  const void* dt;            // [M, R], 16-bit or fp32 (wide)
+  const uint16_t* ap;        // [K, R]
   uint16_t* dx;
   int64_t lddy, lddx;
   int M, N, K, KT;
   int tiles_m, tiles_k;
   float* part;   // a split over n: [slices][M][K], `slice` n each
   int slice;
+  bool wide;
+};
+
+// dx += dt A^T: row m of dt (that of lane % 32), then tiles of 32 columns k (from kk) x 32 rows
+template <int DT, int R>
+struct LowRank {
+  v4i hi[R ? R / 16 : 1], lo[R ? R / 16 : 1];
+  __device__ __forceinline__ LowRank(const DxArgs& p, int m, int lane) {
+    RankPiece t[R ? R / 16 : 1];
+#pragma unroll
+    for (int s = 0; s < R / 16; ++s) t[s].load(p.dt, (int64_t)min(m, p.M - 1) * R + 16 * s + 8 * (lane >> 5), p.wide);
+#pragma unroll
+    for (int s = 0; s < R / 16; ++s) t[s].template parts<DT>(hi[s], lo[s], p.wide);
+  }
+  __device__ __forceinline__ v16f add(const DxArgs& p, int kk, int lane, v16f acc) const {
+#pragma unroll
+    for (int s = 0; s < R / 16; ++s) {
+      const v4i a = *reinterpret_cast<const v4i*>(p.ap + (int64_t)min(kk + (lane & 31), p.K - 1) * R + 16 * s + 8 * (lane >> 5));
+      acc = rank_product<DT>(a, hi[s], lo[s], acc, p.wide);
+    }
+    return acc;
+  }
 };
 
 // Few blocks: a workgroup of four waves takes 64 rows m x 128 columns k (one stage of the packed weight), 64 n a step. dy and
@@ -124,10 +147,12 @@ __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
     if (n0 + 64 < end) step(next[0], next[1], n0 + 64, 1);
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < TJ; ++j) {
+    const int m = m0 + wm + 32 * j + l32;
+    const LowRank<DT, SPLIT ? 0 : R> low(p, m, lane);
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) {
-      const int m = m0 + wm + 32 * j + l32, kk = k0 + wk + 32 * i;
+    for (int i = 0; i < 2; ++i) {
+      const int kk = k0 + wk + 32 * i;
       if (SPLIT) {
         if (m < p.M && kk < p.K) {
 #pragma unroll
@@ -137,14 +162,7 @@ __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
         }
         continue;
       }
-      if constexpr (R > 0) {
-#pragma unroll
-        for (int s = 0; s < R / 16; ++s) {
-          const v4i b = *reinterpret_cast<const v4i*>(p.ap + (int64_t)min(kk + l32, p.K - 1) * R + 16 * s + 8 * half);
-          const v4i t = *reinterpret_cast<const v4i*>(p.dt + (int64_t)min(m, p.M - 1) * R + 16 * s + 8 * half);
-          acc[i][j] = mfma16<DT>(b, t, acc[i][j]);
-        }
-      }
+      acc[i][j] = low.add(p, kk, lane, acc[i][j]);
       if (m < p.M && kk < p.K) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -152,6 +170,7 @@ __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
               v2u{pack2<DT>(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack2<DT>(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
       }
     }
+  }
 }
 
 // dx from the slices' sums, added in order, and the low-rank term. A wave takes 32 rows x 32 columns. Bound by reading the sums:
@@ -173,14 +192,7 @@ __global__ __launch_bounds__(256) void mx_dx_join_kernel(const DxArgs p, int sli
       }
     }
   }
-  if constexpr (R > 0) {
-#pragma unroll
-    for (int s = 0; s < R / 16; ++s) {
-      const v4i b = *reinterpret_cast<const v4i*>(p.ap + (int64_t)(kk + l32) * R + 16 * s + 8 * half);
-      const v4i t = *reinterpret_cast<const v4i*>(p.dt + (int64_t)min(m, p.M - 1) * R + 16 * s + 8 * half);
-      acc = mfma16<DT>(b, t, acc);
-    }
-  }
+  acc = LowRank<DT, R>(p, m, lane).add(p, kk, lane, acc);
   if (m < p.M) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -425,21 +437,14 @@ void mx_dx_ring_kernel(const DxArgs p) {
   }
   uint8_t* const stage = smem + wave * 32 * T::PITCH;
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < 2; ++j) {
+    const LowRank<DT, R> low(p, mb + 32 * j + l32, lane);
 #pragma unroll
     for (int ih = 0; ih < 2; ++ih) {
 #pragma unroll
       for (int ii = 0; ii < 2; ++ii) {
         const int i = 2 * ih + ii;
-        v16f y = acc[i][j];
-        if constexpr (R > 0) {
-#pragma unroll
-          for (int s = 0; s < R / 16; ++s) {
-            const v4i l = *reinterpret_cast<const v4i*>(p.ap + (int64_t)min(kb0 + 32 * i + l32, p.K - 1) * R + 16 * s + 8 * half);
-            const v4i t = *reinterpret_cast<const v4i*>(p.dt + (int64_t)min(mb + 32 * j + l32, p.M - 1) * R + 16 * s + 8 * half);
-            y = mfma16<DT>(l, t, y);
-          }
-        }
+        const v16f y = low.add(p, kb0 + 32 * i, lane, acc[i][j]);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<v2u*>(stage + l32 * T::PITCH + (ii * 32 + 8 * q + 4 * half) * 2) =
@@ -456,17 +461,18 @@ void mx_dx_ring_kernel(const DxArgs p) {
       wave_sync();
       __builtin_amdgcn_sched_barrier(0);
     }
+  }
 }
 
 // ---- sums over rows: part[s][r][c] = sum over the rows of slice s of v[m, r] z[m, c] -------------------------------------
-// z is dy (EIGHT false) or the 8-bit codes of x with their scales; v is t or dt, the sum of its two parts [2, M, R]. Column sums of z too (COLS). A
+// z is dy (EIGHT false) or the 8-bit codes of x with their scales; v is t or dt, [M, R] in fp32. Column sums of z too (COLS). A
 // workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step, the next step's rows on their way into
 // registers meanwhile; the order of the sums is fixed. Bound by reading z: 460 MB of 16384 x 3072 x 12288 in 92 us, 5.0 TB/s
 // (87 with the first part of v alone; results' errors then grow by 1.4).
 struct SumArgs {
   const void* z;
   const uint8_t* scales;
-  const uint16_t* v;
+  const float* v;
   float *part, *part_cols;
   int64_t ldz;
   int M, C, KT, rows;   // rows a slice, a multiple of 64
@@ -485,7 +491,8 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
   const uint32_t one2 = DT == PQ_BF16 ? 0x3f803f80u : 0x3c003c00u;
   const v4i ones = {(int)one2, (int)one2, (int)one2, (int)one2};
   v16f acc[R / 32] = {}, cols = {};
-  v4u zr[EIGHT ? 2 : 4], vr[R / 16];   // v: 64 rows of the first part, then of the second
+  v4u zr[EIGHT ? 2 : 4];
+  v4f vr[R / 16];
   int byte = 0;
   auto load = [&](int m0) {
     if constexpr (EIGHT) {
@@ -508,9 +515,9 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
     }
 #pragma unroll
     for (int i = 0; i < R / 16; ++i) {
-      const int at = i % (R / 32) * 256 + tid, m = m0 + at / (R / 8);
-      vr[i] = v4u{0, 0, 0, 0};
-      if (m < end) vr[i] = *reinterpret_cast<const v4u*>(p.v + ((int64_t)(i / (R / 32)) * p.M + m) * R + at % (R / 8) * 8);
+      const int at = i * 256 + tid, m = m0 + at / (R / 4);
+      vr[i] = v4f{};
+      if (m < end) vr[i] = *reinterpret_cast<const v4f*>(p.v + (int64_t)m * R + at % (R / 4) * 4);
     }
   };
   load(s0);
@@ -529,7 +536,18 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
       for (int i = 0; i < 4; ++i) *reinterpret_cast<v4u*>(z_at(i * 16 + (tid >> 4), tid & 15)) = zr[i];
     }
 #pragma unroll
-    for (int i = 0; i < R / 16; ++i) *reinterpret_cast<v4u*>(sv + (i * 256 + tid) * 16) = vr[i];
+    for (int i = 0; i < R / 16; ++i) {   // 64 rows of the first part, then of the second
+      v2u hi, lo;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint32_t h, l;
+        two_parts<DT>(vr[i][2 * e], vr[i][2 * e + 1], h, l);
+        hi[e] = h;
+        lo[e] = l;
+      }
+      *reinterpret_cast<v2u*>(sv + (i * 256 + tid) * 8) = hi;
+      *reinterpret_cast<v2u*>(sv + 64 * R * 2 + (i * 256 + tid) * 8) = lo;
+    }
     __syncthreads();
     if (m0 + 64 < end) load(m0 + 64);   // in flight while this step's products run
 #pragma unroll
@@ -718,6 +736,8 @@ extern "C" int64_t pq_mx_grad_input_workspace_size(int64_t M, int64_t N, int64_t
 extern "C" int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, const uint8_t* w, const uint8_t* w_scales,
                                 const void* dt, const void* ap, int64_t R, void* dx, int64_t lddx, int64_t M, int64_t N,
                                 int64_t K, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  const bool wide = (dtype & PQ_MX_T32) != 0;
+  dtype &= ~PQ_MX_T32;
   if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || lddy < N || lddx < K || M > (1 << 30) ||
       lddy > (1 << 21) || K > (1 << 22))
     return set_error(PQ_ESHAPE, "pq_mx_grad_input: M=%lld N=%lld K=%lld lddy=%lld (N %% 16 == 0, K %% 32 == 0, lddy <= 2^21)",
@@ -729,8 +749,8 @@ extern "C" int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, con
   if ((uintptr_t)dy % 16 || lddy % 8 || (uintptr_t)w % 16 || (uintptr_t)w_scales % 16 || (uintptr_t)dx % 16 || lddx % 8 ||
       (uintptr_t)dt % 16 || (uintptr_t)ap % 16)
     return set_error(PQ_EALIGN, "pq_mx_grad_input: operands 16-byte aligned, lddy and lddx multiples of 8");
-  mx::DxArgs p{static_cast<const uint16_t*>(dy), w, w_scales, static_cast<const uint16_t*>(dt), static_cast<const uint16_t*>(ap),
-               static_cast<uint16_t*>(dx), lddy, lddx, (int)M, (int)N, (int)K, mx::stages(K), 0, 0, static_cast<float*>(workspace), 0};
+  mx::DxArgs p{static_cast<const uint16_t*>(dy), w, w_scales, dt, static_cast<const uint16_t*>(ap),
+               static_cast<uint16_t*>(dx), lddy, lddx, (int)M, (int)N, (int)K, mx::stages(K), 0, 0, static_cast<float*>(workspace), 0, wide};
   const int64_t need = pq_mx_grad_input_workspace_size(M, N, K);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return set_error(PQ_EINVAL, "pq_mx_grad_input: a workspace of %lld bytes, 16-byte aligned", (long long)need);
@@ -742,7 +762,7 @@ extern "C" int64_t pq_mx_grad_factors_workspace_size(int64_t M, int64_t K, int64
   return 4 * ((int64_t)mx::row_slices(M, N) * (P + 1) * N + (int64_t)mx::row_slices(M, K) * P * K);
 }
 
-extern "C" int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, const void* t, const void* dt, const int8_t* q8,
+extern "C" int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, const float* t, const float* dt, const int8_t* q8,
                                   const uint8_t* x_scales, int64_t M, int64_t K, int64_t N, int64_t R, int64_t P, void* dA,
                                   void* dB, float* dbias, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   if (M < 1 || N < 16 || N % 16 || K < 32 || K % 32 || lddy < N || R < 1 || R > P || (P != 32 && P != 64) ||
@@ -762,9 +782,9 @@ extern "C" int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, c
   float* const part_a = part + (int64_t)sb * (P + 1) * N;
   const int pb = (int)((N + 127) / 128), pk = (int)((K + 127) / 128);
   const bool want_b = dB || dbias, want_a = dA != nullptr;
-  const mx::SumArgs b{dy, nullptr, static_cast<const uint16_t*>(t), part, part + (int64_t)sb * P * N, lddy, (int)M, (int)N, 0,
+  const mx::SumArgs b{dy, nullptr, t, part, part + (int64_t)sb * P * N, lddy, (int)M, (int)N, 0,
                       rows(sb), pb, want_b ? pb * sb : 0};
-  const mx::SumArgs a{q8, x_scales, static_cast<const uint16_t*>(dt), part_a, nullptr, K, (int)M, (int)K, mx::stages(K), rows(sk),
+  const mx::SumArgs a{q8, x_scales, dt, part_a, nullptr, K, (int)M, (int)K, mx::stages(K), rows(sk),
                       pk, want_a ? pk * sk : 0};
   const int quads = (int)((R + 3) / 4), gb = (int)((N + 63) / 64), ga = (int)((K + 63) / 64);
   const mx::JoinArgs jb{part, b.part_cols, static_cast<uint16_t*>(dB), dbias, sb, (int)N, gb, !want_b ? 0 : gb * (dB ? quads : 1)};

@@ -71,6 +71,10 @@ def _check_matrix(q: Mxfp4Matrix) -> None:
         assert t.dtype == torch.uint8 and t.is_contiguous() and t.numel() >= units * size, (t.dtype, tuple(t.shape), q.rows, q.cols)
 
 
+def _t_flag(t: torch.Tensor) -> int:
+    return _lib.PQ_MX_T32 if t.dtype == torch.float32 else 0
+
+
 def _dtype16(dt: torch.dtype) -> int:
     return _lib.dtype_code(dt)
 
@@ -118,8 +122,8 @@ def checkpoint_values(q8: torch.Tensor, q: Mxfp4Matrix, dtype: torch.dtype = tor
 def mxfp4_gemm(xq: Mxfp4Matrix, wq: Mxfp4Matrix, bias: Optional[torch.Tensor], out_dtype: torch.dtype, *,
                t: Optional[torch.Tensor] = None, l2t: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """[M, N] = xq @ wq^T (+ t @ l2t^T) (+ bias), summed in fp32, rounded once. t [M, R] and l2t [N, R] in out_dtype, R 32 or
-    64; bias fp32 [N]; N % 16 == 0."""
+    """[M, N] = xq @ wq^T (+ t @ l2t^T) (+ bias), summed in fp32, rounded once. t [M, R] in fp32 (taken to twice out_dtype's
+    bits) or out_dtype, l2t [N, R] in out_dtype, R 32 or 64; bias fp32 [N]; N % 16 == 0."""
     _check_matrix(xq)
     _check_matrix(wq)
     _check_cuda(xq.codes, xq.scales, wq.codes, wq.scales, bias, t, l2t, out)
@@ -130,9 +134,10 @@ def mxfp4_gemm(xq: Mxfp4Matrix, wq: Mxfp4Matrix, bias: Optional[torch.Tensor], o
         assert bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == N, (bias.dtype, tuple(bias.shape), N)
     R, ldt = 0, 0
     if t is not None:
-        assert l2t is not None and t.dtype == l2t.dtype == out_dtype and t.stride(1) == 1 and l2t.is_contiguous()
-        assert t.dim() == 2 and t.shape[0] >= M and tuple(l2t.shape) == (N, t.shape[1]), (tuple(t.shape), tuple(l2t.shape), M, N)
+        assert l2t is not None and l2t.dtype == out_dtype and t.dtype in (out_dtype, torch.float32) and l2t.is_contiguous()
+        assert t.dim() == 2 and t.stride(1) == 1 and t.shape[0] >= M and tuple(l2t.shape) == (N, t.shape[1]), (tuple(t.shape), tuple(l2t.shape), M, N)
         R, ldt = t.shape[1], _stride(t)
+        code |= _t_flag(t)
     if out is None:
         out = torch.empty((M, N), dtype=out_dtype, device=xq.codes.device)
     assert out.dtype == out_dtype and tuple(out.shape) == (M, N) and out.stride(1) == 1, (out.dtype, tuple(out.shape))
@@ -144,8 +149,8 @@ def mxfp4_gemm(xq: Mxfp4Matrix, wq: Mxfp4Matrix, bias: Optional[torch.Tensor], o
 
 def mxfp4_grad_input(dy: torch.Tensor, wq: Mxfp4Matrix, dt: Optional[torch.Tensor] = None,
                      lr_Ap: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """dx [M, K] = dy @ wq (+ dt @ lr_Ap^T): wq's values in dy's type, sums in fp32. dt [M, R] and lr_Ap [K, R] contiguous, R 32
-    or 64."""
+    """dx [M, K] = dy @ wq (+ dt @ lr_Ap^T): wq's values in dy's type, sums in fp32. dt [M, R] in fp32 or dy's type, lr_Ap
+    [K, R] in dy's type, contiguous, R 32 or 64."""
     _check_matrix(wq)
     _check_cuda(dy, wq.codes, wq.scales, dt, lr_Ap)
     assert dy.dim() == 2 and dy.shape[1] == wq.rows, (tuple(dy.shape), wq.rows)
@@ -155,8 +160,9 @@ def mxfp4_grad_input(dy: torch.Tensor, wq: Mxfp4Matrix, dt: Optional[torch.Tenso
     R = 0
     if dt is not None:
         R = dt.shape[1]
-        assert lr_Ap is not None and dt.dtype == lr_Ap.dtype == dy.dtype and dt.is_contiguous() and lr_Ap.is_contiguous()
+        assert lr_Ap is not None and lr_Ap.dtype == dy.dtype and dt.dtype in (dy.dtype, torch.float32) and dt.is_contiguous() and lr_Ap.is_contiguous()
         assert tuple(dt.shape) == (M, R) and tuple(lr_Ap.shape) == (K, R), (tuple(dt.shape), tuple(lr_Ap.shape), M, K)
+        code |= _t_flag(dt)
     dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
     L = _lib.load()
     size = L.pq_mx_grad_input_workspace_size(M, N, K)
@@ -167,27 +173,38 @@ def mxfp4_grad_input(dy: torch.Tensor, wq: Mxfp4Matrix, dt: Optional[torch.Tenso
     return dx
 
 
+def _ranks(t: torch.Tensor, M: int, P: int, dtype: torch.dtype) -> torch.Tensor:
+    """t or dt as lowrank_grads' kernels read it: fp32 [M, P], from that or from its two parts."""
+    if t.dim() == 3:
+        assert t.dtype == dtype and tuple(t.shape) == (2, M, P), (t.dtype, tuple(t.shape), dtype, M, P)
+        t = t[0].float() + t[1].float()
+    assert t.dtype == torch.float32 and tuple(t.shape) == (M, P), (t.dtype, tuple(t.shape), M, P)
+    return _plain(t).contiguous()
+
+
 def lowrank_grads(dy: Optional[torch.Tensor], t: Optional[torch.Tensor], dt: Optional[torch.Tensor], q8: Optional[torch.Tensor],
                   x_scales: Optional[torch.Tensor], rank: int, want_A: bool = True, want_B: bool = True, want_bias: bool = True):
     """(dA [K, rank], dB [rank, N], dbias [N] fp32), None for those not wanted: dB = t^T dy, dbias = sum of dy's rows, dA =
-    checkpoint^T dt. t and dt are [2, M, P], P 32 or 64 >= rank, zero past rank, each the sum of its two parts (the value in 16
-    bits, and what that rounding left out); q8 and x_scales as quant_mxfp4 gave them. What no wanted gradient needs may be
-    None."""
+    checkpoint^T dt, in dy's type. t and dt are [M, P] in fp32, P 32 or 64 >= rank, zero past rank, or [2, M, P] in the type of
+    the results, each the sum of its two parts (the value, and what that rounding left out); q8 and x_scales as quant_mxfp4 gave
+    them. What no wanted gradient needs may be None; without a dy, fp32 dt gives dA in bf16."""
     if not (want_A or want_B or want_bias):
         return None, None, None
     ref = dt if want_A else t
     _check_cuda(dy, t, dt, q8, x_scales)
-    assert ref.dim() == 3 and ref.shape[0] == 2, tuple(ref.shape)
-    _, M, P = ref.shape
-    dt16, dev = ref.dtype, ref.device
+    M, P = ref.shape[-2:]
+    dev = ref.device
+    dt16 = dy.dtype if want_B or want_bias else ref.dtype if ref.dtype != torch.float32 else torch.bfloat16
     code = _dtype16(dt16)
     K = N = BLOCK
     if want_A:
-        assert q8.dtype == torch.int8 and q8.is_contiguous() and q8.shape[0] == M and dt.is_contiguous()
+        dt = _ranks(dt, M, P, dt16)
+        assert q8.dtype == torch.int8 and q8.is_contiguous() and q8.shape[0] == M
         K = q8.shape[1]
         assert x_scales.dtype == torch.uint8 and x_scales.numel() >= _stages(M, K) * 64
     if want_B or want_bias:
-        assert dy.dim() == 2 and dy.shape[0] == M and dy.dtype == dt16 and tuple(t.shape) == (2, M, P) and t.is_contiguous()
+        t = _ranks(t, M, P, dt16)
+        assert dy.dim() == 2 and dy.shape[0] == M, (tuple(dy.shape), M)
         dy = _rows(dy)
         N = dy.shape[1]
     assert 1 <= rank <= P, (rank, P)

@@ -1,0 +1,107 @@
+"""Microscaled 4-bit layers where a wrong or a lost result would go unseen by a comparison at ordinary values: what is held in
+between, values at the ends of their types, every choice of operands and of what is wanted.
+
+Bounds as in test_mxfp4_gpu: u is the unit roundoff of the 16-bit type with half a place to spare (2^-8 for bf16, 2^-11 for fp16), a
+sum of n products in fp32 is within n 2^-23 of the sum of the magnitudes of its terms."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+BOTH = (torch.bfloat16, torch.float16)
+F = 2.0 ** -23
+
+
+def _layer(K, N, R, dtype, seed, std=0.3, bias=False, weight=0.0, factors=None, trainable=True):
+    """A layer whose weight is N(0, weight) (all zeros by default: what it computes is its low-rank branch) and its factors."""
+    from pyraquant_amd.mxfp4 import Mxfp4Linear
+
+    g = torch.Generator().manual_seed(seed)
+    lin = torch.nn.Linear(K, N, bias=bias)
+    with torch.no_grad():
+        lin.weight.copy_(torch.randn(N, K, generator=g) * weight)
+        if bias:
+            lin.bias.copy_(torch.randn(N, generator=g))
+    A, B = ((torch.randn(*s, generator=g) * std).to(factors or dtype).cuda() for s in ((K, R), (R, N))) if R else (None, None)
+    return Mxfp4Linear(lin.to(dtype), device="cuda", lowrank=(A, B) if R else None, trainable=trainable), A, B
+
+
+def _rand(*shape, dtype, seed, std=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype).cuda()
+
+
+def _within(got, want, bound, what):
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), f"{what}: {float((off / bound.clamp_min(1e-300)).max()):.3g} of the bound"
+
+
+# ---- what is held in between ----------------------------------------------------------------------------------------
+
+def _through(x, A, B, dtype):
+    """(x A) B in 64 bits, and how far from it a result may be whose x A lost no more than u^2 of itself: twice the type's bits
+    (in fp16, and 2^-25: its subnormals' half place)."""
+    u, small = U[dtype], 2.0 ** -25 if dtype == torch.float16 else 0.0
+    x, A, B = x.double(), A.double(), B.double()
+    t = x @ A
+    lost = x.shape[1] * F * (x.abs() @ A.abs())
+    t_off = lost + u * u * (t.abs() + lost) + small
+    y = t @ B
+    off = t_off @ B.abs() + 2 * (A.shape[1] + 2) * F * ((t.abs() + t_off) @ B.abs())
+    return y, off + u * (y.abs() + off) + small
+
+
+# rows quantized inside the product; a split product; blocks of 128 x 64, of 128 x 64 in three groups, of 128 x 256 and of 256 x
+# 256; and with them the input gradient in both kinds of block, whole and in slices
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("M,K,N,R", [(20, 64, 96, 8), (154, 2048, 1280, 32), (300, 640, 5120, 64), (329, 4320, 2512, 40), (600, 1056, 7056, 64),
+                                     (2100, 160, 4112, 64), (4200, 416, 4208, 32), (4128, 2080, 496, 32), (2050, 1312, 5136, 64),
+                                     (40, 96, 4112, 33)])
+def test_low_rank_terms_lose_nothing_in_between(cuda, dtype, M, K, N, R):
+    """Over a weight of zeros y is (x A) B and dx is (dy B^T) A^T: sums of mixed signs, most of them far smaller than their terms,
+    so a rounding of x A or dy B^T to 16 bits on the way would show."""
+    layer, A, B = _layer(K, N, R, dtype, K + N, std=0.1)
+    x, dy = _rand(M, K, dtype=dtype, seed=M).requires_grad_(), _rand(M, N, dtype=dtype, seed=N)
+    y = layer(x)
+    dx, = torch.autograd.grad(y, x, dy)
+    _within(y.detach(), *_through(x.detach(), A, B, dtype), "y")
+    _within(dx, *_through(dy, B.t(), A.t(), dtype), "dx")
+    layer.freeze()
+    with torch.no_grad():
+        assert torch.equal(layer(x), y)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_32_bit_low_rank_operands(cuda, dtype):
+    """mxfp4_gemm and mxfp4_grad_input take t and dt in fp32 as the layer's own calls do, rows with a stride among them, and
+    lowrank_grads takes them in fp32 or as two parts that add up to it."""
+    from pyraquant_amd.mxfp4 import lowrank_grads, mxfp4_gemm, mxfp4_grad_input, quant_mxfp4
+
+    M, K, N, R = 70, 96, 80, 32
+    x, w, dy = _rand(M, K, dtype=dtype, seed=1), torch.zeros(N, K, device=cuda), _rand(M, N, dtype=dtype, seed=2)
+    wide = _rand(M, 36, dtype=torch.float32, seed=3)
+    t, l2t, ap = wide[:, :32], _rand(N, R, dtype=dtype, seed=4), _rand(K, R, dtype=dtype, seed=5)
+    xq, q8 = quant_mxfp4(x, checkpoint=True)
+    wq = quant_mxfp4(w)
+    u, small = U[dtype], 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for got, l in ((mxfp4_gemm(xq, wq, None, dtype, t=t, l2t=l2t), l2t), (mxfp4_grad_input(dy, wq, t.contiguous(), ap), ap)):
+        want, terms = t.double() @ l.double().t(), t.double().abs() @ l.double().abs().t()
+        off = (u * u + 2 * R * F) * terms + small * l.double().abs().sum(1)
+        _within(got, want, off + u * (want.abs() + off) + small, "low-rank term")
+    parts = [torch.stack([v.to(dtype), (v - v.to(dtype).float()).to(dtype)]) for v in (t, wide[:, 4:])]
+    whole = [p[0].float() + p[1].float() for p in parts]
+    a, b = (lowrank_grads(dy, *v, q8, xq.scales, 20) for v in (parts, whole))
+    assert all(torch.equal(g, h) for g, h in zip(a, b)) and a[0].dtype == a[1].dtype == dtype
+
+
+def test_lowrank_grads_checks_both_operands(cuda):
+    """t and dt are read through raw pointers: another type or shape of either is refused, whatever is wanted."""
+    from pyraquant_amd.mxfp4 import lowrank_grads, quant_mxfp4
+
+    dy, (q, q8) = _rand(4, 32, dtype=torch.bfloat16, seed=1), quant_mxfp4(_rand(4, 64, dtype=torch.bfloat16, seed=2), checkpoint=True)
+    good = torch.zeros(2, 4, 32, dtype=torch.bfloat16, device=cuda)
+    for bad in (good.float(), good.half(), good[:1], good[:, :, :16], good[:, :3], good[0]):
+        with pytest.raises(AssertionError):
+            lowrank_grads(dy, bad, good, q8, q.scales, 8)
+        with pytest.raises(AssertionError):
+            lowrank_grads(dy, good, bad, q8, q.scales, 8)
