@@ -397,13 +397,12 @@ int pq_mx_values(const void* codes, const uint8_t* scales, int32_t bits, int64_t
 
 /*
  * y[m, n] = sum_k xh[m, k] wh[n, k] (+ sum_r t[m, r] l2t[n, r]) (+ bias[n]), summed in fp32, rounded once to dtype (PQ_BF16 or
- * PQ_F16). a, w: packed 4-bit matrices [M, K] and [N, K]. t [M, R] (row stride ldt) and l2t [N, R] of dtype, R in {32, 64}, or
- * NULL. K % 32 == 0, N % 16 == 0, M <= 2^30; operands 16-byte aligned, ldc (<= 2^21) and ldt multiples of 8. With dtype |
- * PQ_MX_T32 t is fp32, as pq_mx_lowrank_down gives it (ldt a multiple of 4), and taken to twice dtype's bits.
+ * PQ_F16). a, w: packed 4-bit matrices [M, K] and [N, K]. t [M, R] (fp32, row stride ldt, taken to twice dtype's bits) and l2t [N, R] of
+ * dtype, R in {32, 64}, or NULL. K % 32 == 0, N % 16 == 0, M <= 2^30; operands 16-byte aligned, ldc (<= 2^21) and ldt multiples
+ * of 8.
  */
-#define PQ_MX_T32 0x200
 int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales, const float* bias,
-               const void* t, int64_t ldt, const void* l2t, int64_t R, void* c, int64_t ldc, int32_t dtype, int64_t M, int64_t N,
+               const float* t, int64_t ldt, const void* l2t, int64_t R, void* c, int64_t ldc, int32_t dtype, int64_t M, int64_t N,
                int64_t K, hipStream_t stream);
 
 /*
@@ -444,12 +443,12 @@ int pq_mx_lowrank_down(const void* x, int32_t dtype, int64_t M, int64_t K, int64
 /*
  * dx[m, k] = sum_n dy[m, n] wh[n, k] (+ sum_r dt[m, r] ap[k, r]): the gradient of a layer's input over its packed 4-bit weight
  * [N, K], widened to dtype on the way to the matrix instructions (exact; in fp16, for 2^-22 <= 2^E <= 2^13), summed in fp32.
- * dy [M, N], dx [M, K] of dtype; dt [M, R] and ap [K, R] contiguous, R in {32, 64}, or NULL, dt fp32 with dtype | PQ_MX_T32.
- * Operands 16-byte aligned, lddy and lddx multiples of 8, lddy <= 2^21. A workspace of pq_mx_grad_input_workspace_size bytes (0 for most sizes) that may hold
+ * dy [M, N], dx [M, K] of dtype; dt [M, R] (fp32, taken to twice dtype's bits) and ap [K, R] (of dtype) contiguous, R in {32,
+ * 64}, or NULL. Operands 16-byte aligned, lddy and lddx multiples of 8, lddy <= 2^21. A workspace of pq_mx_grad_input_workspace_size bytes (0 for most sizes) that may hold
  * anything.
  */
 int64_t pq_mx_grad_input_workspace_size(int64_t M, int64_t N, int64_t K);
-int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, const uint8_t* w, const uint8_t* w_scales, const void* dt,
+int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, const uint8_t* w, const uint8_t* w_scales, const float* dt,
                      const void* ap, int64_t R, void* dx, int64_t lddx, int64_t M, int64_t N, int64_t K, void* workspace,
                      int64_t workspace_bytes, hipStream_t stream);
 

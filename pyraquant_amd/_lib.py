@@ -18,7 +18,6 @@ PQ_OK, PQ_EINVAL, PQ_ESHAPE, PQ_EALIGN, PQ_EDTYPE, PQ_ELAUNCH = 0, -1, -2, -3, -
 PQ_BF16, PQ_F16, PQ_I32, PQ_F32 = 0, 1, 2, 3
 PQ_MX_BY_COLUMN, PQ_MX_BY_RANK, PQ_MX_FRAGMENTS = 0, 1, 2   # orders of a low-rank factor (pq_mx_factors)
 PQ_ACCUMULATE = 0x100   # OR'ed into pq_int8_gemm_packed's out_dtype
-PQ_MX_T32 = 0x200       # OR'ed into pq_mx_gemm's and pq_mx_grad_input's dtype: t (dt) is fp32
 ABI_VERSION = 4
 
 # every entry point declared in include/pyraquant_amd.h

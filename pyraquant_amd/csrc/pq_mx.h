@@ -173,16 +173,24 @@ __device__ __forceinline__ float restore_scale(int byte) {
   return byte == kNaN ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(1.0f, byte - 131);
 }
 
-// t and dt are kept in fp32 and taken as two 16-bit parts by the products that read them: the value rounded, and what that rounding
-// left out, rounded too (0 where the value is not finite). The two together hold it to twice the bits; with the first alone the
-// rounding of t shows in every result, as large as the results' own where the low-rank term is the larger one.
+// t and dt are kept in fp32 and taken as two 16-bit parts by the products that read them, hi + lo: twice the bits. With the first
+// alone the rounding of t shows in every result, as large as the results' own where the low-rank term is the larger one.
+// hi is cut towards zero from the next value nearer zero, so that lo has the sign of the value and is no zero where hi is none: an
+// infinity on the other side of a product meets two parts of one sign and gives what it gives with the value itself, where a lo of
+// 0 or of the other sign would make it NaN. (An infinite value is a finite hi and an infinite lo; in fp16, whose lo must not fall
+// below the smallest subnormal, hi lies at least that much nearer zero, and values under 2^-23 may have a hi of 0.)
 template <int DT>
 __device__ __forceinline__ void two_parts(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack2<DT>(a, b);
-  float r0 = a - lo16_to_f32<DT>(hi), r1 = b - hi16_to_f32<DT>(hi);
-  if (!(fabsf(r0) < INFINITY)) r0 = 0.0f;
-  if (!(fabsf(r1) < INFINITY)) r1 = 0.0f;
-  lo = pack2<DT>(r0, r1);
+  auto nearer = [](float v) { return __uint_as_float(__builtin_elementwise_sub_sat(__float_as_uint(v), 1u)); };
+  a += 0.0f;   // (-0 to 0: its bits are no magnitude to step down from)
+  b += 0.0f;
+  if constexpr (DT == PQ_BF16) {
+    hi = __builtin_amdgcn_perm(__float_as_uint(nearer(b)), __float_as_uint(nearer(a)), 0x07060302);
+  } else {
+    const float tiny = 0x1p-24f;
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(nearer(a) - copysignf(tiny, a), nearer(b) - copysignf(tiny, b)));
+  }
+  lo = pack2<DT>(a - lo16_to_f32<DT>(hi), b - hi16_to_f32<DT>(hi));
 }
 
 // ---- shared by the products ------------------------------------------------------------------------------------------
@@ -205,39 +213,28 @@ __device__ __forceinline__ v16f mfma16(v4i a, v4i b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// Eight consecutive ranks of a row of t (or dt), operand of a low-rank product. `load` asks for them, `parts` makes the operands:
-// fp32 values (wide) in two parts, 16-bit values as they are. `wide` is the same for the whole launch.
+// Eight consecutive ranks of a row of t (or dt), operand of a low-rank product: the values, and their two parts.
 struct RankPiece {
   v4f raw[2];
-  __device__ __forceinline__ void load(const void* t, int64_t at, bool wide) {
-    if (wide) {
-      const v4f* const src = reinterpret_cast<const v4f*>(static_cast<const float*>(t) + at);
-      raw[0] = src[0];
-      raw[1] = src[1];
-    } else {
-      raw[0] = *reinterpret_cast<const v4f*>(static_cast<const uint16_t*>(t) + at);
-    }
+  __device__ __forceinline__ void load(const float* at) {
+    raw[0] = reinterpret_cast<const v4f*>(at)[0];
+    raw[1] = reinterpret_cast<const v4f*>(at)[1];
   }
   template <int DT>
-  __device__ __forceinline__ void parts(v4i& hi, v4i& lo, bool wide) const {
-    hi = __builtin_bit_cast(v4i, raw[0]);
-    lo = v4i{0, 0, 0, 0};
-    if (wide) {
+  __device__ __forceinline__ void parts(v4i& hi, v4i& lo) const {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t h, l;
-        two_parts<DT>(raw[e >> 1][2 * (e & 1)], raw[e >> 1][2 * (e & 1) + 1], h, l);
-        hi[e] = (int)h;
-        lo[e] = (int)l;
-      }
+    for (int e = 0; e < 4; ++e) {
+      uint32_t h, l;
+      two_parts<DT>(raw[e >> 1][2 * (e & 1)], raw[e >> 1][2 * (e & 1) + 1], h, l);
+      hi[e] = (int)h;
+      lo[e] = (int)l;
     }
   }
 };
 // y += l t^T over the 16 ranks of a piece
 template <int DT>
-__device__ __forceinline__ v16f rank_product(v4i l, v4i hi, v4i lo, v16f y, bool wide) {
-  if (wide) y = mfma16<DT>(l, lo, y);
-  return mfma16<DT>(l, hi, y);
+__device__ __forceinline__ v16f rank_product(v4i l, v4i hi, v4i lo, v16f y) {
+  return mfma16<DT>(l, hi, mfma16<DT>(l, lo, y));
 }
 
 // Workgroup id -> (tile_m, tile_n): ids are dealt round-robin over the 8 XCDs, so each XCD takes a contiguous run of the

@@ -174,7 +174,7 @@ struct Layer : torch::autograd::Function<Layer> {
                                  data<void>(out[2]), data<float>(out[3]), s + s_dt, ws_sums, stream),
               "mxfp4 factor gradients");
       if (w.x)
-        check(pq_mx_grad_input(dy.const_data_ptr(), code | PQ_MX_T32, stride_of(dy), data<uint8_t>(codes), data<uint8_t>(scales),
+        check(pq_mx_grad_input(dy.const_data_ptr(), code, stride_of(dy), data<uint8_t>(codes), data<uint8_t>(scales),
                                P ? dt : nullptr, P ? h + k.ap : nullptr, P, out[0].data_ptr(), K, M, N, K,
                                ws_dx ? s + s_dt : nullptr, ws_dx, stream),
               "mxfp4 input gradient");

@@ -20,13 +20,12 @@ namespace {
 struct GemmArgs {
   const uint8_t *a, *as, *w, *ws;   // codes and scales of x and of the weight
   const float* bias;
-  const void* t;                    // 16-bit, or fp32 (wide)
+  const float* t;
   const uint16_t* l2t;
   uint16_t* c;
-  int64_t ldt, ldc;
+  int ldt, ldc;
   int M, N, KT;
   int tiles_m, tiles_n;
-  bool wide;
 };
 
 // One step over 64 values: both operands 4-bit (format code 4), scale byte S of each scale word.
@@ -225,12 +224,12 @@ void mx_gemm_kernel(const GemmArgs p) {
       for (int s = 0; s < R / 16; ++s) {
         RankPiece t;
         v4i hi, lo;
-        t.load(p.t, (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + 16 * s + 8 * half, p.wide);
-        t.parts<DT>(hi, lo, p.wide);
+        t.load(p.t + (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + 16 * s + 8 * half);
+        t.parts<DT>(hi, lo);
 #pragma unroll
         for (int i = 0; i < TI; ++i) {
           const v4i l = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(nb + 32 * i + l32, p.N - 1) * R + 16 * s + 8 * half);
-          acc[i][j] = rank_product<DT>(l, hi, lo, acc[i][j], p.wide);
+          acc[i][j] = rank_product<DT>(l, hi, lo, acc[i][j]);
         }
       }
     }
@@ -430,7 +429,7 @@ void mx_gemm_large_kernel(const GemmArgs p) {
     // Lane l holds, of tile (i, j): row m = 32 j + l % 32, outputs n = 32 i + 8 q + 4 (l / 32) .. + 3 in elements 4 q ..
     const int nb = n0 + wn * (BN / 2), mb = m0 + wm * (BM / 4);
     const auto rs_c = __builtin_amdgcn_make_buffer_rsrc((void*)(p.c + (int64_t)m0 * p.ldc + n0), (short)0,
-                                                        (int)(((min(BM, p.M - m0) - 1) * p.ldc + min(BN, p.N - n0)) * 2), kBufferWord3);
+                                                        ((min(BM, p.M - m0) - 1) * p.ldc + min(BN, p.N - n0)) * 2, kBufferWord3);
     const int valid_n = p.N - n0;
     const int next = tile + (int)gridDim.x;
     const bool more = next < tiles;
@@ -450,7 +449,7 @@ void mx_gemm_large_kernel(const GemmArgs p) {
         for (int x = 0; x < 2; ++x) {
 #pragma unroll
           for (int j = 0; j < TJ; ++j)
-            tv[j][x].load(p.t, (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + r0 + 16 * x + 8 * half, p.wide);
+            tv[j][x].load(p.t + (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + r0 + 16 * x + 8 * half);
 #pragma unroll
           for (int i = 0; i < TI; ++i)
             lv[i][x] = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(nb + 32 * i + l32, p.N - 1) * R + r0 + 16 * x + 8 * half);
@@ -461,9 +460,9 @@ void mx_gemm_large_kernel(const GemmArgs p) {
 #pragma unroll
           for (int j = 0; j < TJ; ++j) {
             v4i hi, lo;
-            tv[j][x].template parts<DT>(hi, lo, p.wide);
+            tv[j][x].template parts<DT>(hi, lo);
 #pragma unroll
-            for (int i = 0; i < TI; ++i) acc[i][j] = rank_product<DT>(lv[i][x], hi, lo, acc[i][j], p.wide);
+            for (int i = 0; i < TI; ++i) acc[i][j] = rank_product<DT>(lv[i][x], hi, lo, acc[i][j]);
           }
       }
     } else {
@@ -496,7 +495,7 @@ void mx_gemm_large_kernel(const GemmArgs p) {
           for (int r0 = 0; r0 < 16; r0 += 8) {
             const int m = wm * (BM / 4) + 32 * j + 16 * rows + r0 + (lane >> 3);
             const v4u v = *reinterpret_cast<const v4u*>(out + (r0 + (lane >> 3)) * PITCH + (lane & 7) * 16);
-            const int off = n < valid_n ? (m * (int)p.ldc + n) * 2 : kOOB;
+            const int off = n < valid_n ? (m * p.ldc + n) * 2 : kOOB;
             __builtin_amdgcn_raw_buffer_store_b128(v, rs_c, off, 0, 2);   // (2: streamed past the L2)
           }
           wave_sync();
@@ -635,9 +634,9 @@ __global__ __launch_bounds__(64 * NW) void mx_gemm_split_kernel(const SplitArgs 
             const v4i l = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(n0 + 32 * i + l32, p.N - 1) * R + 16 * s + 8 * half);
             RankPiece t;
             v4i hi, lo;
-            t.load(p.t, (int64_t)min(m, p.M - 1) * p.ldt + 16 * s + 8 * half, p.wide);
-            t.parts<DT>(hi, lo, p.wide);
-            y = rank_product<DT>(l, hi, lo, y, p.wide);
+            t.load(p.t + (int64_t)min(m, p.M - 1) * p.ldt + 16 * s + 8 * half);
+            t.parts<DT>(hi, lo);
+            y = rank_product<DT>(l, hi, lo, y);
           }
         }
 #pragma unroll
@@ -713,10 +712,8 @@ inline bool quantized_inside(int64_t M, int64_t K) { return M <= 32 && K <= 2048
 using namespace pq;
 
 extern "C" int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales,
-                          const float* bias, const void* t, int64_t ldt, const void* l2t, int64_t R, void* c, int64_t ldc,
+                          const float* bias, const float* t, int64_t ldt, const void* l2t, int64_t R, void* c, int64_t ldc,
                           int32_t dtype, int64_t M, int64_t N, int64_t K, hipStream_t stream) {
-  const bool wide = (dtype & PQ_MX_T32) != 0;
-  dtype &= ~PQ_MX_T32;
   if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || ldc < N || ldc > (1 << 21) || M > (1 << 30) ||
       N > (1 << 30) || K > (1 << 22))
     return set_error(PQ_ESHAPE, "pq_mx_gemm: M=%lld N=%lld K=%lld ldc=%lld (N %% 16 == 0, K %% 32 == 0, ldc <= 2^21)", (long long)M,
@@ -727,10 +724,10 @@ extern "C" int pq_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8
   if (M == 0) return PQ_OK;
   if (!a || !a_scales || !w || !w_scales || !c || (t && !l2t)) return set_error(PQ_EINVAL, "pq_mx_gemm: null pointer");
   if ((uintptr_t)a % 16 || (uintptr_t)w % 16 || (uintptr_t)a_scales % 16 || (uintptr_t)w_scales % 16 || (uintptr_t)c % 16 ||
-      ldc % 8 || (uintptr_t)bias % 16 || (t && ((uintptr_t)t % 16 || (uintptr_t)l2t % 16 || ldt % (wide ? 4 : 8))))
-    return set_error(PQ_EALIGN, "pq_mx_gemm: operands 16-byte aligned, ldc and ldt multiples of 8 (ldt of an fp32 t: 4)");
+      ldc % 8 || (uintptr_t)bias % 16 || (t && ((uintptr_t)t % 16 || (uintptr_t)l2t % 16 || ldt % 8)))
+    return set_error(PQ_EALIGN, "pq_mx_gemm: operands 16-byte aligned, ldc and ldt multiples of 8");
   mx::GemmArgs p{a, a_scales, w, w_scales, bias, t, static_cast<const uint16_t*>(l2t),
-                 static_cast<uint16_t*>(c), ldt, ldc, (int)M, (int)N, mx::stages(K), 0, 0, wide};
+                 static_cast<uint16_t*>(c), (int)ldt, (int)ldc, (int)M, (int)N, mx::stages(K), 0, 0};
   return mx::launch_gemm(p, dtype, t ? (int)R : 0, stream);
 }
 
@@ -752,7 +749,7 @@ extern "C" int pq_mx_linear(const void* x, int32_t dtype, int64_t M, int64_t K, 
       (R && ((uintptr_t)l1f % 16 || (uintptr_t)l2t % 16 || (uintptr_t)t % 16)))
     return set_error(PQ_EALIGN, "pq_mx_linear: operands 16-byte aligned, ldx and ldy multiples of 8");
   mx::GemmArgs p{codes, scales, w, w_scales, bias, R ? t : nullptr, static_cast<const uint16_t*>(l2t),
-                 static_cast<uint16_t*>(y), R, ldy, (int)M, (int)N, mx::stages(K), 0, 0, true};
+                 static_cast<uint16_t*>(y), (int)R, (int)ldy, (int)M, (int)N, mx::stages(K), 0, 0};
   const int64_t need = R ? mx::lowrank_workspace(M, K, R) : 0;
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return set_error(PQ_EINVAL, "pq_mx_linear: a workspace of %lld bytes, 16-byte aligned", (long long)need);

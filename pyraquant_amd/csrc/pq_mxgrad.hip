@@ -36,7 +36,7 @@ __device__ __forceinline__ v4i read_columns(At at, int r0, int c0, int lane) {
 struct DxArgs {
   const uint16_t* dy;
   const uint8_t *w, *ws;
-  const void* dt;            // [M, R], 16-bit or fp32 (wide)
+  const float* dt;           // [M, R]
   const uint16_t* ap;        // [K, R]
   uint16_t* dx;
   int64_t lddy, lddx;
@@ -44,7 +44,6 @@ struct DxArgs {
   int tiles_m, tiles_k;
   float* part;   // a split over n: [slices][M][K], `slice` n each
   int slice;
-  bool wide;
 };
 
 // dx += dt A^T: row m of dt (that of lane % 32), then tiles of 32 columns k (from kk) x 32 rows
@@ -54,15 +53,15 @@ struct LowRank {
   __device__ __forceinline__ LowRank(const DxArgs& p, int m, int lane) {
     RankPiece t[R ? R / 16 : 1];
 #pragma unroll
-    for (int s = 0; s < R / 16; ++s) t[s].load(p.dt, (int64_t)min(m, p.M - 1) * R + 16 * s + 8 * (lane >> 5), p.wide);
+    for (int s = 0; s < R / 16; ++s) t[s].load(p.dt + (int64_t)min(m, p.M - 1) * R + 16 * s + 8 * (lane >> 5));
 #pragma unroll
-    for (int s = 0; s < R / 16; ++s) t[s].template parts<DT>(hi[s], lo[s], p.wide);
+    for (int s = 0; s < R / 16; ++s) t[s].template parts<DT>(hi[s], lo[s]);
   }
   __device__ __forceinline__ v16f add(const DxArgs& p, int kk, int lane, v16f acc) const {
 #pragma unroll
     for (int s = 0; s < R / 16; ++s) {
       const v4i a = *reinterpret_cast<const v4i*>(p.ap + (int64_t)min(kk + (lane & 31), p.K - 1) * R + 16 * s + 8 * (lane >> 5));
-      acc = rank_product<DT>(a, hi[s], lo[s], acc, p.wide);
+      acc = rank_product<DT>(a, hi[s], lo[s], acc);
     }
     return acc;
   }
@@ -734,10 +733,8 @@ extern "C" int64_t pq_mx_grad_input_workspace_size(int64_t M, int64_t N, int64_t
 }
 
 extern "C" int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, const uint8_t* w, const uint8_t* w_scales,
-                                const void* dt, const void* ap, int64_t R, void* dx, int64_t lddx, int64_t M, int64_t N,
+                                const float* dt, const void* ap, int64_t R, void* dx, int64_t lddx, int64_t M, int64_t N,
                                 int64_t K, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-  const bool wide = (dtype & PQ_MX_T32) != 0;
-  dtype &= ~PQ_MX_T32;
   if (M < 0 || N < 16 || N % 16 || K < 32 || K % 32 || lddy < N || lddx < K || M > (1 << 30) ||
       lddy > (1 << 21) || K > (1 << 22))
     return set_error(PQ_ESHAPE, "pq_mx_grad_input: M=%lld N=%lld K=%lld lddy=%lld (N %% 16 == 0, K %% 32 == 0, lddy <= 2^21)",
@@ -750,7 +747,7 @@ extern "C" int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, con
       (uintptr_t)dt % 16 || (uintptr_t)ap % 16)
     return set_error(PQ_EALIGN, "pq_mx_grad_input: operands 16-byte aligned, lddy and lddx multiples of 8");
   mx::DxArgs p{static_cast<const uint16_t*>(dy), w, w_scales, dt, static_cast<const uint16_t*>(ap),
-               static_cast<uint16_t*>(dx), lddy, lddx, (int)M, (int)N, (int)K, mx::stages(K), 0, 0, static_cast<float*>(workspace), 0, wide};
+               static_cast<uint16_t*>(dx), lddy, lddx, (int)M, (int)N, (int)K, mx::stages(K), 0, 0, static_cast<float*>(workspace), 0};
   const int64_t need = pq_mx_grad_input_workspace_size(M, N, K);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return set_error(PQ_EINVAL, "pq_mx_grad_input: a workspace of %lld bytes, 16-byte aligned", (long long)need);

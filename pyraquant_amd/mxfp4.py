@@ -71,10 +71,6 @@ def _check_matrix(q: Mxfp4Matrix) -> None:
         assert t.dtype == torch.uint8 and t.is_contiguous() and t.numel() >= units * size, (t.dtype, tuple(t.shape), q.rows, q.cols)
 
 
-def _t_flag(t: torch.Tensor) -> int:
-    return _lib.PQ_MX_T32 if t.dtype == torch.float32 else 0
-
-
 def _dtype16(dt: torch.dtype) -> int:
     return _lib.dtype_code(dt)
 
@@ -136,8 +132,10 @@ def mxfp4_gemm(xq: Mxfp4Matrix, wq: Mxfp4Matrix, bias: Optional[torch.Tensor], o
     if t is not None:
         assert l2t is not None and l2t.dtype == out_dtype and t.dtype in (out_dtype, torch.float32) and l2t.is_contiguous()
         assert t.dim() == 2 and t.stride(1) == 1 and t.shape[0] >= M and tuple(l2t.shape) == (N, t.shape[1]), (tuple(t.shape), tuple(l2t.shape), M, N)
+        t = _rows(_plain(t).float())   # (as the layer's own is)
+        if _stride(t) % 8:
+            t = t.contiguous()
         R, ldt = t.shape[1], _stride(t)
-        code |= _t_flag(t)
     if out is None:
         out = torch.empty((M, N), dtype=out_dtype, device=xq.codes.device)
     assert out.dtype == out_dtype and tuple(out.shape) == (M, N) and out.stride(1) == 1, (out.dtype, tuple(out.shape))
@@ -162,7 +160,7 @@ def mxfp4_grad_input(dy: torch.Tensor, wq: Mxfp4Matrix, dt: Optional[torch.Tenso
         R = dt.shape[1]
         assert lr_Ap is not None and lr_Ap.dtype == dy.dtype and dt.dtype in (dy.dtype, torch.float32) and dt.is_contiguous() and lr_Ap.is_contiguous()
         assert tuple(dt.shape) == (M, R) and tuple(lr_Ap.shape) == (K, R), (tuple(dt.shape), tuple(lr_Ap.shape), M, K)
-        code |= _t_flag(dt)
+        dt = _plain(dt).float()
     dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
     L = _lib.load()
     size = L.pq_mx_grad_input_workspace_size(M, N, K)

@@ -105,3 +105,44 @@ def test_lowrank_grads_checks_both_operands(cuda):
             lowrank_grads(dy, bad, good, q8, q.scales, 8)
         with pytest.raises(AssertionError):
             lowrank_grads(dy, good, bad, q8, q.scales, 8)
+
+
+# ---- infinities and NaNs ------------------------------------------------------------------------------------------
+
+def _same_kind(got, want, what):
+    """NaN, an infinity with its sign, or finite: as want is."""
+    got = got.detach().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: NaN in {int(torch.isnan(got).sum())}, not in {int(torch.isnan(want).sum())} values"
+    assert torch.equal(torch.where(torch.isinf(got), got, 0.0).nan_to_num(0, 1, -1), torch.where(torch.isinf(want), want, 0.0).nan_to_num(0, 1, -1)), what
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("M,K,N,R", [(20, 64, 96, 8), (90, 128, 48, 33), (300, 640, 1040, 64), (2100, 160, 4112, 32), (4128, 2080, 496, 32)])
+def test_infinities_stay_infinities(cuda, dtype, M, K, N, R):
+    """An infinity in x, dy or a factor gives what the formulas give: infinities of the products' signs, NaN where it meets a zero
+    or the other sign. Rows of one or two values make some of t and dt 16-bit values, with nothing left for a second part."""
+    from pyraquant_amd.mxfp4 import checkpoint_values, dequant_mxfp4, quant_mxfp4
+
+    layer, A, B = _layer(K, N, R, dtype, K, weight=0.1, std=0.5)
+    x, dy = _rand(M, K, dtype=dtype, seed=M), _rand(M, N, dtype=dtype, seed=N)
+    x[: M // 2] = torch.where(torch.arange(K, device=cuda) == torch.arange(M // 2, device=cuda).unsqueeze(1) % K, 1.0, 0.0)
+    dy[M // 4 : M // 2] = torch.where(torch.arange(N, device=cuda) == torch.arange(M // 2 - M // 4, device=cuda).unsqueeze(1) % N, -0.5, 0.0)
+    inf = float("inf")
+    for name in ("dy", "x", "A", "B"):
+        v = {"x": x.clone(), "dy": dy.clone(), "A": A.clone(), "B": B.clone()}
+        for i, j, value in ((1, 3, inf), (M // 3, 17, -inf), (M - 1, 40, inf)):
+            rows = v[name].shape[0]
+            v[name][i % rows, j % v[name].shape[1]] = value
+        with torch.no_grad():
+            layer.lr_A.copy_(v["A"])
+            layer.lr_B.copy_(v["B"])
+        xg = v["x"].requires_grad_()
+        y = layer(xg)
+        dx, dA, dB = torch.autograd.grad(y, [xg, layer.lr_A, layer.lr_B], v["dy"])
+        q, q8 = quant_mxfp4(v["x"].detach(), checkpoint=True)
+        X, D, a, b, w = v["x"].detach().double(), v["dy"].double(), v["A"].double(), v["B"].double(), layer.weight(torch.float32).double()
+        t, dt = X @ a, D @ b.t()
+        want = {"y": dequant_mxfp4(q, torch.float32).double() @ w.t() + t @ b, "dx": D @ w + dt @ a.t(),
+                "dA": checkpoint_values(q8, q, torch.float32).double().t() @ dt, "dB": t.t() @ D}
+        for k, got in (("y", y), ("dx", dx), ("dA", dA), ("dB", dB)):
+            _same_kind(got, want[k], f"{k} of an infinite {name}")
