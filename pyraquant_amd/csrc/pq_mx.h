@@ -213,28 +213,81 @@ __device__ __forceinline__ v16f mfma16(v4i a, v4i b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// Eight consecutive ranks of a row of t (or dt), operand of a low-rank product: the values, and their two parts.
+// fp16 ends at 65504, and t and dt may go past it where the results do not. Values of a row (of a column, where sums run over
+// rows) whose largest magnitude is 2^16 or more are taken times 2^-e, so that it falls below 2^16, and the sums that they join times
+// 2^-e before and 2^e after: no bit changes. 2^-e from that largest magnitude's bits (2^-113 for an infinity: its sums are no numbers).
+__device__ __forceinline__ float scale_down(uint32_t bits) {
+  const int e = max((int)(bits >> 23) - 127 - 15, 0);
+  return __uint_as_float((uint32_t)(127 - min(e, 113)) << 23);
+}
+__device__ __forceinline__ float scale_back(float down) { return __uint_as_float(0x7f000000u - __float_as_uint(down)); }   // 1 / down
+
+// Eight consecutive ranks of a row of t (or dt), lane % 32 of which is the operand of a low-rank product: lanes l and l + 32 hold
+// the 16 ranks of a step.
 struct RankPiece {
   v4f raw[2];
   __device__ __forceinline__ void load(const float* at) {
     raw[0] = reinterpret_cast<const v4f*>(at)[0];
     raw[1] = reinterpret_cast<const v4f*>(at)[1];
   }
-  template <int DT>
-  __device__ __forceinline__ void parts(v4i& hi, v4i& lo) const {
+  __device__ __forceinline__ float largest() const {
+    float m = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      uint32_t h, l;
-      two_parts<DT>(raw[e >> 1][2 * (e & 1)], raw[e >> 1][2 * (e & 1) + 1], h, l);
-      hi[e] = (int)h;
-      lo[e] = (int)l;
-    }
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(raw[e >> 2][e & 3]));
+    return m;
   }
 };
-// y += l t^T over the 16 ranks of a piece
+struct RankParts {
+  v4i hi, lo;
+};
 template <int DT>
-__device__ __forceinline__ v16f rank_product(v4i l, v4i hi, v4i lo, v16f y) {
-  return mfma16<DT>(l, hi, mfma16<DT>(l, lo, y));
+__device__ __forceinline__ RankParts parts_of(const RankPiece& p) {
+  RankParts t;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t h, l;
+    two_parts<DT>(p.raw[e >> 1][2 * (e & 1)], p.raw[e >> 1][2 * (e & 1) + 1], h, l);
+    t.hi[e] = (int)h;
+    t.lo[e] = (int)l;
+  }
+  return t;
+}
+// acc[i] += l_i t^T for NI tiles of 32 x 32 whose rows (lane % 32) are the pieces' and for NP pieces; l(i, s): the other operand.
+// Where some row's values are far (rare) its pieces and sums are scaled.
+template <int DT, int NI, int NP, typename L>
+__device__ __forceinline__ void rank_products(v16f* const (&acc)[NI], RankPiece (&piece)[NP], L l) {
+  bool far = false;
+  float down = 1.0f;
+  auto scale = [&](float by) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) (*acc[i])[e] *= by;
+  };
+  if constexpr (DT == PQ_F16) {
+    float m = piece[0].largest();
+#pragma unroll
+    for (int s = 1; s < NP; ++s) m = fmaxf(m, piece[s].largest());
+    far = __ballot(m >= 65536.0f) != 0;
+    if (far) {
+      down = scale_down(__float_as_uint(fmaxf(m, __shfl_xor(m, 32))));
+#pragma unroll
+      for (int s = 0; s < NP; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) piece[s].raw[e >> 2][e & 3] *= down;
+      scale(down);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < NP; ++s) {
+    const RankParts t = parts_of<DT>(piece[s]);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const v4i a = l(i, s);
+      *acc[i] = mfma16<DT>(a, t.hi, mfma16<DT>(a, t.lo, *acc[i]));
+    }
+  }
+  if (DT == PQ_F16 && far) scale(scale_back(down));
 }
 
 // Workgroup id -> (tile_m, tile_n): ids are dealt round-robin over the 8 XCDs, so each XCD takes a contiguous run of the

@@ -221,16 +221,14 @@ void mx_gemm_kernel(const GemmArgs p) {
   for (int j = 0; j < TJ; ++j) {
     if constexpr (R > 0) {
 #pragma unroll
-      for (int s = 0; s < R / 16; ++s) {
-        RankPiece t;
-        v4i hi, lo;
-        t.load(p.t + (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + 16 * s + 8 * half);
-        t.parts<DT>(hi, lo);
+      for (int r0 = 0; r0 < R; r0 += 32) {
+        RankPiece t[2];
 #pragma unroll
-        for (int i = 0; i < TI; ++i) {
-          const v4i l = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(nb + 32 * i + l32, p.N - 1) * R + 16 * s + 8 * half);
-          acc[i][j] = rank_product<DT>(l, hi, lo, acc[i][j]);
-        }
+        for (int s = 0; s < 2; ++s) t[s].load(p.t + (int64_t)min(mb + 32 * j + l32, p.M - 1) * p.ldt + r0 + 16 * s + 8 * half);
+        static_assert(TI == 2, "tiles of a wave");
+        rank_products<DT, TI, 2>({&acc[0][j], &acc[1][j]}, t, [&](int i, int s) {
+          return *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(nb + 32 * i + l32, p.N - 1) * R + r0 + 16 * s + 8 * half);
+        });
       }
     }
 #pragma unroll
@@ -428,9 +426,7 @@ void mx_gemm_large_kernel(const GemmArgs p) {
 
     // Lane l holds, of tile (i, j): row m = 32 j + l % 32, outputs n = 32 i + 8 q + 4 (l / 32) .. + 3 in elements 4 q ..
     const int nb = n0 + wn * (BN / 2), mb = m0 + wm * (BM / 4);
-    const auto rs_c = __builtin_amdgcn_make_buffer_rsrc((void*)(p.c + (int64_t)m0 * p.ldc + n0), (short)0,
-                                                        ((min(BM, p.M - m0) - 1) * p.ldc + min(BN, p.N - n0)) * 2, kBufferWord3);
-    const int valid_n = p.N - n0;
+    const int m_out = m0, n_out = n0;
     const int next = tile + (int)gridDim.x;
     const bool more = next < tiles;
     auto go_on = [&] {
@@ -456,18 +452,15 @@ void mx_gemm_large_kernel(const GemmArgs p) {
         }
         if (r0 + 32 == R) go_on();
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int j = 0; j < TJ; ++j) {
-            v4i hi, lo;
-            tv[j][x].template parts<DT>(hi, lo);
-#pragma unroll
-            for (int i = 0; i < TI; ++i) acc[i][j] = rank_product<DT>(lv[i][x], hi, lo, acc[i][j]);
-          }
+        for (int j = 0; j < TJ; ++j)
+          rank_products<DT, TI, 2>({&acc[0][j], &acc[1][j], &acc[2][j], &acc[3][j]}, tv[j], [&](int i, int x) { return lv[i][x]; });
       }
     } else {
       go_on();
     }
+    const int valid_n = p.N - n_out;
+    const auto rs_c = __builtin_amdgcn_make_buffer_rsrc((void*)(p.c + (int64_t)m_out * p.ldc + n_out), (short)0,
+                                                        ((min(BM, p.M - m_out) - 1) * p.ldc + min(BN, valid_n)) * 2, kBufferWord3);
     uint8_t* const out = smem + AT_STAGING + wave * 16 * PITCH;
 #pragma unroll
     for (int j = 0; j < TJ; ++j)
@@ -630,13 +623,13 @@ __global__ __launch_bounds__(64 * NW) void mx_gemm_split_kernel(const SplitArgs 
         const int m = m0 + 32 * j + l32;
         if constexpr (R > 0) {
 #pragma unroll
-          for (int s = 0; s < R / 16; ++s) {
-            const v4i l = *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(n0 + 32 * i + l32, p.N - 1) * R + 16 * s + 8 * half);
-            RankPiece t;
-            v4i hi, lo;
-            t.load(p.t + (int64_t)min(m, p.M - 1) * p.ldt + 16 * s + 8 * half);
-            t.parts<DT>(hi, lo);
-            y = rank_product<DT>(l, hi, lo, y);
+          for (int r0 = 0; r0 < R; r0 += 32) {
+            RankPiece t[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) t[s].load(p.t + (int64_t)min(m, p.M - 1) * p.ldt + r0 + 16 * s + 8 * half);
+            rank_products<DT, 1, 2>({&y}, t, [&](int, int s) {
+              return *reinterpret_cast<const v4i*>(p.l2t + (int64_t)min(n0 + 32 * i + l32, p.N - 1) * R + r0 + 16 * s + 8 * half);
+            });
           }
         }
 #pragma unroll

@@ -46,26 +46,20 @@ struct DxArgs {
   int slice;
 };
 
-// dx += dt A^T: row m of dt (that of lane % 32), then tiles of 32 columns k (from kk) x 32 rows
-template <int DT, int R>
-struct LowRank {
-  v4i hi[R ? R / 16 : 1], lo[R ? R / 16 : 1];
-  __device__ __forceinline__ LowRank(const DxArgs& p, int m, int lane) {
-    RankPiece t[R ? R / 16 : 1];
+// dx += dt A^T for NI tiles of 32 columns k (from kk on) x 32 rows, lane % 32 of which is m
+template <int DT, int R, int NI>
+__device__ __forceinline__ void add_low_rank(const DxArgs& p, int kk, int m, int lane, v16f* const (&acc)[NI]) {
 #pragma unroll
-    for (int s = 0; s < R / 16; ++s) t[s].load(p.dt + (int64_t)min(m, p.M - 1) * R + 16 * s + 8 * (lane >> 5));
+  for (int r0 = 0; r0 < R; r0 += 32) {
+    const int r = r0 + 8 * (lane >> 5);
+    RankPiece t[2];
 #pragma unroll
-    for (int s = 0; s < R / 16; ++s) t[s].template parts<DT>(hi[s], lo[s]);
+    for (int s = 0; s < 2; ++s) t[s].load(p.dt + (int64_t)min(m, p.M - 1) * R + r + 16 * s);
+    rank_products<DT, NI, 2>(acc, t, [&](int i, int s) {
+      return *reinterpret_cast<const v4i*>(p.ap + (int64_t)min(kk + 32 * i + (lane & 31), p.K - 1) * R + r + 16 * s);
+    });
   }
-  __device__ __forceinline__ v16f add(const DxArgs& p, int kk, int lane, v16f acc) const {
-#pragma unroll
-    for (int s = 0; s < R / 16; ++s) {
-      const v4i a = *reinterpret_cast<const v4i*>(p.ap + (int64_t)min(kk + (lane & 31), p.K - 1) * R + 16 * s + 8 * (lane >> 5));
-      acc = rank_product<DT>(a, hi[s], lo[s], acc);
-    }
-    return acc;
-  }
-};
+}
 
 // Few blocks: a workgroup of four waves takes 64 rows m x 128 columns k (one stage of the packed weight), 64 n a step. dy and
 // the 4-bit weights of the next two steps are on their way into registers while the products of this one run, then go to the
@@ -148,7 +142,7 @@ __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
 #pragma unroll
   for (int j = 0; j < TJ; ++j) {
     const int m = m0 + wm + 32 * j + l32;
-    const LowRank<DT, SPLIT ? 0 : R> low(p, m, lane);
+    if constexpr (!SPLIT) add_low_rank<DT, R, 2>(p, k0 + wk, m, lane, {&acc[0][j], &acc[1][j]});
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int kk = k0 + wk + 32 * i;
@@ -161,7 +155,6 @@ __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
         }
         continue;
       }
-      acc[i][j] = low.add(p, kk, lane, acc[i][j]);
       if (m < p.M && kk < p.K) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -191,7 +184,7 @@ __global__ __launch_bounds__(256) void mx_dx_join_kernel(const DxArgs p, int sli
       }
     }
   }
-  acc = LowRank<DT, R>(p, m, lane).add(p, kk, lane, acc);
+  add_low_rank<DT, R, 1>(p, kk, m, lane, {&acc});
   if (m < p.M) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -437,13 +430,13 @@ void mx_dx_ring_kernel(const DxArgs p) {
   uint8_t* const stage = smem + wave * 32 * T::PITCH;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const LowRank<DT, R> low(p, mb + 32 * j + l32, lane);
+    add_low_rank<DT, R, 4>(p, kb0, mb + 32 * j + l32, lane, {&acc[0][j], &acc[1][j], &acc[2][j], &acc[3][j]});
 #pragma unroll
     for (int ih = 0; ih < 2; ++ih) {
 #pragma unroll
       for (int ii = 0; ii < 2; ++ii) {
         const int i = 2 * ih + ii;
-        const v16f y = low.add(p, kb0 + 32 * i, lane, acc[i][j]);
+        const v16f& y = acc[i][j];
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<v2u*>(stage + l32 * T::PITCH + (ii * 32 + 8 * q + 4 * half) * 2) =
@@ -479,7 +472,7 @@ struct SumArgs {
 };
 
 template <int DT, int R, bool EIGHT, bool COLS>
-__device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* sz, uint8_t* sv) {
+__device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* sz, uint8_t* sv, uint32_t* top) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int slice = block / p.panels, panel = block - slice * p.panels;
   const int c0 = panel * 128, s0 = slice * p.rows;
@@ -521,7 +514,37 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
   };
   load(s0);
   for (int m0 = s0; m0 < end; m0 += 64) {
+    bool far = false;   // some value of v is 2^16 or more (fp16: scale_down); the waves tell each other in top[0 .. 3]
+    if constexpr (DT == PQ_F16) {
+      float m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < R / 16; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(vr[i][e]));
+      top[wave] = __ballot(m >= 65536.0f) != 0;
+    }
     __syncthreads();
+    if constexpr (DT == PQ_F16) {
+      const v4u all = *reinterpret_cast<const v4u*>(top);
+      far = __builtin_amdgcn_readfirstlane((int)(all[0] | all[1] | all[2] | all[3])) != 0;
+      if (far) {   // rare: the largest magnitude of each rank's 64 values, in top[4 ..]
+        if (tid < R) top[4 + tid] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < R / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) atomicMax(&top[4 + (i * 256 + tid) % (R / 4) * 4 + e], __float_as_uint(vr[i][e]) & 0x7fffffffu);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < R / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vr[i][e] *= scale_down(top[4 + (i * 256 + tid) % (R / 4) * 4 + e]);
+#pragma unroll
+        for (int j = 0; j < R / 32; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[j][e] *= scale_down(top[4 + 32 * j + (lane & 31)]);
+      }
+    }
     if constexpr (EIGHT) {
       const int row = tid >> 2, b = tid & 3;
       const float s = restore_scale(byte);   // (past the end the codes are zeros)
@@ -559,6 +582,12 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
       }
       if constexpr (COLS) cols = mfma16<DT>(z, ones, cols);
     }
+    if (DT == PQ_F16 && far) {
+#pragma unroll
+      for (int j = 0; j < R / 32; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[j][e] *= scale_back(scale_down(top[4 + 32 * j + (lane & 31)]));
+    }
   }
   // lane: r = 32 j + lane % 32, columns c0 + 32 wave + 8 q + 4 (lane / 32) + e
   const int c = c0 + wave * 32 + 4 * (lane >> 5);
@@ -581,8 +610,9 @@ template <int DT, int R, bool COLS>
 __global__ __launch_bounds__(256) void mx_rowsum_kernel(const SumArgs b, const SumArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t sz[64 * 256];      // [m][128 c]
   __shared__ __attribute__((aligned(16))) uint8_t sv[2 * 64 * R * 2];   // [2][m][R]
-  if ((int)blockIdx.x < b.blocks) row_sums<DT, R, false, COLS>(b, blockIdx.x, sz, sv);
-  else row_sums<DT, R, true, false>(a, blockIdx.x - b.blocks, sz, sv);
+  __shared__ __attribute__((aligned(16))) uint32_t top[4 + R];
+  if ((int)blockIdx.x < b.blocks) row_sums<DT, R, false, COLS>(b, blockIdx.x, sz, sv, top);
+  else row_sums<DT, R, true, false>(a, blockIdx.x - b.blocks, sz, sv, top);
 }
 
 // The slices' sums added in order, rounded to 16 bits: dB [R, N] and dA [K, R]; and the column sums in 32. A thread sums one

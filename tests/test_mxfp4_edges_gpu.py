@@ -146,3 +146,57 @@ def test_infinities_stay_infinities(cuda, dtype, M, K, N, R):
                 "dA": checkpoint_values(q8, q, torch.float32).double().t() @ dt, "dB": t.t() @ D}
         for k, got in (("y", y), ("dx", dx), ("dA", dA), ("dB", dB)):
             _same_kind(got, want[k], f"{k} of an infinite {name}")
+
+
+# ---- past the end of fp16 -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("M,K,N,R", [(20, 64, 96, 8), (90, 128, 48, 33), (300, 640, 1040, 64), (2100, 160, 4112, 32), (4128, 2080, 496, 32),
+                                     (329, 4320, 2512, 40), (600, 1056, 7056, 64)])
+@pytest.mark.parametrize("which", ("t", "dt"))
+def test_low_rank_values_past_fp16(cuda, which, M, K, N, R):
+    """x A (or dy B^T) of some 10^5 to 10^7 in most rows and of 1 in others, results inside fp16: they are as exact as elsewhere. A
+    row's (in sums over rows, a rank's) values share a scale, so that 2^-25 of 2^15 below its largest may be missing."""
+    from pyraquant_amd.mxfp4 import checkpoint_values, quant_mxfp4
+
+    dtype, u, tiny = torch.float16, U[torch.float16], 2.0 ** -25
+    large, small = 16000.0, 1e-3 / R ** 0.5
+    g = torch.Generator().manual_seed(K)
+    layer, *_ = _layer(K, N, R, dtype, 1)
+    A = (torch.randn(K, R, generator=g) * (large / K ** 0.5 if which == "t" else small)).half().cuda()
+    B = (torch.randn(R, N, generator=g) * (small if which == "t" else large / N ** 0.5)).half().cuda()
+    with torch.no_grad():
+        layer.lr_A.copy_(A)
+        layer.lr_B.copy_(B)
+    x, dy = (torch.randn(M, n, generator=g) for n in (K, N))
+    far, near = (x, dy) if which == "t" else (dy, x)
+    far *= 30.0
+    far[::8] *= 10.0
+    far[3::8] *= 1e-5
+    near *= 0.002 / M ** 0.5
+    x, dy = x.half().cuda().requires_grad_(), dy.half().cuda()
+    y = layer(x)
+    dx, dA, dB = torch.autograd.grad(y, [x, layer.lr_A, layer.lr_B], dy)
+    q, q8 = quant_mxfp4(x.detach(), checkpoint=True)
+    X, D, a, b = x.detach().double(), dy.double(), A.double(), B.double()
+    xt = checkpoint_values(q8, q, torch.float32).double()
+
+    def through(X, a, b):     # (X a) b and its bound, X a and its bounds as rows and as columns share scales
+        t = X @ a
+        lost = X.shape[1] * F * (X.abs() @ a.abs())
+        off = [lost + u * u * (t.abs() + lost) + tiny * (t.abs().amax(d, keepdim=True) * 2.0 ** -15).clamp_min(1) for d in (1, 0)]
+        want = t @ b
+        bound = off[0] @ b.abs() + 2 * (R + 2) * F * ((t.abs() + off[0]) @ b.abs())
+        return want, bound + u * (want.abs() + bound) + tiny, t, off[1]
+
+    def summed(z, t, off):    # z^T t
+        want, bound = z.t() @ t, z.abs().t() @ off + 2 * M * F * (z.abs().t() @ (t.abs() + off))
+        return want, bound + u * (want.abs() + bound) + tiny
+
+    y_want, y_bound, t, t_off = through(X, a, b)
+    dx_want, dx_bound, dt, dt_off = through(D, b.t(), a.t())
+    assert float((t if which == "t" else dt).abs().max()) > 1e6 and float(torch.stack([v.abs().max() for v in (y_want, dx_want)]).max()) < 6e4
+    _within(y.detach(), y_want, y_bound, "y")
+    _within(dx, dx_want, dx_bound, "dx")
+    _within(dA, *summed(xt, dt, dt_off), "dA")
+    want, bound = summed(D, t, t_off)
+    _within(dB, want.t(), bound.t(), "dB")
