@@ -18,6 +18,8 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/pyraquant_amd.h"
@@ -181,7 +183,24 @@ struct Layer : torch::autograd::Function<Layer> {
     } catch (const Refused& r) {
       throw std::runtime_error(r.text);
     }
+    if (at::GradMode::is_enabled()) once(out, grads[0], P != 0);
     return out;
+  }
+
+  // The gradients of a pass with create_graph: each gets edges to what it depends on by the formulas, through a node that raises. (What
+  // the kernels write has no history: without this it would count as a constant wherever it is differentiated.)
+  static void once(variable_list& out, const Tensor& dy, bool branch) {
+    const torch::autograd::edge_list& inputs = torch::autograd::get_current_node()->next_edges();   // x, lr_A and lr_B, bias
+    const torch::autograd::Edge none, x = inputs[0], A = branch ? inputs[1] : none, B = branch ? inputs[2] : none;
+    const torch::autograd::Edge back = dy.requires_grad() ? torch::autograd::impl::gradient_edge(dy) : none;
+    const torch::autograd::edge_list on[4] = {{back, A, B}, {back, B, x}, {back, A, x}, {back}};   // dx, dlr_A, dlr_B, dbias
+    for (int i = 0; i < 4; ++i) {
+      torch::autograd::edge_list edges;
+      for (const auto& e : on[i])
+        if (e.is_valid()) edges.push_back(e);
+      if (out[i].defined() && !edges.empty())
+        torch::autograd::set_history(out[i], std::make_shared<torch::autograd::Error>("the 4-bit layers have no second derivatives", std::move(edges)));
+    }
   }
 };
 

@@ -200,3 +200,39 @@ def test_low_rank_values_past_fp16(cuda, which, M, K, N, R):
     _within(dA, *summed(xt, dt, dt_off), "dA")
     want, bound = summed(D, t, t_off)
     _within(dB, want.t(), bound.t(), "dB")
+
+
+# ---- autograd beyond a first derivative ---------------------------------------------------------------------------
+
+def test_second_derivatives_raise(cuda):
+    """A pass with create_graph gives the same gradients, and differentiating one that depends on what requires a gradient raises:
+    never a sum in which this layer's part is missing."""
+    dtype = torch.bfloat16
+    layer, *_ = _layer(64, 32, 8, dtype, 1, weight=0.1, bias=True)
+    x0, scale, dy = _rand(5, 64, dtype=dtype, seed=1), _rand(64, dtype=dtype, seed=2).requires_grad_(), _rand(5, 32, dtype=dtype, seed=3)
+    wanted = lambda x: [x, layer.lr_A, layer.lr_B, layer.bias]   # noqa: E731
+    x = x0.clone().requires_grad_()
+    first = torch.autograd.grad(layer(x), wanted(x), dy)
+    grads = torch.autograd.grad(layer(x), wanted(x), dy, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, grads))
+    on = {0: [1, 2], 1: [0, 2], 2: [0, 1], 3: []}      # what each depends on (dy, too, which requires none here)
+    for i, g in enumerate(grads):
+        assert g.requires_grad == bool(on[i])
+        for j in on[i]:
+            with pytest.raises(RuntimeError, match="second derivatives"):
+                torch.autograd.grad(g.float().square().sum() + wanted(x)[j].float().sum(), wanted(x)[j], retain_graph=True)
+    # a gradient penalty through an operation before the layer: the sum of both losses
+    y = layer(x * scale)
+    dx, = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+    for wrt in (None, [scale], [x, layer.lr_A]):
+        loss = y.float().sum() + dx.float().square().sum()
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            loss.backward(retain_graph=True) if wrt is None else torch.autograd.grad(loss, wrt, retain_graph=True)
+    # nothing that requires a gradient besides x: dx is a constant, and a gradient of dy makes it none
+    frozen, *_ = _layer(64, 32, 8, dtype, 1, weight=0.1, trainable=False)
+    y = frozen(x)
+    assert not torch.autograd.grad(y, x, dy, create_graph=True)[0].requires_grad
+    d = dy.clone().requires_grad_()
+    dx, = torch.autograd.grad(frozen(x), x, d, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(dx.float().sum(), d)
