@@ -264,6 +264,11 @@ PyObject* layer(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     PyErr_SetString(PyExc_AssertionError, text);
     return nullptr;
   }
+  for (const Tensor* t : {&x, &A, &B, &bias})
+    if (t->defined() && t->_fw_grad(0).defined()) {
+      PyErr_SetString(PyExc_RuntimeError, "the 4-bit layers have no forward-mode derivatives");
+      return nullptr;
+    }
   Tensor y;
   int status = PQ_OK;
   std::string text;

@@ -236,3 +236,26 @@ def test_second_derivatives_raise(cuda):
     dx, = torch.autograd.grad(frozen(x), x, d, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivatives"):
         torch.autograd.grad(dx.float().sum(), d)
+
+
+def test_forward_mode_tangents_raise(cuda):
+    """A tangent of x, of a factor or of the bias is never dropped, with or without gradients of the reverse kind."""
+    import torch.autograd.forward_ad as fwd
+
+    for trainable in (True, False):
+        layer, *_ = _layer(64, 32, 8, torch.bfloat16, 1, weight=0.1, bias=True, trainable=trainable)
+        x = _rand(5, 64, dtype=torch.bfloat16, seed=1)
+        want = layer(x)
+        with fwd.dual_level():
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    layer(fwd.make_dual(x, torch.ones_like(x)))
+            if not trainable:
+                for name in ("bias", "lr_Af", "lr_Bt"):
+                    kept = layer._buffers[name]
+                    layer._buffers[name] = fwd.make_dual(kept, torch.ones_like(kept))
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        layer(x)
+                    layer._buffers[name] = kept
+            assert torch.equal(layer(x), want)
+        assert torch.equal(layer(x), want)
