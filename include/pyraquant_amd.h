@@ -455,9 +455,10 @@ int pq_mx_grad_input(const void* dy, int32_t dtype, int64_t lddy, const uint8_t*
 /*
  * The gradients of the low-rank factors and the bias: dB[r, n] = sum_m t[m, r] dy[m, n] ([R, N]), dA[k, r] = sum_m xt[m, k]
  * dt[m, r] ([K, R], xt: the values of the checkpoint q8 with x_scales), dbias[n] = sum_m dy[m, n] (fp32). An output that is
- * NULL is not computed, and what only it needs (dy and t for dB and dbias; dt, q8 and x_scales for dA) may be NULL too. t and
+ * NULL is not computed, and what only it needs (dy for dB and dbias, t for dB; dt, q8 and x_scales for dA) may be NULL too. t and
  * dt are [M, P] in fp32, as pq_mx_lowrank_down gives them, zero past rank R, and taken to twice dtype's bits. Sums in fp32, in an
- * order that depends on the sizes alone; dA and dB rounded to dtype. The workspace (pq_mx_grad_factors_workspace_size bytes) may hold anything.
+ * order that depends on the sizes alone; dA and dB rounded to dtype. The workspace (pq_mx_grad_factors_workspace_size bytes) may
+ * hold anything.
  */
 int64_t pq_mx_grad_factors_workspace_size(int64_t M, int64_t K, int64_t N, int64_t P);
 int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, const float* t, const float* dt, const int8_t* q8,

@@ -457,9 +457,9 @@ void mx_dx_ring_kernel(const DxArgs p) {
 }
 
 // ---- sums over rows: part[s][r][c] = sum over the rows of slice s of v[m, r] z[m, c] -------------------------------------
-// z is dy (EIGHT false) or the 8-bit codes of x with their scales; v is t or dt, [M, R] in fp32. Column sums of z too (COLS). A
-// workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step, the next step's rows on their way into
-// registers meanwhile; the order of the sums is fixed. Bound by reading z: 460 MB of 16384 x 3072 x 12288 in 92 us, 5.0 TB/s
+// z is dy (EIGHT false) or the 8-bit codes of x with their scales; v is t or dt, [M, R] in fp32. Column sums of z too
+// (COLS), and these alone where v is NULL. A workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step, the
+// next step's rows on their way into registers meanwhile; the order of the sums is fixed. Bound by reading z: 460 MB of 16384 x 3072 x 12288 in 92 us, 5.0 TB/s
 // (87 with the first part of v alone; results' errors then grow by 1.4).
 struct SumArgs {
   const void* z;
@@ -509,7 +509,7 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
     for (int i = 0; i < R / 16; ++i) {
       const int at = i * 256 + tid, m = m0 + at / (R / 4);
       vr[i] = v4f{};
-      if (m < end) vr[i] = *reinterpret_cast<const v4f*>(p.v + (int64_t)m * R + at % (R / 4) * 4);
+      if (p.v && m < end) vr[i] = *reinterpret_cast<const v4f*>(p.v + (int64_t)m * R + at % (R / 4) * 4);
     }
   };
   load(s0);
@@ -575,10 +575,12 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const v4i z = read_columns(z_at, 16 * s, wave * 32, lane);
+      if (p.v) {
 #pragma unroll
-      for (int j = 0; j < R / 32; ++j) {
-        acc[j] = mfma16<DT>(z, read_columns(hi_at, 16 * s, 32 * j, lane), acc[j]);
-        acc[j] = mfma16<DT>(z, read_columns(lo_at, 16 * s, 32 * j, lane), acc[j]);
+        for (int j = 0; j < R / 32; ++j) {
+          acc[j] = mfma16<DT>(z, read_columns(hi_at, 16 * s, 32 * j, lane), acc[j]);
+          acc[j] = mfma16<DT>(z, read_columns(lo_at, 16 * s, 32 * j, lane), acc[j]);
+        }
       }
       if constexpr (COLS) cols = mfma16<DT>(z, ones, cols);
     }
@@ -595,10 +597,12 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     if (c + 8 * q >= p.C) break;
+    if (p.v) {
 #pragma unroll
-    for (int j = 0; j < R / 32; ++j)
-      *reinterpret_cast<v4f*>(p.part + ((int64_t)slice * R + 32 * j + (lane & 31)) * p.C + c + 8 * q) =
-          v4f{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
+      for (int j = 0; j < R / 32; ++j)
+        *reinterpret_cast<v4f*>(p.part + ((int64_t)slice * R + 32 * j + (lane & 31)) * p.C + c + 8 * q) =
+            v4f{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
+    }
     if (COLS && (lane & 31) == 0)
       *reinterpret_cast<v4f*>(p.part_cols + (int64_t)slice * p.C + c + 8 * q) =
           v4f{cols[4 * q], cols[4 * q + 1], cols[4 * q + 2], cols[4 * q + 3]};
@@ -797,7 +801,7 @@ extern "C" int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, c
     return set_error(PQ_ESHAPE, "pq_mx_grad_factors: M=%lld N=%lld K=%lld R=%lld P=%lld", (long long)M, (long long)N,
                      (long long)K, (long long)R, (long long)P);
   if (dtype != PQ_BF16 && dtype != PQ_F16) return set_error(PQ_EDTYPE, "pq_mx_grad_factors: dtype %d", dtype);
-  if (((dB || dbias) && (!dy || !t)) || (dA && (!dt || !q8 || !x_scales)) || !workspace)
+  if (((dB || dbias) && !dy) || (dB && !t) || (dA && (!dt || !q8 || !x_scales)) || !workspace)
     return set_error(PQ_EINVAL, "pq_mx_grad_factors: null pointer");
   if ((uintptr_t)dy % 16 || lddy % 8 || (uintptr_t)t % 16 || (uintptr_t)dt % 16 || (uintptr_t)q8 % 16 || (uintptr_t)workspace % 16)
     return set_error(PQ_EALIGN, "pq_mx_grad_factors: operands 16-byte aligned, lddy a multiple of 8");
@@ -809,7 +813,7 @@ extern "C" int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, c
   float* const part_a = part + (int64_t)sb * (P + 1) * N;
   const int pb = (int)((N + 127) / 128), pk = (int)((K + 127) / 128);
   const bool want_b = dB || dbias, want_a = dA != nullptr;
-  const mx::SumArgs b{dy, nullptr, t, part, part + (int64_t)sb * P * N, lddy, (int)M, (int)N, 0,
+  const mx::SumArgs b{dy, nullptr, dB ? t : nullptr, part, part + (int64_t)sb * P * N, lddy, (int)M, (int)N, 0,
                       rows(sb), pb, want_b ? pb * sb : 0};
   const mx::SumArgs a{q8, x_scales, dt, part_a, nullptr, K, (int)M, (int)K, mx::stages(K), rows(sk),
                       pk, want_a ? pk * sk : 0};

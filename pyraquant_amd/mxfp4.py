@@ -188,20 +188,29 @@ def lowrank_grads(dy: Optional[torch.Tensor], t: Optional[torch.Tensor], dt: Opt
     them. What no wanted gradient needs may be None; without a dy, fp32 dt gives dA in bf16."""
     if not (want_A or want_B or want_bias):
         return None, None, None
-    ref = dt if want_A else t
     _check_cuda(dy, t, dt, q8, x_scales)
-    M, P = ref.shape[-2:]
-    dev = ref.device
-    dt16 = dy.dtype if want_B or want_bias else ref.dtype if ref.dtype != torch.float32 else torch.bfloat16
+    if not want_A:
+        dt = q8 = x_scales = None
+    if not want_B:
+        t = None
+    if not (want_B or want_bias):
+        dy = None
+    for wanted, operands in ((want_A, (dt, q8, x_scales)), (want_B, (dy, t)), (want_bias, (dy,))):
+        assert not wanted or all(v is not None for v in operands), "an operand of a wanted gradient is None"
+    ranks = dt if want_A else t
+    P = _padded_rank(rank) if ranks is None else ranks.shape[-1]
+    M, dev = (q8 if want_A else dy).shape[0], (q8 if want_A else dy).device
+    dt16 = dy.dtype if dy is not None else dt.dtype if dt.dtype != torch.float32 else torch.bfloat16
     code = _dtype16(dt16)
     K = N = BLOCK
     if want_A:
         dt = _ranks(dt, M, P, dt16)
-        assert q8.dtype == torch.int8 and q8.is_contiguous() and q8.shape[0] == M
+        assert q8.dim() == 2 and q8.dtype == torch.int8 and q8.is_contiguous(), (q8.dtype, tuple(q8.shape))
         K = q8.shape[1]
         assert x_scales.dtype == torch.uint8 and x_scales.numel() >= _stages(M, K) * 64
-    if want_B or want_bias:
+    if want_B:
         t = _ranks(t, M, P, dt16)
+    if dy is not None:
         assert dy.dim() == 2 and dy.shape[0] == M, (tuple(dy.shape), M)
         dy = _rows(dy)
         N = dy.shape[1]
@@ -213,7 +222,7 @@ def lowrank_grads(dy: Optional[torch.Tensor], t: Optional[torch.Tensor], dt: Opt
         return tuple(None if g is None else g.zero_() for g in (dA, dB, db))
     L = _lib.load()
     ws = torch.empty(L.pq_mx_grad_factors_workspace_size(M, K, N, P), dtype=torch.uint8, device=dev)
-    _lib.check(L.pq_mx_grad_factors(_lib.ptr(dy), code, _stride(dy) if want_B or want_bias else N, _lib.ptr(t), _lib.ptr(dt),
+    _lib.check(L.pq_mx_grad_factors(_lib.ptr(dy), code, N if dy is None else _stride(dy), _lib.ptr(t), _lib.ptr(dt),
                                     _lib.ptr(q8), _lib.ptr(x_scales), M, K, N, rank, P, _lib.ptr(dA), _lib.ptr(dB),
                                     _lib.ptr(db), _lib.ptr(ws), ws.numel(), _lib.stream_of(dev)), "lowrank_grads")
     return dA, dB, db

@@ -259,3 +259,31 @@ def test_forward_mode_tangents_raise(cuda):
                     layer._buffers[name] = kept
             assert torch.equal(layer(x), want)
         assert torch.equal(layer(x), want)
+
+
+# ---- every choice of operands -------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_lowrank_grads_of_every_choice(cuda, dtype):
+    """Each choice of what is wanted, with None for what it does not need: the values that all of them together have."""
+    from pyraquant_amd.mxfp4 import lowrank_grads, quant_mxfp4
+
+    M, K, N, rank = 150, 96, 80, 20
+    dy, (q, q8) = _rand(M, N, dtype=dtype, seed=1), quant_mxfp4(_rand(M, K, dtype=dtype, seed=2), checkpoint=True)
+    t, dt = (torch.nn.functional.pad(_rand(M, rank, dtype=torch.float32, seed=s), (0, 12)) for s in (3, 4))
+    parts = torch.stack([dt.to(dtype), (dt - dt.to(dtype).float()).to(dtype)])
+    dt = parts[0].float() + parts[1].float()
+    every = lowrank_grads(dy, t, dt, q8, q.scales, rank)
+    want = dy.double().sum(0)
+    assert bool(((every[2].double() - want).abs() <= M * F * dy.double().abs().sum(0)).all())
+    for A in (False, True):
+        for B in (False, True):
+            for b in (False, True):
+                # (without a dy the type of the results is that of dt's parts)
+                got = lowrank_grads(dy if B or b else None, t if B else None, (dt if B or b else parts) if A else None, q8 if A else None,
+                                    q.scales if A else None, rank, A, B, b)
+                for g, e, w in zip(got, every, (A, B, b)):
+                    assert (g is None) == (not w) and (g is None or (g.dtype == e.dtype and torch.equal(g, e))), (A, B, b)
+    for missing in range(5):
+        with pytest.raises(AssertionError):
+            lowrank_grads(*[None if i == missing else v for i, v in enumerate((dy, t, dt, q8, q.scales))], rank)
