@@ -207,7 +207,7 @@ def lowrank_grads(dy: Optional[torch.Tensor], t: Optional[torch.Tensor], dt: Opt
         dt = _ranks(dt, M, P, dt16)
         assert q8.dim() == 2 and q8.dtype == torch.int8 and q8.is_contiguous(), (q8.dtype, tuple(q8.shape))
         K = q8.shape[1]
-        assert x_scales.dtype == torch.uint8 and x_scales.numel() >= _stages(M, K) * 64
+        assert x_scales.dtype == torch.uint8 and x_scales.is_contiguous() and x_scales.numel() >= _stages(M, K) * 64
     if want_B:
         t = _ranks(t, M, P, dt16)
     if dy is not None:

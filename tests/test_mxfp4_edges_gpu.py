@@ -287,3 +287,15 @@ def test_lowrank_grads_of_every_choice(cuda, dtype):
     for missing in range(5):
         with pytest.raises(AssertionError):
             lowrank_grads(*[None if i == missing else v for i, v in enumerate((dy, t, dt, q8, q.scales))], rank)
+
+
+def test_scales_that_are_not_contiguous_are_refused(cuda):
+    from pyraquant_amd.mxfp4 import Mxfp4Matrix, checkpoint_values, dequant_mxfp4, lowrank_grads, mxfp4_gemm, quant_mxfp4
+
+    q, q8 = quant_mxfp4(_rand(20, 64, dtype=torch.bfloat16, seed=1), checkpoint=True)
+    spread = torch.stack([q.scales, q.scales], 1)[:, 0]
+    bad, dt = Mxfp4Matrix(q.codes, spread, q.rows, q.cols), torch.zeros(2, 20, 32, dtype=torch.bfloat16, device=cuda)
+    for call in (lambda: lowrank_grads(None, None, dt, q8, spread, 8, True, False, False), lambda: dequant_mxfp4(bad),
+                 lambda: checkpoint_values(q8, bad), lambda: mxfp4_gemm(bad, quant_mxfp4(torch.zeros(32, 64, device=cuda)), None, torch.bfloat16)):
+        with pytest.raises(AssertionError):
+            call()
