@@ -84,10 +84,10 @@ Tensor forward(const Tensor& x0, const Tensor& codes, const Tensor& scales, cons
   const c10::DeviceGuard guard(x.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream(x.device().index()).stream();
   const int64_t M = x.size(0), K = x.size(1), R = !A.defined() ? 0 : A.size(1), P = R == 0 ? 0 : R <= 32 ? 32 : 64;
-  const Kept k(M, K, N, P, w.A, w.B || w.b, P && w.any());
+  const Kept k(M, K, N, P, w.A, w.B, P && w.any());
   // scratch: the codes, and what is not kept of scales and t; the forward pass's order of the factors where they come in theirs
   const int64_t s_scales = up(units(M, K) * 1024), s_t = s_scales + (w.A ? 0 : up(units(M, K) * 64));
-  const int64_t s_at = s_t + (w.B || w.b ? 0 : up(4 * M * P)), s_bt = s_at + (P && !laid_out ? up(2 * P * padded(K)) : 0);
+  const int64_t s_at = s_t + (w.B ? 0 : up(4 * M * P)), s_bt = s_at + (P && !laid_out ? up(2 * P * padded(K)) : 0);
   const int64_t s_ws = s_bt + (P && !laid_out ? up(2 * N * P) : 0), ws = P && M ? pq_mx_lowrank_workspace_size(M, K, P) : 0;
   const Tensor scratch = bytes(s_ws + ws, x);
   if (w.any()) kept = bytes(k.total, x);
@@ -109,7 +109,7 @@ Tensor forward(const Tensor& x0, const Tensor& codes, const Tensor& scales, cons
   }
   check(pq_mx_linear(x.const_data_ptr(), code_of(x), M, K, stride_of(x), data<uint8_t>(codes), data<uint8_t>(scales),
                      data<float>(bias), at, bt, P, y.data_ptr(), N, N, s, w.A ? h + k.scales : s + s_scales,
-                     w.A ? reinterpret_cast<int8_t*>(h + k.q8) : nullptr, P ? reinterpret_cast<float*>(w.B || w.b ? h + k.t : s + s_t) : nullptr,
+                     w.A ? reinterpret_cast<int8_t*>(h + k.q8) : nullptr, P ? reinterpret_cast<float*>(w.B ? h + k.t : s + s_t) : nullptr,
                      ws ? s + s_ws : nullptr, ws, stream),
         "mxfp4 layer");
   return y;
@@ -136,7 +136,7 @@ struct Layer : torch::autograd::Function<Layer> {
     const std::vector<int64_t> z = ctx->saved_data["sizes"].toIntVector();
     const int64_t M = z[0], K = z[1], N = z[2], R = z[3], P = R == 0 ? 0 : R <= 32 ? 32 : 64;
     const Wanted had{(z[4] & 1) != 0, (z[4] & 2) != 0, (z[4] & 4) != 0, (z[4] & 8) != 0};
-    const Kept k(M, K, N, P, had.A, had.B || had.b, P && had.any());
+    const Kept k(M, K, N, P, had.A, had.B, P && had.any());
     variable_list out(8);
     if (!grads[0].defined()) return out;
     // (needs_input_grad counts the inputs that are there)
@@ -160,8 +160,9 @@ struct Layer : torch::autograd::Function<Layer> {
       if (w.B) out[2] = at::empty({R, N}, opt);
       if (w.b) out[3] = at::empty({N}, opt.dtype(at::kFloat));
       const bool sums = w.A || w.B || w.b, need_dt = P && (w.x || w.A);
+      const int64_t P_sums = P ? P : 32;   // (the bias's gradient has no rank)
       const int64_t s_dt = need_dt ? up(4 * M * P) : 0;
-      const int64_t ws_sums = sums ? pq_mx_grad_factors_workspace_size(M, K, N, P) : 0;
+      const int64_t ws_sums = sums ? pq_mx_grad_factors_workspace_size(M, K, N, P_sums) : 0;
       const int64_t ws_dx = w.x ? pq_mx_grad_input_workspace_size(M, N, K) : 0;
       const int64_t ws_dt = need_dt ? pq_mx_lowrank_workspace_size(M, N, P) : 0;
       const Tensor scratch = bytes(s_dt + std::max({ws_sums, ws_dx, ws_dt}), dy);   // (one after the other on the stream)
@@ -171,8 +172,8 @@ struct Layer : torch::autograd::Function<Layer> {
         check(pq_mx_lowrank_down(dy.const_data_ptr(), code, M, N, stride_of(dy), h + k.bp, P, dt, ws_dt ? s + s_dt : nullptr, ws_dt, stream),
               "mxfp4 dt");
       if (sums)
-        check(pq_mx_grad_factors(dy.const_data_ptr(), code, stride_of(dy), w.B || w.b ? reinterpret_cast<float*>(h + k.t) : nullptr, dt,
-                                 reinterpret_cast<int8_t*>(h + k.q8), h + k.scales, M, K, N, R, P, data<void>(out[1]),
+        check(pq_mx_grad_factors(dy.const_data_ptr(), code, stride_of(dy), w.B ? reinterpret_cast<float*>(h + k.t) : nullptr, dt,
+                                 reinterpret_cast<int8_t*>(h + k.q8), h + k.scales, M, K, N, P ? R : 1, P_sums, data<void>(out[1]),
                                  data<void>(out[2]), data<float>(out[3]), s + s_dt, ws_sums, stream),
               "mxfp4 factor gradients");
       if (w.x)

@@ -299,3 +299,18 @@ def test_scales_that_are_not_contiguous_are_refused(cuda):
                  lambda: checkpoint_values(q8, bad), lambda: mxfp4_gemm(bad, quant_mxfp4(torch.zeros(32, 64, device=cuda)), None, torch.bfloat16)):
         with pytest.raises(AssertionError):
             call()
+
+
+def test_gradient_of_a_bias_without_a_branch(cuda):
+    """A frozen layer's bias buffer that requires a gradient, with and without a low-rank branch and a gradient of x."""
+    for R in (0, 8):
+        layer, *_ = _layer(64, 48, R, torch.bfloat16, 1, weight=0.1, bias=True, trainable=False)
+        layer.bias.requires_grad_()
+        dy = _rand(70, 48, dtype=torch.bfloat16, seed=1)
+        want, bound = dy.double().sum(0), 70 * F * dy.double().abs().sum(0)
+        for x in (_rand(70, 64, dtype=torch.bfloat16, seed=2), _rand(70, 64, dtype=torch.bfloat16, seed=2).requires_grad_()):
+            g, *dx = torch.autograd.grad(layer(x), [layer.bias] + [x] * x.requires_grad, dy)
+            assert g.dtype == torch.float32
+            _within(g, want, bound, "dbias")
+        layer.bias.requires_grad_(False)
+        assert torch.equal(dx[0], torch.autograd.grad(layer(x), x, dy)[0])
