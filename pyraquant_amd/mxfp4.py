@@ -334,12 +334,12 @@ class Mxfp4Linear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         assert x.shape[-1] == self.in_features, (tuple(x.shape), self.in_features)
-        d, trainable = self._buffers, self.trainable
+        d, p, trainable = self._buffers, self._parameters, self.trainable
         if trainable:
-            p = self._parameters
-            A, B, bias = p["lr_A"], p["lr_B"], p["bias"]
+            A, B = p["lr_A"], p["lr_B"]
         else:
-            A, B, bias = d["lr_Af"], d["lr_Bt"], d["bias"]
+            A, B = d["lr_Af"], d["lr_Bt"]
+        bias = d["bias"] if "bias" in d else p["bias"] if "bias" in p else self.bias   # (assigning one makes it a parameter or not)
         dt = x.dtype
         if A is not None and (A.dtype != dt or B.dtype != dt) and dt in (torch.bfloat16, torch.float16):
             A, B = A.to(dt), B.to(dt)

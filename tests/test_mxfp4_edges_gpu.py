@@ -314,3 +314,22 @@ def test_gradient_of_a_bias_without_a_branch(cuda):
             _within(g, want, bound, "dbias")
         layer.bias.requires_grad_(False)
         assert torch.equal(dx[0], torch.autograd.grad(layer(x), x, dy)[0])
+
+
+def test_an_assigned_bias_counts(cuda):
+    """A bias made a parameter, replaced by one or taken away, on a frozen and on a trainable layer."""
+    x, dy = _rand(9, 64, dtype=torch.bfloat16, seed=1), _rand(9, 48, dtype=torch.bfloat16, seed=2)
+    for trainable in (False, True):
+        layer, *_ = _layer(64, 48, 8, torch.bfloat16, 1, weight=0.1, bias=True, trainable=trainable)
+        other, *_ = _layer(64, 48, 8, torch.bfloat16, 1, weight=0.1, bias=True, trainable=trainable)
+        value = torch.randn(48, generator=torch.Generator().manual_seed(3)).cuda()
+        with torch.no_grad():
+            other.bias.copy_(value)
+        layer.bias = torch.nn.Parameter(value.clone())
+        assert torch.equal(layer(x), other(x)) and "bias" in dict(layer.named_parameters())
+        g, = torch.autograd.grad(layer(x), layer.bias, dy)
+        _within(g, dy.double().sum(0), 9 * F * dy.double().abs().sum(0), "dbias")
+        layer.bias = None
+        with torch.no_grad():
+            other.bias.zero_()
+        assert torch.equal(layer(x), other(x))
