@@ -270,6 +270,10 @@ PyObject* layer(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       PyErr_SetString(PyExc_RuntimeError, "the 4-bit layers have no forward-mode derivatives");
       return nullptr;
     }
+  if (laid_out && at::GradMode::is_enabled() && A.defined() && (A.requires_grad() || B.requires_grad())) {
+    PyErr_SetString(PyExc_AssertionError, "a frozen layer's factors, in the kernels' order, have no gradients (trainable=True tunes them)");
+    return nullptr;
+  }
   Tensor y;
   int status = PQ_OK;
   std::string text;

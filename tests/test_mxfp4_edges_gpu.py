@@ -333,3 +333,18 @@ def test_an_assigned_bias_counts(cuda):
         with torch.no_grad():
             other.bias.zero_()
         assert torch.equal(layer(x), other(x))
+
+
+def test_factors_in_the_kernels_order_take_no_gradient(cuda):
+    """lr_Af and lr_Bt are a permutation of padded factors: a gradient in lr_A's own order would be wrong for them."""
+    for K in (64, 128):
+        layer, *_ = _layer(K, 48, 32, torch.bfloat16, 1, weight=0.1, trainable=False)
+        x = _rand(9, K, dtype=torch.bfloat16, seed=1)
+        want = layer(x)
+        for name in ("lr_Af", "lr_Bt"):
+            getattr(layer, name).requires_grad_()
+            with pytest.raises(AssertionError):
+                layer(x)
+            with torch.no_grad():
+                assert torch.equal(layer(x), want)
+            getattr(layer, name).requires_grad_(False)
