@@ -357,21 +357,23 @@ def convert_linears_to_mxfp4(model: nn.Module, device: Optional[str] = "cuda",
                              whitelist: Callable[[str], bool] = is_bf16_whitelisted,
                              trainable: bool = False) -> Dict[str, object]:
     """Replaces the token-level nn.Linear layers by Mxfp4Linear in place, as convert_linears_to_int8 does by Int8Linear, and
-    returns the same kind of statistics. Layers whose sizes the 4-bit kernels do not take (in_features % 32, out_features %
-    16) stay as they are, with the whitelisted ones. A low-rank branch attached under LOWRANK_A_ATTR / LOWRANK_B_ATTR is
+    returns the same kind of statistics. Layers that the 4-bit kernels do not take (in_features % 32, out_features % 16, a
+    branch of a rank above 64, 64-bit weights) stay as they are, with the whitelisted ones. A low-rank branch attached under LOWRANK_A_ATTR / LOWRANK_B_ATTR is
     carried over; ``trainable`` makes the branches and biases of the layers that have one parameters, and every other
     parameter of the model is left as it is."""
     dev = torch.device(device) if device is not None else None
     n4, n_keep, p4, p_keep, kept = 0, 0, 0, 0, []
     for name, lin in [(n, m) for n, m in model.named_modules() if isinstance(m, nn.Linear)]:
-        if whitelist(name) or lin.in_features % BLOCK or lin.out_features % 16:
+        A, B = getattr(lin, LOWRANK_A_ATTR, None), getattr(lin, LOWRANK_B_ATTR, None)
+        has_lr = A is not None and B is not None
+        if (whitelist(name) or lin.in_features % BLOCK or lin.out_features % 16 or has_lr and not 1 <= A.shape[-1] <= MAX_RANK
+                or lin.weight.dtype not in (torch.bfloat16, torch.float16, torch.float32)):
             n_keep += 1
             p_keep += lin.weight.numel()
             kept.append(name)
             continue
         parent_name, _, attr = name.rpartition(".")
         parent = model.get_submodule(parent_name) if parent_name else model
-        has_lr = getattr(lin, LOWRANK_A_ATTR, None) is not None and getattr(lin, LOWRANK_B_ATTR, None) is not None
         setattr(parent, attr, Mxfp4Linear(lin, device=dev, trainable=trainable and has_lr))
         n4 += 1
         p4 += lin.weight.numel()

@@ -348,3 +348,20 @@ def test_factors_in_the_kernels_order_take_no_gradient(cuda):
             with torch.no_grad():
                 assert torch.equal(layer(x), want)
             getattr(layer, name).requires_grad_(False)
+
+
+# ---- conversion ---------------------------------------------------------------------------------------------------
+
+def test_layers_that_are_not_taken_stay(cuda):
+    """A branch of rank 65 or 0, 64-bit weights, sizes that do not fit, in the middle of a model: kept, and the rest converted."""
+    from pyraquant_amd.mxfp4 import Mxfp4Linear, convert_linears_to_mxfp4
+
+    for trainable in (False, True):
+        lins = [torch.nn.Linear(64, 64).bfloat16() for _ in range(4)] + [torch.nn.Linear(64, 64).double(), torch.nn.Linear(60, 64).bfloat16(),
+                                                                            torch.nn.Linear(64, 24).bfloat16()]
+        for lin, rank in zip(lins, (64, 65, 0)):
+            lin._lowrank_A, lin._lowrank_B = torch.zeros(64, rank).bfloat16(), torch.zeros(rank, 64).bfloat16()
+        net = torch.nn.Sequential(*lins)
+        stats = convert_linears_to_mxfp4(net, trainable=trainable)
+        assert [isinstance(m, Mxfp4Linear) for m in net] == [True, False, False, True, False, False, False]
+        assert stats["n_mxfp4_linear"] == 2 and stats["n_bf16_linear_kept"] == 5 and stats["bf16_kept_names"] == ["1", "2", "4", "5", "6"]
