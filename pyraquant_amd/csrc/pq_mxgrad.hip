@@ -64,17 +64,18 @@ __device__ __forceinline__ void add_low_rank(const DxArgs& p, int kk, int m, int
 // Few blocks: a workgroup of four waves takes 64 rows m x 128 columns k (one stage of the packed weight), 64 n a step. dy and
 // the 4-bit weights of the next two steps are on their way into registers while the products of this one run, then go to the
 // other of two LDS buffers, the weights widened to 16 bits on the way; they are read back by columns. One barrier a step.
-// SPLIT: blockIdx.z takes a slice of n and leaves its sums in fp32 in p.part [slices][M][K] for mx_dx_join_kernel.
+// (Blocks of one row of blocks are neighbours in blockIdx.x: a grid's y ends at 65535.)
+// SPLIT: blockIdx.y takes a slice of n and leaves its sums in fp32 in p.part [slices][M][K] for mx_dx_join_kernel.
 // Bound by the steps' latency, one workgroup to a compute unit or less: 154 x 2048 x 640 9 us, 1000 x 1312 x 1040 13.
 template <int DT, int R, bool SPLIT>
 __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
   constexpr int BM = 64, A = BM * 128, W = 64 * 256, LA = BM / 32, TJ = BM / 64;   // 16-byte loads of dy a thread; m tiles of a wave
   __shared__ __attribute__((aligned(16))) uint8_t smem[2 * (A + W)];      // [m][64 n] and [n][128 k], twice
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int kt = blockIdx.x, k0 = kt * 128, m0 = blockIdx.y * BM;
+  const int kt = blockIdx.x % p.KT, k0 = kt * 128, m0 = blockIdx.x / p.KT * BM;
   const int wk = (wave & 1) * 64, wm = (wave >> 1) * (BM / 2);
   const int l32 = lane & 31, half = lane >> 5;
-  const int first = SPLIT ? blockIdx.z * p.slice : 0, end = SPLIT ? min(p.N, first + p.slice) : p.N;
+  const int first = SPLIT ? blockIdx.y * p.slice : 0, end = SPLIT ? min(p.N, first + p.slice) : p.N;
   const int arow = tid >> 3, achunk = tid & 7, wrow = tid >> 2, wb = tid & 3;
   const bool in_k = k0 + wb * 32 < p.K;
   struct Step {
@@ -150,7 +151,7 @@ __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
         if (m < p.M && kk < p.K) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<v4f*>(p.part + ((int64_t)blockIdx.z * p.M + m) * p.K + kk + 8 * q + 4 * half) =
+            *reinterpret_cast<v4f*>(p.part + ((int64_t)blockIdx.y * p.M + m) * p.K + kk + 8 * q + 4 * half) =
                 v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
         }
         continue;
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
 template <int DT, int R>
 __global__ __launch_bounds__(256) void mx_dx_join_kernel(const DxArgs p, int slices) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, half = lane >> 5;
-  const int kk = blockIdx.x * 128 + wave * 32, m = blockIdx.y * 32 + l32;
+  const int kk = blockIdx.x % p.KT * 128 + wave * 32, m = blockIdx.x / p.KT * 32 + l32;
   if (kk >= p.K) return;
   v16f acc = {};
   if (m < p.M) {
@@ -712,10 +713,11 @@ int launch_dx(DxArgs p, int dtype, int r, hipStream_t stream) {
   p.slice = plan.slice;
   p.tiles_m = (p.M + 255) / 256;
   p.tiles_k = (p.K + 255) / 256;
-  const int64_t blocks = (int64_t)p.tiles_m * p.tiles_k * plan.slices;
-  if (plan.ring)
-    if (const int st = check_grid(blocks, 512, "mx_grad_input")) return st;
-  const dim3 ring((unsigned)blocks), grid((unsigned)p.KT, (unsigned)((p.M + 63) / 64), (unsigned)plan.slices);
+  const int64_t blocks = plan.ring ? (int64_t)p.tiles_m * p.tiles_k * plan.slices : (int64_t)p.KT * ((p.M + 63) / 64);
+  const int64_t join_blocks = plan.slices > 1 ? (int64_t)p.KT * ((p.M + 31) / 32) : 0;
+  if (const int st = check_grid(blocks, plan.ring ? 512 : 256, "mx_grad_input")) return st;
+  if (const int st = check_grid(join_blocks, 256, "mx_grad_input")) return st;
+  const dim3 ring((unsigned)blocks), grid((unsigned)blocks, (unsigned)plan.slices);
   if (plan.slices == 1) {
     if (plan.ring) {
 #define PQ_MXK(D, RR) hipLaunchKernelGGL((mx_dx_ring_kernel<D, RR, false>), ring, dim3(512), 0, stream, p)
@@ -736,7 +738,7 @@ int launch_dx(DxArgs p, int dtype, int r, hipStream_t stream) {
     if (bf16) hipLaunchKernelGGL((mx_dx_kernel<PQ_BF16, 0, true>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((mx_dx_kernel<PQ_F16, 0, true>), grid, dim3(256), 0, stream, p);
   }
-  const dim3 join((unsigned)((p.K + 127) / 128), (unsigned)((p.M + 31) / 32));
+  const dim3 join((unsigned)join_blocks);
 #define PQ_MXK(D, RR) hipLaunchKernelGGL((mx_dx_join_kernel<D, RR>), join, dim3(256), 0, stream, p, plan.slices)
   PQ_MXD();
 #undef PQ_MXK

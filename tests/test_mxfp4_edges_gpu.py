@@ -365,3 +365,24 @@ def test_layers_that_are_not_taken_stay(cuda):
         stats = convert_linears_to_mxfp4(net, trainable=trainable)
         assert [isinstance(m, Mxfp4Linear) for m in net] == [True, False, False, True, False, False, False]
         assert stats["n_mxfp4_linear"] == 2 and stats["n_bf16_linear_kept"] == 5 and stats["bf16_kept_names"] == ["1", "2", "4", "5", "6"]
+
+
+# ---- many rows ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("M,K", [(65536 * 64 + 70, 32), (65536 * 64 + 1, 96)])
+def test_input_gradient_of_millions_of_rows(cuda, M, K):
+    """More blocks of rows than a grid's second dimension counts."""
+    from pyraquant_amd.mxfp4 import dequant_mxfp4, mxfp4_grad_input, quant_mxfp4
+
+    N, R, u = 16, 32, U[torch.bfloat16]
+    g = torch.Generator(device=cuda).manual_seed(M)
+    dy = torch.randn(M, N, generator=g, device=cuda, dtype=torch.bfloat16)
+    dt, ap = torch.randn(M, R, generator=g, device=cuda), torch.randn(K, R, generator=g, device=cuda).bfloat16()
+    wq = quant_mxfp4(torch.randn(N, K, generator=g, device=cuda))
+    wh = dequant_mxfp4(wq, torch.float32).double()
+    got = mxfp4_grad_input(dy, wq, dt, ap)
+    for r in range(0, M, 1 << 19):
+        d, t = dy[r : r + (1 << 19)].double(), dt[r : r + (1 << 19)].double()
+        want, terms = d @ wh + t @ ap.double().t(), d.abs() @ wh.abs() + t.abs() @ ap.double().abs().t()
+        off = ((N + 2 * R) * F + u * u) * terms
+        _within(got[r : r + (1 << 19)], want, off + u * (want.abs() + off), f"dx from row {r}")
