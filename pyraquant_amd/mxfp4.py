@@ -235,14 +235,17 @@ def _padded_rank(R: int) -> int:
 
 def lay_out_factors(lr_A: torch.Tensor, lr_B: torch.Tensor):
     """lr_A [K, R] and lr_B [R, N] as the forward pass reads them, zero-padded to rank P (32 or 64): (lr_A's fragments
-    [ceil(K / 128) * 128, P], pq_mx_factors' order, lr_B's rows [N, P])."""
+    [ceil(K / 128) * 128, P], pq_mx_factors' order, lr_B's rows [N, P]). Each in its own type."""
     _check_cuda(lr_A, lr_B)
     assert lr_A.dim() == 2 and lr_B.dim() == 2 and lr_A.shape[1] == lr_B.shape[0], (tuple(lr_A.shape), tuple(lr_B.shape))
-    assert lr_A.dtype == lr_B.dtype, (lr_A.dtype, lr_B.dtype)
-    _dtype16(lr_A.dtype)
     A, B = _plain(lr_A).contiguous(), _plain(lr_B).contiguous()
     (K, R), N = A.shape, B.shape[1]
     P = _padded_rank(R)
+    if A.dtype != B.dtype or A.dtype not in (torch.bfloat16, torch.float16):   # (the kernel moves 16-bit values)
+        Af, Bt = A.new_zeros(((K + 127) // 128 * 128, P)), B.new_zeros((N, P))
+        Af[:K, :R], Bt[:, :R] = A, B.t()
+        f = Af.reshape(-1, 4, 4, 8, P // 16, 16)    # stage, block, group, k, rank / 16, rank % 16
+        return f.permute(0, 2, 4, 1, 5, 3).reshape(Af.shape).contiguous(), Bt
     Af = torch.empty(((K + 127) // 128 * 128, P), dtype=A.dtype, device=A.device)
     Bt = torch.empty((N, P), dtype=A.dtype, device=A.device)
     _lib.check(_lib.load().pq_mx_factors(_lib.ptr(A), R, _lib.PQ_MX_BY_COLUMN, _lib.ptr(B), N, _lib.PQ_MX_BY_RANK, K, N, R, P,
@@ -256,13 +259,15 @@ class Mxfp4Linear(nn.Module):
     and the weight; in_features % 32 == 0, out_features % 16 == 0, low rank up to 64. Inputs are bf16 or fp16, and the
     low-rank factors are used in the input's type.
 
-    Buffers ``weight_codes`` and ``weight_scales`` hold the weight. ``trainable=False`` keeps the low-rank branch in the
-    kernels' order (``lr_Af``, ``lr_Bt``: lay_out_factors; ``lr_A`` and ``lr_B`` give it back) and
-    the bias in fp32 as buffers. ``trainable=True`` (needs a low-rank branch) makes ``lr_A`` [K, R], ``lr_B`` [R, N] and
-    ``bias`` parameters; freeze() turns such a layer into the other kind. Gradients flow to the input of either."""
+    Buffers ``weight_codes`` and ``weight_scales`` hold the weight. ``trainable=False`` keeps the bias in fp32 and the low-rank
+    branch in the kernels' order as buffers (``lr_Af``, ``lr_Bt``: lay_out_factors; ``lr_A`` and ``lr_B`` give it back), in its own
+    type or in ``dtype``: each call casts it where that is not the input's type. ``trainable=True`` (needs a low-rank branch) makes
+    ``lr_A`` [K, R], ``lr_B`` [R, N] and ``bias`` parameters; freeze() turns such a layer into the other kind. Gradients flow to the
+    input of either."""
 
     def __init__(self, lin: nn.Linear, device: Optional[torch.device] = None,
-                 lowrank: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, trainable: bool = False):
+                 lowrank: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, trainable: bool = False,
+                 dtype: Optional[torch.dtype] = None):
         super().__init__()
         w = lin.weight.detach()
         if device is not None:
@@ -287,26 +292,25 @@ class Mxfp4Linear(nn.Module):
             self.lr_A, self.lr_B = nn.Parameter(A.clone().contiguous()), nn.Parameter(B.clone().contiguous())
             self.register_parameter("bias", None if bias is None else nn.Parameter(bias.clone()))
         else:
-            self._keep(A if self.rank else None, B if self.rank else None, bias)
+            self._keep(A if self.rank else None, B if self.rank else None, bias, dtype)
 
-    def _keep(self, A, B, bias) -> None:
+    def _keep(self, A, B, bias, dtype) -> None:
         """The low-rank branch and the bias as buffers, the branch in the kernels' order."""
         Af = Bt = None
         if A is not None:
-            if A.dtype not in (torch.bfloat16, torch.float16):
-                A, B = A.to(torch.bfloat16), B.to(torch.bfloat16)
-            Af, Bt = lay_out_factors(A, B.to(A.dtype))
+            Af, Bt = lay_out_factors(A.to(dtype or A.dtype), B.to(dtype or B.dtype))
         self.register_buffer("lr_Af", Af)
         self.register_buffer("lr_Bt", Bt)
         self.register_buffer("bias", bias)
 
-    def freeze(self) -> "Mxfp4Linear":
-        """Turns a trainable layer into one that serves: its low-rank branch laid out once, nothing left to tune."""
+    def freeze(self, dtype: Optional[torch.dtype] = None) -> "Mxfp4Linear":
+        """Turns a trainable layer into one that serves: its low-rank branch laid out once, nothing left to tune, the same outputs.
+        Give the inputs' type as ``dtype`` where the factors are in another (fp32 masters), and no call has to cast them."""
         if self.trainable:
             A, B, bias = self.lr_A.detach(), self.lr_B.detach(), self.bias
             del self.lr_A, self.lr_B, self.bias
             self.trainable = False
-            self._keep(A, B, None if bias is None else bias.detach().float().contiguous())
+            self._keep(A, B, None if bias is None else bias.detach().float().contiguous(), dtype)
         return self
 
     def __getattr__(self, name):
@@ -358,9 +362,10 @@ def convert_linears_to_mxfp4(model: nn.Module, device: Optional[str] = "cuda",
                              trainable: bool = False) -> Dict[str, object]:
     """Replaces the token-level nn.Linear layers by Mxfp4Linear in place, as convert_linears_to_int8 does by Int8Linear, and
     returns the same kind of statistics. Layers that the 4-bit kernels do not take (in_features % 32, out_features % 16, a
-    branch of a rank above 64, 64-bit weights) stay as they are, with the whitelisted ones. A low-rank branch attached under LOWRANK_A_ATTR / LOWRANK_B_ATTR is
-    carried over; ``trainable`` makes the branches and biases of the layers that have one parameters, and every other
-    parameter of the model is left as it is."""
+    branch of a rank above 64, 64-bit weights) stay as they are, with the whitelisted ones. A low-rank branch attached under
+    LOWRANK_A_ATTR / LOWRANK_B_ATTR is carried over: frozen in the weight's type where that has 16 bits (an nn.Linear's inputs
+    have it); with ``trainable`` the branches, as they are, and the biases of the layers that have one become parameters, and every
+    other parameter of the model is left as it is."""
     dev = torch.device(device) if device is not None else None
     n4, n_keep, p4, p_keep, kept = 0, 0, 0, 0, []
     for name, lin in [(n, m) for n, m in model.named_modules() if isinstance(m, nn.Linear)]:
@@ -374,7 +379,8 @@ def convert_linears_to_mxfp4(model: nn.Module, device: Optional[str] = "cuda",
             continue
         parent_name, _, attr = name.rpartition(".")
         parent = model.get_submodule(parent_name) if parent_name else model
-        setattr(parent, attr, Mxfp4Linear(lin, device=dev, trainable=trainable and has_lr))
+        setattr(parent, attr, Mxfp4Linear(lin, device=dev, trainable=trainable and has_lr,
+                                          dtype=lin.weight.dtype if lin.weight.dtype != torch.float32 else None))
         n4 += 1
         p4 += lin.weight.numel()
         del lin

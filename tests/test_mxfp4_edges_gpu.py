@@ -386,3 +386,42 @@ def test_input_gradient_of_millions_of_rows(cuda, M, K):
         want, terms = d @ wh + t @ ap.double().t(), d.abs() @ wh.abs() + t.abs() @ ap.double().abs().t()
         off = ((N + 2 * R) * F + u * u) * terms
         _within(got[r : r + (1 << 19)], want, off + u * (want.abs() + off), f"dx from row {r}")
+
+
+# ---- freezing -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("a_type,b_type", [(torch.float32,) * 2, (torch.bfloat16,) * 2, (torch.float16,) * 2, (torch.bfloat16, torch.float32),
+                                           (torch.float32, torch.float16), (torch.float16, torch.bfloat16)])
+def test_frozen_layers_answer_as_the_tuned_ones(cuda, dtype, a_type, b_type):
+    """Factors of any type, inputs of either: a trainable layer, frozen, gives the same bits, and so does one built frozen; lr_A and
+    lr_B come back as they were."""
+    from pyraquant_amd.mxfp4 import Mxfp4Linear
+
+    for K, N, R in ((128, 48, 16), (416, 80, 40)):
+        g = torch.Generator().manual_seed(K)
+        A, B = (torch.randn(K, R, generator=g) * 0.1).to(a_type).cuda(), (torch.randn(R, N, generator=g) * 0.1).to(b_type).cuda()
+        lin = torch.nn.Linear(K, N).to(dtype)
+        layer = Mxfp4Linear(lin, device="cuda", lowrank=(A, B), trainable=True)
+        x = _rand(70, K, dtype=dtype, seed=1)
+        with torch.no_grad():
+            want = layer(x)
+            assert torch.equal(Mxfp4Linear(lin, device="cuda", lowrank=(A, B))(x), want)
+            given = Mxfp4Linear(lin, device="cuda", lowrank=(A, B), trainable=True).freeze(dtype)
+            assert torch.equal(given(x), want) and given.lr_Af.dtype == given.lr_Bt.dtype == dtype
+            layer.freeze()
+            assert torch.equal(layer(x), want)
+        assert torch.equal(layer.lr_A, A) and torch.equal(layer.lr_B, B) and layer.lr_A.dtype == a_type and layer.lr_B.dtype == b_type
+
+
+def test_conversion_keeps_factors_in_the_weights_type(cuda):
+    from pyraquant_amd.mxfp4 import Mxfp4Linear, convert_linears_to_mxfp4
+
+    for dtype in BOTH:
+        lin = torch.nn.Linear(64, 48).to(dtype)
+        lin._lowrank_A, lin._lowrank_B = torch.randn(64, 8) * 0.1, torch.randn(8, 48) * 0.1
+        net = torch.nn.Sequential(lin)
+        convert_linears_to_mxfp4(net)
+        assert net[0].lr_Af.dtype == net[0].lr_Bt.dtype == dtype
+        x = _rand(9, 64, dtype=dtype, seed=1)
+        assert torch.equal(net(x), Mxfp4Linear(lin, device="cuda")(x))
