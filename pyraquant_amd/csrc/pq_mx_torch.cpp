@@ -45,11 +45,12 @@ int32_t code_of(const Tensor& x) { return x.scalar_type() == at::kBFloat16 ? PQ_
 template <typename T>
 T* data(const Tensor& t) { return t.defined() ? static_cast<T*>(const_cast<void*>(t.const_data_ptr())) : nullptr; }
 
-// Rows as the kernels read them: consecutive elements, 16-byte aligned, none over another (a copy where not).
-Tensor rows_of(const Tensor& t) {
+// Rows as the kernels read them: consecutive elements, 16-byte aligned, none over another, no further apart than `most` (a copy
+// where not).
+Tensor rows_of(const Tensor& t, int64_t most = INT64_MAX) {
   Tensor x = t.is_neg() ? t.resolve_neg() : t;
   const int64_t M = x.size(0), K = x.size(1);
-  if ((K > 1 && x.stride(1) != 1) || (M > 1 && (x.stride(0) < K || x.stride(0) % 8)) || (uintptr_t)x.const_data_ptr() % 16)
+  if ((K > 1 && x.stride(1) != 1) || (M > 1 && (x.stride(0) < K || x.stride(0) % 8 || x.stride(0) > most)) || (uintptr_t)x.const_data_ptr() % 16)
     x = x.clone(at::MemoryFormat::Contiguous);
   return x;
 }
@@ -143,7 +144,7 @@ struct Layer : torch::autograd::Function<Layer> {
     const Wanted w{had.x && ctx->needs_input_grad(0), had.A && ctx->needs_input_grad(1), had.B && ctx->needs_input_grad(2),
                    had.b && ctx->needs_input_grad(P ? 3 : 1)};
     try {
-      const Tensor dy = rows_of(grads[0]);
+      const Tensor dy = rows_of(grads[0], 1 << 21);   // (pq_mx_grad_input's limit)
       const c10::DeviceGuard guard(dy.device());
       const hipStream_t stream = c10::hip::getCurrentHIPStream(dy.device().index()).stream();
       const auto opt = dy.options().requires_grad(false);

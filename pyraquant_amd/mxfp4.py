@@ -80,11 +80,13 @@ def _plain(x: torch.Tensor) -> torch.Tensor:
     return x.resolve_neg() if x.is_neg() else x
 
 
-def _rows(x2: torch.Tensor) -> torch.Tensor:
-    """x2 as the kernels read it: rows of consecutive elements, 16-byte aligned, none over another (a copy where not)."""
+def _rows(x2: torch.Tensor, most: Optional[int] = None) -> torch.Tensor:
+    """x2 as the kernels read it: rows of consecutive elements, 16-byte aligned, none over another, no further apart than ``most``
+    (a copy where not)."""
     x2 = _plain(x2)
     M, K = x2.shape
-    if x2.stride(1) != 1 or (M > 1 and (x2.stride(0) < K or x2.stride(0) * x2.element_size() % 16)) or x2.data_ptr() % 16:
+    if (x2.stride(1) != 1 or x2.data_ptr() % 16
+            or M > 1 and (x2.stride(0) < K or x2.stride(0) * x2.element_size() % 16 or most is not None and x2.stride(0) > most)):
         x2 = x2.clone(memory_format=torch.contiguous_format)
     return x2
 
@@ -153,7 +155,7 @@ def mxfp4_grad_input(dy: torch.Tensor, wq: Mxfp4Matrix, dt: Optional[torch.Tenso
     _check_cuda(dy, wq.codes, wq.scales, dt, lr_Ap)
     assert dy.dim() == 2 and dy.shape[1] == wq.rows, (tuple(dy.shape), wq.rows)
     code = _dtype16(dy.dtype)
-    dy = _rows(dy)
+    dy = _rows(dy, 1 << 21)   # (pq_mx_grad_input's limit)
     M, N, K = dy.shape[0], wq.rows, wq.cols
     R = 0
     if dt is not None:

@@ -425,3 +425,22 @@ def test_conversion_keeps_factors_in_the_weights_type(cuda):
         assert net[0].lr_Af.dtype == net[0].lr_Bt.dtype == dtype
         x = _rand(9, 64, dtype=dtype, seed=1)
         assert torch.equal(net(x), Mxfp4Linear(lin, device="cuda")(x))
+
+
+# ---- strides ------------------------------------------------------------------------------------------------------
+
+def test_output_gradients_far_apart(cuda):
+    """Rows of dy further apart than the input gradient's kernels address."""
+    from pyraquant_amd.mxfp4 import mxfp4_grad_input, quant_mxfp4
+
+    step = 2 ** 21 + 64
+    base = torch.zeros(6 * step, dtype=torch.bfloat16, device=cuda)
+    far = torch.as_strided(base, (5, 48), (step, 1))
+    far.copy_(_rand(5, 48, dtype=torch.bfloat16, seed=1))
+    wq = quant_mxfp4(_rand(48, 64, dtype=torch.float32, seed=2))
+    assert torch.equal(mxfp4_grad_input(far, wq), mxfp4_grad_input(far.contiguous(), wq))
+    layer, *_ = _layer(64, 48, 8, torch.bfloat16, 1, weight=0.1, bias=True)
+    x = _rand(5, 64, dtype=torch.bfloat16, seed=3).requires_grad_()
+    wanted = [x, layer.lr_A, layer.lr_B, layer.bias]
+    for a, b in zip(*(torch.autograd.grad(layer(x), wanted, d) for d in (far, far.contiguous()))):
+        assert torch.equal(a, b)
