@@ -444,3 +444,70 @@ def test_output_gradients_far_apart(cuda):
     wanted = [x, layer.lr_A, layer.lr_B, layer.bias]
     for a, b in zip(*(torch.autograd.grad(layer(x), wanted, d) for d in (far, far.contiguous()))):
         assert torch.equal(a, b)
+
+
+# ---- memory around the outputs, in every kind of block ------------------------------------------------------------
+
+def _framed(M, N, dtype, cuda):
+    """An [M, N] window of a larger tensor of sevens, and whether all around it still holds them."""
+    big = torch.full((M + 9, N + 24), 7.0, dtype=dtype, device=cuda)
+    window = big[4 : 4 + M, 8 : 8 + N]
+
+    def untouched():
+        frame = big.clone()
+        frame[4 : 4 + M, 8 : 8 + N] = 7.0
+        return bool((frame == 7.0).all())
+
+    return window, untouched
+
+
+# a split product; blocks of 128 x 64, of 128 x 64 in three groups, of 128 x 256 and of 256 x 256, one and several to a workgroup
+@pytest.mark.parametrize("M,K,N,R", [(40, 96, 80, 32), (1100, 352, 912, 0), (513, 96, 2064, 64), (329, 4320, 2512, 32), (600, 1056, 7056, 32),
+                                     (2100, 160, 4112, 64), (4200, 96, 4208, 32), (8500, 160, 4368, 0)])
+def test_products_write_their_output_alone(cuda, M, K, N, R):
+    from pyraquant_amd.mxfp4 import dequant_mxfp4, mxfp4_gemm, quant_mxfp4
+
+    for dtype in BOTH:
+        g = torch.Generator(device=cuda).manual_seed(M)
+        xq, wq = (quant_mxfp4(torch.randn(n, K, generator=g, device=cuda)) for n in (M, N))
+        t, bias = torch.randn(M, R, generator=g, device=cuda) if R else None, torch.randn(N, generator=g, device=cuda)
+        l2t = torch.randn(N, R, generator=g, device=cuda).to(dtype) if R else None
+        out, untouched = _framed(M, N, dtype, cuda)
+        mxfp4_gemm(xq, wq, bias, dtype, t=t, l2t=l2t, out=out)
+        assert untouched() and torch.equal(out, mxfp4_gemm(xq, wq, bias, dtype, t=t, l2t=l2t))
+        xh, wh, u = dequant_mxfp4(xq, torch.float32).double(), dequant_mxfp4(wq, torch.float32).double(), U[dtype]
+        want, terms = xh @ wh.t() + bias, xh.abs() @ wh.abs().t() + bias.abs()
+        if R:
+            want, terms = want + t.double() @ l2t.double().t(), terms + t.double().abs() @ l2t.double().abs().t()
+        off = ((K + 2 * R + 2) * F + u * u) * terms + (2.0 ** -25 * l2t.double().abs().sum(1) if R else 0)
+        _within(out, want, off + u * (want.abs() + off) + 2.0 ** -25, (dtype, M, K, N))
+
+
+# 64 x 128 blocks and 256 x 256 blocks, each whole and in slices (slices: whether the call has a workspace)
+@pytest.mark.parametrize("M,K,N,slices", [(1000, 1312, 1040, False), (300, 288, 2080, True), (4128, 2080, 496, False), (8300, 1056, 112, False),
+                                          (2050, 1312, 5136, True)])
+def test_input_gradients_write_their_output_alone(cuda, M, K, N, slices):
+    from pyraquant_amd import _lib
+    from pyraquant_amd.mxfp4 import dequant_mxfp4, mxfp4_grad_input, quant_mxfp4
+
+    L = _lib.load()
+    size = L.pq_mx_grad_input_workspace_size(M, N, K)
+    assert (size > 0) == slices
+    for dtype in BOTH:
+        for R in (0, 32, 64):
+            g = torch.Generator(device=cuda).manual_seed(M)
+            wq = quant_mxfp4(torch.randn(N, K, generator=g, device=cuda))
+            dy = torch.randn(M, N, generator=g, device=cuda).to(dtype)
+            dt, ap = (torch.randn(M, R, generator=g, device=cuda), torch.randn(K, R, generator=g, device=cuda).to(dtype)) if R else (None, None)
+            dx, untouched = _framed(M, K, dtype, cuda)
+            ws = torch.full((size + 256,), 255, dtype=torch.uint8, device=cuda)
+            _lib.check(L.pq_mx_grad_input(_lib.ptr(dy), _lib.dtype_code(dtype), N, _lib.ptr(wq.codes), _lib.ptr(wq.scales), _lib.ptr(dt), _lib.ptr(ap),
+                                          R, _lib.ptr(dx), dx.stride(0), M, N, K, _lib.ptr(ws), size, _lib.stream_of(dy.device)), "dx")
+            assert untouched() and bool((ws[size:] == 255).all())
+            assert torch.equal(dx, mxfp4_grad_input(dy, wq, dt, ap))
+            wh, u = dequant_mxfp4(wq, torch.float32).double(), U[dtype]
+            want, terms = dy.double() @ wh, dy.double().abs() @ wh.abs()
+            if R:
+                want, terms = want + dt.double() @ ap.double().t(), terms + dt.double().abs() @ ap.double().abs().t()
+            off = ((N + 2 * R) * F + u * u) * terms + (2.0 ** -25 * ap.double().abs().sum(1) if R else 0)
+            _within(dx, want, off + u * (want.abs() + off) + 2.0 ** -25, (dtype, M, K, N, R))
