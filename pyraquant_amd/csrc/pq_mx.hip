@@ -51,8 +51,8 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(const void* __restrict__ 
 // of the 16 x 16 x 32 products (8 consecutive values of a row; the order of k within the sum is free as long as l1t's operand
 // has the same), so x is read once and needs no other lane or LDS. l1t comes from the cache in fragment order (1 KB a load, zeros
 // past K), once per RG row groups. The waves' sums are added in LDS in a fixed order. dt, of dy, is made here too.
-// Bound by reading x and by l1t from the cache: 65536 x 3072 with codes 101 us (the quantizer alone: 88), dy of 16384 x 12288
-// to dt in 103-110 us, 3.7-3.9 TB/s.
+// Bound by reading x and by l1t from the cache: 65536 x 3072 with codes 103 us (the quantizer alone: 88), dy of 16384 x 12288
+// to dt in 104-116 us, 3.5-3.9 TB/s.
 template <int DT, int R, int RG, int NW, bool QUANT, bool CKPT>
 __global__ __launch_bounds__(64 * NW) void mx_lowrank_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t M, int K, int KT,
                                                              const uint16_t* __restrict__ l1f, uint8_t* __restrict__ codes,
@@ -308,13 +308,17 @@ int64_t pq::mx::lowrank_workspace(int64_t M, int64_t K, int64_t R) {
   return slices > 1 ? 4 * slices * M * R : 0;
 }
 
-// Rows a workgroup takes, and its waves (us, bf16, rank 32, with the 4-bit codes):
-//   M x K            16 rows, 16 waves  32 rows, 8 waves  64 rows, 4 waves    quantizer and product of their own
-//   65536 x 3072          134.4             105.7             100.6            160.6
-//   16384 x 3072           35.2              31.1              34.2             47.7
-//   4352 x 3072            14.1              11.8              22.9             21.0
-//   4096 x 3072             9.9              11.7              22.8             20.4
-//   2050 x 1280             5.4               6.2              11.8             11.6
+// Rows a workgroup takes, and its waves: 16 and 16, 32 and 8, or 64 and 4 (us, bf16; t alone / with the 4-bit codes / with these and
+// the 8-bit ones; quantizer and product of their own, rank 32: 65536 x 3072 161, 16384 x 3072 48, 4096 x 3072 20, 2050 x 1280 12):
+//   M x K           rank 32: 16 rows       32 rows          64 rows         rank 64: 16 rows       32 rows          64 rows
+//   65536 x 3072     120 / 126 / 179   105 / 107 / 160    95 / 103 / 153    142 / 193 / 241   117 / 130 / 180   103 / 115 / 163
+//   16384 x 12288    119 / 132 / 196   104 / 117 / 178   101 / 124 / 182    146 / 169 / 233   118 / 133 / 192   110 / 134 / 193
+//   16384 x 3072      23 /  26 /  35    21 /  25 /  35    22 /  30 /  43     33 /  46 /  55    25 /  31 /  40    25 /  32 /  44
+//   8192 x 3072       14 /  16 /  20    13 /  15 /  20    19 /  24 /  34     18 /  25 /  30    15 /  18 /  22    22 /  26 /  36
+//   4352 x 3072       10 /  14 /  18    11 /  12 /  17    19 /  23 /  32     15 /  20 /  26    12 /  14 /  19    20 /  25 /  34
+//   4096 x 3072      6.5 / 9.8 /  12    10 /  12 /  17    16 /  23 /  32    8.5 /  14 /  16    12 /  14 /  19    18 /  25 /  34
+//   2050 x 5120      8.9 /  13 /  16    13 /  17 /  25    25 /  36 /  50     12 /  18 /  21    16 /  21 /  28    27 /  38 /  53
+//   2050 x 1280      4.0 / 4.8 / 5.7   5.2 / 5.6 / 7.3   8.3 /  11 /  16    4.9 / 6.1 / 7.0   5.9 / 6.4 / 8.0   9.2 /  13 /  17
 int pq::mx::lowrank(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* l1f, int64_t R, uint8_t* codes,
                     uint8_t* scales, int8_t* q8, float* t, void* workspace, hipStream_t stream) {
   const int slices = lowrank_slices(M, K);

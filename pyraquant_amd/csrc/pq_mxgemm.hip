@@ -5,9 +5,10 @@
 // 64 values of k a step, one scale byte per lane and operand) and sum in fp32. The row operand is a weight row n and the
 // column operand an activation row m, so each lane holds 4 consecutive n of one output row.
 //
-// Large products are bound by the matrix units at the power limit (52-62 % busy at 1.7-1.5 GHz; from registers alone the same
-// instructions reach 6.5 PFLOP/s): 16384 x 12288 x 12288 in 1170 us, 4.2 PFLOP/s, 65536 x 3072 x 12288 in 1387 us, 3.6. With a
-// short K the output's bytes bind (8202 x 640 x 5120: 33 us, 84 MB out), with few rows the start of a launch and LDS.
+// Large products are bound by the matrix units at the power limit (50-62 % busy at 1.7-1.5 GHz; from registers alone the same
+// instructions reach 6.5 PFLOP/s): 16384 x 12288 x 12288 in 1070 us, 4.6 PFLOP/s, with rank 32 1126 to 1180; 65536 x 3072 x 12288 with
+// rank 32 in 1390 to 1475 us, 3.6 to 3.4, without 1259 (both parts of t: 70 us more than the first alone). With a short K the
+// output's bytes bind (8202 x 640 x 5120: 32 us, 84 MB out), with few rows the start of a launch and LDS.
 #include "pq_mx.h"
 
 #include <algorithm>
@@ -295,7 +296,7 @@ int launch_ring(GemmArgs p, int dtype, int r, hipStream_t stream) {
 //    the last barrier freed, then the results go out through a staging area of their own, 16 rows of 64 outputs at a time;
 //  * results are stored with buffer stores, whose bounds replace branches: every wave issues the same 16, and the ring's waits
 //    count them (vmcnt completes in order: 16 more may be outstanding until stage NS is waited for).
-// Against one block a workgroup: 65536 x 3072 x 12288 1562 -> 1387 us, 4096 x 3072 x 3072 31.1 -> 27.0.
+// Against one block a workgroup (with the first part of t alone): 65536 x 3072 x 12288 1562 -> 1387 us, 4096 x 3072 x 3072 31.1 -> 27.0.
 template <int DT, int R>
 __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
 void mx_gemm_large_kernel(const GemmArgs p) {
@@ -518,7 +519,7 @@ int launch_large(GemmArgs p, int r, int cus, hipStream_t stream) {
 // TJ and its waves every NW-th stage of K, each with all of the block's sums; fragments come from memory into registers, D
 // stages ahead, and the waves' sums are added in LDS in a fixed order. QUANT: x is 16-bit, and each lane quantizes the very
 // blocks its fragments are (32 consecutive values of a row), so few rows need no quantizer of their own before the product.
-// Bound by the latency of a launch and of a wave's first loads: 154 x 2048 x 1280 4.2 us; 1 x 12288 x 3072 7 us for 20 MB.
+// Bound by the latency of a launch and of a wave's first loads: 154 x 2048 x 1280 4.3 us; 1 x 12288 x 3072 8.3 us for 20 MB.
 struct SplitArgs {
   GemmArgs g;
   const uint16_t* x;   // QUANT
@@ -602,7 +603,7 @@ __global__ __launch_bounds__(64 * NW) void mx_gemm_split_kernel(const SplitArgs 
       }
     }
   }
-  // The waves' sums, a tile at a time; thread t adds element t of the 1024 (4 outputs of a row for each of 256 threads).
+  // The waves' sums, a tile at a time: all of them leave theirs in LDS, and one wave adds them up.
 #pragma unroll
   for (int i = 0; i < TI; ++i)
 #pragma unroll
@@ -611,7 +612,7 @@ __global__ __launch_bounds__(64 * NW) void mx_gemm_split_kernel(const SplitArgs 
 #pragma unroll
       for (int r = 0; r < 16; ++r) part[wave][lane * 17 + r] = acc[i][j][r];
       __syncthreads();
-      if (wave == (i * TJ + j) % NW) {   // one wave joins the tile: its lanes hold the layout the low-rank products have
+      if (wave == (i * TJ + j) % NW) {   // (its lanes hold the layout the low-rank products have)
         v16f y = {};
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -668,17 +669,17 @@ int launch_split(const SplitArgs& p, int dtype, int r, hipStream_t stream) {
 
 // The block of a product, by how its blocks fill the chip. us of the kernel (bf16, rank 32, bias):
 //   M x K x N            256x256  128x256  128x64  128x64, 3 groups  32x32 split   (n x m; 256x256, 128x256: one workgroup per CU)
-//   65536 x 3072 x 12288   1387     1893    2294                                   (256x256: persistent, times the CUs' rounds)
-//   4096 x 3072 x 3072     27.0     38.9    39.0                       92.3
-//   2050 x 1280 x 5120     16.0     22.9    22.5                       48.3        180 blocks of 256 x 256
-//   512 x 3072 x 12288     24.9     20.0    24.3                       47.6        192 blocks of 128 x 256, 384 of 128 x 128
-//   1024 x 3072 x 3072     23.3     17.5    11.7                       24.8        384 blocks of 128 x 64
-//   512 x 12288 x 3072     65.9     49.3    26.3         22.4          39.3        192 blocks of 128 x 64, one to a CU
-//   512 x 3072 x 3072                       10.6         10.4                      the same, 24 stages of K
-//   300 x 640 x 5120                         6.2          7.4                      5 stages: the groups' join costs more
-//   256 x 3072 x 3072      23.3     17.0     8.5                        8.1        768 blocks of 32 x 32
-//   154 x 2048 x 1280      18.5     13.1     6.7                        4.2
-//   1 x 12288 x 3072       62.6     47.3    21.4                        8.7
+//   65536 x 3072 x 12288   1390     1848    2253                                   (256x256: persistent, times the CUs' rounds)
+//   4096 x 3072 x 3072     27.2     38.3    38.2         50.4          97.8
+//   2050 x 1280 x 5120     15.9     24.2    22.6         37.5          48.2        180 blocks of 256 x 256
+//   512 x 3072 x 12288     24.0     20.9    22.0         27.4          50.0        192 blocks of 128 x 256, 384 of 128 x 128
+//   1024 x 3072 x 3072     23.7     18.8    12.2         16.6          25.3        384 blocks of 128 x 64
+//   512 x 12288 x 3072     68.6     50.7    24.9         21.2          35.0        192 blocks of 128 x 64, one to a CU
+//   512 x 3072 x 3072      23.5     18.9     9.6          9.4          14.1        the same, 24 stages of K
+//   300 x 640 x 5120       11.8     10.5     5.6          6.9           8.7        5 stages: the groups' join costs more
+//   256 x 3072 x 3072      23.6     18.6     9.2          9.1           8.3        768 blocks of 32 x 32
+//   154 x 2048 x 1280      18.0     14.2     7.3          7.8           4.4
+//   1 x 12288 x 3072       67.4     47.5    22.3         17.5           8.8
 // (128 x 128 won nowhere and is not built. What the last column gets fits two of its workgroups per CU at once. A lone
 // workgroup of four waves leaves LDS idle between its barriers; three groups of four keep it busy: 96 stages of 12 KB in and 24
 // KB out at 128 B a clock are 14 us. Deeper rings alone changed nothing.)

@@ -66,7 +66,7 @@ __device__ __forceinline__ void add_low_rank(const DxArgs& p, int kk, int m, int
 // other of two LDS buffers, the weights widened to 16 bits on the way; they are read back by columns. One barrier a step.
 // (Blocks of one row of blocks are neighbours in blockIdx.x: a grid's y ends at 65535.)
 // SPLIT: blockIdx.y takes a slice of n and leaves its sums in fp32 in p.part [slices][M][K] for mx_dx_join_kernel.
-// Bound by the steps' latency, one workgroup to a compute unit or less: 154 x 2048 x 640 9 us, 1000 x 1312 x 1040 13.
+// Bound by the steps' latency, one workgroup to a compute unit or less: 154 x 2048 x 640 9.5 us, 1000 x 1312 x 1040 14.
 template <int DT, int R, bool SPLIT>
 __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
   constexpr int BM = 64, A = BM * 128, W = 64 * 256, LA = BM / 32, TJ = BM / 64;   // 16-byte loads of dy a thread; m tiles of a wave
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(256) void mx_dx_kernel(const DxArgs p) {
 }
 
 // dx from the slices' sums, added in order, and the low-rank term. A wave takes 32 rows x 32 columns. Bound by reading the sums:
-// five slices of 2050 x 1280 (52 MB) and rank 64 in 15 us.
+// five slices of 2050 x 1280 (52 MB) and rank 64 in 17 us.
 template <int DT, int R>
 __global__ __launch_bounds__(256) void mx_dx_join_kernel(const DxArgs p, int slices) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, half = lane >> 5;
@@ -206,8 +206,8 @@ __global__ __launch_bounds__(256) void mx_dx_join_kernel(const DxArgs p, int sli
 // and codes s + 2, all issued by phase s - 3; the barrier before it has every wave wait for all but its two younger phases.
 // LDS, per step: fragments 8 waves x 12 KB, dy 16 KB in, weights 16 KB in: as many cycles as the products take (bf16 products
 // of 32 x 32 x 16 at 32 cycles, 128 bytes of LDS a cycle), so the kernel is bound by both at once, and by the power limit:
-// 16384 x 3072 x 12288 in 1003 us, 1.24 PFLOP/s (a library's product of the weight in bf16: 1.36-1.38); 4352 x 3072 x 3072, 204
-// blocks on 256 compute units, in 77.5 us, 1.06. Moving the loads or the reads of codes between the products cost 10 %.
+// 16384 x 3072 x 12288 in 1000 us, 1.24 PFLOP/s (a library's product of the weight in bf16: 1.36-1.38); 4352 x 3072 x 3072, 204
+// blocks on 256 compute units, in 79.5 us, 1.03. Moving the loads or the reads of codes between the products cost 10 %.
 struct DxTile {
   // (64 bytes after each KB of codes: the 128 values that two of them hold of a row are read together)
   static constexpr int DY = 256 * 128, BLOCK = 1024 + 64, CODES = 4 * BLOCK + 1024, W = 32 * 512;
@@ -460,8 +460,8 @@ void mx_dx_ring_kernel(const DxArgs p) {
 // ---- sums over rows: part[s][r][c] = sum over the rows of slice s of v[m, r] z[m, c] -------------------------------------
 // z is dy (EIGHT false) or the 8-bit codes of x with their scales; v is t or dt, [M, R] in fp32. Column sums of z too
 // (COLS), and these alone where v is NULL. A workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step, the
-// next step's rows on their way into registers meanwhile; the order of the sums is fixed. Bound by reading z: 460 MB of 16384 x 3072 x 12288 in 92 us, 5.0 TB/s
-// (87 with the first part of v alone; results' errors then grow by 1.4).
+// next step's rows on their way into registers meanwhile; the order of the sums is fixed. Bound by reading z: 460 MB of 16384 x 3072 x
+// 12288 in 98 us, 4.7 TB/s.
 struct SumArgs {
   const void* z;
   const uint8_t* scales;
@@ -655,26 +655,27 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const JoinArgs b, const Jo
 }
 
 // How dx is computed: in blocks of 256 x 256 (m x k) or 64 x 128, with n cut into `slices` where that ends sooner, by an
-// estimate in us. A 256 x 256 block, one to a compute unit: 9 for its start and end, and for 64 n 1.25 alone to 1.7 with all 256 at
-// work (the clock falls with the power they draw). A 64 x 128 block: 0.62 for 64 n, more where a compute unit holds more than
-// one, 1 for the end of each past the third, and 4 for the launch. Slices: 4 for another launch; 1.2 for 10^6 values of their sums (fp32,
-// written and read again). Measured (bf16, rank 32, * the plan's):
+// estimate in us for the card's 256 compute units (the workspace's size comes from the same plan, and knows no device). A 256 x 256
+// block, one to a compute unit: 9 for its start and end, and for 64 n 1.25 alone to 1.7 with all 256 at work (the clock falls with
+// the power they draw). A 64 x 128 block: 0.62 for 64 n, more where a compute unit holds more than one, 1 for the end of each past
+// the third, and 4 for the launch. Slices: 4 for another launch; 1.2 for 10^6 values of their sums (fp32, written and read again).
+// Measured (bf16, rank 32, * the plan's):
 //   M x K x N            256 x 256, slices: 1  2      4      5      8   64 x 128: 1      2      4      8
-//   16384 x 3072 x 12288      999*  1139   1256   1339   1578      1698   1882   2000   2303
-//   4352 x 3072 x 3072       77.2*   122    166    182    272       130    156    187    306
-//   2050 x 5120 x 1280       36.4*  76.1   96.2    114              50.2   75.9   97.5
-//   2050 x 1280 x 5120        112   73.6   54.1   51.1*  72.5      68.9   60.3   66.4   76.6
-//   1024 x 3072 x 12288       254    146   93.0   87.6*   114       151    125    129    139
-//   1024 x 3072 x 3072       70.6   54.2   44.7   44.5   64.1      42.2*  43.3   50.4   62.5
-//   512 x 3072 x 12288        254    142   83.4   73.3   58.8*      124   90.2   69.2   75.4
-//   512 x 12288 x 3072       71.2   61.7*  81.1   82.2    106      60.4   77.2   89.3    118
-//   5150 x 9248 x 416        70.7*   260    415                    92.4    264    428
-//   11734 x 608 x 1680       44.6*  71.5          84.7             51.6   72.8   86.5
-//   13664 x 1344 x 4704       217*   241    302    328    419       282    338    394    508
-//   3000 x 2048 x 2048       50.8   50.7   69.5   72.5   95.3      44.6*  59.4   72.5   97.4
-//   1000 x 1312 x 1040       29.0   33.2   30.7   30.0             13.2*  20.3   22.2
-//   154 x 2048 x 640         20.1   18.9   18.3   18.1              9.0*   9.6    9.6
-//   64 x 3072 x 3072         67.8   40.1   26.7   25.2   22.3      29.7   21.0   14.9   13.4*
+//   16384 x 3072 x 12288      999*  1160   1259   1344   1580      1730   1936   2052   2322
+//   4352 x 3072 x 3072       79.7*   124    169    184    275       132    161    193    308
+//   2050 x 5120 x 1280       38.5*  78.4   98.7    117              51.7   80.2    101
+//   2050 x 1280 x 5120        113   74.8   55.3   53.0*  73.5      69.6   62.0   67.8   77.8
+//   1024 x 3072 x 12288       255    147   95.7   89.8*   114       153    127    133    143
+//   1024 x 3072 x 3072       72.0   54.7   45.4   46.3   65.0      43.0*  44.4   50.6   63.9
+//   512 x 3072 x 12288        255    142   84.2   73.9   60.2*      127   91.6   70.8   78.7
+//   512 x 12288 x 3072       72.6   63.1*  82.3   83.3    107      62.4   79.8   93.5    118
+//   5150 x 9248 x 416        74.2*   268    422                    95.9    273    433
+//   11734 x 608 x 1680       46.0*  73.6   87.4   93.1             54.9   74.3   89.3
+//   13664 x 1344 x 4704       220*   246    303    331    422       290    343    398    511
+//   3000 x 2048 x 2048       52.0   52.4   70.9   74.0   97.0      45.6*  63.2   76.5   99.2
+//   1000 x 1312 x 1040       30.3   33.8   31.5   30.7             13.9*  20.9   22.5
+//   154 x 2048 x 640         21.0   19.3   18.8   18.5              9.5*  10.1   10.1
+//   64 x 3072 x 3072         68.3   40.4   27.0   25.3   22.6      30.8   21.8   15.5   14.0*
 struct DxPlan {
   bool ring;
   int slices, slice;
@@ -747,8 +748,9 @@ int launch_dx(DxArgs p, int dtype, int r, hipStream_t stream) {
 }
 
 // Row slices of mx_rowsum_kernel: about 384 workgroups a sum. More only add sums to write and join; fewer read too little at once.
-// us of both launches, for 256 / 384 / 512 / 1024 workgroups (bf16, one part of v): 2050 x 1280 x 5120 rank 64 19.0 / 19.6 / 20.9 / 25.2,
-// 4352 x 3072 x 3072 rank 32 17.1 / 17.3 / 21.4 / 26.1, 16384 x 3072 x 12288 116 / 104 / 103 / 105.
+// us of both launches, for 256 / 384 / 512 / 1024 workgroups (bf16): 2050 x 1280 x 5120 rank 64 21.8 / 21.9 / 20.5 / 24.5,
+// 4352 x 3072 x 3072 rank 32 17.5 / 19.7 / 19.1 / 24.3, 8192 x 3072 x 3072 rank 64 42.1 / 39.1 / 43.6 / 52.9, 16384 x 3072 x 12288
+// rank 32 123 / 104 / 111 / 106.
 int row_slices(int64_t M, int64_t C) {
   const int64_t panels = (C + 127) / 128, steps = (M + 63) / 64;
   const int64_t want = std::min<int64_t>({(384 + panels - 1) / panels, steps, 256});

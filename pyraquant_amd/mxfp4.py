@@ -15,6 +15,7 @@ The format: E = floor(log2(max |x|)) - 2 over 32 consecutive values of a row, ea
 Tuning. ``Mxfp4Linear(lin, lowrank=(A, B), trainable=True)`` keeps the weight in 4 bits and makes lr_A, lr_B and the bias
 parameters. What its backward pass keeps of the input are 8-bit codes, rint(x 2^(4 - E)) on the same E, written in the
 quantizer's pass over x (half the bytes of x): they give lr_A's gradient. The rounding of x to 4 bits counts as the identity.
+The layer has first derivatives of the reverse kind (a second one, or a forward-mode tangent, raises); the functions have none.
 
 Every kernel runs on the caller's current stream; nothing synchronises. CPU tensors raise AssertionError; a missing library
 raises at the first call.
