@@ -17,6 +17,7 @@ import torch.nn as nn
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from pyraquant_amd.int8_exec import LOWRANK_A_ATTR, LOWRANK_B_ATTR  # noqa: E402
 from pyraquant_amd.mxfp4 import Mxfp4Linear, convert_linears_to_mxfp4, dequant_mxfp4, quant_mxfp4  # noqa: E402
+from pyraquant_amd.optim import AdamW  # noqa: E402
 
 
 def attach_residual_branch(lin: nn.Linear, rank: int) -> None:
@@ -53,7 +54,7 @@ def run(dim=640, tokens=2048, rank=32, steps=60, dtype=torch.bfloat16, seed=0):
         attach_residual_branch(lin, rank)
     convert_linears_to_mxfp4(block, trainable=True)
     started = error(block)
-    opt = torch.optim.Adam(block.parameters(), lr=3e-4)
+    opt = AdamW(block.parameters(), lr=3e-4, weight_decay=0.0)
     for _ in range(steps):
         x = sample()
         loss = (block(x).float() - teacher(x).float()).square().mean()

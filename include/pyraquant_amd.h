@@ -465,6 +465,67 @@ int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, const float*
                        const uint8_t* x_scales, int64_t M, int64_t K, int64_t N, int64_t R, int64_t P, void* dA, void* dB,
                        float* dbias, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
+/*
+ * ---- AdamW over the tensors of a model (no reference counterpart) ---------------------------------------------------
+ *
+ *   g = gradient * min(1, max_norm / (norm + 1e-6))            (where sums of squares are given; norm: of all of them)
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  t = t + 1
+ *   p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * in fp32, p rounded once to its type. A norm that is infinite or NaN leaves everything as it was.
+ *
+ * A list of tensors: `tensors` and `chunks` in device memory, `first_chunk` [n_tensors + 1] and `grads` [n_tensors] in host memory.
+ * Tensor i has n values at p (any alignment of its type; dense, in the gradient's order), its states from value `base` (a multiple of
+ * PQ_ADAMW_BLOCK) of the states on, room for n rounded up to such a block, and the chunks first_chunk[i] .. first_chunk[i + 1] - 1, one for each
+ * PQ_ADAMW_CHUNK values begun; chunks[c] is the tensor of chunk c. grads[i] is its gradient, of its type, or NULL: the tensor is
+ * left as it is. The launches take `grads` by value: the array may go when the call returns, and a captured graph keeps it.
+ *
+ * States: m and v for n values in all. bits 32: fp32. bits 8: a byte each, and two in `exps` for each PQ_ADAMW_BLOCK values, the
+ * exponent E (biased as in fp32) of the block's largest mean and of its largest root. m is the mean's sign and byte, v the byte of the root of the
+ * mean of squares: byte b > 0 is the fp32 number of bits (b + 8 (E - 15)) << 20, or (b + 16 (E - 15)) << 19 for a root; 0 is zero, and
+ * a block of E = 255 is NaN. Values are rounded up or down by a hash of their place, the step count and `seed`. `steps`: a count for each
+ * chunk, of the steps that its tensor has had. All zeros: no step yet.
+ */
+#define PQ_ADAMW_CHUNK 1024
+#define PQ_ADAMW_BLOCK 128
+typedef struct {
+  void* p;
+  int64_t n, base;
+  int32_t dtype, first_chunk;   /* PQ_BF16, PQ_F16 or PQ_F32 */
+} pq_adamw_tensor;
+typedef struct {
+  const pq_adamw_tensor* tensors;
+  const int32_t* chunks;
+  const int64_t* first_chunk;
+  const void* const* grads;
+  int64_t n_tensors;
+} pq_adamw_list;
+typedef struct {
+  void *m, *v;                  /* 16-byte aligned */
+  uint8_t* exps;                /* 2-byte aligned; NULL with 32 bits */
+  int32_t* steps;
+  int64_t n;
+  int32_t bits;
+} pq_adamw_states;
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay, max_norm;
+  const float* lr_at;           /* the rate in device memory, read by the kernel; NULL: lr */
+  uint32_t seed;
+} pq_adamw_rates;
+
+/* The sums of the squares of a list's gradients, in 64 bits, as pq_grad_squares_partials(list) partial sums in device memory, their order fixed by the sizes. */
+int64_t pq_grad_squares_partials(const pq_adamw_list* list);
+int pq_grad_squares(const pq_adamw_list* list, double* partials, int64_t n_partials, hipStream_t stream);
+
+/* One step. n_partials > 0: the gradients (of all lists that share a limit) are held to rates->max_norm by pq_grad_squares' sums, and their
+ * norm is written to `norm` (device memory); else both may be NULL. */
+int pq_adamw_step(const pq_adamw_list* list, const pq_adamw_states* states, const pq_adamw_rates* rates, const double* partials,
+                  int64_t n_partials, float* norm, hipStream_t stream);
+
+/* The states' values: the means and the roots of the means of squares, states->n each, in dtype (8-bit states are exact in PQ_BF16
+ * and PQ_F32); and states from such values in fp32, to nearest (the counts are the caller's to set). 16-byte aligned. */
+int pq_adamw_moments(const pq_adamw_states* states, void* mean, void* root, int32_t dtype, hipStream_t stream);
+int pq_adamw_load(const pq_adamw_states* states, const float* mean, const float* root, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -56,11 +56,39 @@ EXPORTS = (
     "pq_mx_grad_input",
     "pq_mx_grad_factors_workspace_size",
     "pq_mx_grad_factors",
+    "pq_grad_squares_partials",
+    "pq_grad_squares",
+    "pq_adamw_step",
+    "pq_adamw_moments",
+    "pq_adamw_load",
 )
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
+
+
+
+class AdamWList(ctypes.Structure):
+    """pq_adamw_list"""
+
+    _fields_ = [("tensors", _p), ("chunks", _p), ("first_chunk", ctypes.POINTER(_i64)), ("grads", ctypes.POINTER(_p)), ("n_tensors", _i64)]
+
+
+class AdamWStates(ctypes.Structure):
+    """pq_adamw_states"""
+
+    _fields_ = [("m", _p), ("v", _p), ("exps", _p), ("steps", _p), ("n", _i64), ("bits", _i32)]
+
+
+class AdamWRates(ctypes.Structure):
+    """pq_adamw_rates"""
+
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")] + [
+        ("lr_at", _p), ("seed", ctypes.c_uint32)]
+
+
+_list, _states, _rates = (ctypes.POINTER(t) for t in (AdamWList, AdamWStates, AdamWRates))
 
 _SIGNATURES = {
     "pq_abi_version": ([], ctypes.c_int),
@@ -105,6 +133,11 @@ _SIGNATURES = {
     "pq_mx_grad_factors_workspace_size": ([_i64, _i64, _i64, _i64], _i64),
     "pq_mx_grad_factors": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p],
                            ctypes.c_int),
+    "pq_grad_squares_partials": ([_list], _i64),
+    "pq_grad_squares": ([_list, _p, _i64, _p], ctypes.c_int),
+    "pq_adamw_step": ([_list, _states, _rates, _p, _i64, _p, _p], ctypes.c_int),
+    "pq_adamw_moments": ([_states, _p, _p, _i32, _p], ctypes.c_int),
+    "pq_adamw_load": ([_states, _p, _p, _p], ctypes.c_int),
 }
 
 _lib = None
@@ -154,6 +187,17 @@ def load_mx():
         raise LibraryMissing(f"pyraquant_amd/_mx.so is not built or does not load ({e}); run "
                              "`python -m pyraquant_amd.build`") from e
     return _mx
+
+
+def load_tune():
+    """_tune.so (csrc/pq_tune_torch.cpp): the optimizer's plan of a parameter group."""
+    load()
+    try:
+        from . import _tune
+    except ImportError as e:
+        raise LibraryMissing(f"pyraquant_amd/_tune.so is not built or does not load ({e}); run "
+                             "`python -m pyraquant_amd.build`") from e
+    return _tune
 
 
 def check(status: int, what: str) -> None:

@@ -1,7 +1,7 @@
-"""Build libpqint8.so (the gfx950 HIP kernels + C ABI) in-tree with hipcc, and _direct.so and _mx.so (the eager layer
-calls, CPython extensions over torch's C++ API and the library) with the host compiler.
+"""Build libpqint8.so (the gfx950 HIP kernels + C ABI) in-tree with hipcc, and _direct.so, _mx.so and _tune.so (the eager layer
+calls and the optimizer's, CPython extensions over torch's C++ API and the library) with the host compiler.
 
-    python -m pyraquant_amd.build          # compiles every csrc/*.hip, links pyraquant_amd/libpqint8.so, and both extensions
+    python -m pyraquant_amd.build          # compiles every csrc/*.hip, links pyraquant_amd/libpqint8.so, and the extensions
 
 Flags: gfx950 only; -ffp-contract=off so the fp32 epilogue follows source order (multiply, then add, as
 the reference's epilogue is written); correctly rounded fp32 division (the quantizer's codes depend on
@@ -22,7 +22,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libpqint8.so")
 DIRECT_PATH = os.path.join(HERE, "_direct.so")
 MX_PATH = os.path.join(HERE, "_mx.so")
-EXTENSIONS = (("pq_torch.cpp", DIRECT_PATH), ("pq_mx_torch.cpp", MX_PATH))   # host code over torch's C++ API and the library
+TUNE_PATH = os.path.join(HERE, "_tune.so")
+EXTENSIONS = (("pq_torch.cpp", DIRECT_PATH), ("pq_mx_torch.cpp", MX_PATH), ("pq_tune_torch.cpp", TUNE_PATH))   # host code over torch's C++ API and the library
 ARCH = "gfx950"
 
 HIP_FLAGS = [

@@ -1,0 +1,488 @@
+"""AdamW's kernels against its step in 64 bits (oracle/adamw_ref.py).
+
+Every comparison starts from what the kernel held before the step, so one step's roundings count (f = 2^-24, each rounding 1 f at most):
+  limit   c: the norm, its sum with 1e-6, the quotient: 3 f;  d = g c: 4 f
+  mean    b1 m + (1 - b1) d: the rates as fp32 numbers, the products, the sum: 3 f for m's term, 7 f for d's: 8 f (|b1 m| + |(1 - b1) d|)
+  square  b2 v + (1 - b2) d^2: 8 f of d twice and its product 9 f, the rate, the product and the sum 3 f: 12 f v'
+  root    6 f of the square and its own rounding: 8 f
+  p       (1 - lr wd) p - size m' / (root / unbias + eps): with u = size |m'| / den, the mean's bound times size / den, 24 f u (the root's 8 f,
+          unbias, its quotient, the sum with eps, the division, size and its product: 6 f more), 4 f (|p| + u) for the factor of p, its
+          product and the difference; and half a step of the result's type (fp16: at least half its smallest subnormal)
+8-bit values are what the definition holds for some mean (root) within these bounds of the exact one.
+"""
+import copy
+import io
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import adamw_ref as ref
+
+pytestmark = pytest.mark.gpu
+F = 2.0 ** -24
+TYPES = (torch.float32, torch.bfloat16, torch.float16)
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}   # half of torch.finfo(t).eps
+
+
+def _opt(params, **kw):
+    from pyraquant_amd.optim import AdamW
+
+    return AdamW(params, **{"lr": 1e-3, "weight_decay": 0.01, **kw})
+
+
+def _params(shapes, dtype, seed=0, std=0.02):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter((torch.randn(s, generator=g) * std).to(dtype).cuda()) for s in shapes]
+
+
+def _grads(params, seed, std=1e-3):
+    g = torch.Generator().manual_seed(seed)
+    for p in params:
+        p.grad = (torch.randn(p.shape, generator=g) * std).to(p.dtype).cuda()
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _before(opt):
+    """What the step starts from: per parameter (p, m, v) in 64 bits, flat in memory order."""
+    out = []
+    for i, group in enumerate(opt.param_groups):
+        m, r = (_np(x) for x in opt.moments(torch.float32, i))
+        v = _np(opt.states(i)[1]) if group["bits"] == 32 else r * r
+        for at, p in zip(opt.offsets(i), group["params"]):
+            n = p.numel()
+            flat = p.detach().as_strided((n,), (1,))
+            out.append((_np(flat), m[at:at + n], v[at:at + n]))
+    return out
+
+
+def _check_step(opt, before, t, clip=1.0, seed=0):
+    """Every parameter and state after step t against the definition from `before`."""
+    k = 0
+    for i, group in enumerate(opt.param_groups):
+        (b1, b2), lr, eps, wd = group["betas"], group["lr"], group["eps"], group["weight_decay"]
+        m1, r1 = (_np(x) for x in opt.moments(torch.float32, i))
+        v1 = _np(opt.states(i)[1]) if group["bits"] == 32 else None
+        for at, p in zip(opt.offsets(i), group["params"]):
+            p0, m0, v0 = before[k]
+            k += 1
+            n = p.numel()
+            if p.grad is None:
+                assert np.array_equal(_np(p.detach().as_strided((n,), (1,))), p0)
+                assert np.array_equal(m1[at:at + n], m0)
+                continue
+            g = _np(torch.empty_like(p).copy_(p.grad).as_strided((n,), (1,)))
+            want, m, v = ref.step(p0, g, m0, v0, t, lr, (b1, b2), eps, wd, clip)
+            m_off = 8 * F * (np.abs(b1 * m0) + np.abs((1 - b1) * g * clip)) + 2.0 ** -149
+            v_off = 12 * F * v + 2.0 ** -149
+            den = np.sqrt(v / (1 - b2 ** t)) + eps
+            u = lr / (1 - b1 ** t) * np.abs(m) / den
+            off = lr / (1 - b1 ** t) * m_off / den + 24 * F * u + 4 * F * (np.abs(p0) + u)
+            off = off + HALF[p.dtype] * (np.abs(want) + off) + (2.0 ** -25 if p.dtype == torch.float16 else 0)
+            got = _np(p.detach().as_strided((n,), (1,)))
+            assert (np.abs(got - want) <= off).all(), (i, k, float(np.max(np.abs(got - want) - off)))
+            pad = -n % ref.BLOCK
+            end = at + n + pad
+            if group["bits"] == 32:
+                assert (np.abs(m1[at:at + n] - m) <= m_off).all() and (np.abs(v1[at:at + n] - v) <= v_off).all(), k
+                assert not m1[at + n:end].any() and not v1[at + n:end].any()
+                continue
+            um, ur = ref.dither(np.arange(at, end), t, seed)
+            root, r_off = np.sqrt(v), 8 * F * np.sqrt(v) + 2.0 ** -149
+            for got, mid, o, bits, add in ((m1[at:end], m, m_off, 3, um), (r1[at:end], root, r_off, 4, ur)):
+                mid, o = np.pad(mid, (0, pad)), np.pad(o, (0, pad))
+                size = np.abs(mid)
+                # (a value whose bounds hold the border of a step may be held on either side of it)
+                low, high = (ref.held(np.copysign(np.maximum(size + d * o, 0), mid), bits, add) for d in (-1, 1))
+                exact = ref.held(mid, bits, add)
+                assert ((got == exact) | (got == low) | (got == high)).all(), (k, bits, int(((got != exact) & (got != low) & (got != high)).sum()))
+                assert (got != exact).sum() <= 2 + 1e-3 * n       # (a value is that near a border with a probability of 2^-16: one in a small tensor is no fault)
+
+
+SHAPES = [(1,), (7,), (128,), (129, 3), (1023,), (1024,), (1025,), (31, 77), (640, 16), (16, 1288), (5, 4099)]
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+@pytest.mark.parametrize("dtype", TYPES)
+def test_steps_against_the_definition(cuda, dtype, bits):
+    params = _params(SHAPES, dtype)
+    opt = _opt(params, bits=bits, seed=3)
+    for t in range(1, 5):
+        _grads(params, t)
+        before = _before(opt)
+        opt.step()
+        _check_step(opt, before, t, seed=3)
+    assert all(int(s) == 4 for p in params for s in opt.state[p]["step"])
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+def test_rates_and_types_of_groups(cuda, bits):
+    """Groups with rates of their own, of mixed types, one with the other kind of states; betas, eps and decay at their ends."""
+    a, b = _params([(300, 5), (77,)], torch.bfloat16), _params([(1000,), (40, 40)], torch.float32, 1)
+    c, d = _params([(999,)], torch.float16, 2), _params([(130,)], torch.float32, 3)
+    opt = _opt([{"params": a + c, "lr": 1e-2, "betas": (0.0, 0.5), "bits": bits}, {"params": b, "eps": 0.1, "weight_decay": 0.0},
+                {"params": d, "betas": (0.95, 0.0), "weight_decay": 5.0, "bits": 40 - bits}], seed=9)
+    for t in range(1, 4):
+        _grads(a + b + c + d, 10 + t)
+        before = _before(opt)
+        opt.step()
+        _check_step(opt, before, t, seed=9)
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+def test_many_tensors_and_missing_gradients(cuda, bits):
+    """1003 tensors, three launches; a third of them without a gradient, another third in the next step, keep everything and count apart."""
+    params = _params([(1 + 37 * i % 500,) for i in range(1003)], torch.bfloat16)
+    opt = _opt(params, bits=bits)
+    _grads(params, 1)
+    for p in params[::3]:
+        p.grad = None
+    before = _before(opt)
+    opt.step()
+    _check_step(opt, before, 1)
+    assert [int(opt.state[p]["step"][0]) for p in params] == [0 if i % 3 == 0 else 1 for i in range(1003)]
+    for p in params:
+        p.grad = None
+    for p in params[:400:3]:
+        p.grad = torch.ones_like(p)
+    old = [(p.clone(), [s.clone() for s in opt.state[p].values()]) for p in params]
+    opt.step()
+    for i, (p, (was, state)) in enumerate(zip(params, old)):
+        same = torch.equal(p, was) and all(torch.equal(s, w) for s, w in zip(opt.state[p].values(), state))
+        assert same == (p.grad is None), i
+    opt.zero_grad()
+    opt.step()      # nothing to do
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_and_limit(cuda, dtype):
+    params = _params([(640, 33), (1001,), (5,), (0,), (64, 64)], dtype)
+    for limit, std in ((0.5, 1e-2), (1e6, 1e-2), (float("inf"), 1.0)):
+        opt = _opt([{"params": params[:2]}, {"params": params[2:], "bits": 8}], max_norm=limit)
+        _grads(params, 5, std)
+        norm = math.sqrt(sum(float(p.grad.double().square().sum()) for p in params))
+        before = _before(opt)
+        opt.step()
+        # the sum in 64 bits (20 000 terms), one rounding
+        assert abs(float(opt.grad_norm) - norm) <= 2 * F * norm and opt.grad_norm.is_cuda
+        c = min(1.0, limit / (norm + 1e-6))
+        _check_step(opt, before, 1, clip=c)
+
+
+@pytest.mark.parametrize("bad", (float("inf"), float("-inf"), float("nan")))
+@pytest.mark.parametrize("bits", (32, 8))
+def test_a_norm_that_is_no_number_changes_nothing(cuda, bits, bad):
+    params = _params([(640, 3), (100,)], torch.float32)
+    opt = _opt(params, bits=bits, max_norm=1.0)
+    _grads(params, 1)
+    opt.step()
+    old = copy.deepcopy([[p.data] + list(opt.state[p].values()) for p in params])
+    _grads(params, 2)
+    params[1].grad[50] = bad
+    opt.step()
+    assert not math.isfinite(float(opt.grad_norm))
+    for p, was in zip(params, old):
+        assert all(torch.equal(a, b) for a, b in zip([p.data] + list(opt.state[p].values()), was))
+    params[1].grad[50] = 0
+    before = _before(opt)
+    opt.step()
+    _check_step(opt, before, 2, clip=min(1.0, 1.0 / (float(opt.grad_norm) + 1e-6)))
+
+
+def test_large_gradients_have_a_norm(cuda):
+    p = torch.nn.Parameter(torch.zeros(1000, device=cuda))
+    p.grad = torch.full_like(p, 1e30)
+    opt = _opt([p], max_norm=1.0)
+    opt.step()
+    assert abs(float(opt.grad_norm) / (1e30 * math.sqrt(1000)) - 1) < 1e-6 and bool(p.isfinite().all())
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+@pytest.mark.parametrize("dtype", TYPES)
+def test_places_and_orders(cuda, dtype, bits):
+    """Parameters and gradients at odd places of a larger tensor, whose other values stay; transposed parameters; gradients in another
+    order, of a broadcast value."""
+    room = torch.full((4096,), 7.0, dtype=dtype, device=cuda)
+    odd = torch.nn.Parameter(room[3:3 + 2050].view(50, 41))
+    even = torch.nn.Parameter(room[2056 + 8:2056 + 8 + 131])
+    turned = torch.nn.Parameter(torch.randn(30, 70, device=cuda).to(dtype).t())
+    params = [odd, even, turned]
+    opt = _opt(params, bits=bits)
+    grads = torch.randn(5000, device=cuda).to(dtype) * 1e-2
+    for t, (g0, g1, g2) in enumerate(((grads[1:2051].view(50, 41), grads[5:136], grads[7:2107].view(70, 30)),
+                                      (grads[:2050].view(41, 50).t(), grads[:1].expand(131), grads[:2100].view(30, 70).t())), 1):
+        odd.grad, even.grad, turned.grad = g0, g1, g2
+        before = _before(opt)
+        opt.step()
+        _check_step(opt, before, t)
+    assert bool((room[:3] == 7).all()) and bool((room[2053:2064] == 7).all()) and bool((room[2064 + 131:] == 7).all())
+
+
+def test_eight_bit_averages_move_as_32_bit_ones_do(cuda):
+    """The root's average under gradients that fall to a tenth: a move of 5e-4 a step against a grid of 3 to 6 %. A rounding up or
+    down leaves the root unbiased, and its square larger by its variance: by the grid step s (at most 2^-4 of the root) and a move
+    d = 5e-4 each step adds at most d s, over a memory of 1000 steps 2^-4 / 2 of the square: 3.1 %, and a hundredth of that either way
+    for 2^15 values. Rounded to nearest it would not move at all."""
+    p = torch.nn.Parameter(torch.zeros(1 << 15, device=cuda))
+    opt8, q = _opt([p], bits=8, lr=0.0), torch.nn.Parameter(torch.zeros(1 << 15, device=cuda))
+    opt32 = _opt([q], lr=0.0)
+    for steps, size in ((300, 1.0), (1500, 0.1)):
+        for t in range(steps):
+            p.grad = torch.randn(1 << 15, device=cuda) * size
+            q.grad = p.grad
+            opt8.step()
+            opt32.step()
+        v8, v32 = float(opt8.moments()[1].square().mean()), float(opt32.states()[1].mean())
+        assert 0.96 < v8 / v32 < 1.06, (v8, v32)
+        m8, m32 = opt8.moments()[0], opt32.states()[0]
+        # a mean's rounding error is at most 2^-3 of it a step and decays by b1: sqrt(1 / (1 - b1^2)) 2^-3 / 2 of its size, at most 15 %
+        assert float((m8 - m32).norm() / m32.norm()) < 0.15
+
+
+def test_blocks_of_zeros_subnormals_infinities(cuda):
+    p = torch.nn.Parameter(torch.ones(128 * 5, device=cuda))
+    opt = _opt([p], bits=8, lr=1e-3, weight_decay=0.0)
+    g = torch.zeros(5, 128, device=cuda)
+    g[1] = 1e-30
+    g[2, 5] = float("inf")
+    g[3, 7] = 1.0
+    g[3, 9] = 1e-12
+    g[4, 0] = float("nan")
+    p.grad = g.view(-1)
+    opt.step()
+    m, r = (x.view(5, 128) for x in opt.moments())
+    assert not m[0].any() and not r[0].any() and bool(m[2].isnan().all()) and bool(m[4].isnan().all()) and bool(r[2].isnan().all())
+    assert float(r[3, 9]) > 0 and float(m[3, 9]) == 0 and not r[3, 10:].any()
+    v = p.detach().view(5, 128)
+    assert bool((v[0] == 1).all()) and bool(v[1].isfinite().all()) and bool(v[3].isfinite().all())
+    assert bool(v[2].isnan().sum() == 1) and bool(v[4].isnan().sum() == 1)     # (the others of the block, from the next step on)
+
+
+def test_moments_in_and_out(cuda):
+    """Values that 8-bit states hold come back as they are, in bf16 too; others to nearest; 32-bit states take and give fp32."""
+    params = _params([(1000,), (3, 50), (4096,)], torch.bfloat16)
+    eight, full = _opt(params, bits=8), _opt(params)
+    n = 1024 + 256 + 4096
+    assert eight.offsets() == [0, 1024, 1280]
+    g = torch.Generator().manual_seed(0)
+    m, r = torch.randn(n, generator=g) * 1e-3, torch.exp(torch.randn(n, generator=g) * 2 - 7)
+    eight.load_moments(m.cuda(), r.cuda(), 11)
+    a, b = eight.moments()
+    assert np.array_equal(_np(a), ref.held(m.numpy(), 3, 0.5)) and np.array_equal(_np(b), ref.held(r.numpy(), 4, 0.5))
+    for dt in (torch.bfloat16, torch.float32):
+        c, d = eight.moments(dt)
+        assert c.dtype == dt and torch.equal(c.float(), a) and torch.equal(d.float(), b)
+    eight.load_moments(a, b, 12)
+    assert all(torch.equal(x, y) for x, y in zip(eight.moments(), (a, b))) and int(eight.state[params[2]]["step"][3]) == 12
+    full.load_moments(a, b, 5)
+    assert torch.equal(full.states()[0], a) and torch.equal(full.states()[1], b * b) and torch.equal(full.moments()[0], a)
+    c, d = full.moments(torch.float16)
+    assert torch.equal(c, a.half()) and torch.equal(d, (b * b).sqrt().half())
+    for bad in ((m, r), (m.cuda()[:-1], r.cuda()[:-1]), (m.cuda().view(1, -1), r.cuda().view(1, -1))):
+        with pytest.raises(AssertionError):
+            full.load_moments(*bad, 5)
+    with pytest.raises(ValueError):
+        full.load_moments(m.cuda().double(), r.cuda(), 5)
+    with pytest.raises(ValueError):
+        full.moments(torch.float64)
+    with pytest.raises(AssertionError):
+        full.load_moments(m.cuda(), r.cuda(), -1)
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+def test_state_dicts_copies_and_pickles(cuda, bits):
+    """An optimizer that goes on from a saved state takes the same steps to the bit: a state dict through a file, a deep copy, a pickle."""
+    def fresh():
+        return _params([(640, 7), (1001,), (3,)], torch.bfloat16)
+
+    params = fresh()
+    opt = _opt([{"params": params[:1], "seed": 4}, {"params": params[1:]}], bits=bits, max_norm=2.0)
+    for t in range(3):
+        _grads(params, t)
+        opt.step()
+    file = io.BytesIO()
+    torch.save({"opt": opt.state_dict(), "p": params}, file)
+    file.seek(0)
+    saved = torch.load(file, weights_only=False, map_location="cpu")
+    others = [torch.nn.Parameter(p.detach().cuda()) for p in saved["p"]]
+    second = _opt([{"params": others[:1]}, {"params": others[1:]}], bits=40 - bits, max_norm=2.0)
+    _grads(others, 77)
+    second.step()                     # (states to be replaced, of the other kind)
+    with torch.no_grad():
+        for a, b in zip(others, params):
+            a.copy_(b)
+    second.load_state_dict(saved["opt"])
+    third_params, third = copy.deepcopy((params, opt))
+    file = io.BytesIO()
+    torch.save((params, opt), file)
+    file.seek(0)
+    fourth_params, fourth = torch.load(file, weights_only=False)
+    for t in range(5, 8):
+        for ps, o in ((params, opt), (others, second), (third_params, third), (fourth_params, fourth)):
+            _grads(ps, t)
+            o.step()
+    for ps, o in ((others, second), (third_params, third), (fourth_params, fourth)):
+        assert all(torch.equal(a, b) for a, b in zip(params, ps)) and o.max_norm == 2.0
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(opt.states(i), o.states(i)))
+            assert o.param_groups[i]["bits"] == bits
+        assert int(o.state[ps[0]]["step"][0]) == 6
+    wrong = copy.deepcopy(opt.state_dict())
+    wrong["param_groups"][0]["bits"] = 40 - bits
+    second.load_state_dict(wrong)
+    with pytest.raises(AssertionError, match="not those of"):
+        second.step()
+
+
+def test_groups_added_and_parameters_moved(cuda):
+    """A group added later; parameters whose memory is another (p.data assigned, a cast's copy) keep their states; a parameter in two places."""
+    a, b = _params([(700,), (50, 3)], torch.float32)
+    opt = _opt([a])
+    for t in (1, 2):
+        _grads([a], t)
+        before = _before(opt)
+        opt.step()
+        _check_step(opt, before, t)
+        a.data = a.data.clone()
+    opt.add_param_group({"params": [b], "bits": 8})
+    _grads([a, b], 3)
+    before = _before(opt)
+    opt.step()
+    assert int(opt.state[a]["step"][0]) == 3 and int(opt.state[b]["step"][0]) == 1
+    one = torch.zeros(100, device=cuda)
+    x, y = torch.nn.Parameter(one[:60]), torch.nn.Parameter(one[50:])
+    x.grad, y.grad = torch.ones_like(x), torch.ones_like(y)
+    with pytest.raises(AssertionError, match="share memory"):
+        _opt([x, y]).step()
+
+
+def test_refusals(cuda):
+    p = torch.nn.Parameter(torch.zeros(20, 20, device=cuda))
+    opt = _opt([p])
+    p.grad = torch.eye(20, device=cuda).to_sparse()
+    with pytest.raises(RuntimeError, match="sparse"):
+        opt.step()
+    p.grad = torch.ones_like(p)
+    gaps = torch.nn.Parameter(torch.zeros(20, 40, device=cuda)[:, ::2])
+    gaps.grad = torch.ones_like(gaps)
+    with pytest.raises(AssertionError, match="dense"):
+        _opt([gaps]).step()
+    cpu = torch.nn.Parameter(torch.zeros(3))
+    cpu.grad = torch.ones(3)
+    with pytest.raises(AssertionError):
+        _opt([p, cpu]).step()
+    with pytest.raises(AssertionError):
+        bad = _opt([p])
+        bad.param_groups[0]["betas"] = (1.0, 0.9)
+        bad.step()
+    assert not p.any() and not cpu.any()
+
+
+def test_autograd_sees_the_change(cuda):
+    p = torch.nn.Parameter(torch.ones(10, device=cuda))
+    out = (p * p).sum()
+    version = p._version
+    p.grad = torch.ones_like(p)
+    _opt([p]).step()
+    assert p._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+def test_captured_steps(cuda, bits):
+    """A captured step counts on with each replay and follows a rate on the GPU, with eager steps in between; the same steps taken eagerly
+    give the same bits. Two graphs of two optimizers at once."""
+    def make():
+        params = _params([(640, 16), (1001,), (77, 3)], torch.bfloat16)
+        lr = torch.tensor(1e-3, device=cuda)
+        return params, lr, _opt(params, bits=bits, lr=lr, max_norm=0.5)
+
+    (pa, la, a), (pb, lb, b) = make(), make()
+    _grads(pa, 0)
+    _grads(pb, 0)
+    static = [p.grad for p in pa]
+    new = _opt(_params([(5,)], torch.float32))
+    new.param_groups[0]["params"][0].grad = torch.ones(5, device=cuda)
+    a.step()
+    b.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    norm = a.grad_norm
+    for t in range(1, 7):
+        _grads(pb, t)
+        for g, p in zip(static, pb):
+            g.copy_(p.grad)
+        la.fill_(1e-3 / t)
+        lb.fill_(1e-3 / t)
+        if t == 4:
+            for g, p in zip(static, pa):
+                p.grad = g
+            a.step()                        # eager, between replays
+        else:
+            graph.replay()
+        b.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(pa, pb)), t
+        assert all(torch.equal(x, y) for x, y in zip(a.states(), b.states())), t
+        assert t == 4 or torch.equal(norm, b.grad_norm)
+    assert int(a.state[pa[0]]["step"][0]) == 7
+    fresh = _opt(_params([(5,)], torch.float32))
+    fresh.param_groups[0]["params"][0].grad = torch.ones(5, device=cuda)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(graph):
+            fresh.step()
+
+
+def test_other_streams(cuda):
+    params = _params([(640, 64)], torch.float32)
+    same = copy.deepcopy(params)
+    opt, again = _opt(params, bits=8, max_norm=1.0), _opt(same, bits=8, max_norm=1.0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for t in range(3):
+        with torch.cuda.stream(side):
+            _grads(params, t)
+            opt.step()
+        _grads(same, t)
+        again.step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(params[0], same[0]) and all(torch.equal(a, b) for a, b in zip(opt.states(), again.states()))
+
+
+def test_places_past_32_bits(cuda):
+    """One tensor of 2^31 + 1500 values in bf16 with 8-bit states: its first and last values against a small one's of the same place in
+    their blocks (the last by the definition: the hash takes the place's low 32 bits)."""
+    n = (1 << 31) + 1500
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device=cuda))
+    p.grad = torch.zeros_like(p)
+    ends = (slice(0, 1024), slice(n - 1500, n))
+    g = torch.Generator().manual_seed(1)
+    for e in ends:
+        p.data[e] = (torch.randn(e.stop - e.start, generator=g) * 0.02).bfloat16().cuda()
+        p.grad[e] = (torch.randn(e.stop - e.start, generator=g) * 1e-3).bfloat16().cuda()
+    was = [_np(p[e]) for e in ends]
+    opt = _opt([p], bits=8)
+    opt.step()
+    codes, roots, exps = opt.states()
+    assert not p[1024:1 << 30].any() and not p[1 << 30:n - 1500].any()
+    for e, p0 in zip(ends, was):
+        gr = _np(p.grad[e])
+        want, m, v = ref.step(p0, gr, 0 * gr, 0 * gr, 1, 1e-3)
+        off = 64 * F * (np.abs(p0) + 1e-3)
+        assert (np.abs(_np(p[e]) - want) <= off + HALF[torch.bfloat16] * (np.abs(want) + off)).all()
+        pad = -len(m) % 128
+        _, ur = ref.dither(np.arange(e.start, e.stop + pad), 1, 0)
+        blocks = slice(e.start // 128, (e.stop + 127) // 128)
+        E = exps[blocks, 1].cpu().numpy().astype(np.int64).repeat(128)
+        c = roots[e.start:e.stop + pad].cpu().numpy().astype(np.int64)
+        got = np.where(c > 0, (c + 16 * (E - 15)) << 19, 0).astype(np.uint32).view(np.float32).astype(np.float64)
+        exact = ref.held(np.pad(np.sqrt(v), (0, pad)), 4, ur)
+        assert (got != exact).mean() < 1e-2 and (np.abs(got - exact) <= 2.0 ** -4 * np.abs(exact)).all()
+    del codes
