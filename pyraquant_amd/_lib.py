@@ -56,6 +56,12 @@ EXPORTS = (
     "pq_mx_grad_input",
     "pq_mx_grad_factors_workspace_size",
     "pq_mx_grad_factors",
+    "pq_adapter_factors",
+    "pq_adapter_slices",
+    "pq_adapter_down",
+    "pq_adapter_up",
+    "pq_adapter_grads_workspace_size",
+    "pq_adapter_grads",
     "pq_grad_squares_partials",
     "pq_grad_squares",
     "pq_adamw_step",
@@ -133,6 +139,13 @@ _SIGNATURES = {
     "pq_mx_grad_factors_workspace_size": ([_i64, _i64, _i64, _i64], _i64),
     "pq_mx_grad_factors": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p],
                            ctypes.c_int),
+    "pq_adapter_factors": ([_p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
+    "pq_adapter_slices": ([_i64, _i64], _i64),
+    "pq_adapter_down": ([_p, _i32, _i64, _i64, _i64, _p, _i64, _i64, _p, _i32, _i64, _p, _p], ctypes.c_int),
+    "pq_adapter_up": ([_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _p, _i64, _i32, _i64, _p], ctypes.c_int),
+    "pq_adapter_grads_workspace_size": ([_i64, _i64, _i64, _i64, _i64], _i64),
+    "pq_adapter_grads": ([_p, _i64, _p, _i64, _i32, _p, _i64, _p, _i64, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p,
+                          _p, _i64, _p], ctypes.c_int),
     "pq_grad_squares_partials": ([_list], _i64),
     "pq_grad_squares": ([_list, _p, _i64, _p], ctypes.c_int),
     "pq_adamw_step": ([_list, _states, _rates, _p, _i64, _p, _p], ctypes.c_int),
@@ -187,6 +200,17 @@ def load_mx():
         raise LibraryMissing(f"pyraquant_amd/_mx.so is not built or does not load ({e}); run "
                              "`python -m pyraquant_amd.build`") from e
     return _mx
+
+
+def load_adapt():
+    """_adapt.so (csrc/pq_adapt_torch.cpp): adapters' call, differentiable, and the factors' orders."""
+    load()
+    try:
+        from . import _adapt
+    except ImportError as e:
+        raise LibraryMissing(f"pyraquant_amd/_adapt.so is not built or does not load ({e}); run "
+                             "`python -m pyraquant_amd.build`") from e
+    return _adapt
 
 
 def load_tune():

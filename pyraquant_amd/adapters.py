@@ -1,0 +1,248 @@
+"""Low-rank adapters of many requests at once beside one shared projection, for MI355X (gfx950).
+
+  LowRankAdapters(in, out, slots, rank)(x, y, ids)    y + scale[id] (x lr_A[id]) lr_B[id], id the adapter of each row's request
+  AdaptedLinear, add_adapters(model, slots, rank)     a model's Linears with adapters beside them
+  AdapterSet                                          the handle of a model's adapters: load, clear, and choose them for a batch
+
+The layers of int8_exec and mxfp4 hold one low-rank branch that belongs to the weight. Adapters belong to requests: a model is
+quantized once, styles or customers are tuned as small factors, and one batch serves any of them together, or tunes them together.
+``ids`` is an integer tensor on the GPU, one for each row or for each of x's leading dimensions (a batch of images: one an image);
+an id that names no adapter (-1) leaves its rows as they are. The kernels read ids, factors and scales when they run, so a
+captured graph follows what is written there.
+
+No request's results depend on the others of its batch. t = x lr_A is held in fp32 and taken to twice the factors' bits. Calls have first
+derivatives of the reverse kind (a second one, or a forward-mode tangent, raises). Every kernel runs on the caller's
+current stream; nothing synchronises. CPU tensors raise AssertionError; a missing library raises at the first call.
+"""
+from __future__ import annotations
+
+from typing import Callable, Dict, List, Mapping, Optional, Tuple
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from .int8_exec import Int8Linear, is_bf16_whitelisted
+from .mxfp4 import Mxfp4Linear
+from .weights import SplitInLinear
+
+MAX_RANK = 64     # of an adapter (the kernels hold 16, 32 or 64; other ranks run zero-padded)
+
+_adapt = None   # _adapt.so, loaded at the first use
+
+
+def _load_adapt():
+    global _adapt
+    _adapt = _lib.load_adapt().adapt
+    return _adapt
+
+
+def _padded(rank: int) -> int:
+    return 16 if rank <= 16 else 32 if rank <= 32 else 64
+
+
+class LowRankAdapters(nn.Module):
+    """``slots`` adapters of a projection: ``adapters(x, y, ids)`` is y + scale[id] (x lr_A[id]) lr_B[id]. x [..., in_features] and y
+    [..., out_features] in bf16 or fp16, features multiples of 8, ranks up to 64; ids as the module says. ``out=`` takes the result, y
+    itself for one: rows without an adapter are not touched then. (Only where nothing needs a gradient.)
+
+    ``trainable=False`` keeps the factors in the kernels' order as buffers (``lr_At`` [slots, P, K], ``lr_Bt`` [slots, N, P], zeros past
+    their ranks; ``lr_A`` and ``lr_B`` give them back). ``trainable=True`` makes ``lr_A`` [slots, K, rank] and ``lr_B`` [slots, rank, N]
+    parameters; freeze() turns such a module into the other kind. Factors of another type than x's are cast in each call. ``scale``
+    is a buffer in fp32, 0 for an empty slot. Gradients flow to x and y of either kind; adapters without rows get zeros."""
+
+    def __init__(self, in_features: int, out_features: int, slots: int, rank: int, *, dtype: torch.dtype = torch.bfloat16,
+                 device=None, trainable: bool = False):
+        super().__init__()
+        assert in_features > 0 and in_features % 8 == 0, f"in_features {in_features} is not a multiple of 8"
+        assert out_features > 0 and out_features % 8 == 0, f"out_features {out_features} is not a multiple of 8"
+        assert 1 <= slots <= 65535, f"{slots} adapters (1 to 65535)"
+        assert 1 <= rank <= MAX_RANK, f"rank {rank}: adapters take 1 to {MAX_RANK}"
+        if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise ValueError(f"unsupported dtype {dtype} (expected bfloat16, float16 or float32)")
+        self.in_features, self.out_features, self.slots, self.rank = in_features, out_features, slots, rank
+        self.trainable = bool(trainable)
+        zeros = lambda *shape: torch.zeros(shape, dtype=dtype, device=device)   # noqa: E731
+        if trainable:
+            self.lr_A = nn.Parameter(zeros(slots, in_features, rank))
+            self.lr_B = nn.Parameter(zeros(slots, rank, out_features))
+        else:
+            P = _padded(rank)
+            self.register_buffer("lr_At", zeros(slots, P, in_features))
+            self.register_buffer("lr_Bt", zeros(slots, out_features, P))
+        self.register_buffer("scale", torch.zeros(slots, device=device))
+
+    def _slot(self, slot: int) -> int:
+        assert 0 <= slot < self.slots, f"slot {slot} of {self.slots}"
+        return slot
+
+    @torch.no_grad()
+    def set(self, slot: int, lr_A: torch.Tensor, lr_B: torch.Tensor, scale: float = 1.0) -> None:
+        """An adapter into a slot: lr_A [K, r], lr_B [r, N], r up to the rank (zeros past it). On the current stream; captured graphs
+        take it from their next replay on."""
+        slot = self._slot(slot)
+        r = lr_A.shape[-1]
+        assert tuple(lr_A.shape) == (self.in_features, r) and tuple(lr_B.shape) == (r, self.out_features) and 1 <= r <= self.rank, (
+            tuple(lr_A.shape), tuple(lr_B.shape), self.in_features, self.out_features, self.rank)
+        if self.trainable:
+            A, B = self.lr_A[slot], self.lr_B[slot].t()
+        else:
+            A, B = self.lr_At[slot].t(), self.lr_Bt[slot]
+        for to, what in ((A, lr_A), (B, lr_B.t())):
+            to[:, :r].copy_(what)
+            to[:, r:].zero_()
+        self.scale[slot] = float(scale)
+
+    @torch.no_grad()
+    def clear(self, slot: int) -> None:
+        """An empty slot: its rows get y + 0."""
+        slot = self._slot(slot)
+        for t in (self.lr_A, self.lr_B) if self.trainable else (self.lr_At, self.lr_Bt):
+            t[slot].zero_()
+        self.scale[slot] = 0.0
+
+    def freeze(self, dtype: Optional[torch.dtype] = None) -> "LowRankAdapters":
+        """Turns a trainable module into one that serves, in ``dtype`` (give the inputs' type where the factors are in another), with the
+        same outputs."""
+        if self.trainable:
+            A, B, P = self.lr_A.detach(), self.lr_B.detach(), _padded(self.rank)
+            A, B = A.to(dtype or A.dtype), B.to(dtype or B.dtype)
+            del self.lr_A, self.lr_B
+            self.trainable = False
+            At, Bt = A.new_zeros((self.slots, P, self.in_features)), B.new_zeros((self.slots, self.out_features, P))
+            At[:, :self.rank] = A.transpose(1, 2)
+            Bt[:, :, :self.rank] = B.transpose(1, 2)
+            self.register_buffer("lr_At", At)
+            self.register_buffer("lr_Bt", Bt)
+        return self
+
+    def __getattr__(self, name):
+        if name in ("lr_A", "lr_B") and "lr_At" in self.__dict__.get("_buffers", ()):
+            return (self.lr_At[:, :self.rank] if name == "lr_A" else self.lr_Bt[:, :, :self.rank]).transpose(1, 2).contiguous()
+        return super().__getattr__(name)
+
+    def _apply(self, fn, recurse=True):
+        """A module-wide cast leaves the scales in fp32, as the kernels read them."""
+        keep = self._buffers["scale"]
+        super()._apply(fn, recurse)
+        new = self._buffers["scale"]
+        if new.dtype != torch.float32:
+            self._buffers["scale"] = keep.to(new.device)
+        return self
+
+    def forward(self, x: torch.Tensor, y: torch.Tensor, ids: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if self.trainable:
+            p = self._parameters
+            A, B = p["lr_A"], p["lr_B"]
+        else:
+            d = self._buffers
+            A, B = d["lr_At"], d["lr_Bt"]
+        dt = x.dtype
+        if (A.dtype != dt or B.dtype != dt) and dt in (torch.bfloat16, torch.float16):
+            A, B = A.to(dt), B.to(dt)
+        return (_adapt or _load_adapt())(x, y, ids, A, B, self._buffers["scale"], self.rank, not self.trainable, out)
+
+    def extra_repr(self) -> str:
+        kind = " (trainable)" if self.trainable else ""
+        return f"in={self.in_features}, out={self.out_features}, {self.slots} adapters, r={self.rank}{kind} (HIP gfx950)"
+
+
+class AdapterSet:
+    """The adapters of a model (add_adapters): one slot in every adapted layer. ``use(ids)`` chooses those of the batches that follow, None
+    none of them; as a context manager it puts the earlier choice back."""
+
+    def __init__(self, layers: Dict[str, LowRankAdapters]):
+        self.layers = layers
+        self.ids: Optional[torch.Tensor] = None
+
+    def use(self, ids: Optional[torch.Tensor]) -> "_Chosen":
+        chosen = _Chosen(self, self.ids)
+        self.ids = ids
+        return chosen
+
+    def set(self, slot: int, factors: Mapping[str, Tuple[torch.Tensor, torch.Tensor]], scale: float = 1.0) -> None:
+        """An adapter of the model into a slot: {layer's name: (lr_A, lr_B)}; layers that it does not name get none."""
+        unknown = sorted(set(factors) - set(self.layers))
+        assert not unknown, f"not adapted layers: {unknown[:4]}"
+        for name, bank in self.layers.items():
+            if name in factors:
+                bank.set(slot, *factors[name], scale)
+            else:
+                bank.clear(slot)
+
+    def get(self, slot: int) -> Dict[str, Tuple[torch.Tensor, torch.Tensor]]:
+        """{layer's name: (lr_A, lr_B)} of a slot, as set() takes them."""
+        return {name: (bank.lr_A[bank._slot(slot)].detach().clone(), bank.lr_B[slot].detach().clone()) for name, bank in self.layers.items()}
+
+    def clear(self, slot: int) -> None:
+        for bank in self.layers.values():
+            bank.clear(slot)
+
+    def parameters(self) -> List[nn.Parameter]:
+        """What tuning the adapters steps (none of frozen ones)."""
+        return [p for bank in self.layers.values() for p in bank.parameters()]
+
+    def freeze(self, dtype: Optional[torch.dtype] = None) -> "AdapterSet":
+        for bank in self.layers.values():
+            bank.freeze(dtype)
+        return self
+
+
+class _Chosen:
+    def __init__(self, adapters: AdapterSet, before: Optional[torch.Tensor]):
+        self._adapters, self._before = adapters, before
+
+    def __enter__(self) -> AdapterSet:
+        return self._adapters
+
+    def __exit__(self, *exc) -> None:
+        self._adapters.ids = self._before
+
+
+class AdaptedLinear(nn.Module):
+    """A projection that requests share and the adapters beside it: layer(x), and what ``chosen.ids`` says is added to it. (Routed
+    calls, with rows gathered or scattered, are a TypeError: their rows are not a batch's.)"""
+
+    def __init__(self, layer: nn.Module, adapters: LowRankAdapters, chosen: AdapterSet):
+        super().__init__()
+        self.layer, self.adapters = layer, adapters
+        self._chosen = chosen
+
+    @property
+    def in_features(self) -> int:
+        return self.layer.in_features
+
+    @property
+    def out_features(self) -> int:
+        return self.layer.out_features
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        y = self.layer(x)
+        ids = self._chosen.ids
+        if ids is None:
+            return y
+        # (the layer's result is a new tensor: without gradients what is added goes into it)
+        return self.adapters(x, y, ids, out=None if torch.is_grad_enabled() or not y.is_contiguous() else y)
+
+
+def add_adapters(model: nn.Module, slots: int, rank: int, *, dtype: Optional[torch.dtype] = None, trainable: bool = False,
+                 whitelist: Callable[[str], bool] = is_bf16_whitelisted) -> AdapterSet:
+    """Puts adapters beside the token-level Linears of a model in place (Int8Linear, Mxfp4Linear, SplitInLinear and nn.Linear whose features
+    are multiples of 8, but for whitelisted names, as the converters take them; convert first). All slots are empty. ``dtype``: the factors', bf16 if
+    not given. Where ``trainable``, the factors are the only parameters added; every other is left as it is."""
+    chosen = AdapterSet({})
+    inside = set()      # (modules of a layer that is taken)
+    for name, layer in list(model.named_modules()):
+        if not isinstance(layer, (nn.Linear, Int8Linear, Mxfp4Linear, SplitInLinear)) or whitelist(name) or layer in inside:
+            continue
+        assert name, "the model is itself a Linear: wrap it in a module"
+        if layer.in_features % 8 or layer.out_features % 8:
+            continue
+        first = next(iter([*layer.buffers(), *layer.parameters()]))
+        bank = LowRankAdapters(layer.in_features, layer.out_features, slots, rank, dtype=dtype or torch.bfloat16, device=first.device,
+                               trainable=trainable)
+        inside.update(layer.modules())
+        parent, _, attr = name.rpartition(".")
+        setattr(model.get_submodule(parent) if parent else model, attr, AdaptedLinear(layer, bank, chosen))
+        chosen.layers[name] = bank
+    return chosen

@@ -1,5 +1,5 @@
-"""Build libpqint8.so (the gfx950 HIP kernels + C ABI) in-tree with hipcc, and _direct.so, _mx.so and _tune.so (the eager layer
-calls and the optimizer's, CPython extensions over torch's C++ API and the library) with the host compiler.
+"""Build libpqint8.so (the gfx950 HIP kernels + C ABI) in-tree with hipcc, and _direct.so, _mx.so, _adapt.so and _tune.so (the
+eager layer calls and the optimizer's, CPython extensions over torch's C++ API and the library) with the host compiler.
 
     python -m pyraquant_amd.build          # compiles every csrc/*.hip, links pyraquant_amd/libpqint8.so, and the extensions
 
@@ -22,8 +22,10 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libpqint8.so")
 DIRECT_PATH = os.path.join(HERE, "_direct.so")
 MX_PATH = os.path.join(HERE, "_mx.so")
+ADAPT_PATH = os.path.join(HERE, "_adapt.so")
 TUNE_PATH = os.path.join(HERE, "_tune.so")
-EXTENSIONS = (("pq_torch.cpp", DIRECT_PATH), ("pq_mx_torch.cpp", MX_PATH), ("pq_tune_torch.cpp", TUNE_PATH))   # host code over torch's C++ API and the library
+EXTENSIONS = (("pq_torch.cpp", DIRECT_PATH), ("pq_mx_torch.cpp", MX_PATH), ("pq_adapt_torch.cpp", ADAPT_PATH),
+              ("pq_tune_torch.cpp", TUNE_PATH))   # host code over torch's C++ API and the library
 ARCH = "gfx950"
 
 HIP_FLAGS = [

@@ -11,26 +11,7 @@ namespace pq {
 namespace mx {
 namespace {
 
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4s lds_v4s_t;
 typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
-
-// Matrix operand from a tile held row-major along the other axis: lane l gets, of column c0 + l % 32, the 8 rows
-// r0 + 8 (l / 32) .. + 7. Each 16 lanes read a 4 x 16 patch (8 bytes a lane) that the transposing read hands back by
-// columns. `at(row, chunk)`: address of the 16 bytes holding columns 8 chunk .. of a row.
-//
-// Such a tile's rows are a multiple of 256 bytes, and 16 lanes read 32 bytes of each of 4 consecutive rows (32 lanes 64): chunk c
-// of a row sits at c ^ spread(row), so that those fall on distinct banks in 128- and in 256-byte windows (bits 1-2 of the
-// four values of spread are distinct, and so are bits 2-3).
-__device__ __forceinline__ int spread(int row) { return (0xca60 >> ((row & 3) << 2)) & 15; }
-template <typename At>
-__device__ __forceinline__ v4i read_columns(At at, int r0, int c0, int lane) {
-  const int i = lane & 15, row = r0 + 8 * (lane >> 5) + (i >> 2), col = c0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
-  union { v4s h[2]; v4i v; } u;
-  u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(at(row, col >> 3) + (col & 4) * 2));
-  u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(at(row + 4, col >> 3) + (col & 4) * 2));
-  return u.v;
-}
 
 // ---- dx = dy wh + dt A^T ---------------------------------------------------------------------------------------------
 struct DxArgs {
