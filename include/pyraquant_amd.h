@@ -473,35 +473,44 @@ int pq_mx_grad_factors(const void* dy, int32_t dtype, int64_t lddy, const float*
  *   t[m] = x[m] A[id],  y[m] = base[m] + scale[id] t[m] B[id]
  *   dt[m] = dy[m] B[id]^T,  dx[m] = scale[id] dt[m] A[id]^T,  dA[i] = scale[i] sum x^T dt,  dB[i] = scale[i] sum t^T dy over adapter i's rows
  * No row's result depends on another row's values or adapter. R is at most P, P 16, 32 or 64: what the factors are padded to with
- * zeros. K and N are multiples of 8, M at most 2^30; operands 16-byte aligned, row strides multiples of 8. dtype PQ_BF16 or PQ_F16.
+ * zeros. K and N are multiples of 8, M at most 2^30; operands 16-byte aligned, row strides multiples of 8 (of base
+ * and out at most 2^30). dtype PQ_BF16 or PQ_F16.
  *
- * The factors' orders, of all slots: by_rank [slots, P, C] and by_column [slots, C, P], C the columns (k of A, n of B).
- * pq_adapter_factors writes them from A [slots, K, R] (at: by rank, ap: by column) and B [slots, R, N] (bt: by column, bp: by rank),
- * contiguous; NULL where not wanted. The forward pass reads at and bt, the backward pass bp and ap. (A with R = P is its own ap, B its bp.)
+ * The factors' orders, C the columns (k of A, n of B): by column [slots, C, R] and by rank [slots, R, C], contiguous; and those that the
+ * kernels read, slots of pq_adapter_factor_size(C, P) values (C rounded up to 128, times P), zeros past C and R. Value (c, r) lies at
+ *   PQ_ADAPTER_DOWN  ((((c >> 5) * (P >> 4) + (r >> 4)) * 64 + ((c >> 3) & 3) * 16 + (r & 15)) * 8 + (c & 7)
+ *   PQ_ADAPTER_UP    (((c >> 7) * 8 + (c & 7)) * L + (r >> 3) * 16 + ((c >> 3) & 15)) * 8 + (r & 7), L = 2 P
+ * pq_adapter_factors writes these from A [K, R] and B [R, N] of each slot in any order (R = P where that is one of these); NULL where not
+ * wanted. The forward pass reads a_down and b_up, the backward pass b_down and a_up.
  */
-int pq_adapter_factors(const void* A, const void* B, int64_t slots, int64_t K, int64_t N, int64_t R, int64_t P, void* at, void* ap,
-                       void* bt, void* bp, hipStream_t stream);
+#define PQ_ADAPTER_BY_COLUMN 0
+#define PQ_ADAPTER_BY_RANK 1
+#define PQ_ADAPTER_DOWN 2
+#define PQ_ADAPTER_UP 3
+int64_t pq_adapter_factor_size(int64_t C, int64_t P);
+int pq_adapter_factors(const void* A, int32_t a_order, const void* B, int32_t b_order, int64_t slots, int64_t K, int64_t N, int64_t R,
+                       int64_t P, void* a_down, void* a_up, void* b_down, void* b_up, hipStream_t stream);
 
-/* part[s][m][r] ([slices, M, P] in fp32, slices = pq_adapter_slices(M, K)) = the sum over slice s of k of x[m, k] f[id][r][k], f by rank: t or
- * dt in parts. Rows without an adapter are left as they were. */
+/* part[s][m][r] ([slices, M, P] in fp32, slices = pq_adapter_slices(M, K)) = the sum over slice s of k of x[m, k] f[id][k, r], f in
+ * PQ_ADAPTER_DOWN: t or dt in parts. Rows without an adapter are left as they were. */
 int64_t pq_adapter_slices(int64_t M, int64_t K);
 int pq_adapter_down(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* f, int64_t slots, int64_t P,
                     const void* ids, int32_t id_bits, int64_t each, float* part, hipStream_t stream);
 
-/* out[m, c] = base[m, c] + scale[id] sum_r t[m, r] g[id][c][r] ([M, C]), t the sum of `slices` parts, g by column; summed in fp32 with t taken to
+/* out[m, c] = base[m, c] + scale[id] sum_r t[m, r] g[id][c, r] ([M, C]), t the sum of `slices` parts, g in PQ_ADAPTER_UP; summed in fp32 with t taken to
  * twice dtype's bits, rounded once. Rows without an adapter get base's bits. base NULL: zeros. out may be base, with the same stride (rows
- * without an adapter are not touched then), and must not overlap it otherwise. */
+ * without an adapter are not touched then), and must not overlap it otherwise. joined [M, P] in fp32, unless NULL, gets scale[id] t (zeros
+ * past R; rows without an adapter are left as they were); with out NULL, that alone. */
 int pq_adapter_up(const float* part, int64_t slices, const float* scale, const void* g, int64_t slots, int64_t C, int64_t R,
                   int64_t P, const void* ids, int32_t id_bits, int64_t each, const void* base, int64_t ldb, void* out, int64_t ldo,
-                  int32_t dtype, int64_t M, hipStream_t stream);
+                  float* joined, int32_t dtype, int64_t M, hipStream_t stream);
 
-/* dA [slots, K, R] and dB [slots, R, N] (zeros for an adapter without rows; NULL: not wanted, and its operands may be NULL), from t and dt in
- * parts as pq_adapter_down gives them, without the scale. Sums in fp32 in an order that depends on the sizes alone. The workspace may hold anything. */
+/* dA [slots, K, R] and dB [slots, R, N] (zeros for an adapter without rows; NULL: not wanted, and its operands may be NULL), from t and dt
+ * [M, P] with their scale, as pq_adapter_up joins them. Sums in fp32 in an order that depends on the sizes alone. The workspace may hold anything. */
 int64_t pq_adapter_grads_workspace_size(int64_t M, int64_t K, int64_t N, int64_t slots, int64_t P);
-int pq_adapter_grads(const void* x, int64_t ldx, const void* dy, int64_t lddy, int32_t dtype, const float* t, int64_t t_slices,
-                     const float* dt, int64_t dt_slices, const float* scale, const void* ids, int32_t id_bits, int64_t each,
-                     int64_t M, int64_t K, int64_t N, int64_t slots, int64_t R, int64_t P, void* dA, void* dB, void* workspace,
-                     int64_t workspace_bytes, hipStream_t stream);
+int pq_adapter_grads(const void* x, int64_t ldx, const void* dy, int64_t lddy, int32_t dtype, const float* t,
+                     const float* dt, const void* ids, int32_t id_bits, int64_t each, int64_t M, int64_t K, int64_t N, int64_t slots,
+                     int64_t R, int64_t P, void* dA, void* dB, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /*
  * ---- AdamW over the tensors of a model (no reference counterpart) ---------------------------------------------------

@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpqint8.s
 PQ_OK, PQ_EINVAL, PQ_ESHAPE, PQ_EALIGN, PQ_EDTYPE, PQ_ELAUNCH = 0, -1, -2, -3, -4, -5
 PQ_BF16, PQ_F16, PQ_I32, PQ_F32 = 0, 1, 2, 3
 PQ_MX_BY_COLUMN, PQ_MX_BY_RANK, PQ_MX_FRAGMENTS = 0, 1, 2   # orders of a low-rank factor (pq_mx_factors)
+PQ_ADAPTER_BY_COLUMN, PQ_ADAPTER_BY_RANK, PQ_ADAPTER_DOWN, PQ_ADAPTER_UP = 0, 1, 2, 3   # orders of an adapter's factor (pq_adapter_factors)
 PQ_ACCUMULATE = 0x100   # OR'ed into pq_int8_gemm_packed's out_dtype
 ABI_VERSION = 4
 
@@ -56,6 +57,7 @@ EXPORTS = (
     "pq_mx_grad_input",
     "pq_mx_grad_factors_workspace_size",
     "pq_mx_grad_factors",
+    "pq_adapter_factor_size",
     "pq_adapter_factors",
     "pq_adapter_slices",
     "pq_adapter_down",
@@ -139,13 +141,14 @@ _SIGNATURES = {
     "pq_mx_grad_factors_workspace_size": ([_i64, _i64, _i64, _i64], _i64),
     "pq_mx_grad_factors": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p],
                            ctypes.c_int),
-    "pq_adapter_factors": ([_p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
+    "pq_adapter_factor_size": ([_i64, _i64], _i64),
+    "pq_adapter_factors": ([_p, _i32, _p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p], ctypes.c_int),
     "pq_adapter_slices": ([_i64, _i64], _i64),
     "pq_adapter_down": ([_p, _i32, _i64, _i64, _i64, _p, _i64, _i64, _p, _i32, _i64, _p, _p], ctypes.c_int),
-    "pq_adapter_up": ([_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _p, _i64, _i32, _i64, _p], ctypes.c_int),
+    "pq_adapter_up": ([_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _p, _i64, _p, _i32, _i64, _p], ctypes.c_int),
     "pq_adapter_grads_workspace_size": ([_i64, _i64, _i64, _i64, _i64], _i64),
-    "pq_adapter_grads": ([_p, _i64, _p, _i64, _i32, _p, _i64, _p, _i64, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p,
-                          _p, _i64, _p], ctypes.c_int),
+    "pq_adapter_grads": ([_p, _i64, _p, _i64, _i32, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
+                         ctypes.c_int),
     "pq_grad_squares_partials": ([_list], _i64),
     "pq_grad_squares": ([_list, _p, _i64, _p], ctypes.c_int),
     "pq_adamw_step": ([_list, _states, _rates, _p, _i64, _p, _p], ctypes.c_int),

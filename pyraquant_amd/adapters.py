@@ -41,13 +41,40 @@ def _padded(rank: int) -> int:
     return 16 if rank <= 16 else 32 if rank <= 32 else 64
 
 
+def _room(columns: int) -> int:
+    return (columns + 127) // 128 * 128
+
+
+# The kernels' orders (pq_adapter_factors' PQ_ADAPTER_DOWN and PQ_ADAPTER_UP) as views with the axes of a matrix [..., columns, ranks]:
+# where a value lies is given by parts of its column and of its rank.
+def _down_axes(f: torch.Tensor) -> torch.Tensor:
+    """f [..., C, P] in the order of `down` -> [..., C / 32, 4, 8, P / 16, 16], the parts of c and of r"""
+    C, P = f.shape[-2:]
+    v = f.reshape(*f.shape[:-2], C // 32, P // 16, 4, 16, 8)      # c / 32, r / 16, c / 8 % 4, r % 16, c % 8
+    return v.movedim((-5, -3, -1, -4, -2), (-5, -4, -3, -2, -1))
+
+
+def _up_axes(f: torch.Tensor) -> torch.Tensor:
+    """f [..., C, P] in the order of `up` -> [..., C / 128, 16, 8, P / 8, 8], the parts of c and of r"""
+    C, P = f.shape[-2:]
+    v = f.reshape(*f.shape[:-2], C // 128, 8, P // 8, 16, 8)      # c / 128, c % 8, r / 8, c / 8 % 16, r % 8
+    return v.movedim((-5, -2, -4, -3, -1), (-5, -4, -3, -2, -1))
+
+
+def _write(axes: torch.Tensor, m: torch.Tensor, C: int, P: int) -> None:
+    """m [..., c, r] into a factor's order, zeros past its columns and ranks."""
+    full = m.new_zeros((*m.shape[:-2], C, P))
+    full[..., : m.shape[-2], : m.shape[-1]] = m
+    axes.copy_(full.view(axes.shape))
+
+
 class LowRankAdapters(nn.Module):
     """``slots`` adapters of a projection: ``adapters(x, y, ids)`` is y + scale[id] (x lr_A[id]) lr_B[id]. x [..., in_features] and y
     [..., out_features] in bf16 or fp16, features multiples of 8, ranks up to 64; ids as the module says. ``out=`` takes the result, y
     itself for one: rows without an adapter are not touched then. (Only where nothing needs a gradient.)
 
-    ``trainable=False`` keeps the factors in the kernels' order as buffers (``lr_At`` [slots, P, K], ``lr_Bt`` [slots, N, P], zeros past
-    their ranks; ``lr_A`` and ``lr_B`` give them back). ``trainable=True`` makes ``lr_A`` [slots, K, rank] and ``lr_B`` [slots, rank, N]
+    ``trainable=False`` keeps the factors in the kernels' orders as buffers (``lr_Af`` and ``lr_Bf``, [slots, features rounded up to 128,
+    P]; ``lr_A`` and ``lr_B`` give them back). ``trainable=True`` makes ``lr_A`` [slots, K, rank] and ``lr_B`` [slots, rank, N]
     parameters; freeze() turns such a module into the other kind. Factors of another type than x's are cast in each call. ``scale``
     is a buffer in fp32, 0 for an empty slot. Gradients flow to x and y of either kind; adapters without rows get zeros."""
 
@@ -68,8 +95,8 @@ class LowRankAdapters(nn.Module):
             self.lr_B = nn.Parameter(zeros(slots, rank, out_features))
         else:
             P = _padded(rank)
-            self.register_buffer("lr_At", zeros(slots, P, in_features))
-            self.register_buffer("lr_Bt", zeros(slots, out_features, P))
+            self.register_buffer("lr_Af", zeros(slots, _room(in_features), P))
+            self.register_buffer("lr_Bf", zeros(slots, _room(out_features), P))
         self.register_buffer("scale", torch.zeros(slots, device=device))
 
     def _slot(self, slot: int) -> int:
@@ -85,19 +112,19 @@ class LowRankAdapters(nn.Module):
         assert tuple(lr_A.shape) == (self.in_features, r) and tuple(lr_B.shape) == (r, self.out_features) and 1 <= r <= self.rank, (
             tuple(lr_A.shape), tuple(lr_B.shape), self.in_features, self.out_features, self.rank)
         if self.trainable:
-            A, B = self.lr_A[slot], self.lr_B[slot].t()
+            for to, what in ((self.lr_A[slot], lr_A), (self.lr_B[slot].t(), lr_B.t())):
+                to[:, :r].copy_(what)
+                to[:, r:].zero_()
         else:
-            A, B = self.lr_At[slot].t(), self.lr_Bt[slot]
-        for to, what in ((A, lr_A), (B, lr_B.t())):
-            to[:, :r].copy_(what)
-            to[:, r:].zero_()
+            for axes, f, what in ((_down_axes, self.lr_Af, lr_A), (_up_axes, self.lr_Bf, lr_B.t())):
+                _write(axes(f[slot]), what.to(f.device, f.dtype), *f.shape[1:])
         self.scale[slot] = float(scale)
 
     @torch.no_grad()
     def clear(self, slot: int) -> None:
         """An empty slot: its rows get y + 0."""
         slot = self._slot(slot)
-        for t in (self.lr_A, self.lr_B) if self.trainable else (self.lr_At, self.lr_Bt):
+        for t in (self.lr_A, self.lr_B) if self.trainable else (self.lr_Af, self.lr_Bf):
             t[slot].zero_()
         self.scale[slot] = 0.0
 
@@ -109,16 +136,17 @@ class LowRankAdapters(nn.Module):
             A, B = A.to(dtype or A.dtype), B.to(dtype or B.dtype)
             del self.lr_A, self.lr_B
             self.trainable = False
-            At, Bt = A.new_zeros((self.slots, P, self.in_features)), B.new_zeros((self.slots, self.out_features, P))
-            At[:, :self.rank] = A.transpose(1, 2)
-            Bt[:, :, :self.rank] = B.transpose(1, 2)
-            self.register_buffer("lr_At", At)
-            self.register_buffer("lr_Bt", Bt)
+            for name, axes, m, features in (("lr_Af", _down_axes, A, self.in_features), ("lr_Bf", _up_axes, B.transpose(1, 2), self.out_features)):
+                f = m.new_zeros((self.slots, _room(features), P))
+                _write(axes(f), m, _room(features), P)
+                self.register_buffer(name, f)
         return self
 
     def __getattr__(self, name):
-        if name in ("lr_A", "lr_B") and "lr_At" in self.__dict__.get("_buffers", ()):
-            return (self.lr_At[:, :self.rank] if name == "lr_A" else self.lr_Bt[:, :, :self.rank]).transpose(1, 2).contiguous()
+        if name in ("lr_A", "lr_B") and "lr_Af" in self.__dict__.get("_buffers", ()):
+            if name == "lr_A":
+                return _down_axes(self.lr_Af).reshape(self.lr_Af.shape)[:, : self.in_features, : self.rank].contiguous()
+            return _up_axes(self.lr_Bf).reshape(self.lr_Bf.shape)[:, : self.out_features, : self.rank].transpose(1, 2).contiguous()
         return super().__getattr__(name)
 
     def _apply(self, fn, recurse=True):
@@ -131,12 +159,13 @@ class LowRankAdapters(nn.Module):
         return self
 
     def forward(self, x: torch.Tensor, y: torch.Tensor, ids: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        assert x.shape[-1] == self.in_features and y.shape[-1] == self.out_features, (tuple(x.shape), tuple(y.shape), self.in_features, self.out_features)
         if self.trainable:
             p = self._parameters
             A, B = p["lr_A"], p["lr_B"]
         else:
             d = self._buffers
-            A, B = d["lr_At"], d["lr_Bt"]
+            A, B = d["lr_Af"], d["lr_Bf"]
         dt = x.dtype
         if (A.dtype != dt or B.dtype != dt) and dt in (torch.bfloat16, torch.float16):
             A, B = A.to(dt), B.to(dt)

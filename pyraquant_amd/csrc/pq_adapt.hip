@@ -6,15 +6,16 @@
 // adapters of a tile of 64 rows are taken one after the other, each with its own rows packed together (`passes`), so a NaN in one
 // request or adapter stays there.
 //
-//   down  part[s][m][r] = sum over slice s of k of x[m, k] f[id][r][k]          (t and dt without the scale; slices are added where
+//   down  part[s][m][r] = sum over slice s of k of x[m, k] f[id][k, r]          (t and dt without the scale; slices are added where
 //                                                                                    they are read)
-//   up    out[m, c] = base[m, c] + scale[id] sum_r part[m, r] g[id][c][r]
+//   up    out[m, c] = base[m, c] + scale[id] sum_r part[m, r] g[id][c, r], and scale[id] part[m], the slices added, for `sums`
 //   sums  the two sums over rows, per adapter, over chunks of the rows, added by `join` in their order
 // All sums are fp32. t and dt are taken by the 16-bit matrix instructions in two parts (two_parts), so their rounding shows in no
 // result. No atomics: the same bits every time. Bound by memory: 2 R operations for each value that is read.
 #include "pq_mx.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace pq {
 namespace adapt {
@@ -60,9 +61,26 @@ __device__ __forceinline__ void passes(int mine, int z, bool shared, F f) {
   }
 }
 
+// Memory wants neighbouring lanes in neighbouring 16 bytes. With a row a lane (what a matrix operand is), each lane needs a line of its own from
+// the first cache, and 65536 x 5120 x rank 64 ran at 3.6 TB/s, bound by that; so x goes through LDS, a result's lane is eight columns
+// (`up`), and the factors are kept in the order in which a wave's lanes read them.
+//
+// The factors' orders, of a factor with columns c (k of A, n of B) and ranks r < P: C rounded up to 128, P values each.
+__host__ __device__ __forceinline__ int64_t factor_size(int64_t C, int P) { return (C + 127) / 128 * 128 * P; }
+// for `down`: of 32 columns and 16 ranks, lane 16 ((c >> 3) & 3) + (r & 15) holds eight columns
+__device__ __forceinline__ int64_t down_at(int c, int r, int P) {
+  return ((int64_t)((c >> 5) * (P >> 4) + (r >> 4)) * 64 + (c >> 3 & 3) * 16 + (r & 15)) * 8 + (c & 7);
+}
+// for `up`: of the 16 columns c with one c & 7 of 128, and 32 ranks (16 with P 16), lane 16 ((r >> 3) & 3) + ((c >> 3) & 15) holds eight ranks
+__device__ __forceinline__ int64_t up_at(int c, int r, int P) {
+  return ((int64_t)((c >> 7) * 8 + (c & 7)) * (2 * P) + (r >> 3) * 16 + (c >> 3 & 15)) * 8 + (r & 7);
+}
+
 // ---- down ----------------------------------------------------------------------------------------------------------------
-// A workgroup takes 64 rows and a slice of k, 128 k a step, 32 for each of its four waves, whose sums are added in LDS. The factor is the
-// first operand, so that a lane's sums are of one row and four consecutive ranks.
+// A wave takes 16 NS rows and 64 k a step, the next step on its way meanwhile; x goes through its part of LDS (8 lanes a row; chunk c of a
+// row at c ^ (row % 8), so that neither direction meets a bank twice). The factor is the first operand, so that a lane's sums are of one row
+// and four consecutive ranks. The four waves of a workgroup take 32 rows each and the same slice of k; with few rows (ROWS false) the same 64
+// rows, 16 at a time, and every fourth step, and add their sums in LDS.
 struct DownArgs {
   const uint16_t *x, *f;
   Ids ids;
@@ -71,126 +89,194 @@ struct DownArgs {
   int M, K, slice;
 };
 
-template <int DT, int J, int NS>
-__device__ __forceinline__ void down_pass(const DownArgs& p, int id, int row0, int list, int count, v4f* lds) {
+template <int DT, int J, int NS, bool ROWS, bool ONE>
+__device__ __forceinline__ void down_pass(const DownArgs& p, int id, int row0, int list, int count, uint8_t* lds) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
-  const int k0 = (int)blockIdx.y * p.slice, k1 = min(p.K, k0 + p.slice);
-  const uint16_t* x[NS];
-  int row[NS];
+  const int k0 = (int)blockIdx.y * p.slice, k1 = min(p.K, k0 + p.slice), stride = ROWS ? 64 : 256;
+  const int piece = lane & 7;
+  uint8_t* const turn = lds + wave * (ROWS ? 4096 : 2048);   // (waves may hold different NS)
+  const uint16_t* x[NS * 2];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    row[s] = row0 + __shfl(list, 16 * s + l16);
-    x[s] = p.x + (int64_t)min(row[s], p.M - 1) * p.ldx;
-  }
-  const uint16_t* const f = p.f + ((int64_t)id * (16 * J) + l16) * p.K;
+  for (int i = 0; i < NS * 2; ++i) x[i] = p.x + (int64_t)(row0 + __shfl(list, min(8 * i + (lane >> 3), count - 1))) * p.ldx;
+  constexpr int SLAB = 2 * J * 64, MINE = SLAB / 256 ? SLAB / 256 : 1;   // 16-byte pieces of 64 k; of a thread
+  const v4u* const f = reinterpret_cast<const v4u*>(p.f + id * factor_size(p.K, 16 * J)) + (ONE ? threadIdx.x % SLAB : lane);
+  v4u* const slab = reinterpret_cast<v4u*>(lds + 16384);
   v4f acc[J][NS] = {};
-  for (int k = k0 + wave * 32; k < k1; k += 128) {
-    const int at = k + 8 * g, from = min(at, p.K - 8);
-    const bool in = at < k1;
-    v4i xs[NS], fs[J];
+  struct Step {
+    v4u x[NS * 2], f[ONE ? MINE : 2 * J];
+  };
+  auto load = [&](Step& b, int k) {
+    const int from = min(k + 8 * piece, p.K - 8);
 #pragma unroll
-    for (int s = 0; s < NS; ++s) xs[s] = *reinterpret_cast<const v4i*>(x[s] + from);
+    for (int i = 0; i < NS * 2; ++i) b.x[i] = *reinterpret_cast<const v4u*>(x[i] + from);
 #pragma unroll
-    for (int j = 0; j < J; ++j) fs[j] = *reinterpret_cast<const v4i*>(f + (int64_t)(16 * j) * p.K + from);
+    for (int i = 0; i < (ONE ? MINE : 2 * J); ++i) b.f[i] = f[(int64_t)(k >> 6) * SLAB + i * (ONE ? 256 : 64)];
+  };
+  auto products = [&](const Step& b, int k, int n) {
+    const uint32_t in = k + 8 * piece < k1 ? ~0u : 0u;   // zeros past the end (the factor's are, but an infinity times zero would be NaN)
+    wave_sync();
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) xs[s][e] = in ? xs[s][e] : 0;
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) fs[j][e] = in ? fs[j][e] : 0;
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int j = 0; j < J; ++j) acc[j][s] = mfma16_16<DT>(fs[j], xs[s], acc[j][s]);
-  }
-  // wave w adds the tiles (j, s) of those with index % 4 == w; the others' go through LDS
-#pragma unroll
-  for (int i = 0; i < J * NS; ++i)
-    if ((i & 3) != wave) lds[(wave * (J * NS) + i) * 64 + lane] = acc[i / NS][i % NS];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < J * NS; ++i) {
-    if ((i & 3) != wave) continue;
-    v4f sum = acc[i / NS][i % NS];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      const v4f o = lds[((wave ^ w) * (J * NS) + i) * 64 + lane];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += o[e];
+    for (int i = 0; i < NS * 2; ++i) {
+      const int r = 8 * i + (lane >> 3);
+      *reinterpret_cast<v4u*>(turn + r * 128 + ((piece ^ (r & 7)) << 4)) = b.x[i] & in;
     }
-    const int s = i % NS, j = i / NS;
-    if (16 * s + l16 < count)
-      *reinterpret_cast<v4f*>(p.part + ((int64_t)blockIdx.y * p.M + row[s]) * (16 * J) + 16 * j + 4 * g) = sum;
+    wave_sync();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const v4i xs = *reinterpret_cast<const v4i*>(turn + (16 * s + l16) * 128 + (((4 * h + g) ^ (l16 & 7)) << 4));
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          acc[j][s] = mfma16_16<DT>(__builtin_bit_cast(v4i, ONE ? slab[n * SLAB + (h * J + j) * 64 + lane] : b.f[ONE ? 0 : h * J + j]), xs, acc[j][s]);
+      }
+  };
+  int k = k0 + (ROWS ? 0 : wave * 64);
+  if (k < k1) {   // (past the end the first step is loaded again: no branch between a step's loads and the products that wait for the one before)
+    const int first = k;
+    Step b[2];
+    load(b[0], k);
+    for (int n = 0; k < k1; k += stride, n ^= 1) {
+      if constexpr (ONE) {   // the workgroup's rows have one adapter: its waves share a step's factor in LDS. Two slabs, one barrier a step
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) slab[n * SLAB + (i * 256 + threadIdx.x) % SLAB] = b[0].f[i];
+      }
+      load(b[1], k + stride < k1 ? k + stride : first);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (ONE) ring_barrier();
+      products(b[0], k, n);
+      b[0] = b[1];
+    }
   }
-  __syncthreads();
+  if constexpr (ROWS) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const int row = row0 + __shfl(list, min(16 * s + l16, count - 1));   // (the last one's sums are written more than once)
+      float* const to = p.part + ((int64_t)blockIdx.y * p.M + row) * (16 * J) + 4 * g;
+#pragma unroll
+      for (int j = 0; j < J; ++j) *reinterpret_cast<v4f*>(to + 16 * j) = acc[j][s];
+    }
+  } else {   // wave w adds ranks 16 w .. 16 w + 15 of the four waves' sums
+    v4f* const sums = reinterpret_cast<v4f*>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < J; ++j) sums[(wave * J + j) * 64 + lane] = acc[j][0];
+    __syncthreads();
+    if (wave < J) {
+      v4f sum = sums[wave * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        const v4f o = sums[(w * J + wave) * 64 + lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += o[e];
+      }
+      const int row = row0 + __shfl(list, min(l16, count - 1));
+      *reinterpret_cast<v4f*>(p.part + ((int64_t)blockIdx.y * p.M + row) * (16 * J) + 16 * wave + 4 * g) = sum;
+    }
+    __syncthreads();
+  }
 }
 
-template <int DT, int J>
+template <int DT, int J, bool ROWS>
 __global__ __launch_bounds__(256) void adapter_down_kernel(const DownArgs p) {
-  __shared__ v4f lds[4 * J * 4 * 64];
-  const int lane = threadIdx.x & 63, row0 = (int)blockIdx.x * 64;
-  const int mine = row0 + lane < p.M ? p.ids.of(row0 + lane) : -1;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[ROWS ? 16384 + 4096 * J : (J < 2 ? 8192 : 4096 * J)];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int row0 = (int)blockIdx.x * (ROWS ? 128 : 64);
+  if constexpr (ROWS) {
+    const int a = row0 + lane < p.M ? p.ids.of(row0 + lane) : -1, b = row0 + 64 + lane < p.M ? p.ids.of(row0 + 64 + lane) : -1;
+    const int id = __builtin_amdgcn_readfirstlane(a);
+    if (id >= 0 && __ballot(a == id && b == id) == ~0ull) {
+      if (blockIdx.z == 0) down_pass<DT, J, 2, true, true>(p, id, row0 + wave * 32, lane, 32, lds);
+      return;
+    }
+    row0 += wave * 32;
+  }
+  const int mine = (!ROWS || lane < 32) && row0 + lane < p.M ? p.ids.of(row0 + lane) : -1;
   passes(mine, blockIdx.z, gridDim.z > 1, [&](int id, uint64_t match) {
-    const int list = packed_rows(match, lane), count = __popcll(match);
-    if (count <= 16) down_pass<DT, J, 1>(p, id, row0, list, count, lds);
-    else if (count <= 32) down_pass<DT, J, 2>(p, id, row0, list, count, lds);
-    else down_pass<DT, J, 4>(p, id, row0, list, count, lds);
+    int list = packed_rows(match, lane), count = __popcll(match);
+    if constexpr (ROWS) {
+      if (count <= 16) down_pass<DT, J, 1, true, false>(p, id, row0, list, count, lds);
+      else down_pass<DT, J, 2, true, false>(p, id, row0, list, count, lds);
+    } else {
+      for (; count > 0; count -= 16, list = __shfl(list, lane + 16)) down_pass<DT, J, 1, false, false>(p, id, row0, list, count, lds);
+    }
   });
 }
 
 // ---- up ------------------------------------------------------------------------------------------------------------------
-// A workgroup takes 64 rows and `cols` columns, a wave 64 columns a step. The factor is the first operand, its rows in an order in
-// which a lane's sums over four tiles are 16 consecutive columns of one row. With rank 16 one instruction takes both parts of t.
+// A wave takes 16 rows and 128 columns a step: eight tiles of 16 x 16, tile u of the columns with c % 8 == u, so that a lane's sums are
+// eight consecutive columns of four rows, and 16 lanes' 256 bytes of a row. The four waves of a workgroup take 16 rows each and the same `cols`
+// columns; with few rows (ROWS false) the same 64 rows, 16 at a time, and every fourth step. With rank 16 one instruction takes both
+// parts of t.
 struct UpArgs {
   const float *part, *scale;
   const uint16_t* g;
   Ids ids;
   const uint16_t* base;   // BASE; zeros without
   uint16_t* out;
-  int64_t ldb, ldo;
-  int M, C, R, slices, cols, blocks;   // blocks of columns
+  float* joined;          // [M, P]: t with its scale, or NULL
+  int ldb, ldo, M, C, R, slices, cols, blocks;   // columns of a workgroup, such blocks of columns
+  int stream;                          // whether results go past the caches
 };
 
-template <int DT, int P, bool BASE, int NS>
-__device__ __forceinline__ void up_pass(const UpArgs& p, int id, int row0, int list, int count, int c_begin, int c_end) {
-  constexpr int KS = P == 16 ? 1 : P / 32, PARTS = P == 16 ? 1 : 2;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
+template <int DT, int P, bool BASE, int NS, bool ROWS, bool ONE>
+__device__ __forceinline__ void up_pass(const UpArgs& p, int id, int row0, int list, int count, int c, int c_end, bool join, uint8_t* lds) {
+  constexpr int KS = P == 16 ? 1 : P / 32, PARTS = P == 16 ? 1 : 2, STEP = ROWS ? 128 : 512, LANES = P == 16 ? 32 : 64;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4, gr = P == 16 ? g & 1 : g;
   const float scale = p.scale[id];
-  int row[NS];
+  int line[NS][4];   // rows of the sums; past the count the last one, whose results are written more than once
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) line[s][i] = row0 + __shfl(list, min(16 * s + 4 * g + i, count - 1));
   v4i t[NS][KS][PARTS];
-  float back[NS];
+  float back[NS][4];
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
-    row[s] = row0 + __shfl(list, 16 * s + l16);
-    float m = 0.0f;
+    const int row = row0 + __shfl(list, min(16 * s + l16, count - 1));
     RankPiece piece[KS];
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      const int r = 32 * k + 8 * (P == 16 ? g & 1 : g);
-      const float* at = p.part + (int64_t)min(row[s], p.M - 1) * P + r;
+      const float* at = p.part + (int64_t)row * P + 32 * k + 8 * gr;
+      const int64_t step = (int64_t)p.M * P;
       piece[k].load(at);
-      for (int i = 1; i < p.slices; ++i) {
-        at += (int64_t)p.M * P;
+      int i = 1;
+      constexpr int AT_ONCE = 4;   // loads in flight
+      for (; i + AT_ONCE <= p.slices; i += AT_ONCE) {
+        RankPiece more[AT_ONCE];
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; ++n) more[n].load(at + (i + n) * step);
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; ++n)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) piece[k].raw[e >> 2][e & 3] += more[n].raw[e >> 2][e & 3];
+      }
+      for (; i < p.slices; ++i) {
         RankPiece more;
-        more.load(at);
+        more.load(at + i * step);
 #pragma unroll
         for (int e = 0; e < 8; ++e) piece[k].raw[e >> 2][e & 3] += more.raw[e >> 2][e & 3];
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {   // (ranks past R are sums of zeros times x, and may be NaN)
         const float v = piece[k].raw[e >> 2][e & 3] * scale;
-        piece[k].raw[e >> 2][e & 3] = r + e < p.R ? v : 0.0f;
+        piece[k].raw[e >> 2][e & 3] = 32 * k + 8 * gr + e < p.R ? v : 0.0f;
       }
-      m = fmaxf(m, piece[k].largest());
+      if (join && (P != 16 || g < 2)) {
+        v4f* const to = reinterpret_cast<v4f*>(p.joined + (int64_t)row * P + 32 * k + 8 * gr);
+        to[0] = piece[k].raw[0];
+        to[1] = piece[k].raw[1];
+      }
     }
-    back[s] = 1.0f;
     if constexpr (DT == PQ_F16) {   // rows past fp16's end are taken times a power of two
+      float m = piece[0].largest();
+#pragma unroll
+      for (int k = 1; k < KS; ++k) m = fmaxf(m, piece[k].largest());
       m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
       const float down = scale_down(__float_as_uint(m));
-      back[s] = scale_back(down);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) back[s][i] = scale_back(__shfl(down, 4 * g + i));
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -208,83 +294,169 @@ __device__ __forceinline__ void up_pass(const UpArgs& p, int id, int row0, int l
       }
     }
   }
-  const uint16_t* const f = p.g + (int64_t)id * p.C * P + 8 * (P == 16 ? g & 1 : g);
-  for (int c0 = c_begin + wave * 64; c0 < c_end; c0 += 256) {
-    v4i fs[4][KS];
+  v4u b[NS][4], ahead[NS][4];   // this step's base, and the next one's
+  v4f acc[NS][8];
+  auto load = [&](int c0) {
+    if constexpr (BASE) {
+      const int from = min(c0 + 8 * l16, p.C - 8);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int c = min(c0 + 16 * (l16 >> 2) + 4 * u + (l16 & 3), p.C - 1);
+      for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int k = 0; k < KS; ++k) fs[u][k] = *reinterpret_cast<const v4i*>(f + (int64_t)c * P + 32 * k);
+        for (int i = 0; i < 4; ++i) ahead[s][i] = *reinterpret_cast<const v4u*>(p.base + (int64_t)line[s][i] * p.ldb + from);
     }
-    v4u b[NS][2];
-    const int c = c0 + 16 * g;
+  };
+  auto take = [&] {
+    if constexpr (BASE) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[s][i] = ahead[s][i];
+    }
+  };
+  auto products = [&](const v4u* from, int step) {   // from, step: the lane's place in a tile's factor, and from tile to tile
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        b[s][h] = BASE ? *reinterpret_cast<const v4u*>(p.base + (int64_t)min(row[s], p.M - 1) * p.ldb + min(c + 8 * h, p.C - 8)) : v4u{0, 0, 0, 0};
+      for (int u = 0; u < 8; ++u) acc[s][u] = v4f{};
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      v4f acc[4] = {};
+    for (int u = 0; u < 8; ++u)
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
+      for (int k = 0; k < KS; ++k) {
+        const v4i fs = __builtin_bit_cast(v4i, from[(u * KS + k) * step]);
 #pragma unroll
-        for (int part = PARTS - 1; part >= 0; --part)
+        for (int s = 0; s < NS; ++s)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) acc[u] = mfma16_16<DT>(fs[u][k], t[s][k][part], acc[u]);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        v4u o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const v4f& a = acc[2 * h + (e >> 1)];
-          float lo = a[2 * (e & 1)], hi = a[2 * (e & 1) + 1];
-          if constexpr (DT == PQ_F16) lo *= back[s], hi *= back[s];
-          o[e] = BASE ? pack2<DT>(lo + lo16_to_f32<DT>(b[s][h][e]), hi + hi16_to_f32<DT>(b[s][h][e])) : pack2<DT>(lo, hi);
-        }
-        if (16 * s + l16 < count && c + 8 * h < p.C) *reinterpret_cast<v4u*>(p.out + (int64_t)row[s] * p.ldo + c + 8 * h) = o;
+          for (int part = PARTS - 1; part >= 0; --part) acc[s][u] = mfma16_16<DT>(t[s][k][part], fs, acc[s][u]);
       }
+  };
+  auto result = [&](int s, int i) {
+    v4u o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float lo = acc[s][2 * e][i], hi = acc[s][2 * e + 1][i];
+      if constexpr (DT == PQ_F16) lo *= back[s][i], hi *= back[s][i];
+      if constexpr (BASE) lo += lo16_to_f32<DT>(b[s][i][e]), hi += hi16_to_f32<DT>(b[s][i][e]);
+      o[e] = pack2<DT>(lo, hi);
+    }
+    return o;
+  };
+  auto place = [&](int s, int i, int c0) { return reinterpret_cast<v4u*>(p.out + (int64_t)line[s][i] * p.ldo + c0 + 8 * l16); };
+  const v4u* const factor = reinterpret_cast<const v4u*>(p.g + id * factor_size(p.C, P));
+  constexpr int SLAB = 8 * KS * LANES;   // 16-byte pieces of 128 columns
+  const int first = c;
+  if (c < c_end) load(c);
+  if constexpr (ONE) {
+    // The workgroup's rows have one adapter: its waves share a step's factor in LDS, where it costs the way from memory a quarter of what
+    // it does from the first cache (65536 x 5120 x rank 64: 389 us without). Two slabs, one barrier a step.
+    constexpr int MINE = SLAB / 256 ? SLAB / 256 : 1;
+    const int tid = threadIdx.x;
+    v4u* const slab = reinterpret_cast<v4u*>(lds);
+    v4u next[MINE];
+    auto fetch = [&](int c0) {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) next[i] = factor[(int64_t)(c0 >> 7) * SLAB + i * 256 + tid];
+    };
+    auto put = [&](int which) {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) slab[which * SLAB + i * 256 + tid] = next[i];
+    };
+    if (c + 128 <= c_end) {
+      fetch(c);
+      put(0);
+      ring_barrier();
+      for (int n = 0; c + 128 <= c_end; c += 128, n ^= 1) {   // (past the end the first step again: no branch between loads and what waits for those before)
+        take();
+        fetch(c + 256 <= c_end ? c + 128 : first);
+        load(c + 128 < c_end ? c + 128 : first);
+        __builtin_amdgcn_sched_barrier(0);
+        products(slab + n * SLAB + (lane & (LANES - 1)), LANES);
+        if (p.stream) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) __builtin_nontemporal_store(result(0, i), place(0, i, c));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *place(0, i, c) = result(0, i);
+        }
+        put(n ^ 1);
+        ring_barrier();
+      }
+    }
+  }
+  for (; c < c_end; c += STEP) {
+    take();
+    if (c + STEP < c_end) load(c + STEP);
+    products(factor + (int64_t)(c >> 7) * SLAB + (lane & (LANES - 1)), LANES);
+    if (c + 8 * l16 < p.C) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *place(s, i, c) = result(s, i);
     }
   }
 }
 
-template <int DT, int P, bool BASE>
+template <int DT, int P, bool BASE, bool ROWS>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const UpArgs p) {
-  const int lane = threadIdx.x & 63, tile = (int)blockIdx.x / p.blocks, row0 = tile * 64;
-  const int c_begin = ((int)blockIdx.x - tile * p.blocks) * p.cols, c_end = min(p.C, c_begin + p.cols);
-  const int mine = row0 + lane < p.M ? p.ids.of(row0 + lane) : -1;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[ROWS ? 512 * P : 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = (int)blockIdx.x / p.blocks, block = (int)blockIdx.x - tile * p.blocks;
+  const int c_begin = block * p.cols + (ROWS ? 0 : wave * 128), c_end = min(p.C, (block + 1) * p.cols);
+  const bool join = p.joined && block == 0 && (ROWS || wave == 0);
+  int row0 = tile * 64;
+  bool mine_in = row0 + lane < p.M;
+  int mine = mine_in ? p.ids.of(row0 + lane) : -1;
+  if constexpr (ROWS) {
+    const int id = __builtin_amdgcn_readfirstlane(mine);
+    if (id >= 0 && __ballot(mine == id) == ~0ull) {
+      if (blockIdx.z == 0) up_pass<DT, P, BASE, 1, true, true>(p, id, row0 + wave * 16, lane, 16, c_begin, c_end, join, lds);
+      return;
+    }
+    row0 += wave * 16;
+    mine = __shfl(mine, wave * 16 + (lane & 15));
+    mine_in = lane < 16 && row0 + lane < p.M;
+    if (!mine_in) mine = -1;
+  }
   passes(mine, blockIdx.z, gridDim.z > 1, [&](int id, uint64_t match) {
-    const int list = packed_rows(match, lane), count = __popcll(match);
-    if (count <= 16) up_pass<DT, P, BASE, 1>(p, id, row0, list, count, c_begin, c_end);
-    else if (count <= 32) up_pass<DT, P, BASE, 2>(p, id, row0, list, count, c_begin, c_end);
-    else up_pass<DT, P, BASE, 4>(p, id, row0, list, count, c_begin, c_end);
+    int list = packed_rows(match, lane), count = __popcll(match);
+    for (; count > 0; count -= 16, list = __shfl(list, lane + 16)) up_pass<DT, P, BASE, 1, ROWS, false>(p, id, row0, list, count, c_begin, c_end, join, lds);
   });
   if (blockIdx.z || (BASE && p.out == p.base)) return;
-  const uint64_t none = __ballot(mine < 0 && row0 + lane < p.M);   // rows without an adapter, 16 at a time, 16 lanes a row
+  // rows without an adapter, 16 at a time, 16 lanes a row, eight loads in flight
+  const uint64_t none = __ballot(mine < 0 && mine_in);
   const int list = packed_rows(none, lane), count = __popcll(none);
+  constexpr int STEP = ROWS ? 128 : 512;
   for (int i0 = 0; i0 < count; i0 += 16) {
-    const int i = i0 + (threadIdx.x >> 4), row = row0 + __shfl(list, i);
-    if (i >= count) continue;
-    for (int c = c_begin + (threadIdx.x & 15) * 8; c < c_end; c += 128) {
-      v4u v = v4u{0, 0, 0, 0};
-      if (BASE) v = *reinterpret_cast<const v4u*>(p.base + (int64_t)row * p.ldb + c);
-      *reinterpret_cast<v4u*>(p.out + (int64_t)row * p.ldo + c) = v;
+    int64_t row[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) row[i] = row0 + __shfl(list, min(i0 + 4 * i + (lane >> 4), count - 1));   // (the last one more than once)
+    for (int c = c_begin + (lane & 15) * 8; c < c_end; c += 2 * STEP) {
+      v4u v[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[h][i] = BASE ? *reinterpret_cast<const v4u*>(p.base + row[i] * p.ldb + min(c + h * STEP, p.C - 8)) : v4u{0, 0, 0, 0};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (c + h * STEP < c_end) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<v4u*>(p.out + row[i] * p.ldo + c + h * STEP) = v[h][i];
+        }
     }
   }
 }
 
 // ---- sums over the rows of an adapter ------------------------------------------------------------------------------------
-// part[chunk][slot][r][c] = sum over the chunk's rows m of that adapter of v[m, r] z[m, c], v = scale (the sum of `slices` parts). A
+// part[chunk][slot][r][c] = sum over the chunk's rows m of that adapter of v[m, r] z[m, c], v: t or dt with its scale (`joined`). A
 // workgroup of four waves takes 128 columns, a chunk of rows and an adapter; of its rows, 64 a step, only steps that hold a row of
 // the adapter are read, the next one's on their way into registers meanwhile, with zeros in the place of other adapters' rows.
 struct SumArgs {
   const uint16_t* z;
-  const float *v, *scale;
+  const float* v;
   float* part;
   int32_t* used;          // [chunk][slot]: whether part was written
   int64_t ldz;
-  int M, C, slices, rows, panels, blocks;   // rows of a chunk (a multiple of 64), panels of 128 columns, blocks: panels * chunks, or 0
+  int M, C, rows, panels, blocks;   // rows of a chunk (a multiple of 64), panels of 128 columns, blocks: panels * chunks, or 0
 };
 
 template <int DT, int P>
@@ -309,7 +481,6 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int b
     }
     return end;
   };
-  const float scale = p.scale[slot];
   v16f acc[TILES] = {};
   v4u zr[4];
   v4f vr[P / 16];
@@ -325,18 +496,7 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int b
     for (int i = 0; i < P / 16; ++i) {
       const int at = i * 256 + tid, r = at / (P / 4);
       vr[i] = v4f{};
-      if (match >> r & 1) {
-        const float* from = p.v + (int64_t)(m0 + r) * P + at % (P / 4) * 4;
-        vr[i] = *reinterpret_cast<const v4f*>(from);
-        for (int s = 1; s < p.slices; ++s) {
-          from += (int64_t)p.M * P;
-          const v4f more = *reinterpret_cast<const v4f*>(from);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vr[i][e] += more[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vr[i][e] *= scale;
-      }
+      if (match >> r & 1) vr[i] = *reinterpret_cast<const v4f*>(p.v + (int64_t)(m0 + r) * P + at % (P / 4) * 4);
     }
   };
   auto rank = [&](int j) { return P == 16 ? lane & 15 : 32 * j + (lane & 31); };
@@ -452,53 +612,99 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(const JoinArgs b, con
   const bool is_b = (int)blockIdx.x < b.blocks;
   const JoinArgs p = is_b ? b : a;
   const int block = (int)blockIdx.x - (is_b ? 0 : b.blocks), slot = blockIdx.y;
-  const int c = block % p.groups * 64 + (threadIdx.x & 63), r = block / p.groups * 4 + (threadIdx.x >> 6);
-  if (c >= p.C || r >= R) return;
+  const int lane = threadIdx.x & 63, c = block % p.groups * 64 + lane, r = block / p.groups * 4 + (threadIdx.x >> 6);
   float s = 0.0f;
-  for (int i = 0; i < p.chunks; ++i)
-    if (p.used[i * slots + slot]) s += p.part[(((int64_t)i * slots + slot) * P + r) * p.C + c];
+  const float* const at = p.part + ((int64_t)slot * P + min(r, P - 1)) * p.C + min(c, p.C - 1);
+  const int64_t step = (int64_t)slots * P * p.C;
+  for (int i0 = 0; i0 < p.chunks; i0 += 64) {
+    uint64_t used = __ballot(i0 + lane < p.chunks && p.used[min(i0 + lane, p.chunks - 1) * slots + slot]);
+    while (used) {   // eight loads in flight
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = 0.0f;
+        if (used) v[e] = at[(i0 + __ffsll((unsigned long long)used) - 1) * step];
+        used &= used - 1;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += v[e];
+    }
+  }
+  if (c >= p.C || r >= R) return;
   p.out[(int64_t)slot * R * p.C + (is_b ? (int64_t)r * p.C + c : (int64_t)c * R + r)] = (uint16_t)f32_to_16_bits<DT>(s);
 }
 
 // ---- the factors' orders -------------------------------------------------------------------------------------------------
-// A [C, R] or [R, C] of each slot, to [P, C] and [C, P] with zeros past R: 64 columns a workgroup, turned in LDS.
+// A factor of each slot from any of its orders to those of `down` and `up`, with zeros past R and C: 128 columns a workgroup, in LDS between.
 struct FactorArgs {
   const uint16_t* from;
-  uint16_t *by_rank, *by_column;   // [P, C], [C, P]
-  int C, blocks, ranks_first;
+  uint16_t *down, *up;
+  int C, blocks, order;   // of `from`
 };
 __global__ __launch_bounds__(256) void adapter_factors_kernel(const FactorArgs a, const FactorArgs b, int R, int P) {
-  __shared__ uint16_t tile[64][66];   // [c][r]; a pitch of 33 words: both directions spread over the banks
+  __shared__ uint16_t tile[128][66];   // [c][r]; a pitch of 33 words: both directions spread over the banks
   const bool is_a = (int)blockIdx.x < a.blocks;
   const FactorArgs p = is_a ? a : b;
-  const int c0 = ((int)blockIdx.x - (is_a ? 0 : a.blocks)) * 64, slot = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint16_t* const from = p.from + (int64_t)slot * R * p.C;
-  for (int i = threadIdx.x; i < 64 * P; i += 256) {
-    const int c = p.ranks_first ? i & 63 : i / P, r = p.ranks_first ? i >> 6 : i % P;
-    uint16_t v = 0;
-    if (r < R && c0 + c < p.C) v = from[p.ranks_first ? (int64_t)r * p.C + c0 + c : (int64_t)(c0 + c) * R + r];
-    tile[c][r] = v;
+  const int c0 = ((int)blockIdx.x - (is_a ? 0 : a.blocks)) * 128, slot = blockIdx.y;
+  const bool packed = p.order >= PQ_ADAPTER_DOWN;
+  const uint16_t* const from = p.from + slot * (packed ? factor_size(p.C, P) : (int64_t)R * p.C);
+  const bool wide = (uintptr_t)p.from % 16 == 0;
+  for (int i = threadIdx.x; i < 16 * P; i += 256) {   // eight values: of columns c .. c + 7, or of ranks r .. r + 7
+    const bool by_rank = p.order == PQ_ADAPTER_BY_RANK || p.order == PQ_ADAPTER_DOWN;
+    int c, r;
+    if (p.order == PQ_ADAPTER_DOWN) r = i % P, c = i / P * 8;
+    else if (p.order == PQ_ADAPTER_UP) c = i % 16 * 8 + i / 16 % 8, r = i / 128 * 8;
+    else if (by_rank) c = i % 16 * 8, r = i / 16;
+    else c = i / (P / 8), r = i % (P / 8) * 8;
+    uint16_t v[8] = {};
+    if (r < R && c0 + c < p.C) {
+      const uint16_t* const at = from + (p.order == PQ_ADAPTER_DOWN ? down_at(c0 + c, r, P) : p.order == PQ_ADAPTER_UP ? up_at(c0 + c, r, P)
+                                         : by_rank ? (int64_t)r * p.C + c0 + c : (int64_t)(c0 + c) * R + r);
+      if (packed || (wide && (by_rank || R % 8 == 0))) {
+        const v4u w = *reinterpret_cast<const v4u*>(at);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (by_rank || r + e < R) v[e] = at[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tile[c + (by_rank ? e : 0)][r + (by_rank ? 0 : e)] = v[e];
   }
   __syncthreads();
-  if (p.by_rank && c0 + lane < p.C)
-    for (int r = wave; r < P; r += 4) p.by_rank[((int64_t)slot * P + r) * p.C + c0 + lane] = tile[lane][r];
-  if (p.by_column)
-    for (int i = threadIdx.x; i < 64 * P; i += 256)
-      if (c0 + i / P < p.C) p.by_column[((int64_t)slot * p.C + c0) * P + i] = tile[i / P][i % P];
+  const int64_t to = slot * factor_size(p.C, P);
+  for (int i = threadIdx.x; i < 16 * P; i += 256) {
+    v4u w;
+    if (p.down) {
+      const int r = i % 16 + i / 64 % (P / 16) * 16, c = i / 16 % 4 * 8 + i / (4 * P) * 32;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = tile[c + 2 * e][r] | (uint32_t)tile[c + 2 * e + 1][r] << 16;
+      *reinterpret_cast<v4u*>(p.down + to + down_at(c0 + c, r, P)) = w;
+    }
+    if (p.up) {
+      const int c = i % 16 * 8 + i / (2 * P) % 8, r = i / 16 % (P / 8) * 8;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = tile[c][r + 2 * e] | (uint32_t)tile[c][r + 2 * e + 1] << 16;
+      *reinterpret_cast<v4u*>(p.up + to + up_at(c0 + c, r, P)) = w;
+    }
+  }
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------------
 constexpr int kMostSlices = 16;
-int64_t tiles_of(int64_t M) { return (M + 63) / 64; }
-// k of a slice: about 1024 workgroups, but 256 k each or more
+bool by_rows(int64_t M) { return M >= 128; }   // the waves of a workgroup take rows of their own (128 of them), else 64 rows together
+int64_t tiles_of(int64_t M) { return by_rows(M) ? (M + 127) / 128 : (M + 63) / 64; }
+// k of a slice: about 512 workgroups, but four steps of a wave each or more (with few rows one)
 int slice_of(int64_t M, int64_t K) {
-  const int64_t steps = (K + 255) / 256, want = std::min<int64_t>({1024 / std::max<int64_t>(tiles_of(M), 1), steps, (int64_t)kMostSlices});
+  const int64_t steps = (K + 255) / 256, want = std::min<int64_t>({512 / std::max<int64_t>(tiles_of(M), 1), steps, (int64_t)kMostSlices});
   const int64_t n = std::max<int64_t>(want, 1);
   return (int)((steps + n - 1) / n * 256);
 }
 int slices_of(int64_t M, int64_t K) { const int s = slice_of(M, K); return (int)((K + s - 1) / s); }
-// Workgroups that share a tile's adapters: 64 where few rows may hold many adapters, else each takes them in turn.
-int sharers(int64_t M, int64_t each) { return each < 16 && M <= 1024 ? 64 : 1; }
+// Workgroups that share a tile's adapters: one for each of its rows where few rows may hold many adapters, else one takes them in turn.
+int sharers(int64_t M, int64_t each) { return each < 16 && M <= 1024 ? (by_rows(M) ? 32 : 64) : 1; }
 
 int64_t chunk_rows(int64_t M, int64_t C, int64_t slots, int64_t P) {
   const int64_t steps = std::max<int64_t>((M + 63) / 64, 1), panels = (C + 127) / 128;
@@ -556,7 +762,11 @@ extern "C" int pq_adapter_down(const void* x, int32_t dtype, int64_t M, int64_t 
   const DownArgs p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(f), ids_of(ids, id_bits, each, slots), part, ldx, (int)M, (int)K, slice};
   if (const int st = check_grid(tiles_of(M), 256, "pq_adapter_down")) return st;
   const dim3 grid((unsigned)tiles_of(M), (unsigned)slices_of(M, K), (unsigned)sharers(M, each));
-#define PQ_DOWN(D, PP) hipLaunchKernelGGL((adapter_down_kernel<D, PP / 16>), grid, dim3(256), 0, stream, p)
+#define PQ_DOWN(D, PP)                                                                                              \
+  do {                                                                                                              \
+    if (by_rows(M)) hipLaunchKernelGGL((adapter_down_kernel<D, PP / 16, true>), grid, dim3(256), 0, stream, p);     \
+    else hipLaunchKernelGGL((adapter_down_kernel<D, PP / 16, false>), grid, dim3(256), 0, stream, p);               \
+  } while (0)
   PQ_BY_TYPE(PQ_DOWN);
 #undef PQ_DOWN
   return check_launch("pq_adapter_down");
@@ -564,31 +774,39 @@ extern "C" int pq_adapter_down(const void* x, int32_t dtype, int64_t M, int64_t 
 
 extern "C" int pq_adapter_up(const float* part, int64_t slices, const float* scale, const void* g, int64_t slots, int64_t C, int64_t R,
                              int64_t P, const void* ids, int32_t id_bits, int64_t each, const void* base, int64_t ldb, void* out,
-                             int64_t ldo, int32_t dtype, int64_t M, hipStream_t stream) {
-  if (M < 0 || M > (1 << 30) || !size_ok(C) || ldo < C || (base && ldb < C) || !rank_ok(R, P) || slices < 1 || slices > kMostSlices)
+                             int64_t ldo, float* joined, int32_t dtype, int64_t M, hipStream_t stream) {
+  if (M < 0 || M > (1 << 30) || !size_ok(C) || (out && (ldo < C || ldo > (1 << 30))) || (base && (ldb < C || ldb > (1 << 30))) || !rank_ok(R, P) || slices < 1 || slices > kMostSlices)
     return set_error(PQ_ESHAPE, "pq_adapter_up: M=%lld C=%lld ldb=%lld ldo=%lld R=%lld P=%lld slices=%lld (C a multiple of 8)", (long long)M,
                      (long long)C, (long long)ldb, (long long)ldo, (long long)R, (long long)P, (long long)slices);
   if (dtype != PQ_BF16 && dtype != PQ_F16) return set_error(PQ_EDTYPE, "pq_adapter_up: dtype %d", dtype);
   if (const int st = check_ids(ids, id_bits, each, M, slots, "pq_adapter_up")) return st;
   if (M == 0) return PQ_OK;
-  if (!part || !scale || !g || !out) return set_error(PQ_EINVAL, "pq_adapter_up: null pointer");
-  if ((uintptr_t)part % 16 || (uintptr_t)g % 16 || (uintptr_t)base % 16 || (base && ldb % 8) || (uintptr_t)out % 16 || ldo % 8)
+  if (!part || !scale || (!out && (!joined || base)) || (out && !g)) return set_error(PQ_EINVAL, "pq_adapter_up: null pointer");
+  if ((uintptr_t)part % 16 || (uintptr_t)g % 16 || (uintptr_t)base % 16 || (base && ldb % 8) || (uintptr_t)out % 16 || ldo % 8 || (uintptr_t)joined % 16)
     return set_error(PQ_EALIGN, "pq_adapter_up: operands 16-byte aligned, strides multiples of 8");
-  if (base == out && ldb != ldo) return set_error(PQ_ESHAPE, "pq_adapter_up: out is base, with another stride");
-  const int64_t tiles = tiles_of(M), steps = (C + 255) / 256;
-  const int64_t want = std::min<int64_t>(steps, std::max<int64_t>(2048 / tiles, 1)), each_steps = (steps + want - 1) / want;
-  const int blocks = (int)((steps + each_steps - 1) / each_steps);
+  if (out && base == out && ldb != ldo) return set_error(PQ_ESHAPE, "pq_adapter_up: out is base, with another stride");
+  // about 1024 workgroups
+  const bool rows = by_rows(M);
+  const int64_t tiles = (M + 63) / 64, width = rows ? 128 : 512, steps = out ? (C + width - 1) / width : 0;
+  const int64_t want = std::max<int64_t>(std::min<int64_t>(steps, 1024 / tiles), 1), each_steps = (steps + want - 1) / want;
+  const int blocks = steps ? (int)((steps + each_steps - 1) / each_steps) : 1;   // (no output: no columns)
   const UpArgs p{part, scale, static_cast<const uint16_t*>(g), ids_of(ids, id_bits, each, slots), static_cast<const uint16_t*>(base),
-                 static_cast<uint16_t*>(out), ldb, ldo, (int)M, (int)C, (int)R, (int)slices, (int)each_steps * 256, blocks};
+                 static_cast<uint16_t*>(out), joined, (int)ldb, (int)ldo, (int)M, (int)C, (int)R, (int)slices, (int)(each_steps * width), blocks,
+                 M * C >= 32 << 20};   // (64 MB: they would drive out what is read next. 8202 x 5120 78 -> 73 us with `down`, 16384 x 5120 and its backward pass 240 -> 227)
   if (const int st = check_grid(tiles * blocks, 256, "pq_adapter_up")) return st;
-  const dim3 grid((unsigned)(tiles * blocks), 1, (unsigned)sharers(M, each));
-#define PQ_UP(D, PP)                                                                                     \
-  do {                                                                                                   \
-    if (base) hipLaunchKernelGGL((adapter_up_kernel<D, PP, true>), grid, dim3(256), 0, stream, p);       \
-    else hipLaunchKernelGGL((adapter_up_kernel<D, PP, false>), grid, dim3(256), 0, stream, p);           \
+  const dim3 grid((unsigned)(tiles * blocks), 1, (unsigned)(rows ? std::min(sharers(M, each), 16) : sharers(M, each)));
+#define PQ_UP2(D, PP, B)                                                                                    \
+  do {                                                                                                      \
+    if (rows) hipLaunchKernelGGL((adapter_up_kernel<D, PP, B, true>), grid, dim3(256), 0, stream, p);       \
+    else hipLaunchKernelGGL((adapter_up_kernel<D, PP, B, false>), grid, dim3(256), 0, stream, p);           \
+  } while (0)
+#define PQ_UP(D, PP)                                          \
+  do {                                                        \
+    if (base) PQ_UP2(D, PP, true); else PQ_UP2(D, PP, false); \
   } while (0)
   PQ_BY_TYPE(PQ_UP);
 #undef PQ_UP
+#undef PQ_UP2
   return check_launch("pq_adapter_up");
 }
 
@@ -604,18 +822,17 @@ extern "C" int64_t pq_adapter_grads_workspace_size(int64_t M, int64_t K, int64_t
   return bytes;
 }
 
-extern "C" int pq_adapter_grads(const void* x, int64_t ldx, const void* dy, int64_t lddy, int32_t dtype, const float* t, int64_t t_slices,
-                                const float* dt, int64_t dt_slices, const float* scale, const void* ids, int32_t id_bits, int64_t each,
+extern "C" int pq_adapter_grads(const void* x, int64_t ldx, const void* dy, int64_t lddy, int32_t dtype, const float* t,
+                                const float* dt, const void* ids, int32_t id_bits, int64_t each,
                                 int64_t M, int64_t K, int64_t N, int64_t slots, int64_t R, int64_t P, void* dA, void* dB, void* workspace,
                                 int64_t workspace_bytes, hipStream_t stream) {
-  if (M < 0 || M > (1 << 30) || !size_ok(K) || !size_ok(N) || (dA && ldx < K) || (dB && lddy < N) || !rank_ok(R, P) ||
-      (dB && (t_slices < 1 || t_slices > kMostSlices)) || (dA && (dt_slices < 1 || dt_slices > kMostSlices)))
+  if (M < 0 || M > (1 << 30) || !size_ok(K) || !size_ok(N) || (dA && ldx < K) || (dB && lddy < N) || !rank_ok(R, P))
     return set_error(PQ_ESHAPE, "pq_adapter_grads: M=%lld K=%lld N=%lld R=%lld P=%lld (K and N multiples of 8)", (long long)M, (long long)K,
                      (long long)N, (long long)R, (long long)P);
   if (dtype != PQ_BF16 && dtype != PQ_F16) return set_error(PQ_EDTYPE, "pq_adapter_grads: dtype %d", dtype);
   if (const int st = check_ids(ids, id_bits, each, M, slots, "pq_adapter_grads")) return st;
   if (!dA && !dB) return PQ_OK;
-  if (!workspace || !scale || (M && ((dB && (!dy || !t)) || (dA && (!x || !dt))))) return set_error(PQ_EINVAL, "pq_adapter_grads: null pointer");
+  if (!workspace || (M && ((dB && (!dy || !t)) || (dA && (!x || !dt))))) return set_error(PQ_EINVAL, "pq_adapter_grads: null pointer");
   if ((dA && ((uintptr_t)x % 16 || ldx % 8 || (uintptr_t)dt % 16)) || (dB && ((uintptr_t)dy % 16 || lddy % 8 || (uintptr_t)t % 16)) ||
       (uintptr_t)workspace % 16)
     return set_error(PQ_EALIGN, "pq_adapter_grads: operands 16-byte aligned, strides multiples of 8");
@@ -631,8 +848,7 @@ extern "C" int pq_adapter_grads(const void* x, int64_t ldx, const void* dy, int6
     at += padded_bytes(4 * chunks * slots * P * C);
     int32_t* const used = reinterpret_cast<int32_t*>(at);
     at += padded_bytes(4 * chunks * slots);
-    sums[i] = {static_cast<const uint16_t*>(b ? dy : x), b ? t : dt, scale, part, used, b ? lddy : ldx, (int)M, (int)C,
-               (int)(b ? t_slices : dt_slices), (int)rows, (int)panels, wanted ? (int)(panels * chunks) : 0};
+    sums[i] = {static_cast<const uint16_t*>(b ? dy : x), b ? t : dt, part, used, b ? lddy : ldx, (int)M, (int)C, (int)rows, (int)panels, wanted ? (int)(panels * chunks) : 0};
     join[i] = {part, used, static_cast<uint16_t*>(b ? dB : dA), (int)chunks, (int)C, (int)groups, wanted ? (int)(groups * ((R + 3) / 4)) : 0};
   }
   // (no rows: no adapter has any, and the ids are not read)
@@ -648,16 +864,22 @@ extern "C" int pq_adapter_grads(const void* x, int64_t ldx, const void* dy, int6
   return check_launch("pq_adapter_grads");
 }
 
-extern "C" int pq_adapter_factors(const void* A, const void* B, int64_t slots, int64_t K, int64_t N, int64_t R, int64_t P, void* at, void* ap,
-                                  void* bt, void* bp, hipStream_t stream) {
+extern "C" int64_t pq_adapter_factor_size(int64_t C, int64_t P) { return size_ok(C) && rank_ok(1, P) ? factor_size(C, (int)P) : 0; }
+
+extern "C" int pq_adapter_factors(const void* A, int32_t a_order, const void* B, int32_t b_order, int64_t slots, int64_t K, int64_t N, int64_t R,
+                                  int64_t P, void* a_down, void* a_up, void* b_down, void* b_up, hipStream_t stream) {
   if (!size_ok(K) || !size_ok(N) || !rank_ok(R, P) || slots < 1 || slots > 65535)
     return set_error(PQ_ESHAPE, "pq_adapter_factors: %lld adapters, K=%lld N=%lld R=%lld P=%lld", (long long)slots, (long long)K, (long long)N,
                      (long long)R, (long long)P);
-  const bool want_a = at || ap, want_b = bt || bp;
+  if (a_order < 0 || a_order > PQ_ADAPTER_UP || b_order < 0 || b_order > PQ_ADAPTER_UP)
+    return set_error(PQ_EINVAL, "pq_adapter_factors: orders %d and %d", a_order, b_order);
+  const bool want_a = a_down || a_up, want_b = b_down || b_up;
   if ((want_a && !A) || (want_b && !B)) return set_error(PQ_EINVAL, "pq_adapter_factors: null pointer");
-  const FactorArgs a{static_cast<const uint16_t*>(A), static_cast<uint16_t*>(at), static_cast<uint16_t*>(ap), (int)K, want_a ? (int)((K + 63) / 64) : 0, 0};
-  const FactorArgs b{static_cast<const uint16_t*>(B), static_cast<uint16_t*>(bp), static_cast<uint16_t*>(bt), (int)N, want_b ? (int)((N + 63) / 64) : 0, 1};
+  for (const void* to : {(const void*)a_down, (const void*)a_up, (const void*)b_down, (const void*)b_up, a_order >= PQ_ADAPTER_DOWN ? A : nullptr, b_order >= PQ_ADAPTER_DOWN ? B : nullptr})
+    if ((uintptr_t)to % 16) return set_error(PQ_EALIGN, "pq_adapter_factors: orders of `down` and `up` 16-byte aligned");
   if (!want_a && !want_b) return PQ_OK;
+  const FactorArgs a{static_cast<const uint16_t*>(A), static_cast<uint16_t*>(a_down), static_cast<uint16_t*>(a_up), (int)K, want_a ? (int)((K + 127) / 128) : 0, a_order};
+  const FactorArgs b{static_cast<const uint16_t*>(B), static_cast<uint16_t*>(b_down), static_cast<uint16_t*>(b_up), (int)N, want_b ? (int)((N + 127) / 128) : 0, b_order};
   hipLaunchKernelGGL(adapter_factors_kernel, dim3((unsigned)(a.blocks + b.blocks), (unsigned)slots), dim3(256), 0, stream, a, b, (int)R, (int)P);
   return check_launch("pq_adapter_factors");
 }

@@ -2,7 +2,7 @@
 //
 //   adapt(x, y, ids, lr_A, lr_B, scale, rank, laid_out, out or None) -> y + scale[id] (x lr_A[id]) lr_B[id]
 //
-// lr_A [slots, K, R] and lr_B [slots, R, N], or (laid_out) lr_A by rank [slots, P, K] and lr_B by column [slots, N, P]. Work goes to the current stream of x's device.
+// lr_A [slots, K, R] and lr_B [slots, R, N], or (laid_out) lr_A in PQ_ADAPTER_DOWN and lr_B in PQ_ADAPTER_UP, [slots, C, P] with C rounded up to 128. Work goes to the current stream of x's device.
 #include <Python.h>
 
 #include <ATen/core/grad_mode.h>
@@ -45,7 +45,7 @@ Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options
 Tensor rows_of(const Tensor& t) {
   Tensor x = t.is_neg() ? t.resolve_neg() : t;
   const int64_t M = x.size(0), K = x.size(1);
-  if ((K > 1 && x.stride(1) != 1) || (M > 1 && (x.stride(0) < K || x.stride(0) % 8)) || (uintptr_t)x.const_data_ptr() % 16)
+  if ((K > 1 && x.stride(1) != 1) || (M > 1 && (x.stride(0) < K || x.stride(0) % 8 || x.stride(0) > (1 << 30))) || (uintptr_t)x.const_data_ptr() % 16)
     x = x.clone(at::MemoryFormat::Contiguous);
   return x;
 }
@@ -63,19 +63,20 @@ struct Factors {   // in the orders that a pass reads
   const void *down, *up;
 };
 
-// out [M, N] from x [M, K] and y [M, N]; parts: [slices, M, P] in fp32, kept by the backward pass.
+// out [M, N] from x [M, K] and y [M, N]; parts: scratch; joined: t with its scale [M, P], kept for the backward pass, or NULL.
 void forward(const Tensor& x, const Tensor& y, const Tensor& ids, const Tensor& scale, Factors f, const Sizes& z, const Tensor& out,
-             float* parts, hipStream_t stream) {
+             float* parts, float* joined, hipStream_t stream) {
   check(pq_adapter_down(x.const_data_ptr(), code_of(x), z.M, z.K, stride_of(x), f.down, z.slots, z.P, ids.const_data_ptr(), z.id_bits,
                         z.each, parts, stream),
         "adapters");
   check(pq_adapter_up(parts, pq_adapter_slices(z.M, z.K), data<float>(scale), f.up, z.slots, z.N, z.R, z.P, ids.const_data_ptr(), z.id_bits,
-                      z.each, y.const_data_ptr(), stride_of(y), out.data_ptr(), stride_of(out), code_of(x), z.M, stream),
+                      z.each, y.const_data_ptr(), stride_of(y), out.data_ptr(), stride_of(out), joined, code_of(x), z.M, stream),
         "adapters");
 }
+int64_t factor_bytes(const Sizes& z, int64_t C) { return up(2 * z.slots * pq_adapter_factor_size(C, z.P)); }
 int64_t parts_bytes(const Sizes& z, int64_t C) { return up(4 * pq_adapter_slices(z.M, C) * z.M * z.P); }
 
-// The whole call. `kept`, where the backward pass will need it: t in parts.
+// The whole call. `kept`, where the backward pass will need it: t.
 Tensor run(const Tensor& x0, const Tensor& y0, const Tensor& ids, const Tensor& A, const Tensor& B, const Tensor& scale, const Sizes& z,
            bool laid_out, Tensor out, bool keep, Tensor& kept) {
   const c10::DeviceGuard guard(x0.device());
@@ -83,17 +84,19 @@ Tensor run(const Tensor& x0, const Tensor& y0, const Tensor& ids, const Tensor& 
   const bool in_place = out.defined() && out.const_data_ptr() == y0.const_data_ptr();
   const Tensor x = rows_of(x0), y = in_place ? y0 : rows_of(y0);
   if (!out.defined()) out = at::empty({z.M, z.N}, x.options().requires_grad(false));
-  const int64_t parts = parts_bytes(z, z.K), at = laid_out ? 0 : up(2 * z.slots * z.P * z.K), bt = laid_out ? 0 : up(2 * z.slots * z.P * z.N);
-  if (keep) kept = bytes(parts, x);
-  const Tensor scratch = keep && laid_out ? Tensor() : bytes((keep ? 0 : parts) + at + bt, x);
+  const int64_t parts = parts_bytes(z, z.K), at = laid_out ? 0 : factor_bytes(z, z.K), bt = laid_out ? 0 : factor_bytes(z, z.N);
+  if (keep) kept = at::empty({z.M, z.P}, x.options().dtype(at::kFloat).requires_grad(false));
+  const Tensor scratch = bytes(parts + at + bt, x);
   uint8_t* const s = data<uint8_t>(scratch);
   Factors f{A.const_data_ptr(), B.const_data_ptr()};
   if (!laid_out) {
     const Tensor a = dense(A), b = dense(B);
     f = {s, s + at};
-    check(pq_adapter_factors(a.const_data_ptr(), b.const_data_ptr(), z.slots, z.K, z.N, z.R, z.P, s, nullptr, s + at, nullptr, stream), "adapters");
+    check(pq_adapter_factors(a.const_data_ptr(), PQ_ADAPTER_BY_COLUMN, b.const_data_ptr(), PQ_ADAPTER_BY_RANK, z.slots, z.K, z.N, z.R, z.P, s, nullptr,
+                             nullptr, s + at, stream),
+          "adapters");
   }
-  forward(x, y, ids, scale, f, z, out, reinterpret_cast<float*>(keep ? data<uint8_t>(kept) : s + at + bt), stream);
+  forward(x, y, ids, scale, f, z, out, reinterpret_cast<float*>(s + at + bt), data<float>(kept), stream);
   return out;
 }
 
@@ -129,35 +132,31 @@ struct Adapt : torch::autograd::Function<Adapt> {
       if (want_x) out[0] = at::empty({z.M, z.K}, opt);
       if (want_A) out[3] = at::empty({z.slots, z.K, z.R}, opt);
       if (want_B) out[4] = at::empty({z.slots, z.R, z.N}, opt);
-      // the factors by the backward pass's orders: as they are where no rank is padded
-      const bool need_dt = want_x || want_A, turn = need_dt && (laid_out || z.R != z.P);
-      const int64_t parts = need_dt ? parts_bytes(z, z.N) : 0, ap = turn ? up(2 * z.slots * z.P * z.K) : 0, bp = turn ? up(2 * z.slots * z.P * z.N) : 0;
+      const bool need_dt = want_x || want_A;
+      const int64_t joined = want_A ? up(4 * z.M * z.P) : 0, parts = joined + (need_dt ? parts_bytes(z, z.N) : 0);
+      const int64_t ap = need_dt ? factor_bytes(z, z.K) : 0, bp = need_dt ? factor_bytes(z, z.N) : 0;
       const int64_t ws = want_A || want_B ? pq_adapter_grads_workspace_size(z.M, z.K, z.N, z.slots, z.P) : 0;
       const Tensor scratch = bytes(parts + ap + bp + ws, dy);
       uint8_t* const s = data<uint8_t>(scratch);
-      float* const dt = reinterpret_cast<float*>(s);
+      float* const dt = want_A ? reinterpret_cast<float*>(s) : nullptr;   // with its scale
+      float* const dt_parts = reinterpret_cast<float*>(s + joined);
       if (need_dt) {
         const Tensor a = dense(A), b = dense(B);
-        const void *f = b.const_data_ptr(), *g = a.const_data_ptr();
-        if (turn) {
-          f = s + parts + ap, g = s + parts;
-          if (laid_out)   // lr_B by column and lr_A by rank, turned: as if they were each other's
-            check(pq_adapter_factors(b.const_data_ptr(), a.const_data_ptr(), z.slots, z.N, z.K, z.P, z.P, s + parts + ap, nullptr, s + parts, nullptr, stream), "adapters");
-          else
-            check(pq_adapter_factors(a.const_data_ptr(), b.const_data_ptr(), z.slots, z.K, z.N, z.R, z.P, nullptr, s + parts, nullptr, s + parts + ap, stream), "adapters");
-        }
-        check(pq_adapter_down(dy.const_data_ptr(), code, z.M, z.N, stride_of(dy), f, z.slots, z.P, ids.const_data_ptr(), z.id_bits, z.each, dt, stream),
+        uint8_t *const g = s + parts, *const f = s + parts + ap;
+        check(pq_adapter_factors(a.const_data_ptr(), laid_out ? PQ_ADAPTER_DOWN : PQ_ADAPTER_BY_COLUMN, b.const_data_ptr(),
+                                 laid_out ? PQ_ADAPTER_UP : PQ_ADAPTER_BY_RANK, z.slots, z.K, z.N, laid_out ? z.P : z.R, z.P, nullptr,
+                                 want_x ? g : nullptr, f, nullptr, stream),
+              "adapters");
+        check(pq_adapter_down(dy.const_data_ptr(), code, z.M, z.N, stride_of(dy), f, z.slots, z.P, ids.const_data_ptr(), z.id_bits, z.each, dt_parts, stream),
               "adapters' dt");
-        if (want_x)
-          check(pq_adapter_up(dt, pq_adapter_slices(z.M, z.N), data<float>(scale), g, z.slots, z.K, z.R, z.P, ids.const_data_ptr(), z.id_bits, z.each,
-                              nullptr, 0, out[0].data_ptr(), z.K, code, z.M, stream),
-                "adapters' input gradient");
+        check(pq_adapter_up(dt_parts, pq_adapter_slices(z.M, z.N), data<float>(scale), g, z.slots, z.K, z.R, z.P, ids.const_data_ptr(), z.id_bits,
+                            z.each, nullptr, 0, data<void>(out[0]), z.K, dt, code, z.M, stream),
+              "adapters' input gradient");
       }
       if (want_A || want_B)
         check(pq_adapter_grads(x.defined() ? x.const_data_ptr() : nullptr, x.defined() ? stride_of(x) : z.K, dy.const_data_ptr(), stride_of(dy), code,
-                               data<float>(kept), pq_adapter_slices(z.M, z.K), dt, pq_adapter_slices(z.M, z.N), data<float>(scale),
-                               ids.const_data_ptr(), z.id_bits, z.each, z.M, z.K, z.N, z.slots, z.R, z.P, data<void>(out[3]), data<void>(out[4]),
-                               s + parts + ap + bp, ws, stream),
+                               data<float>(kept), dt, ids.const_data_ptr(), z.id_bits, z.each, z.M, z.K, z.N, z.slots, z.R, z.P,
+                               data<void>(out[3]), data<void>(out[4]), s + parts + ap + bp, ws, stream),
               "adapters' factor gradients");
     } catch (const Refused& r) {
       throw std::runtime_error(r.text);
@@ -217,7 +216,7 @@ const char* wrong(const Tensor& x, const Tensor& y, const Tensor& ids, const Ten
   if (R < 1 || R > 64) return "adapters have ranks of 1 to 64";
   if (slots < 1 || slots > 65535 || B.size(0) != slots) return "lr_A and lr_B hold the same adapters, 1 to 65535";
   const int64_t P = padded(R);
-  if (laid_out ? A.size(1) != P || A.size(2) != K || B.size(1) != N || B.size(2) != P || !A.is_contiguous() || !B.is_contiguous() ||
+  if (laid_out ? A.size(1) != (K + 127) / 128 * 128 || A.size(2) != P || B.size(1) != (N + 127) / 128 * 128 || B.size(2) != P || !A.is_contiguous() || !B.is_contiguous() ||
                      (uintptr_t)A.const_data_ptr() % 16 || (uintptr_t)B.const_data_ptr() % 16
                : A.size(1) != K || A.size(2) != R || B.size(1) != R || B.size(2) != N)
     return "lr_A and lr_B do not fit x and y";

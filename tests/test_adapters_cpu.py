@@ -29,12 +29,14 @@ def test_down_and_up_refusals():
     assert down(ids=ctypes.c_void_p(260), bits=64) == L.PQ_EALIGN
     assert down(M=0, x=None, f=None, ids=None, part=None) == L.PQ_OK
 
-    def up(part=P, slices=1, scale=P, g=P, slots=2, C=64, R=8, PP=16, ids=P, bits=32, each=1, base=P, ldb=64, out=P, ldo=64, ty=0, M=4):
-        return lib.pq_adapter_up(part, slices, scale, g, slots, C, R, PP, ids, bits, each, base, ldb, out, ldo, ty, M, None)
+    def up(part=P, slices=1, scale=P, g=P, slots=2, C=64, R=8, PP=16, ids=P, bits=32, each=1, base=P, ldb=64, out=P, ldo=64, joined=None, ty=0, M=4):
+        return lib.pq_adapter_up(part, slices, scale, g, slots, C, R, PP, ids, bits, each, base, ldb, out, ldo, joined, ty, M, None)
 
     assert up(C=60) == L.PQ_ESHAPE and up(ldo=56) == L.PQ_ESHAPE and up(ldb=56) == L.PQ_ESHAPE and up(R=17) == L.PQ_ESHAPE and up(R=0) == L.PQ_ESHAPE
     assert up(slices=0) == L.PQ_ESHAPE and up(slices=17) == L.PQ_ESHAPE and up(ty=3) == L.PQ_EDTYPE and up(ldb=72) == L.PQ_ESHAPE
+    assert up(ldo=(1 << 30) + 8) == L.PQ_ESHAPE and up(base=ctypes.c_void_p(512), ldb=(1 << 30) + 8) == L.PQ_ESHAPE
     assert up(part=None) == L.PQ_EINVAL and up(scale=None) == L.PQ_EINVAL and up(g=None) == L.PQ_EINVAL and up(out=None) == L.PQ_EINVAL
+    assert up(out=None, joined=P) == L.PQ_EINVAL and up(joined=ODD) == L.PQ_EALIGN       # (a base without a result)
     assert up(out=ODD) == L.PQ_EALIGN and up(base=ODD) == L.PQ_EALIGN and up(ldo=68) == L.PQ_EALIGN and up(base=ctypes.c_void_p(512), ldb=68) == L.PQ_EALIGN
     assert up(M=0, part=None, out=None) == L.PQ_OK
 
@@ -42,23 +44,26 @@ def test_down_and_up_refusals():
 def test_gradient_and_order_refusals():
     L, lib = _lib()
 
-    def grads(x=P, ldx=64, dy=P, lddy=64, ty=0, t=P, ts=1, dt=P, dts=1, scale=P, ids=P, bits=32, each=1, M=4, K=64, N=64, slots=2, R=8, PP=16,
+    def grads(x=P, ldx=64, dy=P, lddy=64, ty=0, t=P, dt=P, ids=P, bits=32, each=1, M=4, K=64, N=64, slots=2, R=8, PP=16,
               dA=P, dB=P, ws=P, size=1 << 40):
-        return lib.pq_adapter_grads(x, ldx, dy, lddy, ty, t, ts, dt, dts, scale, ids, bits, each, M, K, N, slots, R, PP, dA, dB, ws, size, None)
+        return lib.pq_adapter_grads(x, ldx, dy, lddy, ty, t, dt, ids, bits, each, M, K, N, slots, R, PP, dA, dB, ws, size, None)
 
     assert grads(K=60) == L.PQ_ESHAPE and grads(N=4) == L.PQ_ESHAPE and grads(ldx=56) == L.PQ_ESHAPE and grads(lddy=56) == L.PQ_ESHAPE
-    assert grads(R=17) == L.PQ_ESHAPE and grads(ts=0) == L.PQ_ESHAPE and grads(dts=17) == L.PQ_ESHAPE and grads(size=64) == L.PQ_ESHAPE
+    assert grads(R=17) == L.PQ_ESHAPE and grads(size=64) == L.PQ_ESHAPE
     assert grads(ty=2) == L.PQ_EDTYPE and grads(bits=8) == L.PQ_EDTYPE and grads(each=3) == L.PQ_ESHAPE
     assert grads(x=None) == L.PQ_EINVAL and grads(t=None) == L.PQ_EINVAL and grads(dt=None) == L.PQ_EINVAL and grads(dy=None) == L.PQ_EINVAL
-    assert grads(ws=None) == L.PQ_EINVAL and grads(scale=None) == L.PQ_EINVAL
+    assert grads(ws=None) == L.PQ_EINVAL
     assert grads(x=ODD) == L.PQ_EALIGN and grads(lddy=68) == L.PQ_EALIGN and grads(ws=ODD) == L.PQ_EALIGN
     assert grads(dA=None, dB=None) == L.PQ_OK
     size = lib.pq_adapter_grads_workspace_size
     assert size(4, 60, 64, 2, 16) == 0 and size(4, 64, 64, 0, 16) == 0 and 0 < size(4, 64, 64, 2, 16) < size(100000, 64, 64, 2, 16)
     assert 1 <= lib.pq_adapter_slices(1, 65536) <= 16 and lib.pq_adapter_slices(1 << 20, 64) == 1 and lib.pq_adapter_slices(0, 64) == 1
-    lay = lambda A=P, B=P, slots=2, K=64, N=64, R=8, PP=16, at=P, bt=P: lib.pq_adapter_factors(A, B, slots, K, N, R, PP, at, None, bt, None, None)   # noqa: E731
+    lay = lambda A=P, B=P, slots=2, K=64, N=64, R=8, PP=16, at=P, bt=P, oa=0, ob=1: lib.pq_adapter_factors(   # noqa: E731
+        A, oa, B, ob, slots, K, N, R, PP, at, None, None, bt, None)
+    assert lay(oa=4) == L.PQ_EINVAL and lay(ob=-1) == L.PQ_EINVAL and lay(A=ODD, oa=2) == L.PQ_EALIGN
+    assert lib.pq_adapter_factor_size(136, 32) == 256 * 32 and lib.pq_adapter_factor_size(60, 32) == 0 and lib.pq_adapter_factor_size(64, 8) == 0
     assert lay(K=4) == L.PQ_ESHAPE and lay(R=17) == L.PQ_ESHAPE and lay(slots=0) == L.PQ_ESHAPE
-    assert lay(A=None) == L.PQ_EINVAL and lay(B=None) == L.PQ_EINVAL and lay(A=None, B=None, at=None, bt=None) == L.PQ_OK
+    assert lay(A=None) == L.PQ_EINVAL and lay(B=None) == L.PQ_EINVAL and lay(A=None, B=None, at=None, bt=None) == L.PQ_OK and lay(at=ODD) == L.PQ_EALIGN
 
 
 def test_module_refusals():

@@ -286,7 +286,7 @@ def test_factors_of_another_type(cuda):
     exact = _bank(A, B, scale, trainable=True)
     assert torch.equal(exact(x, y, i), out)
     with torch.no_grad():
-        assert torch.equal(bank.freeze()(x, y, i), out) and bank.lr_At.dtype == torch.float32
+        assert torch.equal(bank.freeze()(x, y, i), out) and bank.lr_Af.dtype == torch.float32
         assert torch.equal(exact.freeze()(x, y, i), out) and torch.equal(bank.freeze(torch.bfloat16)(x, y, i), out)
 
 
@@ -314,7 +314,7 @@ def test_refusals(cuda):
     with pytest.raises(AssertionError, match="no gradients"):
         from pyraquant_amd.adapters import _load_adapt
 
-        _load_adapt()(x, y, i, bank.lr_At.requires_grad_(), bank.lr_Bt, bank.scale, 8, True, None)
+        _load_adapt()(x, y, i, bank.lr_Af.requires_grad_(), bank.lr_Bf, bank.scale, 8, True, None)
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             tuned(torch.autograd.forward_ad.make_dual(x, x), y, i)
@@ -407,6 +407,7 @@ def test_places_past_32_bits(cuda):
 def test_kernels_write_what_they_say(cuda):
     """Through the C ABI, with guards around every output: parts only in rows with an adapter, gradients and orders whole."""
     from pyraquant_amd import _lib
+    from pyraquant_amd.adapters import _down_axes, _up_axes
 
     L = _lib.load()
     for (M, K, N, slots, R), ids in itertools.product(((70, 264, 136, 3, 20), (1, 8, 8, 1, 1), (333, 72, 1032, 2, 64)), ("rows", "runs")):
@@ -423,29 +424,44 @@ def test_kernels_write_what_they_say(cuda):
             for t, _ in pairs:
                 assert bool((t[:128] == 7).all()) and bool((t[-128:] == 7).all())
 
-        at, bt, ap, bp = (guarded(slots * P * c, torch.bfloat16) for c in (K, N, K, N))
-        _lib.check(L.pq_adapter_factors(p(A), p(B), slots, K, N, R, P, p(at[1]), p(ap[1]), p(bt[1]), p(bp[1]), stream), "factors")
-        whole(at, bt, ap, bp)
-        Ap, Bp = torch.zeros(slots, K, P, device=cuda).bfloat16(), torch.zeros(slots, P, N, device=cuda).bfloat16()
-        Ap[:, :, :R], Bp[:, :R] = A, B
-        assert torch.equal(ap[1].view(slots, K, P), Ap) and torch.equal(at[1].view(slots, P, K), Ap.transpose(1, 2))
-        assert torch.equal(bp[1].view(slots, P, N), Bp) and torch.equal(bt[1].view(slots, N, P), Bp.transpose(1, 2))
+        size = L.pq_adapter_factor_size
+        ad, au, bd, bu = (guarded(slots * size(c, P), torch.bfloat16) for c in (K, K, N, N))
+        _lib.check(L.pq_adapter_factors(p(A), 0, p(B), 1, slots, K, N, R, P, p(ad[1]), p(au[1]), p(bd[1]), p(bu[1]), stream), "factors")
+        whole(ad, au, bd, bu)
+        for f, axes, m in ((ad, _down_axes, A), (au, _up_axes, A), (bd, _down_axes, B.transpose(1, 2)), (bu, _up_axes, B.transpose(1, 2))):
+            v = f[1].view(slots, -1, P)
+            v = axes(v).reshape(v.shape)
+            assert torch.equal(v[:, : m.shape[1], :R], m) and not v[:, m.shape[1]:].any() and not v[:, :, R:].any()
+        again = [guarded(slots * size(c, P), torch.bfloat16) for c in (K, K, N, N)]      # from these orders, and by the other natural one
+        _lib.check(L.pq_adapter_factors(p(ad[1]), 2, p(bu[1]), 3, slots, K, N, P, P, *(p(t[1]) for t in again), stream), "factors")
+        whole(*again)
+        assert all(torch.equal(x[1], y[1]) for x, y in zip(again, (ad, au, bd, bu)))
+        At, Bt = A.transpose(1, 2).contiguous(), B.transpose(1, 2).contiguous()
+        _lib.check(L.pq_adapter_factors(p(At), 1, p(Bt), 0, slots, K, N, R, P, *(p(t[1]) for t in again), stream), "factors")
+        assert all(torch.equal(x[1], y[1]) for x, y in zip(again, (ad, au, bd, bu)))
         S, Sd = L.pq_adapter_slices(M, K), L.pq_adapter_slices(M, N)
         t, dt = guarded(S * M * P, torch.float32), guarded(Sd * M * P, torch.float32)
         dy = torch.randn(M, N, device=cuda).bfloat16()
-        _lib.check(L.pq_adapter_down(p(x), 0, M, K, K, p(at[1]), slots, P, p(i), 32, 1, p(t[1]), stream), "down")
-        _lib.check(L.pq_adapter_down(p(dy), 0, M, N, N, p(bp[1]), slots, P, p(i), 32, 1, p(dt[1]), stream), "down")
+        _lib.check(L.pq_adapter_down(p(x), 0, M, K, K, p(ad[1]), slots, P, p(i), 32, 1, p(t[1]), stream), "down")
+        _lib.check(L.pq_adapter_down(p(dy), 0, M, N, N, p(bd[1]), slots, P, p(i), 32, 1, p(dt[1]), stream), "down")
         whole(t, dt)
         none = (i < 0) | (i >= slots)
         assert bool((t[1].view(S, M, P)[:, none] == 7).all())
         dx, dA, dB = guarded(M * K, torch.bfloat16), guarded(slots * K * R, torch.bfloat16), guarded(slots * R * N, torch.bfloat16)
-        _lib.check(L.pq_adapter_up(p(dt[1]), Sd, p(scale), p(ap[1]), slots, K, R, P, p(i), 32, 1, None, 0, p(dx[1]), K, 0, M, stream), "up")
-        size = L.pq_adapter_grads_workspace_size(M, K, N, slots, P)
-        ws = torch.full((size + 256,), 255, dtype=torch.uint8, device=cuda)
-        _lib.check(L.pq_adapter_grads(p(x), K, p(dy), N, 0, p(t[1]), S, p(dt[1]), Sd, p(scale), p(i), 32, 1, M, K, N, slots, R, P, p(dA[1]),
-                                      p(dB[1]), p(ws), size, stream), "grads")
+        tj, dtj, alone = (guarded(M * P, torch.float32) for _ in range(3))
+        up = lambda parts, n, g, C, out, joined: _lib.check(L.pq_adapter_up(   # noqa: E731
+            p(parts[1]), n, p(scale), g, slots, C, R, P, p(i), 32, 1, None, 0, out, C, p(joined[1]), 0, M, stream), "up")
+        up(t, S, None, N, None, tj)
+        up(dt, Sd, p(au[1]), K, p(dx[1]), dtj)
+        up(dt, Sd, None, K, None, alone)
+        whole(tj, dtj, alone)
+        assert torch.equal(alone[1], dtj[1]) and bool((tj[1].view(M, P)[none] == 7).all()) and not tj[1].view(M, P)[~none][:, R:].any()
+        room = L.pq_adapter_grads_workspace_size(M, K, N, slots, P)
+        ws = torch.full((room + 256,), 255, dtype=torch.uint8, device=cuda)
+        _lib.check(L.pq_adapter_grads(p(x), K, p(dy), N, 0, p(tj[1]), p(dtj[1]), p(i), 32, 1, M, K, N, slots, R, P, p(dA[1]), p(dB[1]), p(ws), room,
+                                      stream), "grads")
         whole(dx, dA, dB)
-        assert bool((ws[size:] == 255).all())
+        assert bool((ws[room:] == 255).all())
         want, off = _want(x, y, i, A, B, scale, dy)
         for got, k in ((dx, "dx"), (dA, "dA"), (dB, "dB")):
             _near(got[1].view(want[k].shape), want[k], off[k], k)
