@@ -562,6 +562,8 @@ typedef struct {
 /* The sums of the squares of a list's gradients, in 64 bits, as pq_grad_squares_partials(list) partial sums in device memory, their order fixed by the sizes. */
 int64_t pq_grad_squares_partials(const pq_adamw_list* list);
 int pq_grad_squares(const pq_adamw_list* list, double* partials, int64_t n_partials, hipStream_t stream);
+/* Their sum as one (each wave of a step adds all that it is given: worth a launch from some 512 on). */
+int pq_grad_squares_join(const double* partials, int64_t n_partials, double* sum, hipStream_t stream);
 
 /* One step. n_partials > 0: the gradients (of all lists that share a limit) are held to rates->max_norm by pq_grad_squares' sums, and their
  * norm is written to `norm` (device memory); else both may be NULL. */

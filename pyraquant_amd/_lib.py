@@ -66,6 +66,7 @@ EXPORTS = (
     "pq_adapter_grads",
     "pq_grad_squares_partials",
     "pq_grad_squares",
+    "pq_grad_squares_join",
     "pq_adamw_step",
     "pq_adamw_moments",
     "pq_adamw_load",
@@ -151,6 +152,7 @@ _SIGNATURES = {
                          ctypes.c_int),
     "pq_grad_squares_partials": ([_list], _i64),
     "pq_grad_squares": ([_list, _p, _i64, _p], ctypes.c_int),
+    "pq_grad_squares_join": ([_p, _i64, _p, _p], ctypes.c_int),
     "pq_adamw_step": ([_list, _states, _rates, _p, _i64, _p, _p], ctypes.c_int),
     "pq_adamw_moments": ([_states, _p, _p, _i32, _p], ctypes.c_int),
     "pq_adamw_load": ([_states, _p, _p, _p], ctypes.c_int),

@@ -18,7 +18,8 @@
 // and 0 stands for zero: what lies below the grid is zero, but a root that is no zero is at least the grid's first value, so
 // that no mean is divided by a root that went to zero before it. A block with an infinity or a NaN is NaN (E 255).
 //
-// Bound by memory: a bf16 value with 8-bit states moves 10 bytes, with 32-bit ones 22.
+// A bf16 value with 8-bit states moves 10 bytes, with 32-bit ones 22, an fp32 value with 8-bit states 16: these are bound by memory (12.7 M fp32 values
+// 43 us, 4.8 TB/s), the first by its arithmetic, 64 instructions a value (88.6 M bf16 values in three launches 258 us, without arithmetic 169).
 #include "pq_common.h"
 
 #include <math.h>
@@ -29,7 +30,7 @@ namespace {
 
 constexpr int kChunk = PQ_ADAMW_CHUNK, kBlock = PQ_ADAMW_BLOCK;
 constexpr int kGrads = 448;            // gradients to a launch: 3584 bytes of arguments
-constexpr int kGroups = 2048;          // workgroups at most: 8 to a compute unit, 4 chunks (waves) each
+constexpr int kGroups = 1024;          // workgroups at most: 4 to a compute unit, which its registers hold, a chunk to a wave
 static_assert(kChunk == 1024 && kBlock == 128, "a lane holds two times eight values, 16 lanes a block");
 
 struct Grads {
@@ -76,13 +77,14 @@ __device__ __forceinline__ void load8(const void* base, int64_t at, int left, bo
     }
   }
 }
-template <int DT>
+template <int DT, bool NT = false>
 __device__ __forceinline__ void store8(void* base, int64_t at, int left, bool wide, const float (&x)[8]) {
   if constexpr (DT == PQ_F32) {
     float* const p = static_cast<float*>(base) + at;
     if (wide && left >= 8) {
-      reinterpret_cast<v4f*>(p)[0] = v4f{x[0], x[1], x[2], x[3]};
-      reinterpret_cast<v4f*>(p)[1] = v4f{x[4], x[5], x[6], x[7]};
+      const v4f a = {x[0], x[1], x[2], x[3]}, b = {x[4], x[5], x[6], x[7]};
+      if (NT) __builtin_nontemporal_store(a, reinterpret_cast<v4f*>(p)), __builtin_nontemporal_store(b, reinterpret_cast<v4f*>(p) + 1);
+      else reinterpret_cast<v4f*>(p)[0] = a, reinterpret_cast<v4f*>(p)[1] = b;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -94,7 +96,8 @@ __device__ __forceinline__ void store8(void* base, int64_t at, int left, bool wi
       v4u a;
 #pragma unroll
       for (int e = 0; e < 4; ++e) a[e] = pack2<DT>(x[2 * e], x[2 * e + 1]);
-      *reinterpret_cast<v4u*>(p) = a;
+      if (NT) __builtin_nontemporal_store(a, reinterpret_cast<v4u*>(p));
+      else *reinterpret_cast<v4u*>(p) = a;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -104,8 +107,8 @@ __device__ __forceinline__ void store8(void* base, int64_t at, int left, bool wi
 }
 
 // ---- the 8-bit states ----------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t mixed(uint32_t place, uint32_t key) {
-  uint32_t z = place * 0x9E3779B1u + key;
+constexpr uint32_t kPlace = 0x9E3779B1u;
+__device__ __forceinline__ uint32_t mixed(uint32_t z) {   // z: the place times kPlace, and the step's key
   z = (z ^ (z >> 15)) * 0x7FB5D329u;
   z = (z ^ (z >> 13)) * 0x4C957F2Bu;
   return z ^ (z >> 16);
@@ -117,21 +120,20 @@ __device__ __forceinline__ int block_max(int x) {
   x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false));
   return max(x, __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false));
 }
+// Two values' R, bytes and the like as two 16-bit numbers of a word. R is kept 15 exponents up (R + 15 2^bits): no number falls below zero,
+// and a difference that would is 0.
+__device__ __forceinline__ us2 two(uint32_t w) { return __builtin_bit_cast(us2, w); }
+__device__ __forceinline__ us2 both(uint32_t v) { return two(v | v << 16); }
 template <int BITS>
-__device__ __forceinline__ int rounded(float a, uint32_t u) {   // R; at most an infinity's
-  return (int)min(((__float_as_uint(a) & 0x7fffffffu) + u) >> (23 - BITS), 255u << BITS);
+__device__ __forceinline__ us2 rounded2(uint32_t a, uint32_t ua, uint32_t b, uint32_t ub) {   // of magnitudes' bits; at most an infinity's
+  constexpr uint32_t up = 15u << 23;
+  const uint32_t ra = (a + ua + up) >> (23 - BITS), rb = (b + ub + up) >> (23 - BITS);
+  return __builtin_elementwise_min(two(ra | rb << 16), both((255u + 15u) << BITS));
 }
-// The byte of R in a block of exponent E, without a sign.
-template <int BITS, bool ROOT>
-__device__ __forceinline__ uint32_t byte_of(int r, int E) {
-  const int zero = (E - 15) << BITS;
-  if (r > zero) return (uint32_t)(r - zero);
-  return ROOT && r > 0 ? 1u : 0u;
-}
+// fp32 bits of two bytes (without signs) of a block of exponent E
 template <int BITS>
-__device__ __forceinline__ float value_of(uint32_t byte, int E) {   // byte: without a sign
-  const float a = __uint_as_float(byte == 0 ? 0u : (byte + (uint32_t)((E - 15) << BITS)) << (23 - BITS));
-  return E == 255 ? __uint_as_float(0x7fc00000u) : a;
+__device__ __forceinline__ us2 widened2(us2 bytes, int E) {
+  return (bytes + both((uint32_t)((E - 15) << BITS) & 0xffffu)) * __builtin_elementwise_min(bytes, both(1));   // (0 is zero)
 }
 struct Moments8 {
   v2u m, root;
@@ -142,29 +144,46 @@ struct Moments8 {
     root = *reinterpret_cast<const v2u*>(static_cast<const uint8_t*>(p.v) + at);
     exps = *reinterpret_cast<const uint16_t*>(p.exps + at / kBlock * 2);
   }
-  __device__ __forceinline__ float mean(int e) const {
-    const uint32_t b = m[e >> 2] >> (8 * (e & 3)) & 0xffu;
-    return __uint_as_float(__float_as_uint(value_of<3>(b & 0x7fu, exps & 0xff)) | (b & 0x80u) << 24);
+  __device__ __forceinline__ void values(float (&mean)[8], float (&roots)[8]) const {
+    const int em = exps & 0xff, er = exps >> 8;
+    const uint32_t nan_m = em == 255 ? 0x7fc00000u : 0u, nan_r = er == 255 ? 0x7fc00000u : 0u;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const uint32_t wm = m[e >> 2] >> (e & 2 ? 16 : 0), wr = root[e >> 2];
+      const uint32_t am = __builtin_bit_cast(uint32_t, widened2<3>(two(__builtin_amdgcn_perm(0, wm, 0x0c010c00) & 0x007f007fu), em));
+      const uint32_t ar = __builtin_bit_cast(uint32_t, widened2<4>(two(__builtin_amdgcn_perm(0, wr, e & 2 ? 0x0c030c02 : 0x0c010c00)), er));
+      mean[e] = __uint_as_float(am << 20 | (wm << 24 & 0x80000000u) | nan_m);
+      mean[e + 1] = __uint_as_float((am << 4 & 0xfff00000u) | (wm << 16 & 0x80000000u) | nan_m);
+      roots[e] = __uint_as_float(ar << 19 | nan_r);
+      roots[e + 1] = __uint_as_float((ar << 3 & 0x7ff80000u) | nan_r);
+    }
   }
-  __device__ __forceinline__ float root_of(int e) const { return value_of<4>(root[e >> 2] >> (8 * (e & 3)) & 0xffu, exps >> 8); }
-  // the values as they are kept; um and ur: what the rounding adds
+  // the values as they are kept; add(e, um, ur): what the rounding adds
   template <typename U>
   __device__ __forceinline__ void keep(const float (&mean)[8], const float (&roots)[8], U add) {
-    int rm[8], rr[8], tm = 0, tr = 0;
+    us2 rm[4], rr[4], tm = both(0), tr = both(0);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      uint32_t um, ur;
-      add(e, um, ur);
-      tm = max(tm, rm[e] = rounded<3>(mean[e], um));
-      tr = max(tr, rr[e] = rounded<4>(roots[e], ur));
+    for (int i = 0; i < 4; ++i) {
+      uint32_t um[2], ur[2];
+      add(2 * i, um[0], ur[0]);
+      add(2 * i + 1, um[1], ur[1]);
+      rm[i] = rounded2<3>(__float_as_uint(mean[2 * i]) & 0x7fffffffu, um[0], __float_as_uint(mean[2 * i + 1]) & 0x7fffffffu, um[1]);
+      rr[i] = rounded2<4>(__float_as_uint(roots[2 * i]), ur[0], __float_as_uint(roots[2 * i + 1]), ur[1]);
+      tm = __builtin_elementwise_max(tm, rm[i]);
+      tr = __builtin_elementwise_max(tr, rr[i]);
     }
-    const int em = block_max(tm) >> 3, er = block_max(tr) >> 4;
-    m = root = v2u{0, 0};
+    const int em = (block_max(max((int)tm[0], (int)tm[1])) >> 3) - 15, er = (block_max(max((int)tr[0], (int)tr[1])) >> 4) - 15;
+    const us2 zero_m = both((uint32_t)em << 3), zero_r = both((uint32_t)er << 4), none = both(15 << 4);
+    uint32_t bm[4], br[4];   // two bytes each, in 16 bits
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      m[e >> 2] |= (byte_of<3, false>(rm[e], em) | (__float_as_uint(mean[e]) >> 24 & 0x80u)) << (8 * (e & 3));
-      root[e >> 2] |= byte_of<4, true>(rr[e], er) << (8 * (e & 3));
+    for (int i = 0; i < 4; ++i) {
+      bm[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(rm[i], zero_m)) | (__float_as_uint(mean[2 * i]) >> 24 & 0x80u) |
+              (__float_as_uint(mean[2 * i + 1]) >> 8 & 0x800000u);
+      const us2 some = __builtin_elementwise_min(__builtin_elementwise_sub_sat(rr[i], none), both(1));   // (a root that is no zero: at least 1)
+      br[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_elementwise_sub_sat(rr[i], zero_r), some));
     }
+    m = v2u{__builtin_amdgcn_perm(bm[1], bm[0], 0x06040200), __builtin_amdgcn_perm(bm[3], bm[2], 0x06040200)};
+    root = v2u{__builtin_amdgcn_perm(br[1], br[0], 0x06040200), __builtin_amdgcn_perm(br[3], br[2], 0x06040200)};
     exps = em | er << 8;
   }
   __device__ __forceinline__ void store(void* ms, void* roots, uint8_t* ex, int64_t at) const {
@@ -182,7 +201,7 @@ __device__ __forceinline__ double wave_sum(double s) {
 
 // ---- the step ------------------------------------------------------------------------------------------------------------
 struct Rates {   // of one step count
-  float size, unbias, keep;   // lr / (1 - b1^t), sqrt(1 - b2^t), 1 - lr wd
+  float size, unbias, keep;   // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
 };
 
 template <int DT, bool EIGHT>
@@ -211,24 +230,39 @@ __device__ __forceinline__ void step_chunk(const StepArgs& p, void* param, const
     const int64_t at = c0 + i * 512 + lane * 8;
     if (at - at % kBlock >= n) continue;
     float root[8];
+    if constexpr (EIGHT) {
+      s[i].values(m[i], v[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] *= v[i][e];
+    }
+    uint32_t least = ~0u;   // of the squares that are no zeros (bits - 1)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if constexpr (EIGHT) {
-        m[i][e] = s[i].mean(e);
-        const float w = s[i].root_of(e);
-        v[i][e] = w * w;
-      }
       const float d = g[i][e] * clip;
-      m[i][e] = m[i][e] * p.b1 + d * p.b1c;
-      v[i][e] = v[i][e] * p.b2 + (d * d) * p.b2c;
-      root[e] = sqrtf(v[i][e]);
-      x[i][e] = x[i][e] * r.keep - r.size * m[i][e] / (root[e] / r.unbias + p.eps);
+      m[i][e] = fmaf(d, p.b1c, m[i][e] * p.b1);
+      v[i][e] = fmaf(d * d, p.b2c, v[i][e] * p.b2);
+      least = min(least, __float_as_uint(v[i][e]) - 1);
+    }
+    // The instructions for roots and reciprocals are within 1 of the last place, but take subnormal numbers for zeros: where a square is
+    // below 2^-96, or eps is, the exact ones are taken (12 and 10 instructions; a step of 88 M bf16 values was bound by them).
+    if (__ballot(least < 0x0f7fffffu) || p.eps < 0x1p-96f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        root[e] = sqrtf(v[i][e]);
+        x[i][e] = x[i][e] * r.keep - r.size * m[i][e] / fmaf(root[e], r.unbias, p.eps);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        root[e] = __builtin_amdgcn_sqrtf(v[i][e]);
+        x[i][e] = fmaf(-r.size * m[i][e], __builtin_amdgcn_rcpf(fmaf(root[e], r.unbias, p.eps)), x[i][e] * r.keep);
+      }
     }
     store8<DT>(param, at, left[i], wide_p, x[i]);
     if constexpr (EIGHT) {
-      const uint32_t place = (uint32_t)(base + at);
+      const uint32_t place = (uint32_t)(base + at) * kPlace + key;
       s[i].keep(m[i], root, [&](int e, uint32_t& um, uint32_t& ur) {
-        const uint32_t h = mixed(place + e, key);
+        const uint32_t h = mixed(place + e * kPlace);
         um = (h & 0xffffu) << 4;
         ur = (h >> 16) << 3;
       });
@@ -265,7 +299,7 @@ __global__ __launch_bounds__(256) void adamw_step_kernel(const StepArgs p, const
     if (step != last) {
       last = step;
       r.size = (float)(lr / (1.0 - exp(step * p.log_b1)));
-      r.unbias = (float)sqrt(1.0 - exp(step * p.log_b2));
+      r.unbias = (float)(1.0 / sqrt(1.0 - exp(step * p.log_b2)));
       r.keep = (float)(1.0 - lr * p.decay);
     }
     const int64_t c0 = (int64_t)(c - t.first_chunk) * kChunk;
@@ -313,6 +347,20 @@ __global__ __launch_bounds__(256) void grad_squares_kernel(const StepArgs p, con
   if (threadIdx.x == 0) out[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
+// Many partial sums in one, in a fixed order.
+__global__ __launch_bounds__(1024) void grad_join_kernel(const double* sums, int n, double* out) {
+  __shared__ double part[16];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) s += sums[i];
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) s += part[i];
+    *out = s;
+  }
+}
+
 // ---- states out and in -----------------------------------------------------------------------------------------------------
 template <int DT, bool EIGHT>
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const StepArgs p, int64_t n, void* mean, void* root) {
@@ -322,16 +370,15 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const StepArgs p, in
   if constexpr (EIGHT) {
     Moments8 s;
     s.load(p, at);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m[e] = s.mean(e), w[e] = s.root_of(e);
+    s.values(m, w);
   } else {
     load8<PQ_F32>(p.m, at, 8, true, m);
     load8<PQ_F32>(p.v, at, 8, true, w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = sqrtf(w[e]);
   }
-  store8<DT>(mean, at, 8, true, m);
-  store8<DT>(root, at, 8, true, w);
+  store8<DT, true>(mean, at, 8, true, m);   // (past the caches: what they hold is read again before this is. The next step's sums 21 -> 17 us a launch)
+  store8<DT, true>(root, at, 8, true, w);
 }
 template <bool EIGHT>
 __global__ __launch_bounds__(256) void adamw_load_kernel(const StepArgs p, int64_t n, const float* mean, const float* root) {
@@ -396,7 +443,7 @@ int batches(const pq_adamw_list* l, StepArgs p, int most, F f) {
   }
   return PQ_OK;
 }
-constexpr int kPartials = 512;   // workgroups of a launch that sums squares
+constexpr int kPartials = 2048;   // workgroups of a launch that sums squares
 }  // namespace
 }  // namespace optim
 }  // namespace pq
@@ -422,6 +469,13 @@ extern "C" int pq_grad_squares(const pq_adamw_list* list, double* partials, int6
     partials += groups;
     return check_launch("pq_grad_squares");
   });
+}
+
+extern "C" int pq_grad_squares_join(const double* partials, int64_t n_partials, double* sum, hipStream_t stream) {
+  if (n_partials < 1 || n_partials > (1 << 30)) return set_error(PQ_ESHAPE, "pq_grad_squares_join: %lld sums", (long long)n_partials);
+  if (!partials || !sum) return set_error(PQ_EINVAL, "pq_grad_squares_join: null pointer");
+  hipLaunchKernelGGL(grad_join_kernel, dim3(1), dim3(1024), 0, stream, partials, (int)n_partials, sum);
+  return check_launch("pq_grad_squares_join");
 }
 
 extern "C" int pq_adamw_step(const pq_adamw_list* list, const pq_adamw_states* states, const pq_adamw_rates* rates,

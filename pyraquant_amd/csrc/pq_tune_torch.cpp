@@ -223,6 +223,7 @@ py::object step(const py::list& groups, double max_norm) {
   }
   Tensor norm, partials;
   std::vector<int64_t> sums;
+  int64_t n_partials = 0;
   if (max_norm && !all.empty()) {
     const c10::DeviceGuard guard(all[0].plan->like().device());
     int64_t total = 0;
@@ -231,21 +232,28 @@ py::object step(const py::list& groups, double max_norm) {
       sums.push_back(pq_grad_squares_partials(&l));
       total += sums.back();
     }
-    norm = at::zeros({}, all[0].plan->like().options().dtype(at::kFloat));
+    norm = at::empty({}, all[0].plan->like().options().dtype(at::kFloat));
     if (total) {
-      partials = at::empty({total}, norm.options().dtype(at::kDouble));
-      double* to = data<double>(partials);
+      const bool join = total > 512;   // a place for their sum, in front
+      partials = at::empty({total + join}, norm.options().dtype(at::kDouble));
+      double* to = data<double>(partials) + join;
       for (size_t i = 0; i < all.size(); to += sums[i++]) {
         const pq_adamw_list l = all[i].plan->c_list();
         check(pq_grad_squares(&l, to, sums[i], stream_of(norm)), "AdamW");
       }
+      n_partials = total;
+      if (join) {
+        check(pq_grad_squares_join(data<double>(partials) + 1, total, data<double>(partials), stream_of(norm)), "AdamW");
+        n_partials = 1;
+      }
     }
   }
+  if (norm.defined() && !n_partials) norm.zero_();   // no gradient at all
   for (const Group& g : all) {
     const c10::DeviceGuard guard(g.plan->like().device());
     const pq_adamw_list l = g.plan->c_list();
     const pq_adamw_states s = g.plan->c_states();
-    check(pq_adamw_step(&l, &s, &g.rates, data<double>(partials), partials.defined() ? partials.numel() : 0, data<float>(norm),
+    check(pq_adamw_step(&l, &s, &g.rates, data<double>(partials), n_partials, data<float>(norm),
                         stream_of(g.plan->like())),
           "AdamW");
     g.plan->changed();

@@ -53,9 +53,11 @@ def test_norm_and_moments_refusals():
     assert lib.pq_grad_squares_partials(ctypes.byref(lst)) == 1     # four chunks: one workgroup
     assert lib.pq_grad_squares_partials(ctypes.byref(_list(L, grads=(None, None)))) == 0
     many = _list(L, [5000] * 1000, [256] * 1000)
-    assert 3 <= lib.pq_grad_squares_partials(ctypes.byref(many)) <= 3 * 512
+    assert 3 <= lib.pq_grad_squares_partials(ctypes.byref(many)) <= 3 * 2048
     assert lib.pq_grad_squares(ctypes.byref(lst), None, 1, None) == L.PQ_EINVAL
     assert lib.pq_grad_squares(ctypes.byref(many), P, 2, None) == L.PQ_ESHAPE
+    join = lib.pq_grad_squares_join
+    assert join(None, 4, P, None) == L.PQ_EINVAL and join(P, 4, None, None) == L.PQ_EINVAL and join(P, 0, P, None) == L.PQ_ESHAPE
     s = L.AdamWStates(P, P, P, P, 4096, 8)
     empty = L.AdamWStates(P, P, P, P, 0, 8)
     assert lib.pq_adamw_moments(ctypes.byref(s), None, P, 0, None) == L.PQ_EINVAL
