@@ -206,7 +206,7 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(const DownArgs p) {
 // ---- up ------------------------------------------------------------------------------------------------------------------
 // A wave takes 16 rows and 128 columns a step: eight tiles of 16 x 16, tile u of the columns with c % 8 == u, so that a lane's sums are
 // eight consecutive columns of four rows, and 16 lanes' 256 bytes of a row. The four waves of a workgroup take 16 rows each and the same `cols`
-// columns; with few rows (ROWS false) the same 64 rows, 16 at a time, and every fourth step. With rank 16 one instruction takes both
+// columns; with few rows (ROWS false) the same 64 rows, 16 at a time, and every fourth step. PAST: results go past the caches. With rank 16 one instruction takes both
 // parts of t.
 struct UpArgs {
   const float *part, *scale;
@@ -216,10 +216,9 @@ struct UpArgs {
   uint16_t* out;
   float* joined;          // [M, P]: t with its scale, or NULL
   int ldb, ldo, M, C, R, slices, cols, blocks;   // columns of a workgroup, such blocks of columns
-  int stream;                          // whether results go past the caches
 };
 
-template <int DT, int P, bool BASE, int NS, bool ROWS, bool ONE>
+template <int DT, int P, bool BASE, int NS, bool ROWS, bool ONE, bool PAST>
 __device__ __forceinline__ void up_pass(const UpArgs& p, int id, int row0, int list, int count, int c, int c_end, bool join, uint8_t* lds) {
   constexpr int KS = P == 16 ? 1 : P / 32, PARTS = P == 16 ? 1 : 2, STEP = ROWS ? 128 : 512, LANES = P == 16 ? 32 : 64;
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4, gr = P == 16 ? g & 1 : g;
@@ -370,12 +369,10 @@ __device__ __forceinline__ void up_pass(const UpArgs& p, int id, int row0, int l
         load(c + 128 < c_end ? c + 128 : first);
         __builtin_amdgcn_sched_barrier(0);
         products(slab + n * SLAB + (lane & (LANES - 1)), LANES);
-        if (p.stream) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) __builtin_nontemporal_store(result(0, i), place(0, i, c));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) *place(0, i, c) = result(0, i);
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (PAST) __builtin_nontemporal_store(result(0, i), place(0, i, c));
+          else *place(0, i, c) = result(0, i);
         }
         put(n ^ 1);
         ring_barrier();
@@ -395,7 +392,7 @@ __device__ __forceinline__ void up_pass(const UpArgs& p, int id, int row0, int l
   }
 }
 
-template <int DT, int P, bool BASE, bool ROWS>
+template <int DT, int P, bool BASE, bool ROWS, bool PAST>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const UpArgs p) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[ROWS ? 512 * P : 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -408,7 +405,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const UpArgs p) {
   if constexpr (ROWS) {
     const int id = __builtin_amdgcn_readfirstlane(mine);
     if (id >= 0 && __ballot(mine == id) == ~0ull) {
-      if (blockIdx.z == 0) up_pass<DT, P, BASE, 1, true, true>(p, id, row0 + wave * 16, lane, 16, c_begin, c_end, join, lds);
+      if (blockIdx.z == 0) up_pass<DT, P, BASE, 1, true, true, PAST>(p, id, row0 + wave * 16, lane, 16, c_begin, c_end, join, lds);
       return;
     }
     row0 += wave * 16;
@@ -418,7 +415,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const UpArgs p) {
   }
   passes(mine, blockIdx.z, gridDim.z > 1, [&](int id, uint64_t match) {
     int list = packed_rows(match, lane), count = __popcll(match);
-    for (; count > 0; count -= 16, list = __shfl(list, lane + 16)) up_pass<DT, P, BASE, 1, ROWS, false>(p, id, row0, list, count, c_begin, c_end, join, lds);
+    for (; count > 0; count -= 16, list = __shfl(list, lane + 16)) up_pass<DT, P, BASE, 1, ROWS, false, false>(p, id, row0, list, count, c_begin, c_end, join, lds);
   });
   if (blockIdx.z || (BASE && p.out == p.base)) return;
   // rows without an adapter, 16 at a time, 16 lanes a row, eight loads in flight
@@ -457,14 +454,38 @@ struct SumArgs {
   int32_t* used;          // [chunk][slot]: whether part was written
   int64_t ldz;
   int M, C, rows, panels, blocks;   // rows of a chunk (a multiple of 64), panels of 128 columns, blocks: panels * chunks, or 0
+  int by_entry;                     // a chunk's rows have at most 64 ids, and gridDim.y workgroups take an adapter of theirs each
 };
 
 template <int DT, int P>
-__device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int block, int slot, uint8_t* sz, uint8_t* sv, uint32_t* top) {
+__device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int block, int which, uint8_t* sz, uint8_t* sv, uint32_t* top) {
   constexpr int TILES = P == 16 ? 1 : P / 32, PITCH = P == 16 ? 64 : P * 2;   // of v's tiles: with P 16, the first part in ranks 0-15, the second in 16-31
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunk = block / p.panels, panel = block - chunk * p.panels;
   const int c0 = panel * 128, s0 = chunk * p.rows, end = min(p.M, s0 + p.rows);
+  int slot = p.by_entry ? -1 : which;
+  if (p.by_entry) {   // the which-th adapter among the chunk's ids
+    const uint32_t e0 = (uint32_t)s0 / ids.each;
+    const int mine = (int64_t)(e0 + lane) * ids.each < end ? ids.entry(e0 + lane) : -1;
+    uint64_t left = __ballot(mine >= 0);
+    if (which == 0 && panel == 0 && wave == 0)
+      for (int at = lane; at - lane < ids.slots; at += 64) {
+        int has = 0;
+        for (uint64_t more = left; more;) {
+          const int id = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)more) - 1);
+          more &= ~__ballot(mine == id);
+          has |= id == at;
+        }
+        if (at < ids.slots) p.used[chunk * ids.slots + at] = has;
+      }
+    for (int i = 0; left; ++i) {
+      slot = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)left) - 1);
+      left &= ~__ballot(mine == slot);
+      if (i == which) break;
+      slot = -1;
+    }
+    if (slot < 0) return;
+  }
   auto z_at = [&](int row, int at) { return sz + row * 256 + ((at ^ spread(row)) << 4); };
   auto hi_at = [&](int row, int at) { return sv + row * PITCH + (at << 4); };
   auto lo_at = [&](int row, int at) { return sv + (64 + row) * PITCH + (at << 4); };
@@ -501,7 +522,7 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int b
   };
   auto rank = [&](int j) { return P == 16 ? lane & 15 : 32 * j + (lane & 31); };
   int m0 = next(s0);
-  if (panel == 0 && tid == 0) p.used[chunk * ids.slots + slot] = m0 < end;
+  if (!p.by_entry && panel == 0 && tid == 0) p.used[chunk * ids.slots + slot] = m0 < end;
   if (m0 >= end) return;
   load(m0);
   while (m0 < end) {
@@ -605,33 +626,41 @@ struct JoinArgs {
   const float* part;
   const int32_t* used;
   uint16_t* out;
-  int chunks, C, groups, blocks;   // groups of 64 columns; workgroups (0: not wanted)
+  int chunks, C, groups, blocks;   // groups of 256 columns; workgroups (0: not wanted)
 };
 template <int DT>
 __global__ __launch_bounds__(256) void adapter_join_kernel(const JoinArgs b, const JoinArgs a, int slots, int P, int R) {
   const bool is_b = (int)blockIdx.x < b.blocks;
   const JoinArgs p = is_b ? b : a;
   const int block = (int)blockIdx.x - (is_b ? 0 : b.blocks), slot = blockIdx.y;
-  const int lane = threadIdx.x & 63, c = block % p.groups * 64 + lane, r = block / p.groups * 4 + (threadIdx.x >> 6);
-  float s = 0.0f;
-  const float* const at = p.part + ((int64_t)slot * P + min(r, P - 1)) * p.C + min(c, p.C - 1);
+  const int lane = threadIdx.x & 63, c = block % p.groups * 256 + 4 * lane, r = block / p.groups * 4 + (threadIdx.x >> 6);
+  v4f s = {};
+  const float* const at = p.part + ((int64_t)slot * P + min(r, P - 1)) * p.C + min(c, p.C - 4);
   const int64_t step = (int64_t)slots * P * p.C;
   for (int i0 = 0; i0 < p.chunks; i0 += 64) {
     uint64_t used = __ballot(i0 + lane < p.chunks && p.used[min(i0 + lane, p.chunks - 1) * slots + slot]);
-    while (used) {   // eight loads in flight
-      float v[8];
+    while (used) {   // four loads in flight
+      v4f v[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] = 0.0f;
-        if (used) v[e] = at[(i0 + __ffsll((unsigned long long)used) - 1) * step];
+      for (int e = 0; e < 4; ++e) {
+        v[e] = v4f{};
+        if (used) v[e] = *reinterpret_cast<const v4f*>(at + (i0 + __ffsll((unsigned long long)used) - 1) * step);
         used &= used - 1;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += v[e];
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) s[n] += v[e][n];
     }
   }
   if (c >= p.C || r >= R) return;
-  p.out[(int64_t)slot * R * p.C + (is_b ? (int64_t)r * p.C + c : (int64_t)c * R + r)] = (uint16_t)f32_to_16_bits<DT>(s);
+  uint16_t* const out = p.out + (int64_t)slot * R * p.C;
+  if (is_b) {
+    *reinterpret_cast<v2u*>(out + (int64_t)r * p.C + c) = v2u{pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3])};
+  } else {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) out[(int64_t)(c + n) * R + r] = (uint16_t)f32_to_16_bits<DT>(s[n]);
+  }
 }
 
 // ---- the factors' orders -------------------------------------------------------------------------------------------------
@@ -706,10 +735,12 @@ int slices_of(int64_t M, int64_t K) { const int s = slice_of(M, K); return (int)
 // Workgroups that share a tile's adapters: one for each of its rows where few rows may hold many adapters, else one takes them in turn.
 int sharers(int64_t M, int64_t each) { return each < 16 && M <= 1024 ? (by_rows(M) ? 32 : 64) : 1; }
 
+// Rows of a chunk: about 512 workgroups a sum (us of `sums` for 256, 384, 512, 768: 16384 x 5120 and 1280, rank 32, 71.8, 75.9, 70.1, 68.5; 2051 rows
+// of the same 15.3, 17.2, 16.2, 16.4), and parts of no more than 256 MB.
 int64_t chunk_rows(int64_t M, int64_t C, int64_t slots, int64_t P) {
   const int64_t steps = std::max<int64_t>((M + 63) / 64, 1), panels = (C + 127) / 128;
   const int64_t room = std::max<int64_t>(((int64_t)256 << 20) / (slots * P * C * 4), 1);
-  const int64_t want = std::min<int64_t>({(384 + panels - 1) / panels, steps, (int64_t)256, room});
+  const int64_t want = std::min<int64_t>({(512 + panels - 1) / panels, steps, (int64_t)256, room});
   return (steps + want - 1) / want * 64;
 }
 int chunks_of(int64_t M, int64_t rows) { return (int)std::max<int64_t>((M + rows - 1) / rows, 1); }
@@ -785,20 +816,23 @@ extern "C" int pq_adapter_up(const float* part, int64_t slices, const float* sca
   if ((uintptr_t)part % 16 || (uintptr_t)g % 16 || (uintptr_t)base % 16 || (base && ldb % 8) || (uintptr_t)out % 16 || ldo % 8 || (uintptr_t)joined % 16)
     return set_error(PQ_EALIGN, "pq_adapter_up: operands 16-byte aligned, strides multiples of 8");
   if (out && base == out && ldb != ldo) return set_error(PQ_ESHAPE, "pq_adapter_up: out is base, with another stride");
-  // about 1024 workgroups
-  const bool rows = by_rows(M);
+  // About 1024 workgroups; where a tile may hold several adapters, and take so many times as long, 3072 (8202 x 5120 with some twenty requests
+  // end to end: 65.7 us with 1024, 51.1 with 2048, 47.0 with 3072, 47.6 with 4096; 16384 x 5120 with 16 of them: 62.7, 67.0, 69.0, 70.4).
+  // Results of 64 MB and more go past the caches, where they would only drive out what is read next (8202 x 5120 with `down`: 78 -> 73 us,
+  // 65536 x 5120 327 -> 314, 16384 x 5120 and its backward pass 240 -> 227).
+  const bool rows = by_rows(M), past = rows && M * C >= 32 << 20;
   const int64_t tiles = (M + 63) / 64, width = rows ? 128 : 512, steps = out ? (C + width - 1) / width : 0;
-  const int64_t want = std::max<int64_t>(std::min<int64_t>(steps, 1024 / tiles), 1), each_steps = (steps + want - 1) / want;
+  const int64_t want = std::max<int64_t>(std::min<int64_t>(steps, (each < 64 ? 3072 : 1024) / tiles), 1), each_steps = (steps + want - 1) / want;
   const int blocks = steps ? (int)((steps + each_steps - 1) / each_steps) : 1;   // (no output: no columns)
   const UpArgs p{part, scale, static_cast<const uint16_t*>(g), ids_of(ids, id_bits, each, slots), static_cast<const uint16_t*>(base),
-                 static_cast<uint16_t*>(out), joined, (int)ldb, (int)ldo, (int)M, (int)C, (int)R, (int)slices, (int)(each_steps * width), blocks,
-                 M * C >= 32 << 20};   // (64 MB: they would drive out what is read next. 8202 x 5120 78 -> 73 us with `down`, 16384 x 5120 and its backward pass 240 -> 227)
+                 static_cast<uint16_t*>(out), joined, (int)ldb, (int)ldo, (int)M, (int)C, (int)R, (int)slices, (int)(each_steps * width), blocks};
   if (const int st = check_grid(tiles * blocks, 256, "pq_adapter_up")) return st;
   const dim3 grid((unsigned)(tiles * blocks), 1, (unsigned)(rows ? std::min(sharers(M, each), 16) : sharers(M, each)));
 #define PQ_UP2(D, PP, B)                                                                                    \
   do {                                                                                                      \
-    if (rows) hipLaunchKernelGGL((adapter_up_kernel<D, PP, B, true>), grid, dim3(256), 0, stream, p);       \
-    else hipLaunchKernelGGL((adapter_up_kernel<D, PP, B, false>), grid, dim3(256), 0, stream, p);           \
+    if (past) hipLaunchKernelGGL((adapter_up_kernel<D, PP, B, true, true>), grid, dim3(256), 0, stream, p);       \
+    else if (rows) hipLaunchKernelGGL((adapter_up_kernel<D, PP, B, true, false>), grid, dim3(256), 0, stream, p); \
+    else hipLaunchKernelGGL((adapter_up_kernel<D, PP, B, false, false>), grid, dim3(256), 0, stream, p);          \
   } while (0)
 #define PQ_UP(D, PP)                                          \
   do {                                                        \
@@ -843,19 +877,28 @@ extern "C" int pq_adapter_grads(const void* x, int64_t ldx, const void* dy, int6
   JoinArgs join[2];
   for (int i = 0; i < 2; ++i) {   // dB, dA
     const bool b = i == 0, wanted = b ? dB != nullptr : dA != nullptr;
-    const int64_t C = b ? N : K, rows = chunk_rows(M, C, slots, P), chunks = chunks_of(M, rows), panels = (C + 127) / 128, groups = (C + 63) / 64;
+    const int64_t C = b ? N : K, rows = chunk_rows(M, C, slots, P), chunks = chunks_of(M, rows), panels = (C + 127) / 128, groups = (C + 255) / 256;
     float* const part = reinterpret_cast<float*>(at);
     at += padded_bytes(4 * chunks * slots * P * C);
     int32_t* const used = reinterpret_cast<int32_t*>(at);
     at += padded_bytes(4 * chunks * slots);
-    sums[i] = {static_cast<const uint16_t*>(b ? dy : x), b ? t : dt, part, used, b ? lddy : ldx, (int)M, (int)C, (int)rows, (int)panels, wanted ? (int)(panels * chunks) : 0};
+    sums[i] = {static_cast<const uint16_t*>(b ? dy : x), b ? t : dt, part, used, b ? lddy : ldx, (int)M, (int)C, (int)rows, (int)panels, wanted ? (int)(panels * chunks) : 0, 0};
     join[i] = {part, used, static_cast<uint16_t*>(b ? dB : dA), (int)chunks, (int)C, (int)groups, wanted ? (int)(groups * ((R + 3) / 4)) : 0};
   }
+  // Adapters that a chunk may have, where that is fewer than there are: workgroups without rows cost a microsecond or two of a place.
+  int64_t among[2];
+  for (int i = 0; i < 2; ++i) {
+    among[i] = M ? (sums[i].rows - 1) / std::min<int64_t>(each, M) + 2 : 1;
+    sums[i].by_entry = M && among[i] <= 64 && among[i] < slots;
+  }
+  const bool by_entry = (sums[0].by_entry || !dB) && (sums[1].by_entry || !dA);
+  for (int i = 0; i < 2; ++i) sums[i].by_entry = by_entry;
+  const int64_t ways = !by_entry ? slots : std::max(dB ? among[0] : 1, dA ? among[1] : 1);
   // (no rows: no adapter has any, and the ids are not read)
   const Ids id = ids_of(ids, id_bits, M ? each : 1, slots);
   if (const int st = check_grid((int64_t)sums[0].blocks + sums[1].blocks, 256, "pq_adapter_grads")) return st;
   if (const int st = check_grid((int64_t)join[0].blocks + join[1].blocks, 256, "pq_adapter_grads")) return st;
-  const dim3 grid((unsigned)(sums[0].blocks + sums[1].blocks), (unsigned)slots), joins((unsigned)(join[0].blocks + join[1].blocks), (unsigned)slots);
+  const dim3 grid((unsigned)(sums[0].blocks + sums[1].blocks), (unsigned)ways), joins((unsigned)(join[0].blocks + join[1].blocks), (unsigned)slots);
 #define PQ_SUMS(D, PP) hipLaunchKernelGGL((adapter_sums_kernel<D, PP>), grid, dim3(256), 0, stream, sums[0], sums[1], id)
   PQ_BY_TYPE(PQ_SUMS);
 #undef PQ_SUMS

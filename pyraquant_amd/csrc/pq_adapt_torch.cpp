@@ -76,27 +76,41 @@ void forward(const Tensor& x, const Tensor& y, const Tensor& ids, const Tensor& 
 int64_t factor_bytes(const Sizes& z, int64_t C) { return up(2 * z.slots * pq_adapter_factor_size(C, z.P)); }
 int64_t parts_bytes(const Sizes& z, int64_t C) { return up(4 * pq_adapter_slices(z.M, C) * z.M * z.P); }
 
-// The whole call. `kept`, where the backward pass will need it: t.
+// What the backward pass keeps of a call: t with its scale, and the factors in the orders that it reads (those of a laid out call are
+// turned there).
+struct Kept {
+  Tensor t, a_up, b_down;
+};
+struct Wanted {
+  bool x, A, B;
+};
+Tensor order(const Sizes& z, int64_t C, const Tensor& like) {
+  return at::empty({z.slots * pq_adapter_factor_size(C, z.P)}, like.options().requires_grad(false));
+}
+
+// The whole call; `kept` is filled with what is wanted.
 Tensor run(const Tensor& x0, const Tensor& y0, const Tensor& ids, const Tensor& A, const Tensor& B, const Tensor& scale, const Sizes& z,
-           bool laid_out, Tensor out, bool keep, Tensor& kept) {
+           bool laid_out, Tensor out, Wanted w, Kept& kept) {
   const c10::DeviceGuard guard(x0.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream(x0.device().index()).stream();
   const bool in_place = out.defined() && out.const_data_ptr() == y0.const_data_ptr();
   const Tensor x = rows_of(x0), y = in_place ? y0 : rows_of(y0);
   if (!out.defined()) out = at::empty({z.M, z.N}, x.options().requires_grad(false));
   const int64_t parts = parts_bytes(z, z.K), at = laid_out ? 0 : factor_bytes(z, z.K), bt = laid_out ? 0 : factor_bytes(z, z.N);
-  if (keep) kept = at::empty({z.M, z.P}, x.options().dtype(at::kFloat).requires_grad(false));
+  if (w.B) kept.t = at::empty({z.M, z.P}, x.options().dtype(at::kFloat).requires_grad(false));
+  if (!laid_out && w.x) kept.a_up = order(z, z.K, x);
+  if (!laid_out && (w.x || w.A)) kept.b_down = order(z, z.N, x);
   const Tensor scratch = bytes(parts + at + bt, x);
   uint8_t* const s = data<uint8_t>(scratch);
   Factors f{A.const_data_ptr(), B.const_data_ptr()};
   if (!laid_out) {
     const Tensor a = dense(A), b = dense(B);
     f = {s, s + at};
-    check(pq_adapter_factors(a.const_data_ptr(), PQ_ADAPTER_BY_COLUMN, b.const_data_ptr(), PQ_ADAPTER_BY_RANK, z.slots, z.K, z.N, z.R, z.P, s, nullptr,
-                             nullptr, s + at, stream),
+    check(pq_adapter_factors(a.const_data_ptr(), PQ_ADAPTER_BY_COLUMN, b.const_data_ptr(), PQ_ADAPTER_BY_RANK, z.slots, z.K, z.N, z.R, z.P, s,
+                             data<void>(kept.a_up), data<void>(kept.b_down), s + at, stream),
           "adapters");
   }
-  forward(x, y, ids, scale, f, z, out, reinterpret_cast<float*>(s + at + bt), data<float>(kept), stream);
+  forward(x, y, ids, scale, f, z, out, reinterpret_cast<float*>(s + at + bt), data<float>(kept.t), stream);
   return out;
 }
 
@@ -104,9 +118,9 @@ struct Adapt : torch::autograd::Function<Adapt> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& y, const Tensor& ids, const Tensor& A, const Tensor& B,
                         const Tensor& scale, std::vector<int64_t> sizes, bool laid_out) {
     const Sizes z{sizes[0], sizes[1], sizes[2], sizes[3], sizes[4], sizes[5], sizes[6], (int32_t)sizes[7]};
-    Tensor kept;
-    const Tensor out = run(x, y, ids, A, B, scale, z, laid_out, Tensor(), B.requires_grad(), kept);
-    ctx->save_for_backward({A.requires_grad() ? x : Tensor(), ids, A, B, scale, kept});
+    Kept kept;
+    const Tensor out = run(x, y, ids, A, B, scale, z, laid_out, Tensor(), {x.requires_grad(), A.requires_grad(), B.requires_grad()}, kept);
+    ctx->save_for_backward({A.requires_grad() ? x : Tensor(), ids, A, B, scale, kept.t, kept.a_up, kept.b_down});
     ctx->saved_data["sizes"] = sizes;
     ctx->saved_data["laid_out"] = laid_out;
     return out;
@@ -114,7 +128,7 @@ struct Adapt : torch::autograd::Function<Adapt> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &ids = saved[1], &A = saved[2], &B = saved[3], &scale = saved[4], &kept = saved[5];
+    const Tensor &ids = saved[1], &A = saved[2], &B = saved[3], &scale = saved[4], &kept = saved[5], &a_up = saved[6], &b_down = saved[7];
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
     const Sizes z{sizes[0], sizes[1], sizes[2], sizes[3], sizes[4], sizes[5], sizes[6], (int32_t)sizes[7]};
     const bool laid_out = ctx->saved_data["laid_out"].toBool();
@@ -134,19 +148,20 @@ struct Adapt : torch::autograd::Function<Adapt> {
       if (want_B) out[4] = at::empty({z.slots, z.R, z.N}, opt);
       const bool need_dt = want_x || want_A;
       const int64_t joined = want_A ? up(4 * z.M * z.P) : 0, parts = joined + (need_dt ? parts_bytes(z, z.N) : 0);
-      const int64_t ap = need_dt ? factor_bytes(z, z.K) : 0, bp = need_dt ? factor_bytes(z, z.N) : 0;
+      const int64_t ap = need_dt && laid_out ? factor_bytes(z, z.K) : 0, bp = need_dt && laid_out ? factor_bytes(z, z.N) : 0;
       const int64_t ws = want_A || want_B ? pq_adapter_grads_workspace_size(z.M, z.K, z.N, z.slots, z.P) : 0;
       const Tensor scratch = bytes(parts + ap + bp + ws, dy);
       uint8_t* const s = data<uint8_t>(scratch);
       float* const dt = want_A ? reinterpret_cast<float*>(s) : nullptr;   // with its scale
       float* const dt_parts = reinterpret_cast<float*>(s + joined);
       if (need_dt) {
-        const Tensor a = dense(A), b = dense(B);
-        uint8_t *const g = s + parts, *const f = s + parts + ap;
-        check(pq_adapter_factors(a.const_data_ptr(), laid_out ? PQ_ADAPTER_DOWN : PQ_ADAPTER_BY_COLUMN, b.const_data_ptr(),
-                                 laid_out ? PQ_ADAPTER_UP : PQ_ADAPTER_BY_RANK, z.slots, z.K, z.N, laid_out ? z.P : z.R, z.P, nullptr,
-                                 want_x ? g : nullptr, f, nullptr, stream),
-              "adapters");
+        const void *g = data<void>(a_up), *f = data<void>(b_down);
+        if (laid_out) {
+          g = s + parts, f = s + parts + ap;
+          check(pq_adapter_factors(A.const_data_ptr(), PQ_ADAPTER_DOWN, B.const_data_ptr(), PQ_ADAPTER_UP, z.slots, z.K, z.N, z.P, z.P, nullptr,
+                                   want_x ? s + parts : nullptr, s + parts + ap, nullptr, stream),
+                "adapters");
+        }
         check(pq_adapter_down(dy.const_data_ptr(), code, z.M, z.N, stride_of(dy), f, z.slots, z.P, ids.const_data_ptr(), z.id_bits, z.each, dt_parts, stream),
               "adapters' dt");
         check(pq_adapter_up(dt_parts, pq_adapter_slices(z.M, z.N), data<float>(scale), g, z.slots, z.K, z.R, z.P, ids.const_data_ptr(), z.id_bits,
@@ -297,8 +312,8 @@ PyObject* adapt(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (any) {
         result = Adapt::apply(x2, y2, i2, A, B, scale, std::vector<int64_t>{z.M, z.K, z.N, z.slots, z.R, z.P, z.each, z.id_bits}, laid_out != 0);
       } else {
-        Tensor kept;
-        result = run(x2, y2, i2, A, B, scale, z, laid_out != 0, o2, false, kept);
+        Kept kept;
+        result = run(x2, y2, i2, A, B, scale, z, laid_out != 0, o2, {false, false, false}, kept);
       }
       if (out.defined()) {
         if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();

@@ -276,6 +276,32 @@ def test_shapes_strides_and_ids(cuda):
     assert not any(t.any() for t in g) and g[1].shape == tuned.lr_A.shape
 
 
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("n,each,K,N,slots,R", [(9, 300, 136, 264, 9, 24), (5, 1000, 520, 72, 12, 16), (40, 70, 64, 1032, 30, 64), (3, 2000, 1032, 64, 65, 8),
+                                                (128, 128, 8, 136, 6, 32)])
+def test_batches_of_long_requests(cuda, n, each, K, N, slots, R, dtype):
+    """An id for each request of many rows: the same bits as with an id for each row, forward and back, whole tiles of one adapter among
+    others with several and with none, and every adapter's gradient written."""
+    x, y, _, A, B, scale = _problem(n * each, K, N, slots, R, dtype, "one", seed=n)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    ids = torch.randint(-1, slots + 1, (n,), generator=g, device=cuda)
+    dy = torch.randn(n * each, N, device=cuda).to(dtype)
+    bank = _bank(A, B, scale, trainable=True)
+    x.requires_grad_()
+    rows = ids.repeat_interleave(each)
+    out = bank(x.view(n, each, K), y.view(n, each, N), ids)
+    junk = torch.full((1 << 26,), float("nan"), device=cuda)      # (memory that the workspaces may get)
+    del junk
+    got = torch.autograd.grad(out, (x, bank.lr_A, bank.lr_B), dy.view(n, each, N))
+    flat = bank(x, y, rows)
+    want = torch.autograd.grad(flat, (x, bank.lr_A, bank.lr_B), dy)
+    assert torch.equal(out.view(flat.shape), flat) and all(torch.equal(a, b) for a, b in zip(got, want))
+    exact, off = _want(x.detach(), y, rows, A, B, scale, dy)
+    _near(flat.detach(), exact["y"], off["y"], "y")
+    for k, v in zip(("dx", "dA", "dB"), got):
+        _near(v, exact[k], off[k], k)
+
+
 def test_factors_of_another_type(cuda):
     """fp32 factors are cast in each call, and get gradients in fp32; a frozen module answers as the tuned one."""
     x, y, i, A, B, scale = _problem(40, 64, 72, 3, 12, torch.bfloat16, "runs")
