@@ -261,17 +261,20 @@ def add_adapters(model: nn.Module, slots: int, rank: int, *, dtype: Optional[tor
     not given. Where ``trainable``, the factors are the only parameters added; every other is left as it is."""
     chosen = AdapterSet({})
     inside = set()      # (modules of a layer that is taken)
-    for name, layer in list(model.named_modules()):
+    made: Dict[nn.Module, AdaptedLinear] = {}
+    for name, layer in list(model.named_modules(remove_duplicate=False)):
         if not isinstance(layer, (nn.Linear, Int8Linear, Mxfp4Linear, SplitInLinear)) or whitelist(name) or layer in inside:
             continue
         assert name, "the model is itself a Linear: wrap it in a module"
         if layer.in_features % 8 or layer.out_features % 8:
             continue
-        first = next(iter([*layer.buffers(), *layer.parameters()]))
-        bank = LowRankAdapters(layer.in_features, layer.out_features, slots, rank, dtype=dtype or torch.bfloat16, device=first.device,
-                               trainable=trainable)
-        inside.update(layer.modules())
+        if layer not in made:      # (a layer in several places: one set of adapters, under its first name)
+            first = next(iter([*layer.buffers(), *layer.parameters()]))
+            bank = LowRankAdapters(layer.in_features, layer.out_features, slots, rank, dtype=dtype or torch.bfloat16, device=first.device,
+                                   trainable=trainable)
+            made[layer] = AdaptedLinear(layer, bank, chosen)
+            inside.update(m for m in layer.modules() if m is not layer)
+            chosen.layers[name] = bank
         parent, _, attr = name.rpartition(".")
-        setattr(model.get_submodule(parent) if parent else model, attr, AdaptedLinear(layer, bank, chosen))
-        chosen.layers[name] = bank
+        setattr(model.get_submodule(parent) if parent else model, attr, made[layer])
     return chosen

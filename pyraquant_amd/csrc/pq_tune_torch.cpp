@@ -49,7 +49,7 @@ T* data(const Tensor& t) { return t.defined() ? static_cast<T*>(const_cast<void*
 
 class Plan {
  public:
-  Plan(const std::vector<Tensor>& params, int bits) : params_(params), bits_(bits) {
+  Plan(const std::vector<Tensor>& params, int bits) : params_(params), bits_(bits), device_(params.empty() ? at::Device(at::kCPU) : params[0].device()) {
     need(bits == 8 || bits == 32, "states have 8 or 32 bits (got " + std::to_string(bits) + ")");
     need(!params.empty(), "a parameter group without parameters");
     first_.push_back(0);
@@ -105,7 +105,7 @@ class Plan {
       }
       grads_[i] = d.const_data_ptr();
     }
-    if (moved) list();
+    if (moved) list();   // (after the checks: a step that is refused changes nothing)
   }
 
   pq_adamw_list c_list() const {
@@ -168,7 +168,8 @@ class Plan {
     at_.resize(params_.size());
     for (size_t i = 0; i < params_.size(); ++i) {
       const Tensor& p = params_[i];
-      need(p.numel() == sizes_[i], "a parameter has changed its size");
+      need(p.numel() == sizes_[i] && p.is_non_overlapping_and_dense(), "a parameter has changed its size, or is not dense any more");
+      need(p.device() == device_, "a parameter has left the device that its states are on");
       at_[i] = p.const_data_ptr();
       t[i] = {const_cast<void*>(at_[i]), sizes_[i], offsets_[i], code_of(p.scalar_type()), (int32_t)first_[i]};
       std::fill(chunks.begin() + first_[i], chunks.begin() + first_[i + 1], (int32_t)i);
@@ -188,6 +189,7 @@ class Plan {
 
   std::vector<Tensor> params_, copies_;
   int bits_;
+  at::Device device_;
   int64_t n_ = 0;
   std::vector<int64_t> offsets_, sizes_, first_;
   std::vector<const void*> at_, grads_;
@@ -216,6 +218,9 @@ py::object step(const py::list& groups, double max_norm) {
     g.rates.eps = t[4].cast<double>(), g.rates.weight_decay = t[5].cast<double>();
     g.rates.seed = (uint32_t)t[6].cast<int64_t>();
     g.rates.max_norm = max_norm;
+    const pq_adamw_rates& r = g.rates;   // (checked for all groups before any is stepped)
+    need((r.lr_at || r.lr >= 0) && r.beta1 >= 0 && r.beta1 < 1 && r.beta2 >= 0 && r.beta2 < 1 && r.eps >= 0 && r.weight_decay >= 0,
+         "lr, eps and weight_decay must be 0 or more, betas in [0, 1)");
     need(!max_norm || all.empty() || all[0].plan->like().device() == g.plan->like().device(),
          "a limit on the norm of gradients on several devices is not supported");
     g.plan->collect();

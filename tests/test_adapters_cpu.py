@@ -135,3 +135,13 @@ def test_a_models_layers_get_adapters():
     assert styles.ids is None
     styles.freeze()
     assert not styles.parameters()
+
+
+def test_a_layer_in_two_places_gets_one_set():
+    from pyraquant_amd.adapters import AdaptedLinear, add_adapters
+
+    tied = torch.nn.Linear(64, 64)
+    model = torch.nn.ModuleDict({"a": tied, "b": torch.nn.Sequential(tied), "c": torch.nn.Linear(64, 64)})
+    styles = add_adapters(model, 2, 8, whitelist=lambda n: False)
+    assert sorted(styles.layers) == ["a", "c"] and model["b"][0] is model["a"] and isinstance(model["a"], AdaptedLinear)
+    assert model["a"].layer is tied

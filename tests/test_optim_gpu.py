@@ -375,11 +375,23 @@ def test_refusals(cuda):
     cpu.grad = torch.ones(3)
     with pytest.raises(AssertionError):
         _opt([p, cpu]).step()
-    with pytest.raises(AssertionError):
-        bad = _opt([p])
-        bad.param_groups[0]["betas"] = (1.0, 0.9)
-        bad.step()
-    assert not p.any() and not cpu.any()
+    p.grad = torch.ones_like(p)
+    other = torch.nn.Parameter(torch.zeros(5, device=cuda))
+    other.grad = torch.ones_like(other)
+    for name, value in (("betas", (1.0, 0.9)), ("lr", -1.0), ("eps", -1e-9), ("weight_decay", float("nan"))):
+        bad = _opt([{"params": [other]}, {"params": [p]}], max_norm=1.0)
+        bad.param_groups[1][name] = value
+        with pytest.raises(AssertionError):
+            bad.step()
+    assert not p.any() and not cpu.any() and not other.any()      # (no group is stepped where one is refused)
+    left = torch.nn.Parameter(torch.zeros(5, device=cuda))
+    left.grad = torch.ones_like(left)
+    opt = _opt([left])
+    opt.step()
+    left.grad = None
+    left.data = left.data.cpu()
+    with pytest.raises(AssertionError, match="left the device"):
+        opt.step()
 
 
 def test_autograd_sees_the_change(cuda):
