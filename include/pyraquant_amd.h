@@ -507,7 +507,7 @@ int pq_adapter_up(const float* part, int64_t slices, const float* scale, const v
 
 /* dA [slots, K, R] and dB [slots, R, N] (zeros for an adapter without rows; NULL: not wanted, and its operands may be NULL), from t and dt
  * [M, P] with their scale, as pq_adapter_up joins them. Sums in fp32 in an order that depends on the sizes alone. The workspace may hold anything. */
-int64_t pq_adapter_grads_workspace_size(int64_t M, int64_t K, int64_t N, int64_t slots, int64_t P);
+int64_t pq_adapter_grads_workspace_size(int64_t M, int64_t K, int64_t N, int64_t slots, int64_t P, int64_t each);
 int pq_adapter_grads(const void* x, int64_t ldx, const void* dy, int64_t lddy, int32_t dtype, const float* t,
                      const float* dt, const void* ids, int32_t id_bits, int64_t each, int64_t M, int64_t K, int64_t N, int64_t slots,
                      int64_t R, int64_t P, void* dA, void* dB, void* workspace, int64_t workspace_bytes, hipStream_t stream);

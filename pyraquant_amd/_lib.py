@@ -147,7 +147,7 @@ _SIGNATURES = {
     "pq_adapter_slices": ([_i64, _i64], _i64),
     "pq_adapter_down": ([_p, _i32, _i64, _i64, _i64, _p, _i64, _i64, _p, _i32, _i64, _p, _p], ctypes.c_int),
     "pq_adapter_up": ([_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _p, _i64, _p, _i32, _i64, _p], ctypes.c_int),
-    "pq_adapter_grads_workspace_size": ([_i64, _i64, _i64, _i64, _i64], _i64),
+    "pq_adapter_grads_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64], _i64),
     "pq_adapter_grads": ([_p, _i64, _p, _i64, _i32, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
                          ctypes.c_int),
     "pq_grad_squares_partials": ([_list], _i64),

@@ -453,8 +453,9 @@ struct SumArgs {
   float* part;
   int32_t* used;          // [chunk][slot]: whether part was written
   int64_t ldz;
-  int M, C, rows, panels, blocks;   // rows of a chunk (a multiple of 64), panels of 128 columns, blocks: panels * chunks, or 0
-  int by_entry;                     // a chunk's rows have at most 64 ids, and gridDim.y workgroups take an adapter of theirs each
+  int M, C, panels, blocks;   // panels of 128 columns, blocks: panels * chunks, or 0
+  int unit, parts, rows;      // see Chunks
+  int by_entry;               // a chunk's rows have at most 64 ids, and gridDim.y workgroups take an adapter of theirs each
 };
 
 template <int DT, int P>
@@ -462,7 +463,8 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int b
   constexpr int TILES = P == 16 ? 1 : P / 32, PITCH = P == 16 ? 64 : P * 2;   // of v's tiles: with P 16, the first part in ranks 0-15, the second in 16-31
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunk = block / p.panels, panel = block - chunk * p.panels;
-  const int c0 = panel * 128, s0 = chunk * p.rows, end = min(p.M, s0 + p.rows);
+  const int unit = chunk / p.parts, u0 = unit * p.unit, at0 = (chunk - unit * p.parts) * p.rows;
+  const int c0 = panel * 128, s0 = u0 + at0, end = min(p.M, u0 + min(p.unit, at0 + p.rows));
   int slot = p.by_entry ? -1 : which;
   if (p.by_entry) {   // the which-th adapter among the chunk's ids
     const uint32_t e0 = (uint32_t)s0 / ids.each;
@@ -735,15 +737,24 @@ int slices_of(int64_t M, int64_t K) { const int s = slice_of(M, K); return (int)
 // Workgroups that share a tile's adapters: one for each of its rows where few rows may hold many adapters, else one takes them in turn.
 int sharers(int64_t M, int64_t each) { return each < 16 && M <= 1024 ? (by_rows(M) ? 32 : 64) : 1; }
 
-// Rows of a chunk: about 512 workgroups a sum (us of `sums` for 256, 384, 512, 768: 16384 x 5120 and 1280, rank 32, 71.8, 75.9, 70.1, 68.5; 2051 rows
-// of the same 15.3, 17.2, 16.2, 16.4), and parts of no more than 256 MB.
-int64_t chunk_rows(int64_t M, int64_t C, int64_t slots, int64_t P) {
-  const int64_t steps = std::max<int64_t>((M + 63) / 64, 1), panels = (C + 127) / 128;
-  const int64_t room = std::max<int64_t>(((int64_t)256 << 20) / (slots * P * C * 4), 1);
+// The rows in units of `unit` and each unit in `parts` of `rows`, a chunk each, so that about 512 workgroups take a sum (us of `sums` for 256, 384,
+// 512, 768, with ids of one row: 16384 x 5120 and 1280, rank 32, 71.8, 75.9, 70.1, 68.5; 2051 rows of the same 15.3, 17.2, 16.2, 16.4), and the parts
+// have no more than 256 MB. Units are whole requests, so that a chunk's workgroup has all its rows for one adapter where they are long (the first of
+// these, requests of 1024 rows: 66 us with chunks of 1280 and 320 rows, which two or three requests share, and 53 with 1024 and 384).
+struct Chunks { int64_t unit, parts, rows, count; };
+Chunks chunks_of(int64_t M, int64_t C, int64_t slots, int64_t P, int64_t each) {
+  if (M < 1) return {64, 1, 64, 1};
+  const int64_t steps = (M + 63) / 64, panels = (C + 127) / 128;
+  const int64_t room = std::max<int64_t>(((int64_t)128 << 20) / (slots * P * C * 4), 1);   // (units may come out half as long as wanted)
   const int64_t want = std::min<int64_t>({(512 + panels - 1) / panels, steps, (int64_t)256, room});
-  return (steps + want - 1) / want * 64;
+  const int64_t rows = (steps + want - 1) / want * 64;
+  if (each <= rows) {
+    const int64_t unit = rows / each * each;
+    return {unit, 1, unit, (M + unit - 1) / unit};
+  }
+  const int64_t of_each = (each + 63) / 64, long_steps = (of_each + each / rows - 1) / (each / rows), parts = (of_each + long_steps - 1) / long_steps;
+  return {each, parts, long_steps * 64, M / each * parts};
 }
-int chunks_of(int64_t M, int64_t rows) { return (int)std::max<int64_t>((M + rows - 1) / rows, 1); }
 
 int check_ids(const void* ids, int32_t id_bits, int64_t each, int64_t M, int64_t slots, const char* what) {
   if (id_bits != 32 && id_bits != 64) return set_error(PQ_EDTYPE, "%s: ids of %d bits (32 or 64)", what, id_bits);
@@ -846,11 +857,11 @@ extern "C" int pq_adapter_up(const float* part, int64_t slices, const float* sca
 
 static int64_t padded_bytes(int64_t n) { return (n + 255) / 256 * 256; }
 
-extern "C" int64_t pq_adapter_grads_workspace_size(int64_t M, int64_t K, int64_t N, int64_t slots, int64_t P) {
-  if (M < 0 || M > (1 << 30) || !size_ok(K) || !size_ok(N) || slots < 1 || slots > 65535 || !rank_ok(1, P)) return 0;
+extern "C" int64_t pq_adapter_grads_workspace_size(int64_t M, int64_t K, int64_t N, int64_t slots, int64_t P, int64_t each) {
+  if (M < 0 || M > (1 << 30) || !size_ok(K) || !size_ok(N) || slots < 1 || slots > 65535 || !rank_ok(1, P) || (M && (each < 1 || M % each))) return 0;
   int64_t bytes = 0;
   for (const int64_t C : {N, K}) {
-    const int64_t chunks = chunks_of(M, chunk_rows(M, C, slots, P));
+    const int64_t chunks = chunks_of(M, C, slots, P, each).count;
     bytes += padded_bytes(4 * chunks * slots * P * C) + padded_bytes(4 * chunks * slots);
   }
   return bytes;
@@ -870,25 +881,28 @@ extern "C" int pq_adapter_grads(const void* x, int64_t ldx, const void* dy, int6
   if ((dA && ((uintptr_t)x % 16 || ldx % 8 || (uintptr_t)dt % 16)) || (dB && ((uintptr_t)dy % 16 || lddy % 8 || (uintptr_t)t % 16)) ||
       (uintptr_t)workspace % 16)
     return set_error(PQ_EALIGN, "pq_adapter_grads: operands 16-byte aligned, strides multiples of 8");
-  if (workspace_bytes < pq_adapter_grads_workspace_size(M, K, N, slots, P))
+  if (workspace_bytes < pq_adapter_grads_workspace_size(M, K, N, slots, P, each))
     return set_error(PQ_ESHAPE, "pq_adapter_grads: workspace of %lld bytes", (long long)workspace_bytes);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   SumArgs sums[2];
   JoinArgs join[2];
   for (int i = 0; i < 2; ++i) {   // dB, dA
     const bool b = i == 0, wanted = b ? dB != nullptr : dA != nullptr;
-    const int64_t C = b ? N : K, rows = chunk_rows(M, C, slots, P), chunks = chunks_of(M, rows), panels = (C + 127) / 128, groups = (C + 255) / 256;
+    const int64_t C = b ? N : K, panels = (C + 127) / 128, groups = (C + 255) / 256;
+    const Chunks of = chunks_of(M, C, slots, P, each);
+    const int64_t chunks = of.count;
     float* const part = reinterpret_cast<float*>(at);
     at += padded_bytes(4 * chunks * slots * P * C);
     int32_t* const used = reinterpret_cast<int32_t*>(at);
     at += padded_bytes(4 * chunks * slots);
-    sums[i] = {static_cast<const uint16_t*>(b ? dy : x), b ? t : dt, part, used, b ? lddy : ldx, (int)M, (int)C, (int)rows, (int)panels, wanted ? (int)(panels * chunks) : 0, 0};
+    sums[i] = {static_cast<const uint16_t*>(b ? dy : x), b ? t : dt, part, used, b ? lddy : ldx, (int)M, (int)C, (int)panels, wanted ? (int)(panels * chunks) : 0,
+               (int)of.unit, (int)of.parts, (int)of.rows, 0};
     join[i] = {part, used, static_cast<uint16_t*>(b ? dB : dA), (int)chunks, (int)C, (int)groups, wanted ? (int)(groups * ((R + 3) / 4)) : 0};
   }
   // Adapters that a chunk may have, where that is fewer than there are: workgroups without rows cost a microsecond or two of a place.
   int64_t among[2];
   for (int i = 0; i < 2; ++i) {
-    among[i] = M ? (sums[i].rows - 1) / std::min<int64_t>(each, M) + 2 : 1;
+    among[i] = M ? std::max<int64_t>(sums[i].unit / each, 1) : 1;
     sums[i].by_entry = M && among[i] <= 64 && among[i] < slots;
   }
   const bool by_entry = (sums[0].by_entry || !dB) && (sums[1].by_entry || !dA);

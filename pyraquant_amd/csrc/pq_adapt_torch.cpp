@@ -149,7 +149,7 @@ struct Adapt : torch::autograd::Function<Adapt> {
       const bool need_dt = want_x || want_A;
       const int64_t joined = want_A ? up(4 * z.M * z.P) : 0, parts = joined + (need_dt ? parts_bytes(z, z.N) : 0);
       const int64_t ap = need_dt && laid_out ? factor_bytes(z, z.K) : 0, bp = need_dt && laid_out ? factor_bytes(z, z.N) : 0;
-      const int64_t ws = want_A || want_B ? pq_adapter_grads_workspace_size(z.M, z.K, z.N, z.slots, z.P) : 0;
+      const int64_t ws = want_A || want_B ? pq_adapter_grads_workspace_size(z.M, z.K, z.N, z.slots, z.P, z.each) : 0;
       const Tensor scratch = bytes(parts + ap + bp + ws, dy);
       uint8_t* const s = data<uint8_t>(scratch);
       float* const dt = want_A ? reinterpret_cast<float*>(s) : nullptr;   // with its scale

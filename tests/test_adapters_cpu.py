@@ -56,7 +56,8 @@ def test_gradient_and_order_refusals():
     assert grads(x=ODD) == L.PQ_EALIGN and grads(lddy=68) == L.PQ_EALIGN and grads(ws=ODD) == L.PQ_EALIGN
     assert grads(dA=None, dB=None) == L.PQ_OK
     size = lib.pq_adapter_grads_workspace_size
-    assert size(4, 60, 64, 2, 16) == 0 and size(4, 64, 64, 0, 16) == 0 and 0 < size(4, 64, 64, 2, 16) < size(100000, 64, 64, 2, 16)
+    assert size(4, 60, 64, 2, 16, 1) == 0 and size(4, 64, 64, 0, 16, 1) == 0 and size(4, 64, 64, 2, 16, 3) == 0
+    assert 0 < size(4, 64, 64, 2, 16, 1) < size(100000, 64, 64, 2, 16, 1)
     assert 1 <= lib.pq_adapter_slices(1, 65536) <= 16 and lib.pq_adapter_slices(1 << 20, 64) == 1 and lib.pq_adapter_slices(0, 64) == 1
     lay = lambda A=P, B=P, slots=2, K=64, N=64, R=8, PP=16, at=P, bt=P, oa=0, ob=1: lib.pq_adapter_factors(   # noqa: E731
         A, oa, B, ob, slots, K, N, R, PP, at, None, None, bt, None)

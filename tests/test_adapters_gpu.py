@@ -280,8 +280,8 @@ def test_shapes_strides_and_ids(cuda):
 @pytest.mark.parametrize("n,each,K,N,slots,R", [(9, 300, 136, 264, 9, 24), (5, 1000, 520, 72, 12, 16), (40, 70, 64, 1032, 30, 64), (3, 2000, 1032, 64, 65, 8),
                                                 (128, 128, 8, 136, 6, 32)])
 def test_batches_of_long_requests(cuda, n, each, K, N, slots, R, dtype):
-    """An id for each request of many rows: the same bits as with an id for each row, forward and back, whole tiles of one adapter among
-    others with several and with none, and every adapter's gradient written."""
+    """An id for each request of many rows: the same bits as with an id for each row, forward and back (but for the sums over rows, whose
+    chunks are whole requests), whole tiles of one adapter among others with several and with none, and every adapter's gradient written."""
     x, y, _, A, B, scale = _problem(n * each, K, N, slots, R, dtype, "one", seed=n)
     g = torch.Generator(device="cuda").manual_seed(n)
     ids = torch.randint(-1, slots + 1, (n,), generator=g, device=cuda)
@@ -295,11 +295,12 @@ def test_batches_of_long_requests(cuda, n, each, K, N, slots, R, dtype):
     got = torch.autograd.grad(out, (x, bank.lr_A, bank.lr_B), dy.view(n, each, N))
     flat = bank(x, y, rows)
     want = torch.autograd.grad(flat, (x, bank.lr_A, bank.lr_B), dy)
-    assert torch.equal(out.view(flat.shape), flat) and all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(out.view(flat.shape), flat) and torch.equal(got[0], want[0])
     exact, off = _want(x.detach(), y, rows, A, B, scale, dy)
     _near(flat.detach(), exact["y"], off["y"], "y")
-    for k, v in zip(("dx", "dA", "dB"), got):
+    for k, v, r in zip(("dx", "dA", "dB"), got, want):
         _near(v, exact[k], off[k], k)
+        _near(r, exact[k], off[k], k)
 
 
 def test_factors_of_another_type(cuda):
@@ -482,7 +483,7 @@ def test_kernels_write_what_they_say(cuda):
         up(dt, Sd, None, K, None, alone)
         whole(tj, dtj, alone)
         assert torch.equal(alone[1], dtj[1]) and bool((tj[1].view(M, P)[none] == 7).all()) and not tj[1].view(M, P)[~none][:, R:].any()
-        room = L.pq_adapter_grads_workspace_size(M, K, N, slots, P)
+        room = L.pq_adapter_grads_workspace_size(M, K, N, slots, P, 1)
         ws = torch.full((room + 256,), 255, dtype=torch.uint8, device=cuda)
         _lib.check(L.pq_adapter_grads(p(x), K, p(dy), N, 0, p(tj[1]), p(dtj[1]), p(i), 32, 1, M, K, N, slots, R, P, p(dA[1]), p(dB[1]), p(ws), room,
                                       stream), "grads")
