@@ -62,6 +62,8 @@ EXPORTS = (
     "pq_adapter_slices",
     "pq_adapter_down",
     "pq_adapter_up",
+    "pq_adapter_rows_fit",
+    "pq_adapter_rows",
     "pq_adapter_grads_workspace_size",
     "pq_adapter_grads",
     "pq_grad_squares_partials",
@@ -147,6 +149,8 @@ _SIGNATURES = {
     "pq_adapter_slices": ([_i64, _i64], _i64),
     "pq_adapter_down": ([_p, _i32, _i64, _i64, _i64, _p, _i64, _i64, _p, _i32, _i64, _p, _p], ctypes.c_int),
     "pq_adapter_up": ([_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _p, _i64, _p, _i32, _i64, _p], ctypes.c_int),
+    "pq_adapter_rows_fit": ([_i64] * 5, ctypes.c_int),
+    "pq_adapter_rows": ([_p, _i32, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _p, _i64, _p, _p], ctypes.c_int),
     "pq_adapter_grads_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64], _i64),
     "pq_adapter_grads": ([_p, _i64, _p, _i64, _i32, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
                          ctypes.c_int),

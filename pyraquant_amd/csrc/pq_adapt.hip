@@ -80,7 +80,8 @@ __device__ __forceinline__ int64_t up_at(int c, int r, int P) {
 // A wave takes 16 NS rows and 64 k a step, the next step on its way meanwhile; x goes through its part of LDS (8 lanes a row; chunk c of a
 // row at c ^ (row % 8), so that neither direction meets a bank twice). The factor is the first operand, so that a lane's sums are of one row
 // and four consecutive ranks. The four waves of a workgroup take 32 rows each and the same slice of k; with few rows (ROWS false) the same 64
-// rows, 16 at a time, and every fourth step, and add their sums in LDS.
+// rows, 16 at a time, and every fourth step, and add their sums in LDS. Bound by memory where there are many rows: 65536 x 1280 bf16 with rank
+// 64 40 us, 4.2 TB/s of x; 16384 x 5120 with rank 32 39 us, 4.3; 8202 x 640 9.2 us, most of it the start and the end of the launch.
 struct DownArgs {
   const uint16_t *x, *f;
   Ids ids;
@@ -206,8 +207,10 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(const DownArgs p) {
 // ---- up ------------------------------------------------------------------------------------------------------------------
 // A wave takes 16 rows and 128 columns a step: eight tiles of 16 x 16, tile u of the columns with c % 8 == u, so that a lane's sums are
 // eight consecutive columns of four rows, and 16 lanes' 256 bytes of a row. The four waves of a workgroup take 16 rows each and the same `cols`
-// columns; with few rows (ROWS false) the same 64 rows, 16 at a time, and every fourth step. PAST: results go past the caches. With rank 16 one instruction takes both
-// parts of t.
+// columns; with few rows (ROWS false) the same 64 rows, 16 at a time, and every fourth step. PAST: results go past the caches. With rank 16
+// one instruction takes both parts of t. Bound by memory where there are many rows: 65536 x 5120 bf16 with rank 64, base read and result
+// written, 277 us, 4.8 TB/s; 16384 x 5120 with rank 32 71.5 us, 4.7. 8202 rows whose twenty-odd requests end inside tiles 44 us, 3.8: such a
+// tile's passes read the factors of each of its adapters from the second cache.
 struct UpArgs {
   const float *part, *scale;
   const uint16_t* g;
@@ -443,10 +446,146 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const UpArgs p) {
   }
 }
 
+// ---- a few rows, both products in one launch -----------------------------------------------------------------------------
+// A workgroup of eight waves takes a row and `cols` columns: t whole (32 k a wave at a time, lane 16 q + r the product of eight k and rank r,
+// added over lanes and waves), then 128 columns of the result a wave. No matrix instructions: of 16 rows they would use one. Bound by the latency of
+// three loads that wait for each other (an id, its factor, the launch) and, from some 64 rows on, by the factors' way from the second cache: a row
+// reads K P values for each of its column blocks. A row's workgroups are M apart, on one XCD where M is a multiple of 8.
+struct RowArgs {
+  const uint16_t *x, *f, *g, *base;
+  const float* scale;
+  uint16_t* out;
+  float* joined;
+  Ids ids;
+  int64_t ldx, ldb, ldo;
+  int M, K, C, R, cols;
+};
+
+template <int DT>
+__device__ __forceinline__ float dot8(v4u a, v4u b, float s) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    s = fmaf(lo16_to_f32<DT>(a[e]), lo16_to_f32<DT>(b[e]), s);
+    s = fmaf(hi16_to_f32<DT>(a[e]), hi16_to_f32<DT>(b[e]), s);
+  }
+  return s;
+}
+template <int DT>
+__device__ __forceinline__ float dot8(v4f t0, v4f t1, v4u b, float s) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const v4f t = e < 2 ? t0 : t1;
+    s = fmaf(t[2 * e & 3], lo16_to_f32<DT>(b[e]), s);
+    s = fmaf(t[(2 * e & 3) + 1], hi16_to_f32<DT>(b[e]), s);
+  }
+  return s;
+}
+
+template <int DT, int P, bool BASE>
+__global__ __launch_bounds__(512) void adapter_rows_kernel(const RowArgs p) {
+  constexpr int J = P / 16, G = P / 4, AHEAD = P == 64 ? 2 : 4;   // a wave's loads of 128 columns of g; blocks of 32 k in flight
+  __shared__ __attribute__((aligned(16))) float parts[8][P];
+  __shared__ __attribute__((aligned(16))) float t[P];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int block = (int)blockIdx.x / p.M, m = (int)blockIdx.x - block * p.M;
+  const int c_begin = block * p.cols, c_end = min(p.C, c_begin + p.cols);
+  const int id = __builtin_amdgcn_readfirstlane(p.ids.of(m));
+  const uint16_t* const base = p.base + (int64_t)m * p.ldb;
+  uint16_t* const out = p.out + (int64_t)m * p.ldo;
+  if (id < 0) {
+    if (BASE && p.out == p.base) return;
+    for (int c = c_begin + (int)threadIdx.x * 8; c < c_end; c += 4096)
+      *reinterpret_cast<v4u*>(out + c) = BASE ? *reinterpret_cast<const v4u*>(base + c) : v4u{0, 0, 0, 0};
+    return;
+  }
+  v4u gv[G], bv;
+  const v4u* const g = reinterpret_cast<const v4u*>(p.g + id * factor_size(p.C, P));
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) gv[i] = g[(int64_t)(c0 >> 7) * (16 * P) + i * 64 + lane];
+    if constexpr (BASE) bv = *reinterpret_cast<const v4u*>(base + min(c0 + 8 * (lane & 15), p.C - 8));
+  };
+  int c0 = c_begin + wave * 128;
+  if (c0 < c_end) load(c0);   // in flight while t is summed
+
+  const uint16_t* const x = p.x + m * p.ldx;
+  const v4u* const f = reinterpret_cast<const v4u*>(p.f + id * factor_size(p.K, P));
+  const int blocks = (p.K + 31) >> 5;
+  float acc[J] = {};
+  for (int k0 = wave; k0 < blocks; k0 += 8 * AHEAD) {
+    v4u xv[AHEAD], fv[AHEAD][J];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int k = min(k0 + 8 * a, blocks - 1), c = k * 32 + 8 * (lane >> 4);
+      xv[a] = *reinterpret_cast<const v4u*>(x + min(c, p.K - 8));
+#pragma unroll
+      for (int j = 0; j < J; ++j) fv[a][j] = f[((int64_t)k * J + j) * 64 + lane];
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const bool in = (k0 + 8 * a) * 32 + 8 * (lane >> 4) < p.K;   // zeros on both sides past K: an infinity times zero is none of the sum's
+      if (!in) xv[a] = v4u{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[j] = dot8<DT>(xv[a], in ? fv[a][j] : v4u{0, 0, 0, 0}, acc[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    acc[j] += __shfl_xor(acc[j], 16);
+    acc[j] += __shfl_xor(acc[j], 32);
+    if (lane < 16) parts[wave][16 * j + lane] = acc[j];
+  }
+  __syncthreads();
+  if (threadIdx.x < P) {
+    const int r = threadIdx.x;
+    float sum = parts[0][r];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) sum += parts[w][r];
+    sum = r < p.R ? sum * p.scale[id] : 0.0f;
+    t[r] = sum;
+    if (p.joined && block == 0) p.joined[(int64_t)m * P + r] = sum;
+  }
+  __syncthreads();
+  while (c0 < c_end) {
+    float sum[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {   // column 8 (lane % 16) + u: the ranks of lane / 16, added over the lanes
+      const int at = P == 16 ? (lane >> 4 & 1) * 8 : (lane >> 4) * 8;
+      const v4f t0 = *reinterpret_cast<const v4f*>(t + at), t1 = *reinterpret_cast<const v4f*>(t + at + 4);
+      if constexpr (P == 16) {      // (two columns a load, lanes 0-31 and 32-63)
+        if (u & 1) continue;
+        float one = dot8<DT>(t0, t1, gv[u / 2], 0.0f);
+        one += __shfl_xor(one, 16);
+        const float other = __shfl_xor(one, 32);
+        sum[u] = lane < 32 ? one : other;
+        sum[u + 1] = lane < 32 ? other : one;
+      } else {
+        float one = dot8<DT>(t0, t1, gv[u * (P / 32)], 0.0f);
+        if constexpr (P == 64) {
+          const v4f t2 = *reinterpret_cast<const v4f*>(t + at + 32), t3 = *reinterpret_cast<const v4f*>(t + at + 36);
+          one = dot8<DT>(t2, t3, gv[2 * u + 1], one);
+        }
+        one += __shfl_xor(one, 16);
+        sum[u] = one + __shfl_xor(one, 32);
+      }
+    }
+    v4u o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] = BASE ? pack2<DT>(sum[2 * e] + lo16_to_f32<DT>(bv[e]), sum[2 * e + 1] + hi16_to_f32<DT>(bv[e])) : pack2<DT>(sum[2 * e], sum[2 * e + 1]);
+    const int c = c0 + 8 * (lane & 15);
+    if (lane < 16 && c < c_end) *reinterpret_cast<v4u*>(out + c) = o;
+    c0 += 1024;
+    if (c0 < c_end) load(c0);
+  }
+}
+
 // ---- sums over the rows of an adapter ------------------------------------------------------------------------------------
 // part[chunk][slot][r][c] = sum over the chunk's rows m of that adapter of v[m, r] z[m, c], v: t or dt with its scale (`joined`). A
 // workgroup of four waves takes 128 columns, a chunk of rows and an adapter; of its rows, 64 a step, only steps that hold a row of
-// the adapter are read, the next one's on their way into registers meanwhile, with zeros in the place of other adapters' rows.
+// the adapter are read, the next one's on their way into registers meanwhile, with zeros in the place of other adapters' rows. Both sums of
+// 16384 x (5120 + 1280) bf16 with rank 32: 53 us, 4.0 TB/s of dy and x; beside them each panel reads t, half as many bytes again, from the
+// second cache.
 struct SumArgs {
   const uint16_t* z;
   const float* v;
@@ -623,7 +762,7 @@ __global__ __launch_bounds__(256) void adapter_sums_kernel(const SumArgs b, cons
   row_sums<DT, P>(is_b ? b : a, ids, (int)blockIdx.x - (is_b ? 0 : b.blocks), blockIdx.y, sz, sv, top);
 }
 
-// The chunks' sums in order, rounded: dB [slots, R, N] and dA [slots, K, R].
+// The chunks' sums in order, rounded: dB [slots, R, N] and dA [slots, K, R]. (8 adapters of 5120 + 1280 columns and rank 32, of 16 and 48 chunks, 8 us.)
 struct JoinArgs {
   const float* part;
   const int32_t* used;
@@ -827,13 +966,13 @@ extern "C" int pq_adapter_up(const float* part, int64_t slices, const float* sca
   if ((uintptr_t)part % 16 || (uintptr_t)g % 16 || (uintptr_t)base % 16 || (base && ldb % 8) || (uintptr_t)out % 16 || ldo % 8 || (uintptr_t)joined % 16)
     return set_error(PQ_EALIGN, "pq_adapter_up: operands 16-byte aligned, strides multiples of 8");
   if (out && base == out && ldb != ldo) return set_error(PQ_ESHAPE, "pq_adapter_up: out is base, with another stride");
-  // About 1024 workgroups; where a tile may hold several adapters, and take so many times as long, 3072 (8202 x 5120 with some twenty requests
-  // end to end: 65.7 us with 1024, 51.1 with 2048, 47.0 with 3072, 47.6 with 4096; 16384 x 5120 with 16 of them: 62.7, 67.0, 69.0, 70.4).
+  // About 1024 workgroups; where a tile may hold several adapters, and take so many times as long, 4096 (8202 x 5120 with some twenty requests
+  // end to end: 65.7 us with 1024, 51.1 with 2048, 47.6 with 4096; 16384 x 5120 with 16 of them: 62.7, 67.0, 70.4).
   // Results of 64 MB and more go past the caches, where they would only drive out what is read next (8202 x 5120 with `down`: 78 -> 73 us,
   // 65536 x 5120 327 -> 314, 16384 x 5120 and its backward pass 240 -> 227).
   const bool rows = by_rows(M), past = rows && M * C >= 32 << 20;
   const int64_t tiles = (M + 63) / 64, width = rows ? 128 : 512, steps = out ? (C + width - 1) / width : 0;
-  const int64_t want = std::max<int64_t>(std::min<int64_t>(steps, (each < 64 ? 3072 : 1024) / tiles), 1), each_steps = (steps + want - 1) / want;
+  const int64_t want = std::max<int64_t>(std::min<int64_t>(steps, (each < 64 ? 4096 : 1024) / tiles), 1), each_steps = (steps + want - 1) / want;
   const int blocks = steps ? (int)((steps + each_steps - 1) / each_steps) : 1;   // (no output: no columns)
   const UpArgs p{part, scale, static_cast<const uint16_t*>(g), ids_of(ids, id_bits, each, slots), static_cast<const uint16_t*>(base),
                  static_cast<uint16_t*>(out), joined, (int)ldb, (int)ldo, (int)M, (int)C, (int)R, (int)slices, (int)(each_steps * width), blocks};
@@ -919,6 +1058,42 @@ extern "C" int pq_adapter_grads(const void* x, int64_t ldx, const void* dy, int6
   if (dtype == PQ_BF16) hipLaunchKernelGGL(adapter_join_kernel<PQ_BF16>, joins, dim3(256), 0, stream, join[0], join[1], (int)slots, (int)P, (int)R);
   else hipLaunchKernelGGL(adapter_join_kernel<PQ_F16>, joins, dim3(256), 0, stream, join[0], join[1], (int)slots, (int)P, (int)R);
   return check_launch("pq_adapter_grads");
+}
+
+// One launch for both products (us of two launches and of one in a captured graph, bf16, every row another of up to 32 adapters, P 16: 1280 x 1280,
+// 1 row 5.7 and 3.5, 64 rows 6.2 and 3.8; 4096 x 4096, 1 row 7.1 and 4.7, 64 rows 10.4 and 6.8; 5120 x 1280 6.5 and 5.2. P 32: 5120 x 1280,
+// 1 row 7.2 and 6.9; 8192 x 8192 8.1 and 9.5; P 64: 5120 x 1280 8.6 and 9.1). A workgroup reads a factor for one row alone, so many rows are for `down`
+// and `up`: later where a tile of 64 rows may hold many adapters (1280 x 5120 with 16 adapters in turn, P 16, 1024 rows 47 and 20; P 32, 512 rows 31 and
+// 18) than where requests are long (77 rows each: P 16, 308 rows 11.6 and 10.5; P 32, 154 rows 10.7 and 10.4, 308 12.9 and 14.6).
+extern "C" int pq_adapter_rows_fit(int64_t M, int64_t K, int64_t C, int64_t P, int64_t each) {
+  return size_ok(K) && size_ok(C) && rank_ok(1, P) && K * P <= 160 << 10 && M * P <= (each < 16 ? 16 << 10 : 5 << 10);
+}
+
+extern "C" int pq_adapter_rows(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* f, const float* scale, const void* g,
+                               int64_t slots, int64_t C, int64_t R, int64_t P, const void* ids, int32_t id_bits, int64_t each, const void* base,
+                               int64_t ldb, void* out, int64_t ldo, float* joined, hipStream_t stream) {
+  if (M < 0 || M > (1 << 16) || !size_ok(K) || ldx < K || !size_ok(C) || (out && ldo < C) || (base && ldb < C) || !rank_ok(R, P))
+    return set_error(PQ_ESHAPE, "pq_adapter_rows: M=%lld K=%lld C=%lld ldx=%lld ldb=%lld ldo=%lld R=%lld P=%lld (K and C multiples of 8)",
+                     (long long)M, (long long)K, (long long)C, (long long)ldx, (long long)ldb, (long long)ldo, (long long)R, (long long)P);
+  if (dtype != PQ_BF16 && dtype != PQ_F16) return set_error(PQ_EDTYPE, "pq_adapter_rows: dtype %d", dtype);
+  if (const int st = check_ids(ids, id_bits, each, M, slots, "pq_adapter_rows")) return st;
+  if (M == 0) return PQ_OK;
+  if (!x || !f || !scale || (!out && (!joined || base)) || (out && !g)) return set_error(PQ_EINVAL, "pq_adapter_rows: null pointer");
+  if ((uintptr_t)x % 16 || ldx % 8 || (uintptr_t)f % 16 || (uintptr_t)g % 16 || (uintptr_t)base % 16 || (base && ldb % 8) || (uintptr_t)out % 16 || (out && ldo % 8) || (uintptr_t)joined % 16)
+    return set_error(PQ_EALIGN, "pq_adapter_rows: operands 16-byte aligned, strides multiples of 8");
+  if (out && base == out && ldb != ldo) return set_error(PQ_ESHAPE, "pq_adapter_rows: out is base, with another stride");
+  const int64_t panels = out ? (C + 127) / 128 : 0, blocks = std::max<int64_t>(std::min<int64_t>(panels, 256 / M), 1), cols = (panels + blocks - 1) / blocks * 128;
+  const RowArgs p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(f), static_cast<const uint16_t*>(g), static_cast<const uint16_t*>(base), scale,
+                  static_cast<uint16_t*>(out), joined, ids_of(ids, id_bits, each, slots), ldx, ldb, ldo, (int)M, (int)K, (int)C, (int)R, (int)cols};
+  const dim3 grid((unsigned)(M * (out ? (C + cols - 1) / cols : 1)));   // (no result: no columns)
+#define PQ_ROWS(D, PP)                                                                                    \
+  do {                                                                                                    \
+    if (base) hipLaunchKernelGGL((adapter_rows_kernel<D, PP, true>), grid, dim3(512), 0, stream, p);      \
+    else hipLaunchKernelGGL((adapter_rows_kernel<D, PP, false>), grid, dim3(512), 0, stream, p);          \
+  } while (0)
+  PQ_BY_TYPE(PQ_ROWS);
+#undef PQ_ROWS
+  return check_launch("pq_adapter_rows");
 }
 
 extern "C" int64_t pq_adapter_factor_size(int64_t C, int64_t P) { return size_ok(C) && rank_ok(1, P) ? factor_size(C, (int)P) : 0; }

@@ -59,6 +59,8 @@ struct Sizes {
   int64_t M, K, N, slots, R, P, each;
   int32_t id_bits;
 };
+// (K to C: one launch makes both products)
+bool few_rows(const Sizes& z, int64_t K, int64_t C) { return pq_adapter_rows_fit(z.M, K, C, z.P, z.each); }
 struct Factors {   // in the orders that a pass reads
   const void *down, *up;
 };
@@ -66,6 +68,12 @@ struct Factors {   // in the orders that a pass reads
 // out [M, N] from x [M, K] and y [M, N]; parts: scratch; joined: t with its scale [M, P], kept for the backward pass, or NULL.
 void forward(const Tensor& x, const Tensor& y, const Tensor& ids, const Tensor& scale, Factors f, const Sizes& z, const Tensor& out,
              float* parts, float* joined, hipStream_t stream) {
+  if (few_rows(z, z.K, z.N)) {
+    check(pq_adapter_rows(x.const_data_ptr(), code_of(x), z.M, z.K, stride_of(x), f.down, data<float>(scale), f.up, z.slots, z.N, z.R, z.P,
+                          ids.const_data_ptr(), z.id_bits, z.each, y.const_data_ptr(), stride_of(y), out.data_ptr(), stride_of(out), joined, stream),
+          "adapters");
+    return;
+  }
   check(pq_adapter_down(x.const_data_ptr(), code_of(x), z.M, z.K, stride_of(x), f.down, z.slots, z.P, ids.const_data_ptr(), z.id_bits,
                         z.each, parts, stream),
         "adapters");
@@ -96,11 +104,11 @@ Tensor run(const Tensor& x0, const Tensor& y0, const Tensor& ids, const Tensor& 
   const bool in_place = out.defined() && out.const_data_ptr() == y0.const_data_ptr();
   const Tensor x = rows_of(x0), y = in_place ? y0 : rows_of(y0);
   if (!out.defined()) out = at::empty({z.M, z.N}, x.options().requires_grad(false));
-  const int64_t parts = parts_bytes(z, z.K), at = laid_out ? 0 : factor_bytes(z, z.K), bt = laid_out ? 0 : factor_bytes(z, z.N);
+  const int64_t parts = few_rows(z, z.K, z.N) ? 0 : parts_bytes(z, z.K), at = laid_out ? 0 : factor_bytes(z, z.K), bt = laid_out ? 0 : factor_bytes(z, z.N);
   if (w.B) kept.t = at::empty({z.M, z.P}, x.options().dtype(at::kFloat).requires_grad(false));
   if (!laid_out && w.x) kept.a_up = order(z, z.K, x);
   if (!laid_out && (w.x || w.A)) kept.b_down = order(z, z.N, x);
-  const Tensor scratch = bytes(parts + at + bt, x);
+  const Tensor scratch = parts + at + bt ? bytes(parts + at + bt, x) : Tensor();
   uint8_t* const s = data<uint8_t>(scratch);
   Factors f{A.const_data_ptr(), B.const_data_ptr()};
   if (!laid_out) {
@@ -146,11 +154,11 @@ struct Adapt : torch::autograd::Function<Adapt> {
       if (want_x) out[0] = at::empty({z.M, z.K}, opt);
       if (want_A) out[3] = at::empty({z.slots, z.K, z.R}, opt);
       if (want_B) out[4] = at::empty({z.slots, z.R, z.N}, opt);
-      const bool need_dt = want_x || want_A;
-      const int64_t joined = want_A ? up(4 * z.M * z.P) : 0, parts = joined + (need_dt ? parts_bytes(z, z.N) : 0);
+      const bool need_dt = want_x || want_A, few = few_rows(z, z.N, z.K);
+      const int64_t joined = want_A ? up(4 * z.M * z.P) : 0, parts = joined + (need_dt && !few ? parts_bytes(z, z.N) : 0);
       const int64_t ap = need_dt && laid_out ? factor_bytes(z, z.K) : 0, bp = need_dt && laid_out ? factor_bytes(z, z.N) : 0;
       const int64_t ws = want_A || want_B ? pq_adapter_grads_workspace_size(z.M, z.K, z.N, z.slots, z.P, z.each) : 0;
-      const Tensor scratch = bytes(parts + ap + bp + ws, dy);
+      const Tensor scratch = parts + ap + bp + ws ? bytes(parts + ap + bp + ws, dy) : Tensor();
       uint8_t* const s = data<uint8_t>(scratch);
       float* const dt = want_A ? reinterpret_cast<float*>(s) : nullptr;   // with its scale
       float* const dt_parts = reinterpret_cast<float*>(s + joined);
@@ -162,11 +170,17 @@ struct Adapt : torch::autograd::Function<Adapt> {
                                    want_x ? s + parts : nullptr, s + parts + ap, nullptr, stream),
                 "adapters");
         }
-        check(pq_adapter_down(dy.const_data_ptr(), code, z.M, z.N, stride_of(dy), f, z.slots, z.P, ids.const_data_ptr(), z.id_bits, z.each, dt_parts, stream),
-              "adapters' dt");
-        check(pq_adapter_up(dt_parts, pq_adapter_slices(z.M, z.N), data<float>(scale), g, z.slots, z.K, z.R, z.P, ids.const_data_ptr(), z.id_bits,
-                            z.each, nullptr, 0, data<void>(out[0]), z.K, dt, code, z.M, stream),
-              "adapters' input gradient");
+        if (few) {
+          check(pq_adapter_rows(dy.const_data_ptr(), code, z.M, z.N, stride_of(dy), f, data<float>(scale), g, z.slots, z.K, z.R, z.P,
+                                ids.const_data_ptr(), z.id_bits, z.each, nullptr, 0, data<void>(out[0]), z.K, dt, stream),
+                "adapters' input gradient");
+        } else {
+          check(pq_adapter_down(dy.const_data_ptr(), code, z.M, z.N, stride_of(dy), f, z.slots, z.P, ids.const_data_ptr(), z.id_bits, z.each, dt_parts, stream),
+                "adapters' dt");
+          check(pq_adapter_up(dt_parts, pq_adapter_slices(z.M, z.N), data<float>(scale), g, z.slots, z.K, z.R, z.P, ids.const_data_ptr(), z.id_bits,
+                              z.each, nullptr, 0, data<void>(out[0]), z.K, dt, code, z.M, stream),
+                "adapters' input gradient");
+        }
       }
       if (want_A || want_B)
         check(pq_adapter_grads(x.defined() ? x.const_data_ptr() : nullptr, x.defined() ? stride_of(x) : z.K, dy.const_data_ptr(), stride_of(dy), code,

@@ -327,6 +327,7 @@ __device__ __forceinline__ double squares(const void* grad, int64_t n, int64_t c
     for (int e = 0; e < 8; ++e) s += (double)g[i][e] * (double)g[i][e];
   return s;
 }
+// (29.5 M bf16 gradients of 420 tensors a launch: 17 us, 3.4 TB/s; they come from memory, with the stores of what ran before them.)
 __global__ __launch_bounds__(256) void grad_squares_kernel(const StepArgs p, const Grads grads, double* out) {
   __shared__ double sums[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -362,6 +363,7 @@ __global__ __launch_bounds__(1024) void grad_join_kernel(const double* sums, int
 }
 
 // ---- states out and in -----------------------------------------------------------------------------------------------------
+// Bound by memory: 88.6 M values of 8-bit states to two bf16 tensors 85 us, 6.2 TB/s, their bytes in part from the caches.
 template <int DT, bool EIGHT>
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const StepArgs p, int64_t n, void* mean, void* root) {
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;

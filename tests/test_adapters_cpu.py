@@ -40,6 +40,21 @@ def test_down_and_up_refusals():
     assert up(out=ODD) == L.PQ_EALIGN and up(base=ODD) == L.PQ_EALIGN and up(ldo=68) == L.PQ_EALIGN and up(base=ctypes.c_void_p(512), ldb=68) == L.PQ_EALIGN
     assert up(M=0, part=None, out=None) == L.PQ_OK
 
+    def rows(x=P, ty=0, M=4, K=64, ldx=64, f=P, scale=P, g=P, slots=2, C=64, R=8, PP=16, ids=P, bits=32, each=1, base=P, ldb=64, out=P, ldo=64, joined=None):
+        return lib.pq_adapter_rows(x, ty, M, K, ldx, f, scale, g, slots, C, R, PP, ids, bits, each, base, ldb, out, ldo, joined, None)
+
+    far = ctypes.c_void_p(512)
+    assert rows(K=60) == L.PQ_ESHAPE and rows(C=60) == L.PQ_ESHAPE and rows(ldx=56) == L.PQ_ESHAPE and rows(ldo=56) == L.PQ_ESHAPE and rows(ldb=56) == L.PQ_ESHAPE
+    assert rows(M=-1) == L.PQ_ESHAPE and rows(M=(1 << 16) + 1) == L.PQ_ESHAPE and rows(R=17) == L.PQ_ESHAPE and rows(PP=8) == L.PQ_ESHAPE
+    assert rows(each=3) == L.PQ_ESHAPE and rows(slots=0) == L.PQ_ESHAPE and rows(ldb=72) == L.PQ_ESHAPE and rows(ty=2) == L.PQ_EDTYPE and rows(bits=8) == L.PQ_EDTYPE
+    assert all(rows(**{k: None}) == L.PQ_EINVAL for k in ("x", "f", "scale", "g", "ids")) and rows(out=None) == L.PQ_EINVAL
+    assert rows(out=None, joined=P) == L.PQ_EINVAL and rows(out=None, base=None) == L.PQ_EINVAL
+    assert all(rows(**{k: ODD}) == L.PQ_EALIGN for k in ("x", "f", "g", "base", "out", "joined"))
+    assert rows(ldx=68) == L.PQ_EALIGN and rows(base=far, ldb=68) == L.PQ_EALIGN and rows(base=far, ldo=68) == L.PQ_EALIGN
+    assert rows(M=0, x=None, out=None) == L.PQ_OK
+    fit = lib.pq_adapter_rows_fit
+    assert fit(1, 1280, 1280, 16, 1) and fit(154, 2048, 1280, 16, 77) and not fit(8192, 640, 640, 16, 1) and not fit(1, 1 << 20, 64, 16, 1) and not fit(1, 60, 64, 16, 1)
+
 
 def test_gradient_and_order_refusals():
     L, lib = _lib()

@@ -101,7 +101,7 @@ def _near(got, want, off, what):
 
 SIZES = [(1, 8, 8, 1, 1), (1, 1280, 1288, 4, 16), (2, 24, 40, 2, 3), (15, 64, 72, 3, 8), (17, 136, 16, 5, 17), (33, 320, 264, 2, 24),
          (63, 128, 520, 40, 32), (64, 256, 64, 3, 33), (65, 1288, 8, 2, 64), (127, 40, 1000, 6, 15), (300, 2048, 136, 4, 48), (1025, 96, 328, 7, 16),
-         (2051, 520, 808, 3, 32)]
+         (2051, 520, 808, 3, 32), (40, 2600, 72, 5, 64), (70, 72, 2600, 4, 64), (1, 10752, 16, 2, 8), (700, 136, 264, 9, 40)]
 
 
 @pytest.mark.parametrize("dtype", BOTH)
@@ -483,6 +483,19 @@ def test_kernels_write_what_they_say(cuda):
         up(dt, Sd, None, K, None, alone)
         whole(tj, dtj, alone)
         assert torch.equal(alone[1], dtj[1]) and bool((tj[1].view(M, P)[none] == 7).all()) and not tj[1].view(M, P)[~none][:, R:].any()
+        # both products in one launch
+        y1, dx1, t1, dt1, t2 = guarded(M * N, torch.bfloat16), guarded(M * K, torch.bfloat16), *(guarded(M * P, torch.float32) for _ in range(3))
+        one = lambda v, C, f, g, D, base, out, joined: _lib.check(L.pq_adapter_rows(   # noqa: E731
+            p(v), 0, M, C, C, p(f[1]), p(scale), p(g[1]), slots, D, R, P, p(i), 32, 1, p(base), D, p(out[1]) if out else None, D, p(joined[1]), stream), "rows")
+        one(x, K, ad, bu, N, y, y1, t1)
+        one(dy, N, bd, au, K, None, dx1, dt1)
+        one(x, K, ad, bu, N, None, None, t2)
+        whole(y1, dx1, t1, dt1, t2)
+        assert torch.equal(t1[1], t2[1]) and bool((t1[1].view(M, P)[none] == 7).all()) and not t1[1].view(M, P)[~none][:, R:].any()
+        want, off = _want(x, y, i, A, B, scale, dy)
+        _near(y1[1].view(M, N), want["y"], off["y"], "y")
+        _near(dx1[1].view(M, K), want["dx"], off["dx"], "dx")
+        assert torch.equal(y1[1].view(M, N)[none], y[none]) and not dx1[1].view(M, K)[none].any()
         room = L.pq_adapter_grads_workspace_size(M, K, N, slots, P, 1)
         ws = torch.full((room + 256,), 255, dtype=torch.uint8, device=cuda)
         _lib.check(L.pq_adapter_grads(p(x), K, p(dy), N, 0, p(tj[1]), p(dtj[1]), p(i), 32, 1, M, K, N, slots, R, P, p(dA[1]), p(dB[1]), p(ws), room,
