@@ -10,7 +10,8 @@ quantized once, styles or customers are tuned as small factors, and one batch se
 an id that names no adapter (-1) leaves its rows as they are. The kernels read ids, factors and scales when they run, so a
 captured graph follows what is written there.
 
-No request's results depend on the others of its batch. t = x lr_A is held in fp32 and taken to twice the factors' bits. Calls have first
+No request's results depend on what the others of its batch hold or choose (the number of rows chooses the kernels, and with them
+the last bit). t = x lr_A is held in fp32 and taken to twice the factors' bits. Calls have first
 derivatives of the reverse kind (a second one, or a forward-mode tangent, raises). Every kernel runs on the caller's
 current stream; nothing synchronises. CPU tensors raise AssertionError; a missing library raises at the first call.
 """
