@@ -506,7 +506,7 @@ int pq_adapter_up(const float* part, int64_t slices, const float* scale, const v
                   float* joined, int32_t dtype, int64_t M, hipStream_t stream);
 
 /* Both of the above in one launch, for a few rows: out = base + t g with t = scale[id] x f, f in PQ_ADAPTER_DOWN, g in PQ_ADAPTER_UP; base, out and
- * joined as there. Every column block sums t anew: pq_adapter_rows_fit says where that is the faster way. */
+ * joined as there, and out must not overlap x. Every column block sums t anew: pq_adapter_rows_fit says where that is the faster way. */
 int pq_adapter_rows_fit(int64_t M, int64_t K, int64_t C, int64_t P, int64_t each);
 int pq_adapter_rows(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ldx, const void* f, const float* scale, const void* g,
                     int64_t slots, int64_t C, int64_t R, int64_t P, const void* ids, int32_t id_bits, int64_t each, const void* base,
