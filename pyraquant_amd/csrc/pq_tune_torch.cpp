@@ -13,10 +13,13 @@
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/StreamGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <optional>
 
 #include "../../include/pyraquant_amd.h"
 
@@ -44,6 +47,8 @@ int32_t code_of(at::ScalarType t) {
   refuse(PyExc_ValueError, "unsupported dtype (expected bfloat16, float16 or float32)");
 }
 hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+c10::Stream current(at::Device d) { return c10::impl::VirtualGuardImpl(d.type()).getStream(d); }
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 template <typename T>
 T* data(const Tensor& t) { return t.defined() ? static_cast<T*>(const_cast<void*>(t.const_data_ptr())) : nullptr; }
 
@@ -53,6 +58,7 @@ class Plan {
     need(bits == 8 || bits == 32, "states have 8 or 32 bits (got " + std::to_string(bits) + ")");
     need(!params.empty(), "a parameter group without parameters");
     first_.push_back(0);
+    if (device_.is_cuda()) home_ = current(device_);
     for (const Tensor& p : params) {
       need(p.is_cuda(), "the optimizer runs on the GPU only (got a CPU tensor)");
       need(p.device() == params[0].device(), "a parameter group lies on one device");
@@ -67,6 +73,7 @@ class Plan {
     need(first_.back() < (1 << 30), "a parameter group holds at most 2^40 values");
     list();
     const c10::DeviceGuard guard(params[0].device());
+    const c10::StreamGuard stream(*home_);
     const auto opt = at::TensorOptions().device(params[0].device());
     m_ = at::zeros({n_}, opt.dtype(bits == 8 ? at::kByte : at::kFloat));
     v_ = at::zeros({n_}, m_.options());
@@ -119,12 +126,27 @@ class Plan {
     copies_.clear();
   }
 
-  std::pair<Tensor, Tensor> moments(at::ScalarType type) const {
+  // What is the plan's own is on the current stream until the work there is done, and in a captured graph for good: a list that such
+  // a graph reads stays.
+  void used() {
+    if (capturing()) {
+      captured_ = true;
+      return;
+    }
+    const c10::Stream now = current(device_);
+    if (now != *home_)
+      for (const Tensor* t : {&tensors_, &chunks_, &m_, &v_, &exps_, &steps_})
+        if (t->defined()) t->record_stream(now);
+  }
+  bool captured() const { return captured_; }
+
+  std::pair<Tensor, Tensor> moments(at::ScalarType type) {
     const int32_t code = code_of(type);
     const c10::DeviceGuard guard(m_.device());
     const Tensor m = at::empty({n_}, m_.options().dtype(type)), r = at::empty({n_}, m_.options().dtype(type));
     const pq_adamw_states s = c_states();
     check(pq_adamw_moments(&s, m.data_ptr(), r.data_ptr(), code, stream_of(m_)), "moments");
+    used();
     return {m, r};
   }
   void load(const Tensor& mean, const Tensor& root, int64_t steps) {
@@ -143,6 +165,7 @@ class Plan {
     const pq_adamw_states s = c_states();
     check(pq_adamw_load(&s, data<float>(a), data<float>(b), stream_of(m_)), "load_moments");
     steps_.fill_(steps);
+    used();
   }
 
   const Tensor& like() const { return m_; }
@@ -160,7 +183,7 @@ class Plan {
  private:
   // The list of tensors and chunks in device memory, from where the parameters lie now.
   void list() {
-    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+    if (capturing())
       refuse(PyExc_RuntimeError, "the optimizer's first step, and the first after its parameters moved, cannot be captured: take one before");
     std::vector<pq_adamw_tensor> t(params_.size());
     std::vector<int32_t> chunks((size_t)first_.back());
@@ -178,6 +201,8 @@ class Plan {
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i) need(spans[i].first >= spans[i - 1].second, "two parameters of a group share memory");
     const c10::DeviceGuard guard(params_[0].device());
+    const c10::StreamGuard stream(*home_);
+    if (captured_) kept_.insert(kept_.end(), {tensors_, chunks_});
     auto up = [&](const void* from, int64_t bytes) {
       Tensor host = at::empty({std::max<int64_t>(bytes, 1)}, at::TensorOptions().dtype(at::kByte));
       std::copy_n(static_cast<const uint8_t*>(from), bytes, data<uint8_t>(host));
@@ -187,7 +212,9 @@ class Plan {
     chunks_ = up(chunks.data(), (int64_t)(chunks.size() * sizeof(int32_t)));
   }
 
-  std::vector<Tensor> params_, copies_;
+  std::vector<Tensor> params_, copies_, kept_;
+  std::optional<c10::Stream> home_;   // where all that is the plan's own was allocated
+  bool captured_ = false;
   int bits_;
   at::Device device_;
   int64_t n_ = 0;
@@ -261,6 +288,7 @@ py::object step(const py::list& groups, double max_norm) {
     check(pq_adamw_step(&l, &s, &g.rates, data<double>(partials), n_partials, data<float>(norm),
                         stream_of(g.plan->like())),
           "AdamW");
+    g.plan->used();
     g.plan->changed();
   }
   return norm.defined() ? py::cast(norm) : py::object(py::none());
@@ -272,10 +300,11 @@ PYBIND11_MODULE(_tune, m) {
   py::class_<Plan>(m, "Plan")
       .def(py::init<const std::vector<Tensor>&, int>())
       .def("holds", &Plan::holds)
+      .def("captured", &Plan::captured)
       .def("states", &Plan::states)
       .def("of", &Plan::of)
       .def("offsets", &Plan::offsets)
-      .def("moments", [](const Plan& p, py::handle dtype) {
+      .def("moments", [](Plan& p, py::handle dtype) {
         if (!THPDtype_Check(dtype.ptr())) refuse(PyExc_TypeError, "moments(dtype)");
         return p.moments(reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type);
       })

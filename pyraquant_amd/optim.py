@@ -13,7 +13,9 @@ step and ``seed``, so that averages move by less than a step of the grid. Elsewh
 parameters in one place and, in a group, several devices are refused.
 
 ``lr`` may be a tensor of one fp32 value on the GPU, which the kernel reads: a captured step then follows it. Steps can be
-captured after the first one has been taken; the step counts live on the GPU, so replays go on counting.
+captured after the first one has been taken; the step counts live on the GPU, so replays go on counting. A graph goes on with the
+parameters, gradients and states that it was captured with: capture again where they are replaced (load_state_dict, parameters that
+moved), and keep the optimizer as long as its graphs.
 """
 from __future__ import annotations
 
@@ -40,6 +42,7 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm = max_norm
         self.grad_norm: Optional[torch.Tensor] = None
         self._plans = {}
+        self._in_graphs = []   # plans that were replaced and that captured graphs go on with
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, bits=bits, seed=seed))
 
     def add_param_group(self, group) -> None:
@@ -73,8 +76,12 @@ class AdamW(torch.optim.Optimizer):
                         for n in names:
                             new[n].copy_(old[n].reshape(new[n].shape))
                 self.state[p] = new
+            self._drop(i)
             self._plans[i] = plan
         return plan
+
+    def _drop(self, *groups: int) -> None:
+        self._in_graphs += [plan for plan in (self._plans.pop(i, None) for i in groups) if plan is not None and plan.captured()]
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -112,7 +119,7 @@ class AdamW(torch.optim.Optimizer):
         super().load_state_dict({**state_dict, "state": {}})   # (torch casts states to the parameters' types)
         params = [p for g in self.param_groups for p in g["params"]]
         self.state.clear()
-        self._plans.clear()
+        self._drop(*list(self._plans))
         for i, p in zip(ids, params):
             if i in state_dict["state"]:
                 self.state[p] = {k: v.detach().clone() for k, v in state_dict["state"][i].items()}
@@ -123,4 +130,7 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
         self.__dict__.setdefault("max_norm", None)
-        self.grad_norm, self._plans = None, {}
+        self.grad_norm = None
+        self.__dict__.setdefault("_plans", {})
+        self.__dict__.setdefault("_in_graphs", [])
+        self._drop(*list(self._plans))

@@ -452,6 +452,39 @@ def test_captured_steps(cuda, bits):
             fresh.step()
 
 
+@pytest.mark.parametrize("bits", (32, 8))
+def test_captured_steps_keep_what_they_read(cuda, bits):
+    """A graph goes on with the parameters and states that it was captured with: where the parameters have moved, and where a state dict was
+    loaded, the memory of its list and its states is nobody else's."""
+    params = _params([(640, 16), (1001,), (77, 3)], torch.float32)
+    opt = _opt(params, bits=bits)
+    _grads(params, 0)
+    grads, old = [p.grad for p in params], [p.data for p in params]
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+
+    def replay():
+        junk = [torch.full((n,), 0x7f, dtype=torch.uint8, device=cuda) for n in (64, 128, 512, 2048, 16384, 1 << 20) for _ in range(40)]
+        before = [t.clone() for t in old], [p.detach().clone() for p in params], [t.clone() for t in opt.states()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(not torch.equal(a, b) and bool(a.isfinite().all()) for a, b in zip(old, before[0]))
+        assert all(torch.equal(a, b) for a, b in zip(params, before[1]))
+        assert all(bool((t == 0x7f).all()) for t in junk)
+        return all(torch.equal(a, b) for a, b in zip(opt.states(), before[2]))
+
+    for p, g in zip(params, grads):
+        p.data = p.data.clone()
+        p.grad = g
+    opt.step()
+    assert not replay()                    # (the same states)
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    opt.step()
+    assert replay() and replay()           # (the states that the graph was captured with)
+
+
 def test_other_streams(cuda):
     params = _params([(640, 64)], torch.float32)
     same = copy.deepcopy(params)
