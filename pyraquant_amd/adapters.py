@@ -12,7 +12,8 @@ captured graph follows what is written there.
 
 No request's results depend on what the others of its batch hold or choose (the number of rows chooses the kernels, and with them
 the last bit). t = x lr_A is held in fp32 and taken to twice the factors' bits. Calls have first
-derivatives of the reverse kind (a second one, or a forward-mode tangent, raises). Every kernel runs on the caller's
+derivatives of the reverse kind (a second one, or a forward-mode tangent, raises; so does a step that is captured while an eager graph of
+its leaves lives). Every kernel runs on the caller's
 current stream; nothing synchronises. CPU tensors raise AssertionError; a missing library raises at the first call.
 """
 from __future__ import annotations

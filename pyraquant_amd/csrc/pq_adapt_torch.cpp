@@ -9,9 +9,12 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -231,6 +234,23 @@ bool meet(const Tensor& a, const Tensor& b) {
   return s.first < t.second && t.first < s.second;
 }
 
+// Whether the gradient of t's leaf (t, or what t is a view or a cast of) would be accumulated on another stream than the current one: a graph that
+// was made there lives.
+bool elsewhere(const Tensor& t) {
+  if (!t.defined() || !t.requires_grad()) return false;
+  std::shared_ptr<torch::autograd::Node> node = t.grad_fn();
+  if (!node) node = torch::autograd::impl::try_get_grad_accumulator(t);
+  for (int i = 0; i < 8 && node; ++i) {
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) {
+      const std::optional<c10::Stream> at = node->stream();
+      return at && *at != c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device());
+    }
+    if (node->num_outputs() != 1) return false;
+    node = node->next_edge(0).function;
+  }
+  return false;
+}
+
 // What the kernels need, as AssertionError.
 const char* wrong(const Tensor& x, const Tensor& y, const Tensor& ids, const Tensor& A, const Tensor& B, const Tensor& scale, int64_t R,
                   bool laid_out, const Tensor& out) {
@@ -309,6 +329,12 @@ PyObject* adapt(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     refused = "out is for calls without gradients";
   if (refused) {
     PyErr_SetString(PyExc_AssertionError, refused);
+    return nullptr;
+  }
+  // A captured backward pass would wait for that stream, which is not captured, in autograd's own thread: the process would end there.
+  if (any && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None &&
+      (elsewhere(x) || elsewhere(y) || elsewhere(A) || elsewhere(B))) {
+    PyErr_SetString(PyExc_RuntimeError, "a graph of the same leaves that was made outside the capture lives: drop its results before a step is captured");
     return nullptr;
   }
   Tensor result;

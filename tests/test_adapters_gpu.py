@@ -401,6 +401,41 @@ def test_same_bits_streams_and_graphs(cuda):
         assert all(torch.equal(a, b) for a, b in zip(graphs[1][1], both(tuned, ids.clone())))
 
 
+def test_captured_training_step(cuda):
+    """A backward pass that accumulates, captured: replays add the same gradients; one that would meet an eager graph of the same leaves is
+    refused before anything runs, through views and casts of them too."""
+    n, each, K, N, slots, R = 3, 50, 136, 72, 4, 8
+    x, y, _, A, B, scale = _problem(n * each, K, N, slots, R, torch.bfloat16, "runs", seed=5)
+    ids = torch.tensor([2, -1, 0], device=cuda)
+    dy = torch.randn(n, each, N, device=cuda).bfloat16()
+    for dtype in (torch.bfloat16, torch.float32):
+        tuned = _bank(A.to(dtype), B.to(dtype), scale, trainable=True)
+        leaves = [x.clone().requires_grad_(), tuned.lr_A, tuned.lr_B]
+
+        def step():
+            tuned(leaves[0].view(n, each, K), y.view(n, each, N), ids).backward(dy)
+
+        step()
+        want = [v.grad.clone() for v in leaves]
+        kept = tuned(leaves[0].view(n, each, K), y.view(n, each, N), ids)
+        with pytest.raises(RuntimeError, match="outside the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                step()
+        del kept
+        for v in leaves:
+            v.grad.zero_()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        for k in range(3):
+            for v in leaves:
+                v.grad.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(v.grad, w) for v, w in zip(leaves, want))
+            _bank(A, B, scale)(x, y, ids.repeat_interleave(each))      # (eager work between)
+
+
 def test_places_past_32_bits(cuda):
     """Rows beyond 2^31 values of y, then of x: the last rows answer as alone, forward and back, and the others too by their sums."""
     M, slots, R = 270000, 2, 8
