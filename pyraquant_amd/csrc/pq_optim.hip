@@ -239,8 +239,10 @@ __device__ __forceinline__ void step_chunk(const StepArgs& p, void* param, const
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float d = g[i][e] * clip;
-      m[i][e] = fmaf(d, p.b1c, m[i][e] * p.b1);
-      v[i][e] = fmaf(d * d, p.b2c, v[i][e] * p.b2);
+      // b m as m - (1 - b) m in one rounding: b in fp32 is off by as much as half a step itself, and what is cut to 8 bits next falls to the
+      // other side of a grid step as often as m is off (an infinity there is NaN either way; in 32-bit states it stays one).
+      m[i][e] = fmaf(d, p.b1c, EIGHT ? fmaf(m[i][e], -p.b1c, m[i][e]) : m[i][e] * p.b1);
+      v[i][e] = fmaf(d * d, p.b2c, EIGHT ? fmaf(v[i][e], -p.b2c, v[i][e]) : v[i][e] * p.b2);
       least = min(least, __float_as_uint(v[i][e]) - 1);
     }
     // The instructions for roots and reciprocals are within 1 of the last place, but take subnormal numbers for zeros: where a square is
