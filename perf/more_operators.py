@@ -176,9 +176,6 @@ def prepare(case, seed):
         for i, scale in enumerate(s.pop("scale").tolist()):
             bank.set(i, t["lr_A"][i], t["lr_B"][i], scale)
         s["bank"] = bank
-        if case["each"]:      # a batch of requests of one length, with an id for each
-            for k in {"x", "y", "dy"} & set(s):
-                s[k] = s[k].view(-1, case["each"], s[k].shape[1])
         if case["kind"] == "tune":
             s["x"].requires_grad_()
     return s
@@ -273,11 +270,11 @@ def run(state):
     bank = state["bank"]
     if state["kind"] == "serve":
         with torch.no_grad():
-            return bank(state["x"], state["y"], state["ids"]).flatten(0, -2)
+            return bank(state["x"], state["y"], state["ids"])
     x = state["x"]
     y = bank(x, state["y"], state["ids"])
-    dx, dA, dB = torch.autograd.grad(y, [x, bank.lr_A, bank.lr_B], state["dy"])
-    return {"y": y.detach().flatten(0, -2), "dx": dx.flatten(0, -2), "dlr_A": dA, "dlr_B": dB}
+    grads = torch.autograd.grad(y, [x, bank.lr_A, bank.lr_B], state["dy"])
+    return dict(zip(("y", "dx", "dlr_A", "dlr_B"), (y.detach(), *grads)))
 
 
 def work(case):
