@@ -6,7 +6,8 @@
 
 The layers of int8_exec and mxfp4 hold one low-rank branch that belongs to the weight. Adapters belong to requests: a model is
 quantized once, styles or customers are tuned as small factors, and one batch serves any of them together, or tunes them together.
-``ids`` is an integer tensor on the GPU, one for each row or for each of x's leading dimensions (a batch of images: one an image);
+``ids`` is an integer tensor on the GPU, one for each row or for each of x's leading dimensions (a batch of images: one an image), or, where
+LowRankAdapters is called with flat rows, one for each request of M / len(ids) rows that follow each other;
 an id that names no adapter (-1) leaves its rows as they are. The kernels read ids, factors and scales when they run, so a
 captured graph follows what is written there.
 
@@ -252,6 +253,7 @@ class AdaptedLinear(nn.Module):
         ids = self._chosen.ids
         if ids is None:
             return y
+        assert x.dim() != 2 or ids.dim() != 1 or ids.shape[0] == x.shape[0], f"{x.shape[0]} rows and ids of {ids.shape[0]}: a layer's rows are the batch's"
         # (the layer's result is a new tensor: without gradients what is added goes into it)
         return self.adapters(x, y, ids, out=None if torch.is_grad_enabled() or not y.is_contiguous() else y)
 

@@ -271,8 +271,12 @@ const char* wrong(const Tensor& x, const Tensor& y, const Tensor& ids, const Ten
     return "lr_A and lr_B do not fit x and y";
   if (scale.scalar_type() != at::kFloat || scale.dim() != 1 || scale.size(0) != slots || !scale.is_contiguous()) return "scale is contiguous fp32 [slots]";
   if (ids.dim() > x.dim() - 1) return "ids have some of x's leading dimensions";
-  for (int64_t d = 0; d < ids.dim(); ++d)
-    if (ids.size(d) != x.size(d)) return "ids have some of x's leading dimensions";
+  if (x.dim() == 2 && ids.dim() == 1) {   // rows, or requests of equally many rows end to end
+    if (ids.size(0) != x.size(0) && (!ids.size(0) || !x.size(0) || x.size(0) % ids.size(0))) return "ids are one for each row, or for each request of as many rows";
+  } else {
+    for (int64_t d = 0; d < ids.dim(); ++d)
+      if (ids.size(d) != x.size(d)) return "ids have some of x's leading dimensions";
+  }
   if (out.defined()) {
     if (out.sizes() != y.sizes()) return "out has another shape than y";
     if (out.dim() > 1 && !out.is_contiguous()) return "out must be contiguous";
