@@ -98,7 +98,8 @@ class Plan {
     bool moved = false;
     for (size_t i = 0; i < params_.size(); ++i) {
       const Tensor& p = params_[i];
-      moved |= p.const_data_ptr() != at_[i];
+      moved |= p.const_data_ptr() != at_[i] || p.numel() != sizes_[i] || p.scalar_type() != types_[i] || p.device() != device_ ||
+               !p.is_non_overlapping_and_dense();
       const Tensor& g = p.grad();
       if (!g.defined()) continue;
       if (g.layout() != at::kStrided) refuse(PyExc_RuntimeError, "sparse gradients are not supported");
@@ -181,7 +182,7 @@ class Plan {
   const std::vector<int64_t>& offsets() const { return offsets_; }
 
  private:
-  // The list of tensors and chunks in device memory, from where the parameters lie now.
+  // The list of tensors and chunks in device memory, from where the parameters lie now and what they are.
   void list() {
     if (capturing())
       refuse(PyExc_RuntimeError, "the optimizer's first step, and the first after its parameters moved, cannot be captured: take one before");
@@ -189,11 +190,13 @@ class Plan {
     std::vector<int32_t> chunks((size_t)first_.back());
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
     at_.resize(params_.size());
+    types_.resize(params_.size());
     for (size_t i = 0; i < params_.size(); ++i) {
       const Tensor& p = params_[i];
       need(p.numel() == sizes_[i] && p.is_non_overlapping_and_dense(), "a parameter has changed its size, or is not dense any more");
       need(p.device() == device_, "a parameter has left the device that its states are on");
       at_[i] = p.const_data_ptr();
+      types_[i] = p.scalar_type();
       t[i] = {const_cast<void*>(at_[i]), sizes_[i], offsets_[i], code_of(p.scalar_type()), (int32_t)first_[i]};
       std::fill(chunks.begin() + first_[i], chunks.begin() + first_[i + 1], (int32_t)i);
       if (sizes_[i]) spans.emplace_back((uintptr_t)at_[i], (uintptr_t)at_[i] + p.numel() * p.element_size());
@@ -220,6 +223,7 @@ class Plan {
   int64_t n_ = 0;
   std::vector<int64_t> offsets_, sizes_, first_;
   std::vector<const void*> at_, grads_;
+  std::vector<at::ScalarType> types_;
   Tensor tensors_, chunks_, m_, v_, exps_, steps_;
 };
 

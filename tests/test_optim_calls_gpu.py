@@ -1,0 +1,52 @@
+"""Calls that AdamW answers or refuses beside those of test_optim_gpu.py, whose bounds these use."""
+import copy
+import gc
+
+import pytest
+import torch
+
+from test_optim_gpu import TYPES, _before, _check_step, _grads, _opt, _params
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+def test_parameters_that_change_where_they_lie(cuda, bits):
+    """A parameter that is shorter, longer, has gaps, or another type than its states' at the same address as before."""
+    room = torch.full((4000,), 3.0, device=cuda)
+    p = torch.nn.Parameter(room[:1000])
+    opt = _opt([p], bits=bits)
+    _grads([p], 0)
+    opt.step()
+    was, state = room.clone(), [t.clone() for t in opt.states()]
+    for view, why in ((room[:4], "size"), (room[:2000], "size"), (room[:2000:2], "dense"), (room[:0], "size")):
+        p.grad = None
+        p.data = view
+        assert p.data_ptr() == room.data_ptr() or not p.numel()
+        with pytest.raises(AssertionError, match=why):
+            opt.step()
+        p.grad = torch.ones_like(p)
+        with pytest.raises(AssertionError, match=why):
+            opt.step()
+        assert torch.equal(room, was) and all(torch.equal(a, b) for a, b in zip(opt.states(), state))
+    p.grad = None
+    p.data = room[:1000]
+    _grads([p], 1)
+    before = _before(opt)
+    opt.step()
+    _check_step(opt, before, 2)
+    half = torch.nn.Parameter(torch.randn(1000, device=cuda).bfloat16())
+    opt = _opt([half], bits=bits)
+    _grads([half], 0)
+    opt.step()
+    at = half.data_ptr()
+    half.data, half.grad = half.data.view(torch.float16), None      # (the same bits as values of another type)
+    half.data.copy_(torch.randn(1000, device=cuda))
+    assert half.data_ptr() == at and half.dtype == torch.float16
+    _grads([half], 1)
+    before = _before(opt)
+    opt.step()
+    _check_step(opt, before, 2)
+    half.data, half.grad = half.data.double(), None
+    with pytest.raises(ValueError, match="dtype"):
+        opt.step()
