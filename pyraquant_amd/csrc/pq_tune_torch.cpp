@@ -182,37 +182,39 @@ class Plan {
   const std::vector<int64_t>& offsets() const { return offsets_; }
 
  private:
-  // The list of tensors and chunks in device memory, from where the parameters lie now and what they are.
+  // The list of tensors and chunks in device memory, from where the parameters lie now and what they are. (at_ and types_ are those of the
+  // list: they change with it, or where anything is refused neither does.)
   void list() {
     if (capturing())
       refuse(PyExc_RuntimeError, "the optimizer's first step, and the first after its parameters moved, cannot be captured: take one before");
     std::vector<pq_adamw_tensor> t(params_.size());
     std::vector<int32_t> chunks((size_t)first_.back());
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-    at_.resize(params_.size());
-    types_.resize(params_.size());
+    std::vector<const void*> places(params_.size());
+    std::vector<at::ScalarType> types(params_.size());
     for (size_t i = 0; i < params_.size(); ++i) {
       const Tensor& p = params_[i];
       need(p.numel() == sizes_[i] && p.is_non_overlapping_and_dense(), "a parameter has changed its size, or is not dense any more");
       need(p.device() == device_, "a parameter has left the device that its states are on");
-      at_[i] = p.const_data_ptr();
-      types_[i] = p.scalar_type();
-      t[i] = {const_cast<void*>(at_[i]), sizes_[i], offsets_[i], code_of(p.scalar_type()), (int32_t)first_[i]};
+      places[i] = p.const_data_ptr();
+      types[i] = p.scalar_type();
+      t[i] = {const_cast<void*>(places[i]), sizes_[i], offsets_[i], code_of(types[i]), (int32_t)first_[i]};
       std::fill(chunks.begin() + first_[i], chunks.begin() + first_[i + 1], (int32_t)i);
-      if (sizes_[i]) spans.emplace_back((uintptr_t)at_[i], (uintptr_t)at_[i] + p.numel() * p.element_size());
+      if (sizes_[i]) spans.emplace_back((uintptr_t)places[i], (uintptr_t)places[i] + p.numel() * p.element_size());
     }
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i) need(spans[i].first >= spans[i - 1].second, "two parameters of a group share memory");
     const c10::DeviceGuard guard(params_[0].device());
     const c10::StreamGuard stream(*home_);
-    if (captured_) kept_.insert(kept_.end(), {tensors_, chunks_});
     auto up = [&](const void* from, int64_t bytes) {
       Tensor host = at::empty({std::max<int64_t>(bytes, 1)}, at::TensorOptions().dtype(at::kByte));
       std::copy_n(static_cast<const uint8_t*>(from), bytes, data<uint8_t>(host));
       return host.to(params_[0].device());   // (waits: the host's copy goes away)
     };
-    tensors_ = up(t.data(), (int64_t)(t.size() * sizeof(pq_adamw_tensor)));
-    chunks_ = up(chunks.data(), (int64_t)(chunks.size() * sizeof(int32_t)));
+    const Tensor tensors = up(t.data(), (int64_t)(t.size() * sizeof(pq_adamw_tensor)));
+    const Tensor its_chunks = up(chunks.data(), (int64_t)(chunks.size() * sizeof(int32_t)));
+    if (captured_) kept_.insert(kept_.end(), {tensors_, chunks_});
+    tensors_ = tensors, chunks_ = its_chunks, at_ = std::move(places), types_ = std::move(types);
   }
 
   std::vector<Tensor> params_, copies_, kept_;

@@ -50,3 +50,31 @@ def test_parameters_that_change_where_they_lie(cuda, bits):
     half.data, half.grad = half.data.double(), None
     with pytest.raises(ValueError, match="dtype"):
         opt.step()
+
+
+def test_a_step_that_was_refused(cuda):
+    """What a refused step has seen of parameters that moved counts for nothing: the next one is refused too, or finds all of them."""
+    a, b = _params([(1000,), (500,)], torch.float32)
+    opt = _opt([a, b])
+    _grads([a, b], 0)
+    opt.step()
+    old, room = a.data, b.data
+    was = old.clone()
+    a.data = old.clone()
+    b.grad, b.data = None, room[:100]
+    for _ in range(2):
+        with pytest.raises(AssertionError, match="size"):
+            opt.step()
+    b.data = room
+    _grads([a, b], 1)
+    before = _before(opt)
+    opt.step()
+    _check_step(opt, before, 2)
+    assert torch.equal(old, was) and not torch.equal(a, was)
+    both = torch.zeros(1200, device=cuda)
+    a.data, b.data = both[:1000], both[700:]
+    _grads([a, b], 2)
+    for _ in range(2):
+        with pytest.raises(AssertionError, match="share memory"):
+            opt.step()
+    assert not both.any()
