@@ -279,7 +279,7 @@ const char* wrong(const Tensor& x, const Tensor& y, const Tensor& ids, const Ten
   }
   if (out.defined()) {
     if (out.sizes() != y.sizes()) return "out has another shape than y";
-    if (out.dim() > 1 && !out.is_contiguous()) return "out must be contiguous";
+    if (!out.is_contiguous()) return "out must be contiguous";
     if ((uintptr_t)out.const_data_ptr() % 16) return "out must be 16-byte aligned";
     const bool same = out.const_data_ptr() == y.const_data_ptr() && y.is_contiguous() && !y.is_neg();
     if (out.is_neg() || meet(out, x) || (meet(out, y) && !same) || meet(out, A) || meet(out, B) || meet(out, ids) || meet(out, scale))

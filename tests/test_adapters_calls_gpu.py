@@ -57,3 +57,19 @@ def test_layers_take_no_ids_of_flat_rows(cuda):
         assert net(torch.zeros(2, 64, device=cuda, dtype=torch.bfloat16)).shape == (2, 40)
         with pytest.raises(AssertionError):
             net(torch.zeros(6, 64, device=cuda, dtype=torch.bfloat16))
+
+
+def test_one_row_into_out(cuda):
+    """A result of one dimension goes into memory whose values follow each other, and into no other."""
+    x, y, _, A, B, scale = _problem(1, 64, 40, 3, 8, torch.bfloat16, "one")
+    bank, i = _bank(A, B, scale), torch.tensor(1, device=cuda)
+    room = torch.full((160,), 7.0, dtype=torch.bfloat16, device=cuda)
+    with torch.no_grad():
+        want = bank(x[0], y[0], i)
+        assert bank(x[0], y[0], i, out=room[40:80]) is not None and torch.equal(room[40:80], want)
+        assert bool((room[:40] == 7).all()) and bool((room[80:] == 7).all())
+        room.fill_(7)
+        for out in (room[:80:2], room[:1].expand(40), room.view(40, 4)[:, 1], room[1:41]):
+            with pytest.raises(AssertionError, match="contiguous|aligned"):
+                bank(x[0], y[0], i, out=out)
+        assert bool((room == 7).all())
