@@ -128,10 +128,16 @@ class Plan {
   }
 
   // What is the plan's own is on the current stream until the work there is done, and in a captured graph for good: a list that such
-  // a graph reads stays.
-  void used() {
+  // a graph reads stays, with the memory of the parameters that it names and of the rate.
+  void used(const Tensor& rate = Tensor()) {
     if (capturing()) {
       captured_ = true;
+      auto hold = [&](const Tensor& t) {
+        if (held_.empty() || held_.back().unsafeGetStorageImpl() != t.storage().unsafeGetStorageImpl()) held_.push_back(t.storage());
+      };
+      if (!holds_params_) std::for_each(params_.begin(), params_.end(), hold);
+      holds_params_ = true;
+      if (rate.defined()) hold(rate);
       return;
     }
     const c10::Stream now = current(device_);
@@ -214,12 +220,14 @@ class Plan {
     const Tensor tensors = up(t.data(), (int64_t)(t.size() * sizeof(pq_adamw_tensor)));
     const Tensor its_chunks = up(chunks.data(), (int64_t)(chunks.size() * sizeof(int32_t)));
     if (captured_) kept_.insert(kept_.end(), {tensors_, chunks_});
+    holds_params_ = false;
     tensors_ = tensors, chunks_ = its_chunks, at_ = std::move(places), types_ = std::move(types);
   }
 
   std::vector<Tensor> params_, copies_, kept_;
+  std::vector<c10::Storage> held_;    // what graphs go on with beside kept_
   std::optional<c10::Stream> home_;   // where all that is the plan's own was allocated
-  bool captured_ = false;
+  bool captured_ = false, holds_params_ = false;   // (the parameters of this list)
   int bits_;
   at::Device device_;
   int64_t n_ = 0;
@@ -234,15 +242,16 @@ py::object step(const py::list& groups, double max_norm) {
   struct Group {
     Plan* plan;
     pq_adamw_rates rates;
+    Tensor rate;   // in device memory, or none
   };
   std::vector<Group> all;
   for (const py::handle h : groups) {
     const py::tuple t = py::reinterpret_borrow<py::tuple>(h);
-    Group g{t[0].cast<Plan*>(), {}};
+    Group g{t[0].cast<Plan*>(), {}, {}};
     if (THPVariable_Check(t[1].ptr())) {
       const Tensor lr = THPVariable_Unpack(t[1].ptr());
       need(lr.numel() == 1, "lr is one number");
-      if (lr.is_cuda() && lr.scalar_type() == at::kFloat && lr.device() == g.plan->like().device()) g.rates.lr_at = data<float>(lr);
+      if (lr.is_cuda() && lr.scalar_type() == at::kFloat && lr.device() == g.plan->like().device()) g.rate = lr, g.rates.lr_at = data<float>(lr);
       else g.rates.lr = lr.item().toDouble();
     } else {
       g.rates.lr = t[1].cast<double>();
@@ -294,7 +303,7 @@ py::object step(const py::list& groups, double max_norm) {
     check(pq_adamw_step(&l, &s, &g.rates, data<double>(partials), n_partials, data<float>(norm),
                         stream_of(g.plan->like())),
           "AdamW");
-    g.plan->used();
+    g.plan->used(g.rate);
     g.plan->changed();
   }
   return norm.defined() ? py::cast(norm) : py::object(py::none());

@@ -14,8 +14,8 @@ parameters in one place and, in a group, several devices are refused.
 
 ``lr`` may be a tensor of one fp32 value on the GPU, which the kernel reads: a captured step then follows it. Steps can be
 captured after the first one has been taken; the step counts live on the GPU, so replays go on counting. A graph goes on with the
-parameters, gradients and states that it was captured with: capture again where they are replaced (load_state_dict, parameters that
-moved), and keep the optimizer as long as its graphs.
+rate, parameters, gradients and states that it was captured with: capture again where they are replaced (load_state_dict, parameters that
+moved), and keep the optimizer, which holds them, as long as its graphs. Gradients that were not made in the capture are the caller's to keep.
 """
 from __future__ import annotations
 

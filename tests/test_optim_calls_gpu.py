@@ -78,3 +78,31 @@ def test_a_step_that_was_refused(cuda):
         with pytest.raises(AssertionError, match="share memory"):
             opt.step()
     assert not both.any()
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+def test_captured_steps_keep_rates_and_parameters(cuda, bits):
+    """The rate and the parameters' memory that a captured step goes on with are the optimizer's, where nobody else holds them any more."""
+    params = _params([(640, 16), (1001,)], torch.float32)
+    opt = _opt(params, bits=bits, lr=torch.full((4096,), 1e-3, device=cuda)[0], weight_decay=0.0)
+    _grads(params, 0)
+    grads = [p.grad for p in params]
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    places = [(p.data_ptr(), p.numel() * 4) for p in params] + [(opt.param_groups[0]["lr"].data_ptr(), 4)]
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))             # (the group's rate is another tensor now)
+    for p, g in zip(params, grads):
+        p.data = p.data.clone()
+        p.grad = g
+    opt.step()
+    gc.collect()
+    junk = [torch.full((n,), 0x7f, dtype=torch.uint8, device=cuda) for n in (4, 512, 4004, 4096, 16384, 40960, 65536) for _ in range(60)]
+    for at, n in places:
+        assert all(t.data_ptr() + t.numel() <= at or at + n <= t.data_ptr() for t in junk)
+    now = [p.detach().clone() for p in params]
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(params, now)) and all(bool((t == 0x7f).all()) for t in junk)
