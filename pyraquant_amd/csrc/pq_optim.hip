@@ -168,7 +168,7 @@ struct Moments8 {
       add(2 * i, um[0], ur[0]);
       add(2 * i + 1, um[1], ur[1]);
       rm[i] = rounded2<3>(__float_as_uint(mean[2 * i]) & 0x7fffffffu, um[0], __float_as_uint(mean[2 * i + 1]) & 0x7fffffffu, um[1]);
-      rr[i] = rounded2<4>(__float_as_uint(roots[2 * i]), ur[0], __float_as_uint(roots[2 * i + 1]), ur[1]);
+      rr[i] = rounded2<4>(__float_as_uint(roots[2 * i]) & 0x7fffffffu, ur[0], __float_as_uint(roots[2 * i + 1]) & 0x7fffffffu, ur[1]);   // (a NaN may have a sign)
       tm = __builtin_elementwise_max(tm, rm[i]);
       tr = __builtin_elementwise_max(tr, rr[i]);
     }

@@ -106,3 +106,21 @@ def test_captured_steps_keep_rates_and_parameters(cuda, bits):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(params, now)) and all(bool((t == 0x7f).all()) for t in junk)
+
+
+@pytest.mark.parametrize("nan", (0x7fc00000, -0x400000, 0x7fffffff, -1, -0x7fffff))      # (with the sign bit: from -0x7fffff to -1)
+def test_blocks_with_any_nan_are_nan(cuda, nan):
+    p = torch.nn.Parameter(torch.ones(128 * 3, device=cuda))
+    opt = _opt([p], bits=8)
+    g = torch.ones(3, 128, device=cuda)
+    g.view(torch.int32)[1, 7] = nan
+    assert bool(g[1, 7].isnan())
+    p.grad = g.view(-1)
+    opt.step()
+    for t in opt.moments():
+        t = t.view(3, 128)
+        assert bool(t[1].isnan().all()) and bool(t[0].isfinite().all()) and bool(t[2].isfinite().all())
+    assert int(p.detach().isnan().sum()) == 1
+    opt.step()
+    for t in opt.moments():
+        assert bool(t.view(3, 128)[1].isnan().all())
