@@ -10,8 +10,9 @@
 //                                                                                    they are read)
 //   up    out[m, c] = base[m, c] + scale[id] sum_r part[m, r] g[id][c, r], and scale[id] part[m], the slices added, for `sums`
 //   sums  the two sums over rows, per adapter, over chunks of the rows, added by `join` in their order
-// All sums are fp32. t and dt are taken by the 16-bit matrix instructions in two parts (two_parts), so their rounding shows in no
-// result. No atomics: the same bits every time. Bound by memory: 2 R operations for each value that is read.
+// All sums are fp32. t and dt are taken by the 16-bit matrix instructions in two parts (two_parts), in fp16 on a scale of each row's (`up`) or of each
+// rank's in 64 rows (`sums`), so that their rounding shows in no result, however small they are (the scales of `sums` cost a step of tuning 16384 x
+// 1280 x 5120 with rank 32 205 -> 208 us). No atomics: the same bits every time. Bound by memory: 2 R operations for each value that is read.
 #include "pq_mx.h"
 
 #include <algorithm>
@@ -270,19 +271,19 @@ __device__ __forceinline__ void up_pass(const UpArgs& p, int id, int row0, int l
         to[1] = piece[k].raw[1];
       }
     }
-    if constexpr (DT == PQ_F16) {   // rows past fp16's end are taken times a power of two
+    if constexpr (DT == PQ_F16) {   // a row on a scale of its own, that its largest value gives
       float m = piece[0].largest();
 #pragma unroll
       for (int k = 1; k < KS; ++k) m = fmaxf(m, piece[k].largest());
       m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
-      const float down = scale_down(__float_as_uint(m));
+      const int by = scale_exponent(m);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) back[s][i] = scale_back(__shfl(down, 4 * g + i));
+      for (int i = 0; i < 4; ++i) back[s][i] = power(__shfl(by, 4 * g + i));
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) piece[k].raw[e >> 2][e & 3] *= down;
+        for (int e = 0; e < 8; ++e) piece[k].raw[e >> 2][e & 3] *= power(-by);
     }
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
@@ -598,7 +599,7 @@ struct SumArgs {
 };
 
 template <int DT, int P>
-__device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int block, int which, uint8_t* sz, uint8_t* sv, uint32_t* top) {
+__device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int block, int which, uint8_t* sz, uint8_t* sv, float* top) {
   constexpr int TILES = P == 16 ? 1 : P / 32, PITCH = P == 16 ? 64 : P * 2;   // of v's tiles: with P 16, the first part in ranks 0-15, the second in 16-31
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunk = block / p.panels, panel = block - chunk * p.panels;
@@ -667,37 +668,13 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int b
   if (m0 >= end) return;
   load(m0);
   while (m0 < end) {
-    bool far = false;   // some value of v is 2^16 or more (fp16: scale_down); the waves tell each other in top[0 .. 3]
-    if constexpr (DT == PQ_F16) {
-      float m = 0.0f;
-#pragma unroll
-      for (int i = 0; i < P / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(vr[i][e]));
-      const bool any = __ballot(m >= 65536.0f) != 0;
-      if (lane == 0) top[wave] = any;
-    }
+    float back[TILES];   // fp16: the inverse of the scale on which the lane's ranks are taken in this step
+    if constexpr (DT == PQ_F16) tell_largest<P>(vr, top, tid);
     __syncthreads();
     if constexpr (DT == PQ_F16) {
-      const v4u all = *reinterpret_cast<const v4u*>(top);
-      far = __builtin_amdgcn_readfirstlane((int)(all[0] | all[1] | all[2] | all[3])) != 0;
-      if (far) {   // rare: the largest magnitude of each rank's 64 values, in top[4 ..]
-        if (tid < P) top[4 + tid] = 0;
-        __syncthreads();
+      scale_values<P>(vr, top, tid);
 #pragma unroll
-        for (int i = 0; i < P / 16; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) atomicMax(&top[4 + (i * 256 + tid) % (P / 4) * 4 + e], __float_as_uint(vr[i][e]) & 0x7fffffffu);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < P / 16; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vr[i][e] *= scale_down(top[4 + (i * 256 + tid) % (P / 4) * 4 + e]);
-#pragma unroll
-        for (int j = 0; j < TILES; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[j][e] *= scale_down(top[4 + rank(j)]);
-      }
+      for (int j = 0; j < TILES; ++j) back[j] = power(scale_exponent(largest_of<P>(top, rank(j))));
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) *reinterpret_cast<v4u*>(z_at(i * 16 + (tid >> 4), tid & 15)) = zr[i];
@@ -718,20 +695,23 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int b
     __syncthreads();
     const int m1 = next(m0 + 64);
     if (m1 < end) load(m1);   // in flight while this step's products run
+    v4i z[4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const v4i z = read_columns(z_at, 16 * s, wave * 32, lane);
+    for (int s = 0; s < 4; ++s) z[s] = read_columns(z_at, 16 * s, wave * 32, lane);
 #pragma unroll
-      for (int j = 0; j < TILES; ++j) {
-        acc[j] = mfma16<DT>(z, read_columns(hi_at, 16 * s, 32 * j, lane), acc[j]);
-        if constexpr (P != 16) acc[j] = mfma16<DT>(z, read_columns(lo_at, 16 * s, 32 * j, lane), acc[j]);
+    for (int j = 0; j < TILES; ++j) {
+      v16f sum = DT == PQ_F16 ? v16f{} : acc[j];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        sum = mfma16<DT>(z[s], read_columns(hi_at, 16 * s, 32 * j, lane), sum);
+        if constexpr (P != 16) sum = mfma16<DT>(z[s], read_columns(lo_at, 16 * s, 32 * j, lane), sum);
       }
-    }
-    if (DT == PQ_F16 && far) {
+      if constexpr (DT == PQ_F16) {
 #pragma unroll
-      for (int j = 0; j < TILES; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[j][e] *= scale_back(scale_down(top[4 + rank(j)]));
+        for (int e = 0; e < 16; ++e) acc[j][e] = fmaf(sum[e], back[j], acc[j][e]);
+      } else {
+        acc[j] = sum;
+      }
     }
     m0 = m1;
   }
@@ -757,7 +737,7 @@ template <int DT, int P>
 __global__ __launch_bounds__(256) void adapter_sums_kernel(const SumArgs b, const SumArgs a, const Ids ids) {
   __shared__ __attribute__((aligned(16))) uint8_t sz[64 * 256];
   __shared__ __attribute__((aligned(16))) uint8_t sv[2 * 64 * (P == 16 ? 32 : P * 2)];
-  __shared__ __attribute__((aligned(16))) uint32_t top[4 + P];
+  __shared__ __attribute__((aligned(16))) float top[DT == PQ_F16 ? 4 * P : 4];
   const bool is_b = (int)blockIdx.x < b.blocks;
   row_sums<DT, P>(is_b ? b : a, ids, (int)blockIdx.x - (is_b ? 0 : b.blocks), blockIdx.y, sz, sv, top);
 }

@@ -222,6 +222,51 @@ __device__ __forceinline__ float scale_down(uint32_t bits) {
 }
 __device__ __forceinline__ float scale_back(float down) { return __uint_as_float(0x7f000000u - __float_as_uint(down)); }   // 1 / down
 
+// Below 2^-10 a second part is cut to fp16's smallest subnormal, and below 2^-24 nothing is left of the first. Where the sums are t's or
+// dt's alone, values are therefore taken times a power of two that brings the largest of them to 2^15 .. 2^16, up or down, and what is cut off is
+// 2^-40 of that one. scale_exponent: minus that power's exponent (of zeros -126, so that both powers are normal numbers; of an infinity 113).
+__device__ __forceinline__ int scale_exponent(float largest) { return max((int)(__float_as_uint(largest) >> 23) - 127 - 15, -126); }
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// The scales of a step's values v [64][P] in sums over rows, four consecutive ranks of four rows of each of P / 16 a lane: each rank's from the largest
+// of its values, so that neither other ranks nor other steps lose bits to it. The waves tell each other in top[4][P]: tell_largest() before a
+// barrier, scale_values() and largest_of() after it.
+template <int P>
+__device__ __forceinline__ void tell_largest(const v4f (&v)[P / 16], float* top, int tid) {
+  v4f m;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    m[e] = fabsf(v[0][e]);
+#pragma unroll
+    for (int i = 1; i < P / 16; ++i) m[e] = fmaxf(m[e], fabsf(v[i][e]));
+    if constexpr (P == 16) m[e] = fmaxf(m[e], __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m[e]), 0x124, 0xf, 0xf, false)));   // row_ror 4
+    if constexpr (P <= 32) m[e] = fmaxf(m[e], __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m[e]), 0x128, 0xf, 0xf, false)));   // row_ror 8
+    m[e] = fmaxf(m[e], __shfl_xor(m[e], 16));
+    m[e] = fmaxf(m[e], __shfl_xor(m[e], 32));
+  }
+  if ((tid & 63) < P / 4) *reinterpret_cast<v4f*>(top + (tid >> 6) * P + 4 * (tid & 63)) = m;
+}
+template <int P>
+__device__ __forceinline__ void scale_values(v4f (&v)[P / 16], const float* top, int tid) {
+  v4f m = {};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const v4f o = *reinterpret_cast<const v4f*>(top + w * P + tid % (P / 4) * 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], o[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float by = power(-scale_exponent(m[e]));
+#pragma unroll
+    for (int i = 0; i < P / 16; ++i) v[i][e] *= by;
+  }
+}
+template <int P>
+__device__ __forceinline__ float largest_of(const float* top, int rank) {
+  return fmaxf(fmaxf(top[rank], top[P + rank]), fmaxf(top[2 * P + rank], top[3 * P + rank]));
+}
+
 // Eight consecutive ranks of a row of t (or dt), lane % 32 of which is the operand of a low-rank product: lanes l and l + 32 hold
 // the 16 ranks of a step.
 struct RankPiece {

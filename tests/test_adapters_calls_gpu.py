@@ -73,3 +73,60 @@ def test_one_row_into_out(cuda):
             with pytest.raises(AssertionError, match="contiguous|aligned"):
                 bank(x[0], y[0], i, out=out)
         assert bool((room == 7).all())
+
+
+def _near_small(M, K, N, slots, R, x_std, A_std, B_std, dy_std, ids, spread, seed):
+    """fp16 values far below 1: every product of t and dt against 64 bits. Two parts hold a value to 2 u^2 of it, or to half of fp16's smallest
+    subnormal, 2^-25, on a scale on which the largest of the values that share one is at least 2^15: those of a row in the products with t or
+    dt, those of a rank of the adapter's rows in the sums over rows. So w |v| + 2^-40 max |v|, without the 2^-25 that the values themselves
+    would lose."""
+    f, u = 2.0 ** -24, 2.0 ** -11
+    w, least, tiny = 2 * u * u, 2.0 ** -40, 2.0 ** -25
+    x, y, i, A, B, scale = _problem(M, K, N, slots, R, torch.float16, ids, seed=seed)
+    dy = torch.randn(M, N, device="cuda")
+    x, A, B, dy = x.float() * x_std, A.float() * K ** 0.5 * A_std, B.float() * R ** 0.5 * B_std, dy * dy_std
+    if spread:      # ranks of other sizes, and rows that grow
+        A = A * 4.0 ** -(torch.arange(R, device="cuda") % 8)
+        x = x * torch.logspace(-3, 0, M, device="cuda")[:, None]
+        dy = dy * torch.logspace(0, -3, M, device="cuda")[:, None]
+    x, A, B, dy, y = x.half(), A.half(), B.half(), dy.half(), y * 0
+    bank = _bank(A, B, scale, trainable=True)
+    v = x.clone().requires_grad_()
+    out = bank(v, y, i)
+    got = dict(zip(("dx", "dA", "dB"), torch.autograd.grad(out, (v, bank.lr_A, bank.lr_B), dy)), y=out.detach())
+    for s in range(slots):
+        rows = torch.nonzero(i == s).flatten()
+        if not len(rows):
+            continue
+        n = len(rows)
+        a, b, xs, d, sc = A[s].double(), B[s].double(), x[rows].double(), dy[rows].double(), float(scale[s])
+        t, dt = xs @ a * sc, d @ b.t() * sc
+        t_off, d_off = sc * (K + 2) * f * (xs.abs() @ a.abs()), sc * (N + 2) * f * (d.abs() @ b.abs().t())
+        for name, v0, v_off, other, result in (("y", t, t_off, b, t @ b), ("dx", dt, d_off, a.t(), dt @ a.t())):
+            mag = v0.abs() + v_off
+            o = (v_off + w * mag + least * mag.amax(1, keepdim=True) + (R + 4) * f * mag) @ other.abs() + 2 * f * result.abs()
+            _near(got[name][rows], result, o + u * (result.abs() + o) + tiny, name)
+        for name, v0, v_off, z in (("dA", dt, d_off, xs), ("dB", t, t_off, d)):
+            mag = v0.abs() + v_off
+            result = z.t() @ v0
+            o = z.abs().t() @ (v_off + w * mag + least * mag.amax(0, keepdim=True) + (n + 300) * f * mag)
+            o = o + u * (result.abs() + o) + tiny
+            if name == "dB":
+                result, o = result.t(), o.t()
+            _near(got[name][s], result, o, name)
+
+
+@pytest.mark.parametrize("ids", ("one", "runs", "rows"))
+@pytest.mark.parametrize("size", [(2051, 520, 808, 3, 32), (1030, 96, 328, 7, 16), (700, 136, 264, 9, 40), (4096, 64, 128, 2, 8)], ids=str)
+def test_small_values_in_fp16(cuda, size, ids):
+    """t or dt of 1e-6 and 1e-8, as little-scaled gradients and new factors make them, where the sums that they enter are well inside fp16."""
+    for x_std, A_std, B_std, dy_std in ((30.0, 1e-2, 4e-6, 1e-2), (1e3, 1e-3, 1e-6, 4e-4), (1e-2, 4e-6, 1e-2, 30.0), (1e-3, 1e-6, 1e-1, 1e3)):
+        _near_small(*size, x_std, A_std, B_std, dy_std, ids, False, seed=size[0])
+
+
+@pytest.mark.parametrize("size", [(2051, 520, 808, 3, 32), (1030, 96, 328, 7, 16), (700, 136, 264, 9, 64), (5000, 64, 128, 2, 8)], ids=str)
+def test_sizes_that_differ_in_fp16(cuda, size):
+    """Ranks whose values are 2^-14 of others', and rows that grow or fall by a thousand, up to values past fp16's end."""
+    for x_std, A_std, B_std, dy_std in ((1.0, 1e-2, 1e-3, 1e-2), (100.0, 10.0, 1e-3, 1.0), (1.0, 1e-3, 10.0, 300.0)):
+        for ids in ("one", "runs"):
+            _near_small(*size, x_std, A_std, B_std, dy_std, ids, True, seed=size[0] + 1)
