@@ -672,7 +672,7 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int b
     if constexpr (DT == PQ_F16) tell_largest<P>(vr, top, tid);
     __syncthreads();
     if constexpr (DT == PQ_F16) {
-      scale_values<P>(vr, top, tid);
+      scale_values<P>(vr, largest_four<P>(top, tid));
 #pragma unroll
       for (int j = 0; j < TILES; ++j) back[j] = power(scale_exponent(largest_of<P>(top, rank(j))));
     }

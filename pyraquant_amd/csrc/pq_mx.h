@@ -230,7 +230,7 @@ __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t
 
 // The scales of a step's values v [64][P] in sums over rows, four consecutive ranks of four rows of each of P / 16 a lane: each rank's from the largest
 // of its values, so that neither other ranks nor other steps lose bits to it. The waves tell each other in top[4][P]: tell_largest() before a
-// barrier, scale_values() and largest_of() after it.
+// barrier, largest_four() and largest_of() after it.
 template <int P>
 __device__ __forceinline__ void tell_largest(const v4f (&v)[P / 16], float* top, int tid) {
   v4f m;
@@ -241,13 +241,15 @@ __device__ __forceinline__ void tell_largest(const v4f (&v)[P / 16], float* top,
     for (int i = 1; i < P / 16; ++i) m[e] = fmaxf(m[e], fabsf(v[i][e]));
     if constexpr (P == 16) m[e] = fmaxf(m[e], __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m[e]), 0x124, 0xf, 0xf, false)));   // row_ror 4
     if constexpr (P <= 32) m[e] = fmaxf(m[e], __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m[e]), 0x128, 0xf, 0xf, false)));   // row_ror 8
-    m[e] = fmaxf(m[e], __shfl_xor(m[e], 16));
-    m[e] = fmaxf(m[e], __shfl_xor(m[e], 32));
+    const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(m[e]), __float_as_uint(m[e]), false, false);   // lanes 16 apart
+    m[e] = fmaxf(__uint_as_float(rows[0]), __uint_as_float(rows[1]));
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(m[e]), __float_as_uint(m[e]), false, false);
+    m[e] = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
   }
   if ((tid & 63) < P / 4) *reinterpret_cast<v4f*>(top + (tid >> 6) * P + 4 * (tid & 63)) = m;
 }
 template <int P>
-__device__ __forceinline__ void scale_values(v4f (&v)[P / 16], const float* top, int tid) {
+__device__ __forceinline__ v4f largest_four(const float* top, int tid) {   // of the lane's four ranks of v
   v4f m = {};
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -255,9 +257,13 @@ __device__ __forceinline__ void scale_values(v4f (&v)[P / 16], const float* top,
 #pragma unroll
     for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], o[e]);
   }
+  return m;
+}
+template <int P>
+__device__ __forceinline__ void scale_values(v4f (&v)[P / 16], v4f largest) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float by = power(-scale_exponent(m[e]));
+    const float by = power(-scale_exponent(largest[e]));
 #pragma unroll
     for (int i = 0; i < P / 16; ++i) v[i][e] *= by;
   }

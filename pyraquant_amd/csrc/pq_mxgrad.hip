@@ -442,7 +442,8 @@ void mx_dx_ring_kernel(const DxArgs p) {
 // z is dy (EIGHT false) or the 8-bit codes of x with their scales; v is t or dt, [M, R] in fp32. Column sums of z too
 // (COLS), and these alone where v is NULL. A workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step, the
 // next step's rows on their way into registers meanwhile; the order of the sums is fixed. Bound by reading z: 460 MB of 16384 x 3072 x
-// 12288 in 98 us, 4.7 TB/s.
+// 12288 in 98 us, 4.7 TB/s. In fp16 a rank's 64 values of a step are taken on a scale of their own, so that small ones keep their bits: both launches
+// 139 us instead of 122 at these sizes with rank 32, 23.0 instead of 20.0 at 4352 x 3072 x 3072, nothing with rank 64.
 struct SumArgs {
   const void* z;
   const uint8_t* scales;
@@ -454,7 +455,7 @@ struct SumArgs {
 };
 
 template <int DT, int R, bool EIGHT, bool COLS>
-__device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* sz, uint8_t* sv, uint32_t* top) {
+__device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* sz, uint8_t* sv, float* top) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int slice = block / p.panels, panel = block - slice * p.panels;
   const int c0 = panel * 128, s0 = slice * p.rows;
@@ -496,36 +497,14 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
   };
   load(s0);
   for (int m0 = s0; m0 < end; m0 += 64) {
-    bool far = false;   // some value of v is 2^16 or more (fp16: scale_down); the waves tell each other in top[0 .. 3]
-    if constexpr (DT == PQ_F16) {
-      float m = 0.0f;
-#pragma unroll
-      for (int i = 0; i < R / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(vr[i][e]));
-      top[wave] = __ballot(m >= 65536.0f) != 0;
-    }
+    float back[R / 32];   // fp16: the inverse of the scale on which the lane's ranks are taken in this step
+    v4f big;
+    if constexpr (DT == PQ_F16) tell_largest<R>(vr, top, tid);
     __syncthreads();
     if constexpr (DT == PQ_F16) {
-      const v4u all = *reinterpret_cast<const v4u*>(top);
-      far = __builtin_amdgcn_readfirstlane((int)(all[0] | all[1] | all[2] | all[3])) != 0;
-      if (far) {   // rare: the largest magnitude of each rank's 64 values, in top[4 ..]
-        if (tid < R) top[4 + tid] = 0;
-        __syncthreads();
+      big = largest_four<R>(top, tid);
 #pragma unroll
-        for (int i = 0; i < R / 16; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) atomicMax(&top[4 + (i * 256 + tid) % (R / 4) * 4 + e], __float_as_uint(vr[i][e]) & 0x7fffffffu);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < R / 16; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vr[i][e] *= scale_down(top[4 + (i * 256 + tid) % (R / 4) * 4 + e]);
-#pragma unroll
-        for (int j = 0; j < R / 32; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[j][e] *= scale_down(top[4 + 32 * j + (lane & 31)]);
-      }
+      for (int j = 0; j < R / 32; ++j) back[j] = power(scale_exponent(largest_of<R>(top, 32 * j + (lane & 31))));
     }
     if constexpr (EIGHT) {
       const int row = tid >> 2, b = tid & 3;
@@ -539,6 +518,7 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
 #pragma unroll
       for (int i = 0; i < 4; ++i) *reinterpret_cast<v4u*>(z_at(i * 16 + (tid >> 4), tid & 15)) = zr[i];
     }
+    if constexpr (DT == PQ_F16) scale_values<R>(vr, big);
 #pragma unroll
     for (int i = 0; i < R / 16; ++i) {   // 64 rows of the first part, then of the second
       v2u hi, lo;
@@ -554,23 +534,39 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
     }
     __syncthreads();
     if (m0 + 64 < end) load(m0 + 64);   // in flight while this step's products run
+    if constexpr (DT == PQ_F16) {
+      v4i z[4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const v4i z = read_columns(z_at, 16 * s, wave * 32, lane);
+      for (int s = 0; s < 4; ++s) {
+        z[s] = read_columns(z_at, 16 * s, wave * 32, lane);
+        if constexpr (COLS) cols = mfma16<DT>(z[s], ones, cols);
+      }
       if (p.v) {
 #pragma unroll
         for (int j = 0; j < R / 32; ++j) {
-          acc[j] = mfma16<DT>(z, read_columns(hi_at, 16 * s, 32 * j, lane), acc[j]);
-          acc[j] = mfma16<DT>(z, read_columns(lo_at, 16 * s, 32 * j, lane), acc[j]);
+          v16f sum = {};   // of a step by themselves, then on no scale
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            sum = mfma16<DT>(z[s], read_columns(hi_at, 16 * s, 32 * j, lane), sum);
+            sum = mfma16<DT>(z[s], read_columns(lo_at, 16 * s, 32 * j, lane), sum);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[j][e] = fmaf(sum[e], back[j], acc[j][e]);
         }
       }
-      if constexpr (COLS) cols = mfma16<DT>(z, ones, cols);
-    }
-    if (DT == PQ_F16 && far) {
+    } else {
 #pragma unroll
-      for (int j = 0; j < R / 32; ++j)
+      for (int s = 0; s < 4; ++s) {
+        const v4i z = read_columns(z_at, 16 * s, wave * 32, lane);
+        if (p.v) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[j][e] *= scale_back(scale_down(top[4 + 32 * j + (lane & 31)]));
+          for (int j = 0; j < R / 32; ++j) {
+            acc[j] = mfma16<DT>(z, read_columns(hi_at, 16 * s, 32 * j, lane), acc[j]);
+            acc[j] = mfma16<DT>(z, read_columns(lo_at, 16 * s, 32 * j, lane), acc[j]);
+          }
+        }
+        if constexpr (COLS) cols = mfma16<DT>(z, ones, cols);
+      }
     }
   }
   // lane: r = 32 j + lane % 32, columns c0 + 32 wave + 8 q + 4 (lane / 32) + e
@@ -596,7 +592,7 @@ template <int DT, int R, bool COLS>
 __global__ __launch_bounds__(256) void mx_rowsum_kernel(const SumArgs b, const SumArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t sz[64 * 256];      // [m][128 c]
   __shared__ __attribute__((aligned(16))) uint8_t sv[2 * 64 * R * 2];   // [2][m][R]
-  __shared__ __attribute__((aligned(16))) uint32_t top[4 + R];
+  __shared__ __attribute__((aligned(16))) float top[DT == PQ_F16 ? 4 * R : 4];
   if ((int)blockIdx.x < b.blocks) row_sums<DT, R, false, COLS>(b, blockIdx.x, sz, sv, top);
   else row_sums<DT, R, true, false>(a, blockIdx.x - b.blocks, sz, sv, top);
 }
