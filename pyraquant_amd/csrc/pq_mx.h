@@ -304,7 +304,8 @@ __device__ __forceinline__ RankParts parts_of(const RankPiece& p) {
   return t;
 }
 // acc[i] += l_i t^T for NI tiles of 32 x 32 whose rows (lane % 32) are the pieces' and for NP pieces; l(i, s): the other operand.
-// Where some row's values are far (rare) its pieces and sums are scaled.
+// Where some row's values are far (rare) its pieces and sums are scaled. (Small ones are not, the sums being the layer's own too: fp16 values
+// below 2^-4 are held to 2^-25, and that times |l| is what a result loses, of which fp16 itself holds no more than 2^-25.)
 template <int DT, int NI, int NP, typename L>
 __device__ __forceinline__ void rank_products(v16f* const (&acc)[NI], RankPiece (&piece)[NP], L l) {
   bool far = false;
