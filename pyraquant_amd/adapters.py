@@ -23,6 +23,7 @@ from typing import Callable, Dict, List, Mapping, Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.nn.modules import module as _module
 
 from . import _lib
 from .int8_exec import Int8Linear, is_bf16_whitelisted
@@ -231,6 +232,15 @@ class _Chosen:
         self._adapters.ids = self._before
 
 
+def _gives_new(layer: nn.Module) -> bool:
+    """Whether a layer's result is a new tensor that no hook has seen. (A class of the user's own, or a call in the place of the layer's, may
+    hand out anything.)"""
+    if layer._forward_hooks or _module._global_forward_hooks or "forward" in layer.__dict__:
+        return False
+    kind = type(layer)
+    return kind in (nn.Linear, Int8Linear, Mxfp4Linear) or kind is SplitInLinear and all(map(_gives_new, layer.linears))
+
+
 class AdaptedLinear(nn.Module):
     """A projection that requests share and the adapters beside it: layer(x), and what ``chosen.ids`` says is added to it. (Routed
     calls, with rows gathered or scattered, are a TypeError: their rows are not a batch's.)"""
@@ -254,8 +264,8 @@ class AdaptedLinear(nn.Module):
         if ids is None:
             return y
         assert x.dim() != 2 or ids.dim() != 1 or ids.shape[0] == x.shape[0], f"{x.shape[0]} rows and ids of {ids.shape[0]}: a layer's rows are the batch's"
-        # (the layer's result is a new tensor: without gradients what is added goes into it)
-        return self.adapters(x, y, ids, out=None if torch.is_grad_enabled() or not y.is_contiguous() else y)
+        # without gradients what is added goes into the layer's result, where nobody else can hold that
+        return self.adapters(x, y, ids, out=y if not torch.is_grad_enabled() and _gives_new(self.layer) and y.is_contiguous() else None)
 
 
 def add_adapters(model: nn.Module, slots: int, rank: int, *, dtype: Optional[torch.dtype] = None, trainable: bool = False,

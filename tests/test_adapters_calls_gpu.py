@@ -130,3 +130,73 @@ def test_sizes_that_differ_in_fp16(cuda, size):
     for x_std, A_std, B_std, dy_std in ((1.0, 1e-2, 1e-3, 1e-2), (100.0, 10.0, 1e-3, 1.0), (1.0, 1e-3, 10.0, 300.0)):
         for ids in ("one", "runs"):
             _near_small(*size, x_std, A_std, B_std, dy_std, ids, True, seed=size[0] + 1)
+
+
+def _styles(net, **kw):
+    from pyraquant_amd import add_adapters
+
+    styles = add_adapters(net, 3, 8, whitelist=lambda n: False, **kw)
+    for bank in styles.layers.values():
+        for s in range(3):
+            bank.set(s, torch.randn(bank.in_features, 8) * 0.1, torch.randn(8, bank.out_features) * 0.1)
+    return styles
+
+
+@pytest.mark.parametrize("kind", ("linear", "int8", "mxfp4", "split", "split int8"))
+def test_what_hooks_keep_stays(cuda, kind):
+    """A layer's result that a forward hook keeps, of the layer, of a part of it or of every module, is the layer's own afterwards too."""
+    from pyraquant_amd import convert_linears_to_int8, convert_linears_to_mxfp4
+    from pyraquant_amd.weights import SplitInLinear
+
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Linear(256, 128)).to(cuda, torch.bfloat16)
+    if "split" in kind:
+        net[0] = SplitInLinear(net[0], 128)
+    if "int8" in kind:
+        convert_linears_to_int8(net, whitelist=lambda n: False)
+    if kind == "mxfp4":
+        convert_linears_to_mxfp4(net, whitelist=lambda n: False)
+    styles = _styles(net.requires_grad_(False))
+    layer = net[0].layer
+    x = torch.randn(3, 20, 256, device=cuda, dtype=torch.bfloat16)
+    ids = torch.tensor([1, -1, 2], device=cuda)
+    places = [layer.register_forward_hook, torch.nn.modules.module.register_module_forward_hook]
+    if "split" in kind:
+        places.append(layer.linears[0].register_forward_hook)
+    with torch.no_grad():
+        own = layer(x)
+        with styles.use(ids):
+            want = net(x)
+        for place in places:
+            seen = []
+            handle = place(lambda m, a, out: seen.append((m, out)))
+            with styles.use(ids):
+                assert torch.equal(net(x), want)
+            handle.remove()
+            kept = [out for m, out in seen if m is layer]
+            if place == places[-1] and "split" in kind:
+                kept = [seen[0][1]] if "int8" in kind else []      # (of two parts in one, the first's result is the layer's)
+            assert all(torch.equal(out, own) for out in kept) and (kept or place == places[-1])
+        layer.forward, inner = lambda v: held, layer.forward     # (a call that was put in the place of the layer's own)
+        held = inner(x)
+        with styles.use(ids):
+            assert torch.equal(net(x), want) and torch.equal(held, own)
+
+
+def test_a_linear_that_holds_its_result(cuda):
+    """An nn.Linear of a class of its own may hand out a tensor that it holds, at any place."""
+    class Held(torch.nn.Linear):
+        def forward(self, x):
+            if not hasattr(self, "out"):
+                y = super().forward(x)
+                self.out = torch.empty(y.numel() + 1, dtype=y.dtype, device=y.device)[1:].view(y.shape).copy_(y)
+            return self.out
+
+    net = torch.nn.Sequential(Held(64, 40)).to(cuda, torch.bfloat16).requires_grad_(False)
+    styles = _styles(net)
+    x = torch.randn(3, 20, 64, device=cuda, dtype=torch.bfloat16)
+    with torch.no_grad():
+        plain = net(x).clone()
+        with styles.use(torch.tensor([1, -1, 2], device=cuda)):
+            first = net(x)
+            assert torch.equal(net(x), first) and not torch.equal(first, plain) and torch.equal(net[0].layer.out, plain)
