@@ -19,7 +19,9 @@ current stream; nothing synchronises. CPU tensors raise AssertionError; a missin
 """
 from __future__ import annotations
 
-from typing import Callable, Dict, List, Mapping, Optional, Tuple
+import threading
+import weakref
+from typing import Callable, Dict, List, Mapping, Optional, Set, Tuple
 
 import torch
 import torch.nn as nn
@@ -180,18 +182,65 @@ class LowRankAdapters(nn.Module):
         return f"in={self.in_features}, out={self.out_features}, {self.slots} adapters, r={self.rank}{kind} (HIP gfx950)"
 
 
+class _Choice:
+    """What a thread has chosen."""
+
+    __slots__ = ("ids", "__weakref__")
+
+    def __init__(self, ids: Optional[torch.Tensor]):
+        self.ids = ids
+
+
 class AdapterSet:
     """The adapters of a model (add_adapters): one slot in every adapted layer. ``use(ids)`` chooses those of the batches that follow, None
-    none of them; as a context manager it puts the earlier choice back."""
+    none of them; as a context manager it puts the earlier choice back.
+
+    A choice is its thread's own. Threads that have made none, autograd's among them, go by the others' while those agree; where they do not,
+    ``ids`` raises."""
 
     def __init__(self, layers: Dict[str, LowRankAdapters]):
         self.layers = layers
-        self.ids: Optional[torch.Tensor] = None
+        self._mine = threading.local()
+        self._all: Set["weakref.ref[_Choice]"] = set()      # of threads that live (each operation on it is one of the interpreter's)
+
+    def __getstate__(self):
+        own = getattr(self._mine, "choice", None)
+        return {"layers": self.layers, "choice": own and (own.ids,)}
+
+    def __setstate__(self, state) -> None:
+        self.__init__(state["layers"])
+        if state["choice"]:
+            self.use(*state["choice"])
+
+    @property
+    def ids(self) -> Optional[torch.Tensor]:
+        """What is chosen in this thread."""
+        own = getattr(self._mine, "choice", None)
+        if own is not None:
+            return own.ids
+        if not self._all:
+            return None
+        others = [c.ids for c in (r() for r in list(self._all)) if c is not None]
+        for other in others[1:]:
+            if other is not others[0]:
+                raise RuntimeError("threads have chosen different adapters of a set, and this one has not: use(ids) here too")
+        return others[0] if others else None
+
+    @ids.setter
+    def ids(self, ids: Optional[torch.Tensor]) -> None:
+        self.use(ids)
+
+    def _choose(self, choice: Optional[_Choice]) -> Optional[_Choice]:
+        before = getattr(self._mine, "choice", None)
+        if before is not None:
+            self._all.discard(weakref.ref(before))
+        if choice is not None:
+            self._all.add(weakref.ref(choice, self._all.discard))
+        self._mine.choice = choice
+        return before
 
     def use(self, ids: Optional[torch.Tensor]) -> "_Chosen":
-        chosen = _Chosen(self, self.ids)
-        self.ids = ids
-        return chosen
+        return _Chosen(self, self._choose(_Choice(ids)))
 
     def set(self, slot: int, factors: Mapping[str, Tuple[torch.Tensor, torch.Tensor]], scale: float = 1.0) -> None:
         """An adapter of the model into a slot: {layer's name: (lr_A, lr_B)}; layers that it does not name get none."""
@@ -222,14 +271,14 @@ class AdapterSet:
 
 
 class _Chosen:
-    def __init__(self, adapters: AdapterSet, before: Optional[torch.Tensor]):
+    def __init__(self, adapters: AdapterSet, before: Optional[_Choice]):
         self._adapters, self._before = adapters, before
 
     def __enter__(self) -> AdapterSet:
         return self._adapters
 
     def __exit__(self, *exc) -> None:
-        self._adapters.ids = self._before
+        self._adapters._choose(self._before)
 
 
 def _gives_new(layer: nn.Module) -> bool:
