@@ -196,7 +196,8 @@ class AdapterSet:
     none of them; as a context manager it puts the earlier choice back.
 
     A choice is its thread's own. Threads that have made none, autograd's among them, go by the others' while those agree; where they do not,
-    ``ids`` raises."""
+    ``ids`` raises. A block that is computed again in a backward pass (checkpointed) needs the choice of its forward pass there too; a layer whose
+    last call had one raises where none is left."""
 
     def __init__(self, layers: Dict[str, LowRankAdapters]):
         self.layers = layers
@@ -298,6 +299,7 @@ class AdaptedLinear(nn.Module):
         super().__init__()
         self.layer, self.adapters = layer, adapters
         self._chosen = chosen
+        self._adapted = False      # whether its last call had a choice
 
     @property
     def in_features(self) -> int:
@@ -309,9 +311,14 @@ class AdaptedLinear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         y = self.layer(x)
-        ids = self._chosen.ids
+        ids, d = self._chosen.ids, self.__dict__
         if ids is None:
+            if d["_adapted"] and torch.is_grad_enabled() and torch._C._current_graph_task_id() != -1:
+                raise RuntimeError("a layer is computed again in a backward pass, and the adapters that its forward pass had are not chosen any more: "
+                                   "call backward inside `with use(ids)` where blocks are checkpointed")
+            d["_adapted"] = False
             return y
+        d["_adapted"] = True
         assert x.dim() != 2 or ids.dim() != 1 or ids.shape[0] == x.shape[0], f"{x.shape[0]} rows and ids of {ids.shape[0]}: a layer's rows are the batch's"
         # without gradients what is added goes into the layer's result, where nobody else can hold that
         return self.adapters(x, y, ids, out=y if not torch.is_grad_enabled() and _gives_new(self.layer) and y.is_contiguous() else None)

@@ -90,3 +90,35 @@ def test_models_with_adapters_are_copied():
             assert its is not styles and its.layers["0"] is other[0].adapters and other[0]._chosen is its and torch.equal(its.ids, ids)
             with its.use(None):
                 assert styles.ids is ids and its.ids is None
+
+
+class _Twice(torch.nn.Module):
+    """Stands for adapters, which need a GPU: 2 y, with something kept for the backward pass (what keeps nothing is not computed again)."""
+
+    def forward(self, x, y, ids, out=None):
+        return y * torch.full_like(y, 2)
+
+
+@pytest.mark.parametrize("reentrant", (True, False))
+def test_a_block_computed_again_without_its_choice_raises(reentrant):
+    styles = AdapterSet({})
+    net = torch.nn.Sequential(AdaptedLinear(torch.nn.Linear(4, 4), _Twice(), styles))
+    x = torch.randn(3, 4, requires_grad=True)
+    ids = torch.tensor([0, 1, 2])
+    with styles.use(ids):
+        net(x).sum().backward()
+        want = x.grad.clone()
+        x.grad = None
+        checkpoint(net, x, use_reentrant=reentrant).sum().backward()
+        assert torch.equal(x.grad, want)
+        out = checkpoint(net, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="chosen"):
+        out.sum().backward()
+    x.grad = None
+    checkpoint(net, x, use_reentrant=reentrant).sum().backward()       # without adapters in both passes
+    assert torch.equal(2 * x.grad, want)
+    styles.use(ids)                                                    # (a choice that stays)
+    out = checkpoint(net, x, use_reentrant=reentrant)
+    x.grad = None
+    out.sum().backward()
+    assert torch.equal(x.grad, want)

@@ -200,3 +200,35 @@ def test_a_linear_that_holds_its_result(cuda):
         with styles.use(torch.tensor([1, -1, 2], device=cuda)):
             first = net(x)
             assert torch.equal(net(x), first) and not torch.equal(first, plain) and torch.equal(net[0].layer.out, plain)
+
+
+@pytest.mark.parametrize("reentrant", (True, False))
+def test_blocks_computed_again_in_the_backward_pass(cuda, reentrant):
+    """A checkpointed block gets the choice of its forward pass, where that still holds in the backward pass; else it raises."""
+    from torch.utils.checkpoint import checkpoint
+
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Linear(64, 40)).to(cuda, torch.bfloat16).requires_grad_(False)
+    styles = _styles(net, trainable=True)
+    x = torch.randn(3, 20, 64, device=cuda, dtype=torch.bfloat16, requires_grad=True)
+    ids = torch.tensor([1, -1, 2], device=cuda)
+    with styles.use(ids):
+        net(x).sum().backward()
+    want = [p.grad.clone() for p in styles.parameters()]
+    for p in styles.parameters():
+        p.grad = None
+    with styles.use(ids):
+        checkpoint(net, x, use_reentrant=reentrant).sum().backward()
+    assert all(torch.equal(p.grad, w) for p, w in zip(styles.parameters(), want))
+    with styles.use(ids):
+        out = checkpoint(net, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="chosen"):
+        out.sum().backward()
+    with styles.use(ids):
+        out = checkpoint(net, x, use_reentrant=reentrant)
+    with styles.use(ids):
+        out.sum().backward()
+    plain = checkpoint(net, x, use_reentrant=reentrant)      # no adapters, in either pass
+    x.grad = None
+    plain.sum().backward()
+    assert torch.equal(x.grad, torch.autograd.grad(net[0].layer(x).sum(), x)[0])
