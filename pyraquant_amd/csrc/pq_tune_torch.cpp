@@ -81,15 +81,23 @@ class Plan {
     steps_ = at::zeros({first_.back()}, opt.dtype(at::kInt));
   }
 
-  // Whether this is the plan of these parameters (the objects; where they lie may change).
-  bool holds(py::handle params, int bits) const {
+  // Whether this is the plan of these parameters (the objects; where they lie may change), and `state` still holds what was given out for each: in
+  // their order, as give() and its caller put them there.
+  bool holds(py::handle params, int bits, py::handle state) const {
     if (!PyList_Check(params.ptr()) || PyList_GET_SIZE(params.ptr()) != (Py_ssize_t)params_.size() || bits != bits_) return false;
     for (size_t i = 0; i < params_.size(); ++i) {
       PyObject* const o = PyList_GET_ITEM(params.ptr(), i);
       if (!THPVariable_Check(o) || THPVariable_Unpack(o).unsafeGetTensorImpl() != params_[i].unsafeGetTensorImpl()) return false;
     }
-    return true;
+    if (!PyDict_Check(state.ptr()) || given_.size() != params_.size()) return false;
+    size_t k = 0;
+    Py_ssize_t at = 0;
+    for (PyObject *key, *value; k < given_.size() && PyDict_Next(state.ptr(), &at, &key, &value);)
+      k += key == PyList_GET_ITEM(params.ptr(), k) && value == given_[k].ptr();
+    return k == given_.size();
   }
+  // What the caller puts into the optimizer's state for each parameter.
+  void give(std::vector<py::object> given) { given_ = std::move(given); }
 
   // This step's gradients; copies of those that lie in another order than their parameter.
   void collect() {
@@ -235,6 +243,7 @@ class Plan {
   std::vector<const void*> at_, grads_;
   std::vector<at::ScalarType> types_;
   Tensor tensors_, chunks_, m_, v_, exps_, steps_;
+  std::vector<py::object> given_;
 };
 
 py::object step(const py::list& groups, double max_norm) {
@@ -315,6 +324,7 @@ PYBIND11_MODULE(_tune, m) {
   py::class_<Plan>(m, "Plan")
       .def(py::init<const std::vector<Tensor>&, int>())
       .def("holds", &Plan::holds)
+      .def("give", &Plan::give)
       .def("captured", &Plan::captured)
       .def("states", &Plan::states)
       .def("of", &Plan::of)

@@ -32,7 +32,8 @@ class AdamW(torch.optim.Optimizer):
     """AdamW (see the module). A group may have ``lr``, ``betas``, ``eps``, ``weight_decay``, ``bits`` and ``seed`` of its own;
     ``max_norm`` counts for all groups together.
 
-    A group's states lie end to end, each parameter's from a multiple of 128 values on (``offsets``). ``state[p]`` holds views of them:
+    A group's states lie end to end, each parameter's from a multiple of 128 values on (``offsets``), room for every parameter, whether it gets
+    gradients or not. A parameter whose entry of ``state`` is taken away begins anew. ``state[p]`` holds views of them:
     ``step`` (a count for each 1024 values, all alike), and ``exp_avg`` and ``exp_avg_sq`` in fp32, or ``exp_avg_8bit``, ``exp_avg_root_8bit``
     and ``exponents`` (pq_adamw_states of the C header)."""
 
@@ -61,12 +62,14 @@ class AdamW(torch.optim.Optimizer):
             raise
 
     def _plan(self, i: int):
-        """The plan of group i, made at its first use and where its parameters are others; their states go with them."""
+        """The plan of group i, made at its first use and where its parameters, or the states that they have in ``state``, are others; states that
+        are there go with them."""
         g = self.param_groups[i]
         plan = self._plans.get(i)
-        if plan is None or not plan.holds(g["params"], g["bits"]):
+        if plan is None or not plan.holds(g["params"], g["bits"], self.state):
             plan = _lib.load_tune().Plan(g["params"], g["bits"])
             names = _PARTS[g["bits"]]
+            given = []
             for k, p in enumerate(g["params"]):
                 old, new = self.state.get(p, {}), dict(zip(names, plan.of(k)))
                 if old:
@@ -75,7 +78,11 @@ class AdamW(torch.optim.Optimizer):
                     with torch.no_grad():
                         for n in names:
                             new[n].copy_(old[n].reshape(new[n].shape))
+                given.append(new)
+            for p, new in zip(g["params"], given):
+                self.state.pop(p, None)      # (in the parameters' order)
                 self.state[p] = new
+            plan.give(given)
             self._drop(i)
             self._plans[i] = plan
         return plan

@@ -124,3 +124,39 @@ def test_blocks_with_any_nan_are_nan(cuda, nan):
     opt.step()
     for t in opt.moments():
         assert bool(t.view(3, 128)[1].isnan().all())
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+def test_states_that_are_taken_away_or_replaced(cuda, bits):
+    """opt.state says what a parameter's states are: those that are gone begin anew, others' go on, and given ones count."""
+    from collections import defaultdict
+
+    params = _params([(1000,), (33, 7), (2050,)], torch.float32)
+    opt = _opt(params, bits=bits, seed=5)
+
+    def step(seed, t):
+        _grads(params, seed)
+        before = _before(opt)
+        opt.step()
+        for k, n in enumerate(t):
+            assert opt.state[params[k]]["step"].tolist() == [n] * opt.state[params[k]]["step"].numel()
+        if len(set(t)) == 1:
+            _check_step(opt, before, t[0], seed=5)
+
+    step(0, (1, 1, 1))
+    step(1, (2, 2, 2))
+    opt.state.clear()
+    step(2, (1, 1, 1))
+    step(3, (2, 2, 2))
+    kept = [t.clone() for t in opt.state[params[0]].values()]
+    opt.state.pop(params[1])
+    assert not opt.moments()[0][1024:1024 + 231].any() and all(torch.equal(a, b) for a, b in zip(kept, opt.state[params[0]].values()))
+    step(4, (3, 1, 3))
+    opt.state[params[2]] = {}
+    step(5, (4, 2, 1))
+    given = {k: v.clone() for k, v in opt.state[params[0]].items()}
+    step(6, (5, 3, 2))
+    opt.state[params[0]] = given
+    step(7, (5, 4, 3))
+    opt.state = defaultdict(dict)
+    step(8, (1, 1, 1))
