@@ -19,6 +19,7 @@ moved), and keep the optimizer, which holds them, as long as its graphs. Gradien
 """
 from __future__ import annotations
 
+from collections import defaultdict
 from typing import List, Optional, Tuple
 
 import torch
@@ -44,6 +45,7 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm: Optional[torch.Tensor] = None
         self._plans = {}
         self._in_graphs = []   # plans that were replaced and that captured graphs go on with
+        self._loading = None   # the state dict that is being loaded
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, bits=bits, seed=seed))
 
     def add_param_group(self, group) -> None:
@@ -122,22 +124,34 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """A state dict of this class. Groups take the bits and the seed that it was saved with."""
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        super().load_state_dict({**state_dict, "state": {}})   # (torch casts states to the parameters' types)
-        params = [p for g in self.param_groups for p in g["params"]]
-        self.state.clear()
-        self._drop(*list(self._plans))
-        for i, p in zip(ids, params):
-            if i in state_dict["state"]:
-                self.state[p] = {k: v.detach().clone() for k, v in state_dict["state"][i].items()}
+        def take(_, d):      # the last hook before the load: what others made of the dict (torch would cast states to the parameters' types)
+            self._loading = d
+            return {**d, "state": {}}
+
+        handle = self.register_load_state_dict_pre_hook(take)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            handle.remove()
+            self._loading = None
 
     def __getstate__(self):
         return {**super().__getstate__(), "max_norm": self.max_norm}
 
     def __setstate__(self, state) -> None:
+        loading = self.__dict__.get("_loading")
+        if loading is not None:
+            ids = [i for g in loading["param_groups"] for i in g["params"]]
+            params = [p for g in state["param_groups"] for p in g["params"]]
+            own = defaultdict(dict)
+            for i, p in zip(ids, params):
+                if i in loading["state"]:
+                    own[p] = {k: v.detach().clone() for k, v in loading["state"][i].items()}
+            state = {**state, "state": own}
         super().__setstate__(state)
         self.__dict__.setdefault("max_norm", None)
         self.grad_norm = None
         self.__dict__.setdefault("_plans", {})
         self.__dict__.setdefault("_in_graphs", [])
+        self.__dict__.setdefault("_loading", None)
         self._drop(*list(self._plans))
