@@ -66,6 +66,7 @@ class AdamW(torch.optim.Optimizer):
     def _plan(self, i: int):
         """The plan of group i, made at its first use and where its parameters, or the states that they have in ``state``, are others; states that
         are there go with them."""
+        i = range(len(self.param_groups))[i]      # (from the end, too)
         g = self.param_groups[i]
         plan = self._plans.get(i)
         if plan is None or not plan.holds(g["params"], g["bits"], self.state):

@@ -126,6 +126,28 @@ def test_blocks_with_any_nan_are_nan(cuda, nan):
         assert bool(t.view(3, 128)[1].isnan().all())
 
 
+def test_groups_from_the_end(cuda):
+    """A group's number counted from the end is that group, and no other memory."""
+    a, b = _params([(300,), (77, 3)], torch.float32)
+    opt = _opt([{"params": [a]}, {"params": [b], "bits": 8}])
+    _grads([a, b], 0)
+    opt.step()
+    assert opt.offsets(-1) == opt.offsets(1)
+    assert all(x.data_ptr() == y.data_ptr() for x, y in zip(opt.states(-1), opt.states(1)))
+    assert all(torch.equal(x, y) for x, y in zip(opt.moments(group=-2), opt.moments(group=0)))
+    m, r = opt.moments(group=-1)
+    opt.load_moments(m, r, 7, group=-1)
+    _grads([a, b], 1)
+    before = _before(opt)
+    opt.step()
+    assert int(opt.state[b]["step"][0]) == 8 and int(opt.state[a]["step"][0]) == 2
+    assert opt.state[b]["exp_avg_8bit"].data_ptr() == opt.states(1)[0].data_ptr()
+    del before
+    for i in (2, -3):
+        with pytest.raises(IndexError):
+            opt.moments(group=i)
+
+
 @pytest.mark.parametrize("bits", (32, 8))
 def test_states_that_are_taken_away_or_replaced(cuda, bits):
     """opt.state says what a parameter's states are: those that are gone begin anew, others' go on, and given ones count."""
