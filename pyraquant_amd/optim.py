@@ -81,6 +81,8 @@ class AdamW(torch.optim.Optimizer):
                     with torch.no_grad():
                         for n in names:
                             new[n].copy_(old[n].reshape(new[n].shape))
+                            if old[n].is_cuda:      # (it goes away, and may be another stream's)
+                                old[n].record_stream(torch.cuda.current_stream(old[n].device))
                 given.append(new)
             for p, new in zip(g["params"], given):
                 self.state.pop(p, None)      # (in the parameters' order)

@@ -182,3 +182,25 @@ def test_states_that_are_taken_away_or_replaced(cuda, bits):
     step(7, (5, 4, 3))
     opt.state = defaultdict(dict)
     step(8, (1, 1, 1))
+
+
+def test_states_loaded_on_another_stream(cuda):
+    """States that a state dict brings on one stream and a step takes on another, which is behind."""
+    p = _params([(1 << 20,)], torch.float32)
+    opt, want = _opt(p), _opt(copy.deepcopy(p))
+    q = want.param_groups[0]["params"]
+    for t in (0, 1):
+        for ps, o in ((p, opt), (q, want)):
+            _grads(ps, t)
+            o.step()
+    side = torch.cuda.Stream()
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        opt.step()
+    junk = [torch.full((1 << 20,), 1e9, device=cuda) for _ in range(8)]      # (memory that the loaded states may have had)
+    torch.cuda.current_stream().wait_stream(side)
+    want.step()
+    assert torch.equal(p[0], q[0]) and all(torch.equal(a, b) for a, b in zip(opt.states(), want.states()))
+    del junk
