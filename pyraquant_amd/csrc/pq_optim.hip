@@ -245,9 +245,10 @@ __device__ __forceinline__ void step_chunk(const StepArgs& p, void* param, const
       v[i][e] = fmaf(d * d, p.b2c, EIGHT ? fmaf(v[i][e], -p.b2c, v[i][e]) : v[i][e] * p.b2);
       least = min(least, __float_as_uint(v[i][e]) - 1);
     }
-    // The instructions for roots and reciprocals are within 1 of the last place, but take subnormal numbers for zeros: where a square is
-    // below 2^-96, or eps is, the exact ones are taken (12 and 10 instructions; a step of 88 M bf16 values was bound by them).
-    if (__ballot(least < 0x0f7fffffu) || p.eps < 0x1p-96f) {
+    // The instructions for roots and reciprocals are within 1 of the last place, but take subnormal numbers for zeros: with 8-bit states, whose
+    // step of 88 M bf16 values was bound by the exact ones (12 and 10 instructions), those are taken where a square of the wave's is below 2^-96, or
+    // eps is. 32-bit states always take them, so that no value's last bit depends on its neighbours' (88 M bf16 values 390 us for 394, 0.1 M 5.7 for 5.2).
+    if (!EIGHT || __ballot(least < 0x0f7fffffu) || p.eps < 0x1p-96f) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         root[e] = sqrtf(v[i][e]);

@@ -204,3 +204,23 @@ def test_states_loaded_on_another_stream(cuda):
     want.step()
     assert torch.equal(p[0], q[0]) and all(torch.equal(a, b) for a, b in zip(opt.states(), want.states()))
     del junk
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_values_do_not_depend_on_their_neighbours(cuda, dtype):
+    """With 32-bit states a value's step is the same to the bit whatever else is in its tensor: squares that are subnormal beside it, or infinite."""
+    g = torch.Generator().manual_seed(0)
+    values, grads = torch.randn(4096, generator=g) * 0.02, torch.randn(2, 4096, generator=g) * 1e-3
+    out = []
+    for odd in (None, 1e-14, float("inf")):
+        p = torch.nn.Parameter(values.to(dtype).to(cuda))
+        opt = _opt([p])
+        for gr in grads:
+            p.grad = gr.to(dtype).to(cuda)
+            if odd is not None:
+                p.grad[::64] = odd
+            opt.step()
+        keep = torch.arange(4096, device=cuda) % 64 != 0
+        out.append([p.detach()[keep]] + [t[keep] for t in opt.states()])
+    for other in out[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out[0], other))
