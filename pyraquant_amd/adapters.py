@@ -43,6 +43,11 @@ def _load_adapt():
     return _adapt
 
 
+def _check_dtype(dtype: torch.dtype) -> None:
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"unsupported dtype {dtype} (expected bfloat16, float16 or float32)")
+
+
 def _padded(rank: int) -> int:
     return 16 if rank <= 16 else 32 if rank <= 32 else 64
 
@@ -91,8 +96,7 @@ class LowRankAdapters(nn.Module):
         assert out_features > 0 and out_features % 8 == 0, f"out_features {out_features} is not a multiple of 8"
         assert 1 <= slots <= 65535, f"{slots} adapters (1 to 65535)"
         assert 1 <= rank <= MAX_RANK, f"rank {rank}: adapters take 1 to {MAX_RANK}"
-        if dtype not in (torch.bfloat16, torch.float16, torch.float32):
-            raise ValueError(f"unsupported dtype {dtype} (expected bfloat16, float16 or float32)")
+        _check_dtype(dtype)
         self.in_features, self.out_features, self.slots, self.rank = in_features, out_features, slots, rank
         self.trainable = bool(trainable)
         zeros = lambda *shape: torch.zeros(shape, dtype=dtype, device=device)   # noqa: E731
@@ -109,14 +113,17 @@ class LowRankAdapters(nn.Module):
         assert 0 <= slot < self.slots, f"slot {slot} of {self.slots}"
         return slot
 
+    def _fitting(self, slot: int, lr_A: torch.Tensor, lr_B: torch.Tensor, scale: float) -> Tuple[int, int, float]:
+        r = lr_A.shape[-1] if lr_A.dim() else 0
+        assert tuple(lr_A.shape) == (self.in_features, r) and tuple(lr_B.shape) == (r, self.out_features) and 1 <= r <= self.rank, (
+            tuple(lr_A.shape), tuple(lr_B.shape), self.in_features, self.out_features, self.rank)
+        return self._slot(slot), r, float(scale)
+
     @torch.no_grad()
     def set(self, slot: int, lr_A: torch.Tensor, lr_B: torch.Tensor, scale: float = 1.0) -> None:
         """An adapter into a slot: lr_A [K, r], lr_B [r, N], r up to the rank (zeros past it). On the current stream; captured graphs
         take it from their next replay on."""
-        slot = self._slot(slot)
-        r = lr_A.shape[-1]
-        assert tuple(lr_A.shape) == (self.in_features, r) and tuple(lr_B.shape) == (r, self.out_features) and 1 <= r <= self.rank, (
-            tuple(lr_A.shape), tuple(lr_B.shape), self.in_features, self.out_features, self.rank)
+        slot, r, scale = self._fitting(slot, lr_A, lr_B, scale)
         if self.trainable:
             for to, what in ((self.lr_A[slot], lr_A), (self.lr_B[slot].t(), lr_B.t())):
                 to[:, :r].copy_(what)
@@ -124,7 +131,7 @@ class LowRankAdapters(nn.Module):
         else:
             for axes, f, what in ((_down_axes, self.lr_Af, lr_A), (_up_axes, self.lr_Bf, lr_B.t())):
                 _write(axes(f[slot]), what.to(f.device, f.dtype), *f.shape[1:])
-        self.scale[slot] = float(scale)
+        self.scale[slot] = scale
 
     @torch.no_grad()
     def clear(self, slot: int) -> None:
@@ -137,6 +144,8 @@ class LowRankAdapters(nn.Module):
     def freeze(self, dtype: Optional[torch.dtype] = None) -> "LowRankAdapters":
         """Turns a trainable module into one that serves, in ``dtype`` (give the inputs' type where the factors are in another), with the
         same outputs."""
+        if dtype is not None:
+            _check_dtype(dtype)
         if self.trainable:
             A, B, P = self.lr_A.detach(), self.lr_B.detach(), _padded(self.rank)
             A, B = A.to(dtype or A.dtype), B.to(dtype or B.dtype)
@@ -247,6 +256,8 @@ class AdapterSet:
         """An adapter of the model into a slot: {layer's name: (lr_A, lr_B)}; layers that it does not name get none."""
         unknown = sorted(set(factors) - set(self.layers))
         assert not unknown, f"not adapted layers: {unknown[:4]}"
+        for name, (lr_A, lr_B) in factors.items():      # (all, before any slot changes)
+            self.layers[name]._fitting(slot, lr_A, lr_B, scale)
         for name, bank in self.layers.items():
             if name in factors:
                 bank.set(slot, *factors[name], scale)

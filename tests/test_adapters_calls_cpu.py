@@ -122,3 +122,21 @@ def test_a_block_computed_again_without_its_choice_raises(reentrant):
     x.grad = None
     out.sum().backward()
     assert torch.equal(x.grad, want)
+
+
+def test_a_set_that_is_refused_changes_nothing():
+    a, b = LowRankAdapters(16, 8, 2, 4), LowRankAdapters(8, 8, 2, 4)
+    styles = AdapterSet({"a": a, "b": b})
+    good = {"a": (torch.ones(16, 4), torch.ones(4, 8)), "b": (torch.ones(8, 2), torch.ones(2, 8))}
+    styles.set(0, good)
+    before = [t.clone() for t in (*a.buffers(), *b.buffers())]
+    for slot, factors, scale in ((0, {"a": good["b"]}, 1.0), (0, {"a": (good["a"][0] * 2, good["a"][1]), "b": (torch.ones(8, 5), torch.ones(5, 8))}, 1.0),
+                                 (2, good, 1.0), (0, {"a": good["a"], "c": good["b"]}, 1.0), (1, {"b": (torch.ones(8), torch.ones(8))}, 1.0),
+                                 (1, good, "x")):
+        with pytest.raises((AssertionError, ValueError)):
+            styles.set(slot, factors, scale)
+        assert all(torch.equal(t, o) for t, o in zip((*a.buffers(), *b.buffers()), before))
+    with pytest.raises(ValueError, match="dtype"):
+        LowRankAdapters(16, 8, 2, 4, trainable=True).freeze(torch.float64)
+    with pytest.raises(ValueError, match="dtype"):
+        styles.freeze(torch.int8)
