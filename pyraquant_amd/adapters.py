@@ -79,6 +79,24 @@ def _write(axes: torch.Tensor, m: torch.Tensor, C: int, P: int) -> None:
     axes.copy_(full.view(axes.shape))
 
 
+def _lay_out(A: torch.Tensor, B: torch.Tensor, a: torch.Tensor, b: torch.Tensor) -> None:
+    """A [slots, K, r] and B [slots, r, N] into a and b, [slots, C, P] in the orders of `down` and of `up`: one launch on the GPU for 16 bits. (4096 x
+    4096, rank 16, 32 slots set one by one: 1.1 ms, 1.9 with tensor operations; frozen at once 60 us, 119.)"""
+    P = a.shape[-1]
+    if a.is_cuda and b.device == a.device and b.dtype == a.dtype and a.dtype in (torch.bfloat16, torch.float16) and a.is_contiguous() and b.is_contiguous():
+        A, B = A.resolve_neg().contiguous(), B.resolve_neg().contiguous()
+        (slots, K, r), N = A.shape, B.shape[2]
+        with torch.cuda.device(a.device):
+            _lib.check(_lib.load().pq_adapter_factors(_lib.ptr(A), _lib.PQ_ADAPTER_BY_COLUMN, _lib.ptr(B), _lib.PQ_ADAPTER_BY_RANK, slots, K, N, r, P,
+                                                      _lib.ptr(a), None, None, _lib.ptr(b), _lib.stream_of(a.device)), "adapters")
+        for t in (a, b):
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
+    else:
+        _write(_down_axes(a), A, a.shape[1], P)
+        _write(_up_axes(b), B.transpose(1, 2), b.shape[1], P)
+
+
 class LowRankAdapters(nn.Module):
     """``slots`` adapters of a projection: ``adapters(x, y, ids)`` is y + scale[id] (x lr_A[id]) lr_B[id]. x [..., in_features] and y
     [..., out_features] in bf16 or fp16, features multiples of 8, ranks up to 64; ids as the module says. ``out=`` takes the result, y
@@ -129,8 +147,8 @@ class LowRankAdapters(nn.Module):
                 to[:, :r].copy_(what)
                 to[:, r:].zero_()
         else:
-            for axes, f, what in ((_down_axes, self.lr_Af, lr_A), (_up_axes, self.lr_Bf, lr_B.t())):
-                _write(axes(f[slot]), what.to(f.device, f.dtype), *f.shape[1:])
+            a, b = self.lr_Af, self.lr_Bf
+            _lay_out(lr_A[None].to(a.device, a.dtype), lr_B[None].to(b.device, b.dtype), a[slot : slot + 1], b[slot : slot + 1])
         self.scale[slot] = scale
 
     @torch.no_grad()
@@ -151,10 +169,11 @@ class LowRankAdapters(nn.Module):
             A, B = A.to(dtype or A.dtype), B.to(dtype or B.dtype)
             del self.lr_A, self.lr_B
             self.trainable = False
-            for name, axes, m, features in (("lr_Af", _down_axes, A, self.in_features), ("lr_Bf", _up_axes, B.transpose(1, 2), self.out_features)):
-                f = m.new_zeros((self.slots, _room(features), P))
-                _write(axes(f), m, _room(features), P)
-                self.register_buffer(name, f)
+            a, b = A.new_zeros((self.slots, _room(self.in_features), P)), B.new_zeros((self.slots, _room(self.out_features), P))
+            with torch.no_grad():
+                _lay_out(A, B, a, b)
+            self.register_buffer("lr_Af", a)
+            self.register_buffer("lr_Bf", b)
         return self
 
     def __getattr__(self, name):

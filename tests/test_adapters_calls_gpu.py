@@ -75,6 +75,43 @@ def test_one_row_into_out(cuda):
         assert bool((room == 7).all())
 
 
+@pytest.mark.parametrize("dtype", (*BOTH, torch.float32))
+@pytest.mark.parametrize("K,N,rank", [(8, 8, 1), (136, 264, 20), (1280, 72, 64), (520, 1032, 16)])
+def test_factors_laid_out_on_the_gpu(cuda, K, N, rank, dtype):
+    """set() and freeze() on the GPU and on the CPU hold the same: ranks below the module's, factors of other types, orders and devices."""
+    from pyraquant_amd.adapters import LowRankAdapters
+
+    g = torch.Generator().manual_seed(K)
+    here, there = (LowRankAdapters(K, N, 3, rank, dtype=dtype, device=d) for d in (cuda, "cpu"))
+    tuned, again = (LowRankAdapters(K, N, 3, rank, dtype=dtype, device=d, trainable=True) for d in (cuda, "cpu"))
+    wide_a, wide_b = torch.randn(rank, K + 1, generator=g), torch.randn(N, 2 * rank, generator=g)
+    for slot, r, move in ((1, rank, lambda t: t), (0, max(rank - 3, 1), lambda t: t.to(cuda, torch.float16)), (2, 1, lambda t: t.double()),
+                          (1, max(rank // 2, 1), lambda t: t.to(cuda))):
+        A, B = move(wide_a)[:r, 1:].t(), move(wide_b)[:, ::2].t()[:r]
+        for bank in (here, there, tuned, again):
+            bank.set(slot, A.requires_grad_(), B, 0.5 + slot)
+        assert torch.equal(here.lr_Af.cpu(), there.lr_Af) and torch.equal(here.lr_Bf.cpu(), there.lr_Bf), slot
+        assert torch.equal(here.scale.cpu(), there.scale) and torch.equal(here.lr_A[slot, :, :r].cpu(), A.detach().cpu().to(dtype))
+    here.set(1, torch._neg_view(torch.ones(K, rank, dtype=dtype, device=cuda)), torch.ones(rank, N, device=cuda))
+    assert bool((here.lr_A[1] == -1).all()) and bool((here.lr_B[1] == 1).all()) and torch.equal(here.lr_Af[0].cpu(), there.lr_Af[0])
+    for to in (None, torch.float16):
+        a, b = (LowRankAdapters(K, N, 3, rank, dtype=dtype, device=m.scale.device, trainable=True) for m in (tuned, again))
+        a.load_state_dict(tuned.state_dict())
+        b.load_state_dict(again.state_dict())
+        a.freeze(to)
+        b.freeze(to)
+        assert a.lr_Af.dtype == (to or dtype) and torch.equal(a.lr_Af.cpu(), b.lr_Af) and torch.equal(a.lr_Bf.cpu(), b.lr_Bf)
+
+
+def test_backward_sees_that_factors_were_set(cuda):
+    x, y, i, A, B, scale = _problem(24, 64, 40, 3, 8, torch.bfloat16, "runs")
+    bank = _bank(A, B, scale)
+    out = bank(x.requires_grad_(), y, i)
+    bank.set(1, A[0], B[0])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
 def _near_small(M, K, N, slots, R, x_std, A_std, B_std, dy_std, ids, spread, seed):
     """fp16 values far below 1: every product of t and dt against 64 bits. Two parts hold a value to 2 u^2 of it, or to half of fp16's smallest
     subnormal, 2^-25, on a scale on which the largest of the values that share one is at least 2^15: those of a row in the products with t or
