@@ -234,12 +234,12 @@ class AdapterSet:
 
     def __getstate__(self):
         own = getattr(self._mine, "choice", None)
-        return {"layers": self.layers, "choice": own and (own.ids,)}
+        return {"layers": self.layers, "ids": own and own.ids}
 
     def __setstate__(self, state) -> None:
         self.__init__(state["layers"])
-        if state["choice"]:
-            self.use(*state["choice"])
+        if state["ids"] is not None:
+            self.use(state["ids"])
 
     @property
     def ids(self) -> Optional[torch.Tensor]:
@@ -329,7 +329,7 @@ class AdaptedLinear(nn.Module):
         super().__init__()
         self.layer, self.adapters = layer, adapters
         self._chosen = chosen
-        self._adapted = False      # whether its last call had a choice
+        self._adapted = False      # whether the last call had a choice
 
     @property
     def in_features(self) -> int:
@@ -343,7 +343,7 @@ class AdaptedLinear(nn.Module):
         y = self.layer(x)
         ids, d = self._chosen.ids, self.__dict__
         if ids is None:
-            if d["_adapted"] and torch.is_grad_enabled() and torch._C._current_graph_task_id() != -1:
+            if d.get("_adapted") and torch.is_grad_enabled() and torch._C._current_graph_task_id() != -1:
                 raise RuntimeError("a layer is computed again in a backward pass, and the adapters that its forward pass had are not chosen any more: "
                                    "call backward inside `with use(ids)` where blocks are checkpointed")
             d["_adapted"] = False

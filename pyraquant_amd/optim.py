@@ -9,8 +9,8 @@ tensor on the GPU. A norm that is infinite or NaN leaves parameters, states and 
 
 ``bits=8`` keeps two bytes a value and two more for each 128: the mean of the gradients with 3 mantissa bits, the root of the mean of their squares
 with 4, over 16 powers of two below the block's largest. What is cut off is rounded up or down by a hash of the value's place, the
-step and ``seed``, so that averages move by less than a step of the grid. Elsewhere AdamW is the usual one; sparse gradients, several
-parameters in one place and, in a group, several devices are refused.
+step and ``seed``, so that averages move by less than a step of the grid. Elsewhere AdamW is the usual one, but that a group's states are all there from its
+first use on, in one piece; sparse gradients, several parameters in one place and, in a group, several devices are refused.
 
 ``lr`` may be a tensor of one fp32 value on the GPU, which the kernel reads: a captured step then follows it. Steps can be
 captured after the first one has been taken; the step counts live on the GPU, so replays go on counting. A graph goes on with the
