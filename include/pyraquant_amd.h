@@ -554,7 +554,7 @@ typedef struct {
   int64_t n_tensors;
 } pq_adamw_list;
 typedef struct {
-  void *m, *v;                  /* 16-byte aligned */
+  void *m, *v;                  /* 16-byte aligned; with n 0, these may all be NULL */
   uint8_t* exps;                /* 2-byte aligned; NULL with 32 bits */
   int32_t* steps;
   int64_t n;

@@ -407,7 +407,7 @@ __global__ __launch_bounds__(256) void adamw_load_kernel(const StepArgs p, int64
 }
 
 int check_states(const pq_adamw_states* s, const char* what) {
-  if (!s || !s->m || !s->v || (s->bits == 8 && !s->exps)) return set_error(PQ_EINVAL, "%s: null pointer", what);
+  if (!s || (s->n && (!s->m || !s->v || (s->bits == 8 && !s->exps)))) return set_error(PQ_EINVAL, "%s: null pointer", what);
   if (s->bits != 8 && s->bits != 32) return set_error(PQ_EINVAL, "%s: states of %d bits (8 or 32)", what, s->bits);
   if (s->n < 0 || s->n % kBlock || s->n > ((int64_t)1 << 40)) return set_error(PQ_ESHAPE, "%s: %lld values (a multiple of %d)", what, (long long)s->n, kBlock);
   if ((uintptr_t)s->m % 16 || (uintptr_t)s->v % 16 || (uintptr_t)s->exps % 2) return set_error(PQ_EALIGN, "%s: states 16-byte aligned", what);
@@ -487,7 +487,8 @@ extern "C" int pq_adamw_step(const pq_adamw_list* list, const pq_adamw_states* s
                              const double* partials, int64_t n_partials, float* norm, hipStream_t stream) {
   if (const int st = check_list(list, "pq_adamw_step")) return st;
   if (const int st = check_states(states, "pq_adamw_step")) return st;
-  if (!rates || !states->steps) return set_error(PQ_EINVAL, "pq_adamw_step: null pointer");
+  if (!rates || (states->n && !states->steps)) return set_error(PQ_EINVAL, "pq_adamw_step: null pointer");
+  if (list->n_tensors && list->first_chunk[list->n_tensors] && !states->n) return set_error(PQ_ESHAPE, "pq_adamw_step: no states for the list's values");
   if (!(rates->beta1 >= 0 && rates->beta1 < 1 && rates->beta2 >= 0 && rates->beta2 < 1 && rates->eps >= 0 && rates->weight_decay >= 0) ||
       (!rates->lr_at && !(rates->lr >= 0)))
     return set_error(PQ_EINVAL, "pq_adamw_step: lr %g, betas %g and %g, eps %g, weight decay %g", rates->lr, rates->beta1, rates->beta2,

@@ -7,6 +7,21 @@ import torch
 from pyraquant_amd.optim import AdamW
 
 
+def test_states_without_values():
+    """Null pointers where there are no states, and then no list that has values."""
+    import ctypes
+
+    import pyraquant_amd._lib as L
+
+    lib, P = L.load(), ctypes.c_void_p(256)
+    for bits in (8, 32):
+        s, r = L.AdamWStates(None, None, None, None, 0, bits), L.AdamWRates(1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None, 0)
+        for size, want in ((0, L.PQ_OK), (1000, L.PQ_ESHAPE)):
+            lst = L.AdamWList(P, P, (ctypes.c_int64 * 2)(0, (size + 1023) // 1024), (ctypes.c_void_p * 1)(256), 1)
+            assert lib.pq_adamw_step(ctypes.byref(lst), ctypes.byref(s), ctypes.byref(r), None, 0, None, None) == want
+        assert lib.pq_adamw_moments(ctypes.byref(s), None, None, 0, None) == L.PQ_OK and lib.pq_adamw_load(ctypes.byref(s), None, None, None) == L.PQ_OK
+
+
 def _saved(opt, n=8):
     state = {0: {"step": torch.tensor([3], dtype=torch.int32), "exp_avg": torch.arange(n, dtype=torch.float32), "exp_avg_sq": torch.full((n,), 2.0 ** -40)}}
     return {"state": state, "param_groups": copy.deepcopy(opt.state_dict()["param_groups"])}

@@ -52,6 +52,22 @@ def test_parameters_that_change_where_they_lie(cuda, bits):
         opt.step()
 
 
+@pytest.mark.parametrize("bits", (32, 8))
+def test_a_group_of_empty_parameters(cuda, bits):
+    """Parameters without a value, alone in their group, with a gradient and with a limit."""
+    empty, full = (torch.nn.Parameter(torch.ones(n, device=cuda)) for n in (0, 100))
+    for p in (empty, full):
+        p.grad = torch.ones_like(p)
+    for groups in ([{"params": [empty]}], [{"params": [empty]}, {"params": [full]}]):
+        for limit in (None, 1.0):
+            opt = _opt(groups, bits=bits, max_norm=limit)
+            opt.step()
+            opt.step()
+            assert limit is None or abs(float(opt.grad_norm) - 10.0 * (len(groups) - 1)) < 1e-5
+            assert all(t.numel() == 0 for t in opt.moments()) and opt.offsets() == [0]
+    assert bool((full < 1).all())
+
+
 def test_a_step_that_was_refused(cuda):
     """What a refused step has seen of parameters that moved counts for nothing: the next one is refused too, or finds all of them."""
     a, b = _params([(1000,), (500,)], torch.float32)
