@@ -18,8 +18,9 @@
 // and 0 stands for zero: what lies below the grid is zero, but a root that is no zero is at least the grid's first value, so
 // that no mean is divided by a root that went to zero before it. A block with an infinity or a NaN is NaN (E 255).
 //
-// A bf16 value with 8-bit states moves 10 bytes, with 32-bit ones 22, an fp32 value with 8-bit states 16: these are bound by memory (12.7 M fp32 values
-// 43 us, 4.8 TB/s), the first by its arithmetic, 64 instructions a value (88.6 M bf16 values in three launches 258 us, without arithmetic 169).
+// A bf16 value with 8-bit states moves 10 bytes, with 32-bit ones 22, an fp32 value with 8-bit states 16. The latter two are bound by memory (88.2 M bf16
+// values with 32-bit states 390 us, 5.0 TB/s; 12.7 M fp32 values 43 us, 4.8). The first takes 234 us for 88.2 M values in a graph (three launches, 89 us each alone)
+// where its memory would take 169: a wave loads, computes some 64 instructions a value, and stores, one chunk after the other.
 #include "pq_common.h"
 
 #include <math.h>
@@ -245,9 +246,10 @@ __device__ __forceinline__ void step_chunk(const StepArgs& p, void* param, const
       v[i][e] = fmaf(d * d, p.b2c, EIGHT ? fmaf(v[i][e], -p.b2c, v[i][e]) : v[i][e] * p.b2);
       least = min(least, __float_as_uint(v[i][e]) - 1);
     }
-    // The instructions for roots and reciprocals are within 1 of the last place, but take subnormal numbers for zeros: with 8-bit states, whose
-    // step of 88 M bf16 values was bound by the exact ones (12 and 10 instructions), those are taken where a square of the wave's is below 2^-96, or
-    // eps is. 32-bit states always take them, so that no value's last bit depends on its neighbours' (88 M bf16 values 390 us for 394, 0.1 M 5.7 for 5.2).
+    // The instructions for roots and reciprocals are within 1 of the last place, but take subnormal numbers for zeros: with 8-bit states (the step of 88 M
+    // bf16 values, its states' values read out, 488 us with the exact ones, 12 and 10 instructions, and 430 with these) those are taken where a square of
+    // the wave's is below 2^-96, or eps is. 32-bit states always take them, so that no value's last bit depends on its neighbours' (88 M bf16 values 390
+    // us for 394, 0.1 M 5.7 for 5.2).
     if (!EIGHT || __ballot(least < 0x0f7fffffu) || p.eps < 0x1p-96f) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
