@@ -12,7 +12,7 @@
 //   sums  the two sums over rows, per adapter, over chunks of the rows, added by `join` in their order
 // All sums are fp32. t and dt are taken by the 16-bit matrix instructions in two parts (two_parts), in fp16 on a scale of each row's (`up`) or of each
 // rank's in 64 rows (`sums`), so that their rounding shows in no result, however small they are (the scales of `sums` cost a step of tuning 16384 x
-// 1280 x 5120 with rank 32 205 -> 208 us). No atomics: the same bits every time. Bound by memory: 2 R operations for each value that is read.
+// 1280 x 5120 with rank 32 205 -> 206 us). No atomics: the same bits every time. Bound by memory: 2 R operations for each value that is read.
 #include "pq_mx.h"
 
 #include <algorithm>
@@ -599,7 +599,7 @@ struct SumArgs {
 };
 
 template <int DT, int P>
-__device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int block, int which, uint8_t* sz, uint8_t* sv, float* top) {
+__device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int block, int which, uint8_t* sz, uint8_t* sv, uint32_t* top, float* back) {
   constexpr int TILES = P == 16 ? 1 : P / 32, PITCH = P == 16 ? 64 : P * 2;   // of v's tiles: with P 16, the first part in ranks 0-15, the second in 16-31
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunk = block / p.panels, panel = block - chunk * p.panels;
@@ -668,14 +668,9 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int b
   if (m0 >= end) return;
   load(m0);
   while (m0 < end) {
-    float back[TILES];   // fp16: the inverse of the scale on which the lane's ranks are taken in this step
     if constexpr (DT == PQ_F16) tell_largest<P>(vr, top, tid);
     __syncthreads();
-    if constexpr (DT == PQ_F16) {
-      scale_values<P>(vr, largest_four<P>(top, tid));
-#pragma unroll
-      for (int j = 0; j < TILES; ++j) back[j] = power(scale_exponent(largest_of<P>(top, rank(j))));
-    }
+    if constexpr (DT == PQ_F16) scale_values<P>(vr, top, back, tid);
 #pragma unroll
     for (int i = 0; i < 4; ++i) *reinterpret_cast<v4u*>(z_at(i * 16 + (tid >> 4), tid & 15)) = zr[i];
 #pragma unroll
@@ -707,8 +702,9 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, const Ids& ids, int b
         if constexpr (P != 16) sum = mfma16<DT>(z[s], read_columns(lo_at, 16 * s, 32 * j, lane), sum);
       }
       if constexpr (DT == PQ_F16) {
+        const float by = back[rank(j)];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[j][e] = fmaf(sum[e], back[j], acc[j][e]);
+        for (int e = 0; e < 16; ++e) acc[j][e] = fmaf(sum[e], by, acc[j][e]);
       } else {
         acc[j] = sum;
       }
@@ -737,9 +733,10 @@ template <int DT, int P>
 __global__ __launch_bounds__(256) void adapter_sums_kernel(const SumArgs b, const SumArgs a, const Ids ids) {
   __shared__ __attribute__((aligned(16))) uint8_t sz[64 * 256];
   __shared__ __attribute__((aligned(16))) uint8_t sv[2 * 64 * (P == 16 ? 32 : P * 2)];
-  __shared__ __attribute__((aligned(16))) float top[DT == PQ_F16 ? 4 * P : 4];
+  __shared__ __attribute__((aligned(16))) uint32_t top[DT == PQ_F16 ? 2 * P : 4];
+  __shared__ __attribute__((aligned(16))) float back[DT == PQ_F16 ? P : 4];
   const bool is_b = (int)blockIdx.x < b.blocks;
-  row_sums<DT, P>(is_b ? b : a, ids, (int)blockIdx.x - (is_b ? 0 : b.blocks), blockIdx.y, sz, sv, top);
+  row_sums<DT, P>(is_b ? b : a, ids, (int)blockIdx.x - (is_b ? 0 : b.blocks), blockIdx.y, sz, sv, top, back);
 }
 
 // The chunks' sums in order, rounded: dB [slots, R, N] and dA [slots, K, R]. (8 adapters of 5120 + 1280 columns and rank 32, of 16 and 48 chunks, 8 us.)

@@ -229,48 +229,56 @@ __device__ __forceinline__ int scale_exponent(float largest) { return max((int)(
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // The scales of a step's values v [64][P] in sums over rows, four consecutive ranks of four rows of each of P / 16 a lane: each rank's from the largest
-// of its values, so that neither other ranks nor other steps lose bits to it. The waves tell each other in top[4][P]: tell_largest() before a
-// barrier, largest_four() and largest_of() after it.
+// of its values, so that neither other ranks nor other steps lose bits to it. Only exponents count, so two ranks share a word and its instructions
+// (upper halves of fp32; with a word each, 16384 x 3072 x 12288 of rank 32 took 139 us). The waves tell each other in top[4][P / 2]: tell_largest() before a barrier,
+// scale_values() after it, and after the next one back[P] holds what brings a rank's sums back.
+__device__ __forceinline__ us2 halves_of(uint32_t w) { return __builtin_bit_cast(us2, w); }   // (by value: the cast takes a vector's element for its first one)
+__device__ __forceinline__ uint32_t most(uint32_t x, uint32_t y) { return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(halves_of(x), halves_of(y))); }
 template <int P>
-__device__ __forceinline__ void tell_largest(const v4f (&v)[P / 16], float* top, int tid) {
-  v4f m;
+__device__ __forceinline__ void tell_largest(const v4f (&v)[P / 16], uint32_t* top, int tid) {
+  auto upper = [](float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302) & 0x7fff7fffu; };
+  v2u m;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    m[e] = fabsf(v[0][e]);
+  for (int h = 0; h < 2; ++h) {
+    m[h] = upper(v[0][2 * h], v[0][2 * h + 1]);
 #pragma unroll
-    for (int i = 1; i < P / 16; ++i) m[e] = fmaxf(m[e], fabsf(v[i][e]));
-    if constexpr (P == 16) m[e] = fmaxf(m[e], __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m[e]), 0x124, 0xf, 0xf, false)));   // row_ror 4
-    if constexpr (P <= 32) m[e] = fmaxf(m[e], __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m[e]), 0x128, 0xf, 0xf, false)));   // row_ror 8
-    const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(m[e]), __float_as_uint(m[e]), false, false);   // lanes 16 apart
-    m[e] = fmaxf(__uint_as_float(rows[0]), __uint_as_float(rows[1]));
-    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(m[e]), __float_as_uint(m[e]), false, false);
-    m[e] = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+    for (int i = 1; i < P / 16; ++i) m[h] = most(m[h], upper(v[i][2 * h], v[i][2 * h + 1]));
+    if constexpr (P == 16) m[h] = most(m[h], (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m[h], 0x124, 0xf, 0xf, false));   // row_ror 4
+    if constexpr (P <= 32) m[h] = most(m[h], (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m[h], 0x128, 0xf, 0xf, false));   // row_ror 8
+    const auto rows = __builtin_amdgcn_permlane16_swap(m[h], m[h], false, false);   // lanes 16 apart
+    m[h] = most(rows[0], rows[1]);
+    const auto halves = __builtin_amdgcn_permlane32_swap(m[h], m[h], false, false);
+    m[h] = most(halves[0], halves[1]);
   }
-  if ((tid & 63) < P / 4) *reinterpret_cast<v4f*>(top + (tid >> 6) * P + 4 * (tid & 63)) = m;
+  if ((tid & 63) < P / 4) *reinterpret_cast<v2u*>(top + (tid >> 6) * (P / 2) + 2 * (tid & 63)) = m;
 }
 template <int P>
-__device__ __forceinline__ v4f largest_four(const float* top, int tid) {   // of the lane's four ranks of v
-  v4f m = {};
+__device__ __forceinline__ void scale_values(v4f (&v)[P / 16], const uint32_t* top, float* back, int tid) {
+  v2u m = {0, 0};
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const v4f o = *reinterpret_cast<const v4f*>(top + w * P + tid % (P / 4) * 4);
+    const v2u o = *reinterpret_cast<const v2u*>(top + w * (P / 2) + tid % (P / 4) * 2);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], o[e]);
+    for (int h = 0; h < 2; ++h) m[h] = most(m[h], o[h]);
   }
-  return m;
-}
-template <int P>
-__device__ __forceinline__ void scale_values(v4f (&v)[P / 16], v4f largest) {
+  v4f by, inverse;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float by = power(-scale_exponent(largest[e]));
-#pragma unroll
-    for (int i = 0; i < P / 16; ++i) v[i][e] *= by;
+  for (int h = 0; h < 2; ++h) {
+    // exponents E of both ranks, biased and 16 at least (a NaN's is an infinity's): the scale 2^(142 - E), as bits (269 - E) << 23
+    const us2 e = __builtin_elementwise_max(halves_of(m[h]) >> (uint16_t)7, us2{16, 16});
+    const uint32_t w = __builtin_bit_cast(uint32_t, us2{269, 269} - e);
+    by[2 * h] = __uint_as_float(w << 23);
+    by[2 * h + 1] = __uint_as_float((w & 0xffff0000u) << 7);
   }
-}
-template <int P>
-__device__ __forceinline__ float largest_of(const float* top, int rank) {
-  return fmaxf(fmaxf(top[rank], top[P + rank]), fmaxf(top[2 * P + rank], top[3 * P + rank]));
+#pragma unroll
+  for (int i = 0; i < P / 16; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[i][e] *= by[e];
+  if (tid < P / 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) inverse[e] = __uint_as_float(0x7f000000u - __float_as_uint(by[e]));
+    *reinterpret_cast<v4f*>(back + 4 * tid) = inverse;
+  }
 }
 
 // Eight consecutive ranks of a row of t (or dt), lane % 32 of which is the operand of a low-rank product: lanes l and l + 32 hold

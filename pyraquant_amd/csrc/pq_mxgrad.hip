@@ -443,7 +443,7 @@ void mx_dx_ring_kernel(const DxArgs p) {
 // (COLS), and these alone where v is NULL. A workgroup of four waves takes 128 columns and a slice of the rows, 64 rows a step, the
 // next step's rows on their way into registers meanwhile; the order of the sums is fixed. Bound by reading z: 460 MB of 16384 x 3072 x
 // 12288 in 98 us, 4.7 TB/s. In fp16 a rank's 64 values of a step are taken on a scale of their own, so that small ones keep their bits: both launches
-// 139 us instead of 122 at these sizes with rank 32, 23.0 instead of 20.0 at 4352 x 3072 x 3072, nothing with rank 64.
+// 133 us instead of 125 at these sizes with rank 32, 21.8 instead of 19.8 at 4352 x 3072 x 3072, nothing with rank 64.
 struct SumArgs {
   const void* z;
   const uint8_t* scales;
@@ -455,7 +455,7 @@ struct SumArgs {
 };
 
 template <int DT, int R, bool EIGHT, bool COLS>
-__device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* sz, uint8_t* sv, float* top) {
+__device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* sz, uint8_t* sv, uint32_t* top, float* back) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int slice = block / p.panels, panel = block - slice * p.panels;
   const int c0 = panel * 128, s0 = slice * p.rows;
@@ -497,15 +497,8 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
   };
   load(s0);
   for (int m0 = s0; m0 < end; m0 += 64) {
-    float back[R / 32];   // fp16: the inverse of the scale on which the lane's ranks are taken in this step
-    v4f big;
     if constexpr (DT == PQ_F16) tell_largest<R>(vr, top, tid);
     __syncthreads();
-    if constexpr (DT == PQ_F16) {
-      big = largest_four<R>(top, tid);
-#pragma unroll
-      for (int j = 0; j < R / 32; ++j) back[j] = power(scale_exponent(largest_of<R>(top, 32 * j + (lane & 31))));
-    }
     if constexpr (EIGHT) {
       const int row = tid >> 2, b = tid & 3;
       const float s = restore_scale(byte);   // (past the end the codes are zeros)
@@ -518,7 +511,7 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
 #pragma unroll
       for (int i = 0; i < 4; ++i) *reinterpret_cast<v4u*>(z_at(i * 16 + (tid >> 4), tid & 15)) = zr[i];
     }
-    if constexpr (DT == PQ_F16) scale_values<R>(vr, big);
+    if constexpr (DT == PQ_F16) scale_values<R>(vr, top, back, tid);
 #pragma unroll
     for (int i = 0; i < R / 16; ++i) {   // 64 rows of the first part, then of the second
       v2u hi, lo;
@@ -545,13 +538,14 @@ __device__ __forceinline__ void row_sums(const SumArgs& p, int block, uint8_t* s
 #pragma unroll
         for (int j = 0; j < R / 32; ++j) {
           v16f sum = {};   // of a step by themselves, then on no scale
+          const float by = back[32 * j + (lane & 31)];
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             sum = mfma16<DT>(z[s], read_columns(hi_at, 16 * s, 32 * j, lane), sum);
             sum = mfma16<DT>(z[s], read_columns(lo_at, 16 * s, 32 * j, lane), sum);
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[j][e] = fmaf(sum[e], back[j], acc[j][e]);
+          for (int e = 0; e < 16; ++e) acc[j][e] = fmaf(sum[e], by, acc[j][e]);
         }
       }
     } else {
@@ -592,9 +586,10 @@ template <int DT, int R, bool COLS>
 __global__ __launch_bounds__(256) void mx_rowsum_kernel(const SumArgs b, const SumArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t sz[64 * 256];      // [m][128 c]
   __shared__ __attribute__((aligned(16))) uint8_t sv[2 * 64 * R * 2];   // [2][m][R]
-  __shared__ __attribute__((aligned(16))) float top[DT == PQ_F16 ? 4 * R : 4];
-  if ((int)blockIdx.x < b.blocks) row_sums<DT, R, false, COLS>(b, blockIdx.x, sz, sv, top);
-  else row_sums<DT, R, true, false>(a, blockIdx.x - b.blocks, sz, sv, top);
+  __shared__ __attribute__((aligned(16))) uint32_t top[DT == PQ_F16 ? 2 * R : 4];
+  __shared__ __attribute__((aligned(16))) float back[DT == PQ_F16 ? R : 4];
+  if ((int)blockIdx.x < b.blocks) row_sums<DT, R, false, COLS>(b, blockIdx.x, sz, sv, top, back);
+  else row_sums<DT, R, true, false>(a, blockIdx.x - b.blocks, sz, sv, top, back);
 }
 
 // The slices' sums added in order, rounded to 16 bits: dB [R, N] and dA [K, R]; and the column sums in 32. A thread sums one
