@@ -19,8 +19,8 @@
 // that no mean is divided by a root that went to zero before it. A block with an infinity or a NaN is NaN (E 255).
 //
 // A bf16 value with 8-bit states moves 10 bytes, with 32-bit ones 22, an fp32 value with 8-bit states 16. The latter two are bound by memory (88.2 M bf16
-// values with 32-bit states 390 us, 5.0 TB/s; 12.7 M fp32 values 43 us, 4.8). The first takes 234 us for 88.2 M values in a graph (three launches, 89 us each alone)
-// where its memory would take 169: a wave loads, computes some 64 instructions a value, and stores, one chunk after the other.
+// values with 32-bit states 390 us, 5.0 TB/s; 12.7 M fp32 values 43 us, 4.8). The first takes 243 us for 88.2 M values in a graph (three launches, 89 us each alone)
+// where its memory would take 169: a wave loads, computes some 68 instructions a value, and stores, one chunk after the other.
 #include "pq_common.h"
 
 #include <math.h>
@@ -48,7 +48,7 @@ struct StepArgs {
   const double* partials;              // sums of squares, or NULL
   float* norm_out;
   double lr, log_b1, log_b2, decay;
-  float b1, b2, b1c, b2c, eps, max_norm;
+  float b1, b2, b1c, b2c, b1l, eps, max_norm;   // (b1l: what b1c lacks)
   uint32_t seed_key;
   int n_partials, first_tensor, first_chunk, end_chunk;
 };
@@ -129,7 +129,7 @@ template <int BITS>
 __device__ __forceinline__ us2 rounded2(uint32_t a, uint32_t ua, uint32_t b, uint32_t ub) {   // of magnitudes' bits; at most an infinity's
   constexpr uint32_t up = 15u << 23;
   const uint32_t ra = (a + ua + up) >> (23 - BITS), rb = (b + ub + up) >> (23 - BITS);
-  return __builtin_elementwise_min(two(ra | rb << 16), both((255u + 15u) << BITS));
+  return __builtin_elementwise_max(__builtin_elementwise_min(two(ra | rb << 16), both((255u + 15u) << BITS)), both(15u << BITS));   // (u may be -1)
 }
 // fp32 bits of two bytes (without signs) of a block of exponent E
 template <int BITS>
@@ -159,7 +159,7 @@ struct Moments8 {
       roots[e + 1] = __uint_as_float((ar << 3 & 0x7ff80000u) | nan_r);
     }
   }
-  // the values as they are kept; add(e, um, ur): what the rounding adds
+  // the values as they are kept, from magnitudes of roots; add(e, um, ur): what the rounding adds
   template <typename U>
   __device__ __forceinline__ void keep(const float (&mean)[8], const float (&roots)[8], U add) {
     us2 rm[4], rr[4], tm = both(0), tr = both(0);
@@ -169,7 +169,7 @@ struct Moments8 {
       add(2 * i, um[0], ur[0]);
       add(2 * i + 1, um[1], ur[1]);
       rm[i] = rounded2<3>(__float_as_uint(mean[2 * i]) & 0x7fffffffu, um[0], __float_as_uint(mean[2 * i + 1]) & 0x7fffffffu, um[1]);
-      rr[i] = rounded2<4>(__float_as_uint(roots[2 * i]) & 0x7fffffffu, ur[0], __float_as_uint(roots[2 * i + 1]) & 0x7fffffffu, ur[1]);   // (a NaN may have a sign)
+      rr[i] = rounded2<4>(__float_as_uint(roots[2 * i]), ur[0], __float_as_uint(roots[2 * i + 1]), ur[1]);
       tm = __builtin_elementwise_max(tm, rm[i]);
       tr = __builtin_elementwise_max(tr, rr[i]);
     }
@@ -237,15 +237,31 @@ __device__ __forceinline__ void step_chunk(const StepArgs& p, void* param, const
       for (int e = 0; e < 8; ++e) v[i][e] *= v[i][e];
     }
     uint32_t least = ~0u;   // of the squares that are no zeros (bits - 1)
+    int past[8] = {};       // -1 where the exact mean's magnitude lies below m's
+    if (EIGHT && p.b1c <= 0.5f && p.b2c <= 0.5f) {
+      // b m + (1 - b) d as m + (1 - b) (d - m), in few roundings: b in fp32 is off by as much as half a step itself. What is cut to 8 bits next goes by the
+      // exact mean: where this one was rounded up, and that may be to a border of the grid, by the number below it. (The step of 88 M bf16 values 290 ->
+      // 300 us, of 12.7 M fp32 values 41 -> 43; a half to a third as many means fall to another step of the grid than the exact one, and fewer than from
+      // elementary operations in fp32.)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float d = g[i][e] * clip;
-      // b m as m - (1 - b) m in one rounding: b in fp32 is off by as much as half a step itself, and what is cut to 8 bits next falls to the
-      // other side of a grid step as often as m is off (an infinity there is NaN either way; in 32-bit states it stays one).
-      m[i][e] = fmaf(d, p.b1c, EIGHT ? fmaf(m[i][e], -p.b1c, m[i][e]) : m[i][e] * p.b1);
-      v[i][e] = fmaf(d * d, p.b2c, EIGHT ? fmaf(v[i][e], -p.b2c, v[i][e]) : v[i][e] * p.b2);
-      least = min(least, __float_as_uint(v[i][e]) - 1);
+      for (int e = 0; e < 8; ++e) {
+        const float d = g[i][e] * clip, w = fmaf(d, d, -v[i][e]), before = m[i][e], q = d - before;
+        m[i][e] = fmaf(q, p.b1c, before);
+        float lacks = fmaf(q, p.b1c, before - m[i][e]);
+        if constexpr (DT == PQ_F32) lacks = fmaf((d - q) - before, p.b1c, fmaf(q, p.b1l, lacks));   // (and what q and 1 - b lack)
+        past[e] = fmaf(m[i][e], 0x1p-27f, lacks) * m[i][e] < 0.0f ? -1 : 0;   // (less than 1 / 16 is what lacks itself may be off; of an infinity it is NaN)
+        v[i][e] = fmaf(w, p.b2c, v[i][e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = g[i][e] * clip;
+        m[i][e] = fmaf(d, p.b1c, m[i][e] * p.b1);
+        v[i][e] = fmaf(d * d, p.b2c, v[i][e] * p.b2);
+      }
     }
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) least = min(least, min(__float_as_uint(v[i][e]) - 1, __float_as_uint(v[i][e + 1]) - 1));
     // The instructions for roots and reciprocals are within 1 of the last place, but take subnormal numbers for zeros: with 8-bit states (the step of 88 M
     // bf16 values, its states' values read out, 488 us with the exact ones, 12 and 10 instructions, and 430 with these) those are taken where a square of
     // the wave's is below 2^-96, or eps is. 32-bit states always take them, so that no value's last bit depends on its neighbours' (88 M bf16 values 390
@@ -253,13 +269,13 @@ __device__ __forceinline__ void step_chunk(const StepArgs& p, void* param, const
     if (!EIGHT || __ballot(least < 0x0f7fffffu) || p.eps < 0x1p-96f) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        root[e] = sqrtf(v[i][e]);
+        root[e] = fabsf(sqrtf(v[i][e]));   // (a NaN may have a sign)
         x[i][e] = x[i][e] * r.keep - r.size * m[i][e] / fmaf(root[e], r.unbias, p.eps);
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        root[e] = __builtin_amdgcn_sqrtf(v[i][e]);
+        root[e] = __builtin_amdgcn_sqrtf(fabsf(v[i][e]));
         x[i][e] = fmaf(-r.size * m[i][e], __builtin_amdgcn_rcpf(fmaf(root[e], r.unbias, p.eps)), x[i][e] * r.keep);
       }
     }
@@ -268,7 +284,7 @@ __device__ __forceinline__ void step_chunk(const StepArgs& p, void* param, const
       const uint32_t place = (uint32_t)(base + at) * kPlace + key;
       s[i].keep(m[i], root, [&](int e, uint32_t& um, uint32_t& ur) {
         const uint32_t h = mixed(place + e * kPlace);
-        um = (h & 0xffffu) << 4;
+        um = ((h & 0xffffu) << 4) + (uint32_t)past[e];
         ur = (h >> 16) << 3;
       });
       s[i].store(p.m, p.v, p.exps, base + at);
@@ -502,7 +518,7 @@ extern "C" int pq_adamw_step(const pq_adamw_list* list, const pq_adamw_states* s
   p.steps = states->steps, p.m = states->m, p.v = states->v, p.exps = states->exps;
   p.lr_at = rates->lr_at, p.lr = rates->lr;
   p.log_b1 = log(rates->beta1), p.log_b2 = log(rates->beta2), p.decay = rates->weight_decay;
-  p.b1 = (float)rates->beta1, p.b1c = (float)(1.0 - rates->beta1), p.b2 = (float)rates->beta2, p.b2c = (float)(1.0 - rates->beta2);
+  p.b1 = (float)rates->beta1, p.b1c = (float)(1.0 - rates->beta1), p.b1l = (float)(1.0 - rates->beta1 - (double)p.b1c), p.b2 = (float)rates->beta2, p.b2c = (float)(1.0 - rates->beta2);
   p.eps = (float)rates->eps, p.max_norm = (float)rates->max_norm;
   p.partials = n_partials ? partials : nullptr, p.n_partials = (int)n_partials, p.norm_out = norm;
   p.seed_key = rates->seed * 0x5851F42Du;

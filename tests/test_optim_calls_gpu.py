@@ -2,9 +2,11 @@
 import copy
 import gc
 
+import numpy as np
 import pytest
 import torch
 
+from oracle import adamw_ref as ref
 from test_optim_gpu import TYPES, _before, _check_step, _grads, _opt, _params
 
 pytestmark = pytest.mark.gpu
@@ -240,3 +242,49 @@ def test_values_do_not_depend_on_their_neighbours(cuda, dtype):
         out.append([p.detach()[keep]] + [t[keep] for t in opt.states()])
     for other in out[1:]:
         assert all(torch.equal(a, b) for a, b in zip(out[0], other))
+
+
+def test_means_beside_a_border_of_their_grid(cuda):
+    """8-bit means whose exact value lies a third of fp32's last place below or above a border of the grid (what the hash adds counted in) are held on
+    that side of it. The gradients that lead there are found in 64 bits: m' = m + (1 - b1) (g - m) moves by a tenth of g's last place."""
+    n, seed, t, b1 = 1 << 16, 3, 1, 0.9
+    rng = np.random.default_rng(0)
+    m = ref.held(np.where(rng.random(n) < 0.5, 1, -1) * rng.uniform(1e-3, 4e-3, n), 3, 0.5)
+    um, _ = ref.dither(np.arange(n), t, seed)
+    add = (um * 65536).astype(np.int64) << 4
+    bits = np.float32(0.95 * np.abs(m)).view(np.int32).astype(np.int64)
+    border = ((bits + add) >> 20 << 20) - add + (1 << 20)                       # the next place in fp32 from which on the sum has one step more
+    low = border.astype(np.int32).view(np.float32).astype(np.float64)
+    last = np.ldexp(1.0, np.frexp(low)[1] - 24)
+    side = np.where(rng.random(n) < 0.5, -1, 1)
+    target = np.sign(m) * (low + side * last / 3)
+    g = np.float32((target - b1 * m) / (1 - b1))
+    exact = b1 * m + (1 - b1) * g.astype(np.float64)
+    off = (np.abs(exact) - low) / last
+    sure = (off * side > 0.1) & (np.abs(off) < 0.5)                              # (g's own rounding)
+    assert sure.mean() > 0.9
+    p = torch.nn.Parameter(torch.zeros(n, device=cuda))
+    opt = _opt([p], bits=8, seed=seed)
+    opt.load_moments(torch.tensor(m, dtype=torch.float32, device=cuda), torch.full((n,), 1e-3, device=cuda), 0)
+    assert np.array_equal(opt.moments()[0].double().cpu().numpy(), m)
+    p.grad = torch.tensor(g, device=cuda)
+    opt.step()
+    got, want = opt.moments()[0].double().cpu().numpy(), ref.held(exact, 3, um)
+    assert np.array_equal(got[sure], want[sure]), int((got[sure] != want[sure]).sum())
+
+
+def test_infinite_gradients_where_nothing_is_added(cuda):
+    """A block with one infinity is NaN also where the hash adds nothing to it."""
+    n = 1 << 22
+    places = np.nonzero(ref.dither(np.arange(n), 1, 0)[0] == 0)[0]
+    assert len(places) > 20
+    for sign in (1.0, -1.0):
+        p = torch.nn.Parameter(torch.zeros(n, device=cuda))
+        opt = _opt([p], bits=8)
+        p.grad = torch.zeros_like(p)
+        p.grad[torch.tensor(places, device=cuda)] = sign * float("inf")
+        opt.step()
+        blocks = torch.zeros(n // 128, dtype=torch.bool, device=cuda)
+        blocks[torch.tensor(places // 128, device=cuda)] = True
+        for v in opt.moments():
+            assert torch.equal(v.view(-1, 128).isnan().all(1), blocks) and not v.view(-1, 128)[~blocks].any()
